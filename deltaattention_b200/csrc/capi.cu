@@ -10,6 +10,8 @@
 #include <mutex>
 #include <string>
 
+#include "evict.cuh"
+#include "kv4.cuh"
 #include "params.cuh"
 #include "../../include/deltaattn_b200.h"
 
@@ -54,6 +56,15 @@ cudaError_t launch_dpxa_compact(int, const void*, const int64_t*, const int32_t*
 cudaError_t launch_dpxa_score(int, const void*, const int32_t*, const int32_t*, const void*, const int32_t*,
                               const int32_t*, float*, float*, float, int, int, int, int, int, cudaStream_t);
 cudaError_t launch_dpxa_select(const float*, const float*, uint32_t*, float, int, int, int, int, cudaStream_t);
+cudaError_t launch_kv4_quantize(int, const void*, const int64_t*, const void*, const int64_t*, const Kv4Hist&, int64_t,
+                                int64_t, int64_t, int64_t, cudaStream_t);
+cudaError_t launch_kv4_dequantize(int, const Kv4Hist&, void*, void*, const int64_t*, int64_t, int64_t, int64_t, int64_t,
+                                  cudaStream_t);
+cudaError_t launch_kv4_update(int, int64_t, bool, const Kv4Update&, cudaStream_t);
+cudaError_t launch_kv4_attn(int, int64_t, Kv4Attn, uint8_t*, cudaStream_t);
+size_t kv4_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, bool);
+cudaError_t launch_evict(EvictParams, uint8_t*, cudaStream_t);
+size_t evict_workspace(int64_t, int64_t, int64_t);
 }  // namespace dab
 
 using namespace dab;
@@ -808,6 +819,199 @@ int dab_nm_select(const void* k, const int64_t* k_strides, int32_t* keep_mask, c
                                       static_cast<int>(n_keep), static_cast<int>(m_group), stride,
                                       static_cast<cudaStream_t>(stream)),
                      "nm_select");
+}
+
+// ------------------------------------------------------------- decode history in 4 bits
+namespace {
+// what every entry on a 4-bit history checks; `nm` names the entry
+int kv4_check(const char* nm, const void* kc, const void* vc, const void* ks, const void* vs, const int64_t* cst,
+              const int64_t* sst, int64_t batch, int64_t heads, int64_t rows, int64_t head_dim) {
+  if (!cst || !sst || (rows > 0 && (!kc || !vc || !ks || !vs))) return fail(1, std::string(nm) + ": null pointer");
+  if (head_dim != 64 && head_dim != 128) return fail(1, std::string(nm) + ": head_dim must be 64 or 128");
+  if (batch < 0 || heads < 0 || batch * heads > 65535) return fail(1, std::string(nm) + ": need batch * heads <= 65535");
+  const uintptr_t srow = static_cast<uintptr_t>(head_dim / 8);  // bytes of a row's scales
+  if ((reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc)) % 16 || cst[0] % 16 || cst[1] % 16)
+    return fail(1, std::string(nm) + ": code rows must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) % srow || sst[0] * 2 % static_cast<int64_t>(srow) ||
+      sst[1] * 2 % static_cast<int64_t>(srow))
+    return fail(1, std::string(nm) + ": scale rows must be aligned to their size");
+  return 0;
+}
+Kv4Hist kv4_hist(const void* kc, const void* vc, const void* ks, const void* vs, const int64_t* cst,
+                 const int64_t* sst) {
+  Kv4Hist h;
+  h.k_codes = static_cast<uint8_t*>(const_cast<void*>(kc));
+  h.v_codes = static_cast<uint8_t*>(const_cast<void*>(vc));
+  h.k_scales = static_cast<__nv_bfloat16*>(const_cast<void*>(ks));
+  h.v_scales = static_cast<__nv_bfloat16*>(const_cast<void*>(vs));
+  h.cb = cst[0]; h.ch = cst[1]; h.sb = sst[0]; h.sh = sst[1];
+  return h;
+}
+}  // namespace
+
+int dab_kv4_quantize(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* k_codes,
+                     void* v_codes, const int64_t* code_strides, void* k_scales, void* v_scales,
+                     const int64_t* scale_strides, int dtype, int64_t batch, int64_t heads, int64_t rows,
+                     int64_t head_dim, void* stream) {
+  const char* nm = "dab_kv4_quantize";
+  if (!k || !v || !k_strides || !v_strides) return fail(1, std::string(nm) + ": null pointer");
+  if (dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": rows must be bf16 or fp16");
+  if (rows < 0 || rows >= (int64_t{1} << 31)) return fail(1, std::string(nm) + ": bad row count");
+  if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, code_strides, scale_strides, batch, heads, rows,
+                         head_dim))
+    return rc;
+  return cuda_status(launch_kv4_quantize(dtype, k, k_strides, v, v_strides,
+                                         kv4_hist(k_codes, v_codes, k_scales, v_scales, code_strides, scale_strides),
+                                         batch, heads, rows, head_dim, static_cast<cudaStream_t>(stream)),
+                     "kv4_quantize");
+}
+
+int dab_kv4_dequantize(const void* k_codes, const void* v_codes, const int64_t* code_strides, const void* k_scales,
+                       const void* v_scales, const int64_t* scale_strides, void* k, void* v,
+                       const int64_t* out_strides, int dtype, int64_t batch, int64_t heads, int64_t rows,
+                       int64_t head_dim, void* stream) {
+  const char* nm = "dab_kv4_dequantize";
+  if (!k || !v || !out_strides) return fail(1, std::string(nm) + ": null pointer");
+  if (dtype != F32 && dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": bad dtype");
+  if (rows < 0 || rows >= (int64_t{1} << 31)) return fail(1, std::string(nm) + ": bad row count");
+  if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, code_strides, scale_strides, batch, heads, rows,
+                         head_dim))
+    return rc;
+  return cuda_status(
+      launch_kv4_dequantize(dtype, kv4_hist(k_codes, v_codes, k_scales, v_scales, code_strides, scale_strides), k, v,
+                            out_strides, batch, heads, rows, head_dim, static_cast<cudaStream_t>(stream)),
+      "kv4_dequantize");
+}
+
+int dab_decode_update_kv4(const void* k_new, const void* v_new, void* k_codes, void* v_codes, void* k_scales,
+                          void* v_scales, int32_t* counts, int32_t* timestamps, float* mass, int32_t* lengths,
+                          void* last_key, void* k_exact, void* v_exact, float* exact_mass, const int64_t* seq_state,
+                          const int64_t* strides, float threshold, int use_cosine, int dtype, int64_t batch,
+                          int64_t heads, int64_t head_dim, int64_t capacity, int64_t exact_window, int* err_word,
+                          void* stream) {
+  const char* nm = "dab_decode_update_kv4";
+  if (!k_new || !v_new || !counts || !timestamps || !lengths || !last_key || !k_exact || !v_exact || !strides)
+    return fail(1, std::string(nm) + ": null pointer");
+  if (!seq_state) return fail(1, std::string(nm) + ": null seq_state");
+  if (dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": keys must be bf16 or fp16");
+  if (exact_window < 1 || exact_window >= (int64_t{1} << 31) || capacity < 0 || capacity >= (int64_t{1} << 31))
+    return fail(1, std::string(nm) + ": need exact_window >= 1 and capacity >= 0");
+  // strides: k_new(3) v_new(3) codes(2) scales(2) meta(2) lengths(2) last(2) exact(3) exact_mass(2) = 21
+  const int64_t* s = strides;
+  if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, s + 6, s + 8, batch, heads, capacity, head_dim)) return rc;
+  Kv4Update p;
+  p.k_new = k_new; p.v_new = v_new;
+  p.kb = s[0]; p.kh = s[1]; p.kd = s[2]; p.vb = s[3]; p.vh = s[4]; p.vd = s[5];
+  p.hist = kv4_hist(k_codes, v_codes, k_scales, v_scales, s + 6, s + 8);
+  p.counts = counts; p.times = timestamps; p.mass = mass; p.mb = s[10]; p.mh = s[11];
+  p.lengths = lengths; p.lb = s[12]; p.lh = s[13];
+  p.last_key = last_key; p.lkb = s[14]; p.lkh = s[15];
+  p.k_exact = k_exact; p.v_exact = v_exact; p.eb = s[16]; p.eh = s[17]; p.en = s[18];
+  p.exact_mass = exact_mass; p.emb = s[19]; p.emh = s[20];
+  p.state = seq_state; p.err = err_word; p.threshold = threshold;
+  p.B = static_cast<int>(batch); p.H = static_cast<int>(heads);
+  p.cap = static_cast<int>(capacity); p.W = static_cast<int>(exact_window);
+  return cuda_status(launch_kv4_update(dtype, head_dim, use_cosine != 0, p, static_cast<cudaStream_t>(stream)),
+                     "decode_update_kv4");
+}
+
+size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t num_q_heads, int64_t head_dim, int64_t capacity,
+                                               int64_t exact_window, int with_mass) {
+  if (batch < 0 || num_q_heads < 0 || head_dim < 1 || capacity < 0 || exact_window < 0) return 0;
+  return kv4_attn_workspace(batch, num_q_heads, head_dim, capacity, exact_window, with_mass != 0);
+}
+
+int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, const void* v_codes, const void* k_scales,
+                             const void* v_scales, const int32_t* counts, float* mass, const int32_t* lengths,
+                             const void* k_exact, const void* v_exact, float* exact_mass, int64_t* seq_state,
+                             int advance, int64_t exact_len, const int64_t* strides, float sm_scale, int dtype,
+                             int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim, int64_t capacity,
+                             int64_t exact_window, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* nm = "dab_decode_attention_kv4";
+  if (!q || !out || !lengths || !strides || (!counts && capacity > 0)) return fail(1, std::string(nm) + ": null pointer");
+  if (dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": queries must be bf16 or fp16");
+  if (kv_group < 1 || kv_group > 1024) return fail(1, std::string(nm) + ": need 1 to 1024 q-heads per kv-head");
+  if (exact_window < 0 || exact_window >= (int64_t{1} << 30) || capacity < 0 || capacity >= (int64_t{1} << 30))
+    return fail(1, std::string(nm) + ": bad sizes");
+  if (exact_window > 0 && (!k_exact || !v_exact)) return fail(1, std::string(nm) + ": null pointer");
+  if (!seq_state && (exact_len < 0 || exact_len > exact_window || advance))
+    return fail(1, std::string(nm) + ": exact_len must be in [0, exact_window], and advance needs seq_state");
+  if (mass && exact_window > 0 && !exact_mass) return fail(1, std::string(nm) + ": mass needs exact_mass");
+  // strides: q(2) out(2) codes(2) scales(2) meta(2) lengths(2) exact(3) exact_mass(2) = 17
+  const int64_t* s = strides;
+  if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, s + 4, s + 6, batch, heads, capacity, head_dim)) return rc;
+  const uintptr_t any = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_exact) |
+                        reinterpret_cast<uintptr_t>(v_exact);
+  if (any % 16 || (s[0] | s[1] | s[12] | s[13] | s[14]) % 8)
+    return fail(1, std::string(nm) + ": query and exact rows must be 16-byte aligned");
+  if (!workspace || workspace_bytes < kv4_attn_workspace(batch, heads * kv_group, head_dim, capacity, exact_window,
+                                                         mass != nullptr))
+    return fail(1, std::string(nm) + ": workspace too small");
+  Kv4Attn p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q; p.qb = s[0]; p.qh = s[1];
+  p.out = out; p.ob = s[2]; p.oh = s[3];
+  p.hist = kv4_hist(k_codes, v_codes, k_scales, v_scales, s + 4, s + 6);
+  p.counts = counts; p.mass = mass; p.mb = s[8]; p.mh = s[9];
+  p.lengths = lengths; p.lb = s[10]; p.lh = s[11];
+  p.k_exact = k_exact; p.v_exact = v_exact; p.eb = s[12]; p.eh = s[13]; p.en = s[14];
+  p.exact_mass = exact_mass; p.emb = s[15]; p.emh = s[16];
+  p.state = seq_state; p.lag = seq_state && advance ? 1 : 0;
+  p.exact_len = static_cast<int>(exact_len);
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.B = static_cast<int>(batch); p.H = static_cast<int>(heads); p.G = static_cast<int>(kv_group);
+  p.cap = static_cast<int>(capacity); p.W = static_cast<int>(exact_window);
+  return cuda_status(launch_kv4_attn(dtype, head_dim, p, static_cast<uint8_t*>(workspace),
+                                     static_cast<cudaStream_t>(stream)),
+                     "decode_attention_kv4");
+}
+
+size_t dab_evict_by_mass_workspace_size(int64_t batch, int64_t heads, int64_t capacity) {
+  if (batch < 0 || heads < 0 || capacity < 0) return 0;
+  return evict_workspace(batch, heads, capacity);
+}
+
+int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths, const int64_t* length_strides,
+                      int64_t num_rows, void* const* rows, const int64_t* row_bytes, const int64_t* row_strides,
+                      int64_t batch, int64_t heads, int64_t capacity, int64_t budget, int64_t trigger,
+                      int64_t keep_first, int64_t keep_recent, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* nm = "dab_evict_by_mass";
+  if (!mass || !lengths || !mass_strides || !length_strides) return fail(1, std::string(nm) + ": null pointer");
+  if (num_rows < 0 || num_rows > EVICT_MAX_ROWS)
+    return fail(1, std::string(nm) + ": at most " + std::to_string(EVICT_MAX_ROWS) + " row buffers");
+  if (num_rows > 0 && (!rows || !row_bytes || !row_strides)) return fail(1, std::string(nm) + ": null pointer");
+  if (batch < 0 || heads < 0 || batch * heads > 65535 || capacity < 0 || capacity >= (int64_t{1} << 30))
+    return fail(1, std::string(nm) + ": need batch * heads <= 65535 and capacity below 2^30");
+  if (budget < 1 || keep_first < 0 || keep_recent < 0 || keep_first > budget || keep_recent > budget - keep_first)
+    return fail(1, std::string(nm) + ": need budget >= 1 and keep_first + keep_recent <= budget");
+  if (trigger < budget) return fail(1, std::string(nm) + ": trigger must be at least budget");
+  if (!workspace || workspace_bytes < evict_workspace(batch, heads, capacity))
+    return fail(1, std::string(nm) + ": workspace too small");
+  EvictParams p;
+  std::memset(&p, 0, sizeof(p));
+  for (int64_t i = 0; i < num_rows; ++i) {
+    if (!rows[i]) return fail(1, std::string(nm) + ": null pointer");
+    if (row_bytes[i] < 4 || row_bytes[i] > 65536)
+      return fail(1, std::string(nm) + ": rows must have 4 to 65536 bytes");
+    const uint64_t all = reinterpret_cast<uintptr_t>(rows[i]) | static_cast<uint64_t>(row_strides[2 * i]) |
+                         static_cast<uint64_t>(row_strides[2 * i + 1]) | static_cast<uint64_t>(row_bytes[i]);
+    if (all % 4) return fail(1, std::string(nm) + ": rows must be multiples of 4 bytes, 4-byte aligned");
+    p.row[i] = static_cast<uint8_t*>(rows[i]);
+    p.rb[i] = row_strides[2 * i];
+    p.rh[i] = row_strides[2 * i + 1];
+    p.bytes[i] = static_cast<int>(row_bytes[i]);
+    p.unit[i] = all % 16 == 0 ? 16 : all % 8 == 0 ? 8 : 4;
+  }
+  if (budget >= capacity) return 0;  // no head can be longer
+  p.mass = mass; p.mb = mass_strides[0]; p.mh = mass_strides[1];
+  p.lengths = lengths; p.lb = length_strides[0]; p.lh = length_strides[1];
+  p.n_rows = static_cast<int>(num_rows);
+  p.B = static_cast<int>(batch); p.H = static_cast<int>(heads); p.cap = static_cast<int>(capacity);
+  p.budget = static_cast<int>(budget);
+  p.trigger = static_cast<int>(trigger < capacity ? trigger : capacity);
+  p.first = static_cast<int>(keep_first); p.recent = static_cast<int>(keep_recent);
+  return cuda_status(launch_evict(p, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream)),
+                     "evict_by_mass");
 }
 
 }  // extern "C"

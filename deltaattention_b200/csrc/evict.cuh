@@ -1,0 +1,23 @@
+// Parameters of the eviction by accumulated attention weight (evict.cu).
+#pragma once
+#include "common.cuh"
+
+namespace dab {
+
+constexpr int EVICT_MAX_ROWS = 8;
+
+struct EvictParams {
+  float* mass; int64_t mb, mh;           // [B, H, cap], strides in elements
+  int32_t* lengths; int64_t lb, lh;      // [B, H]
+  // row buffers moved with the mass: base, strides over batch and head in bytes, bytes per row,
+  // and the widest unit (4, 8 or 16 bytes) that its base, strides and rows are multiples of
+  uint8_t* row[EVICT_MAX_ROWS];
+  int64_t rb[EVICT_MAX_ROWS], rh[EVICT_MAX_ROWS];
+  int bytes[EVICT_MAX_ROWS], unit[EVICT_MAX_ROWS];
+  int n_rows;
+  int B, H, cap;
+  int budget, trigger, first, recent;
+  uint2* cut;                            // workspace: (threshold key, ties kept) per head
+};
+
+}  // namespace dab

@@ -628,6 +628,316 @@ def release_host_prefill_buffers():
     _host_ws.clear()
 
 
+@dataclass
+class KV4:
+    """K and V rows of a decode history in 4 bits: codes [B, Hkv, M, d / 2] uint8 and scales
+    [B, Hkv, M, d / 16] bf16 (per row, d / 32 scales and then d / 32 zeros; the layout of the codes
+    is given in ``include/deltaattn_b200.h``). K and V have the same shapes and strides, rows are
+    contiguous; views of a larger cache are fine."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+    @staticmethod
+    def empty(batch, heads, rows, head_dim, device) -> "KV4":
+        shp = (batch, heads, rows)
+        c = [torch.empty((*shp, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
+        s = [torch.empty((*shp, head_dim // 16), dtype=torch.bfloat16, device=device) for _ in range(2)]
+        return KV4(c[0], s[0], c[1], s[1])
+
+    def rows(self, n0, n1) -> "KV4":
+        """The rows [n0, n1) of every head, as views."""
+        return KV4(*(t[:, :, n0:n1] for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales)))
+
+    def check(self, what, shape=None):
+        """Raises unless the four tensors are one history (of ``shape`` (B, Hkv, M, d), when given);
+        returns that shape."""
+        kc, ks, vc, vs = self.k_codes, self.k_scales, self.v_codes, self.v_scales
+        L.require_cuda(kc, ks, vc, vs)
+        if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.bfloat16 or vs.dtype != torch.bfloat16:
+            raise TypeError(f"{what}: codes are uint8 and scales bf16")
+        B, H, M, half = kc.shape
+        if half not in (32, 64):
+            raise ValueError(f"{what}: head_dim must be 64 or 128")
+        if vc.shape != kc.shape or ks.shape != (B, H, M, half // 8) or vs.shape != ks.shape:
+            raise ValueError(f"{what}: codes must be [B, H, M, d / 2] and scales [B, H, M, d / 16], alike for K and V")
+        if (kc.stride() != vc.stride() or ks.stride() != vs.stride() or kc.stride(3) != 1 or ks.stride(3) != 1
+                or (M > 1 and (kc.stride(2) != half or ks.stride(2) != half // 8))):
+            raise ValueError(f"{what}: rows must be contiguous, with the same strides for K and V")
+        if shape is not None and shape != (B, H, M, 2 * half):
+            raise ValueError(f"{what}: history is {(B, H, M, 2 * half)}, expected {shape}")
+        return B, H, M, 2 * half
+
+
+def _same_device(what, first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: tensors are on {first.device} and {t.device}")
+
+
+def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) -> KV4:
+    """K and V rows [B, Hkv, M, d] (any strides; bf16 / fp16, d 64 or 128) in 4 bits.
+
+    Per group of 32 elements of a row: zero = its minimum rounded down to bf16, scale = (maximum -
+    zero) / 15 rounded to bf16, code = round((x - zero) / scale) to even, cut to [0, 15]. A group
+    that holds a NaN or an infinity reads back as NaN. ``out`` may be views of a cache
+    (``KV4.rows``)."""
+    L.require_cuda(k, v)
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("kv4_quantize: k and v must be [B, H, M, d] of one shape and dtype")
+    B, H, M, D = k.shape
+    if k.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError("kv4_quantize: rows must be bf16 or fp16")
+    if D not in (64, 128):
+        raise ValueError("kv4_quantize: head_dim must be 64 or 128")
+    if out is None:
+        out = KV4.empty(B, H, M, D, k.device)
+    else:
+        out.check("kv4_quantize", (B, H, M, D))
+    _same_device("kv4_quantize", k, v, out.k_codes, out.k_scales, out.v_codes, out.v_scales)
+    if k.numel() == 0:
+        return out
+    L.check(L.load().dab_kv4_quantize(
+        L.ptr(k), L.strides(k.stride()), L.ptr(v), L.strides(v.stride()), L.ptr(out.k_codes), L.ptr(out.v_codes),
+        L.strides(out.k_codes.stride()), L.ptr(out.k_scales), L.ptr(out.v_scales), L.strides(out.k_scales.stride()),
+        L.dtype_code(k), B, H, M, D, L.stream_of(k)), "kv4_quantize")
+    return out
+
+
+def kv4_dequantize(hist: KV4, dtype: torch.dtype = torch.bfloat16):
+    """The K and V rows that a 4-bit history stands for, [B, Hkv, M, d] each, rounded to ``dtype``
+    (bf16, fp16 or fp32) from fp32."""
+    B, H, M, D = hist.check("kv4_dequantize")
+    _same_device("kv4_dequantize", hist.k_codes, hist.k_scales, hist.v_codes, hist.v_scales)
+    k = torch.empty((B, H, M, D), dtype=dtype, device=hist.k_codes.device)
+    v = torch.empty_like(k)
+    if k.numel() == 0:
+        L.dtype_code(k)
+        return k, v
+    L.check(L.load().dab_kv4_dequantize(
+        L.ptr(hist.k_codes), L.ptr(hist.v_codes), L.strides(hist.k_codes.stride()), L.ptr(hist.k_scales),
+        L.ptr(hist.v_scales), L.strides(hist.k_scales.stride()), L.ptr(k), L.ptr(v), L.strides(k.stride()),
+        L.dtype_code(k), B, H, M, D, L.stream_of(k)), "kv4_dequantize")
+    return k, v
+
+
+def _plane(what, name, t, shape, dtype):
+    """Checks a per-entry tensor ([B, Hkv, n], contiguous along n)."""
+    if t.dtype != dtype or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+        raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)}, contiguous along the last dimension")
+
+
+def _exact_window(what, k_exact, v_exact, B, H, D, dtype):
+    """(W, strides) of the exact window's K / V rows."""
+    if k_exact.shape != v_exact.shape or k_exact.stride() != v_exact.stride() or k_exact.dtype != dtype \
+            or v_exact.dtype != dtype:
+        raise ValueError(f"{what}: k_exact and v_exact must agree in shape, strides and dtype with each other and "
+                         f"the token ({dtype})")
+    if k_exact.dim() != 4 or k_exact.shape[:2] != (B, H) or k_exact.shape[3] != D or k_exact.stride(3) != 1:
+        raise ValueError(f"{what}: the exact window must be [{B}, {H}, W, {D}] with contiguous rows")
+    return k_exact.shape[2], k_exact.stride()[:3]
+
+
+def decode_update_kv4(k_new, v_new, hist: KV4, counts, timestamps, lengths, last_key, k_exact, v_exact, seq_state, *,
+                      threshold: float, similarity: str = "euclidean", mass=None, exact_mass=None, err=None):
+    """Takes one token per (batch, kv-head) into a 4-bit decode cache (deltaDecoding.py:9-104).
+
+    k_new / v_new [B, Hkv, 1, d]. When the exact ring [B, Hkv, W, d] is full, the token in the new
+    one's slot is compared with ``last_key`` [B, Hkv, d], the last anchor's key in 16 bits, as
+    ``decode_update`` compares with the last packed key (``threshold`` raw, squared for Euclidean):
+    near ones add 1 to the last anchor's count, others are appended in 4 bits with count 1 and
+    timestamp total - W. ``mass`` [B, Hkv, capacity] and ``exact_mass`` [B, Hkv, W] (fp32; both or
+    neither) are the attention weight that entries have drawn; a slot's goes with its token. The
+    (exact, total) lengths in ``seq_state`` (int64 on the device) are read and not advanced. An
+    append to a full history writes 0x201 into ``err`` (int32 on the device) and nothing else."""
+    what = "decode_update_kv4"
+    B, H, cap, D = hist.check(what)
+    L.require_cuda(k_new, v_new, counts, timestamps, lengths, last_key, k_exact, v_exact, seq_state, mass, exact_mass, err)
+    if k_new.shape != (B, H, 1, D) or v_new.shape != k_new.shape:
+        raise ValueError(f"{what}: k_new and v_new must be [{B}, {H}, 1, {D}]")
+    if k_new.dtype not in (torch.bfloat16, torch.float16) or v_new.dtype != k_new.dtype:
+        raise TypeError(f"{what}: tokens must be bf16 or fp16")
+    W, es = _exact_window(what, k_exact, v_exact, B, H, D, k_new.dtype)
+    if last_key.shape != (B, H, D) or last_key.dtype != k_new.dtype or last_key.stride(2) != 1:
+        raise ValueError(f"{what}: last_key must be {k_new.dtype} [{B}, {H}, {D}] with contiguous rows")
+    _plane(what, "counts", counts, (B, H, cap), torch.int32)
+    _plane(what, "timestamps", timestamps, (B, H, cap), torch.int32)
+    if lengths.shape != (B, H) or lengths.dtype != torch.int32:
+        raise ValueError(f"{what}: lengths must be int32 [{B}, {H}]")
+    if seq_state.shape != (2,) or seq_state.dtype != torch.int64 or not seq_state.is_contiguous():
+        raise ValueError(f"{what}: seq_state must be int64 [2]")
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+        raise ValueError(f"{what}: err must be int32")
+    if (mass is None) != (exact_mass is None):
+        raise ValueError(f"{what}: mass and exact_mass come together")
+    em = (0, 0)
+    if mass is not None:
+        _plane(what, "mass", mass, (B, H, cap), torch.float32)
+        _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
+        em = exact_mass.stride()[:2]
+    ms = counts.stride()[:2]
+    if timestamps.stride()[:2] != ms or (mass is not None and mass.stride()[:2] != ms):
+        raise ValueError(f"{what}: counts, timestamps and mass must have the same strides")
+    if W < 1:
+        raise ValueError(f"{what}: the exact window needs at least one row")
+    _same_device(what, k_new, v_new, hist.k_codes, counts, lengths, last_key, k_exact, seq_state, mass, exact_mass, err)
+    if k_new.numel() == 0:
+        return
+    use_cos = similarity == "cosine"
+    kn, vn = k_new.stride(), v_new.stride()
+    strides = L.strides((kn[0], kn[1], kn[3], vn[0], vn[1], vn[3], *hist.k_codes.stride()[:2],
+                         *hist.k_scales.stride()[:2], *ms, *lengths.stride(), *last_key.stride()[:2], *es, *em))
+    L.check(L.load().dab_decode_update_kv4(
+        L.ptr(k_new), L.ptr(v_new), L.ptr(hist.k_codes), L.ptr(hist.v_codes), L.ptr(hist.k_scales),
+        L.ptr(hist.v_scales), L.ptr(counts), L.ptr(timestamps), L.ptr(mass), L.ptr(lengths), L.ptr(last_key),
+        L.ptr(k_exact), L.ptr(v_exact), L.ptr(exact_mass), L.ptr(seq_state), strides,
+        float(threshold if use_cos else threshold ** 2), 1 if use_cos else 0, L.dtype_code(k_new), B, H, D, cap, W,
+        L.ptr(err), L.stream_of(k_new)), what)
+
+
+def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=None, *, exact_len=None, seq_state=None,
+                         advance=False, mass=None, exact_mass=None, sm_scale=None, out=None, workspace=None):
+    """One token's attention over a 4-bit history and the exact window (deltaDecoding.py:236-362).
+
+    q [B, Hq, d] (bf16 / fp16, d 64 or 128), q-head h reads kv-head h // (Hq / Hkv). History entry j
+    of a head takes part when j < ``lengths`` [B, Hkv] (int32) and ``counts`` [B, Hkv, capacity]
+    (int32) is positive, with score sm_scale q.k_j + log(count_j); then the first ``exact_len``
+    rows of k_exact / v_exact [B, Hkv, W, d] (all by default; with ``seq_state``, int64 (exact,
+    total) on the device, the smaller of its exact length and W, and ``advance`` as in
+    ``DeviceDecodeCache.attend``). A row with no entry gives 0.
+
+    With ``mass`` [B, Hkv, capacity] and ``exact_mass`` [B, Hkv, W] (fp32), every entry's attention
+    weight, summed over the q-heads of its kv-head, is added to them: what ``evict_by_mass`` goes
+    by. ``workspace`` (uint8, zero-filled once, ``kv4_attention_workspace`` bytes, used by one
+    stream at a time) replaces the library's own. Returns out [B, Hq, d]."""
+    what = "decode_attention_kv4"
+    B, H, cap, D = hist.check(what)
+    L.require_cuda(q, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.shape[1] % max(H, 1) or q.stride(2) != 1:
+        raise ValueError(f"{what}: q must be [{B}, a multiple of {H}, {D}] with contiguous rows")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: queries must be bf16 or fp16")
+    Hq = q.shape[1]
+    _plane(what, "counts", counts, (B, H, cap), torch.int32)
+    if lengths.shape != (B, H) or lengths.dtype != torch.int32:
+        raise ValueError(f"{what}: lengths must be int32 [{B}, {H}]")
+    W, es = 0, (0, 0, 0)
+    if (k_exact is None) != (v_exact is None):
+        raise ValueError(f"{what}: k_exact and v_exact come together")
+    if k_exact is not None:
+        W, es = _exact_window(what, k_exact, v_exact, B, H, D, q.dtype)
+    if seq_state is None:
+        exact_len = W if exact_len is None else int(exact_len)
+        if not 0 <= exact_len <= W:
+            raise ValueError(f"{what}: exact_len must be in [0, {W}]")
+        if advance:
+            raise ValueError(f"{what}: advance needs seq_state")
+    else:
+        if exact_len is not None:
+            raise ValueError(f"{what}: exact_len comes from seq_state")
+        if seq_state.shape != (2,) or seq_state.dtype != torch.int64 or not seq_state.is_contiguous():
+            raise ValueError(f"{what}: seq_state must be int64 [2]")
+        exact_len = 0
+    if (mass is None) != (exact_mass is None) and (mass is None or W > 0):
+        raise ValueError(f"{what}: mass and exact_mass come together")
+    ms, em = counts.stride()[:2], (0, 0)
+    if mass is not None:
+        _plane(what, "mass", mass, (B, H, cap), torch.float32)
+        if mass.stride()[:2] != ms:
+            raise ValueError(f"{what}: counts and mass must have the same strides")
+        if exact_mass is not None:
+            _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
+            em = exact_mass.stride()[:2]
+    if out is None:
+        out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError(f"{what}: out must be like q, with contiguous rows")
+    _same_device(what, q, hist.k_codes, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
+    if out.numel() == 0:
+        return out
+    lib = L.load()
+    st = L.stream_of(q)
+    if workspace is None:
+        nbytes = lib.dab_decode_attention_kv4_workspace_size(B, Hq, D, cap, W, 1 if mass is not None else 0)
+        workspace = L.workspace(q.device, st.value, nbytes, tag="kv4")
+    strides = L.strides((*q.stride()[:2], *out.stride()[:2], *hist.k_codes.stride()[:2], *hist.k_scales.stride()[:2],
+                         *ms, *lengths.stride(), *es, *em))
+    L.check(lib.dab_decode_attention_kv4(
+        L.ptr(q), L.ptr(out), L.ptr(hist.k_codes), L.ptr(hist.v_codes), L.ptr(hist.k_scales), L.ptr(hist.v_scales),
+        L.ptr(counts), L.ptr(mass), L.ptr(lengths), L.ptr(k_exact), L.ptr(v_exact), L.ptr(exact_mass),
+        L.ptr(seq_state), 1 if advance else 0, exact_len, strides, float(D ** -0.5 if sm_scale is None else sm_scale),
+        L.dtype_code(q), B, H, Hq // H, D, cap, W, L.ptr(workspace), workspace.numel(), st), what)
+    return out
+
+
+def kv4_attention_workspace(batch, q_heads, head_dim, capacity, exact_window, with_mass=True) -> int:
+    """Bytes of the ``workspace`` that ``decode_attention_kv4`` takes."""
+    return int(L.load().dab_decode_attention_kv4_workspace_size(batch, q_heads, head_dim, capacity, exact_window,
+                                                                1 if with_mass else 0))
+
+
+def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = None, keep_first: int = 0,
+                  keep_recent: int = 0, workspace=None):
+    """Cuts a decode cache to the entries that drew the most attention, in place.
+
+    Every (batch, head) with more than ``trigger`` (default ``budget``) entries keeps ``budget`` of
+    them: the first ``keep_first``, the last ``keep_recent`` and, of those between, the ones with
+    the largest ``mass`` [B, H, capacity] (fp32; ties go to the lowest index, NaN is the lightest).
+    Entries keep their order; mass and every tensor of ``rows`` ([B, H, capacity, ...], up to 8,
+    contiguous from the third dimension on, entries of a multiple of 4 bytes) move together, and
+    ``lengths`` [B, H] (int32) become ``budget``. Slots from ``budget`` on keep what they held.
+    Lengths are read on the device: no host synchronisation, and the call can be captured in a
+    CUDA graph and replayed at every token, where it only does work once a head passes
+    ``trigger``. ``workspace`` as in ``decode_attention_kv4`` (``evict_workspace`` bytes)."""
+    what = "evict_by_mass"
+    L.require_cuda(mass, lengths, workspace, *rows)
+    if mass.dim() != 3 or mass.dtype != torch.float32 or (mass.shape[2] > 1 and mass.stride(2) != 1):
+        raise ValueError(f"{what}: mass must be fp32 [B, H, capacity], contiguous along the last dimension")
+    B, H, cap = mass.shape
+    if lengths.shape != (B, H) or lengths.dtype != torch.int32:
+        raise ValueError(f"{what}: lengths must be int32 [{B}, {H}]")
+    budget = int(budget)
+    trigger = budget if trigger is None else int(trigger)
+    if budget < 1 or keep_first < 0 or keep_recent < 0 or keep_first + keep_recent > budget:
+        raise ValueError(f"{what}: need budget >= 1 and keep_first + keep_recent <= budget")
+    if trigger < budget:
+        raise ValueError(f"{what}: trigger must be at least budget")
+    if len(rows) > 8:
+        raise ValueError(f"{what}: at most 8 row tensors")
+    ptrs, nbytes, strides = [], [], []
+    for t in rows:
+        if t.dim() < 3 or t.shape[:3] != (B, H, cap):
+            raise ValueError(f"{what}: row tensors must be [{B}, {H}, {cap}, ...]")
+        size, n = t.element_size(), 1
+        for d in range(t.dim() - 1, 1, -1):
+            if t.shape[d] > 1 and t.stride(d) != n:
+                raise ValueError(f"{what}: row tensors must be contiguous from the third dimension on")
+            n *= t.shape[d]
+        n //= max(cap, 1)
+        if cap and ((n * size) % 4 or n == 0 or t.data_ptr() % 4):
+            raise ValueError(f"{what}: row entries must be multiples of 4 bytes, 4-byte aligned")
+        ptrs.append(t.data_ptr())
+        nbytes.append(n * size)
+        strides += [t.stride(0) * size, t.stride(1) * size]
+    _same_device(what, mass, lengths, workspace, *rows)
+    if B == 0 or H == 0 or cap == 0:
+        return
+    lib = L.load()
+    st = L.stream_of(mass)
+    if workspace is None:
+        workspace = L.workspace(mass.device, st.value, lib.dab_evict_by_mass_workspace_size(B, H, cap), tag="evict")
+    L.check(lib.dab_evict_by_mass(
+        L.ptr(mass), L.strides(mass.stride()[:2]), L.ptr(lengths), L.strides(lengths.stride()), len(ptrs),
+        (L.P * len(ptrs))(*ptrs), L.strides(nbytes), L.strides(strides), B, H, cap, budget, trigger, int(keep_first),
+        int(keep_recent), L.ptr(workspace), workspace.numel(), st), what)
+
+
+def evict_workspace(batch, heads, capacity) -> int:
+    """Bytes of the ``workspace`` that ``evict_by_mass`` takes."""
+    return int(L.load().dab_evict_by_mass_workspace_size(batch, heads, capacity))
+
+
 def tile_count_periodic(N: int, r: int, W: int = 128) -> int:
     """128x128 tiles one head runs under the reference schedule with periodic-r packing."""
     nb = -(-N // 128)

@@ -336,6 +336,80 @@ int dab_nm_select(const void* k, const int64_t* k_strides, int32_t* keep_mask, c
 /* Anchors per head that dab_nm_select keeps. */
 int64_t dab_nm_num_packed(int64_t seq_len, int64_t n_keep, int64_t m_group, int64_t stride);
 
+/* A decode history in 4 bits (no counterpart in the reference, whose cache is 16-bit). K and V
+ * rows are kept as codes [B, H, capacity, head_dim / 2] bytes and scales [B, H, capacity,
+ * head_dim / 16] bf16, both with contiguous rows. Per group g of 32 elements of a row, in fp32:
+ *   zero  = min rounded down to bf16;  scale = (max - zero) * (1 / 15) rounded to bf16;
+ *   code  = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0;  value = zero + scale * code.
+ * A group with an element that is not finite reads back as NaN. With NG = head_dim / 32, word
+ * t * NG + g (32 bits, t = 0..3) of a row's codes holds elements 32 g + 8 t + i in bits 4 i..;
+ * a row's scales are its NG scales, then its NG zeros. bf16 / fp16 rows, head_dim 64 or 128,
+ * batch * heads <= 65535. Code rows must be 16-byte aligned, scale rows aligned to their size.
+ * `code_strides` (bytes) and `scale_strides` (elements) are over (batch, head) and hold for K
+ * and V.
+ *
+ * dab_kv4_quantize: K and V rows [B, H, rows, head_dim] (strides b, h, n, d) into 4 bits. */
+int dab_kv4_quantize(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, void* k_codes,
+                     void* v_codes, const int64_t* code_strides, void* k_scales, void* v_scales,
+                     const int64_t* scale_strides, int dtype, int64_t batch, int64_t heads, int64_t rows,
+                     int64_t head_dim, void* stream);
+/* The values of both, rounded to `dtype` (DAB_F32 too); `out_strides` (b, h, n) hold for k and v,
+ * whose rows are contiguous. */
+int dab_kv4_dequantize(const void* k_codes, const void* v_codes, const int64_t* code_strides, const void* k_scales,
+                       const void* v_scales, const int64_t* scale_strides, void* k, void* v,
+                       const int64_t* out_strides, int dtype, int64_t batch, int64_t heads, int64_t rows,
+                       int64_t head_dim, void* stream);
+/* dab_decode_update_dev on a 4-bit history: the token that leaves the full exact ring is merged
+ * into the last anchor or appended in 4 bits. It is compared with `last_key` [B, H, head_dim], the
+ * last anchor's key in 16 bits, so decisions are those of the 16-bit cache; an append replaces
+ * it. `mass` [B, H, capacity] and `exact_mass` [B, H, exact_window] (fp32, may be NULL) are the
+ * attention weight every entry has drawn: the ring slot's goes with the token and starts again at
+ * 0. `threshold` is the squared distance, or the cosine. An append past `capacity` writes 0x201
+ * into `err_word` (may be NULL) instead of memory.
+ * `strides` (21): k_new (b, h, d), v_new (b, h, d), codes (b, h), scales (b, h), counts /
+ * timestamps / mass (b, h), lengths (b, h), last_key (b, h), exact K / V (b, h, row),
+ * exact_mass (b, h). */
+int dab_decode_update_kv4(const void* k_new, const void* v_new, void* k_codes, void* v_codes, void* k_scales,
+                          void* v_scales, int32_t* counts, int32_t* timestamps, float* mass, int32_t* lengths,
+                          void* last_key, void* k_exact, void* v_exact, float* exact_mass, const int64_t* seq_state,
+                          const int64_t* strides, float threshold, int use_cosine, int dtype, int64_t batch,
+                          int64_t heads, int64_t head_dim, int64_t capacity, int64_t exact_window, int* err_word,
+                          void* stream);
+/* Scratch bytes dab_decode_attention_kv4 needs. Zero it once, then reuse it on one stream. */
+size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t num_q_heads, int64_t head_dim, int64_t capacity,
+                                               int64_t exact_window, int with_mass);
+/* Single-token attention over a 4-bit history and the exact window: q / out [B, heads * kv_group,
+ * head_dim], scores sm_scale * q . k + log(count) over history entries below the head's length
+ * with a positive count (others draw nothing, whatever they hold) and sm_scale * q . k over the
+ * first exact_len window rows. A query row with no entry left gives 0. With `mass` (fp32, else
+ * NULL) every entry's attention weight, summed over the kv-head's q-heads, is added to mass and
+ * exact_mass. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
+ * and `advance` as in dab_decode_attention_dev; without it exact_len is the argument.
+ * `strides` (17): q (b, h), out (b, h), codes (b, h), scales (b, h), counts / mass (b, h), lengths
+ * (b, h), exact K / V (b, h, row), exact_mass (b, h). Query and exact rows contiguous, 16-byte
+ * aligned. */
+int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, const void* v_codes, const void* k_scales,
+                             const void* v_scales, const int32_t* counts, float* mass, const int32_t* lengths,
+                             const void* k_exact, const void* v_exact, float* exact_mass, int64_t* seq_state,
+                             int advance, int64_t exact_len, const int64_t* strides, float sm_scale, int dtype,
+                             int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim, int64_t capacity,
+                             int64_t exact_window, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Scratch bytes dab_evict_by_mass needs. Zero it once, then reuse it on one stream. */
+size_t dab_evict_by_mass_workspace_size(int64_t batch, int64_t heads, int64_t capacity);
+/* Eviction from a cache by accumulated attention weight (no counterpart in the reference). Every
+ * (batch, head) longer than `trigger` (>= budget) is cut to `budget` entries: its first
+ * `keep_first`, its last `keep_recent`, and of the others those with the largest mass, ties to
+ * the lowest index (NaN counts as lighter than anything). Kept entries keep their order; mass
+ * [B, H, capacity] and every row buffer are compacted in place (slots from `budget` on keep what
+ * they held) and the length [B, H] becomes `budget`. Row buffer i has `row_bytes[i]` contiguous
+ * bytes per entry (a multiple of 4) and strides over batch and head of row_strides[2 i], [2 i + 1]
+ * bytes; at most 8 buffers. Strides of mass and lengths (b, h) in elements. */
+int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths, const int64_t* length_strides,
+                      int64_t num_rows, void* const* rows, const int64_t* row_bytes, const int64_t* row_strides,
+                      int64_t batch, int64_t heads, int64_t capacity, int64_t budget, int64_t trigger,
+                      int64_t keep_first, int64_t keep_recent, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
