@@ -70,7 +70,7 @@ SIGNATURES = {
     "dab_kv4_quantize": (I32, [P, PI64, P, PI64, P, P, PI64, P, P, PI64, I32, I64, I64, I64, I64, P]),
     "dab_kv4_dequantize": (I32, [P, P, PI64, P, P, PI64, P, P, PI64, I32, I64, I64, I64, I64, P]),
     "dab_decode_update_kv4": (I32, [P] * 15 + [PI64, F32, I32, I32, I64, I64, I64, I64, I64, P, P]),
-    "dab_decode_attention_kv4_workspace_size": (SZ, [I64, I64, I64, I64, I64, I32]),
+    "dab_decode_attention_kv4_workspace_size": (SZ, [I64, I64, I64, I64, I64, I64, I32]),
     "dab_decode_attention_kv4": (I32, [P] * 13 + [I32, I64, PI64, F32, I32, I64, I64, I64, I64, I64, I64, P, SZ, P]),
     "dab_evict_by_mass_workspace_size": (SZ, [I64, I64, I64]),
     "dab_evict_by_mass": (I32, [P, PI64, P, PI64, I64, ctypes.POINTER(P), PI64, PI64, I64, I64, I64, I64, I64, I64, I64,

@@ -62,7 +62,7 @@ cudaError_t launch_kv4_dequantize(int, const Kv4Hist&, void*, void*, const int64
                                   cudaStream_t);
 cudaError_t launch_kv4_update(int, int64_t, bool, const Kv4Update&, cudaStream_t);
 cudaError_t launch_kv4_attn(int, int64_t, Kv4Attn, uint8_t*, cudaStream_t);
-size_t kv4_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, bool);
+size_t kv4_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, bool);
 cudaError_t launch_evict(EvictParams, uint8_t*, cudaStream_t);
 size_t evict_workspace(int64_t, int64_t, int64_t);
 }  // namespace dab
@@ -915,10 +915,10 @@ int dab_decode_update_kv4(const void* k_new, const void* v_new, void* k_codes, v
                      "decode_update_kv4");
 }
 
-size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t num_q_heads, int64_t head_dim, int64_t capacity,
-                                               int64_t exact_window, int with_mass) {
-  if (batch < 0 || num_q_heads < 0 || head_dim < 1 || capacity < 0 || exact_window < 0) return 0;
-  return kv4_attn_workspace(batch, num_q_heads, head_dim, capacity, exact_window, with_mass != 0);
+size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim,
+                                               int64_t capacity, int64_t exact_window, int with_mass) {
+  if (batch < 0 || heads < 0 || kv_group < 1 || head_dim < 1 || capacity < 0 || exact_window < 0) return 0;
+  return kv4_attn_workspace(batch, heads, kv_group, head_dim, capacity, exact_window, with_mass != 0);
 }
 
 int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, const void* v_codes, const void* k_scales,
@@ -936,7 +936,8 @@ int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, cons
   if (exact_window > 0 && (!k_exact || !v_exact)) return fail(1, std::string(nm) + ": null pointer");
   if (!seq_state && (exact_len < 0 || exact_len > exact_window || advance))
     return fail(1, std::string(nm) + ": exact_len must be in [0, exact_window], and advance needs seq_state");
-  if (mass && exact_window > 0 && !exact_mass) return fail(1, std::string(nm) + ": mass needs exact_mass");
+  if ((mass && exact_window > 0 && !exact_mass) || (exact_mass && capacity > 0 && !mass))
+    return fail(1, std::string(nm) + ": mass and exact_mass come together");
   // strides: q(2) out(2) codes(2) scales(2) meta(2) lengths(2) exact(3) exact_mass(2) = 17
   const int64_t* s = strides;
   if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, s + 4, s + 6, batch, heads, capacity, head_dim)) return rc;
@@ -944,8 +945,8 @@ int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, cons
                         reinterpret_cast<uintptr_t>(v_exact);
   if (any % 16 || (s[0] | s[1] | s[12] | s[13] | s[14]) % 8)
     return fail(1, std::string(nm) + ": query and exact rows must be 16-byte aligned");
-  if (!workspace || workspace_bytes < kv4_attn_workspace(batch, heads * kv_group, head_dim, capacity, exact_window,
-                                                         mass != nullptr))
+  if (!workspace || workspace_bytes < kv4_attn_workspace(batch, heads, kv_group, head_dim, capacity, exact_window,
+                                                         mass || exact_mass))
     return fail(1, std::string(nm) + ": workspace too small");
   Kv4Attn p;
   std::memset(&p, 0, sizeof(p));

@@ -1,5 +1,5 @@
 // A decode history in 4 bits (format in kv4.cuh): quantisation of packed K / V rows, reading
-// back, the single-token cache update and single-token attention.
+// back, and the single-token cache update.
 #include "kv4.cuh"
 
 namespace dab {
@@ -192,221 +192,6 @@ cudaError_t launch_kv4_update(int dtype, int64_t D, bool cosine, const Kv4Update
   if (D == 64) { DAB_U(__half, 64) }
   DAB_U(__half, 128)
 #undef DAB_U
-}
-
-// ----------------------------------------------------------------------------- attention
-// Split over the keys: a CTA scores 128 keys (history, then exact window) for up to 8 q-heads of
-// one kv-head, one key per thread, then sums the values one column per thread. Scores are kept in
-// log2 units without the count, which weights the exponential: p = count * 2^(z - max). A second
-// kernel joins the parts; with `mass` a third adds every key's share, from the scores that the
-// first one left in the workspace.
-constexpr int KV4_CHUNK = 128;
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_attn_kernel(Kv4Attn p) {
-  constexpr int NG = D / 32;
-  __shared__ float sq[8][D];
-  __shared__ float sp[8][KV4_CHUNK];
-  __shared__ float red[4][8];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
-  const int g0 = blockIdx.z * 8, ng = min(8, p.G - g0);
-  int64_t elen = p.exact_len;
-  if (p.state) elen = min(static_cast<int64_t>(p.W), p.state[0] + p.lag);
-  const int64_t n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
-  const int64_t total = n + elen, k0 = static_cast<int64_t>(blockIdx.x) * KV4_CHUNK;
-  float* part = p.part + ((static_cast<int64_t>(bh) * p.G + g0) * p.nsplit + blockIdx.x) * (D + 2);
-  if (k0 >= total) {
-    if (tid < ng) {
-      part[static_cast<int64_t>(tid) * p.nsplit * (D + 2)] = -INFINITY;
-      part[static_cast<int64_t>(tid) * p.nsplit * (D + 2) + 1] = 0.f;
-    }
-    return;
-  }
-  const T* q = static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + g0) * p.qh;
-  for (int i = tid; i < 8 * D; i += 128) {
-    const int g = i / D, d = i - g * D;
-    sq[g][d] = g < ng ? to_f32(q[g * p.qh + d]) * p.scale_log2 : 0.f;
-  }
-  __syncthreads();
-  const int64_t key = k0 + tid;
-  const bool old = key < n;
-  float c = key < total ? 1.f : 0.f;
-  if (old) c = static_cast<float>(max(0, p.counts[b * p.mb + h * p.mh + key]));
-  float z[8];
-#pragma unroll
-  for (int g = 0; g < 8; ++g) z[g] = 0.f;
-  if (c > 0.f) {
-    if (old) {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(p.hist.k_codes + b * p.hist.cb + h * p.hist.ch + key * (D / 2));
-      const __nv_bfloat16* s = p.hist.k_scales + b * p.hist.sb + h * p.hist.sh + key * (2 * NG);
-      for (int i = 0; i < D / 8; ++i) {
-        const int t = i / NG, gr = i - t * NG;
-        const uint32_t word = w[i];
-        const float sc = to_f32(s[gr]), ze = to_f32(s[NG + gr]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float x = fmaf(sc, static_cast<float>((word >> (4 * e)) & 15u), ze);
-#pragma unroll
-          for (int g = 0; g < 8; ++g) z[g] = fmaf(sq[g][32 * gr + 8 * t + e], x, z[g]);
-        }
-      }
-    } else {
-      const T* row = static_cast<const T*>(p.k_exact) + b * p.eb + h * p.eh + (key - n) * p.en;
-      for (int d = 0; d < D; ++d) {
-        const float x = to_f32(row[d]);
-#pragma unroll
-        for (int g = 0; g < 8; ++g) z[g] = fmaf(sq[g][d], x, z[g]);
-      }
-    }
-  }
-#pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    if (!(c > 0.f)) z[g] = -INFINITY;
-    float m = z[g];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (lane == 0) red[warp][g] = m;
-    if (p.scores && g < ng && key < total)
-      p.scores[(static_cast<int64_t>(bh) * p.G + g0 + g) * p.sstride + key] = z[g];
-  }
-  __syncthreads();
-  float mx[8];
-#pragma unroll
-  for (int g = 0; g < 8; ++g) mx[g] = fmaxf(fmaxf(red[0][g], red[1][g]), fmaxf(red[2][g], red[3][g]));
-  __syncthreads();
-#pragma unroll
-  for (int g = 0; g < 8; ++g) {
-    const float pr = c > 0.f ? c * ex2(z[g] - (mx[g] == -INFINITY ? 0.f : mx[g])) : 0.f;
-    sp[g][tid] = pr;
-    float l = pr;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    if (lane == 0) red[warp][g] = l;
-  }
-  __syncthreads();
-  const int kend = static_cast<int>(min(static_cast<int64_t>(KV4_CHUNK), total - k0));
-  if (tid < D) {
-    float acc[8];
-#pragma unroll
-    for (int g = 0; g < 8; ++g) acc[g] = 0.f;
-    const int gr = tid / 32, t = (tid / 8) & 3, e = tid & 7;
-    for (int j = 0; j < kend; ++j) {
-      const int64_t kk = k0 + j;
-      float x;
-      if (kk < n) {
-        if (p.counts[b * p.mb + h * p.mh + kk] <= 0) continue;
-        const uint32_t word = reinterpret_cast<const uint32_t*>(p.hist.v_codes + b * p.hist.cb + h * p.hist.ch + kk * (D / 2))[t * NG + gr];
-        const __nv_bfloat16* s = p.hist.v_scales + b * p.hist.sb + h * p.hist.sh + kk * (2 * NG);
-        x = fmaf(to_f32(s[gr]), static_cast<float>((word >> (4 * e)) & 15u), to_f32(s[NG + gr]));
-      } else {
-        x = to_f32(static_cast<const T*>(p.v_exact)[b * p.eb + h * p.eh + (kk - n) * p.en + tid]);
-      }
-#pragma unroll
-      for (int g = 0; g < 8; ++g) acc[g] = fmaf(sp[g][j], x, acc[g]);
-    }
-    for (int g = 0; g < ng; ++g) part[static_cast<int64_t>(g) * p.nsplit * (D + 2) + 2 + tid] = acc[g];
-  }
-  if (tid < ng) {
-    part[static_cast<int64_t>(tid) * p.nsplit * (D + 2)] = mx[tid];
-    part[static_cast<int64_t>(tid) * p.nsplit * (D + 2) + 1] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
-  }
-}
-
-// One CTA of D threads per q-head: out = sum of the parts' accumulators over their sums, 0 where
-// nothing is left; (max, 1 / sum) of the whole row for the mass.
-template <typename T, int D>
-__global__ void __launch_bounds__(D) kv4_join_kernel(Kv4Attn p) {
-  const int row = blockIdx.x;  // batch * q-heads
-  const float* part = p.part + static_cast<int64_t>(row) * p.nsplit * (D + 2);
-  float m = -INFINITY;
-  for (int s = 0; s < p.nsplit; ++s) m = fmaxf(m, part[static_cast<int64_t>(s) * (D + 2)]);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc = 0.f;
-  for (int s = 0; s < p.nsplit; ++s) {
-    const float* ps = part + static_cast<int64_t>(s) * (D + 2);
-    if (ps[0] == -INFINITY) continue;  // a part without keys has no accumulators
-    const float f = ex2(ps[0] - ref);
-    l = fmaf(ps[1], f, l);
-    acc = fmaf(ps[2 + threadIdx.x], f, acc);
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int hq = p.H * p.G, b = row / hq, h = row - b * hq;
-  static_cast<T*>(p.out)[b * p.ob + h * p.oh + threadIdx.x] = from_f32<T>(l == 0.f ? 0.f : acc * inv);
-  if (threadIdx.x == 0) {
-    p.stats[2 * row] = ref;
-    p.stats[2 * row + 1] = inv;
-    if (p.lag && row == 0) {  // the step's length advance, after the state's last reader
-      p.state[0] += 1;
-      p.state[1] += 1;
-    }
-  }
-}
-
-__global__ void __launch_bounds__(256) kv4_mass_kernel(Kv4Attn p) {
-  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
-  int64_t elen = p.exact_len;
-  if (p.state) elen = min(static_cast<int64_t>(p.W), p.state[0]);  // the join has advanced it
-  const int64_t n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
-  const int64_t key = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (key >= n + elen) return;
-  const float c = key < n ? static_cast<float>(max(0, p.counts[b * p.mb + h * p.mh + key])) : 1.f;
-  if (!(c > 0.f)) return;
-  float w = 0.f;
-  for (int g = 0; g < p.G; ++g) {
-    const int64_t row = static_cast<int64_t>(bh) * p.G + g;
-    w = fmaf(ex2(p.scores[row * p.sstride + key] - p.stats[2 * row]), p.stats[2 * row + 1], w);
-  }
-  float* dst = key < n ? p.mass + b * p.mb + h * p.mh + key : p.exact_mass + b * p.emb + h * p.emh + (key - n);
-  *dst += c * w;
-}
-
-namespace {
-struct Kv4Ws {
-  int nsplit;
-  int64_t sstride, part, scores, stats, total;  // offsets in bytes
-};
-Kv4Ws kv4_ws(int64_t B, int64_t Hq, int64_t D, int64_t cap, int64_t W, bool mass) {
-  auto up = [](int64_t x) { return (x + 255) & ~int64_t{255}; };
-  Kv4Ws w;
-  w.nsplit = static_cast<int>((cap + W + KV4_CHUNK - 1) / KV4_CHUNK);
-  if (w.nsplit < 1) w.nsplit = 1;
-  w.sstride = cap + W;
-  w.part = 256;
-  w.stats = w.part + up(B * Hq * w.nsplit * (D + 2) * 4);
-  w.scores = w.stats + up(B * Hq * 2 * 4);
-  w.total = w.scores + (mass ? up(B * Hq * w.sstride * 4) : 0);
-  return w;
-}
-}  // namespace
-
-size_t kv4_attn_workspace(int64_t B, int64_t Hq, int64_t D, int64_t cap, int64_t W, bool mass) {
-  return static_cast<size_t>(kv4_ws(B, Hq, D, cap, W, mass).total);
-}
-
-cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaStream_t st) {
-  const int64_t Hq = static_cast<int64_t>(p.H) * p.G;
-  if (p.B * Hq == 0) return cudaSuccess;
-  const Kv4Ws w = kv4_ws(p.B, Hq, D, p.cap, p.W, p.mass != nullptr);
-  p.nsplit = w.nsplit;
-  p.sstride = w.sstride;
-  p.part = reinterpret_cast<float*>(ws + w.part);
-  p.stats = reinterpret_cast<float*>(ws + w.stats);
-  p.scores = p.mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
-  dim3 grid(static_cast<unsigned>(w.nsplit), static_cast<unsigned>(p.B * p.H), static_cast<unsigned>((p.G + 7) / 8));
-#define DAB_A(TY, DD)                                                                    \
-  kv4_attn_kernel<TY, DD><<<grid, 128, 0, st>>>(p);                                       \
-  kv4_join_kernel<TY, DD><<<static_cast<unsigned>(p.B * Hq), DD, 0, st>>>(p);
-  if (dtype == BF16 && D == 64) { DAB_A(__nv_bfloat16, 64) }
-  else if (dtype == BF16) { DAB_A(__nv_bfloat16, 128) }
-  else if (D == 64) { DAB_A(__half, 64) }
-  else { DAB_A(__half, 128) }
-#undef DAB_A
-  if (p.mass) {
-    dim3 gm(static_cast<unsigned>((p.cap + p.W + 255) / 256), static_cast<unsigned>(p.B * p.H));
-    kv4_mass_kernel<<<gm, 256, 0, st>>>(p);
-  }
-  return cudaGetLastError();
 }
 
 }  // namespace dab

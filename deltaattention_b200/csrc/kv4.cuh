@@ -57,9 +57,11 @@ struct Kv4Attn {
   int exact_len;                                 // without state
   float scale_log2;                              // sm_scale * log2(e)
   int B, H, G, cap, W;                           // G q-heads per kv-head
-  // workspace
-  float* part; float* stats; float* scores;
-  int64_t sstride;
+  // workspace: per q-head row and split (max, sum) and the unscaled output, per q-head row the
+  // scores of history and window (null without mass)
+  float2* stats; float* part; float* scores;
+  int* used;                                     // with state: the window length this call attends with
+  int64_t sstride;                               // scores per row: cap + W
   int nsplit;
 };
 

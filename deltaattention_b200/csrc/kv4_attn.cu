@@ -1,0 +1,689 @@
+// Single-token attention over a decode history in 4 bits and an exact window in 16 bits.
+//
+// z_hj = sm_scale * q_h . k_j, p_hj = count_j exp(z_hj - max_h), out_h = sum_j p_hj v_j / sum_j p_hj.
+// With k_jd = zero_jg + scale_jg code_jd (g = d / 32) both products are sums over codes:
+//   q . k_j  = sum_g scale_jg (sum_{d in g} q_d code_jd) + sum_g zero_jg qsum_g
+//   sum_j p_j v_jd = sum_j (p_j scale_jg) code_jd + sum_j p_j zero_jg
+// so the matrix instructions take the codes themselves: a code in the mantissa of 16.0 is the
+// 16-bit number 16 + code (one shift and one and-or for two codes), and the 16 is taken off
+// through the zero terms. Nothing is dequantised and q is not rounded.
+//  * Scores: keys are the rows of the product, q-heads its 8 columns. One accumulator per group,
+//    multiplied by the group's scale in fp32. The zero terms are two more products whose rows are
+//    the stored (scales, zeros) and whose columns hold qsum_g and -16 qsum_g in three bf16 parts
+//    (24 bits).
+//  * Values: elements are the rows, q-heads the columns. p scale_g goes in as two bf16 parts, high
+//    and the rest (16 bits of every weight); p alone, in two parts, times the stored (scales,
+//    zeros) gives what is taken off and added at the end.
+#include <atomic>
+
+#include "kv4.cuh"
+#include "mma16.cuh"
+
+namespace dab {
+
+constexpr int KV4_NW = 4;      // warps per CTA, each with its own tiles and its own ring
+constexpr int KV4_TILE = 32;   // keys per tile
+constexpr int KV4_STAGES = 3;  // tiles in a warp's ring
+constexpr int KV4_MAX_SPLIT = 128;
+constexpr float KV4_SLACK = 8.f;  // log2 units a score may exceed the running maximum by before it moves
+
+// one stage of a warp's ring
+template <int D>
+struct Kv4Stage {
+  static constexpr int ROW = D / 2, SROW = D / 8;  // bytes of a row's codes, of its scales
+  static constexpr int K = 0, V = KV4_TILE * ROW, KS = 2 * V, VS = KS + KV4_TILE * SROW, C = VS + KV4_TILE * SROW;
+  static constexpr int BYTES = C + KV4_TILE * 4;
+  // place of 16-byte piece c of row r: pieces are rotated so that the value loads, which take one
+  // piece of every second row, meet different banks
+  __device__ static int piece(int r, int c) { return r * ROW + ((D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1)) << 4); }
+};
+
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes) {  // 16 bytes, or 0: zero fill
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// 16 + code for the codes at bits 4 I.. of both halves of w, as a pair of T
+template <typename T, int I>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
+  constexpr bool B = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int at = B ? 3 : 6;  // lowest mantissa bit that is worth 1 in 16.0
+  constexpr uint32_t mask = (0xFu << at) * 0x10001u, base = B ? 0x41804180u : 0x4C004C00u;
+  const uint32_t x = 4 * I > at ? w >> (4 * I - at) : w << (at - 4 * I);
+  return (x & mask) | base;
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+__device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ uint32_t movm(uint32_t x) {  // transpose of an 8 x 8 fragment of 16-bit numbers
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t bmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t bfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t bneg2(uint32_t a) { return a ^ 0x80008000u; }
+// x as a high T part and the rest, for two numbers
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = pack_t2<T>(x, y);
+  float hx, hy;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    hx = lo_f32(hi);
+    hy = hi_f32(hi);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    hx = f.x;
+    hy = f.y;
+  }
+  lo = pack_t2<T>(x - hx, y - hy);
+}
+
+// What a warp keeps over its tiles: per lane the heads 2 t and 2 t + 1 (t = lane % 4).
+template <int D>
+struct Kv4Acc {
+  float m[2], l[2];
+  float o[D / 16][4];  // [2 g + i / 2]: element 32 g + 4 (lane / 4) + i in [2 (i % 2) + head]
+  float sz[4];         // sums of p scale_g and p zero_g: value lane / 4 of the stored row in [0], [1]
+
+  __device__ __forceinline__ void init() {
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sz[e] = 0.f;
+  }
+
+  // Scores of 16 NT keys (lane: keys lane / 4 + 8 f of each 16, heads 2 t + e in [2 f + e]) to
+  // weights. The maximum moves only when a score is KV4_SLACK above it: weights stay below
+  // 2^KV4_SLACK counts, and the accumulators are hardly ever rescaled.
+  template <int NT>
+  __device__ __forceinline__ void weights(float (&z)[NT][4], const float (&c)[NT][2]) {
+    float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      a = fmaxf(a, fmaxf(z[i][0], z[i][2]));
+      b = fmaxf(b, fmaxf(z[i][1], z[i][3]));
+    }
+    if (__any_sync(0xFFFFFFFFu, a > m[0] + KV4_SLACK || b > m[1] + KV4_SLACK)) {
+#pragma unroll
+      for (int o_ = 4; o_ <= 16; o_ <<= 1) {
+        a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, o_));
+        b = fmaxf(b, __shfl_xor_sync(0xFFFFFFFFu, b, o_));
+      }
+      const float na = fmaxf(m[0], a), nb = fmaxf(m[1], b);
+      const float fa = na == m[0] ? 1.f : ex2(m[0] - na), fb = nb == m[1] ? 1.f : ex2(m[1] - nb);
+      m[0] = na;
+      m[1] = nb;
+      l[0] *= fa;
+      l[1] *= fb;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        o[i][0] *= fa; o[i][1] *= fb;
+        o[i][2] *= fa; o[i][3] *= fb;
+      }
+      sz[0] *= fa; sz[1] *= fb;
+    }
+    const float ra = m[0] == -INFINITY ? 0.f : m[0], rb = m[1] == -INFINITY ? 0.f : m[1];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[i][e] = c[i][e >> 1] * ex2(z[i][e] - (e & 1 ? rb : ra));
+        l[e & 1] += z[i][e];
+      }
+  }
+};
+
+// q of up to 8 heads as column fragments, and the coefficients of the stored scales and zeros
+template <typename T, int D>
+struct Kv4Query {
+  static constexpr int NG = D / 32;
+  uint32_t b[NG][2][2];  // [group][half][..]: pairs (8 t + 2 half + {0, 1}, + 4) of the group
+  uint32_t zc[3];        // coefficient pairs of word t, in three parts
+
+  __device__ __forceinline__ void load(const T* q, int64_t stride, int ng) {
+    const int lane = threadIdx.x & 31, t = lane & 3, head = lane >> 2;
+    float qsum[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (head < ng) w = *reinterpret_cast<const uint4*>(q + head * stride + 32 * g + 8 * t);
+      b[g][0][0] = prmt(w.x, w.z, 0x5410);
+      b[g][0][1] = prmt(w.x, w.z, 0x7632);
+      b[g][1][0] = prmt(w.y, w.w, 0x5410);
+      b[g][1][1] = prmt(w.y, w.w, 0x7632);
+      const T* e = reinterpret_cast<const T*>(&w);
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += to_f32(e[i]);
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
+      qsum[g] = s + __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+    }
+    // word j of a row: values 2 j, 2 j + 1 of (scales, zeros); a scale takes -16 qsum, a zero qsum
+    float x[2];
+    const int j = NG == 4 ? t : t & 1;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int v = 2 * j + e;
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) s = (v % NG) == g ? qsum[g] : s;
+      x[e] = v < NG ? -16.f * s : s;
+    }
+    uint32_t part[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      part[i] = pack_t2<__nv_bfloat16>(x[0], x[1]);
+      x[0] -= lo_f32(part[i]);
+      x[1] -= hi_f32(part[i]);
+    }
+    if constexpr (NG == 4) {  // products (part 0, part 1) and (part 2, -)
+      zc[0] = part[0]; zc[1] = part[1]; zc[2] = part[2];
+    } else {                  // words 2, 3 stand for words 0, 1 again: (part 0 | part 1), (part 2 | -)
+      zc[0] = t < 2 ? part[0] : part[1];
+      zc[1] = t < 2 ? part[2] : 0u;
+      zc[2] = 0u;
+    }
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
+  using St = Kv4Stage<D>;
+  constexpr int NG = D / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, gq = lane >> 2;
+  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
+  const int h0 = blockIdx.z * 8, ng = min(8, p.G - h0);
+  const int n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
+  int elen = p.exact_len;
+  if (p.state) elen = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.W), p.state[0] + p.lag)));
+  if (p.state && threadIdx.x == 0 && (blockIdx.x | blockIdx.y | blockIdx.z) == 0) *p.used = elen;
+  // this CTA's units of the head: tiles of 32 history entries, then tiles of 16 window rows
+  const int n4 = (n + KV4_TILE - 1) / KV4_TILE, units = n4 + (elen + 15) / 16;
+  const int u0 = static_cast<int>(static_cast<int64_t>(units) * blockIdx.x / p.nsplit);
+  const int u1 = static_cast<int>(static_cast<int64_t>(units) * (blockIdx.x + 1) / p.nsplit);
+  const int64_t row0 = static_cast<int64_t>(bh) * p.G + h0;
+
+  const uint8_t* kc = p.hist.k_codes + b * p.hist.cb + h * p.hist.ch;
+  const uint8_t* vc = p.hist.v_codes + b * p.hist.cb + h * p.hist.ch;
+  const uint8_t* ks = reinterpret_cast<const uint8_t*>(p.hist.k_scales + b * p.hist.sb + h * p.hist.sh);
+  const uint8_t* vs = reinterpret_cast<const uint8_t*>(p.hist.v_scales + b * p.hist.sb + h * p.hist.sh);
+  const int32_t* cnt = p.counts + b * p.mb + h * p.mh;
+  uint8_t* ring = smem + warp * (KV4_STAGES * St::BYTES);
+  const uint32_t ring32 = smem_u32(ring);
+
+  auto issue = [&](int unit, int stage) {
+    if (unit < min(u1, n4)) {
+      const int64_t k0 = static_cast<int64_t>(unit) * KV4_TILE;
+      const uint32_t dst = ring32 + stage * St::BYTES;
+      constexpr int PPR = St::ROW / 16;  // 16-byte pieces per row
+#pragma unroll
+      for (int i = 0; i < PPR; ++i) {
+        const int idx = lane + 32 * i, r = idx / PPR, c = idx % PPR;
+        const bool ok = k0 + r < n;
+        const int64_t off = (ok ? k0 + r : k0) * St::ROW + c * 16;
+        cp_async(dst + St::K + St::piece(r, c), kc + off, ok ? 16 : 0);
+        cp_async(dst + St::V + St::piece(r, c), vc + off, ok ? 16 : 0);
+      }
+      const bool ok = k0 + lane < n;
+      const int64_t r = ok ? k0 + lane : k0;
+      cp_async_small<St::SROW>(dst + St::KS + lane * St::SROW, ks + r * St::SROW, ok);
+      cp_async_small<St::SROW>(dst + St::VS + lane * St::SROW, vs + r * St::SROW, ok);
+      cp_async_small<4>(dst + St::C + lane * 4, cnt + r, ok);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < KV4_STAGES - 1; ++s) issue(u0 + warp + s * KV4_NW, s);
+
+  Kv4Query<T, D> q;
+  q.load(static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + h0) * p.qh, p.qh, ng);
+  Kv4Acc<D> acc;
+  acc.init();
+  float* sc0 = p.scores ? p.scores + (row0 + 2 * t) * p.sstride : nullptr;
+
+  int unit = u0 + warp, stage = 0;
+  for (; unit < min(u1, n4); unit += KV4_NW) {
+    cp_wait<KV4_STAGES - 2>();
+    __syncwarp();
+    uint8_t* sp = ring + stage * St::BYTES;
+    const int64_t k0 = static_cast<int64_t>(unit) * KV4_TILE;
+    // ---- scores
+    float z[2][4], c[2][2];
+    bool masked = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r0 = 16 * i + gq, r1 = r0 + 8;
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        c[i][f] = static_cast<float>(max(0, *reinterpret_cast<const int32_t*>(sp + St::C + 4 * (r0 + 8 * f))));
+        masked = masked || !(c[i][f] > 0.f);
+      }
+      uint32_t wa[NG], wb[NG], sa[NG / 2], sb[NG / 2];  // codes (word g), scale pairs of both rows
+      if constexpr (NG == 4) {
+        *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(sp + St::K + St::piece(r0, t));
+        *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(sp + St::K + St::piece(r1, t));
+        *reinterpret_cast<uint2*>(sa) = *reinterpret_cast<const uint2*>(sp + St::KS + r0 * St::SROW);
+        *reinterpret_cast<uint2*>(sb) = *reinterpret_cast<const uint2*>(sp + St::KS + r1 * St::SROW);
+      } else {
+        *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(sp + St::K + St::piece(r0, t >> 1) + 8 * (t & 1));
+        *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(sp + St::K + St::piece(r1, t >> 1) + 8 * (t & 1));
+        sa[0] = *reinterpret_cast<const uint32_t*>(sp + St::KS + r0 * St::SROW);
+        sb[0] = *reinterpret_cast<const uint32_t*>(sp + St::KS + r1 * St::SROW);
+      }
+      const int j = NG == 4 ? t : t & 1;
+      const uint32_t za = *reinterpret_cast<const uint32_t*>(sp + St::KS + r0 * St::SROW + 4 * j);
+      const uint32_t zb = *reinterpret_cast<const uint32_t*>(sp + St::KS + r1 * St::SROW + 4 * j);
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+      mma16816<__nv_bfloat16>(s, za, zb, za, zb, q.zc[0], q.zc[1]);
+      if constexpr (NG == 4) mma16816<__nv_bfloat16>(s, za, zb, 0u, 0u, q.zc[2], 0u);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        float a[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816<T>(a, code_pair<T, 0>(wa[g]), code_pair<T, 0>(wb[g]), code_pair<T, 1>(wa[g]), code_pair<T, 1>(wb[g]),
+                    q.b[g][0][0], q.b[g][0][1]);
+        mma16816<T>(a, code_pair<T, 2>(wa[g]), code_pair<T, 2>(wb[g]), code_pair<T, 3>(wa[g]), code_pair<T, 3>(wb[g]),
+                    q.b[g][1][0], q.b[g][1][1]);
+        const float xa = g & 1 ? hi_f32(sa[g >> 1]) : lo_f32(sa[g >> 1]);
+        const float xb = g & 1 ? hi_f32(sb[g >> 1]) : lo_f32(sb[g >> 1]);
+        s[0] = fmaf(xa, a[0], s[0]);
+        s[1] = fmaf(xa, a[1], s[1]);
+        s[2] = fmaf(xb, a[2], s[2]);
+        s[3] = fmaf(xb, a[3], s[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        z[i][e] = c[i][e >> 1] > 0.f ? s[e] * p.scale_log2 : -INFINITY;
+        if (sc0 && 2 * t + (e & 1) < ng && k0 + r0 + 8 * (e >> 1) < n)
+          sc0[(e & 1) * p.sstride + k0 + r0 + 8 * (e >> 1)] = z[i][e];
+      }
+    }
+    if (__any_sync(0xFFFFFFFFu, masked)) {
+      // a masked row's scales may be anything: 0 times them has to be 0
+      if (*reinterpret_cast<const int32_t*>(sp + St::C + 4 * lane) <= 0) {
+#pragma unroll
+        for (int i = 0; i < St::SROW / 8; ++i)
+          *reinterpret_cast<uint2*>(sp + St::VS + lane * St::SROW + 8 * i) = make_uint2(0u, 0u);
+      }
+      __syncwarp();
+    }
+    acc.template weights<2>(z, c);
+    // ---- values
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t ph[2], pl[2];  // weights of keys 2 t, 2 t + 1 (+ 8) for head lane / 4, two parts
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        split2<__nv_bfloat16>(z[i][2 * f], z[i][2 * f + 1], ph[f], pl[f]);
+        ph[f] = movm(ph[f]);
+        pl[f] = movm(pl[f]);
+      }
+      uint32_t w[4][NG], s[4][NG / 2];  // codes and scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = 16 * i + 2 * t + (k & 1) + 8 * (k >> 1);
+        if constexpr (NG == 4) {
+          *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(sp + St::V + St::piece(r, gq >> 1));
+          *reinterpret_cast<uint2*>(s[k]) = *reinterpret_cast<const uint2*>(sp + St::VS + r * St::SROW);
+        } else {
+          *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(sp + St::V + St::piece(r, gq >> 2) + 8 * ((gq >> 1) & 1));
+          s[k][0] = *reinterpret_cast<const uint32_t*>(sp + St::VS + r * St::SROW);
+        }
+      }
+      // sums of p scale and p zero: rows are the stored values
+      uint32_t a0, a2;
+      if constexpr (NG == 4) {
+        const uint32_t at = smem_u32(sp + St::VS + (16 * i + (lane & 15)) * St::SROW);
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a0), "=r"(a2) : "r"(at));
+      } else {
+        uint32_t v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = 16 * i + 2 * t + (k & 1) + 8 * (k >> 1);
+          v[k] = gq < 4 ? *reinterpret_cast<const uint16_t*>(sp + St::VS + r * St::SROW + 2 * gq) : 0u;
+        }
+        a0 = prmt(v[0], v[1], 0x5410);
+        a2 = prmt(v[2], v[3], 0x5410);
+      }
+      mma16816<__nv_bfloat16>(acc.sz, a0, 0u, a2, 0u, ph[0], ph[1]);
+      mma16816<__nv_bfloat16>(acc.sz, a0, 0u, a2, 0u, pl[0], pl[1]);
+      const uint32_t half = gq & 1 ? 0x7632u : 0x5410u;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        uint32_t bh_[2], bl_[2], x[2];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const uint32_t sc = prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u);
+          bh_[f] = bmul2(ph[f], sc);
+          bl_[f] = bfma2(pl[f], sc, bfma2(ph[f], sc, bneg2(bh_[f])));
+          x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
+        }
+        using B = __nv_bfloat16;
+        uint32_t a[4] = {code_pair<B, 0>(x[0]), code_pair<B, 1>(x[0]), code_pair<B, 0>(x[1]), code_pair<B, 1>(x[1])};
+        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], bh_[0], bh_[1]);
+        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], bl_[0], bl_[1]);
+        uint32_t d[4] = {code_pair<B, 2>(x[0]), code_pair<B, 3>(x[0]), code_pair<B, 2>(x[1]), code_pair<B, 3>(x[1])};
+        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], bh_[0], bh_[1]);
+        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], bl_[0], bl_[1]);
+      }
+    }
+    __syncwarp();  // every lane has read the stage: the slot before it may be filled again
+    issue(unit + (KV4_STAGES - 1) * KV4_NW, stage == 0 ? KV4_STAGES - 1 : stage - 1);
+    stage = stage == KV4_STAGES - 1 ? 0 : stage + 1;
+  }
+  cp_wait<0>();
+
+  // what the 16 of the codes brought in comes off, the zeros go on
+  float sum_s[NG][2], sum_z[NG][2];
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      sum_s[g][e] = __shfl_sync(0xFFFFFFFFu, acc.sz[e], 4 * g + t);
+      sum_z[g][e] = __shfl_sync(0xFFFFFFFFu, acc.sz[e], 4 * (NG + g) + t);
+    }
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float off = fmaf(-16.f, sum_s[g][e], sum_z[g][e]);
+      acc.o[2 * g][e] += off;
+      acc.o[2 * g][2 + e] += off;
+      acc.o[2 * g + 1][e] += off;
+      acc.o[2 * g + 1][2 + e] += off;
+    }
+
+  // ---- window rows, 16 at a time, straight from memory
+  const T* ke = static_cast<const T*>(p.k_exact) + b * p.eb + h * p.eh;
+  const T* ve = static_cast<const T*>(p.v_exact) + b * p.eb + h * p.eh;
+  for (; unit < u1; unit += KV4_NW) {
+    const int j0 = (unit - n4) * 16;
+    float z[1][4], c[1][2];
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool okr[2] = {j0 + gq < elen, j0 + gq + 8 < elen};
+    uint4 ka[NG], kb[NG];
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      ka[g] = kb[g] = make_uint4(0, 0, 0, 0);
+      if (okr[0]) ka[g] = *reinterpret_cast<const uint4*>(ke + static_cast<int64_t>(j0 + gq) * p.en + 32 * g + 8 * t);
+      if (okr[1]) kb[g] = *reinterpret_cast<const uint4*>(ke + static_cast<int64_t>(j0 + gq + 8) * p.en + 32 * g + 8 * t);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      mma16816<T>(s, prmt(ka[g].x, ka[g].z, 0x5410), prmt(kb[g].x, kb[g].z, 0x5410), prmt(ka[g].x, ka[g].z, 0x7632),
+                  prmt(kb[g].x, kb[g].z, 0x7632), q.b[g][0][0], q.b[g][0][1]);
+      mma16816<T>(s, prmt(ka[g].y, ka[g].w, 0x5410), prmt(kb[g].y, kb[g].w, 0x5410), prmt(ka[g].y, ka[g].w, 0x7632),
+                  prmt(kb[g].y, kb[g].w, 0x7632), q.b[g][1][0], q.b[g][1][1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool ok = okr[e >> 1];
+      c[0][e >> 1] = ok ? 1.f : 0.f;
+      z[0][e] = ok ? s[e] * p.scale_log2 : -INFINITY;
+      if (sc0 && 2 * t + (e & 1) < ng && ok) sc0[(e & 1) * p.sstride + p.cap + j0 + gq + 8 * (e >> 1)] = z[0][e];
+    }
+    acc.template weights<1>(z, c);
+    uint32_t ph[2], pl[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      split2<T>(z[0][2 * f], z[0][2 * f + 1], ph[f], pl[f]);
+      ph[f] = movm(ph[f]);
+      pl[f] = movm(pl[f]);
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint2 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int j = j0 + 2 * t + (k & 1) + 8 * (k >> 1);
+        x[k] = make_uint2(0u, 0u);
+        if (j < elen) x[k] = *reinterpret_cast<const uint2*>(ve + static_cast<int64_t>(j) * p.en + 32 * g + 4 * gq);
+      }
+      const uint32_t a[4] = {prmt(x[0].x, x[1].x, 0x5410), prmt(x[0].x, x[1].x, 0x7632), prmt(x[2].x, x[3].x, 0x5410),
+                             prmt(x[2].x, x[3].x, 0x7632)};
+      const uint32_t d[4] = {prmt(x[0].y, x[1].y, 0x5410), prmt(x[0].y, x[1].y, 0x7632), prmt(x[2].y, x[3].y, 0x5410),
+                             prmt(x[2].y, x[3].y, 0x7632)};
+      mma16816<T>(acc.o[2 * g], a[0], a[1], a[2], a[3], ph[0], ph[1]);
+      mma16816<T>(acc.o[2 * g], a[0], a[1], a[2], a[3], pl[0], pl[1]);
+      mma16816<T>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], ph[0], ph[1]);
+      mma16816<T>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], pl[0], pl[1]);
+    }
+  }
+
+  // ---- the warps' parts to one: common maximum, then sums through shared memory
+  __shared__ float sm_m[KV4_NW][8], sm_l[KV4_NW][8];
+#pragma unroll
+  for (int o_ = 4; o_ <= 16; o_ <<= 1) {
+    acc.l[0] += __shfl_xor_sync(0xFFFFFFFFu, acc.l[0], o_);
+    acc.l[1] += __shfl_xor_sync(0xFFFFFFFFu, acc.l[1], o_);
+  }
+  if (gq == 0) {
+    sm_m[warp][2 * t] = acc.m[0];
+    sm_m[warp][2 * t + 1] = acc.m[1];
+  }
+  __syncthreads();  // and every warp is done with its ring
+  float f[2], mm[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float m = sm_m[0][2 * t + e];
+#pragma unroll
+    for (int w = 1; w < KV4_NW; ++w) m = fmaxf(m, sm_m[w][2 * t + e]);
+    mm[e] = m;
+    f[e] = acc.m[e] == m ? 1.f : ex2(acc.m[e] - m);  // a warp without keys has 0 accumulators
+  }
+  if (gq == 0) {
+    sm_l[warp][2 * t] = acc.l[0] * f[0];
+    sm_l[warp][2 * t + 1] = acc.l[1] * f[1];
+  }
+  // [head][element], rows padded against bank conflicts
+  constexpr int OR = D + 4;
+  float* so = reinterpret_cast<float*>(smem) + warp * 8 * OR;
+#pragma unroll
+  for (int g = 0; g < NG; ++g)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float4*>(so + (2 * t + e) * OR + 32 * g + 4 * gq) =
+          make_float4(acc.o[2 * g][e] * f[e], acc.o[2 * g][2 + e] * f[e], acc.o[2 * g + 1][e] * f[e],
+                      acc.o[2 * g + 1][2 + e] * f[e]);
+  __syncthreads();
+  const float* base = reinterpret_cast<const float*>(smem);
+  for (int i = threadIdx.x; i < ng * (D / 4); i += KV4_NW * 32) {
+    const int hd = i / (D / 4), d = (i - hd * (D / 4)) * 4;
+    float4 a = *reinterpret_cast<const float4*>(base + hd * OR + d);
+#pragma unroll
+    for (int w = 1; w < KV4_NW; ++w) {
+      const float4 x = *reinterpret_cast<const float4*>(base + (w * 8 + hd) * OR + d);
+      a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    }
+    *reinterpret_cast<float4*>(p.part + ((row0 + hd) * p.nsplit + blockIdx.x) * D + d) = a;
+  }
+  if (warp == 0 && gq == 0) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int hd = 2 * t + e;
+      float l = sm_l[0][hd];
+#pragma unroll
+      for (int w = 1; w < KV4_NW; ++w) l += sm_l[w][hd];
+      if (hd < ng) p.stats[(row0 + hd) * p.nsplit + blockIdx.x] = make_float2(mm[e], l);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------- joining
+// blockIdx.y: kv-head. The first G CTAs join the splits of one q-head each and write its output;
+// the others add the weights of 1024 entries each (history, then window) to their mass. Every CTA
+// finds its rows' (max, sum) over the splits itself.
+constexpr int KV4_MASS_KEYS = 1024;
+
+// (max, 1 / sum) of a row over its splits, by one warp; 1 / sum is 0 where nothing is left
+__device__ __forceinline__ float2 row_stats(const float2* st, int nsplit, int lane) {
+  float m = -INFINITY, l = 0.f;
+  for (int s = lane; s < nsplit; s += 32) m = fmaxf(m, st[s].x);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int s = lane; s < nsplit; s += 32) l = fmaf(st[s].y, ex2(st[s].x - ref), l);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
+  return make_float2(ref, l == 0.f ? 0.f : 1.f / l);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4Attn p) {
+  __shared__ float2 st[32];
+  __shared__ float wgt[KV4_MAX_SPLIT];
+  __shared__ float red[256];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
+  if (static_cast<int>(blockIdx.x) < p.G) {
+    if (p.lag && (blockIdx.x | blockIdx.y) == 0 && threadIdx.x == 0) {
+      // the step's length advance: this kernel reads the length that was used from the workspace
+      p.state[0] += 1;
+      p.state[1] += 1;
+    }
+    const int64_t row = static_cast<int64_t>(bh) * p.G + blockIdx.x;
+    const float2* rs = p.stats + row * p.nsplit;
+    if (warp == 0) {
+      const float2 r = row_stats(rs, p.nsplit, lane);
+      for (int s = lane; s < p.nsplit; s += 32) wgt[s] = ex2(rs[s].x - r.x) * r.y;
+    }
+    __syncthreads();
+    const int d = threadIdx.x % D;
+    const float* part = p.part + row * p.nsplit * D + d;
+    float a = 0.f;
+    for (int s = threadIdx.x / D; s < p.nsplit; s += 256 / D) a = fmaf(part[static_cast<int64_t>(s) * D], wgt[s], a);
+    red[threadIdx.x] = a;
+    __syncthreads();
+    if (threadIdx.x < D) {
+#pragma unroll
+      for (int i = 1; i < 256 / D; ++i) a += red[threadIdx.x + i * D];
+      static_cast<T*>(p.out)[b * p.ob + (static_cast<int64_t>(h) * p.G + blockIdx.x) * p.oh + d] = from_f32<T>(a);
+    }
+    return;
+  }
+  const int n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
+  const int elen = p.state ? *p.used : p.exact_len;
+  const int k0 = (blockIdx.x - p.G) * KV4_MASS_KEYS;  // over capacity, then window
+  if (k0 >= n && (k0 + KV4_MASS_KEYS <= p.cap || k0 >= p.cap + elen)) return;
+  float w[KV4_MASS_KEYS / 256];
+#pragma unroll
+  for (int i = 0; i < KV4_MASS_KEYS / 256; ++i) w[i] = 0.f;
+  for (int g0 = 0; g0 < p.G; g0 += 32) {
+    const int ng = min(32, p.G - g0);
+    __syncthreads();
+    for (int g = warp; g < ng; g += 8) {
+      const float2 r = row_stats(p.stats + (static_cast<int64_t>(bh) * p.G + g0 + g) * p.nsplit, p.nsplit, lane);
+      if (lane == 0) st[g] = r;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < KV4_MASS_KEYS / 256; ++i) {
+      const int key = k0 + threadIdx.x + 256 * i;
+      if (!(key < n || (key >= p.cap && key < p.cap + elen))) continue;
+      const float* sc = p.scores + (static_cast<int64_t>(bh) * p.G + g0) * p.sstride + key;
+      for (int g = 0; g < ng; ++g) w[i] = fmaf(ex2(sc[g * p.sstride] - st[g].x), st[g].y, w[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < KV4_MASS_KEYS / 256; ++i) {
+    const int key = k0 + threadIdx.x + 256 * i;
+    if (key < n) {
+      const int32_t c = p.counts[b * p.mb + h * p.mh + key];
+      if (c > 0) p.mass[b * p.mb + h * p.mh + key] += static_cast<float>(c) * w[i];
+    } else if (key >= p.cap && key < p.cap + elen) {
+      p.exact_mass[b * p.emb + h * p.emh + key - p.cap] += w[i];
+    }
+  }
+}
+
+namespace {
+struct Kv4Plan {
+  int nsplit;
+  int64_t sstride, stats, part, scores, total;  // offsets in bytes
+};
+Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_t W, bool mass, int sms) {
+  auto up = [](int64_t x) { return (x + 255) & ~int64_t{255}; };
+  Kv4Plan w;
+  const int64_t rows = B * H * G, ctas = B * H * ((G + 7) / 8);
+  const int64_t units = (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16;
+  int64_t ns = ctas > 0 ? 3 * static_cast<int64_t>(sms) / ctas : 1;
+  const int64_t most = (units + 2 * KV4_NW - 1) / (2 * KV4_NW);  // two tiles a warp
+  ns = ns < most ? ns : most;
+  ns = ns < KV4_MAX_SPLIT ? ns : KV4_MAX_SPLIT;
+  w.nsplit = static_cast<int>(ns > 1 ? ns : 1);
+  w.sstride = cap + W;
+  w.stats = 256;
+  w.part = w.stats + up(rows * w.nsplit * 8);
+  w.scores = w.part + up(rows * w.nsplit * D * 4);
+  w.total = w.scores + (mass ? up(rows * w.sstride * 4) : 0);
+  return w;
+}
+int kv4_sms() {
+  int dev = 0, sms = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms > 0 ? sms : 148;
+}
+}  // namespace
+
+size_t kv4_attn_workspace(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_t W, bool mass) {
+  return static_cast<size_t>(kv4_plan(B, H, G, D, cap, W, mass, kv4_sms()).total);
+}
+
+template <typename T, int D>
+static cudaError_t kv4_run(const Kv4Attn& p, cudaStream_t st) {
+  constexpr int RING = KV4_NW * KV4_STAGES * Kv4Stage<D>::BYTES, OUT = KV4_NW * 8 * (D + 4) * 4;
+  constexpr int SMEM = RING > OUT ? RING : OUT;
+  static std::atomic<uint64_t> set{0};  // the shared-memory limit is raised once per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(set.load() & bit)) {
+    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return e;
+    set.fetch_or(bit);
+  }
+  dim3 grid(static_cast<unsigned>(p.nsplit), static_cast<unsigned>(p.B * p.H), static_cast<unsigned>((p.G + 7) / 8));
+  kv4_attn_kernel<T, D><<<grid, KV4_NW * 32, SMEM, st>>>(p);
+  const int mass = p.mass || p.exact_mass ? (p.cap + p.W + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS : 0;
+  dim3 gj(static_cast<unsigned>(p.G + mass), static_cast<unsigned>(p.B * p.H));
+  kv4_join_kernel<T, D><<<gj, 256, 0, st>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaStream_t st) {
+  if (p.B * p.H == 0) return cudaSuccess;
+  const bool mass = p.mass || p.exact_mass;
+  const Kv4Plan w = kv4_plan(p.B, p.H, p.G, D, p.cap, p.W, mass, kv4_sms());
+  p.nsplit = w.nsplit;
+  p.sstride = w.sstride;
+  p.stats = reinterpret_cast<float2*>(ws + w.stats);
+  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.used = reinterpret_cast<int*>(ws + 64);
+  p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
+  if (dtype == BF16) return D == 64 ? kv4_run<__nv_bfloat16, 64>(p, st) : kv4_run<__nv_bfloat16, 128>(p, st);
+  return D == 64 ? kv4_run<__half, 64>(p, st) : kv4_run<__half, 128>(p, st);
+}
+
+}  // namespace dab

@@ -859,7 +859,7 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     lib = L.load()
     st = L.stream_of(q)
     if workspace is None:
-        nbytes = lib.dab_decode_attention_kv4_workspace_size(B, Hq, D, cap, W, 1 if mass is not None else 0)
+        nbytes = lib.dab_decode_attention_kv4_workspace_size(B, H, Hq // H, D, cap, W, 1 if mass is not None else 0)
         workspace = L.workspace(q.device, st.value, nbytes, tag="kv4")
     strides = L.strides((*q.stride()[:2], *out.stride()[:2], *hist.k_codes.stride()[:2], *hist.k_scales.stride()[:2],
                          *ms, *lengths.stride(), *es, *em))
@@ -871,10 +871,10 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     return out
 
 
-def kv4_attention_workspace(batch, q_heads, head_dim, capacity, exact_window, with_mass=True) -> int:
+def kv4_attention_workspace(batch, q_heads, kv_heads, head_dim, capacity, exact_window, with_mass=True) -> int:
     """Bytes of the ``workspace`` that ``decode_attention_kv4`` takes."""
-    return int(L.load().dab_decode_attention_kv4_workspace_size(batch, q_heads, head_dim, capacity, exact_window,
-                                                                1 if with_mass else 0))
+    return int(L.load().dab_decode_attention_kv4_workspace_size(batch, kv_heads, q_heads // kv_heads, head_dim, capacity,
+                                                                exact_window, 1 if with_mass else 0))
 
 
 def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = None, keep_first: int = 0,

@@ -376,8 +376,8 @@ int dab_decode_update_kv4(const void* k_new, const void* v_new, void* k_codes, v
                           int64_t heads, int64_t head_dim, int64_t capacity, int64_t exact_window, int* err_word,
                           void* stream);
 /* Scratch bytes dab_decode_attention_kv4 needs. Zero it once, then reuse it on one stream. */
-size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t num_q_heads, int64_t head_dim, int64_t capacity,
-                                               int64_t exact_window, int with_mass);
+size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim,
+                                               int64_t capacity, int64_t exact_window, int with_mass);
 /* Single-token attention over a 4-bit history and the exact window: q / out [B, heads * kv_group,
  * head_dim], scores sm_scale * q . k + log(count) over history entries below the head's length
  * with a positive count (others draw nothing, whatever they hold) and sm_scale * q . k over the
