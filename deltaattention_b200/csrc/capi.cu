@@ -990,10 +990,12 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
     return fail(1, std::string(nm) + ": workspace too small");
   EvictParams p;
   std::memset(&p, 0, sizeof(p));
+  int64_t total = 0;
   for (int64_t i = 0; i < num_rows; ++i) {
     if (!rows[i]) return fail(1, std::string(nm) + ": null pointer");
-    if (row_bytes[i] < 4 || row_bytes[i] > 65536)
-      return fail(1, std::string(nm) + ": rows must have 4 to 65536 bytes");
+    total += row_bytes[i];
+    if (row_bytes[i] < 4 || row_bytes[i] > EVICT_MAX_BYTES || total > EVICT_MAX_BYTES)
+      return fail(1, std::string(nm) + ": an entry's rows must have 4 to " + std::to_string(EVICT_MAX_BYTES) + " bytes");
     const uint64_t all = reinterpret_cast<uintptr_t>(rows[i]) | static_cast<uint64_t>(row_strides[2 * i]) |
                          static_cast<uint64_t>(row_strides[2 * i + 1]) | static_cast<uint64_t>(row_bytes[i]);
     if (all % 4) return fail(1, std::string(nm) + ": rows must be multiples of 4 bytes, 4-byte aligned");

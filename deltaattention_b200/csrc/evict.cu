@@ -4,13 +4,28 @@
 // and of the entries between the k = budget - first - recent heaviest, ties to the lowest index.
 // Entries keep their order, and every row buffer is compacted in place with the mass.
 //
-//  * evict_select: the k-th largest weight of the middle entries by radix selection over 4 digits
-//    of 8 bits, and how many entries that equal it are kept.
-//  * evict_move: kept entries move to the front. An entry's destination is never behind its
-//    source, so tiles taken in order overwrite only entries that have been read.
+//  * evict_select: one cluster per head finds the k-th largest weight of the middle entries by
+//    radix selection (digits of 11, 11 and 10 bits; every CTA keeps the keys of its slice in shared
+//    memory and counts them, the counts are summed through distributed shared memory), then writes
+//    for every tile how many entries are kept before it and how many of the ties come before it.
+//  * evict_move: one CTA per tile reads its kept rows into shared memory, says so, waits for the
+//    (at most two) tiles on whose rows its own will land to have said so too, and writes. Tiles are
+//    handed out in order by a ticket per head and nothing is waited for before a tile has read
+//    its rows, so the tiles waited for are running and never wait themselves. Every kept row is
+//    read and written once, with no second buffer.
+#include <cooperative_groups.h>
+
 #include "evict.cuh"
 
 namespace dab {
+
+namespace cg = cooperative_groups;
+
+constexpr int SEL_THREADS = 1024;
+constexpr int SEL_KEYS = 16384;  // keys of a slice held in shared memory; later ones are read again
+constexpr int SEL_BINS = 2048;
+constexpr int MOVE_THREADS = 256;
+enum { ERR_EVICT_WAIT = 0x501 };
 
 // Unsigned key of a weight in the order of floats: NaN below everything, -0 equal to +0.
 __device__ __forceinline__ uint32_t mass_key(float x) {
@@ -18,124 +33,300 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
+constexpr uint32_t KEY_ZERO = 0x80000000u;  // weights of 0, which may be many
 
-__global__ void __launch_bounds__(1024) evict_select_kernel(EvictParams p) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t s_prefix, s_k;
-  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
-  const int n = min(p.lengths[b * p.lb + h * p.lh], p.cap);
-  if (n <= p.trigger) return;
-  const float* mass = p.mass + b * p.mb + h * p.mh;
-  const int lo = p.first, hi = n - p.recent;
-  uint32_t k = p.budget - p.first - p.recent;
-  if (k == 0) {  // nothing between the protected ends stays
-    if (threadIdx.x == 0) p.cut[bh] = make_uint2(0xFFFFFFFFu, 0u);
-    return;
-  }
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += blockDim.x) hist[i] = 0;
-    __syncthreads();
-    const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-    for (int i = lo + threadIdx.x; i < hi; i += blockDim.x) {
-      const uint32_t key = mass_key(mass[i]);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      uint32_t left = k;
-      int d = 255;
-      for (; d > 0 && hist[d] < left; --d) left -= hist[d];
-      s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
-      s_k = left;
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    k = s_k;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) p.cut[bh] = make_uint2(prefix, k);
-}
-
-template <typename U>
-__device__ __forceinline__ void move_rows(uint8_t* base, int bytes, const int* src, int dst0, int kept) {
-  const int upr = bytes / static_cast<int>(sizeof(U));
-  const int total = kept * upr;
-  for (int u0 = 0; u0 < total; u0 += blockDim.x) {
-    const int u = u0 + threadIdx.x;
-    const int r = u / upr, c = u - r * upr;
-    U v;
-    if (u < total) v = reinterpret_cast<const U*>(base + static_cast<int64_t>(src[r]) * bytes)[c];
-    __syncthreads();
-    if (u < total) reinterpret_cast<U*>(base + static_cast<int64_t>(dst0 + r) * bytes)[c] = v;
-    __syncthreads();
-  }
-}
-
-__global__ void __launch_bounds__(256) evict_move_kernel(EvictParams p) {
-  __shared__ int src[256];
-  __shared__ int w_tie[8], w_keep[8];
-  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H;
+__global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  cg::cluster_group cl = cg::this_cluster();
+  extern __shared__ uint32_t sel_smem[];
+  uint32_t* keys = sel_smem;                // [SEL_KEYS]
+  uint32_t* hist = sel_smem + SEL_KEYS;     // [3][SEL_BINS]
+  __shared__ uint32_t wsum[32], s_prefix, s_k, s_tot[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
+  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   int32_t* len = p.lengths + b * p.lb + h * p.lh;
   const int n = min(*len, p.cap);
-  if (n <= p.trigger) return;
-  const uint2 cut = p.cut[bh];
-  float* mass = p.mass + b * p.mb + h * p.mh;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const uint32_t below = (1u << lane) - 1u;
-  int ties = 0, dst = 0;
-  for (int i0 = 0; i0 < n; i0 += 256) {
-    const int i = i0 + threadIdx.x;
-    const float m = i < n ? mass[i] : 0.f;
-    const bool mid = i >= p.first && i < n - p.recent;
-    const uint32_t key = mass_key(m);
-    const bool tie = mid && key == cut.x;
-    bool keep = i < n && (!mid || key > cut.x);
-    const uint32_t tb = __ballot_sync(0xFFFFFFFFu, tie);
-    if (lane == 0) w_tie[warp] = __popc(tb);
-    __syncthreads();
-    int before = ties + __popc(tb & below), tt = 0;
-    for (int w = 0; w < 8; ++w) {
-      if (w < warp) before += w_tie[w];
-      tt += w_tie[w];
-    }
-    ties += tt;
-    if (tie && before < static_cast<int>(cut.y)) keep = true;
-    const uint32_t kb = __ballot_sync(0xFFFFFFFFu, keep);
-    if (lane == 0) w_keep[warp] = __popc(kb);
-    __syncthreads();
-    int pos = __popc(kb & below), kept = 0;
-    for (int w = 0; w < 8; ++w) {
-      if (w < warp) pos += w_keep[w];
-      kept += w_keep[w];
-    }
-    if (keep) {
-      src[pos] = i;
-      mass[dst + pos] = m;  // the tile's weights have all been read
-    }
-    __syncthreads();
-    for (int r = 0; r < p.n_rows; ++r) {
-      uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r];
-      if (p.unit[r] == 16) move_rows<uint4>(base, p.bytes[r], src, dst, kept);
-      else if (p.unit[r] == 8) move_rows<uint2>(base, p.bytes[r], src, dst, kept);
-      else move_rows<uint32_t>(base, p.bytes[r], src, dst, kept);
-    }
-    dst += kept;
-    __syncthreads();
+  if (n <= p.trigger) {  // for the whole cluster
+    if (rank == 0 && tid == 0) p.cut[bh] = make_uint4(0u, 0u, 0u, 0u);
+    return;
   }
-  if (threadIdx.x == 0) *len = p.budget;
+  const float* mass = p.mass + b * p.mb + h * p.mh;
+  // this CTA's slice: whole tiles
+  const int tiles = (n + p.tile - 1) / p.tile;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * rank / C);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / C);
+  const int i0 = t0 * p.tile, i1 = min(n, t1 * p.tile);
+  const int lo = p.first, hi = n - p.recent;  // the entries that compete
+  for (int i = i0 + tid; i < min(i1, i0 + SEL_KEYS); i += SEL_THREADS) keys[i - i0] = mass_key(mass[i]);
+  for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) hist[i] = 0;
+  for (int t = t0 + tid; t < t1; t += SEL_THREADS) p.loaded[static_cast<int64_t>(bh) * p.max_tiles + t] = 0u;
+  auto key_at = [&](int i) { return i - i0 < SEL_KEYS ? keys[i - i0] : mass_key(mass[i]); };
+  uint32_t k = p.budget - p.first - p.recent, prefix = k ? 0u : 0xFFFFFFFFu;
+  __syncthreads();
+  if (k) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t dmask = pass == 2 ? 1023u : 2047u;
+      const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+      uint32_t* hp = hist + pass * SEL_BINS;
+      for (int i = i0 + warp * 32; i < i1; i += SEL_THREADS) {
+        const int e = i + lane;
+        bool in = e >= lo && e < hi && e < i1;
+        uint32_t key = 0;
+        if (in) key = key_at(e);
+        in = in && (key & above) == prefix;
+        const uint32_t zeros = __ballot_sync(0xFFFFFFFFu, in && key == KEY_ZERO);
+        if (in && key != KEY_ZERO) atomicAdd(&hp[(key >> shift) & dmask], 1u);
+        if (lane == 0 && zeros) atomicAdd(&hp[(KEY_ZERO >> shift) & dmask], __popc(zeros));
+      }
+      cl.sync();
+      // thread i sums bins 2 i, 2 i + 1 from the top over the cluster
+      const int top = SEL_BINS - 2 - 2 * tid;  // bins top + 1 (first), top
+      uint32_t c1 = 0, c0 = 0;
+      for (int r = 0; r < C; ++r) {
+        const uint2 v = *reinterpret_cast<const uint2*>(cl.map_shared_rank(hp, r) + top);
+        c0 += v.x;
+        c1 += v.y;
+      }
+      uint32_t incl = c0 + c1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) wsum[warp] = incl;
+      __syncthreads();
+      uint32_t before = incl - c0 - c1;
+      for (int w = 0; w < warp; ++w) before += wsum[w];
+      // the digit is where the count from the top reaches k
+      if (before < k && k <= before + c1) {
+        s_prefix = prefix | (static_cast<uint32_t>(top + 1) << shift);
+        s_k = k - before;
+      } else if (before + c1 < k && k <= before + c1 + c0) {
+        s_prefix = prefix | (static_cast<uint32_t>(top) << shift);
+        s_k = k - before - c1;
+      }
+      __syncthreads();
+      prefix = s_prefix;
+      k = s_k;
+      __syncthreads();
+    }
+  }
+  // per tile: entries surely kept, and ties
+  uint2* before = p.before + static_cast<int64_t>(bh) * p.max_tiles;
+  for (int t = t0 + warp; t < t1; t += SEL_THREADS / 32) {
+    uint32_t sure = 0, tie = 0;
+    for (int i = t * p.tile; i < min(n, (t + 1) * p.tile); i += 32) {
+      const int e = i + lane;
+      bool s = false, q = false;
+      if (e < n && e < (t + 1) * p.tile) {
+        const bool mid = e >= lo && e < hi;
+        const uint32_t key = key_at(e);
+        s = !mid || key > prefix;
+        q = mid && key == prefix;
+      }
+      sure += __popc(__ballot_sync(0xFFFFFFFFu, s));
+      tie += __popc(__ballot_sync(0xFFFFFFFFu, q));
+    }
+    if (lane == 0) before[t] = make_uint2(sure, tie);
+  }
+  __syncthreads();
+  if (warp == 0) {  // exclusive sums over this CTA's tiles
+    uint32_t run_s = 0, run_t = 0;
+    for (int t = t0; t < t1; t += 32) {
+      uint2 v = make_uint2(0u, 0u);
+      if (t + lane < t1) v = before[t + lane];
+      uint32_t a = v.x, q = v.y;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, a, o), y = __shfl_up_sync(0xFFFFFFFFu, q, o);
+        if (lane >= o) { a += x; q += y; }
+      }
+      if (t + lane < t1) before[t + lane] = make_uint2(run_s + a - v.x, run_t + q - v.y);
+      run_s += __shfl_sync(0xFFFFFFFFu, a, 31);
+      run_t += __shfl_sync(0xFFFFFFFFu, q, 31);
+    }
+    if (lane == 0) {
+      s_tot[0] = run_s;
+      s_tot[1] = run_t;
+    }
+  }
+  cl.sync();
+  uint32_t base_s = 0, base_t = 0;
+  for (int r = 0; r < rank; ++r) {
+    const uint32_t* o = cl.map_shared_rank(s_tot, r);
+    base_s += o[0];
+    base_t += o[1];
+  }
+  for (int t = t0 + tid; t < t1; t += SEL_THREADS) {
+    const uint2 v = before[t];
+    const uint32_t ties = base_t + v.y;
+    before[t] = make_uint2(base_s + v.x + min(ties, k), ties);
+  }
+  if (rank == 0 && tid == 0) {
+    p.cut[bh] = make_uint4(prefix, k, static_cast<uint32_t>(n), 0u);
+    *len = p.budget;  // every CTA of the cluster has read it
+  }
+  cl.sync();  // no CTA leaves while its counts are read
 }
 
+__device__ __forceinline__ void move_in(uint32_t dst, const uint8_t* src, int unit) {
+  if (unit == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else if (unit == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
+__global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ __align__(16) uint8_t mv_smem[];  // src[tile] and mass[tile], then the rows of each buffer
+  __shared__ int w_tie[8], w_keep[8], s_tile;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
+  const int n = static_cast<int>(p.cut[bh].z);
+  if (n == 0 || static_cast<int>(blockIdx.x) * p.tile >= n) return;
+  if (tid == 0) s_tile = static_cast<int>(atomicAdd(&p.cut[bh].w, 1u));
+  const uint32_t thr = p.cut[bh].x;
+  const int need = static_cast<int>(p.cut[bh].y);
+  __syncthreads();
+  const int tile = s_tile, i0 = tile * p.tile;
+  const uint2 bf = p.before[static_cast<int64_t>(bh) * p.max_tiles + tile];
+  const int dst0 = static_cast<int>(bf.x);
+  int* src = reinterpret_cast<int*>(mv_smem);
+  float* kept_mass = reinterpret_cast<float*>(src + p.tile);
+  uint8_t* rows = reinterpret_cast<uint8_t*>(kept_mass + p.tile);
+  float* mass = p.mass + b * p.mb + h * p.mh;
+  // which entries stay, and where they go (tiles have at most MOVE_THREADS entries)
+  const int i = i0 + tid;
+  const bool live = tid < p.tile && i < n;
+  const float m = live ? mass[i] : 0.f;
+  const bool mid = i >= p.first && i < n - p.recent;
+  const uint32_t key = mass_key(m), below = (1u << lane) - 1u;
+  const bool tie = live && mid && key == thr;
+  bool keep = live && (!mid || key > thr);
+  const uint32_t tb = __ballot_sync(0xFFFFFFFFu, tie);
+  if (lane == 0) w_tie[warp] = __popc(tb);
+  __syncthreads();
+  int ties = static_cast<int>(bf.y) + __popc(tb & below);
+  for (int w = 0; w < warp; ++w) ties += w_tie[w];
+  keep = keep || (tie && ties < need);
+  const uint32_t kb = __ballot_sync(0xFFFFFFFFu, keep);
+  if (lane == 0) w_keep[warp] = __popc(kb);
+  __syncthreads();
+  int pos = __popc(kb & below), kept = 0;
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp) pos += w_keep[w];
+    kept += w_keep[w];
+  }
+  const bool still = dst0 == i0 && kept == min(p.tile, n - i0);  // nothing before or in the tile goes
+  if (keep && !still) {
+    src[pos] = i;
+    kept_mass[pos] = m;
+  }
+  __syncthreads();
+  if (!still && kept) {
+    uint8_t* at = rows;
+    for (int r = 0; r < p.n_rows; ++r) {
+      const uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r];
+      const int bytes = p.bytes[r], unit = p.unit[r], upr = bytes / unit;
+      const uint32_t dst = smem_u32(at);
+      for (int u = tid; u < kept * upr; u += MOVE_THREADS) {
+        const int e = u / upr;
+        move_in(dst + u * unit, base + static_cast<int64_t>(src[e]) * bytes + (u - e * upr) * unit, unit);
+      }
+      at += (p.tile * bytes + 15) & ~15;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  }
+  __syncthreads();
+  uint32_t* loaded = p.loaded + static_cast<int64_t>(bh) * p.max_tiles;
+  if (tid == 0) {
+    __threadfence();  // this tile's rows have been read: others may land on them
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(loaded + tile), "r"(1u) : "memory");
+  }
+  if (still || !kept) return;
+  if (tid < 2) {  // rows land on one tile, or two
+    const int on = (tid == 0 ? dst0 : dst0 + kept - 1) / p.tile;
+    uint32_t v = 1u;
+    if (on != tile) {
+      const uint64_t began = globaltimer();
+      while (true) {
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(loaded + on) : "memory");
+        if (v) break;
+        if (globaltimer() - began > DAB_WAIT_TIMEOUT_NS) {
+          atomicCAS(p.err, 0, static_cast<int>(ERR_EVICT_WAIT));
+          break;
+        }
+      }
+    }
+    w_keep[tid] = static_cast<int>(v);
+  }
+  __syncthreads();
+  if (!w_keep[0] || !w_keep[1]) return;  // timed out: the error word says that the cache is not valid
+  uint8_t* at = rows;
+  for (int r = 0; r < p.n_rows; ++r) {
+    uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r] + static_cast<int64_t>(dst0) * p.bytes[r];
+    const int total = kept * p.bytes[r];
+    if (p.unit[r] == 16) {
+      for (int u = tid * 16; u < total; u += MOVE_THREADS * 16)
+        *reinterpret_cast<uint4*>(base + u) = *reinterpret_cast<const uint4*>(at + u);
+    } else if (p.unit[r] == 8) {
+      for (int u = tid * 8; u < total; u += MOVE_THREADS * 8)
+        *reinterpret_cast<uint2*>(base + u) = *reinterpret_cast<const uint2*>(at + u);
+    } else {
+      for (int u = tid * 4; u < total; u += MOVE_THREADS * 4)
+        *reinterpret_cast<uint32_t*>(base + u) = *reinterpret_cast<const uint32_t*>(at + u);
+    }
+    at += (p.tile * p.bytes[r] + 15) & ~15;
+  }
+  if (tid < kept) mass[dst0 + tid] = kept_mass[tid];
+}
+
+namespace {
+constexpr int EVICT_MIN_TILE = 4;
+int64_t evict_up(int64_t x) { return (x + 255) & ~int64_t{255}; }
+}  // namespace
+
 size_t evict_workspace(int64_t B, int64_t H, int64_t cap) {
-  (void)cap;
-  return static_cast<size_t>(256 + B * H * 8);
+  const int64_t tiles = (cap + EVICT_MIN_TILE - 1) / EVICT_MIN_TILE;
+  return static_cast<size_t>(256 + evict_up(B * H * 16) + evict_up(B * H * tiles * 8) + evict_up(B * H * tiles * 4));
 }
 
 cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   if (p.B * p.H == 0 || p.cap == 0) return cudaSuccess;
-  p.cut = reinterpret_cast<uint2*>(ws + 256);
-  evict_select_kernel<<<p.B * p.H, 1024, 0, st>>>(p);
-  evict_move_kernel<<<p.B * p.H, 256, 0, st>>>(p);
+  // tiles of up to 128 entries and 48 KB of rows
+  int bytes = 0;
+  for (int r = 0; r < p.n_rows; ++r) bytes += p.bytes[r];
+  p.tile = 128;
+  while (p.tile > EVICT_MIN_TILE && p.tile * bytes > 80 * 1024) p.tile >>= 1;
+  p.max_tiles = (p.cap + p.tile - 1) / p.tile;
+  const int64_t heads = static_cast<int64_t>(p.B) * p.H;
+  p.err = reinterpret_cast<int*>(ws);
+  p.cut = reinterpret_cast<uint4*>(ws + 256);
+  p.before = reinterpret_cast<uint2*>(ws + 256 + evict_up(heads * 16));
+  p.loaded = reinterpret_cast<uint32_t*>(ws + 256 + evict_up(heads * 16) + evict_up(heads * p.max_tiles * 8));
+  int C = 1;  // 4096 entries a CTA keep a pass near its latency
+  while (C < 8 && p.cap > C * 4096) C <<= 1;
+  const int sel_smem = (SEL_KEYS + 3 * SEL_BINS) * 4;
+  int move_smem = p.tile * 8;
+  for (int r = 0; r < p.n_rows; ++r) move_smem += (p.tile * p.bytes[r] + 15) & ~15;
+  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sel_smem);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, move_smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(C), static_cast<unsigned>(heads));
+  cfg.blockDim = dim3(SEL_THREADS);
+  cfg.dynamicSmemBytes = static_cast<size_t>(sel_smem);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = static_cast<unsigned>(C);
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
+  if (e != cudaSuccess) return e;
+  evict_move_kernel<<<dim3(static_cast<unsigned>(p.max_tiles), static_cast<unsigned>(heads)), MOVE_THREADS, move_smem, st>>>(p);
   return cudaGetLastError();
 }
 

@@ -5,6 +5,7 @@
 namespace dab {
 
 constexpr int EVICT_MAX_ROWS = 8;
+constexpr int EVICT_MAX_BYTES = 8192;  // of an entry's rows together
 
 struct EvictParams {
   float* mass; int64_t mb, mh;           // [B, H, cap], strides in elements
@@ -17,7 +18,13 @@ struct EvictParams {
   int n_rows;
   int B, H, cap;
   int budget, trigger, first, recent;
-  uint2* cut;                            // workspace: (threshold key, ties kept) per head
+  int tile, max_tiles;                   // entries per moved tile, tiles of a full head
+  // workspace: error word; per head (threshold key, ties kept, length or 0 if left alone, ticket);
+  // per head and tile (kept before it, ties before it) and whether its rows have been read
+  int* err;
+  uint4* cut;
+  uint2* before;
+  uint32_t* loaded;
 };
 
 }  // namespace dab
