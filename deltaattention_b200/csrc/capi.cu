@@ -873,6 +873,9 @@ int dab_kv4_dequantize(const void* k_codes, const void* v_codes, const int64_t* 
   const char* nm = "dab_kv4_dequantize";
   if (!k || !v || !out_strides) return fail(1, std::string(nm) + ": null pointer");
   if (dtype != F32 && dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": bad dtype");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       static_cast<uintptr_t>((out_strides[0] | out_strides[1] | out_strides[2]) * elem_size(dtype))) % 16)
+    return fail(1, std::string(nm) + ": output rows must be 16-byte aligned");
   if (rows < 0 || rows >= (int64_t{1} << 31)) return fail(1, std::string(nm) + ": bad row count");
   if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, code_strides, scale_strides, batch, heads, rows,
                          head_dim))

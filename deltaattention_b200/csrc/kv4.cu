@@ -1,15 +1,98 @@
 // A decode history in 4 bits (format in kv4.cuh): quantisation of packed K / V rows, reading
 // back, and the single-token cache update.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace dab {
 
 // ------------------------------------------------------------------- quantise / read back
-// One warp per row; blockIdx.y: batch * head, blockIdx.z: K or V.
+// Both are bound by memory when every element costs few instructions: K and V rows of 2 D bytes
+// against 5 D / 8 bytes of codes and scales. A lane takes 8 neighbouring elements (one 16-byte
+// piece, one code word), the 4 lanes of a group find its minimum and maximum with two shuffles,
+// and KV4_ROWS pieces per lane are in flight.
+constexpr int KV4_ROWS = 4;
+
+template <typename T> struct Pair;
+template <> struct Pair<__nv_bfloat16> {
+  using V = __nv_bfloat162;
+  static __device__ __forceinline__ float2 f32(V v) { return __bfloat1622float2(v); }
+};
+template <> struct Pair<__half> {
+  using V = __half2;
+  static __device__ __forceinline__ float2 f32(V v) { return __half22float2(v); }
+};
+
+// Codes of 8 elements x (pairs of T) against (scale, zero). The quotient a / scale is corrected
+// from a * (1 / scale) by one step with the exact remainder (Markstein, IBM J. Res. Dev. 34, 1990),
+// so it rounds as a division does; adding 1.5 * 2^23 rounds it to an integer, half to even, in the
+// number's lowest bits. 0 <= a <= 15.06 scale: codes need no clamp.
+template <typename T>
+__device__ __forceinline__ uint32_t kv4_code8(const typename Pair<T>::V* x, float scale, float zero) {
+  const bool ok = scale > 0.f;  // not 0 (a constant group), not NaN
+  const float s = ok ? scale : 1.f, r = __frcp_rn(s);
+  uint32_t w = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 f = Pair<T>::f32(x[i >> 1]);
+    const float a = __fsub_rn(i & 1 ? f.y : f.x, zero);
+    const float q = a * r;
+    const float c = fmaf(fmaf(-q, s, a), r, q);
+    w += __float_as_uint(__fadd_rn(c, 12582912.f)) << (4 * i);  // 0x4B400000 + code
+  }
+  // the constant's own contributions: 0x4B400000 << 4 i, i = 0..7 (those past bit 31 are gone)
+  constexpr uint32_t magic = 0x4B400000u + 0xB4000000u + 0x40000000u;
+  return ok ? w - magic : 0u;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_quantize_kernel(const T* __restrict__ k, const T* __restrict__ v, int64_t kb,
-                                                           int64_t kh, int64_t kn, int64_t kd, int64_t vb, int64_t vh,
-                                                           int64_t vn, int64_t vd, Kv4Hist out, int H, int64_t N) {
+                                                           int64_t kh, int64_t kn, int64_t vb, int64_t vh, int64_t vn,
+                                                           Kv4Hist out, int H, int64_t N) {
+  constexpr int NG = D / 32, LPR = D / 8, RPI = 256 / LPR;  // lanes per row, rows per CTA and step
+  using V = typename Pair<T>::V;
+  const int j = threadIdx.x % LPR, g = j >> 2, t = j & 3;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (RPI * KV4_ROWS) + threadIdx.x / LPR;
+  const int b = blockIdx.y / H, h = blockIdx.y - b * H;
+  const bool is_v = blockIdx.z != 0;
+  const T* x = (is_v ? v + b * vb + h * vh : k + b * kb + h * kh) + 8 * j;
+  const int64_t sn = is_v ? vn : kn;
+  uint4 raw[KV4_ROWS];
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    const int64_t n = n0 + i * RPI;
+    if (n < N) raw[i] = __ldcs(reinterpret_cast<const uint4*>(x + n * sn));
+  }
+  uint32_t* c = reinterpret_cast<uint32_t*>((is_v ? out.v_codes : out.k_codes) + b * out.cb + h * out.ch) + t * NG + g;
+  __nv_bfloat16* s = (is_v ? out.v_scales : out.k_scales) + b * out.sb + h * out.sh + (t == 0 ? g : NG + g);
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    const int64_t n = n0 + i * RPI;
+    const V* e = reinterpret_cast<const V*>(&raw[i]);
+    V lo = __hmin2_nan(__hmin2_nan(e[0], e[1]), __hmin2_nan(e[2], e[3]));
+    V hi = __hmax2_nan(__hmax2_nan(e[0], e[1]), __hmax2_nan(e[2], e[3]));
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      lo = __hmin2_nan(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+      hi = __hmax2_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+    }
+    const float2 l2 = Pair<T>::f32(lo), h2 = Pair<T>::f32(hi);
+    float scale, zero;
+    kv4_scale_zero(fmin_nan(l2.x, l2.y), fmax_nan(h2.x, h2.y), scale, zero);
+    const uint32_t w = kv4_code8<T>(e, scale, zero);
+    if (n < N) {
+      c[n * LPR] = w;
+      if (t < 2) s[n * (2 * NG)] = __float2bfloat16_rn(t == 0 ? scale : zero);
+    }
+  }
+}
+
+// Any strides: one warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_quantize_any_kernel(const T* __restrict__ k, const T* __restrict__ v,
+                                                               int64_t kb, int64_t kh, int64_t kn, int64_t kd,
+                                                               int64_t vb, int64_t vh, int64_t vn, int64_t vd,
+                                                               Kv4Hist out, int H, int64_t N) {
   constexpr int NG = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -26,46 +109,82 @@ __global__ void __launch_bounds__(256) kv4_quantize_kernel(const T* __restrict__
   kv4_quantize_row<NG>(r, reinterpret_cast<uint32_t*>(c), s, lane);
 }
 
-// One thread per code word (8 elements).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_dequantize_kernel(Kv4Hist in, T* __restrict__ k, T* __restrict__ v,
                                                              int64_t ob, int64_t oh, int64_t on, int H, int64_t N) {
-  constexpr int NG = D / 32, NWORD = D / 8;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t n = i / NWORD;
-  if (n >= N) return;
-  const int w = static_cast<int>(i % NWORD), t = w / NG, g = w % NG;
+  constexpr int NG = D / 32, LPR = D / 8, RPI = 256 / LPR;
+  const int j = threadIdx.x % LPR, g = j >> 2, t = j & 3;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * (RPI * KV4_ROWS) + threadIdx.x / LPR;
   const int b = blockIdx.y / H, h = blockIdx.y - b * H;
   const bool is_v = blockIdx.z != 0;
-  const uint8_t* c = (is_v ? in.v_codes : in.k_codes) + b * in.cb + h * in.ch + n * (D / 2);
-  const __nv_bfloat16* s = (is_v ? in.v_scales : in.k_scales) + b * in.sb + h * in.sh + n * (2 * NG);
-  const uint32_t word = reinterpret_cast<const uint32_t*>(c)[w];
-  const float scale = to_f32(s[g]), zero = to_f32(s[NG + g]);
-  T* dst = (is_v ? v : k) + b * ob + h * oh + n * on + 32 * g + 8 * t;
+  const uint32_t* c = reinterpret_cast<const uint32_t*>((is_v ? in.v_codes : in.k_codes) + b * in.cb + h * in.ch) + t * NG + g;
+  const __nv_bfloat16* s = (is_v ? in.v_scales : in.k_scales) + b * in.sb + h * in.sh + g;
+  T* dst = (is_v ? v : k) + b * ob + h * oh + 8 * j;
+  uint32_t w[KV4_ROWS];
+  __nv_bfloat16 sc[KV4_ROWS], ze[KV4_ROWS];
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    dst[e] = from_f32<T>(fmaf(scale, static_cast<float>((word >> (4 * e)) & 15u), zero));
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    const int64_t n = n0 + i * RPI;
+    if (n < N) {
+      w[i] = c[n * LPR];
+      sc[i] = s[n * (2 * NG)];
+      ze[i] = s[n * (2 * NG) + NG];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < KV4_ROWS; ++i) {
+    const int64_t n = n0 + i * RPI;
+    if (n >= N) return;
+    const float scale = to_f32(sc[i]), zero = to_f32(ze[i]);
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)  // 2^23 + code, less 2^23
+      x[e] = fmaf(scale, __uint_as_float(((w[i] >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.f, zero);
+    T* o = dst + n * on;
+    if constexpr (sizeof(T) == 4) {
+      __stcs(reinterpret_cast<float4*>(o), make_float4(x[0], x[1], x[2], x[3]));
+      __stcs(reinterpret_cast<float4*>(o) + 1, make_float4(x[4], x[5], x[6], x[7]));
+    } else {
+      constexpr int bf = TypeOf<T>::value == BF16;
+      __stcs(reinterpret_cast<uint4*>(o),
+             make_uint4(pack2(x[0], x[1], bf), pack2(x[2], x[3], bf), pack2(x[4], x[5], bf), pack2(x[6], x[7], bf)));
+    }
+  }
 }
 
 cudaError_t launch_kv4_quantize(int dtype, const void* k, const int64_t* ks, const void* v, const int64_t* vs,
                                 const Kv4Hist& out, int64_t B, int64_t H, int64_t N, int64_t D, cudaStream_t st) {
   if (B * H * N == 0) return cudaSuccess;
-  dim3 grid(static_cast<unsigned>((N + 7) / 8), static_cast<unsigned>(B * H), 2);
-#define DAB_Q(TY, DD)                                                                                             \
-  kv4_quantize_kernel<TY, DD><<<grid, 256, 0, st>>>(static_cast<const TY*>(k), static_cast<const TY*>(v), ks[0],    \
-                                                    ks[1], ks[2], ks[3], vs[0], vs[1], vs[2], vs[3], out,           \
-                                                    static_cast<int>(H), N);                                       \
-  return cudaGetLastError();
-  if (dtype == BF16) { if (D == 64) { DAB_Q(__nv_bfloat16, 64) } DAB_Q(__nv_bfloat16, 128) }
-  if (D == 64) { DAB_Q(__half, 64) }
-  DAB_Q(__half, 128)
-#undef DAB_Q
+  // 16-byte pieces: contiguous rows on 16-byte boundaries; anything else goes one warp per row
+  const bool rows16 = ks[3] == 1 && vs[3] == 1 &&
+                      ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
+                      ((ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) & 7) == 0;
+  auto run = [&](auto tag, auto dd) -> cudaError_t {
+    using T = decltype(tag);
+    constexpr int DD = decltype(dd)::value;
+    const T* kp = static_cast<const T*>(k);
+    const T* vp = static_cast<const T*>(v);
+    const int64_t per = rows16 ? 256 / (DD / 8) * KV4_ROWS : 8;
+    dim3 grid(static_cast<unsigned>((N + per - 1) / per), static_cast<unsigned>(B * H), 2);
+    if (rows16)
+      kv4_quantize_kernel<T, DD><<<grid, 256, 0, st>>>(kp, vp, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], out,
+                                                       static_cast<int>(H), N);
+    else
+      kv4_quantize_any_kernel<T, DD><<<grid, 256, 0, st>>>(kp, vp, ks[0], ks[1], ks[2], ks[3], vs[0], vs[1], vs[2],
+                                                           vs[3], out, static_cast<int>(H), N);
+    return cudaGetLastError();
+  };
+  using I64 = std::integral_constant<int, 64>;
+  using I128 = std::integral_constant<int, 128>;
+  if (dtype == BF16) return D == 64 ? run(__nv_bfloat16{}, I64{}) : run(__nv_bfloat16{}, I128{});
+  return D == 64 ? run(__half{}, I64{}) : run(__half{}, I128{});
 }
 
 cudaError_t launch_kv4_dequantize(int dtype, const Kv4Hist& in, void* k, void* v, const int64_t* os, int64_t B,
                                   int64_t H, int64_t N, int64_t D, cudaStream_t st) {
   if (B * H * N == 0) return cudaSuccess;
-  dim3 grid(static_cast<unsigned>((N * (D / 8) + 255) / 256), static_cast<unsigned>(B * H), 2);
+  const int64_t per = 256 / (D / 8) * KV4_ROWS;
+  dim3 grid(static_cast<unsigned>((N + per - 1) / per), static_cast<unsigned>(B * H), 2);
 #define DAB_DQ(TY, DD)                                                                                          \
   kv4_dequantize_kernel<TY, DD><<<grid, 256, 0, st>>>(in, static_cast<TY*>(k), static_cast<TY*>(v), os[0], os[1], \
                                                       os[2], static_cast<int>(H), N);                            \

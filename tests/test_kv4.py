@@ -124,6 +124,24 @@ def test_quantize(ops, B, H, N, D, dt, layout):
 
 @gpu
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_quantize_paths_agree(ops, D, dt):
+    """Rows in 16-byte pieces (quotients corrected from the reciprocal) and rows at any strides
+    (divisions) give the same codes and scales, near ties and far from them."""
+    g = torch.Generator().manual_seed(D)
+    x = torch.randn(2, 3, 4001, D, generator=g) * torch.exp(2 * torch.randn(2, 3, 4001, 1, generator=g))
+    x[0, 0] = torch.randint(-40, 40, (4001, D), generator=g) * 0.25   # quotients on ties
+    x[0, 1] = (torch.rand(4001, D, generator=g) < 0.1) * 3.0
+    x = x.clamp(-6e4, 6e4).to(DT[dt]).cuda()
+    wide = torch.zeros(2, 3, 4001, D + 1, dtype=DT[dt], device="cuda")[..., 1:]
+    wide.copy_(x)
+    a, b = ops.kv4_quantize(x, -x), ops.kv4_quantize(wide, -wide)
+    for u, w in ((a.k_codes, b.k_codes), (a.v_codes, b.v_codes), (a.k_scales, b.k_scales), (a.v_scales, b.v_scales)):
+        assert torch.equal(u, w)
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
 def test_quantize_special_groups(ops, dt):
     D = 64
     x = torch.zeros(1, 1, 8, D, dtype=DT[dt])
