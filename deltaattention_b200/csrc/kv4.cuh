@@ -61,7 +61,7 @@ struct Kv4Attn {
   // scores of history and window (null without mass)
   float2* stats; float* part; float* scores;
   int* used;                                     // with state: the window length this call attends with
-  int64_t sstride;                               // scores per row: cap + W
+  int64_t sstride; int wcol;                     // columns of a row of scores, the window's first
   int nsplit;
 };
 

@@ -4,16 +4,20 @@
 // With k_jd = zero_jg + scale_jg code_jd (g = d / 32) both products are sums over codes:
 //   q . k_j  = sum_g scale_jg (sum_{d in g} q_d code_jd) + sum_g zero_jg qsum_g
 //   sum_j p_j v_jd = sum_j (p_j scale_jg) code_jd + sum_j p_j zero_jg
-// so the matrix instructions take the codes themselves: a code in the mantissa of 16.0 is the
-// 16-bit number 16 + code (one shift and one and-or for two codes), and the 16 is taken off
-// through the zero terms. Nothing is dequantised and q is not rounded.
-//  * Scores: keys are the rows of the product, q-heads its 8 columns. One accumulator per group,
-//    multiplied by the group's scale in fp32. The zero terms are two more products whose rows are
-//    the stored (scales, zeros) and whose columns hold qsum_g and -16 qsum_g in three bf16 parts
-//    (24 bits).
-//  * Values: elements are the rows, q-heads the columns. p scale_g goes in as two bf16 parts, high
-//    and the rest (16 bits of every weight); p alone, in two parts, times the stored (scales,
-//    zeros) gives what is taken off and added at the end.
+// so the matrix instructions take the codes themselves, and nothing is dequantised.
+//  * Scores: keys are the rows of the product, q-heads its 8 columns. A code in the mantissa of 256.0
+//    or 16.0 is the fp16 number 256 + code or 16 + code: two shifts and four and-or operations give
+//    8 operands. q goes in as fp16, scaled by a power of two so that its largest element is in [2^13,
+//    2^14): what is below 2^-30 of that is rounded, all else exact. One accumulator per group,
+//    multiplied by the group's scale in fp32. What the 256 and 16 bring in and the zeros are two
+//    more products: rows are the stored (scales, zeros), columns the coefficients in three bf16
+//    parts (24 bits).
+//    (8-bit float operands, a code's byte being code * 2^-9, took 125 us where this took 112 at
+//    4 x 65536 x 8 heads: this matrix path converts them to fp16 first.)
+//  * Values: elements are the rows, q-heads the columns. A code in the mantissa of 16.0 is the bf16
+//    number 16 + code. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every
+//    weight); p alone, in two parts, times the stored (scales, zeros) gives what the 16 brought in
+//    and the zeros, added once at the end.
 #include <atomic>
 
 #include "kv4.cuh"
@@ -45,39 +49,35 @@ template <int N>
 __device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
 }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// 16 + code for the codes at bits 4 I.. of both halves of w, as a pair of T
-template <typename T, int I>
+// 16 + code for the codes at bits 4 I.. of both halves of w, as a pair of bf16
+template <int I>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  constexpr bool B = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int at = B ? 3 : 6;  // lowest mantissa bit that is worth 1 in 16.0
-  constexpr uint32_t mask = (0xFu << at) * 0x10001u, base = B ? 0x41804180u : 0x4C004C00u;
-  const uint32_t x = 4 * I > at ? w >> (4 * I - at) : w << (at - 4 * I);
-  return (x & mask) | base;
+  const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
+  return (x & 0x00780078u) | 0x41804180u;
+}
+// fp16: 256 + code (I even), 16 + code (I odd) for the codes at bits 4 I.. of both halves, from w << 2
+// (I = 0, 1) or w >> 6 (I = 2, 3)
+template <int I>
+__device__ __forceinline__ uint32_t code_pair_h(uint32_t x) {
+  return I & 1 ? (x & 0x03C003C0u) | 0x4C004C00u : (x & 0x003C003Cu) | 0x5C005C00u;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 __device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
 __device__ __forceinline__ uint32_t movm(uint32_t x) {  // transpose of an 8 x 8 fragment of 16-bit numbers
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t bmul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t bfma2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t d;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
-  return d;
-}
-__device__ __forceinline__ uint32_t bneg2(uint32_t a) { return a ^ 0x80008000u; }
 // x as a high T part and the rest, for two numbers
 template <typename T>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
@@ -153,41 +153,66 @@ struct Kv4Acc {
   }
 };
 
-// q of up to 8 heads as column fragments, and the coefficients of the stored scales and zeros
+// q of up to 8 heads as column fragments of the score product, and the coefficients of the stored
+// scales and zeros
 template <typename T, int D>
 struct Kv4Query {
   static constexpr int NG = D / 32;
   uint32_t b[NG][2][2];  // [group][half][..]: pairs (8 t + 2 half + {0, 1}, + 4) of the group
-  uint32_t zc[3];        // coefficient pairs of word t, in three parts
+  uint32_t zc[3];        // coefficient pairs of a row's word, in three parts
+  float back[2];         // of heads 2 t, 2 t + 1: what takes the product to log2 units
 
-  __device__ __forceinline__ void load(const T* q, int64_t stride, int ng) {
+  __device__ __forceinline__ void load(const T* q, int64_t stride, int ng, float scale_log2) {
     const int lane = threadIdx.x & 31, t = lane & 3, head = lane >> 2;
-    float qsum[NG];
+    uint4 w[NG];
+    float top = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (head < ng) w = *reinterpret_cast<const uint4*>(q + head * stride + 32 * g + 8 * t);
-      b[g][0][0] = prmt(w.x, w.z, 0x5410);
-      b[g][0][1] = prmt(w.x, w.z, 0x7632);
-      b[g][1][0] = prmt(w.y, w.w, 0x5410);
-      b[g][1][1] = prmt(w.y, w.w, 0x7632);
-      const T* e = reinterpret_cast<const T*>(&w);
-      float s = 0.f;
+      w[g] = make_uint4(0, 0, 0, 0);
+      if (head < ng) w[g] = *reinterpret_cast<const uint4*>(q + head * stride + 32 * g + 8 * t);
+      const T* e = reinterpret_cast<const T*>(&w[g]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s += to_f32(e[i]);
-      s += __shfl_xor_sync(0xFFFFFFFFu, s, 1);
-      qsum[g] = s + __shfl_xor_sync(0xFFFFFFFFu, s, 2);
+      for (int i = 0; i < 8; ++i) top = fmax_nan(top, fabsf(to_f32(e[i])));
     }
-    // word j of a row: values 2 j, 2 j + 1 of (scales, zeros); a scale takes -16 qsum, a zero qsum
+    top = fmax_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = fmax_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    // 2^k with top * 2^k in [2^13, 2^14); 1 for a row of zeros and one that is not finite
+    const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+    const int k = top > 0.f && ex < 128 ? max(-126, min(126, 13 - ex)) : 0;
+    const float f = __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+    float qsum[NG], osum[NG];  // of the elements, and of the elements times what their codes carry
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const T* e = reinterpret_cast<const T*>(&w[g]);
+      float even = 0.f, odd = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // elements i, i + 4
+        const __half2 x = __floats2half2_rn(to_f32(e[i]) * f, to_f32(e[i + 4]) * f);
+        const float2 y = __half22float2(x);
+        b[g][i >> 1][i & 1] = *reinterpret_cast<const uint32_t*>(&x);
+        if (i & 1) odd += y.x + y.y;
+        else even += y.x + y.y;
+      }
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        even += __shfl_xor_sync(0xFFFFFFFFu, even, o);
+        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
+      }
+      qsum[g] = even + odd;
+      osum[g] = -fmaf(256.f, even, 16.f * odd);
+    }
+    // word j of a row: values 2 j, 2 j + 1 of (scales, zeros)
     float x[2];
     const int j = NG == 4 ? t : t & 1;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int v = 2 * j + e;
-      float s = 0.f;
+      x[e] = 0.f;
 #pragma unroll
-      for (int g = 0; g < NG; ++g) s = (v % NG) == g ? qsum[g] : s;
-      x[e] = v < NG ? -16.f * s : s;
+      for (int g = 0; g < NG; ++g) {
+        if (v == g) x[e] = osum[g];
+        if (v == NG + g) x[e] = qsum[g];
+      }
     }
     uint32_t part[3];
 #pragma unroll
@@ -203,11 +228,14 @@ struct Kv4Query {
       zc[1] = t < 2 ? part[2] : 0u;
       zc[2] = 0u;
     }
+    const float bk = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    back[0] = __shfl_sync(0xFFFFFFFFu, bk, 8 * t);
+    back[1] = __shfl_sync(0xFFFFFFFFu, bk, 8 * t + 4);
   }
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
+__global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
   using St = Kv4Stage<D>;
   constexpr int NG = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -224,108 +252,130 @@ __global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_cons
   const int u1 = static_cast<int>(static_cast<int64_t>(units) * (blockIdx.x + 1) / p.nsplit);
   const int64_t row0 = static_cast<int64_t>(bh) * p.G + h0;
 
-  const uint8_t* kc = p.hist.k_codes + b * p.hist.cb + h * p.hist.ch;
-  const uint8_t* vc = p.hist.v_codes + b * p.hist.cb + h * p.hist.ch;
-  const uint8_t* ks = reinterpret_cast<const uint8_t*>(p.hist.k_scales + b * p.hist.sb + h * p.hist.sh);
-  const uint8_t* vs = reinterpret_cast<const uint8_t*>(p.hist.v_scales + b * p.hist.sb + h * p.hist.sh);
-  const int32_t* cnt = p.counts + b * p.mb + h * p.mh;
   uint8_t* ring = smem + warp * (KV4_STAGES * St::BYTES);
   const uint32_t ring32 = smem_u32(ring);
-
+  // A lane copies pieces lane + 32 i of a tile's codes (they are contiguous), so its rows differ by
+  // multiples of 32 / PPR and their rotation is the same; and its row's scales and count.
+  constexpr int PPR = St::ROW / 16;  // 16-byte pieces per row
+  const int my_row = lane / PPR;
+  const uint32_t code_dst = ring32 + St::piece(my_row, lane % PPR);
+  const uint8_t* kc = p.hist.k_codes + b * p.hist.cb + h * p.hist.ch + lane * 16;
+  const uint8_t* vc = p.hist.v_codes + b * p.hist.cb + h * p.hist.ch + lane * 16;
+  const uint8_t* ks = reinterpret_cast<const uint8_t*>(p.hist.k_scales + b * p.hist.sb + h * p.hist.sh) + lane * St::SROW;
+  const uint8_t* vs = reinterpret_cast<const uint8_t*>(p.hist.v_scales + b * p.hist.sb + h * p.hist.sh) + lane * St::SROW;
+  const int32_t* cnt = p.counts + b * p.mb + h * p.mh + lane;
+  const int last = min(u1, n4);  // history tiles of this CTA end here
   auto issue = [&](int unit, int stage) {
-    if (unit < min(u1, n4)) {
+    if (unit < last) {
       const int64_t k0 = static_cast<int64_t>(unit) * KV4_TILE;
-      const uint32_t dst = ring32 + stage * St::BYTES;
-      constexpr int PPR = St::ROW / 16;  // 16-byte pieces per row
+      const int rem = n - unit * KV4_TILE;
+      const uint32_t dst = code_dst + stage * St::BYTES, row_dst = ring32 + stage * St::BYTES + lane * St::SROW;
+      const uint8_t* kp = kc + k0 * St::ROW;
+      const uint8_t* vp = vc + k0 * St::ROW;
+      if (rem >= KV4_TILE) {
 #pragma unroll
-      for (int i = 0; i < PPR; ++i) {
-        const int idx = lane + 32 * i, r = idx / PPR, c = idx % PPR;
-        const bool ok = k0 + r < n;
-        const int64_t off = (ok ? k0 + r : k0) * St::ROW + c * 16;
-        cp_async(dst + St::K + St::piece(r, c), kc + off, ok ? 16 : 0);
-        cp_async(dst + St::V + St::piece(r, c), vc + off, ok ? 16 : 0);
+        for (int i = 0; i < PPR; ++i) {
+          cp_async(dst + St::K + 512 * i, kp + 512 * i, 16);
+          cp_async(dst + St::V + 512 * i, vp + 512 * i, 16);
+        }
+        cp_async_small<St::SROW>(row_dst + St::KS, ks + k0 * St::SROW, true);
+        cp_async_small<St::SROW>(row_dst + St::VS, vs + k0 * St::SROW, true);
+        cp_async_small<4>(ring32 + stage * St::BYTES + St::C + 4 * lane, cnt + k0, true);
+      } else {  // rows past the end are filled with zeros: count 0 masks them
+#pragma unroll
+        for (int i = 0; i < PPR; ++i) {
+          const bool ok = my_row + i * (32 / PPR) < rem;
+          cp_async(dst + St::K + 512 * i, ok ? kp + 512 * i : kp - lane * 16, ok ? 16 : 0);
+          cp_async(dst + St::V + 512 * i, ok ? vp + 512 * i : vp - lane * 16, ok ? 16 : 0);
+        }
+        const bool ok = lane < rem;
+        const int back = ok ? 0 : lane;  // the tile's first row, of which nothing is read
+        cp_async_small<St::SROW>(row_dst + St::KS, ks + (k0 - back) * St::SROW, ok);
+        cp_async_small<St::SROW>(row_dst + St::VS, vs + (k0 - back) * St::SROW, ok);
+        cp_async_small<4>(ring32 + stage * St::BYTES + St::C + 4 * lane, cnt + k0 - back, ok);
       }
-      const bool ok = k0 + lane < n;
-      const int64_t r = ok ? k0 + lane : k0;
-      cp_async_small<St::SROW>(dst + St::KS + lane * St::SROW, ks + r * St::SROW, ok);
-      cp_async_small<St::SROW>(dst + St::VS + lane * St::SROW, vs + r * St::SROW, ok);
-      cp_async_small<4>(dst + St::C + lane * 4, cnt + r, ok);
     }
     cp_commit();
   };
 #pragma unroll
   for (int s = 0; s < KV4_STAGES - 1; ++s) issue(u0 + warp + s * KV4_NW, s);
 
+  const T* qp = static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + h0) * p.qh;
   Kv4Query<T, D> q;
-  q.load(static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + h0) * p.qh, p.qh, ng);
+  q.load(qp, p.qh, ng, p.scale_log2);
   Kv4Acc<D> acc;
   acc.init();
-  float* sc0 = p.scores ? p.scores + (row0 + 2 * t) * p.sstride : nullptr;
+  float* sc0 = p.scores ? p.scores + (row0 + 2 * t) * p.sstride + gq : nullptr;
+  const bool head0 = 2 * t < ng, head1 = 2 * t + 1 < ng;
 
   int unit = u0 + warp, stage = 0;
-  for (; unit < min(u1, n4); unit += KV4_NW) {
+  for (; unit < last; unit += KV4_NW) {
     cp_wait<KV4_STAGES - 2>();
     __syncwarp();
     uint8_t* sp = ring + stage * St::BYTES;
-    const int64_t k0 = static_cast<int64_t>(unit) * KV4_TILE;
+    // entries that take no part: their scores are -inf, and 0 times their scales has to be 0
+    const bool masked = __any_sync(0xFFFFFFFFu, *reinterpret_cast<const int32_t*>(sp + St::C + 4 * lane) <= 0);
+    if (masked) {
+      if (*reinterpret_cast<const int32_t*>(sp + St::C + 4 * lane) <= 0) {
+        *reinterpret_cast<int32_t*>(sp + St::C + 4 * lane) = 0;
+#pragma unroll
+        for (int i = 0; i < St::SROW / 8; ++i)
+          *reinterpret_cast<uint2*>(sp + St::VS + lane * St::SROW + 8 * i) = make_uint2(0u, 0u);
+      }
+      __syncwarp();
+    }
     // ---- scores
     float z[2][4], c[2][2];
-    bool masked = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r0 = 16 * i + gq, r1 = r0 + 8;
+      uint32_t w[2][NG], s2[2][NG / 2], zw[2];  // codes (word g), scale pairs, word of scales or zeros of both rows
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        c[i][f] = static_cast<float>(max(0, *reinterpret_cast<const int32_t*>(sp + St::C + 4 * (r0 + 8 * f))));
-        masked = masked || !(c[i][f] > 0.f);
+        const int r = f ? r1 : r0;
+        c[i][f] = static_cast<float>(*reinterpret_cast<const int32_t*>(sp + St::C + 4 * r));
+        const uint8_t* sr = sp + St::KS + r * St::SROW;
+        if constexpr (NG == 4) {
+          *reinterpret_cast<uint4*>(w[f]) = *reinterpret_cast<const uint4*>(sp + St::K + St::piece(r, t));
+          *reinterpret_cast<uint2*>(s2[f]) = *reinterpret_cast<const uint2*>(sr);
+          zw[f] = *reinterpret_cast<const uint32_t*>(sr + 4 * t);
+        } else {
+          *reinterpret_cast<uint2*>(w[f]) = *reinterpret_cast<const uint2*>(sp + St::K + St::piece(r, t >> 1) + 8 * (t & 1));
+          s2[f][0] = *reinterpret_cast<const uint32_t*>(sr);
+          zw[f] = *reinterpret_cast<const uint32_t*>(sr + 4 * (t & 1));
+        }
       }
-      uint32_t wa[NG], wb[NG], sa[NG / 2], sb[NG / 2];  // codes (word g), scale pairs of both rows
-      if constexpr (NG == 4) {
-        *reinterpret_cast<uint4*>(wa) = *reinterpret_cast<const uint4*>(sp + St::K + St::piece(r0, t));
-        *reinterpret_cast<uint4*>(wb) = *reinterpret_cast<const uint4*>(sp + St::K + St::piece(r1, t));
-        *reinterpret_cast<uint2*>(sa) = *reinterpret_cast<const uint2*>(sp + St::KS + r0 * St::SROW);
-        *reinterpret_cast<uint2*>(sb) = *reinterpret_cast<const uint2*>(sp + St::KS + r1 * St::SROW);
-      } else {
-        *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(sp + St::K + St::piece(r0, t >> 1) + 8 * (t & 1));
-        *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(sp + St::K + St::piece(r1, t >> 1) + 8 * (t & 1));
-        sa[0] = *reinterpret_cast<const uint32_t*>(sp + St::KS + r0 * St::SROW);
-        sb[0] = *reinterpret_cast<const uint32_t*>(sp + St::KS + r1 * St::SROW);
-      }
-      const int j = NG == 4 ? t : t & 1;
-      const uint32_t za = *reinterpret_cast<const uint32_t*>(sp + St::KS + r0 * St::SROW + 4 * j);
-      const uint32_t zb = *reinterpret_cast<const uint32_t*>(sp + St::KS + r1 * St::SROW + 4 * j);
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-      mma16816<__nv_bfloat16>(s, za, zb, za, zb, q.zc[0], q.zc[1]);
-      if constexpr (NG == 4) mma16816<__nv_bfloat16>(s, za, zb, 0u, 0u, q.zc[2], 0u);
+      float s[4];
+      mma16816_set<__nv_bfloat16>(s, zw[0], zw[1], zw[0], zw[1], q.zc[0], q.zc[1]);
+      if constexpr (NG == 4) mma16816<__nv_bfloat16>(s, zw[0], zw[1], 0u, 0u, q.zc[2], 0u);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float a[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816<T>(a, code_pair<T, 0>(wa[g]), code_pair<T, 0>(wb[g]), code_pair<T, 1>(wa[g]), code_pair<T, 1>(wb[g]),
-                    q.b[g][0][0], q.b[g][0][1]);
-        mma16816<T>(a, code_pair<T, 2>(wa[g]), code_pair<T, 2>(wb[g]), code_pair<T, 3>(wa[g]), code_pair<T, 3>(wb[g]),
-                    q.b[g][1][0], q.b[g][1][1]);
-        const float xa = g & 1 ? hi_f32(sa[g >> 1]) : lo_f32(sa[g >> 1]);
-        const float xb = g & 1 ? hi_f32(sb[g >> 1]) : lo_f32(sb[g >> 1]);
+        float a[4];
+        uint32_t x[2] = {w[0][g] << 2, w[1][g] << 2};
+        mma16816_set<__half>(a, code_pair_h<0>(x[0]), code_pair_h<0>(x[1]), code_pair_h<1>(x[0]), code_pair_h<1>(x[1]),
+                             q.b[g][0][0], q.b[g][0][1]);
+        x[0] = w[0][g] >> 6;
+        x[1] = w[1][g] >> 6;
+        mma16816<__half>(a, code_pair_h<2>(x[0]), code_pair_h<2>(x[1]), code_pair_h<3>(x[0]), code_pair_h<3>(x[1]),
+                         q.b[g][1][0], q.b[g][1][1]);
+        const float xa = g & 1 ? hi_f32(s2[0][g >> 1]) : lo_f32(s2[0][g >> 1]);
+        const float xb = g & 1 ? hi_f32(s2[1][g >> 1]) : lo_f32(s2[1][g >> 1]);
         s[0] = fmaf(xa, a[0], s[0]);
         s[1] = fmaf(xa, a[1], s[1]);
         s[2] = fmaf(xb, a[2], s[2]);
         s[3] = fmaf(xb, a[3], s[3]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        z[i][e] = c[i][e >> 1] > 0.f ? s[e] * p.scale_log2 : -INFINITY;
-        if (sc0 && 2 * t + (e & 1) < ng && k0 + r0 + 8 * (e >> 1) < n)
-          sc0[(e & 1) * p.sstride + k0 + r0 + 8 * (e >> 1)] = z[i][e];
-      }
-    }
-    if (__any_sync(0xFFFFFFFFu, masked)) {
-      // a masked row's scales may be anything: 0 times them has to be 0
-      if (*reinterpret_cast<const int32_t*>(sp + St::C + 4 * lane) <= 0) {
+      for (int e = 0; e < 4; ++e) z[i][e] = s[e] * q.back[e & 1];
+      if (masked) {
 #pragma unroll
-        for (int i = 0; i < St::SROW / 8; ++i)
-          *reinterpret_cast<uint2*>(sp + St::VS + lane * St::SROW + 8 * i) = make_uint2(0u, 0u);
+        for (int e = 0; e < 4; ++e) z[i][e] = c[i][e >> 1] > 0.f ? z[i][e] : -INFINITY;
       }
-      __syncwarp();
+      if (sc0) {  // the rows of the workspace have room for whole tiles
+        float* o = sc0 + static_cast<int64_t>(unit) * KV4_TILE + 16 * i;
+        if (head0) { o[0] = z[i][0]; o[8] = z[i][2]; }
+        if (head1) { o[p.sstride] = z[i][1]; o[p.sstride + 8] = z[i][3]; }
+      }
     }
     acc.template weights<2>(z, c);
     // ---- values
@@ -365,29 +415,30 @@ __global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_cons
         a0 = prmt(v[0], v[1], 0x5410);
         a2 = prmt(v[2], v[3], 0x5410);
       }
-      mma16816<__nv_bfloat16>(acc.sz, a0, 0u, a2, 0u, ph[0], ph[1]);
-      mma16816<__nv_bfloat16>(acc.sz, a0, 0u, a2, 0u, pl[0], pl[1]);
+      using B = __nv_bfloat16;
+      mma16816<B>(acc.sz, a0, 0u, a2, 0u, ph[0], ph[1]);
+      mma16816<B>(acc.sz, a0, 0u, a2, 0u, pl[0], pl[1]);
       const uint32_t half = gq & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        uint32_t bh_[2], bl_[2], x[2];
+        uint32_t wh[2], wl[2], x[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const uint32_t sc = prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u);
-          bh_[f] = bmul2(ph[f], sc);
-          bl_[f] = bfma2(pl[f], sc, bfma2(ph[f], sc, bneg2(bh_[f])));
+          const __nv_bfloat162 sc = as_b2(prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u));
+          const __nv_bfloat162 hi = __hmul2(as_b2(ph[f]), sc);
+          wh[f] = as_u32(hi);
+          wl[f] = as_u32(__hfma2(as_b2(pl[f]), sc, __hfma2(as_b2(ph[f]), sc, __hneg2(hi))));
           x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
         }
-        using B = __nv_bfloat16;
-        uint32_t a[4] = {code_pair<B, 0>(x[0]), code_pair<B, 1>(x[0]), code_pair<B, 0>(x[1]), code_pair<B, 1>(x[1])};
-        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], bh_[0], bh_[1]);
-        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], bl_[0], bl_[1]);
-        uint32_t d[4] = {code_pair<B, 2>(x[0]), code_pair<B, 3>(x[0]), code_pair<B, 2>(x[1]), code_pair<B, 3>(x[1])};
-        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], bh_[0], bh_[1]);
-        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], bl_[0], bl_[1]);
+        const uint32_t a[4] = {code_pair<0>(x[0]), code_pair<1>(x[0]), code_pair<0>(x[1]), code_pair<1>(x[1])};
+        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wh[0], wh[1]);
+        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wl[0], wl[1]);
+        const uint32_t d[4] = {code_pair<2>(x[0]), code_pair<3>(x[0]), code_pair<2>(x[1]), code_pair<3>(x[1])};
+        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wh[0], wh[1]);
+        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wl[0], wl[1]);
       }
     }
-    __syncwarp();  // every lane has read the stage: the slot before it may be filled again
+    __syncwarp();  // every lane has read the stage before: it may be filled again
     issue(unit + (KV4_STAGES - 1) * KV4_NW, stage == 0 ? KV4_STAGES - 1 : stage - 1);
     stage = stage == KV4_STAGES - 1 ? 0 : stage + 1;
   }
@@ -416,6 +467,18 @@ __global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_cons
   // ---- window rows, 16 at a time, straight from memory
   const T* ke = static_cast<const T*>(p.k_exact) + b * p.eb + h * p.eh;
   const T* ve = static_cast<const T*>(p.v_exact) + b * p.eb + h * p.eh;
+  uint32_t qw[NG][2][2];  // pairs (8 t + 2 half + {0, 1}, + 4) of each group, as rows are read below
+  if (unit < u1) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (gq < ng) w = *reinterpret_cast<const uint4*>(qp + gq * p.qh + 32 * g + 8 * t);
+      qw[g][0][0] = prmt(w.x, w.z, 0x5410);
+      qw[g][0][1] = prmt(w.x, w.z, 0x7632);
+      qw[g][1][0] = prmt(w.y, w.w, 0x5410);
+      qw[g][1][1] = prmt(w.y, w.w, 0x7632);
+    }
+  }
   for (; unit < u1; unit += KV4_NW) {
     const int j0 = (unit - n4) * 16;
     float z[1][4], c[1][2];
@@ -431,16 +494,16 @@ __global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_cons
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       mma16816<T>(s, prmt(ka[g].x, ka[g].z, 0x5410), prmt(kb[g].x, kb[g].z, 0x5410), prmt(ka[g].x, ka[g].z, 0x7632),
-                  prmt(kb[g].x, kb[g].z, 0x7632), q.b[g][0][0], q.b[g][0][1]);
+                  prmt(kb[g].x, kb[g].z, 0x7632), qw[g][0][0], qw[g][0][1]);
       mma16816<T>(s, prmt(ka[g].y, ka[g].w, 0x5410), prmt(kb[g].y, kb[g].w, 0x5410), prmt(ka[g].y, ka[g].w, 0x7632),
-                  prmt(kb[g].y, kb[g].w, 0x7632), q.b[g][1][0], q.b[g][1][1]);
+                  prmt(kb[g].y, kb[g].w, 0x7632), qw[g][1][0], qw[g][1][1]);
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const bool ok = okr[e >> 1];
       c[0][e >> 1] = ok ? 1.f : 0.f;
       z[0][e] = ok ? s[e] * p.scale_log2 : -INFINITY;
-      if (sc0 && 2 * t + (e & 1) < ng && ok) sc0[(e & 1) * p.sstride + p.cap + j0 + gq + 8 * (e >> 1)] = z[0][e];
+      if (sc0 && (e & 1 ? head1 : head0) && ok) sc0[(e & 1) * p.sstride + p.wcol + j0 + 8 * (e >> 1)] = z[0][e];
     }
     acc.template weights<1>(z, c);
     uint32_t ph[2], pl[2];
@@ -470,6 +533,7 @@ __global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_cons
     }
   }
 
+  grid_next();
   // ---- the warps' parts to one: common maximum, then sums through shared memory
   __shared__ float sm_m[KV4_NW][8], sm_l[KV4_NW][8];
 #pragma unroll
@@ -530,6 +594,8 @@ __global__ void __launch_bounds__(KV4_NW * 32) kv4_attn_kernel(const __grid_cons
 }
 
 // ---------------------------------------------------------------------------------- joining
+// Launched while the attention kernel ends (programmatic dependent launch): grid_wait returns once
+// that kernel's writes are there.
 // blockIdx.y: kv-head. The first G CTAs join the splits of one q-head each and write its output;
 // the others add the weights of 1024 entries each (history, then window) to their mass. Every CTA
 // finds its rows' (max, sum) over the splits itself.
@@ -550,12 +616,13 @@ __device__ __forceinline__ float2 row_stats(const float2* st, int nsplit, int la
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4Attn p) {
-  __shared__ float2 st[32];
+  __shared__ float2 st[8];
   __shared__ float wgt[KV4_MAX_SPLIT];
   __shared__ float red[256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   if (static_cast<int>(blockIdx.x) < p.G) {
+    grid_wait();
     if (p.lag && (blockIdx.x | blockIdx.y) == 0 && threadIdx.x == 0) {
       // the step's length advance: this kernel reads the length that was used from the workspace
       p.state[0] += 1;
@@ -581,44 +648,54 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
     }
     return;
   }
+  // 4 neighbouring entries a thread: history [0, cap), window from column wcol on
   const int n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
-  const int elen = p.state ? *p.used : p.exact_len;
-  const int k0 = (blockIdx.x - p.G) * KV4_MASS_KEYS;  // over capacity, then window
-  if (k0 >= n && (k0 + KV4_MASS_KEYS <= p.cap || k0 >= p.cap + elen)) return;
-  float w[KV4_MASS_KEYS / 256];
+  const int key = (blockIdx.x - p.G) * KV4_MASS_KEYS + 4 * threadIdx.x;
+  const int32_t* cp = p.counts + b * p.mb + h * p.mh + key;
+  float* mp = p.mass + b * p.mb + h * p.mh + key;
+  float c[4], m[4], w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < KV4_MASS_KEYS / 256; ++i) w[i] = 0.f;
-  for (int g0 = 0; g0 < p.G; g0 += 32) {
-    const int ng = min(32, p.G - g0);
-    __syncthreads();
-    for (int g = warp; g < ng; g += 8) {
-      const float2 r = row_stats(p.stats + (static_cast<int64_t>(bh) * p.G + g0 + g) * p.nsplit, p.nsplit, lane);
-      if (lane == 0) st[g] = r;
+  for (int i = 0; i < 4; ++i) {  // what the attention kernel does not write is read while it ends
+    c[i] = key + i < n ? static_cast<float>(cp[i]) : 0.f;
+    m[i] = key + i < n ? mp[i] : 0.f;
+  }
+  grid_wait();
+  const int elen = p.state ? *p.used : p.exact_len, j = key - p.wcol;
+  if (blockIdx.x * KV4_MASS_KEYS - p.G * KV4_MASS_KEYS >= max(n, p.wcol + elen)) return;
+  const bool some = key < n || (j >= 0 && j < elen);
+  for (int g0 = 0; g0 < p.G; g0 += 8) {
+    const int ng = min(8, p.G - g0);
+    const int64_t row = static_cast<int64_t>(bh) * p.G + g0;
+    float4 sc[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+      if (g < ng && some) sc[g] = *reinterpret_cast<const float4*>(p.scores + (row + g) * p.sstride + key);
+    if (g0) __syncthreads();
+    if (warp < ng) {
+      const float2 r = row_stats(p.stats + (row + warp) * p.nsplit, p.nsplit, lane);
+      if (lane == 0) st[warp] = r;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < KV4_MASS_KEYS / 256; ++i) {
-      const int key = k0 + threadIdx.x + 256 * i;
-      if (!(key < n || (key >= p.cap && key < p.cap + elen))) continue;
-      const float* sc = p.scores + (static_cast<int64_t>(bh) * p.G + g0) * p.sstride + key;
-      for (int g = 0; g < ng; ++g) w[i] = fmaf(ex2(sc[g * p.sstride] - st[g].x), st[g].y, w[i]);
-    }
+    for (int g = 0; g < 8; ++g)
+      if (g < ng && some) {
+        w[0] = fmaf(ex2(sc[g].x - st[g].x), st[g].y, w[0]);
+        w[1] = fmaf(ex2(sc[g].y - st[g].x), st[g].y, w[1]);
+        w[2] = fmaf(ex2(sc[g].z - st[g].x), st[g].y, w[2]);
+        w[3] = fmaf(ex2(sc[g].w - st[g].x), st[g].y, w[3]);
+      }
   }
 #pragma unroll
-  for (int i = 0; i < KV4_MASS_KEYS / 256; ++i) {
-    const int key = k0 + threadIdx.x + 256 * i;
-    if (key < n) {
-      const int32_t c = p.counts[b * p.mb + h * p.mh + key];
-      if (c > 0) p.mass[b * p.mb + h * p.mh + key] += static_cast<float>(c) * w[i];
-    } else if (key >= p.cap && key < p.cap + elen) {
-      p.exact_mass[b * p.emb + h * p.emh + key - p.cap] += w[i];
-    }
+  for (int i = 0; i < 4; ++i) {
+    if (c[i] > 0.f) mp[i] = fmaf(c[i], w[i], m[i]);
+    if (j >= 0 && j + i < elen) p.exact_mass[b * p.emb + h * p.emh + j + i] += w[i];
   }
 }
 
 namespace {
 struct Kv4Plan {
   int nsplit;
+  int wcol;                                     // first window column of a row of scores
   int64_t sstride, stats, part, scores, total;  // offsets in bytes
 };
 Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_t W, bool mass, int sms) {
@@ -631,7 +708,8 @@ Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_
   ns = ns < most ? ns : most;
   ns = ns < KV4_MAX_SPLIT ? ns : KV4_MAX_SPLIT;
   w.nsplit = static_cast<int>(ns > 1 ? ns : 1);
-  w.sstride = cap + W;
+  w.wcol = static_cast<int>((cap + KV4_TILE - 1) / KV4_TILE * KV4_TILE);
+  w.sstride = w.wcol + (W + 3) / 4 * 4;
   w.stats = 256;
   w.part = w.stats + up(rows * w.nsplit * 8);
   w.scores = w.part + up(rows * w.nsplit * D * 4);
@@ -666,10 +744,19 @@ static cudaError_t kv4_run(const Kv4Attn& p, cudaStream_t st) {
   }
   dim3 grid(static_cast<unsigned>(p.nsplit), static_cast<unsigned>(p.B * p.H), static_cast<unsigned>((p.G + 7) / 8));
   kv4_attn_kernel<T, D><<<grid, KV4_NW * 32, SMEM, st>>>(p);
-  const int mass = p.mass || p.exact_mass ? (p.cap + p.W + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS : 0;
-  dim3 gj(static_cast<unsigned>(p.G + mass), static_cast<unsigned>(p.B * p.H));
-  kv4_join_kernel<T, D><<<gj, 256, 0, st>>>(p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  const int mass = p.scores ? static_cast<int>((p.sstride + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS) : 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.G + mass), static_cast<unsigned>(p.B * p.H));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<T, D>, p);
 }
 
 cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaStream_t st) {
@@ -678,6 +765,7 @@ cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaSt
   const Kv4Plan w = kv4_plan(p.B, p.H, p.G, D, p.cap, p.W, mass, kv4_sms());
   p.nsplit = w.nsplit;
   p.sstride = w.sstride;
+  p.wcol = w.wcol;
   p.stats = reinterpret_cast<float2*>(ws + w.stats);
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.used = reinterpret_cast<int*>(ws + 64);
