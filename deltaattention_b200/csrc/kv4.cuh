@@ -57,12 +57,13 @@ struct Kv4Attn {
   int exact_len;                                 // without state
   float scale_log2;                              // sm_scale * log2(e)
   int B, H, G, cap, W;                           // G q-heads per kv-head
-  // workspace: per q-head row and split (max, sum) and the unscaled output, per q-head row the
-  // scores of history and window (null without mass)
-  float2* stats; float* part; float* scores;
+  // workspace: per 8 q-heads (first part, last piece); per q-head row of an unsplit head (max,
+  // 1 / sum); per part and q-head (max, sum) and the unscaled output; per row the scores of history
+  // and window (null without mass)
+  int2* info; float2* row_stats; float2* stats; float* part; float* scores;
   int* used;                                     // with state: the window length this call attends with
   int64_t sstride; int wcol;                     // columns of a row of scores, the window's first
-  int nsplit;
+  int pieces;                                    // 0: one per head
 };
 
 // x rounded down (towards -inf) to bf16, as fp32

@@ -18,6 +18,7 @@
 //    number 16 + code. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every
 //    weight); p alone, in two parts, times the stored (scales, zeros) gives what the 16 brought in
 //    and the zeros, added once at the end.
+#include <algorithm>
 #include <atomic>
 
 #include "kv4.cuh"
@@ -27,8 +28,9 @@ namespace dab {
 
 constexpr int KV4_NW = 4;      // warps per CTA, each with its own tiles and its own ring
 constexpr int KV4_TILE = 32;   // keys per tile
-constexpr int KV4_STAGES = 3;  // tiles in a warp's ring
-constexpr int KV4_MAX_SPLIT = 128;
+constexpr int KV4_STAGES = 2;  // tiles in a warp's ring
+constexpr int KV4_MAX_PIECES = 1024, KV4_MAX_HEADS = 2048;  // that are cut into pieces
+constexpr int KV4_MIN_UNITS = 8;  // of a piece: two tiles a warp
 constexpr float KV4_SLACK = 8.f;  // log2 units a score may exceed the running maximum by before it moves
 
 // one stage of a warp's ring
@@ -42,12 +44,18 @@ struct Kv4Stage {
   __device__ static int piece(int r, int c) { return r * ROW + ((D == 128 ? c ^ ((r >> 1) & 3) : c ^ ((r >> 2) & 1)) << 4); }
 };
 
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, int bytes) {  // 16 bytes, or 0: zero fill
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+// copies of N bytes to shared memory, and of N or 0 (zeros are written)
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (N == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
 }
 template <int N>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
+__device__ __forceinline__ void cp_async_if(uint32_t dst, const void* src, bool valid) {
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? N : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(valid ? N : 0) : "memory");
 }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;"); }
@@ -71,8 +79,44 @@ __device__ __forceinline__ uint32_t code_pair_h(uint32_t x) {
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 __device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi_f32(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
-__device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+__device__ __forceinline__ uint32_t bmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t bfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t bfms2(uint32_t a, uint32_t b, uint32_t c) {  // a b - c
+  uint32_t d;
+  asm("{\n\t.reg .b32 n;\n\tneg.bf16x2 n, %3;\n\tfma.rn.bf16x2 %0, %1, %2, n;\n\t}" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+// shared memory by 32-bit address
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t at) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at) : "memory");
+  return v;
+}
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t* w, uint32_t at) {
+  if constexpr (N == 4)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  else if constexpr (N == 2)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+  else
+    w[0] = lds32(at);
+}
+__device__ __forceinline__ void sts32(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
 __device__ __forceinline__ uint32_t movm(uint32_t x) {  // transpose of an 8 x 8 fragment of 16-bit numbers
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -159,7 +203,7 @@ template <typename T, int D>
 struct Kv4Query {
   static constexpr int NG = D / 32;
   uint32_t b[NG][2][2];  // [group][half][..]: pairs (8 t + 2 half + {0, 1}, + 4) of the group
-  uint32_t zc[3];        // coefficient pairs of a row's word, in three parts
+  uint32_t zc[3];        // coefficient pairs of a row's word of (scales, zeros), in three parts
   float back[2];         // of heads 2 t, 2 t + 1: what takes the product to log2 units
 
   __device__ __forceinline__ void load(const T* q, int64_t stride, int ng, float scale_log2) {
@@ -234,71 +278,86 @@ struct Kv4Query {
   }
 };
 
+// Units of a head: tiles of 32 history entries, then tiles of 16 window rows; at least one, so that
+// every head has a CTA that writes its output.
+__device__ __forceinline__ int kv4_len(const Kv4Attn& p, int bh) {
+  const int b = bh / p.H, h = bh - b * p.H;
+  return max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
+}
+__device__ __forceinline__ int kv4_units(int n, int elen) {
+  return max(1, (n + KV4_TILE - 1) / KV4_TILE + (elen + 15) / 16);
+}
+
+// Units [u0, u1) of group z (8 q-heads) of head bh, by the whole CTA.
 template <typename T, int D>
-__global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
+__device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int bh, int z, int n, int elen, int u0,
+                                            int u1, int slot) {
   using St = Kv4Stage<D>;
   constexpr int NG = D / 32;
-  extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 3, gq = lane >> 2;
-  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
-  const int h0 = blockIdx.z * 8, ng = min(8, p.G - h0);
-  const int n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
-  int elen = p.exact_len;
-  if (p.state) elen = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.W), p.state[0] + p.lag)));
-  if (p.state && threadIdx.x == 0 && (blockIdx.x | blockIdx.y | blockIdx.z) == 0) *p.used = elen;
-  // this CTA's units of the head: tiles of 32 history entries, then tiles of 16 window rows
-  const int n4 = (n + KV4_TILE - 1) / KV4_TILE, units = n4 + (elen + 15) / 16;
-  const int u0 = static_cast<int>(static_cast<int64_t>(units) * blockIdx.x / p.nsplit);
-  const int u1 = static_cast<int>(static_cast<int64_t>(units) * (blockIdx.x + 1) / p.nsplit);
+  const int b = bh / p.H, h = bh - b * p.H;
+  const int h0 = z * 8, ng = min(8, p.G - h0);
+  const int n4 = (n + KV4_TILE - 1) / KV4_TILE;
   const int64_t row0 = static_cast<int64_t>(bh) * p.G + h0;
 
-  uint8_t* ring = smem + warp * (KV4_STAGES * St::BYTES);
-  const uint32_t ring32 = smem_u32(ring);
-  // A lane copies pieces lane + 32 i of a tile's codes (they are contiguous), so its rows differ by
-  // multiples of 32 / PPR and their rotation is the same; and its row's scales and count.
+  // Shared-memory addresses of this lane, within a stage of its warp's ring; rows 8 and 16 further
+  // have the same rotation (Kv4Stage::piece).
   constexpr int PPR = St::ROW / 16;  // 16-byte pieces per row
-  const int my_row = lane / PPR;
-  const uint32_t code_dst = ring32 + St::piece(my_row, lane % PPR);
-  const uint8_t* kc = p.hist.k_codes + b * p.hist.cb + h * p.hist.ch + lane * 16;
-  const uint8_t* vc = p.hist.v_codes + b * p.hist.cb + h * p.hist.ch + lane * 16;
-  const uint8_t* ks = reinterpret_cast<const uint8_t*>(p.hist.k_scales + b * p.hist.sb + h * p.hist.sh) + lane * St::SROW;
-  const uint8_t* vs = reinterpret_cast<const uint8_t*>(p.hist.v_scales + b * p.hist.sb + h * p.hist.sh) + lane * St::SROW;
-  const int32_t* cnt = p.counts + b * p.mb + h * p.mh + lane;
-  const int last = min(u1, n4);  // history tiles of this CTA end here
-  auto issue = [&](int unit, int stage) {
-    if (unit < last) {
-      const int64_t k0 = static_cast<int64_t>(unit) * KV4_TILE;
-      const int rem = n - unit * KV4_TILE;
-      const uint32_t dst = code_dst + stage * St::BYTES, row_dst = ring32 + stage * St::BYTES + lane * St::SROW;
-      const uint8_t* kp = kc + k0 * St::ROW;
-      const uint8_t* vp = vc + k0 * St::ROW;
+  const uint32_t ring = smem_u32(smem) + warp * (KV4_STAGES * St::BYTES);
+  const uint32_t k_at = St::K + (NG == 4 ? St::piece(gq, t) : St::piece(gq, t >> 1) + 8 * (t & 1));
+  const uint32_t v_at = St::V + (NG == 4 ? St::piece(2 * t, gq >> 1) : St::piece(2 * t, gq >> 2) + 8 * ((gq >> 1) & 1));
+  const uint32_t ks_at = St::KS + gq * St::SROW, vs_at = St::VS + 2 * t * St::SROW;
+  // A lane copies pieces lane + 32 i of a tile's codes (they are contiguous), its row's scales and
+  // count.
+  const int last = min(u1, n4);  // history tiles of this segment end here
+  int next = u0 + warp;          // the next tile to copy
+  const uint8_t *kp, *vp, *ksp, *vsp;
+  const int32_t* cp;
+  {
+    const int64_t r = static_cast<int64_t>(next) * KV4_TILE;
+    kp = p.hist.k_codes + b * p.hist.cb + h * p.hist.ch + r * St::ROW + lane * 16;
+    vp = p.hist.v_codes + b * p.hist.cb + h * p.hist.ch + r * St::ROW + lane * 16;
+    ksp = reinterpret_cast<const uint8_t*>(p.hist.k_scales + b * p.hist.sb + h * p.hist.sh) + (r + lane) * St::SROW;
+    vsp = reinterpret_cast<const uint8_t*>(p.hist.v_scales + b * p.hist.sb + h * p.hist.sh) + (r + lane) * St::SROW;
+    cp = p.counts + b * p.mb + h * p.mh + r + lane;
+  }
+  const uint32_t code_at = ring + St::piece(lane / PPR, lane % PPR), row_at = ring + lane * St::SROW;
+  auto issue = [&](int stage) {
+    if (next < last) {
+      const int rem = n - next * KV4_TILE;
+      const uint32_t code = code_at + stage * St::BYTES, row = row_at + stage * St::BYTES;
       if (rem >= KV4_TILE) {
 #pragma unroll
         for (int i = 0; i < PPR; ++i) {
-          cp_async(dst + St::K + 512 * i, kp + 512 * i, 16);
-          cp_async(dst + St::V + 512 * i, vp + 512 * i, 16);
+          cp_async<16>(code + St::K + 512 * i, kp + 512 * i);
+          cp_async<16>(code + St::V + 512 * i, vp + 512 * i);
         }
-        cp_async_small<St::SROW>(row_dst + St::KS, ks + k0 * St::SROW, true);
-        cp_async_small<St::SROW>(row_dst + St::VS, vs + k0 * St::SROW, true);
-        cp_async_small<4>(ring32 + stage * St::BYTES + St::C + 4 * lane, cnt + k0, true);
-      } else {  // rows past the end are filled with zeros: count 0 masks them
+        cp_async<St::SROW>(row + St::KS, ksp);
+        cp_async<St::SROW>(row + St::VS, vsp);
+        cp_async<4>(row - lane * (St::SROW - 4) + St::C, cp);
+      } else {  // rows past the end are filled with zeros (count 0 masks them), read from the first row: nothing
 #pragma unroll
         for (int i = 0; i < PPR; ++i) {
-          const bool ok = my_row + i * (32 / PPR) < rem;
-          cp_async(dst + St::K + 512 * i, ok ? kp + 512 * i : kp - lane * 16, ok ? 16 : 0);
-          cp_async(dst + St::V + 512 * i, ok ? vp + 512 * i : vp - lane * 16, ok ? 16 : 0);
+          const bool ok = lane / PPR + i * (32 / PPR) < rem;
+          cp_async_if<16>(code + St::K + 512 * i, ok ? kp + 512 * i : kp - lane * 16, ok);
+          cp_async_if<16>(code + St::V + 512 * i, ok ? vp + 512 * i : vp - lane * 16, ok);
         }
         const bool ok = lane < rem;
-        const int back = ok ? 0 : lane;  // the tile's first row, of which nothing is read
-        cp_async_small<St::SROW>(row_dst + St::KS, ks + (k0 - back) * St::SROW, ok);
-        cp_async_small<St::SROW>(row_dst + St::VS, vs + (k0 - back) * St::SROW, ok);
-        cp_async_small<4>(ring32 + stage * St::BYTES + St::C + 4 * lane, cnt + k0 - back, ok);
+        cp_async_if<St::SROW>(row + St::KS, ok ? ksp : ksp - lane * St::SROW, ok);
+        cp_async_if<St::SROW>(row + St::VS, ok ? vsp : vsp - lane * St::SROW, ok);
+        cp_async_if<4>(row - lane * (St::SROW - 4) + St::C, ok ? cp : cp - lane, ok);
       }
+      next += KV4_NW;
+      kp += KV4_NW * KV4_TILE * St::ROW;
+      vp += KV4_NW * KV4_TILE * St::ROW;
+      ksp += KV4_NW * KV4_TILE * St::SROW;
+      vsp += KV4_NW * KV4_TILE * St::SROW;
+      cp += KV4_NW * KV4_TILE;
     }
     cp_commit();
   };
 #pragma unroll
-  for (int s = 0; s < KV4_STAGES - 1; ++s) issue(u0 + warp + s * KV4_NW, s);
+  for (int s = 0; s < KV4_STAGES - 1; ++s) issue(s);
 
   const T* qp = static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + h0) * p.qh;
   Kv4Query<T, D> q;
@@ -311,39 +370,32 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   int unit = u0 + warp, stage = 0;
   for (; unit < last; unit += KV4_NW) {
     cp_wait<KV4_STAGES - 2>();
-    __syncwarp();
-    uint8_t* sp = ring + stage * St::BYTES;
+    __syncwarp();  // and every lane has read the tile before this one: its stage may be filled again
+    issue(stage == 0 ? KV4_STAGES - 1 : stage - 1);
+    const uint32_t sp = ring + stage * St::BYTES;
     // entries that take no part: their scores are -inf, and 0 times their scales has to be 0
-    const bool masked = __any_sync(0xFFFFFFFFu, *reinterpret_cast<const int32_t*>(sp + St::C + 4 * lane) <= 0);
+    const bool out = static_cast<int32_t>(lds32(sp + St::C + 4 * lane)) <= 0;
+    const bool masked = __any_sync(0xFFFFFFFFu, out);
     if (masked) {
-      if (*reinterpret_cast<const int32_t*>(sp + St::C + 4 * lane) <= 0) {
-        *reinterpret_cast<int32_t*>(sp + St::C + 4 * lane) = 0;
+      if (out) {
+        sts32(sp + St::C + 4 * lane, 0u);
 #pragma unroll
-        for (int i = 0; i < St::SROW / 8; ++i)
-          *reinterpret_cast<uint2*>(sp + St::VS + lane * St::SROW + 8 * i) = make_uint2(0u, 0u);
+        for (int i = 0; i < St::SROW / 4; ++i) sts32(sp + St::VS + lane * St::SROW + 4 * i, 0u);
       }
       __syncwarp();
     }
     // ---- scores
-    float z[2][4], c[2][2];
+    float zs[2][4], c[2][2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r0 = 16 * i + gq, r1 = r0 + 8;
-      uint32_t w[2][NG], s2[2][NG / 2], zw[2];  // codes (word g), scale pairs, word of scales or zeros of both rows
+      uint32_t w[2][NG], s2[2][NG / 2], zw[2];  // codes (word g), scale pairs, word of (scales, zeros) of rows 16 i + gq, + 8
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const int r = f ? r1 : r0;
-        c[i][f] = static_cast<float>(*reinterpret_cast<const int32_t*>(sp + St::C + 4 * r));
-        const uint8_t* sr = sp + St::KS + r * St::SROW;
-        if constexpr (NG == 4) {
-          *reinterpret_cast<uint4*>(w[f]) = *reinterpret_cast<const uint4*>(sp + St::K + St::piece(r, t));
-          *reinterpret_cast<uint2*>(s2[f]) = *reinterpret_cast<const uint2*>(sr);
-          zw[f] = *reinterpret_cast<const uint32_t*>(sr + 4 * t);
-        } else {
-          *reinterpret_cast<uint2*>(w[f]) = *reinterpret_cast<const uint2*>(sp + St::K + St::piece(r, t >> 1) + 8 * (t & 1));
-          s2[f][0] = *reinterpret_cast<const uint32_t*>(sr);
-          zw[f] = *reinterpret_cast<const uint32_t*>(sr + 4 * (t & 1));
-        }
+        const int r = 16 * i + 8 * f;
+        c[i][f] = static_cast<float>(static_cast<int32_t>(lds32(sp + 4 * gq + (St::C + 4 * r))));
+        lds_words<NG>(w[f], sp + k_at + r * St::ROW);
+        lds_words<NG / 2>(s2[f], sp + ks_at + r * St::SROW);
+        zw[f] = lds32(sp + ks_at + (NG == 4 ? 4 * t : 4 * (t & 1)) + r * St::SROW);
       }
       float s[4];
       mma16816_set<__nv_bfloat16>(s, zw[0], zw[1], zw[0], zw[1], q.zc[0], q.zc[1]);
@@ -366,52 +418,47 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
         s[3] = fmaf(xb, a[3], s[3]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) z[i][e] = s[e] * q.back[e & 1];
+      for (int e = 0; e < 4; ++e) zs[i][e] = s[e] * q.back[e & 1];
       if (masked) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[i][e] = c[i][e >> 1] > 0.f ? z[i][e] : -INFINITY;
+        for (int e = 0; e < 4; ++e) zs[i][e] = c[i][e >> 1] > 0.f ? zs[i][e] : -INFINITY;
       }
       if (sc0) {  // the rows of the workspace have room for whole tiles
         float* o = sc0 + static_cast<int64_t>(unit) * KV4_TILE + 16 * i;
-        if (head0) { o[0] = z[i][0]; o[8] = z[i][2]; }
-        if (head1) { o[p.sstride] = z[i][1]; o[p.sstride + 8] = z[i][3]; }
+        if (head0) { o[0] = zs[i][0]; o[8] = zs[i][2]; }
+        if (head1) { o[p.sstride] = zs[i][1]; o[p.sstride + 8] = zs[i][3]; }
       }
     }
-    acc.template weights<2>(z, c);
+    acc.template weights<2>(zs, c);
     // ---- values
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       uint32_t ph[2], pl[2];  // weights of keys 2 t, 2 t + 1 (+ 8) for head lane / 4, two parts
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        split2<__nv_bfloat16>(z[i][2 * f], z[i][2 * f + 1], ph[f], pl[f]);
+        split2<__nv_bfloat16>(zs[i][2 * f], zs[i][2 * f + 1], ph[f], pl[f]);
         ph[f] = movm(ph[f]);
         pl[f] = movm(pl[f]);
       }
       uint32_t w[4][NG], s[4][NG / 2];  // codes and scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int r = 16 * i + 2 * t + (k & 1) + 8 * (k >> 1);
-        if constexpr (NG == 4) {
-          *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(sp + St::V + St::piece(r, gq >> 1));
-          *reinterpret_cast<uint2*>(s[k]) = *reinterpret_cast<const uint2*>(sp + St::VS + r * St::SROW);
-        } else {
-          *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(sp + St::V + St::piece(r, gq >> 2) + 8 * ((gq >> 1) & 1));
-          s[k][0] = *reinterpret_cast<const uint32_t*>(sp + St::VS + r * St::SROW);
-        }
+        const int r = 16 * i + (k & 1) + 8 * (k >> 1);
+        lds_words<NG>(w[k], sp + v_at + r * St::ROW);
+        lds_words<NG / 2>(s[k], sp + vs_at + r * St::SROW);
       }
       // sums of p scale and p zero: rows are the stored values
       uint32_t a0, a2;
       if constexpr (NG == 4) {
-        const uint32_t at = smem_u32(sp + St::VS + (16 * i + (lane & 15)) * St::SROW);
-        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(a0), "=r"(a2) : "r"(at));
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
+                     : "=r"(a0), "=r"(a2)
+                     : "r"(sp + St::VS + (lane & 15) * St::SROW + 16 * i * St::SROW)
+                     : "memory");
       } else {
         uint32_t v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 16 * i + 2 * t + (k & 1) + 8 * (k >> 1);
-          v[k] = gq < 4 ? *reinterpret_cast<const uint16_t*>(sp + St::VS + r * St::SROW + 2 * gq) : 0u;
-        }
+        for (int k = 0; k < 4; ++k)
+          v[k] = gq < 4 ? lds16(sp + vs_at + 2 * gq + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW) : 0u;
         a0 = prmt(v[0], v[1], 0x5410);
         a2 = prmt(v[2], v[3], 0x5410);
       }
@@ -424,10 +471,9 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
         uint32_t wh[2], wl[2], x[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const __nv_bfloat162 sc = as_b2(prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u));
-          const __nv_bfloat162 hi = __hmul2(as_b2(ph[f]), sc);
-          wh[f] = as_u32(hi);
-          wl[f] = as_u32(__hfma2(as_b2(pl[f]), sc, __hfma2(as_b2(ph[f]), sc, __hneg2(hi))));
+          const uint32_t sc = prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u);
+          wh[f] = bmul2(ph[f], sc);
+          wl[f] = bfma2(pl[f], sc, bfms2(ph[f], sc, wh[f]));
           x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
         }
         const uint32_t a[4] = {code_pair<0>(x[0]), code_pair<1>(x[0]), code_pair<0>(x[1]), code_pair<1>(x[1])};
@@ -438,8 +484,6 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
         mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wl[0], wl[1]);
       }
     }
-    __syncwarp();  // every lane has read the stage before: it may be filled again
-    issue(unit + (KV4_STAGES - 1) * KV4_NW, stage == 0 ? KV4_STAGES - 1 : stage - 1);
     stage = stage == KV4_STAGES - 1 ? 0 : stage + 1;
   }
   cp_wait<0>();
@@ -481,7 +525,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   }
   for (; unit < u1; unit += KV4_NW) {
     const int j0 = (unit - n4) * 16;
-    float z[1][4], c[1][2];
+    float zs[1][4], c[1][2];
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     const bool okr[2] = {j0 + gq < elen, j0 + gq + 8 < elen};
     uint4 ka[NG], kb[NG];
@@ -502,14 +546,14 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     for (int e = 0; e < 4; ++e) {
       const bool ok = okr[e >> 1];
       c[0][e >> 1] = ok ? 1.f : 0.f;
-      z[0][e] = ok ? s[e] * p.scale_log2 : -INFINITY;
-      if (sc0 && (e & 1 ? head1 : head0) && ok) sc0[(e & 1) * p.sstride + p.wcol + j0 + 8 * (e >> 1)] = z[0][e];
+      zs[0][e] = ok ? s[e] * p.scale_log2 : -INFINITY;
+      if (sc0 && (e & 1 ? head1 : head0) && ok) sc0[(e & 1) * p.sstride + p.wcol + j0 + 8 * (e >> 1)] = zs[0][e];
     }
-    acc.template weights<1>(z, c);
+    acc.template weights<1>(zs, c);
     uint32_t ph[2], pl[2];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      split2<T>(z[0][2 * f], z[0][2 * f + 1], ph[f], pl[f]);
+      split2<T>(zs[0][2 * f], zs[0][2 * f + 1], ph[f], pl[f]);
       ph[f] = movm(ph[f]);
       pl[f] = movm(pl[f]);
     }
@@ -533,7 +577,6 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     }
   }
 
-  grid_next();
   // ---- the warps' parts to one: common maximum, then sums through shared memory
   __shared__ float sm_m[KV4_NW][8], sm_l[KV4_NW][8];
 #pragma unroll
@@ -574,12 +617,21 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   for (int i = threadIdx.x; i < ng * (D / 4); i += KV4_NW * 32) {
     const int hd = i / (D / 4), d = (i - hd * (D / 4)) * 4;
     float4 a = *reinterpret_cast<const float4*>(base + hd * OR + d);
+    float l = sm_l[0][hd];
 #pragma unroll
     for (int w = 1; w < KV4_NW; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(base + (w * 8 + hd) * OR + d);
       a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+      l += sm_l[w][hd];
     }
-    *reinterpret_cast<float4*>(p.part + ((row0 + hd) * p.nsplit + blockIdx.x) * D + d) = a;
+    if (slot < 0) {  // the whole head: its output
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* o = static_cast<T*>(p.out) + b * p.ob + (static_cast<int64_t>(h) * p.G + h0 + hd) * p.oh + d;
+      o[0] = from_f32<T>(a.x * inv); o[1] = from_f32<T>(a.y * inv);
+      o[2] = from_f32<T>(a.z * inv); o[3] = from_f32<T>(a.w * inv);
+    } else {
+      *reinterpret_cast<float4*>(p.part + (static_cast<int64_t>(slot) * 8 + hd) * D + d) = a;
+    }
   }
   if (warp == 0 && gq == 0) {
 #pragma unroll
@@ -588,27 +640,128 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
       float l = sm_l[0][hd];
 #pragma unroll
       for (int w = 1; w < KV4_NW; ++w) l += sm_l[w][hd];
-      if (hd < ng) p.stats[(row0 + hd) * p.nsplit + blockIdx.x] = make_float2(mm[e], l);
+      if (hd < ng) {
+        if (slot < 0) p.row_stats[row0 + hd] = make_float2(mm[e] == -INFINITY ? 0.f : mm[e], l == 0.f ? 0.f : 1.f / l);
+        else p.stats[slot * 8 + hd] = make_float2(mm[e], l);
+      }
     }
   }
+  __syncthreads();  // the ring may be filled again
+}
+
+// The units of all heads in a row are cut into even pieces, one per CTA, whatever the heads'
+// lengths: all CTAs run at once and end together. A piece may begin and end inside a head: such
+// heads are joined from the pieces' parts (a CTA's first segment is its part 0, a later one its
+// part 1), a head inside one piece is written here. With far more heads than CTAs a head is a piece.
+template <typename T, int D>
+__global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t warp_sum[KV4_NW];
+  __shared__ int lens[KV4_MAX_HEADS];
+  __shared__ int s_bh, s_at;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hg = (p.G + 7) / 8;
+  int elen = p.exact_len;
+  if (p.state) elen = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.W), p.state[0] + p.lag)));
+  if (p.state && blockIdx.x == 0 && tid == 0) *p.used = elen;
+  // this piece: `left` units from unit `at` of head `bh` (all its groups of q-heads in a row)
+  int bh, at, left;
+  int64_t start = 0, piece = 1;
+  if (p.pieces == 0) {
+    bh = blockIdx.x / hg;
+    left = kv4_units(kv4_len(p, bh), elen);
+    at = (blockIdx.x - bh * hg) * left;
+  } else {
+    // where it begins: the heads' units summed up, each thread a run of heads
+    const int heads = p.B * p.H, per = (heads + KV4_NW * 32 - 1) / (KV4_NW * 32);
+    for (int k = tid; k < heads; k += KV4_NW * 32) lens[k] = kv4_len(p, k);
+    __syncthreads();
+    int64_t mine = 0;
+    for (int k = tid * per; k < min(heads, (tid + 1) * per); ++k) mine += kv4_units(lens[k], elen);
+    mine *= hg;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) warp_sum[warp] = incl;
+    __syncthreads();
+    int64_t first = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < KV4_NW; ++w) {
+      if (w < warp) first += warp_sum[w];
+      total += warp_sum[w];
+    }
+    const int64_t up = total + p.pieces - 1;
+    piece = up >> 32 ? up / p.pieces : static_cast<uint32_t>(up) / static_cast<uint32_t>(p.pieces);
+    piece = max(piece, static_cast<int64_t>(KV4_MIN_UNITS));
+    start = piece * blockIdx.x;
+    if (start >= total) return;
+    left = static_cast<int>(min(piece, total - start));
+    if (first <= start && start < first + mine) {
+      int k = tid * per;
+      int64_t pos = first;
+      while (true) {
+        const int64_t u = static_cast<int64_t>(hg) * kv4_units(lens[k], elen);
+        if (start < pos + u) break;
+        pos += u;
+        ++k;
+      }
+      s_bh = k;
+      s_at = static_cast<int>(start - pos);
+    }
+    __syncthreads();
+    bh = s_bh;
+    at = s_at;
+  }
+  for (int part = 0; left > 0; part = 1) {
+    const int n = p.pieces ? lens[bh] : kv4_len(p, bh), un = kv4_units(n, elen), z = at / un;
+    const int u0 = at - z * un, u1 = min(un, u0 + left);
+    int slot = -1;
+    if (u1 - u0 < un) slot = blockIdx.x * 2 + part;
+    if (u0 == 0 && tid == 0) {
+      // the head's first part and its last piece; -1: no parts
+      int2 info = make_int2(-1, 0);
+      if (slot >= 0) {
+        info = make_int2(slot, static_cast<int>((start + un - 1) / piece));
+      }
+      p.info[bh * hg + z] = info;
+    }
+    kv4_segment<T, D>(p, smem, bh, z, n, elen, u0, u1, slot);
+    left -= u1 - u0;
+    start += u1 - u0;
+    at += u1 - u0;
+    if (at == hg * un) {
+      at = 0;
+      ++bh;
+    }
+  }
+  grid_next();
 }
 
 // ---------------------------------------------------------------------------------- joining
 // Launched while the attention kernel ends (programmatic dependent launch): grid_wait returns once
 // that kernel's writes are there.
-// blockIdx.y: kv-head. The first G CTAs join the splits of one q-head each and write its output;
-// the others add the weights of 1024 entries each (history, then window) to their mass. Every CTA
-// finds its rows' (max, sum) over the splits itself.
+// blockIdx.y: kv-head. The first G CTAs join the parts of one q-head each and write its output;
+// the others add the weights of 1024 entries each (history, then window) to their mass.
 constexpr int KV4_MASS_KEYS = 1024;
 
-// (max, 1 / sum) of a row over its splits, by one warp; 1 / sum is 0 where nothing is left
-__device__ __forceinline__ float2 row_stats(const float2* st, int nsplit, int lane) {
+// part k of a row whose first part and last piece are `info`: part 0 of piece after piece
+__device__ __forceinline__ int64_t part_of(int2 info, int k) { return k == 0 ? info.x : (info.x / 2 + k) * int64_t{2}; }
+
+// (max, 1 / sum) of a row, by one warp; 1 / sum is 0 where nothing is left
+__device__ __forceinline__ float2 row_stats(const Kv4Attn& p, int64_t row, int head, int2 info, int lane) {
+  if (info.x < 0) return p.row_stats[row];
+  const int parts = info.y - info.x / 2 + 1;
   float m = -INFINITY, l = 0.f;
-  for (int s = lane; s < nsplit; s += 32) m = fmaxf(m, st[s].x);
+  for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.stats[part_of(info, k) * 8 + head].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   const float ref = m == -INFINITY ? 0.f : m;
-  for (int s = lane; s < nsplit; s += 32) l = fmaf(st[s].y, ex2(st[s].x - ref), l);
+  for (int k = lane; k < parts; k += 32) {
+    const float2 s = p.stats[part_of(info, k) * 8 + head];
+    l = fmaf(s.y, ex2(s.x - ref), l);
+  }
 #pragma unroll
   for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
   return make_float2(ref, l == 0.f ? 0.f : 1.f / l);
@@ -617,9 +770,9 @@ __device__ __forceinline__ float2 row_stats(const float2* st, int nsplit, int la
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4Attn p) {
   __shared__ float2 st[8];
-  __shared__ float wgt[KV4_MAX_SPLIT];
+  __shared__ float wgt[KV4_MAX_PIECES];
   __shared__ float red[256];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hg = (p.G + 7) / 8;
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   if (static_cast<int>(blockIdx.x) < p.G) {
     grid_wait();
@@ -628,17 +781,18 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
       p.state[0] += 1;
       p.state[1] += 1;
     }
-    const int64_t row = static_cast<int64_t>(bh) * p.G + blockIdx.x;
-    const float2* rs = p.stats + row * p.nsplit;
+    const int2 info = p.info[bh * hg + blockIdx.x / 8];
+    if (info.x < 0) return;  // written already
+    const int parts = info.y - info.x / 2 + 1, head = blockIdx.x & 7;
     if (warp == 0) {
-      const float2 r = row_stats(rs, p.nsplit, lane);
-      for (int s = lane; s < p.nsplit; s += 32) wgt[s] = ex2(rs[s].x - r.x) * r.y;
+      const float2 r = row_stats(p, 0, head, info, lane);
+      for (int k = lane; k < parts; k += 32) wgt[k] = ex2(p.stats[part_of(info, k) * 8 + head].x - r.x) * r.y;
     }
     __syncthreads();
     const int d = threadIdx.x % D;
-    const float* part = p.part + row * p.nsplit * D + d;
     float a = 0.f;
-    for (int s = threadIdx.x / D; s < p.nsplit; s += 256 / D) a = fmaf(part[static_cast<int64_t>(s) * D], wgt[s], a);
+#pragma unroll 4
+    for (int k = threadIdx.x / D; k < parts; k += 256 / D) a = fmaf(p.part[(part_of(info, k) * 8 + head) * D + d], wgt[k], a);
     red[threadIdx.x] = a;
     __syncthreads();
     if (threadIdx.x < D) {
@@ -672,7 +826,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
       if (g < ng && some) sc[g] = *reinterpret_cast<const float4*>(p.scores + (row + g) * p.sstride + key);
     if (g0) __syncthreads();
     if (warp < ng) {
-      const float2 r = row_stats(p.stats + (row + warp) * p.nsplit, p.nsplit, lane);
+      const float2 r = row_stats(p, row + warp, warp, p.info[bh * hg + g0 / 8], lane);
       if (lane == 0) st[warp] = r;
     }
     __syncthreads();
@@ -694,25 +848,27 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
 
 namespace {
 struct Kv4Plan {
-  int nsplit;
+  int pieces;                                   // 0: a piece per head
   int wcol;                                     // first window column of a row of scores
-  int64_t sstride, stats, part, scores, total;  // offsets in bytes
+  int64_t ctas, sstride, info, row_stats, stats, part, scores, total;  // offsets in bytes
 };
 Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_t W, bool mass, int sms) {
   auto up = [](int64_t x) { return (x + 255) & ~int64_t{255}; };
   Kv4Plan w;
-  const int64_t rows = B * H * G, ctas = B * H * ((G + 7) / 8);
-  const int64_t units = (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16;
-  int64_t ns = ctas > 0 ? 3 * static_cast<int64_t>(sms) / ctas : 1;
-  const int64_t most = (units + 2 * KV4_NW - 1) / (2 * KV4_NW);  // two tiles a warp
-  ns = ns < most ? ns : most;
-  ns = ns < KV4_MAX_SPLIT ? ns : KV4_MAX_SPLIT;
-  w.nsplit = static_cast<int>(ns > 1 ? ns : 1);
+  const int64_t rows = B * H * G, heads = B * H * ((G + 7) / 8);
+  const int64_t slots = std::min<int64_t>((D == 64 ? 4 : 3) * static_cast<int64_t>(sms), KV4_MAX_PIECES);
+  const int64_t units = heads * std::max<int64_t>(1, (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16);
+  // Four heads a CTA and more even out by themselves; below that the pieces have to be even
+  // (16 sequences x 8 heads of 1024 to 8192 entries).
+  w.pieces = heads >= std::min<int64_t>(4 * slots, KV4_MAX_HEADS) ? 0 : static_cast<int>(std::min(slots, (units + KV4_MIN_UNITS - 1) / KV4_MIN_UNITS));
+  w.ctas = w.pieces ? w.pieces : heads;
   w.wcol = static_cast<int>((cap + KV4_TILE - 1) / KV4_TILE * KV4_TILE);
   w.sstride = w.wcol + (W + 3) / 4 * 4;
-  w.stats = 256;
-  w.part = w.stats + up(rows * w.nsplit * 8);
-  w.scores = w.part + up(rows * w.nsplit * D * 4);
+  w.info = 256;
+  w.row_stats = w.info + up(heads * 8);
+  w.stats = w.row_stats + up(rows * 8);
+  w.part = w.stats + up(w.pieces * 2 * 8 * 8);
+  w.scores = w.part + up(w.pieces * 2 * 8 * D * 4);
   w.total = w.scores + (mass ? up(rows * w.sstride * 4) : 0);
   return w;
 }
@@ -729,7 +885,7 @@ size_t kv4_attn_workspace(int64_t B, int64_t H, int64_t G, int64_t D, int64_t ca
 }
 
 template <typename T, int D>
-static cudaError_t kv4_run(const Kv4Attn& p, cudaStream_t st) {
+static cudaError_t kv4_run(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
   constexpr int RING = KV4_NW * KV4_STAGES * Kv4Stage<D>::BYTES, OUT = KV4_NW * 8 * (D + 4) * 4;
   constexpr int SMEM = RING > OUT ? RING : OUT;
   static std::atomic<uint64_t> set{0};  // the shared-memory limit is raised once per device
@@ -742,8 +898,7 @@ static cudaError_t kv4_run(const Kv4Attn& p, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     set.fetch_or(bit);
   }
-  dim3 grid(static_cast<unsigned>(p.nsplit), static_cast<unsigned>(p.B * p.H), static_cast<unsigned>((p.G + 7) / 8));
-  kv4_attn_kernel<T, D><<<grid, KV4_NW * 32, SMEM, st>>>(p);
+  kv4_attn_kernel<T, D><<<static_cast<unsigned>(ctas), KV4_NW * 32, SMEM, st>>>(p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   const int mass = p.scores ? static_cast<int>((p.sstride + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS) : 0;
@@ -763,15 +918,17 @@ cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaSt
   if (p.B * p.H == 0) return cudaSuccess;
   const bool mass = p.mass || p.exact_mass;
   const Kv4Plan w = kv4_plan(p.B, p.H, p.G, D, p.cap, p.W, mass, kv4_sms());
-  p.nsplit = w.nsplit;
+  p.pieces = w.pieces;
   p.sstride = w.sstride;
   p.wcol = w.wcol;
+  p.info = reinterpret_cast<int2*>(ws + w.info);
+  p.row_stats = reinterpret_cast<float2*>(ws + w.row_stats);
   p.stats = reinterpret_cast<float2*>(ws + w.stats);
   p.part = reinterpret_cast<float*>(ws + w.part);
   p.used = reinterpret_cast<int*>(ws + 64);
   p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
-  if (dtype == BF16) return D == 64 ? kv4_run<__nv_bfloat16, 64>(p, st) : kv4_run<__nv_bfloat16, 128>(p, st);
-  return D == 64 ? kv4_run<__half, 64>(p, st) : kv4_run<__half, 128>(p, st);
+  if (dtype == BF16) return D == 64 ? kv4_run<__nv_bfloat16, 64>(p, w.ctas, st) : kv4_run<__nv_bfloat16, 128>(p, w.ctas, st);
+  return D == 64 ? kv4_run<__half, 64>(p, w.ctas, st) : kv4_run<__half, 128>(p, w.ctas, st);
 }
 
 }  // namespace dab
