@@ -63,7 +63,8 @@ struct Kv4Attn {
   int2* info; float2* row_stats; float2* stats; float* part; float* scores;
   int* used;                                     // with state: the window length this call attends with
   int64_t sstride; int wcol;                     // columns of a row of scores, the window's first
-  int pieces;                                    // 0: one per head
+  int splits, pieces;                            // per head, or in all
+  int* err;                                      // error word
 };
 
 // x rounded down (towards -inf) to bf16, as fp32

@@ -59,6 +59,11 @@ __device__ __forceinline__ void cp_async_if(uint32_t dst, const void* src, bool 
 }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -114,6 +119,13 @@ __device__ __forceinline__ void lds_words(uint32_t* w, uint32_t at) {
   else
     w[0] = lds32(at);
 }
+template <bool TRANS>
+__device__ __forceinline__ void ldsm_x4(uint32_t* r, uint32_t at) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
 __device__ __forceinline__ void sts32(uint32_t at, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
@@ -156,16 +168,16 @@ struct Kv4Acc {
     for (int e = 0; e < 4; ++e) sz[e] = 0.f;
   }
 
-  // Scores of 16 NT keys (lane: keys lane / 4 + 8 f of each 16, heads 2 t + e in [2 f + e]) to
+  // Scores of 16 NT keys (lane: rows lane / 4 + 8 f of each 16, heads 2 t + e in [2 f + e]) to
   // weights. The maximum moves only when a score is KV4_SLACK above it: weights stay below
-  // 2^KV4_SLACK counts, and the accumulators are hardly ever rescaled.
+  // 2^KV4_SLACK, and the accumulators are hardly ever rescaled.
   template <int NT>
-  __device__ __forceinline__ void weights(float (&z)[NT][4], const float (&c)[NT][2]) {
+  __device__ __forceinline__ void weights(float (&z)[NT][4]) {
     float a = -INFINITY, b = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      a = fmaxf(a, fmaxf(z[i][0], z[i][2]));
-      b = fmaxf(b, fmaxf(z[i][1], z[i][3]));
+      a = fmax3(a, z[i][0], z[i][2]);
+      b = fmax3(b, z[i][1], z[i][3]);
     }
     if (__any_sync(0xFFFFFFFFu, a > m[0] + KV4_SLACK || b > m[1] + KV4_SLACK)) {
 #pragma unroll
@@ -191,7 +203,7 @@ struct Kv4Acc {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        z[i][e] = c[i][e >> 1] * ex2(z[i][e] - (e & 1 ? rb : ra));
+        z[i][e] = ex2(z[i][e] - (e & 1 ? rb : ra));
         l[e & 1] += z[i][e];
       }
   }
@@ -202,11 +214,11 @@ struct Kv4Acc {
 template <typename T, int D>
 struct Kv4Query {
   static constexpr int NG = D / 32;
-  uint32_t b[NG][2][2];  // [group][half][..]: pairs (8 t + 2 half + {0, 1}, + 4) of the group
   uint32_t zc[3];        // coefficient pairs of a row's word of (scales, zeros), in three parts
   float back[2];         // of heads 2 t, 2 t + 1: what takes the product to log2 units
 
-  __device__ __forceinline__ void load(const T* q, int64_t stride, int ng, float scale_log2) {
+  // `frag` gets the pairs (8 t + 2 half + {0, 1}, + 4) of every group, [group][lane][2 half + ..]
+  __device__ __forceinline__ void load(const T* q, int64_t stride, int ng, float scale_log2, uint4* frag) {
     const int lane = threadIdx.x & 31, t = lane & 3, head = lane >> 2;
     uint4 w[NG];
     float top = 0.f;
@@ -229,14 +241,16 @@ struct Kv4Query {
     for (int g = 0; g < NG; ++g) {
       const T* e = reinterpret_cast<const T*>(&w[g]);
       float even = 0.f, odd = 0.f;
+      uint32_t b[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // elements i, i + 4
         const __half2 x = __floats2half2_rn(to_f32(e[i]) * f, to_f32(e[i + 4]) * f);
         const float2 y = __half22float2(x);
-        b[g][i >> 1][i & 1] = *reinterpret_cast<const uint32_t*>(&x);
+        b[i] = *reinterpret_cast<const uint32_t*>(&x);
         if (i & 1) odd += y.x + y.y;
         else even += y.x + y.y;
       }
+      if (threadIdx.x < 32) frag[g * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
 #pragma unroll
       for (int o = 1; o <= 2; o <<= 1) {
         even += __shfl_xor_sync(0xFFFFFFFFu, even, o);
@@ -289,8 +303,8 @@ __device__ __forceinline__ int kv4_units(int n, int elen) {
 }
 
 // Units [u0, u1) of group z (8 q-heads) of head bh, by the whole CTA.
-template <typename T, int D>
-__device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int bh, int z, int n, int elen, int u0,
+template <typename T, int D, bool MASS>
+__device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uint4* frag, int bh, int z, int n, int elen, int u0,
                                             int u1, int slot) {
   using St = Kv4Stage<D>;
   constexpr int NG = D / 32;
@@ -361,10 +375,12 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int
 
   const T* qp = static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + h0) * p.qh;
   Kv4Query<T, D> q;
-  q.load(qp, p.qh, ng, p.scale_log2);
+  q.load(qp, p.qh, ng, p.scale_log2, frag);
+  __syncthreads();  // the fragments are there
   Kv4Acc<D> acc;
   acc.init();
-  float* sc0 = p.scores ? p.scores + (row0 + 2 * t) * p.sstride + gq : nullptr;
+  float* sc0 = MASS ? p.scores + (row0 + 2 * t) * p.sstride + gq : nullptr;
+  const uint32_t frag_at = smem_u32(frag + lane);
   const bool head0 = 2 * t < ng, head1 = 2 * t + 1 < ng;
 
   int unit = u0 + warp, stage = 0;
@@ -373,63 +389,78 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int
     __syncwarp();  // and every lane has read the tile before this one: its stage may be filled again
     issue(stage == 0 ? KV4_STAGES - 1 : stage - 1);
     const uint32_t sp = ring + stage * St::BYTES;
-    // entries that take no part: their scores are -inf, and 0 times their scales has to be 0
-    const bool out = static_cast<int32_t>(lds32(sp + St::C + 4 * lane)) <= 0;
-    const bool masked = __any_sync(0xFFFFFFFFu, out);
-    if (masked) {
-      if (out) {
-        sts32(sp + St::C + 4 * lane, 0u);
+    // log2 of the counts; entries that take no part have -inf, and their scales, which may be
+    // anything, are set to 0
+    const int32_t count = static_cast<int32_t>(lds32(sp + St::C + 4 * lane));
+    sts32(sp + St::C + 4 * lane, __float_as_uint(count > 0 ? lg2(static_cast<float>(count)) : -INFINITY));
+    if (count <= 0) {
 #pragma unroll
-        for (int i = 0; i < St::SROW / 4; ++i) sts32(sp + St::VS + lane * St::SROW + 4 * i, 0u);
+      for (int i = 0; i < St::SROW / 4; ++i) {
+        sts32(sp + St::KS + lane * St::SROW + 4 * i, 0u);
+        sts32(sp + St::VS + lane * St::SROW + 4 * i, 0u);
       }
-      __syncwarp();
     }
+    __syncwarp();
     // ---- scores
-    float zs[2][4], c[2][2];
+    float zs[2][4];
+    {
+      uint32_t w[2][2][NG], s2[2][2][NG / 2];  // codes (word g) and scale pairs of rows 16 i + 8 f + gq
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t w[2][NG], s2[2][NG / 2], zw[2];  // codes (word g), scale pairs, word of (scales, zeros) of rows 16 i + gq, + 8
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const int r = 16 * i + 8 * f;
-        c[i][f] = static_cast<float>(static_cast<int32_t>(lds32(sp + 4 * gq + (St::C + 4 * r))));
-        lds_words<NG>(w[f], sp + k_at + r * St::ROW);
-        lds_words<NG / 2>(s2[f], sp + ks_at + r * St::SROW);
-        zw[f] = lds32(sp + ks_at + (NG == 4 ? 4 * t : 4 * (t & 1)) + r * St::SROW);
+        for (int f = 0; f < 2; ++f) {
+          const int r = 16 * i + 8 * f;
+          lds_words<NG>(w[i][f], sp + k_at + r * St::ROW);
+          lds_words<NG / 2>(s2[i][f], sp + ks_at + r * St::SROW);
+        }
+        uint32_t zw[4];  // word t of (scales, zeros) of both rows, twice
+        if constexpr (NG == 4) {
+          ldsm_x4<false>(zw, sp + St::KS + (lane & 15) * St::SROW + 16 * i * St::SROW);
+        } else {
+#pragma unroll
+          for (int f = 0; f < 2; ++f) zw[f] = zw[f + 2] = lds32(sp + ks_at + 4 * (t & 1) + (16 * i + 8 * f) * St::SROW);
+        }
+        mma16816_set<__nv_bfloat16>(zs[i], zw[0], zw[1], zw[2], zw[3], q.zc[0], q.zc[1]);
+        if constexpr (NG == 4) mma16816<__nv_bfloat16>(zs[i], zw[0], zw[1], zw[2], zw[3], q.zc[2], 0u);
       }
-      float s[4];
-      mma16816_set<__nv_bfloat16>(s, zw[0], zw[1], zw[0], zw[1], q.zc[0], q.zc[1]);
-      if constexpr (NG == 4) mma16816<__nv_bfloat16>(s, zw[0], zw[1], 0u, 0u, q.zc[2], 0u);
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
-        float a[4];
-        uint32_t x[2] = {w[0][g] << 2, w[1][g] << 2};
-        mma16816_set<__half>(a, code_pair_h<0>(x[0]), code_pair_h<0>(x[1]), code_pair_h<1>(x[0]), code_pair_h<1>(x[1]),
-                             q.b[g][0][0], q.b[g][0][1]);
-        x[0] = w[0][g] >> 6;
-        x[1] = w[1][g] >> 6;
-        mma16816<__half>(a, code_pair_h<2>(x[0]), code_pair_h<2>(x[1]), code_pair_h<3>(x[0]), code_pair_h<3>(x[1]),
-                         q.b[g][1][0], q.b[g][1][1]);
-        const float xa = g & 1 ? hi_f32(s2[0][g >> 1]) : lo_f32(s2[0][g >> 1]);
-        const float xb = g & 1 ? hi_f32(s2[1][g >> 1]) : lo_f32(s2[1][g >> 1]);
-        s[0] = fmaf(xa, a[0], s[0]);
-        s[1] = fmaf(xa, a[1], s[1]);
-        s[2] = fmaf(xb, a[2], s[2]);
-        s[3] = fmaf(xb, a[3], s[3]);
-      }
+        uint32_t qf[4];
+        lds_words<4>(qf, frag_at + g * 512);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) zs[i][e] = s[e] * q.back[e & 1];
-      if (masked) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) zs[i][e] = c[i][e >> 1] > 0.f ? zs[i][e] : -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+          float a[4];
+          uint32_t x[2] = {w[i][0][g] << 2, w[i][1][g] << 2};
+          mma16816_set<__half>(a, code_pair_h<0>(x[0]), code_pair_h<0>(x[1]), code_pair_h<1>(x[0]), code_pair_h<1>(x[1]),
+                               qf[0], qf[1]);
+          x[0] = w[i][0][g] >> 6;
+          x[1] = w[i][1][g] >> 6;
+          mma16816<__half>(a, code_pair_h<2>(x[0]), code_pair_h<2>(x[1]), code_pair_h<3>(x[0]), code_pair_h<3>(x[1]),
+                           qf[2], qf[3]);
+          const float xa = g & 1 ? hi_f32(s2[i][0][g >> 1]) : lo_f32(s2[i][0][g >> 1]);
+          const float xb = g & 1 ? hi_f32(s2[i][1][g >> 1]) : lo_f32(s2[i][1][g >> 1]);
+          zs[i][0] = fmaf(xa, a[0], zs[i][0]);
+          zs[i][1] = fmaf(xa, a[1], zs[i][1]);
+          zs[i][2] = fmaf(xb, a[2], zs[i][2]);
+          zs[i][3] = fmaf(xb, a[3], zs[i][3]);
+        }
       }
-      if (sc0) {  // the rows of the workspace have room for whole tiles
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        const float lg = __uint_as_float(lds32(sp + 4 * gq + St::C + 64 * i + 32 * f));
+        zs[i][2 * f] = fmaf(zs[i][2 * f], q.back[0], lg);
+        zs[i][2 * f + 1] = fmaf(zs[i][2 * f + 1], q.back[1], lg);
+      }
+      if constexpr (MASS) {  // the rows of the workspace have room for whole tiles
         float* o = sc0 + static_cast<int64_t>(unit) * KV4_TILE + 16 * i;
         if (head0) { o[0] = zs[i][0]; o[8] = zs[i][2]; }
         if (head1) { o[p.sstride] = zs[i][1]; o[p.sstride + 8] = zs[i][3]; }
       }
     }
-    acc.template weights<2>(zs, c);
+    acc.template weights<2>(zs);
     // ---- values
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -447,24 +478,19 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int
         lds_words<NG>(w[k], sp + v_at + r * St::ROW);
         lds_words<NG / 2>(s[k], sp + vs_at + r * St::SROW);
       }
-      // sums of p scale and p zero: rows are the stored values
-      uint32_t a0, a2;
-      if constexpr (NG == 4) {
-        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
-                     : "=r"(a0), "=r"(a2)
-                     : "r"(sp + St::VS + (lane & 15) * St::SROW + 16 * i * St::SROW)
-                     : "memory");
-      } else {
-        uint32_t v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          v[k] = gq < 4 ? lds16(sp + vs_at + 2 * gq + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW) : 0u;
-        a0 = prmt(v[0], v[1], 0x5410);
-        a2 = prmt(v[2], v[3], 0x5410);
-      }
+      // sums of p scale and p zero: rows are the stored values (and again, for whole operands)
       using B = __nv_bfloat16;
-      mma16816<B>(acc.sz, a0, 0u, a2, 0u, ph[0], ph[1]);
-      mma16816<B>(acc.sz, a0, 0u, a2, 0u, pl[0], pl[1]);
+      uint32_t v[4];
+      if constexpr (NG == 4) {
+        ldsm_x4<true>(v, sp + St::VS + ((lane & 7) + ((lane >> 1) & 8)) * St::SROW + 16 * i * St::SROW);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = lds16(sp + vs_at + 2 * (gq & 3) + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW);
+        v[0] = v[1] = prmt(v[0], v[1], 0x5410);
+        v[2] = v[3] = prmt(v[2], v[3], 0x5410);
+      }
+      mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], ph[0], ph[1]);
+      mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], pl[0], pl[1]);
       const uint32_t half = gq & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -525,7 +551,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int
   }
   for (; unit < u1; unit += KV4_NW) {
     const int j0 = (unit - n4) * 16;
-    float zs[1][4], c[1][2];
+    float zs[1][4];
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     const bool okr[2] = {j0 + gq < elen, j0 + gq + 8 < elen};
     uint4 ka[NG], kb[NG];
@@ -545,11 +571,10 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const bool ok = okr[e >> 1];
-      c[0][e >> 1] = ok ? 1.f : 0.f;
       zs[0][e] = ok ? s[e] * p.scale_log2 : -INFINITY;
-      if (sc0 && (e & 1 ? head1 : head0) && ok) sc0[(e & 1) * p.sstride + p.wcol + j0 + 8 * (e >> 1)] = zs[0][e];
+      if (MASS && (e & 1 ? head1 : head0) && ok) sc0[(e & 1) * p.sstride + p.wcol + j0 + 8 * (e >> 1)] = zs[0][e];
     }
-    acc.template weights<1>(zs, c);
+    acc.template weights<1>(zs);
     uint32_t ph[2], pl[2];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
@@ -649,13 +674,15 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, int
   __syncthreads();  // the ring may be filled again
 }
 
-// The units of all heads in a row are cut into even pieces, one per CTA, whatever the heads'
-// lengths: all CTAs run at once and end together. A piece may begin and end inside a head: such
-// heads are joined from the pieces' parts (a CTA's first segment is its part 0, a later one its
-// part 1), a head inside one piece is written here. With far more heads than CTAs a head is a piece.
-template <typename T, int D>
+// With `splits` every head is cut into that many pieces (as many as it has units). Otherwise the
+// units of all heads in a row are cut into even pieces, one per CTA, whatever the heads' lengths: all
+// CTAs run at once and end together, and a piece may begin and end inside a head. Heads in several
+// pieces are joined from their parts (a CTA's first segment is its part 0, a later one its part 1), a
+// head inside one piece is written here.
+template <typename T, int D, bool MASS>
 __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint4 frag[D];  // q's fragments: D / 32 groups of 32 lanes
   __shared__ int64_t warp_sum[KV4_NW];
   __shared__ int lens[KV4_MAX_HEADS];
   __shared__ int s_bh, s_at;
@@ -664,12 +691,18 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   if (p.state) elen = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.W), p.state[0] + p.lag)));
   if (p.state && blockIdx.x == 0 && tid == 0) *p.used = elen;
   // this piece: `left` units from unit `at` of head `bh` (all its groups of q-heads in a row)
-  int bh, at, left;
+  int bh, at, left, ns = 1, split = 0;
   int64_t start = 0, piece = 1;
-  if (p.pieces == 0) {
-    bh = blockIdx.x / hg;
-    left = kv4_units(kv4_len(p, bh), elen);
-    at = (blockIdx.x - bh * hg) * left;
+  if (p.splits) {
+    const int w = blockIdx.x / p.splits, z = w % hg;
+    bh = w / hg;
+    split = blockIdx.x - w * p.splits;
+    const int un = kv4_units(kv4_len(p, bh), elen);
+    ns = min(p.splits, un);
+    if (split >= ns) return;
+    const int u0 = static_cast<int>(static_cast<int64_t>(un) * split / ns);
+    left = static_cast<int>(static_cast<int64_t>(un) * (split + 1) / ns) - u0;
+    at = z * un + u0;
   } else {
     // where it begins: the heads' units summed up, each thread a run of heads
     const int heads = p.B * p.H, per = (heads + KV4_NW * 32 - 1) / (KV4_NW * 32);
@@ -715,7 +748,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     at = s_at;
   }
   for (int part = 0; left > 0; part = 1) {
-    const int n = p.pieces ? lens[bh] : kv4_len(p, bh), un = kv4_units(n, elen), z = at / un;
+    const int n = p.splits ? kv4_len(p, bh) : lens[bh], un = kv4_units(n, elen), z = at / un;
     const int u0 = at - z * un, u1 = min(un, u0 + left);
     int slot = -1;
     if (u1 - u0 < un) slot = blockIdx.x * 2 + part;
@@ -723,11 +756,11 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
       // the head's first part and its last piece; -1: no parts
       int2 info = make_int2(-1, 0);
       if (slot >= 0) {
-        info = make_int2(slot, static_cast<int>((start + un - 1) / piece));
+        info = make_int2(slot, p.splits ? static_cast<int>(blockIdx.x) + ns - 1 : static_cast<int>((start + un - 1) / piece));
       }
       p.info[bh * hg + z] = info;
     }
-    kv4_segment<T, D>(p, smem, bh, z, n, elen, u0, u1, slot);
+    kv4_segment<T, D, MASS>(p, smem, frag, bh, z, n, elen, u0, u1, slot);
     left -= u1 - u0;
     start += u1 - u0;
     at += u1 - u0;
@@ -805,14 +838,10 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
   // 4 neighbouring entries a thread: history [0, cap), window from column wcol on
   const int n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
   const int key = (blockIdx.x - p.G) * KV4_MASS_KEYS + 4 * threadIdx.x;
-  const int32_t* cp = p.counts + b * p.mb + h * p.mh + key;
   float* mp = p.mass + b * p.mb + h * p.mh + key;
-  float c[4], m[4], w[4] = {0.f, 0.f, 0.f, 0.f};
+  float m[4], w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // what the attention kernel does not write is read while it ends
-    c[i] = key + i < n ? static_cast<float>(cp[i]) : 0.f;
-    m[i] = key + i < n ? mp[i] : 0.f;
-  }
+  for (int i = 0; i < 4; ++i) m[i] = key + i < n ? mp[i] : 0.f;  // read while the attention kernel ends
   grid_wait();
   const int elen = p.state ? *p.used : p.exact_len, j = key - p.wcol;
   if (blockIdx.x * KV4_MASS_KEYS - p.G * KV4_MASS_KEYS >= max(n, p.wcol + elen)) return;
@@ -841,14 +870,14 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (c[i] > 0.f) mp[i] = fmaf(c[i], w[i], m[i]);
+    if (key + i < n) mp[i] = m[i] + w[i];
     if (j >= 0 && j + i < elen) p.exact_mass[b * p.emb + h * p.emh + j + i] += w[i];
   }
 }
 
 namespace {
 struct Kv4Plan {
-  int pieces;                                   // 0: a piece per head
+  int splits, pieces;                           // one of them is 0
   int wcol;                                     // first window column of a row of scores
   int64_t ctas, sstride, info, row_stats, stats, part, scores, total;  // offsets in bytes
 };
@@ -857,18 +886,21 @@ Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_
   Kv4Plan w;
   const int64_t rows = B * H * G, heads = B * H * ((G + 7) / 8);
   const int64_t slots = std::min<int64_t>((D == 64 ? 4 : 3) * static_cast<int64_t>(sms), KV4_MAX_PIECES);
-  const int64_t units = heads * std::max<int64_t>(1, (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16);
-  // Four heads a CTA and more even out by themselves; below that the pieces have to be even
-  // (16 sequences x 8 heads of 1024 to 8192 entries).
-  w.pieces = heads >= std::min<int64_t>(4 * slots, KV4_MAX_HEADS) ? 0 : static_cast<int>(std::min(slots, (units + KV4_MIN_UNITS - 1) / KV4_MIN_UNITS));
-  w.ctas = w.pieces ? w.pieces : heads;
+  const int64_t units = std::max<int64_t>(1, (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16);
+  w.splits = w.pieces = 0;
+  if (heads >= std::min<int64_t>(4 * slots, KV4_MAX_HEADS)) w.splits = 1;  // so many even out by themselves
+  else if (heads * units <= slots * KV4_MIN_UNITS)  // everything at once: where a piece begins needs no search
+    w.splits = static_cast<int>((units + KV4_MIN_UNITS - 1) / KV4_MIN_UNITS);
+  else w.pieces = static_cast<int>(slots);
+  w.ctas = w.pieces ? w.pieces : heads * w.splits;
   w.wcol = static_cast<int>((cap + KV4_TILE - 1) / KV4_TILE * KV4_TILE);
   w.sstride = w.wcol + (W + 3) / 4 * 4;
+  const int64_t slots2 = w.splits == 1 ? 0 : 2 * w.ctas;  // parts
   w.info = 256;
   w.row_stats = w.info + up(heads * 8);
   w.stats = w.row_stats + up(rows * 8);
-  w.part = w.stats + up(w.pieces * 2 * 8 * 8);
-  w.scores = w.part + up(w.pieces * 2 * 8 * D * 4);
+  w.part = w.stats + up(slots2 * 8 * 8);
+  w.scores = w.part + up(slots2 * 8 * D * 4);
   w.total = w.scores + (mass ? up(rows * w.sstride * 4) : 0);
   return w;
 }
@@ -884,8 +916,8 @@ size_t kv4_attn_workspace(int64_t B, int64_t H, int64_t G, int64_t D, int64_t ca
   return static_cast<size_t>(kv4_plan(B, H, G, D, cap, W, mass, kv4_sms()).total);
 }
 
-template <typename T, int D>
-static cudaError_t kv4_run(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
+template <typename T, int D, bool MASS>
+static cudaError_t kv4_start(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
   constexpr int RING = KV4_NW * KV4_STAGES * Kv4Stage<D>::BYTES, OUT = KV4_NW * 8 * (D + 4) * 4;
   constexpr int SMEM = RING > OUT ? RING : OUT;
   static std::atomic<uint64_t> set{0};  // the shared-memory limit is raised once per device
@@ -894,12 +926,17 @@ static cudaError_t kv4_run(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(set.load() & bit)) {
-    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     set.fetch_or(bit);
   }
-  kv4_attn_kernel<T, D><<<static_cast<unsigned>(ctas), KV4_NW * 32, SMEM, st>>>(p);
-  e = cudaGetLastError();
+  kv4_attn_kernel<T, D, MASS><<<static_cast<unsigned>(ctas), KV4_NW * 32, SMEM, st>>>(p);
+  return cudaGetLastError();
+}
+
+template <typename T, int D>
+static cudaError_t kv4_run(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
+  const cudaError_t e = p.scores ? kv4_start<T, D, true>(p, ctas, st) : kv4_start<T, D, false>(p, ctas, st);
   if (e != cudaSuccess) return e;
   const int mass = p.scores ? static_cast<int>((p.sstride + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS) : 0;
   cudaLaunchConfig_t cfg = {};
@@ -918,7 +955,9 @@ cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaSt
   if (p.B * p.H == 0) return cudaSuccess;
   const bool mass = p.mass || p.exact_mass;
   const Kv4Plan w = kv4_plan(p.B, p.H, p.G, D, p.cap, p.W, mass, kv4_sms());
+  p.splits = w.splits;
   p.pieces = w.pieces;
+  p.err = reinterpret_cast<int*>(ws);
   p.sstride = w.sstride;
   p.wcol = w.wcol;
   p.info = reinterpret_cast<int2*>(ws + w.info);
