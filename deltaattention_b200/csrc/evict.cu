@@ -5,9 +5,11 @@
 // Entries keep their order, and every row buffer is compacted in place with the mass.
 //
 //  * evict_select: one cluster per head finds the k-th largest weight of the middle entries by
-//    radix selection (digits of 11, 11 and 10 bits; every CTA keeps the keys of its slice in shared
-//    memory and counts them, the counts are summed through distributed shared memory), then writes
-//    for every tile how many entries are kept before it and how many of the ties come before it.
+//    radix selection, 8 bits a pass. Every CTA keeps the keys of its slice in registers, 16 a
+//    thread, and counts a pass's digits in shared memory; the counts are summed through distributed
+//    shared memory. Then it writes for every tile how many entries are kept before it and how many
+//    of the ties come before it. (Digits of 11 bits need a pass less, but 8 CTAs summing 2048 counts
+//    from each other took 5000 cycles a pass, 256 take a tenth.)
 //  * evict_move: one CTA per tile reads its kept rows into shared memory, says so, waits for the
 //    (at most two) tiles on whose rows its own will land to have said so too, and writes. Tiles are
 //    handed out in order by a ticket per head and nothing is waited for before a tile has read
@@ -21,10 +23,10 @@ namespace dab {
 
 namespace cg = cooperative_groups;
 
-constexpr int SEL_THREADS = 1024;
-constexpr int SEL_KEYS = 16384;  // keys of a slice held in shared memory; later ones are read again
-constexpr int SEL_BINS = 2048;
-constexpr int MOVE_THREADS = 256;
+constexpr int SEL_THREADS = 1024, SEL_MAX_CTAS = 8;  // of a cluster
+constexpr int SEL_KEYS = 16;                         // a thread's keys in registers; longer slices are read again
+constexpr int SEL_CHUNK = SEL_THREADS * SEL_KEYS;
+constexpr int MOVE_THREADS = 128;
 enum { ERR_EVICT_WAIT = 0x501 };
 
 // Unsigned key of a weight in the order of floats: NaN below everything, -0 equal to +0.
@@ -35,12 +37,13 @@ __device__ __forceinline__ uint32_t mass_key(float x) {
 }
 constexpr uint32_t KEY_ZERO = 0x80000000u;  // weights of 0, which may be many
 
+__device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
   cg::cluster_group cl = cg::this_cluster();
-  extern __shared__ uint32_t sel_smem[];
-  uint32_t* keys = sel_smem;                // [SEL_KEYS]
-  uint32_t* hist = sel_smem + SEL_KEYS;     // [3][SEL_BINS]
-  __shared__ uint32_t wsum[32], s_prefix, s_k, s_tot[2];
+  __shared__ uint32_t hist[4][256];
+  __shared__ uint2 cnt[SEL_CHUNK / EVICT_MIN_TILE];  // of a chunk's tiles: surely kept, ties
+  __shared__ uint32_t wsum[8], s_prefix, s_k, s_tot[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
@@ -57,104 +60,120 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
   const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (rank + 1) / C);
   const int i0 = t0 * p.tile, i1 = min(n, t1 * p.tile);
   const int lo = p.first, hi = n - p.recent;  // the entries that compete
-  for (int i = i0 + tid; i < min(i1, i0 + SEL_KEYS); i += SEL_THREADS) keys[i - i0] = mass_key(mass[i]);
-  for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) hist[i] = 0;
+  uint32_t key[SEL_KEYS];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < SEL_KEYS; ++j) {
+      const int e = base + j * SEL_THREADS + tid;
+      key[j] = e < i1 ? mass_key(mass[e]) : 0u;
+    }
+  };
+  load(i0);
+  const bool one = i1 - i0 <= SEL_CHUNK;
+  (&hist[0][0])[tid] = 0;
   for (int t = t0 + tid; t < t1; t += SEL_THREADS) p.loaded[static_cast<int64_t>(bh) * p.max_tiles + t] = 0u;
-  auto key_at = [&](int i) { return i - i0 < SEL_KEYS ? keys[i - i0] : mass_key(mass[i]); };
   uint32_t k = p.budget - p.first - p.recent, prefix = k ? 0u : 0xFFFFFFFFu;
   __syncthreads();
   if (k) {
 #pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const uint32_t dmask = pass == 2 ? 1023u : 2047u;
-      const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
-      uint32_t* hp = hist + pass * SEL_BINS;
-      for (int i = i0 + warp * 32; i < i1; i += SEL_THREADS) {
-        const int e = i + lane;
-        bool in = e >= lo && e < hi && e < i1;
-        uint32_t key = 0;
-        if (in) key = key_at(e);
-        in = in && (key & above) == prefix;
-        const uint32_t zeros = __ballot_sync(0xFFFFFFFFu, in && key == KEY_ZERO);
-        if (in && key != KEY_ZERO) atomicAdd(&hp[(key >> shift) & dmask], 1u);
-        if (lane == 0 && zeros) atomicAdd(&hp[(KEY_ZERO >> shift) & dmask], __popc(zeros));
-      }
-      cl.sync();
-      // thread i sums bins 2 i, 2 i + 1 from the top over the cluster
-      const int top = SEL_BINS - 2 - 2 * tid;  // bins top + 1 (first), top
-      uint32_t c1 = 0, c0 = 0;
-      for (int r = 0; r < C; ++r) {
-        const uint2 v = *reinterpret_cast<const uint2*>(cl.map_shared_rank(hp, r) + top);
-        c0 += v.x;
-        c1 += v.y;
-      }
-      uint32_t incl = c0 + c1;
+    for (int pass = 0; pass < 4; ++pass) {
+      const int shift = 24 - 8 * pass;
+      const uint32_t above = pass == 0 ? 0u : 0xFFFFFFFFu << (shift + 8);
+      uint32_t zeros = 0;  // many weights may be 0: one addition a warp
+      for (int base = i0; base < i1; base += SEL_CHUNK) {
+        if (!one) load(base);
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
-        if (lane >= o) incl += v;
+        for (int j = 0; j < SEL_KEYS; ++j) {
+          const int e = base + j * SEL_THREADS + tid;
+          if (e >= lo && e < hi && e < i1 && (key[j] & above) == prefix) {
+            if (key[j] == KEY_ZERO) ++zeros;
+            else atomicAdd(&hist[pass][(key[j] >> shift) & 255u], 1u);
+          }
+        }
       }
-      if (lane == 31) wsum[warp] = incl;
+      zeros = __reduce_add_sync(0xFFFFFFFFu, zeros);
+      if (lane == 0 && zeros) atomicAdd(&hist[pass][(KEY_ZERO >> shift) & 255u], zeros);
+      cl.sync();
+      // thread i sums bin 255 - i over the cluster; the digit is where the count from the top reaches k
+      uint32_t c = 0, incl = 0;
+      if (tid < 256) {
+#pragma unroll
+        for (int r = 0; r < SEL_MAX_CTAS; ++r)
+          if (r < C) c += cl.map_shared_rank(&hist[pass][0], r)[255 - tid];
+        incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+          if (lane >= o) incl += v;
+        }
+        if (lane == 31) wsum[warp] = incl;
+      }
       __syncthreads();
-      uint32_t before = incl - c0 - c1;
-      for (int w = 0; w < warp; ++w) before += wsum[w];
-      // the digit is where the count from the top reaches k
-      if (before < k && k <= before + c1) {
-        s_prefix = prefix | (static_cast<uint32_t>(top + 1) << shift);
-        s_k = k - before;
-      } else if (before + c1 < k && k <= before + c1 + c0) {
-        s_prefix = prefix | (static_cast<uint32_t>(top) << shift);
-        s_k = k - before - c1;
+      if (tid < 256) {
+        uint32_t before = incl - c;
+#pragma unroll
+        for (int w = 0; w < 7; ++w)
+          if (w < warp) before += wsum[w];
+        if (before < k && k <= before + c) {
+          s_prefix = prefix | (static_cast<uint32_t>(255 - tid) << shift);
+          s_k = k - before;
+        }
       }
       __syncthreads();
       prefix = s_prefix;
       k = s_k;
-      __syncthreads();
     }
   }
   // per tile: entries surely kept, and ties
   uint2* before = p.before + static_cast<int64_t>(bh) * p.max_tiles;
-  for (int t = t0 + warp; t < t1; t += SEL_THREADS / 32) {
-    uint32_t sure = 0, tie = 0;
-    for (int i = t * p.tile; i < min(n, (t + 1) * p.tile); i += 32) {
-      const int e = i + lane;
-      bool s = false, q = false;
-      if (e < n && e < (t + 1) * p.tile) {
-        const bool mid = e >= lo && e < hi;
-        const uint32_t key = key_at(e);
-        s = !mid || key > prefix;
-        q = mid && key == prefix;
-      }
-      sure += __popc(__ballot_sync(0xFFFFFFFFu, s));
-      tie += __popc(__ballot_sync(0xFFFFFFFFu, q));
-    }
-    if (lane == 0) before[t] = make_uint2(sure, tie);
-  }
-  __syncthreads();
-  if (warp == 0) {  // exclusive sums over this CTA's tiles
-    uint32_t run_s = 0, run_t = 0;
-    for (int t = t0; t < t1; t += 32) {
-      uint2 v = make_uint2(0u, 0u);
-      if (t + lane < t1) v = before[t + lane];
-      uint32_t a = v.x, q = v.y;
+  const int seg = min(p.tile, 32);  // neighbouring lanes of a tile
+  const uint32_t seg_mask = seg == 32 ? 0xFFFFFFFFu : (1u << seg) - 1u;
+  uint32_t run_s = 0, run_t = 0;    // of this CTA's tiles so far (warp 0)
+  for (int base = i0; base < i1; base += SEL_CHUNK) {
+    if (!one) load(base);
+    const int ct = (min(i1, base + SEL_CHUNK) - base + p.tile - 1) / p.tile;  // tiles of the chunk
+    for (int t = tid; t < ct; t += SEL_THREADS) cnt[t] = make_uint2(0u, 0u);
+    __syncthreads();
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, a, o), y = __shfl_up_sync(0xFFFFFFFFu, q, o);
-        if (lane >= o) { a += x; q += y; }
+    for (int j = 0; j < SEL_KEYS; ++j) {
+      const int o = j * SEL_THREADS + tid, e = base + o;
+      const bool mid = e >= lo && e < hi;
+      const uint32_t sb = __ballot_sync(0xFFFFFFFFu, e < i1 && (!mid || key[j] > prefix));
+      const uint32_t tb = __ballot_sync(0xFFFFFFFFu, e < i1 && mid && key[j] == prefix);
+      if (lane % seg == 0 && e < i1) {
+        const uint32_t s = __popc((sb >> lane) & seg_mask), q = __popc((tb >> lane) & seg_mask);
+        if (s) atomicAdd(&cnt[o / p.tile].x, s);
+        if (q) atomicAdd(&cnt[o / p.tile].y, q);
       }
-      if (t + lane < t1) before[t + lane] = make_uint2(run_s + a - v.x, run_t + q - v.y);
-      run_s += __shfl_sync(0xFFFFFFFFu, a, 31);
-      run_t += __shfl_sync(0xFFFFFFFFu, q, 31);
     }
-    if (lane == 0) {
-      s_tot[0] = run_s;
-      s_tot[1] = run_t;
+    __syncthreads();
+    if (warp == 0) {  // exclusive sums
+      const int tb = t0 + (base - i0) / p.tile;
+      for (int t = 0; t < ct; t += 32) {
+        uint2 v = make_uint2(0u, 0u);
+        if (t + lane < ct) v = cnt[t + lane];
+        uint32_t a = v.x, q = v.y;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, a, o), y = __shfl_up_sync(0xFFFFFFFFu, q, o);
+          if (lane >= o) { a += x; q += y; }
+        }
+        if (t + lane < ct) before[tb + t + lane] = make_uint2(run_s + a - v.x, run_t + q - v.y);
+        run_s += __shfl_sync(0xFFFFFFFFu, a, 31);
+        run_t += __shfl_sync(0xFFFFFFFFu, q, 31);
+      }
     }
+    __syncthreads();
+  }
+  if (tid == 0) {
+    s_tot[0] = run_s;
+    s_tot[1] = run_t;
   }
   cl.sync();
   uint32_t base_s = 0, base_t = 0;
-  for (int r = 0; r < rank; ++r) {
+#pragma unroll
+  for (int r = 0; r < SEL_MAX_CTAS - 1; ++r) {
+    if (r >= rank) continue;
     const uint32_t* o = cl.map_shared_rank(s_tot, r);
     base_s += o[0];
     base_t += o[1];
@@ -168,20 +187,33 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
     p.cut[bh] = make_uint4(prefix, k, static_cast<uint32_t>(n), 0u);
     *len = p.budget;  // every CTA of the cluster has read it
   }
+  grid_next();
   cl.sync();  // no CTA leaves while its counts are read
 }
 
-__device__ __forceinline__ void move_in(uint32_t dst, const uint8_t* src, int unit) {
-  if (unit == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  else if (unit == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+// Kernels launched after one another with programmatic dependent launch
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// The kept rows of one buffer into shared memory, U bytes a copy; a row has 2^shift of them, or any
+// number (shift < 0).
+template <int U>
+__device__ __forceinline__ void move_rows(uint32_t dst, const uint8_t* base, int bytes, int shift, const int* src, int kept) {
+  const int upr = bytes / U, total = kept * upr;
+#pragma unroll 4
+  for (int u = threadIdx.x; u < total; u += MOVE_THREADS) {
+    const int e = shift >= 0 ? u >> shift : u / upr;
+    const uint8_t* from = base + static_cast<int64_t>(src[e]) * bytes + (u - e * upr) * U;
+    if constexpr (U == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + u * U), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst + u * U), "l"(from), "n"(U) : "memory");
+  }
 }
 
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ __align__(16) uint8_t mv_smem[];  // src[tile] and mass[tile], then the rows of each buffer
-  __shared__ int w_tie[8], w_keep[8], s_tile;
+  __shared__ int w_tie[MOVE_THREADS / 32], w_keep[MOVE_THREADS / 32], s_tile;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
+  grid_wait();
   const int n = static_cast<int>(p.cut[bh].z);
   if (n == 0 || static_cast<int>(blockIdx.x) * p.tile >= n) return;
   if (tid == 0) s_tile = static_cast<int>(atomicAdd(&p.cut[bh].w, 1u));
@@ -213,7 +245,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
   if (lane == 0) w_keep[warp] = __popc(kb);
   __syncthreads();
   int pos = __popc(kb & below), kept = 0;
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < MOVE_THREADS / 32; ++w) {
     if (w < warp) pos += w_keep[w];
     kept += w_keep[w];
   }
@@ -227,20 +259,18 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
     uint8_t* at = rows;
     for (int r = 0; r < p.n_rows; ++r) {
       const uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r];
-      const int bytes = p.bytes[r], unit = p.unit[r], upr = bytes / unit;
       const uint32_t dst = smem_u32(at);
-      for (int u = tid; u < kept * upr; u += MOVE_THREADS) {
-        const int e = u / upr;
-        move_in(dst + u * unit, base + static_cast<int64_t>(src[e]) * bytes + (u - e * upr) * unit, unit);
-      }
-      at += (p.tile * bytes + 15) & ~15;
+      if (p.unit[r] == 16) move_rows<16>(dst, base, p.bytes[r], p.shift[r], src, kept);
+      else if (p.unit[r] == 8) move_rows<8>(dst, base, p.bytes[r], p.shift[r], src, kept);
+      else move_rows<4>(dst, base, p.bytes[r], p.shift[r], src, kept);
+      at += (p.tile * p.bytes[r] + 15) & ~15;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
   __syncthreads();
   uint32_t* loaded = p.loaded + static_cast<int64_t>(bh) * p.max_tiles;
   if (tid == 0) {
-    __threadfence();  // this tile's rows have been read: others may land on them
+    // this tile's rows have been read (the barrier comes after everybody's copies): others may land on them
     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(loaded + tile), "r"(1u) : "memory");
   }
   if (still || !kept) return;
@@ -282,7 +312,6 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
 }
 
 namespace {
-constexpr int EVICT_MIN_TILE = 4;
 int64_t evict_up(int64_t x) { return (x + 255) & ~int64_t{255}; }
 }  // namespace
 
@@ -293,7 +322,7 @@ size_t evict_workspace(int64_t B, int64_t H, int64_t cap) {
 
 cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   if (p.B * p.H == 0 || p.cap == 0) return cudaSuccess;
-  // tiles of up to 128 entries and 48 KB of rows
+  // tiles of up to 128 entries and 80 KB of rows
   int bytes = 0;
   for (int r = 0; r < p.n_rows; ++r) bytes += p.bytes[r];
   p.tile = 128;
@@ -305,18 +334,20 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   p.before = reinterpret_cast<uint2*>(ws + 256 + evict_up(heads * 16));
   p.loaded = reinterpret_cast<uint32_t*>(ws + 256 + evict_up(heads * 16) + evict_up(heads * p.max_tiles * 8));
   int C = 1;  // 4096 entries a CTA keep a pass near its latency
-  while (C < 8 && p.cap > C * 4096) C <<= 1;
-  const int sel_smem = (SEL_KEYS + 3 * SEL_BINS) * 4;
+  while (C < SEL_MAX_CTAS && p.cap > C * 4096) C <<= 1;
   int move_smem = p.tile * 8;
-  for (int r = 0; r < p.n_rows; ++r) move_smem += (p.tile * p.bytes[r] + 15) & ~15;
-  cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, sel_smem);
-  if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, move_smem);
+  for (int r = 0; r < p.n_rows; ++r) {
+    const int upr = p.bytes[r] / p.unit[r];
+    p.shift[r] = (upr & (upr - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(upr)) : -1;
+    move_smem += (p.tile * p.bytes[r] + 15) & ~15;
+  }
+  cudaError_t e = cudaSuccess;
+  if (move_smem > 48 * 1024)
+    e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, move_smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(C), static_cast<unsigned>(heads));
   cfg.blockDim = dim3(SEL_THREADS);
-  cfg.dynamicSmemBytes = static_cast<size_t>(sel_smem);
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -326,8 +357,12 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
   if (e != cudaSuccess) return e;
-  evict_move_kernel<<<dim3(static_cast<unsigned>(p.max_tiles), static_cast<unsigned>(heads)), MOVE_THREADS, move_smem, st>>>(p);
-  return cudaGetLastError();
+  cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles), static_cast<unsigned>(heads));
+  cfg.blockDim = dim3(MOVE_THREADS);
+  cfg.dynamicSmemBytes = static_cast<size_t>(move_smem);
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  return cudaLaunchKernelEx(&cfg, evict_move_kernel, p);
 }
 
 }  // namespace dab

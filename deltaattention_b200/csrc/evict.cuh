@@ -4,7 +4,7 @@
 
 namespace dab {
 
-constexpr int EVICT_MAX_ROWS = 8;
+constexpr int EVICT_MAX_ROWS = 8, EVICT_MIN_TILE = 4;
 constexpr int EVICT_MAX_BYTES = 8192;  // of an entry's rows together
 
 struct EvictParams {
@@ -14,7 +14,7 @@ struct EvictParams {
   // and the widest unit (4, 8 or 16 bytes) that its base, strides and rows are multiples of
   uint8_t* row[EVICT_MAX_ROWS];
   int64_t rb[EVICT_MAX_ROWS], rh[EVICT_MAX_ROWS];
-  int bytes[EVICT_MAX_ROWS], unit[EVICT_MAX_ROWS];
+  int bytes[EVICT_MAX_ROWS], unit[EVICT_MAX_ROWS], shift[EVICT_MAX_ROWS];  // log2(units a row), or -1
   int n_rows;
   int B, H, cap;
   int budget, trigger, first, recent;
