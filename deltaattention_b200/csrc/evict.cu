@@ -5,11 +5,12 @@
 // Entries keep their order, and every row buffer is compacted in place with the mass.
 //
 //  * evict_select: one cluster per head finds the k-th largest weight of the middle entries by
-//    radix selection, 8 bits a pass. Every CTA keeps the keys of its slice in registers, 16 a
-//    thread, and counts a pass's digits in shared memory; the counts are summed through distributed
-//    shared memory. Then it writes for every tile how many entries are kept before it and how many
-//    of the ties come before it. (Digits of 11 bits need a pass less, but 8 CTAs summing 2048 counts
-//    from each other took 5000 cycles a pass, 256 take a tenth.)
+//    radix selection, digits of 11, 11 and 10 bits. Every CTA keeps the keys of its slice in
+//    registers, 16 a thread, and counts a pass's digits in shared memory. The counts are summed
+//    over the cluster in two steps, 256 sums of 8 bins and then the 8 bins of the one where the
+//    count reaches k (8 CTAs reading all 2048 bins from each other took 5000 cycles a pass). Then
+//    it writes for every tile how many entries are kept before it and how many of the ties come
+//    before it.
 //  * evict_move: one CTA per tile reads its kept rows into shared memory, says so, waits for the
 //    (at most two) tiles on whose rows its own will land to have said so too, and writes. Tiles are
 //    handed out in order by a ticket per head and nothing is waited for before a tile has read
@@ -25,6 +26,7 @@ namespace cg = cooperative_groups;
 
 constexpr int SEL_THREADS = 1024, SEL_MAX_CTAS = 8;  // of a cluster
 constexpr int SEL_KEYS = 16;                         // a thread's keys in registers; longer slices are read again
+constexpr int SEL_BINS = 2048;
 constexpr int SEL_CHUNK = SEL_THREADS * SEL_KEYS;
 constexpr int MOVE_THREADS = 128;
 enum { ERR_EVICT_WAIT = 0x501 };
@@ -41,9 +43,10 @@ __device__ __forceinline__ void grid_next() { asm volatile("griddepcontrol.launc
 
 __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
   cg::cluster_group cl = cg::this_cluster();
-  __shared__ uint32_t hist[4][256];
+  __shared__ __align__(16) uint32_t hist[3][SEL_BINS];
+  __shared__ uint32_t coarse[3][256];
   __shared__ uint2 cnt[SEL_CHUNK / EVICT_MIN_TILE];  // of a chunk's tiles: surely kept, ties
-  __shared__ uint32_t wsum[8], s_prefix, s_k, s_tot[2];
+  __shared__ uint32_t wsum[8], s_bin, s_prefix, s_k, s_tot[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
@@ -70,36 +73,47 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
   };
   load(i0);
   const bool one = i1 - i0 <= SEL_CHUNK;
-  (&hist[0][0])[tid] = 0;
+  for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) (&hist[0][0])[i] = 0;
   for (int t = t0 + tid; t < t1; t += SEL_THREADS) p.loaded[static_cast<int64_t>(bh) * p.max_tiles + t] = 0u;
   uint32_t k = p.budget - p.first - p.recent, prefix = k ? 0u : 0xFFFFFFFFu;
   __syncthreads();
   if (k) {
 #pragma unroll 1
-    for (int pass = 0; pass < 4; ++pass) {
-      const int shift = 24 - 8 * pass;
-      const uint32_t above = pass == 0 ? 0u : 0xFFFFFFFFu << (shift + 8);
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t above = pass == 0 ? 0u : pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
+      const uint32_t digits = pass == 2 ? 1023u : 2047u;
+      uint32_t* hp = hist[pass];
       uint32_t zeros = 0;  // many weights may be 0: one addition a warp
       for (int base = i0; base < i1; base += SEL_CHUNK) {
         if (!one) load(base);
 #pragma unroll
         for (int j = 0; j < SEL_KEYS; ++j) {
           const int e = base + j * SEL_THREADS + tid;
+          if (base + j * SEL_THREADS >= i1) break;
           if (e >= lo && e < hi && e < i1 && (key[j] & above) == prefix) {
             if (key[j] == KEY_ZERO) ++zeros;
-            else atomicAdd(&hist[pass][(key[j] >> shift) & 255u], 1u);
+            else atomicAdd(&hp[(key[j] >> shift) & digits], 1u);
           }
         }
       }
       zeros = __reduce_add_sync(0xFFFFFFFFu, zeros);
-      if (lane == 0 && zeros) atomicAdd(&hist[pass][(KEY_ZERO >> shift) & 255u], zeros);
-      cl.sync();
-      // thread i sums bin 255 - i over the cluster; the digit is where the count from the top reaches k
+      if (lane == 0 && zeros) atomicAdd(&hp[(KEY_ZERO >> shift) & digits], zeros);
+      __syncthreads();
+      if (tid < 256) {
+        const uint4 x = reinterpret_cast<const uint4*>(hp)[2 * tid], y = reinterpret_cast<const uint4*>(hp)[2 * tid + 1];
+        coarse[pass][tid] = (x.x + x.y) + (x.z + x.w) + (y.x + y.y) + (y.z + y.w);
+      }
+      if (C > 1) cl.sync();
+      else __syncthreads();
+      // thread i: sum 255 - i over the cluster; the digit is where the count from the top reaches k
       uint32_t c = 0, incl = 0;
       if (tid < 256) {
+        if (C == 1) c = coarse[pass][255 - tid];
+        else
 #pragma unroll
-        for (int r = 0; r < SEL_MAX_CTAS; ++r)
-          if (r < C) c += cl.map_shared_rank(&hist[pass][0], r)[255 - tid];
+          for (int r = 0; r < SEL_MAX_CTAS; ++r)
+            if (r < C) c += cl.map_shared_rank(&coarse[pass][0], r)[255 - tid];
         incl = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -115,8 +129,30 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
         for (int w = 0; w < 7; ++w)
           if (w < warp) before += wsum[w];
         if (before < k && k <= before + c) {
-          s_prefix = prefix | (static_cast<uint32_t>(255 - tid) << shift);
+          s_bin = 255 - tid;
           s_k = k - before;
+        }
+      }
+      __syncthreads();
+      if (warp == 0) {  // lane i: bin 7 - i of the eight
+        const uint32_t bin = 8 * s_bin + 7 - (lane & 7);
+        c = 0;
+        if (C == 1) c = hp[bin];
+        else
+#pragma unroll
+          for (int r = 0; r < SEL_MAX_CTAS; ++r)
+            if (r < C) c += cl.map_shared_rank(hp, r)[bin];
+        incl = c;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) {
+          const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, incl, o, 8);
+          if ((lane & 7) >= o) incl += v;
+        }
+        const uint32_t want = s_k;
+        __syncwarp();
+        if (lane < 8 && incl - c < want && want <= incl) {
+          s_prefix = prefix | (bin << shift);
+          s_k = want - (incl - c);
         }
       }
       __syncthreads();
@@ -137,6 +173,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
 #pragma unroll
     for (int j = 0; j < SEL_KEYS; ++j) {
       const int o = j * SEL_THREADS + tid, e = base + o;
+      if (base + j * SEL_THREADS >= i1) break;
       const bool mid = e >= lo && e < hi;
       const uint32_t sb = __ballot_sync(0xFFFFFFFFu, e < i1 && (!mid || key[j] > prefix));
       const uint32_t tb = __ballot_sync(0xFFFFFFFFu, e < i1 && mid && key[j] == prefix);
@@ -169,7 +206,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
     s_tot[0] = run_s;
     s_tot[1] = run_t;
   }
-  cl.sync();
+  if (C > 1) cl.sync();
   uint32_t base_s = 0, base_t = 0;
 #pragma unroll
   for (int r = 0; r < SEL_MAX_CTAS - 1; ++r) {
@@ -188,7 +225,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
     *len = p.budget;  // every CTA of the cluster has read it
   }
   grid_next();
-  cl.sync();  // no CTA leaves while its counts are read
+  if (C > 1) cl.sync();  // no CTA leaves while its counts are read
 }
 
 // Kernels launched after one another with programmatic dependent launch
@@ -333,8 +370,9 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   p.cut = reinterpret_cast<uint4*>(ws + 256);
   p.before = reinterpret_cast<uint2*>(ws + 256 + evict_up(heads * 16));
   p.loaded = reinterpret_cast<uint32_t*>(ws + 256 + evict_up(heads * 16) + evict_up(heads * p.max_tiles * 8));
-  int C = 1;  // 4096 entries a CTA keep a pass near its latency
-  while (C < SEL_MAX_CTAS && p.cap > C * 4096) C <<= 1;
+  // 4096 entries a CTA keep a pass near its latency, as long as all CTAs run at once (one an SM)
+  int C = 1;
+  while (C < SEL_MAX_CTAS && p.cap > C * 4096 && heads * C * 2 <= 148) C <<= 1;
   int move_smem = p.tile * 8;
   for (int r = 0; r < p.n_rows; ++r) {
     const int upr = p.bytes[r] / p.unit[r];

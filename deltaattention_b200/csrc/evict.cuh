@@ -4,7 +4,7 @@
 
 namespace dab {
 
-constexpr int EVICT_MAX_ROWS = 8, EVICT_MIN_TILE = 4;
+constexpr int EVICT_MAX_ROWS = 8, EVICT_MIN_TILE = 16;
 constexpr int EVICT_MAX_BYTES = 8192;  // of an entry's rows together
 
 struct EvictParams {
