@@ -45,8 +45,10 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
   cg::cluster_group cl = cg::this_cluster();
   __shared__ __align__(16) uint32_t hist[3][SEL_BINS];
   __shared__ uint32_t coarse[3][256];
-  __shared__ uint2 cnt[SEL_CHUNK / EVICT_MIN_TILE];  // of a chunk's tiles: surely kept, ties
-  __shared__ uint32_t wsum[8], s_bin, s_prefix, s_k, s_tot[2];
+  __shared__ uint32_t cnt[SEL_CHUNK / 32];  // of a chunk's 32 entries each: surely kept, ties << 16
+  __shared__ uint32_t wsum[8], s_bin, s_prefix, s_k;
+  __shared__ __align__(8) uint32_t s_tot[2];
+  __shared__ uint2 wcnt[SEL_CHUNK / 1024];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
@@ -68,8 +70,10 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
 #pragma unroll
     for (int j = 0; j < SEL_KEYS; ++j) {
       const int e = base + j * SEL_THREADS + tid;
-      key[j] = e < i1 ? mass_key(mass[e]) : 0u;
+      key[j] = __float_as_uint(mass[min(e, i1 - 1)]);  // all loads in flight
     }
+#pragma unroll
+    for (int j = 0; j < SEL_KEYS; ++j) key[j] = mass_key(__uint_as_float(key[j]));
   };
   load(i0);
   const bool one = i1 - i0 <= SEL_CHUNK;
@@ -112,8 +116,10 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
         if (C == 1) c = coarse[pass][255 - tid];
         else
 #pragma unroll
-          for (int r = 0; r < SEL_MAX_CTAS; ++r)
-            if (r < C) c += cl.map_shared_rank(&coarse[pass][0], r)[255 - tid];
+          for (int r = 0; r < SEL_MAX_CTAS; ++r) {  // all loads in flight
+            const uint32_t v = cl.map_shared_rank(&coarse[pass][0], min(r, C - 1))[255 - tid];
+            c += r < C ? v : 0u;
+          }
         incl = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -140,8 +146,10 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
         if (C == 1) c = hp[bin];
         else
 #pragma unroll
-          for (int r = 0; r < SEL_MAX_CTAS; ++r)
-            if (r < C) c += cl.map_shared_rank(hp, r)[bin];
+          for (int r = 0; r < SEL_MAX_CTAS; ++r) {
+            const uint32_t v = cl.map_shared_rank(hp, min(r, C - 1))[bin];
+            c += r < C ? v : 0u;
+          }
         incl = c;
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) {
@@ -162,58 +170,55 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
   }
   // per tile: entries surely kept, and ties
   uint2* before = p.before + static_cast<int64_t>(bh) * p.max_tiles;
-  const int seg = min(p.tile, 32);  // neighbouring lanes of a tile
-  const uint32_t seg_mask = seg == 32 ? 0xFFFFFFFFu : (1u << seg) - 1u;
-  uint32_t run_s = 0, run_t = 0;    // of this CTA's tiles so far (warp 0)
+  uint32_t run_s = 0, run_t = 0;  // of this CTA's entries so far
   for (int base = i0; base < i1; base += SEL_CHUNK) {
     if (!one) load(base);
-    const int ct = (min(i1, base + SEL_CHUNK) - base + p.tile - 1) / p.tile;  // tiles of the chunk
-    for (int t = tid; t < ct; t += SEL_THREADS) cnt[t] = make_uint2(0u, 0u);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < SEL_KEYS; ++j) {
-      const int o = j * SEL_THREADS + tid, e = base + o;
-      if (base + j * SEL_THREADS >= i1) break;
+      const int e = base + j * SEL_THREADS + tid;
       const bool mid = e >= lo && e < hi;
       const uint32_t sb = __ballot_sync(0xFFFFFFFFu, e < i1 && (!mid || key[j] > prefix));
       const uint32_t tb = __ballot_sync(0xFFFFFFFFu, e < i1 && mid && key[j] == prefix);
-      if (lane % seg == 0 && e < i1) {
-        const uint32_t s = __popc((sb >> lane) & seg_mask), q = __popc((tb >> lane) & seg_mask);
-        if (s) atomicAdd(&cnt[o / p.tile].x, s);
-        if (q) atomicAdd(&cnt[o / p.tile].y, q);
-      }
+      if (lane == 0) cnt[j * (SEL_THREADS / 32) + warp] = __popc(sb) | __popc(tb) << 16;
     }
     __syncthreads();
-    if (warp == 0) {  // exclusive sums
-      const int tb = t0 + (base - i0) / p.tile;
-      for (int t = 0; t < ct; t += 32) {
-        uint2 v = make_uint2(0u, 0u);
-        if (t + lane < ct) v = cnt[t + lane];
-        uint32_t a = v.x, q = v.y;
+    uint2 v = make_uint2(0u, 0u), x = v;  // exclusive sums: thread i, entries [32 i, 32 i + 32) of the chunk
+    if (tid < SEL_CHUNK / 32) {
+      v = x = make_uint2(cnt[tid] & 0xFFFFu, cnt[tid] >> 16);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t x = __shfl_up_sync(0xFFFFFFFFu, a, o), y = __shfl_up_sync(0xFFFFFFFFu, q, o);
-          if (lane >= o) { a += x; q += y; }
-        }
-        if (t + lane < ct) before[tb + t + lane] = make_uint2(run_s + a - v.x, run_t + q - v.y);
-        run_s += __shfl_sync(0xFFFFFFFFu, a, 31);
-        run_t += __shfl_sync(0xFFFFFFFFu, q, 31);
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t a = __shfl_up_sync(0xFFFFFFFFu, x.x, o), q = __shfl_up_sync(0xFFFFFFFFu, x.y, o);
+        if (lane >= o) { x.x += a; x.y += q; }
       }
+      if (lane == 31) wcnt[warp] = x;
     }
     __syncthreads();
+    uint32_t add_s = run_s, add_t = run_t;
+#pragma unroll
+    for (int w = 0; w < SEL_CHUNK / 1024; ++w) {
+      const uint2 y = wcnt[w];
+      if (w < warp) { add_s += y.x; add_t += y.y; }
+      run_s += y.x;
+      run_t += y.y;
+    }
+    const int o = tid * 32;
+    if (tid < SEL_CHUNK / 32 && (o & (p.tile - 1)) == 0 && base + o < i1)
+      before[(base + o) >> p.tile_shift] = make_uint2(add_s + x.x - v.x, add_t + x.y - v.y);
   }
   if (tid == 0) {
     s_tot[0] = run_s;
     s_tot[1] = run_t;
   }
+  __syncthreads();
   if (C > 1) cl.sync();
   uint32_t base_s = 0, base_t = 0;
+  if (C > 1) {
 #pragma unroll
-  for (int r = 0; r < SEL_MAX_CTAS - 1; ++r) {
-    if (r >= rank) continue;
-    const uint32_t* o = cl.map_shared_rank(s_tot, r);
-    base_s += o[0];
-    base_t += o[1];
+    for (int r = 0; r < SEL_MAX_CTAS - 1; ++r) {
+      const uint2 v = *reinterpret_cast<const uint2*>(cl.map_shared_rank(s_tot, min(r, C - 1)));
+      if (r < rank) { base_s += v.x; base_t += v.y; }
+    }
   }
   for (int t = t0 + tid; t < t1; t += SEL_THREADS) {
     const uint2 v = before[t];
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
   }
   if (still || !kept) return;
   if (tid < 2) {  // rows land on one tile, or two
-    const int on = (tid == 0 ? dst0 : dst0 + kept - 1) / p.tile;
+    const int on = (tid == 0 ? dst0 : dst0 + kept - 1) >> p.tile_shift;
     uint32_t v = 1u;
     if (on != tile) {
       const uint64_t began = globaltimer();
@@ -365,6 +370,7 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   p.tile = 128;
   while (p.tile > EVICT_MIN_TILE && p.tile * bytes > 80 * 1024) p.tile >>= 1;
   p.max_tiles = (p.cap + p.tile - 1) / p.tile;
+  p.tile_shift = __builtin_ctz(static_cast<unsigned>(p.tile));
   const int64_t heads = static_cast<int64_t>(p.B) * p.H;
   p.err = reinterpret_cast<int*>(ws);
   p.cut = reinterpret_cast<uint4*>(ws + 256);

@@ -4,8 +4,8 @@
 
 namespace dab {
 
-constexpr int EVICT_MAX_ROWS = 8, EVICT_MIN_TILE = 16;
-constexpr int EVICT_MAX_BYTES = 8192;  // of an entry's rows together
+constexpr int EVICT_MAX_ROWS = 8, EVICT_MIN_TILE = 32;
+constexpr int EVICT_MAX_BYTES = 4096;  // of an entry's rows together
 
 struct EvictParams {
   float* mass; int64_t mb, mh;           // [B, H, cap], strides in elements
@@ -18,7 +18,7 @@ struct EvictParams {
   int n_rows;
   int B, H, cap;
   int budget, trigger, first, recent;
-  int tile, max_tiles;                   // entries per moved tile, tiles of a full head
+  int tile, tile_shift, max_tiles;       // entries per moved tile (a power of two), tiles of a full head
   // workspace: error word; per head (threshold key, ties kept, length or 0 if left alone, ticket);
   // per head and tile (kept before it, ties before it) and whether its rows have been read
   int* err;

@@ -885,7 +885,7 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
     them: the first ``keep_first``, the last ``keep_recent`` and, of those between, the ones with
     the largest ``mass`` [B, H, capacity] (fp32; ties go to the lowest index, NaN is the lightest).
     Entries keep their order; mass and every tensor of ``rows`` ([B, H, capacity, ...], up to 8,
-    contiguous from the third dimension on, entries of a multiple of 4 bytes, 8192 bytes together)
+    contiguous from the third dimension on, entries of a multiple of 4 bytes, 4096 bytes together)
     move together, and
     ``lengths`` [B, H] (int32) become ``budget``. Slots from ``budget`` on keep what they held.
     Lengths are read on the device: no host synchronisation, and the call can be captured in a
