@@ -981,8 +981,8 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
                       int64_t keep_first, int64_t keep_recent, void* workspace, size_t workspace_bytes, void* stream) {
   const char* nm = "dab_evict_by_mass";
   if (!mass || !lengths || !mass_strides || !length_strides) return fail(1, std::string(nm) + ": null pointer");
-  if (num_rows < 0 || num_rows > EVICT_MAX_ROWS)
-    return fail(1, std::string(nm) + ": at most " + std::to_string(EVICT_MAX_ROWS) + " row buffers");
+  if (num_rows < 0 || num_rows > EVICT_MAX_ROWS - 1)
+    return fail(1, std::string(nm) + ": at most " + std::to_string(EVICT_MAX_ROWS - 1) + " row buffers");
   if (num_rows > 0 && (!rows || !row_bytes || !row_strides)) return fail(1, std::string(nm) + ": null pointer");
   if (batch < 0 || heads < 0 || batch * heads > 65535 || capacity < 0 || capacity >= (int64_t{1} << 30))
     return fail(1, std::string(nm) + ": need batch * heads <= 65535 and capacity below 2^30");
@@ -1011,7 +1011,12 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
   if (budget >= capacity) return 0;  // no head can be longer
   p.mass = mass; p.mb = mass_strides[0]; p.mh = mass_strides[1];
   p.lengths = lengths; p.lb = length_strides[0]; p.lh = length_strides[1];
-  p.n_rows = static_cast<int>(num_rows);
+  // the mass moves as a buffer of 4-byte rows
+  const int64_t last = num_rows;
+  p.row[last] = reinterpret_cast<uint8_t*>(mass);
+  p.rb[last] = 4 * p.mb; p.rh[last] = 4 * p.mh;
+  p.bytes[last] = p.unit[last] = 4;
+  p.n_rows = static_cast<int>(num_rows) + 1;
   p.B = static_cast<int>(batch); p.H = static_cast<int>(heads); p.cap = static_cast<int>(capacity);
   p.budget = static_cast<int>(budget);
   p.trigger = static_cast<int>(trigger < capacity ? trigger : capacity);

@@ -9,13 +9,18 @@
 //    registers, 16 a thread, and counts a pass's digits in shared memory. The counts are summed
 //    over the cluster in two steps, 256 sums of 8 bins and then the 8 bins of the one where the
 //    count reaches k (8 CTAs reading all 2048 bins from each other took 5000 cycles a pass). Then
-//    it writes for every tile how many entries are kept before it and how many of the ties come
-//    before it.
-//  * evict_move: one CTA per tile reads its kept rows into shared memory, says so, waits for the
-//    (at most two) tiles on whose rows its own will land to have said so too, and writes. Tiles are
-//    handed out in order by a ticket per head and nothing is waited for before a tile has read
-//    its rows, so the tiles waited for are running and never wait themselves. Every kept row is
-//    read and written once, with no second buffer.
+//    it writes which entries are kept for sure and which are ties, how many of both come before
+//    every tile, and in which tile the entries of every tile of the result begin.
+//  * evict_move: one CTA per tile of the result gathers its rows into shared memory, says so, waits
+//    for the (at most two) tiles of the result that come from the entries it is about to overwrite
+//    to have said so too, and writes. Tiles are handed out in order by a ticket per head, an entry
+//    never moves back, and nothing is waited for before a tile's rows have been read: the tiles
+//    waited for have smaller tickets, so they are running and never wait for this one. Every kept
+//    row is read and written once, with no second buffer. The chain of dependent reads of a tile
+//    (ticket, place, entries, rows, flag) takes about 7 us, so what counts is how many kept rows the
+//    tiles in an SM's shared memory hold: tiles of the result hold nothing else. 8 heads of 131072
+//    16-bit entries cut to half take 98 us, 5.6 TB/s; tiles of the source, half of them evicted, took
+//    130 us.
 #include <cooperative_groups.h>
 
 #include "evict.cuh"
@@ -78,7 +83,9 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
   load(i0);
   const bool one = i1 - i0 <= SEL_CHUNK;
   for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) (&hist[0][0])[i] = 0;
-  for (int t = t0 + tid; t < t1; t += SEL_THREADS) p.loaded[static_cast<int64_t>(bh) * p.max_tiles + t] = 0u;
+  const int out_tiles = (p.budget + p.tile - 1) >> p.tile_shift;
+  for (int t = rank * SEL_THREADS + tid; t < out_tiles; t += C * SEL_THREADS)
+    p.loaded[static_cast<int64_t>(bh) * p.max_tiles + t] = 0u;
   uint32_t k = p.budget - p.first - p.recent, prefix = k ? 0u : 0xFFFFFFFFu;
   __syncthreads();
   if (k) {
@@ -180,7 +187,10 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
       const bool mid = e >= lo && e < hi;
       const uint32_t sb = __ballot_sync(0xFFFFFFFFu, e < i1 && (!mid || key[j] > prefix));
       const uint32_t tb = __ballot_sync(0xFFFFFFFFu, e < i1 && mid && key[j] == prefix);
-      if (lane == 0) cnt[j * (SEL_THREADS / 32) + warp] = __popc(sb) | __popc(tb) << 16;
+      if (lane == 0) {
+        cnt[j * (SEL_THREADS / 32) + warp] = __popc(sb) | __popc(tb) << 16;
+        if (e < i1) p.words[static_cast<int64_t>(bh) * p.max_words + (e >> 5)] = make_uint2(sb, tb);
+      }
     }
     __syncthreads();
     uint2 v = make_uint2(0u, 0u), x = v;  // exclusive sums: thread i, entries [32 i, 32 i + 32) of the chunk
@@ -220,10 +230,19 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
       if (r < rank) { base_s += v.x; base_t += v.y; }
     }
   }
-  for (int t = t0 + tid; t < t1; t += SEL_THREADS) {
-    const uint2 v = before[t];
-    const uint32_t ties = base_t + v.y;
-    before[t] = make_uint2(base_s + v.x + min(ties, k), ties);
+  int* first = p.first_tile + static_cast<int64_t>(bh) * p.max_tiles;
+  for (int t = t0; t < t1; t += SEL_THREADS) {  // kept and ties before every tile; where result tiles begin
+    const int u = t + tid;
+    uint2 v = make_uint2(0u, 0u), w = make_uint2(run_s, run_t);
+    if (u < t1) v = before[u];
+    if (u + 1 < t1) w = before[u + 1];
+    __syncthreads();
+    if (u < t1) {
+      const uint32_t at = base_s + v.x + min(base_t + v.y, k), end = base_s + w.x + min(base_t + w.y, k);
+      before[u] = make_uint2(at, base_t + v.y);
+      for (uint32_t d = (at + p.tile - 1) >> p.tile_shift; (d << p.tile_shift) < end; ++d) first[d] = u;
+    }
+    __syncthreads();
   }
   if (rank == 0 && tid == 0) {
     p.cut[bh] = make_uint4(prefix, k, static_cast<uint32_t>(n), 0u);
@@ -251,61 +270,79 @@ __device__ __forceinline__ void move_rows(uint32_t dst, const uint8_t* base, int
 }
 
 __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictParams p) {
-  extern __shared__ __align__(16) uint8_t mv_smem[];  // src[tile] and mass[tile], then the rows of each buffer
-  __shared__ int w_tie[MOVE_THREADS / 32], w_keep[MOVE_THREADS / 32], s_tile;
+  extern __shared__ __align__(16) uint8_t mv_smem[];  // src[tile], then the rows of mass and each buffer
+  __shared__ uint2 wsum[MOVE_THREADS / 32];
+  __shared__ int s_tile, s_ok[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   grid_wait();
-  const int n = static_cast<int>(p.cut[bh].z);
-  if (n == 0 || static_cast<int>(blockIdx.x) * p.tile >= n) return;
   if (tid == 0) s_tile = static_cast<int>(atomicAdd(&p.cut[bh].w, 1u));
-  const uint32_t thr = p.cut[bh].x;
-  const int need = static_cast<int>(p.cut[bh].y);
+  const uint32_t need = p.cut[bh].y;
+  const int n = static_cast<int>(p.cut[bh].z);
   __syncthreads();
-  const int tile = s_tile, i0 = tile * p.tile;
-  const uint2 bf = p.before[static_cast<int64_t>(bh) * p.max_tiles + tile];
-  const int dst0 = static_cast<int>(bf.x);
+  if (n == 0) return;  // left alone
+  const int tile = s_tile, d0 = tile << p.tile_shift, rows_n = min(p.tile, p.budget - d0);
+  const uint2* before = p.before + static_cast<int64_t>(bh) * p.max_tiles;
+  const int from = p.first_tile[static_cast<int64_t>(bh) * p.max_tiles + tile];
+  // the tiles of the result that come from the entries this one overwrites: from the `on`th to `upto`
+  const int on = static_cast<int>(before[tile].x) >> p.tile_shift;
+  const int next = tile + 1 < (n + p.tile - 1) >> p.tile_shift ? static_cast<int>(before[tile + 1].x) : p.budget;
+  const int upto = max(static_cast<int>(before[tile].x), next - 1) >> p.tile_shift;
+  // the kept entries d0, d0 + 1, .. of the result, 32 source entries a thread
   int* src = reinterpret_cast<int*>(mv_smem);
-  float* kept_mass = reinterpret_cast<float*>(src + p.tile);
-  uint8_t* rows = reinterpret_cast<uint8_t*>(kept_mass + p.tile);
-  float* mass = p.mass + b * p.mb + h * p.mh;
-  // which entries stay, and where they go (tiles have at most MOVE_THREADS entries)
-  const int i = i0 + tid;
-  const bool live = tid < p.tile && i < n;
-  const float m = live ? mass[i] : 0.f;
-  const bool mid = i >= p.first && i < n - p.recent;
-  const uint32_t key = mass_key(m), below = (1u << lane) - 1u;
-  const bool tie = live && mid && key == thr;
-  bool keep = live && (!mid || key > thr);
-  const uint32_t tb = __ballot_sync(0xFFFFFFFFu, tie);
-  if (lane == 0) w_tie[warp] = __popc(tb);
-  __syncthreads();
-  int ties = static_cast<int>(bf.y) + __popc(tb & below);
-  for (int w = 0; w < warp; ++w) ties += w_tie[w];
-  keep = keep || (tie && ties < need);
-  const uint32_t kb = __ballot_sync(0xFFFFFFFFu, keep);
-  if (lane == 0) w_keep[warp] = __popc(kb);
-  __syncthreads();
-  int pos = __popc(kb & below), kept = 0;
-  for (int w = 0; w < MOVE_THREADS / 32; ++w) {
-    if (w < warp) pos += w_keep[w];
-    kept += w_keep[w];
+  uint2 at = before[from];
+  const uint2* words = p.words + static_cast<int64_t>(bh) * p.max_words;
+  const int nw = (n + 31) / 32;
+  for (int w0 = (from << p.tile_shift) / 32; static_cast<int>(at.x) < d0 + rows_n && w0 < nw; w0 += MOVE_THREADS) {
+    uint2 w = make_uint2(0u, 0u);
+    if (w0 + tid < nw) w = words[w0 + tid];
+    uint2 x = make_uint2(__popc(w.x), __popc(w.y));
+    const uint2 own = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t s = __shfl_up_sync(0xFFFFFFFFu, x.x, o), q = __shfl_up_sync(0xFFFFFFFFu, x.y, o);
+      if (lane >= o) { x.x += s; x.y += q; }
+    }
+    __syncthreads();
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    uint2 pre = make_uint2(x.x - own.x, x.y - own.y), all = make_uint2(0u, 0u);
+#pragma unroll
+    for (int v = 0; v < MOVE_THREADS / 32; ++v) {
+      const uint2 y = wsum[v];
+      if (v < warp) { pre.x += y.x; pre.y += y.y; }
+      all.x += y.x;
+      all.y += y.y;
+    }
+    // ties kept before this thread's, and of its own the lowest
+    const uint32_t t0 = at.y + pre.y, t_all = min(t0, need) - min(at.y, need);
+    const uint32_t mine = min(t0 + own.y, need) - min(t0, need);
+    uint32_t bits = w.x | (mine == own.y ? w.y : mine == 0 ? 0u : w.y & ((1u << __fns(w.y, 0, mine + 1)) - 1u));
+    // `at` counts kept entries of both kinds before the first word
+    int pos = static_cast<int>(at.x + pre.x + t_all) - d0;
+    // a warp writes out its words one after another, a lane a bit
+#pragma unroll 1
+    for (uint32_t some = __ballot_sync(0xFFFFFFFFu, bits && pos < rows_n && pos + __popc(bits) > 0); some; some &= some - 1) {
+      const int l = __ffs(some) - 1;
+      const uint32_t wb = __shfl_sync(0xFFFFFFFFu, bits, l);
+      const int wp = __shfl_sync(0xFFFFFFFFu, pos, l) + __popc(wb & ((1u << lane) - 1u));
+      if ((wb >> lane & 1u) && wp >= 0 && wp < rows_n) src[wp] = (w0 + warp * 32 + l) * 32 + lane;
+    }
+    at.x += all.x + min(at.y + all.y, need) - min(at.y, need);
+    at.y += all.y;
   }
-  const bool still = dst0 == i0 && kept == min(p.tile, n - i0);  // nothing before or in the tile goes
-  if (keep && !still) {
-    src[pos] = i;
-    kept_mass[pos] = m;
-  }
   __syncthreads();
-  if (!still && kept) {
-    uint8_t* at = rows;
+  const bool still = src[0] == d0 && src[rows_n - 1] == d0 + rows_n - 1;  // nothing moves
+  uint8_t* rows = mv_smem + p.tile * 4;
+  if (!still) {
+    uint8_t* to = rows;
     for (int r = 0; r < p.n_rows; ++r) {
       const uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r];
-      const uint32_t dst = smem_u32(at);
-      if (p.unit[r] == 16) move_rows<16>(dst, base, p.bytes[r], p.shift[r], src, kept);
-      else if (p.unit[r] == 8) move_rows<8>(dst, base, p.bytes[r], p.shift[r], src, kept);
-      else move_rows<4>(dst, base, p.bytes[r], p.shift[r], src, kept);
-      at += (p.tile * p.bytes[r] + 15) & ~15;
+      const uint32_t dst = smem_u32(to);
+      if (p.unit[r] == 16) move_rows<16>(dst, base, p.bytes[r], p.shift[r], src, rows_n);
+      else if (p.unit[r] == 8) move_rows<8>(dst, base, p.bytes[r], p.shift[r], src, rows_n);
+      else move_rows<4>(dst, base, p.bytes[r], p.shift[r], src, rows_n);
+      to += (p.tile * p.bytes[r] + 15) & ~15;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
@@ -315,14 +352,14 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
     // this tile's rows have been read (the barrier comes after everybody's copies): others may land on them
     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(loaded + tile), "r"(1u) : "memory");
   }
-  if (still || !kept) return;
-  if (tid < 2) {  // rows land on one tile, or two
-    const int on = (tid == 0 ? dst0 : dst0 + kept - 1) >> p.tile_shift;
+  if (still) return;
+  if (tid < 2) {
+    const int wait = tid == 0 ? on : upto;
     uint32_t v = 1u;
-    if (on != tile) {
+    if (wait != tile) {
       const uint64_t began = globaltimer();
       while (true) {
-        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(loaded + on) : "memory");
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(loaded + wait) : "memory");
         if (v) break;
         if (globaltimer() - began > DAB_WAIT_TIMEOUT_NS) {
           atomicCAS(p.err, 0, static_cast<int>(ERR_EVICT_WAIT));
@@ -330,27 +367,27 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
         }
       }
     }
-    w_keep[tid] = static_cast<int>(v);
+    s_ok[tid] = static_cast<int>(v);
   }
   __syncthreads();
-  if (!w_keep[0] || !w_keep[1]) return;  // timed out: the error word says that the cache is not valid
-  uint8_t* at = rows;
+  if (!s_ok[0] || !s_ok[1]) return;  // timed out: the error word says that the cache is not valid
+  const uint8_t* out = rows;
   for (int r = 0; r < p.n_rows; ++r) {
-    uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r] + static_cast<int64_t>(dst0) * p.bytes[r];
-    const int total = kept * p.bytes[r];
+    uint8_t* base = p.row[r] + b * p.rb[r] + h * p.rh[r] + static_cast<int64_t>(d0) * p.bytes[r];
+    const int total = rows_n * p.bytes[r];
     if (p.unit[r] == 16) {
+#pragma unroll 4
       for (int u = tid * 16; u < total; u += MOVE_THREADS * 16)
-        *reinterpret_cast<uint4*>(base + u) = *reinterpret_cast<const uint4*>(at + u);
+        *reinterpret_cast<uint4*>(base + u) = *reinterpret_cast<const uint4*>(out + u);
     } else if (p.unit[r] == 8) {
       for (int u = tid * 8; u < total; u += MOVE_THREADS * 8)
-        *reinterpret_cast<uint2*>(base + u) = *reinterpret_cast<const uint2*>(at + u);
+        *reinterpret_cast<uint2*>(base + u) = *reinterpret_cast<const uint2*>(out + u);
     } else {
       for (int u = tid * 4; u < total; u += MOVE_THREADS * 4)
-        *reinterpret_cast<uint32_t*>(base + u) = *reinterpret_cast<const uint32_t*>(at + u);
+        *reinterpret_cast<uint32_t*>(base + u) = *reinterpret_cast<const uint32_t*>(out + u);
     }
-    at += (p.tile * p.bytes[r] + 15) & ~15;
+    out += (p.tile * p.bytes[r] + 15) & ~15;
   }
-  if (tid < kept) mass[dst0 + tid] = kept_mass[tid];
 }
 
 namespace {
@@ -358,8 +395,9 @@ int64_t evict_up(int64_t x) { return (x + 255) & ~int64_t{255}; }
 }  // namespace
 
 size_t evict_workspace(int64_t B, int64_t H, int64_t cap) {
-  const int64_t tiles = (cap + EVICT_MIN_TILE - 1) / EVICT_MIN_TILE;
-  return static_cast<size_t>(256 + evict_up(B * H * 16) + evict_up(B * H * tiles * 8) + evict_up(B * H * tiles * 4));
+  const int64_t tiles = (cap + EVICT_MIN_TILE - 1) / EVICT_MIN_TILE, heads = B * H;
+  return static_cast<size_t>(256 + evict_up(heads * 16) + evict_up(heads * tiles * 8) + 2 * evict_up(heads * tiles * 4) +
+                             evict_up(heads * ((cap + 31) / 32) * 8));
 }
 
 cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
@@ -367,19 +405,28 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   // tiles of up to 128 entries and 80 KB of rows
   int bytes = 0;
   for (int r = 0; r < p.n_rows; ++r) bytes += p.bytes[r];
-  p.tile = 128;
+  p.tile = MOVE_THREADS;
   while (p.tile > EVICT_MIN_TILE && p.tile * bytes > 80 * 1024) p.tile >>= 1;
-  p.max_tiles = (p.cap + p.tile - 1) / p.tile;
   p.tile_shift = __builtin_ctz(static_cast<unsigned>(p.tile));
+  p.max_tiles = (p.cap + p.tile - 1) / p.tile;
+  p.max_words = (p.cap + 31) / 32;
   const int64_t heads = static_cast<int64_t>(p.B) * p.H;
+  uint8_t* at = ws + 256;
+  auto take = [&](int64_t n) {
+    uint8_t* x = at;
+    at += evict_up(n);
+    return x;
+  };
   p.err = reinterpret_cast<int*>(ws);
-  p.cut = reinterpret_cast<uint4*>(ws + 256);
-  p.before = reinterpret_cast<uint2*>(ws + 256 + evict_up(heads * 16));
-  p.loaded = reinterpret_cast<uint32_t*>(ws + 256 + evict_up(heads * 16) + evict_up(heads * p.max_tiles * 8));
+  p.cut = reinterpret_cast<uint4*>(take(heads * 16));
+  p.before = reinterpret_cast<uint2*>(take(heads * p.max_tiles * 8));
+  p.loaded = reinterpret_cast<uint32_t*>(take(heads * p.max_tiles * 4));
+  p.first_tile = reinterpret_cast<int*>(take(heads * p.max_tiles * 4));
+  p.words = reinterpret_cast<uint2*>(take(heads * p.max_words * 8));
   // 4096 entries a CTA keep a pass near its latency, as long as all CTAs run at once (one an SM)
   int C = 1;
   while (C < SEL_MAX_CTAS && p.cap > C * 4096 && heads * C * 2 <= 148) C <<= 1;
-  int move_smem = p.tile * 8;
+  int move_smem = p.tile * 4;
   for (int r = 0; r < p.n_rows; ++r) {
     const int upr = p.bytes[r] / p.unit[r];
     p.shift[r] = (upr & (upr - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(upr)) : -1;
@@ -393,19 +440,19 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   cfg.gridDim = dim3(static_cast<unsigned>(C), static_cast<unsigned>(heads));
   cfg.blockDim = dim3(SEL_THREADS);
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = static_cast<unsigned>(C);
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(C);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, evict_select_kernel, p);
   if (e != cudaSuccess) return e;
-  cfg.gridDim = dim3(static_cast<unsigned>(p.max_tiles), static_cast<unsigned>(heads));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.budget + p.tile - 1) / p.tile), static_cast<unsigned>(heads));
   cfg.blockDim = dim3(MOVE_THREADS);
   cfg.dynamicSmemBytes = static_cast<size_t>(move_smem);
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   return cudaLaunchKernelEx(&cfg, evict_move_kernel, p);
 }
 

@@ -4,7 +4,8 @@
 
 namespace dab {
 
-constexpr int EVICT_MAX_ROWS = 8, EVICT_MIN_TILE = 32;
+constexpr int EVICT_MAX_ROWS = 9;     // the mass among them
+constexpr int EVICT_MIN_TILE = 32;
 constexpr int EVICT_MAX_BYTES = 4096;  // of an entry's rows together
 
 struct EvictParams {
@@ -18,13 +19,17 @@ struct EvictParams {
   int n_rows;
   int B, H, cap;
   int budget, trigger, first, recent;
-  int tile, tile_shift, max_tiles;       // entries per moved tile (a power of two), tiles of a full head
+  int tile, tile_shift;                  // entries per moved tile, a power of two
+  int max_tiles, max_words;              // of a full head: tiles, words of 32 entries
   // workspace: error word; per head (threshold key, ties kept, length or 0 if left alone, ticket);
-  // per head and tile (kept before it, ties before it) and whether its rows have been read
+  // per head and tile (kept, ties before it); per tile of the result whether its rows have been read
+  // and the tile its first entry comes from; per 32 entries (surely kept, ties)
   int* err;
   uint4* cut;
   uint2* before;
   uint32_t* loaded;
+  int* first_tile;
+  uint2* words;
 };
 
 }  // namespace dab
