@@ -7,6 +7,7 @@ no fallback: if it is missing or a call fails, a RuntimeError is raised (its tex
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -129,13 +130,39 @@ def strides(vals) -> ctypes.Array:
     return (ctypes.c_int64 * len(vals))(*vals)
 
 
+@functools.lru_cache(maxsize=4096)
+def int64s(vals: tuple) -> ctypes.Array:
+    """``strides`` for a tuple of ints, kept by its values (the library only reads it)."""
+    return (ctypes.c_int64 * len(vals))(*vals)
+
+
+# the current stream's handle as an int, without building a Stream object (2 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_of(t: torch.Tensor):
     """Current torch stream of t's device, made current for the library as well."""
-    dev = t.device.index if t.device.index is not None else torch.cuda.current_device()
+    dev = t.get_device()
+    if dev < 0:
+        dev = torch.cuda.current_device()
     if getattr(_dev, "idx", None) != dev:
         check(load().dab_set_device(dev), "set_device")
         _dev.idx = dev
+    if _raw_stream is not None:
+        return ctypes.c_void_p(_raw_stream(dev))
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def same_device(what: str, first: torch.Tensor, *others) -> int:
+    """The CUDA device index that all tensors (None is skipped) are on; raises otherwise."""
+    dev = first.get_device()
+    if dev < 0:
+        require_cuda(first)
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            require_cuda(t)
+            raise ValueError(f"{what}: tensors are on cuda:{dev} and {t.device}")
+    return dev
 
 
 def require_cuda(*tensors):

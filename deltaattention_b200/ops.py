@@ -15,6 +15,7 @@ GQA expansion, two-phase attention) with these B200-specific changes:
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -628,6 +629,9 @@ def release_host_prefill_buffers():
     _host_ws.clear()
 
 
+_HALF = {torch.float16: 1, torch.bfloat16: 2}  # dtype codes of the C ABI
+
+
 @dataclass
 class KV4:
     """K and V rows of a decode history in 4 bits: codes [B, Hkv, M, d / 2] uint8 and scales
@@ -641,39 +645,34 @@ class KV4:
 
     @staticmethod
     def empty(batch, heads, rows, head_dim, device) -> "KV4":
-        shp = (batch, heads, rows)
-        c = [torch.empty((*shp, head_dim // 2), dtype=torch.uint8, device=device) for _ in range(2)]
-        s = [torch.empty((*shp, head_dim // 16), dtype=torch.bfloat16, device=device) for _ in range(2)]
+        c = torch.empty((2, batch, heads, rows, head_dim // 2), dtype=torch.uint8, device=device).unbind(0)
+        s = torch.empty((2, batch, heads, rows, head_dim // 16), dtype=torch.bfloat16, device=device).unbind(0)
         return KV4(c[0], s[0], c[1], s[1])
 
     def rows(self, n0, n1) -> "KV4":
         """The rows [n0, n1) of every head, as views."""
         return KV4(*(t[:, :, n0:n1] for t in (self.k_codes, self.k_scales, self.v_codes, self.v_scales)))
 
-    def check(self, what, shape=None):
-        """Raises unless the four tensors are one history (of ``shape`` (B, Hkv, M, d), when given);
-        returns that shape."""
+    def check(self, what, like, shape=None):
+        """Raises unless the four tensors are one history on ``like``'s device (of ``shape`` (B, Hkv, M,
+        d), when given); returns that shape and the strides of codes and scales over batch and head."""
         kc, ks, vc, vs = self.k_codes, self.k_scales, self.v_codes, self.v_scales
-        L.require_cuda(kc, ks, vc, vs)
+        L.same_device(what, like, kc, ks, vc, vs)
         if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.bfloat16 or vs.dtype != torch.bfloat16:
             raise TypeError(f"{what}: codes are uint8 and scales bf16")
-        B, H, M, half = kc.shape
-        if half not in (32, 64):
-            raise ValueError(f"{what}: head_dim must be 64 or 128")
-        if vc.shape != kc.shape or ks.shape != (B, H, M, half // 8) or vs.shape != ks.shape:
+        size = kc.shape
+        if len(size) != 4 or size[3] not in (32, 64):
+            raise ValueError(f"{what}: codes must be [B, H, M, d / 2] with head_dim 64 or 128")
+        B, H, M, half = size
+        if vc.shape != size or ks.shape != (B, H, M, half // 8) or vs.shape != ks.shape:
             raise ValueError(f"{what}: codes must be [B, H, M, d / 2] and scales [B, H, M, d / 16], alike for K and V")
-        if (kc.stride() != vc.stride() or ks.stride() != vs.stride() or kc.stride(3) != 1 or ks.stride(3) != 1
-                or (M > 1 and (kc.stride(2) != half or ks.stride(2) != half // 8))):
+        c, s = kc.stride(), ks.stride()
+        if (c != vc.stride() or s != vs.stride() or c[3] != 1 or s[3] != 1
+                or (M > 1 and (c[2] != half or s[2] != half // 8))):
             raise ValueError(f"{what}: rows must be contiguous, with the same strides for K and V")
         if shape is not None and shape != (B, H, M, 2 * half):
             raise ValueError(f"{what}: history is {(B, H, M, 2 * half)}, expected {shape}")
-        return B, H, M, 2 * half
-
-
-def _same_device(what, first, *others):
-    for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: tensors are on {first.device} and {t.device}")
+        return (B, H, M, 2 * half), (c[0], c[1], s[0], s[1])
 
 
 def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) -> KV4:
@@ -683,60 +682,70 @@ def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) ->
     zero) / 15 rounded to bf16, code = round((x - zero) / scale) to even, cut to [0, 15]. A group
     that holds a NaN or an infinity reads back as NaN. ``out`` may be views of a cache
     (``KV4.rows``)."""
-    L.require_cuda(k, v)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError("kv4_quantize: k and v must be [B, H, M, d] of one shape and dtype")
-    B, H, M, D = k.shape
-    if k.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError("kv4_quantize: rows must be bf16 or fp16")
+    what = "kv4_quantize"
+    L.same_device(what, k, v)
+    size = k.shape
+    if len(size) != 4 or v.shape != size or k.dtype != v.dtype:
+        raise ValueError(f"{what}: k and v must be [B, H, M, d] of one shape and dtype")
+    B, H, M, D = size
+    if k.dtype not in _HALF:
+        raise TypeError(f"{what}: rows must be bf16 or fp16")
     if D not in (64, 128):
-        raise ValueError("kv4_quantize: head_dim must be 64 or 128")
+        raise ValueError(f"{what}: head_dim must be 64 or 128")
     if out is None:
         out = KV4.empty(B, H, M, D, k.device)
-    else:
-        out.check("kv4_quantize", (B, H, M, D))
-    _same_device("kv4_quantize", k, v, out.k_codes, out.k_scales, out.v_codes, out.v_scales)
+    _, st = out.check(what, k, (B, H, M, D))
     if k.numel() == 0:
         return out
     L.check(L.load().dab_kv4_quantize(
-        L.ptr(k), L.strides(k.stride()), L.ptr(v), L.strides(v.stride()), L.ptr(out.k_codes), L.ptr(out.v_codes),
-        L.strides(out.k_codes.stride()), L.ptr(out.k_scales), L.ptr(out.v_scales), L.strides(out.k_scales.stride()),
-        L.dtype_code(k), B, H, M, D, L.stream_of(k)), "kv4_quantize")
+        k.data_ptr(), L.int64s(k.stride()), v.data_ptr(), L.int64s(v.stride()), out.k_codes.data_ptr(),
+        out.v_codes.data_ptr(), L.int64s(st[:2]), out.k_scales.data_ptr(), out.v_scales.data_ptr(), L.int64s(st[2:]),
+        _HALF[k.dtype], B, H, M, D, L.stream_of(k)), what)
     return out
 
 
 def kv4_dequantize(hist: KV4, dtype: torch.dtype = torch.bfloat16):
     """The K and V rows that a 4-bit history stands for, [B, Hkv, M, d] each, rounded to ``dtype``
     (bf16, fp16 or fp32) from fp32."""
-    B, H, M, D = hist.check("kv4_dequantize")
-    _same_device("kv4_dequantize", hist.k_codes, hist.k_scales, hist.v_codes, hist.v_scales)
-    k = torch.empty((B, H, M, D), dtype=dtype, device=hist.k_codes.device)
-    v = torch.empty_like(k)
+    what = "kv4_dequantize"
+    (B, H, M, D), st = hist.check(what, hist.k_codes)
+    k, v = torch.empty((2, B, H, M, D), dtype=dtype, device=hist.k_codes.device).unbind(0)
+    code = L.dtype_code(k)
     if k.numel() == 0:
-        L.dtype_code(k)
         return k, v
     L.check(L.load().dab_kv4_dequantize(
-        L.ptr(hist.k_codes), L.ptr(hist.v_codes), L.strides(hist.k_codes.stride()), L.ptr(hist.k_scales),
-        L.ptr(hist.v_scales), L.strides(hist.k_scales.stride()), L.ptr(k), L.ptr(v), L.strides(k.stride()),
-        L.dtype_code(k), B, H, M, D, L.stream_of(k)), "kv4_dequantize")
+        hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), L.int64s(st[:2]), hist.k_scales.data_ptr(),
+        hist.v_scales.data_ptr(), L.int64s(st[2:]), k.data_ptr(), v.data_ptr(), L.int64s(k.stride()), code, B, H, M, D,
+        L.stream_of(k)), what)
     return k, v
 
 
 def _plane(what, name, t, shape, dtype):
-    """Checks a per-entry tensor ([B, Hkv, n], contiguous along n)."""
-    if t.dtype != dtype or t.shape != shape or (shape[-1] > 1 and t.stride(-1) != 1):
+    """Checks a per-entry tensor ([B, Hkv, n], contiguous along n); returns its other strides."""
+    st = t.stride()
+    if t.dtype != dtype or t.shape != shape or (st[2] != 1 and shape[2] > 1):
         raise ValueError(f"{what}: {name} must be {dtype} {tuple(shape)}, contiguous along the last dimension")
+    return st[:2]
 
 
 def _exact_window(what, k_exact, v_exact, B, H, D, dtype):
     """(W, strides) of the exact window's K / V rows."""
-    if k_exact.shape != v_exact.shape or k_exact.stride() != v_exact.stride() or k_exact.dtype != dtype \
-            or v_exact.dtype != dtype:
+    size, st = k_exact.shape, k_exact.stride()
+    if v_exact.shape != size or v_exact.stride() != st or k_exact.dtype != dtype or v_exact.dtype != dtype:
         raise ValueError(f"{what}: k_exact and v_exact must agree in shape, strides and dtype with each other and "
                          f"the token ({dtype})")
-    if k_exact.dim() != 4 or k_exact.shape[:2] != (B, H) or k_exact.shape[3] != D or k_exact.stride(3) != 1:
+    if len(size) != 4 or size[0] != B or size[1] != H or size[3] != D or st[3] != 1:
         raise ValueError(f"{what}: the exact window must be [{B}, {H}, W, {D}] with contiguous rows")
-    return k_exact.shape[2], k_exact.stride()[:3]
+    return size[2], st[:3]
+
+
+def _seq_state(what, t):
+    if t.shape != (2,) or t.dtype != torch.int64 or t.stride(0) != 1:
+        raise ValueError(f"{what}: seq_state must be int64 [2]")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
 def decode_update_kv4(k_new, v_new, hist: KV4, counts, timestamps, lengths, last_key, k_exact, v_exact, seq_state, *,
@@ -752,48 +761,46 @@ def decode_update_kv4(k_new, v_new, hist: KV4, counts, timestamps, lengths, last
     (exact, total) lengths in ``seq_state`` (int64 on the device) are read and not advanced. An
     append to a full history writes 0x201 into ``err`` (int32 on the device) and nothing else."""
     what = "decode_update_kv4"
-    B, H, cap, D = hist.check(what)
-    L.require_cuda(k_new, v_new, counts, timestamps, lengths, last_key, k_exact, v_exact, seq_state, mass, exact_mass, err)
+    (B, H, cap, D), hs = hist.check(what, k_new)
+    L.same_device(what, k_new, v_new, counts, timestamps, lengths, last_key, k_exact, v_exact, seq_state, mass,
+                  exact_mass, err)
     if k_new.shape != (B, H, 1, D) or v_new.shape != k_new.shape:
         raise ValueError(f"{what}: k_new and v_new must be [{B}, {H}, 1, {D}]")
-    if k_new.dtype not in (torch.bfloat16, torch.float16) or v_new.dtype != k_new.dtype:
+    dtype = k_new.dtype
+    if dtype not in _HALF or v_new.dtype != dtype:
         raise TypeError(f"{what}: tokens must be bf16 or fp16")
-    W, es = _exact_window(what, k_exact, v_exact, B, H, D, k_new.dtype)
-    if last_key.shape != (B, H, D) or last_key.dtype != k_new.dtype or last_key.stride(2) != 1:
-        raise ValueError(f"{what}: last_key must be {k_new.dtype} [{B}, {H}, {D}] with contiguous rows")
-    _plane(what, "counts", counts, (B, H, cap), torch.int32)
-    _plane(what, "timestamps", timestamps, (B, H, cap), torch.int32)
+    W, es = _exact_window(what, k_exact, v_exact, B, H, D, dtype)
+    ls = last_key.stride()
+    if last_key.shape != (B, H, D) or last_key.dtype != dtype or ls[2] != 1:
+        raise ValueError(f"{what}: last_key must be {dtype} [{B}, {H}, {D}] with contiguous rows")
+    ms = _plane(what, "counts", counts, (B, H, cap), torch.int32)
+    if _plane(what, "timestamps", timestamps, (B, H, cap), torch.int32) != ms:
+        raise ValueError(f"{what}: counts and timestamps must have the same strides")
     if lengths.shape != (B, H) or lengths.dtype != torch.int32:
         raise ValueError(f"{what}: lengths must be int32 [{B}, {H}]")
-    if seq_state.shape != (2,) or seq_state.dtype != torch.int64 or not seq_state.is_contiguous():
-        raise ValueError(f"{what}: seq_state must be int64 [2]")
+    _seq_state(what, seq_state)
     if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
         raise ValueError(f"{what}: err must be int32")
     if (mass is None) != (exact_mass is None):
         raise ValueError(f"{what}: mass and exact_mass come together")
     em = (0, 0)
     if mass is not None:
-        _plane(what, "mass", mass, (B, H, cap), torch.float32)
-        _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
-        em = exact_mass.stride()[:2]
-    ms = counts.stride()[:2]
-    if timestamps.stride()[:2] != ms or (mass is not None and mass.stride()[:2] != ms):
-        raise ValueError(f"{what}: counts, timestamps and mass must have the same strides")
+        if _plane(what, "mass", mass, (B, H, cap), torch.float32) != ms:
+            raise ValueError(f"{what}: counts and mass must have the same strides")
+        em = _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
     if W < 1:
         raise ValueError(f"{what}: the exact window needs at least one row")
-    _same_device(what, k_new, v_new, hist.k_codes, counts, lengths, last_key, k_exact, seq_state, mass, exact_mass, err)
     if k_new.numel() == 0:
         return
     use_cos = similarity == "cosine"
     kn, vn = k_new.stride(), v_new.stride()
-    strides = L.strides((kn[0], kn[1], kn[3], vn[0], vn[1], vn[3], *hist.k_codes.stride()[:2],
-                         *hist.k_scales.stride()[:2], *ms, *lengths.stride(), *last_key.stride()[:2], *es, *em))
+    strides = L.int64s((kn[0], kn[1], kn[3], vn[0], vn[1], vn[3], *hs, *ms, *lengths.stride(), ls[0], ls[1], *es, *em))
     L.check(L.load().dab_decode_update_kv4(
-        L.ptr(k_new), L.ptr(v_new), L.ptr(hist.k_codes), L.ptr(hist.v_codes), L.ptr(hist.k_scales),
-        L.ptr(hist.v_scales), L.ptr(counts), L.ptr(timestamps), L.ptr(mass), L.ptr(lengths), L.ptr(last_key),
-        L.ptr(k_exact), L.ptr(v_exact), L.ptr(exact_mass), L.ptr(seq_state), strides,
-        float(threshold if use_cos else threshold ** 2), 1 if use_cos else 0, L.dtype_code(k_new), B, H, D, cap, W,
-        L.ptr(err), L.stream_of(k_new)), what)
+        k_new.data_ptr(), v_new.data_ptr(), hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), hist.k_scales.data_ptr(),
+        hist.v_scales.data_ptr(), counts.data_ptr(), timestamps.data_ptr(), _ptr(mass), lengths.data_ptr(),
+        last_key.data_ptr(), k_exact.data_ptr(), v_exact.data_ptr(), _ptr(exact_mass), seq_state.data_ptr(), strides,
+        float(threshold if use_cos else threshold ** 2), 1 if use_cos else 0, _HALF[dtype], B, H, D, cap, W, _ptr(err),
+        L.stream_of(k_new)), what)
 
 
 def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=None, *, exact_len=None, seq_state=None,
@@ -812,21 +819,22 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     by. ``workspace`` (uint8, zero-filled once, ``kv4_attention_workspace`` bytes, used by one
     stream at a time) replaces the library's own. Returns out [B, Hq, d]."""
     what = "decode_attention_kv4"
-    B, H, cap, D = hist.check(what)
-    L.require_cuda(q, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
-    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.shape[1] % max(H, 1) or q.stride(2) != 1:
+    (B, H, cap, D), hs = hist.check(what, q)
+    dev = L.same_device(what, q, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
+    size, qs = q.shape, q.stride()
+    if len(size) != 3 or size[0] != B or size[2] != D or size[1] % max(H, 1) or qs[2] != 1:
         raise ValueError(f"{what}: q must be [{B}, a multiple of {H}, {D}] with contiguous rows")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    dtype, Hq = q.dtype, size[1]
+    if dtype not in _HALF:
         raise TypeError(f"{what}: queries must be bf16 or fp16")
-    Hq = q.shape[1]
-    _plane(what, "counts", counts, (B, H, cap), torch.int32)
+    ms = _plane(what, "counts", counts, (B, H, cap), torch.int32)
     if lengths.shape != (B, H) or lengths.dtype != torch.int32:
         raise ValueError(f"{what}: lengths must be int32 [{B}, {H}]")
     W, es = 0, (0, 0, 0)
     if (k_exact is None) != (v_exact is None):
         raise ValueError(f"{what}: k_exact and v_exact come together")
     if k_exact is not None:
-        W, es = _exact_window(what, k_exact, v_exact, B, H, D, q.dtype)
+        W, es = _exact_window(what, k_exact, v_exact, B, H, D, dtype)
     if seq_state is None:
         exact_len = W if exact_len is None else int(exact_len)
         if not 0 <= exact_len <= W:
@@ -836,45 +844,47 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     else:
         if exact_len is not None:
             raise ValueError(f"{what}: exact_len comes from seq_state")
-        if seq_state.shape != (2,) or seq_state.dtype != torch.int64 or not seq_state.is_contiguous():
-            raise ValueError(f"{what}: seq_state must be int64 [2]")
+        _seq_state(what, seq_state)
         exact_len = 0
     if (mass is None) != (exact_mass is None) and (mass is None or W > 0):
         raise ValueError(f"{what}: mass and exact_mass come together")
-    ms, em = counts.stride()[:2], (0, 0)
+    em = (0, 0)
     if mass is not None:
-        _plane(what, "mass", mass, (B, H, cap), torch.float32)
-        if mass.stride()[:2] != ms:
+        if _plane(what, "mass", mass, (B, H, cap), torch.float32) != ms:
             raise ValueError(f"{what}: counts and mass must have the same strides")
         if exact_mass is not None:
-            _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
-            em = exact_mass.stride()[:2]
+            em = _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
     if out is None:
-        out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        out = q.new_empty(size)
+    elif out.shape != size or out.dtype != dtype or out.stride(2) != 1:
         raise ValueError(f"{what}: out must be like q, with contiguous rows")
-    _same_device(what, q, hist.k_codes, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
-    if out.numel() == 0:
+    if B == 0 or Hq == 0:
         return out
-    lib = L.load()
     st = L.stream_of(q)
     if workspace is None:
-        nbytes = lib.dab_decode_attention_kv4_workspace_size(B, H, Hq // H, D, cap, W, 1 if mass is not None else 0)
+        nbytes = _kv4_workspace(dev, B, H, Hq // H, D, cap, W, mass is not None)
         workspace = L.workspace(q.device, st.value, nbytes, tag="kv4")
-    strides = L.strides((*q.stride()[:2], *out.stride()[:2], *hist.k_codes.stride()[:2], *hist.k_scales.stride()[:2],
-                         *ms, *lengths.stride(), *es, *em))
-    L.check(lib.dab_decode_attention_kv4(
-        L.ptr(q), L.ptr(out), L.ptr(hist.k_codes), L.ptr(hist.v_codes), L.ptr(hist.k_scales), L.ptr(hist.v_scales),
-        L.ptr(counts), L.ptr(mass), L.ptr(lengths), L.ptr(k_exact), L.ptr(v_exact), L.ptr(exact_mass),
-        L.ptr(seq_state), 1 if advance else 0, exact_len, strides, float(D ** -0.5 if sm_scale is None else sm_scale),
-        L.dtype_code(q), B, H, Hq // H, D, cap, W, L.ptr(workspace), workspace.numel(), st), what)
+    strides = L.int64s((qs[0], qs[1], *out.stride()[:2], *hs, *ms, *lengths.stride(), *es, *em))
+    L.check(L.load().dab_decode_attention_kv4(
+        q.data_ptr(), out.data_ptr(), hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), hist.k_scales.data_ptr(),
+        hist.v_scales.data_ptr(), counts.data_ptr(), _ptr(mass), lengths.data_ptr(), _ptr(k_exact), _ptr(v_exact),
+        _ptr(exact_mass), _ptr(seq_state), 1 if advance else 0, exact_len, strides,
+        float(D ** -0.5 if sm_scale is None else sm_scale), _HALF[dtype], B, H, Hq // H, D, cap, W, workspace.data_ptr(),
+        workspace.numel(), st), what)
     return out
 
 
-def kv4_attention_workspace(batch, q_heads, kv_heads, head_dim, capacity, exact_window, with_mass=True) -> int:
-    """Bytes of the ``workspace`` that ``decode_attention_kv4`` takes."""
-    return int(L.load().dab_decode_attention_kv4_workspace_size(batch, kv_heads, q_heads // kv_heads, head_dim, capacity,
+@functools.lru_cache(maxsize=1024)
+def _kv4_workspace(device, batch, kv_heads, kv_group, head_dim, capacity, exact_window, with_mass) -> int:
+    # asked with `device` current: the split of the work goes by its number of SMs
+    return int(L.load().dab_decode_attention_kv4_workspace_size(batch, kv_heads, kv_group, head_dim, capacity,
                                                                 exact_window, 1 if with_mass else 0))
+
+
+def kv4_attention_workspace(batch, q_heads, kv_heads, head_dim, capacity, exact_window, with_mass=True) -> int:
+    """Bytes of the ``workspace`` that ``decode_attention_kv4`` takes (on the current device)."""
+    return _kv4_workspace(torch.cuda.current_device(), batch, kv_heads, q_heads // kv_heads, head_dim, capacity,
+                          exact_window, bool(with_mass))
 
 
 def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = None, keep_first: int = 0,
@@ -892,10 +902,11 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
     CUDA graph and replayed at every token, where it only does work once a head passes
     ``trigger``. ``workspace`` as in ``decode_attention_kv4`` (``evict_workspace`` bytes)."""
     what = "evict_by_mass"
-    L.require_cuda(mass, lengths, workspace, *rows)
-    if mass.dim() != 3 or mass.dtype != torch.float32 or (mass.shape[2] > 1 and mass.stride(2) != 1):
+    L.same_device(what, mass, lengths, workspace, *rows)
+    size = mass.shape
+    if len(size) != 3 or mass.dtype != torch.float32 or (size[2] > 1 and mass.stride(2) != 1):
         raise ValueError(f"{what}: mass must be fp32 [B, H, capacity], contiguous along the last dimension")
-    B, H, cap = mass.shape
+    B, H, cap = size
     if lengths.shape != (B, H) or lengths.dtype != torch.int32:
         raise ValueError(f"{what}: lengths must be int32 [{B}, {H}]")
     budget = int(budget)
@@ -908,35 +919,41 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
         raise ValueError(f"{what}: at most 8 row tensors")
     ptrs, nbytes, strides = [], [], []
     for t in rows:
-        if t.dim() < 3 or t.shape[:3] != (B, H, cap):
+        shape, st, width = t.shape, t.stride(), t.element_size()
+        if len(shape) < 3 or shape[:3] != size:
             raise ValueError(f"{what}: row tensors must be [{B}, {H}, {cap}, ...]")
-        size, n = t.element_size(), 1
-        for d in range(t.dim() - 1, 1, -1):
-            if t.shape[d] > 1 and t.stride(d) != n:
+        n = 1
+        for d in range(len(shape) - 1, 2, -1):
+            if st[d] != n and shape[d] > 1:
                 raise ValueError(f"{what}: row tensors must be contiguous from the third dimension on")
-            n *= t.shape[d]
-        n //= max(cap, 1)
-        if cap and ((n * size) % 4 or n == 0 or t.data_ptr() % 4):
+            n *= shape[d]
+        if cap > 1 and st[2] != n:
+            raise ValueError(f"{what}: row tensors must be contiguous from the third dimension on")
+        ptr = t.data_ptr()
+        if n * width % 4 or n == 0 or ptr % 4:
             raise ValueError(f"{what}: row entries must be multiples of 4 bytes, 4-byte aligned")
-        ptrs.append(t.data_ptr())
-        nbytes.append(n * size)
-        strides += [t.stride(0) * size, t.stride(1) * size]
-    _same_device(what, mass, lengths, workspace, *rows)
+        ptrs.append(ptr)
+        nbytes.append(n * width)
+        strides += (st[0] * width, st[1] * width)
     if B == 0 or H == 0 or cap == 0:
         return
-    lib = L.load()
     st = L.stream_of(mass)
     if workspace is None:
-        workspace = L.workspace(mass.device, st.value, lib.dab_evict_by_mass_workspace_size(B, H, cap), tag="evict")
-    L.check(lib.dab_evict_by_mass(
-        L.ptr(mass), L.strides(mass.stride()[:2]), L.ptr(lengths), L.strides(lengths.stride()), len(ptrs),
-        (L.P * len(ptrs))(*ptrs), L.strides(nbytes), L.strides(strides), B, H, cap, budget, trigger, int(keep_first),
-        int(keep_recent), L.ptr(workspace), workspace.numel(), st), what)
+        workspace = L.workspace(mass.device, st.value, _evict_workspace(B, H, cap), tag="evict")
+    L.check(L.load().dab_evict_by_mass(
+        mass.data_ptr(), L.int64s(mass.stride()[:2]), lengths.data_ptr(), L.int64s(lengths.stride()), len(ptrs),
+        (L.P * len(ptrs))(*ptrs), L.int64s(tuple(nbytes)), L.int64s(tuple(strides)), B, H, cap, budget, trigger,
+        int(keep_first), int(keep_recent), workspace.data_ptr(), workspace.numel(), st), what)
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_workspace(batch, heads, capacity) -> int:
+    return int(L.load().dab_evict_by_mass_workspace_size(batch, heads, capacity))
 
 
 def evict_workspace(batch, heads, capacity) -> int:
     """Bytes of the ``workspace`` that ``evict_by_mass`` takes."""
-    return int(L.load().dab_evict_by_mass_workspace_size(batch, heads, capacity))
+    return _evict_workspace(batch, heads, capacity)
 
 
 def tile_count_periodic(N: int, r: int, W: int = 128) -> int:
