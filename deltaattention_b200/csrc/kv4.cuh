@@ -77,8 +77,8 @@ __device__ __forceinline__ float floor_bf16(float x) {
 __device__ __forceinline__ void kv4_scale_zero(float mn, float mx, float& scale, float& zero) {
   zero = floor_bf16(mn);
   scale = round_as<__nv_bfloat16>(__fmul_rn(__fsub_rn(mx, zero), 1.f / 15.f));
-  // x - x is 0 for finite x, NaN otherwise
-  if (!((mx - mx) + (mn - mn) + (scale - scale) + (zero - zero) == 0.f)) scale = zero = __int_as_float(0x7FC00000);
+  // an infinity or NaN in either makes the scale one
+  if (!(scale < INFINITY)) scale = zero = __int_as_float(0x7FC00000);
 }
 
 __device__ __forceinline__ uint32_t kv4_code(float x, float scale, float zero) {
