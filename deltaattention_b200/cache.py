@@ -19,12 +19,16 @@ grows its packed buffers by copying them. ``DeviceDecodeCache`` keeps the same b
 
 Outputs and cache contents are bit-identical to the host-length launches of the same
 kernels (tests/test_gpu_parity.py).
+
+``Kv4DecodeCache`` keeps the packed history in 4 bits and can go on when it is full: heads are cut
+to the entries that drew the most attention.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib as L
+from . import ops
 
 
 class DeviceDecodeCache:
@@ -156,5 +160,143 @@ class DeviceDecodeCache:
         with torch.cuda.graph(g, stream=s):
             for layer in range(self.num_layers):
                 self.step(layer, q[layer], k_new[layer], v_new[layer], out[layer])
+        torch.cuda.current_stream(self.device).wait_stream(s)
+        return g
+
+
+class Kv4DecodeCache:
+    """``DeviceDecodeCache`` with the packed history in 4 bits and a way on when it is full.
+
+    An entry of the history takes 172 bytes at head_dim 128 instead of 520 (codes, scales, count,
+    timestamp, attention weight; ``ops.kv4_quantize`` gives the format), the exact window stays in
+    16 bits. Lengths live on the device as there, so ``step`` and ``evict`` only launch kernels and
+    can be captured. Merge and append decisions are those of the 16-bit cache: the last anchor's key
+    is kept in 16 bits for the comparison.
+
+    Attention adds every entry's weight to ``mass`` (history) and ``exact_mass`` (window; it moves with
+    the token into the history). ``evict`` cuts heads to their heaviest entries by it, in place."""
+
+    def __init__(self, num_layers, batch, kv_heads, head_dim, capacity, exact_window, dtype=torch.bfloat16,
+                 device="cuda", threshold=0.0, use_cosine=False, track_mass=True):
+        if dtype not in (torch.bfloat16, torch.float16) or head_dim not in (64, 128):
+            raise ValueError("Kv4DecodeCache: bf16 / fp16 and head_dim 64 / 128 only")
+        if exact_window < 1 or capacity < 1:
+            raise ValueError("Kv4DecodeCache: capacity and exact_window must be positive")
+        self.num_layers, self.bsz, self.n_kv_heads, self.head_dim = num_layers, batch, kv_heads, head_dim
+        self.capacity, self.exact_window_size, self.dtype = int(capacity), int(exact_window), dtype
+        self.device = torch.device(device)
+        self.threshold, self.similarity = float(threshold), "cosine" if use_cosine else "euclidean"
+        shp, dev, cap, W = (num_layers, batch, kv_heads), self.device, self.capacity, self.exact_window_size
+        z = lambda *s, dt: torch.zeros((*shp, *s), device=dev, dtype=dt)  # noqa: E731
+        self._codes = [z(cap, head_dim // 2, dt=torch.uint8) for _ in range(2)]
+        self._scales = [z(cap, head_dim // 16, dt=torch.bfloat16) for _ in range(2)]
+        self.packed_counts, self.packed_timestamps = z(cap, dt=torch.int32), z(cap, dt=torch.int32)
+        self.packed_lengths = z(dt=torch.int32)
+        self.mass = z(cap, dt=torch.float32) if track_mass else None
+        self.exact_mass = z(W, dt=torch.float32) if track_mass else None
+        self.last_key = z(head_dim, dt=dtype)
+        self.k_exact, self.v_exact = z(W, head_dim, dt=dtype), z(W, head_dim, dt=dtype)
+        self.seq_state = torch.zeros((num_layers, 2), device=dev, dtype=torch.int64)  # (exact, total) per layer
+        self.err = torch.zeros((1,), device=dev, dtype=torch.int32)
+        self.hist = [ops.KV4(self._codes[0][i], self._scales[0][i], self._codes[1][i], self._scales[1][i])
+                     for i in range(num_layers)]
+        self._ws = {}
+
+    def load_prefill(self, layer, k_packed, v_packed, counts, timestamps, k_exact, v_exact, total_len,
+                     batch_index=None, mass=None):
+        """``DeviceDecodeCache.load_prefill``, the packed rows going into 4 bits. ``mass`` [B, Hkv, p_len]
+        is the weight that the anchors start with (0 by default)."""
+        p_len, e_len = k_packed.shape[2], k_exact.shape[2]
+        if p_len > self.capacity:
+            raise ValueError(f"Kv4DecodeCache: {p_len} packed anchors exceed the capacity {self.capacity}")
+        if e_len > self.exact_window_size:
+            raise ValueError(f"Kv4DecodeCache: {e_len} exact tokens exceed the window {self.exact_window_size}")
+        b = slice(None) if batch_index is None else slice(int(batch_index), int(batch_index) + 1)
+        h = self.hist[layer]
+        ops.kv4_quantize(k_packed.to(self.dtype), v_packed.to(self.dtype),
+                         out=ops.KV4(*(t[b, :, :p_len] for t in (h.k_codes, h.k_scales, h.v_codes, h.v_scales))))
+        if p_len:
+            self.last_key[layer, b] = k_packed[:, :, p_len - 1]
+        self.packed_counts[layer, b, :, :p_len] = counts
+        self.packed_timestamps[layer, b, :, :p_len] = timestamps
+        self.packed_lengths[layer, b] = p_len
+        if self.mass is not None:
+            self.mass[layer, b, :, :p_len] = 0.0 if mass is None else mass
+            self.exact_mass[layer, b] = 0.0
+        self.k_exact[layer, b, :, :e_len] = k_exact
+        self.v_exact[layer, b, :, :e_len] = v_exact
+        self.seq_state[layer, 0] = e_len
+        self.seq_state[layer, 1] = int(total_len)
+
+    def _layer(self, t, layer):
+        return None if t is None else t[layer]
+
+    def _workspace(self, name, nbytes):
+        """This cache's own scratch (a captured step keeps using it)."""
+        ws = self._ws.get(name)
+        if ws is None or ws.numel() < nbytes:
+            ws = self._ws[name] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
+        return ws
+
+    def update(self, layer, k_new, v_new, advance=True):
+        """Takes one token per (batch, kv-head): k_new / v_new [B, Hkv, 1, d]; ``advance`` as in
+        ``DeviceDecodeCache.update``."""
+        ops.decode_update_kv4(
+            k_new, v_new, self.hist[layer], self.packed_counts[layer], self.packed_timestamps[layer],
+            self.packed_lengths[layer], self.last_key[layer], self.k_exact[layer], self.v_exact[layer],
+            self.seq_state[layer], threshold=self.threshold, similarity=self.similarity,
+            mass=self._layer(self.mass, layer), exact_mass=self._layer(self.exact_mass, layer), err=self.err)
+        if advance:
+            L.check(L.load().dab_decode_advance(L.ptr(self.seq_state[layer]), 1, L.stream_of(k_new)), "decode_advance")
+
+    def attend(self, layer, q, out=None, sm_scale=None, advance=False):
+        """Attention of q [B, Hq, d] over the layer's history and window, adding to their mass."""
+        ws = self._workspace("attend", ops.kv4_attention_workspace(
+            self.bsz, q.shape[1], self.n_kv_heads, self.head_dim, self.capacity, self.exact_window_size,
+            self.mass is not None))
+        return ops.decode_attention_kv4(
+            q, self.hist[layer], self.packed_counts[layer], self.packed_lengths[layer], self.k_exact[layer],
+            self.v_exact[layer], seq_state=self.seq_state[layer], advance=advance, mass=self._layer(self.mass, layer),
+            exact_mass=self._layer(self.exact_mass, layer), sm_scale=sm_scale, out=out, workspace=ws)
+
+    def step(self, layer, q, k_new, v_new, out=None):
+        """One layer's decode step: update, length advance, attention."""
+        self.update(layer, k_new, v_new, advance=False)
+        return self.attend(layer, q, out, advance=True)
+
+    def evict(self, layer, budget, trigger=None, keep_first=0, keep_recent=1):
+        """Cuts every head of the layer that holds more than ``trigger`` anchors to its ``budget`` heaviest
+        (``ops.evict_by_mass``). The last anchor always stays: the next token may merge into it."""
+        if self.mass is None:
+            raise ValueError("Kv4DecodeCache.evict: the cache does not track attention mass")
+        if keep_recent < 1:
+            raise ValueError("Kv4DecodeCache.evict: keep_recent must be at least 1")
+        h = self.hist[layer]
+        ws = self._workspace("evict", ops.evict_workspace(self.bsz, self.n_kv_heads, self.capacity))
+        ops.evict_by_mass(self.mass[layer], self.packed_lengths[layer],
+                          (h.k_codes, h.k_scales, h.v_codes, h.v_scales, self.packed_counts[layer],
+                           self.packed_timestamps[layer]), budget, trigger=trigger, keep_first=keep_first,
+                          keep_recent=keep_recent, workspace=ws)
+
+    def dequantize(self, layer, dtype=None):
+        """The history's K and V rows [B, Hkv, capacity, d] (rows past a head's length hold anything)."""
+        return ops.kv4_dequantize(self.hist[layer], self.dtype if dtype is None else dtype)
+
+    def lengths(self):
+        """(exact, total) per layer, read back to the host (a synchronising call)."""
+        return [tuple(int(x) for x in row) for row in self.seq_state.cpu()]
+
+    def capture_step(self, q, k_new, v_new, out, evict=None):
+        """``DeviceDecodeCache.capture_step``; with ``evict`` (the arguments of ``evict`` but the layer, as a
+        dict) every replay also cuts the heads that have passed the trigger. Run one eager step (and
+        eviction) first."""
+        s = torch.cuda.Stream(self.device)
+        s.wait_stream(torch.cuda.current_stream(self.device))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for layer in range(self.num_layers):
+                self.step(layer, q[layer], k_new[layer], v_new[layer], out[layer])
+                if evict is not None:
+                    self.evict(layer, **evict)
         torch.cuda.current_stream(self.device).wait_stream(s)
         return g

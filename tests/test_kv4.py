@@ -587,3 +587,122 @@ def test_entries_refuse_on_the_host():
     assert ev(4, 4, 0, 1, 4096) == 1 and "multiples of 4" in said()
     assert ev(4, 4, 0, 0, 8) == 1 and "workspace" in said()
     assert lib.dab_evict_by_mass(p, z, p, z, 0, None, None, None, 1, 1, 64, 64, 64, 0, 0, p, 4096, None) == 0  # cannot be longer
+
+
+# --------------------------------------------------------------------------------- together
+def filled_cache(B=2, H=2, D=64, cap=96, W=8, layers=2, dtype=torch.bfloat16, seed=0, **kw):
+    from deltaattention_b200.cache import Kv4DecodeCache
+    g = torch.Generator().manual_seed(seed)
+    c = Kv4DecodeCache(layers, B, H, D, cap, W, dtype=dtype, threshold=3.0, **kw)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()  # noqa: E731
+    for layer in range(layers):
+        n = 60 - 7 * layer
+        c.load_prefill(layer, r(B, H, n, D), r(B, H, n, D), torch.randint(1, 5, (B, H, n), generator=g).int().cuda(),
+                       torch.arange(0, 4 * n, 4).int().cuda().expand(B, H, n), r(B, H, W, D), r(B, H, W, D), 4 * n)
+    return c, g
+
+
+@gpu
+def test_cache_step_against_its_own_state(ops):
+    """A step is the update, then attention over the state it leaves, its weights added to the mass."""
+    B, H, D, W, Hq = 2, 2, 64, 8, 6
+    c, g = filled_cache(B, H, D, W=W)
+    for step in range(20):
+        q = torch.randn(B, Hq, D, generator=g).bfloat16()
+        k, v = torch.randn(B, H, 1, D, generator=g).bfloat16().cuda(), torch.randn(B, H, 1, D, generator=g).bfloat16().cuda()
+        for layer in range(2):
+            was, ewas = c.mass[layer].clone(), c.exact_mass[layer].clone()
+            total, slot = int(c.seq_state[layer, 1]), int(c.seq_state[layer, 0]) % W
+            n0 = c.packed_lengths[layer].clone()
+            out = c.step(layer, q.cuda(), k, v)
+            assert c.lengths()[layer] == (W + step + 1, total + 1)
+            h = c.hist[layer]
+            kk, vv = values64(h.k_codes, h.k_scales), values64(h.v_codes, h.v_scales)
+            ref, wp, we = attend64(q, kk, vv, c.packed_counts[layer], c.packed_lengths[layer], c.k_exact[layer],
+                                   c.v_exact[layer], W, D ** -0.5)
+            check_attend(out, ref, max(vv.abs().max().item(), c.v_exact[layer].abs().max().item()), torch.bfloat16)
+            # the leaving token's mass went to the entry that took it
+            n = c.packed_lengths[layer].long()
+            assert ((n - n0) <= 1).all()
+            was.scatter_add_(2, (n - 1)[..., None], torch.where(n > n0, 0.0, ewas[:, :, slot])[..., None])
+            put = torch.where((n > n0)[..., None], ewas[:, :, slot, None], was.gather(2, (n - 1)[..., None]))
+            was.scatter_(2, (n - 1)[..., None], put)
+            ewas[:, :, slot] = 0
+            for got, before, w in ((c.mass[layer], was, wp), (c.exact_mass[layer], ewas, we)):
+                err = (got.cpu().double() - (before.cpu().double() + w)).abs()
+                assert (err <= 2.0 ** -14 * w + 2.0 ** -23 * got.cpu().abs()).all()
+    assert int(c.err) == 0
+
+
+@gpu
+def test_cache_evicts_and_goes_on(ops):
+    """Captured steps with eviction run past the capacity and equal the same calls made eagerly."""
+    B, H, D, Hq, cap, layers, steps = 2, 2, 64, 4, 72, 2, 90
+    cut = dict(budget=40, trigger=70, keep_first=2, keep_recent=5)
+    caches = [filled_cache(B, H, D, cap=cap, layers=layers)[0] for _ in range(2)]
+    g = torch.Generator().manual_seed(8)
+    r = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()  # noqa: E731
+    q, k, v = r(layers, B, Hq, D), r(layers, B, H, 1, D), r(layers, B, H, 1, D)
+    outs = [torch.empty_like(q) for _ in caches]
+    for c, o in zip(caches, outs):
+        for layer in range(layers):
+            c.step(layer, q[layer], k[layer], v[layer], o[layer])
+            c.evict(layer, **cut)
+    graph = caches[0].capture_step(q, k, v, outs[0], evict=cut)
+    fell = 0
+    for _ in range(steps):
+        for t in (q, k, v):
+            t.copy_(r(*t.shape))
+        n = caches[0].packed_lengths.clone()
+        graph.replay()
+        for layer in range(layers):
+            caches[1].step(layer, q[layer], k[layer], v[layer], outs[1][layer])
+            caches[1].evict(layer, **cut)
+        fell += int((caches[0].packed_lengths < n).sum())
+        assert torch.equal(outs[0], outs[1]) and torch.isfinite(outs[0].float()).all()
+    a, b = caches
+    assert fell and int(a.err) == 0 and int(a.packed_lengths.max()) <= cut["trigger"]
+    for name in ("packed_counts", "packed_timestamps", "packed_lengths", "mass", "exact_mass", "last_key", "k_exact",
+                 "seq_state"):
+        assert torch.equal(getattr(a, name), getattr(b, name)), name
+    n = a.packed_lengths
+    for layer in range(layers):
+        for bi in range(B):
+            for h in range(H):
+                ts = a.packed_timestamps[layer, bi, h, :int(n[layer, bi, h])]
+                assert (ts[1:] > ts[:-1]).all() and ts[:2].tolist() == [0, 4]  # in order, the first kept
+    assert not L.workspace_errors() or all(c == 0 for c in L.workspace_errors())
+
+
+@gpu
+def test_cache_loads_sequences_one_by_one(ops):
+    """batch_index fills one row of the batch; the others keep what they hold."""
+    c, g = filled_cache(B=3, layers=1)
+    was = [t.clone() for t in (c.hist[0].k_codes, c.hist[0].v_scales, c.packed_counts, c.last_key, c.packed_lengths)]
+    k, v = torch.randn(1, 2, 11, 64, generator=g).bfloat16().cuda(), torch.randn(1, 2, 11, 64, generator=g).bfloat16().cuda()
+    c.load_prefill(0, k, v, torch.full((1, 2, 11), 3, dtype=torch.int32).cuda(), torch.zeros(1, 2, 11, dtype=torch.int32).cuda(),
+                   k[:, :, :8], v[:, :, :8], 99, batch_index=1)
+    one = ops.kv4_quantize(k, v)
+    assert torch.equal(c.hist[0].k_codes[1:2, :, :11], one.k_codes) and torch.equal(c.hist[0].v_scales[1:2, :, :11], one.v_scales)
+    assert torch.equal(c.last_key[0, 1], k[0, :, 10]) and c.packed_lengths[0].tolist() == [[60, 60], [11, 11], [60, 60]]
+    now = (c.hist[0].k_codes, c.hist[0].v_scales, c.packed_counts[0], c.last_key[0], c.packed_lengths[0])
+    for a, b in zip((was[0], was[1], was[2][0], was[3][0], was[4][0]), now):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2])
+    kd, vd = c.dequantize(0, torch.float32)
+    assert torch.equal(kd[1:2, :, :11], ops.kv4_dequantize(one, torch.float32)[0])
+
+
+@gpu
+def test_cache_refusals(ops):
+    from deltaattention_b200.cache import Kv4DecodeCache
+    c, _ = filled_cache(layers=1)
+    x = torch.zeros(2, 2, 97, 64, dtype=torch.bfloat16, device="cuda")
+    n = torch.zeros(2, 2, 97, dtype=torch.int32, device="cuda")
+    plain = Kv4DecodeCache(1, 1, 1, 64, 8, 4, track_mass=False)
+    for call in (lambda: Kv4DecodeCache(1, 1, 1, 96, 8, 4), lambda: Kv4DecodeCache(1, 1, 1, 64, 8, 0),
+                 lambda: Kv4DecodeCache(1, 1, 1, 64, 8, 4, dtype=torch.float32),
+                 lambda: c.load_prefill(0, x, x, n, n, x[:, :, :8], x[:, :, :8], 1),
+                 lambda: c.load_prefill(0, x[:, :, :9], x[:, :, :9], n[:, :, :9], n[:, :, :9], x[:, :, :9], x[:, :, :9], 1),
+                 lambda: c.evict(0, 10, keep_recent=0), lambda: c.evict(0, 10, trigger=9), lambda: plain.evict(0, 4)):
+        with pytest.raises(ValueError):
+            call()
