@@ -427,22 +427,27 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
       for (int g = 0; g < NG; ++g) {
         uint32_t qf[4];
         lds_words<4>(qf, frag_at + g * 512);
+        float a[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float a[4];
-          uint32_t x[2] = {w[i][0][g] << 2, w[i][1][g] << 2};
-          mma16816_set<__half>(a, code_pair_h<0>(x[0]), code_pair_h<0>(x[1]), code_pair_h<1>(x[0]), code_pair_h<1>(x[1]),
+          const uint32_t x[2] = {w[i][0][g] << 2, w[i][1][g] << 2};
+          mma16816_set<__half>(a[i], code_pair_h<0>(x[0]), code_pair_h<0>(x[1]), code_pair_h<1>(x[0]), code_pair_h<1>(x[1]),
                                qf[0], qf[1]);
-          x[0] = w[i][0][g] >> 6;
-          x[1] = w[i][1][g] >> 6;
-          mma16816<__half>(a, code_pair_h<2>(x[0]), code_pair_h<2>(x[1]), code_pair_h<3>(x[0]), code_pair_h<3>(x[1]),
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t x[2] = {w[i][0][g] >> 6, w[i][1][g] >> 6};
+          mma16816<__half>(a[i], code_pair_h<2>(x[0]), code_pair_h<2>(x[1]), code_pair_h<3>(x[0]), code_pair_h<3>(x[1]),
                            qf[2], qf[3]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           const float xa = g & 1 ? hi_f32(s2[i][0][g >> 1]) : lo_f32(s2[i][0][g >> 1]);
           const float xb = g & 1 ? hi_f32(s2[i][1][g >> 1]) : lo_f32(s2[i][1][g >> 1]);
-          zs[i][0] = fmaf(xa, a[0], zs[i][0]);
-          zs[i][1] = fmaf(xa, a[1], zs[i][1]);
-          zs[i][2] = fmaf(xb, a[2], zs[i][2]);
-          zs[i][3] = fmaf(xb, a[3], zs[i][3]);
+          zs[i][0] = fmaf(xa, a[i][0], zs[i][0]);
+          zs[i][1] = fmaf(xa, a[i][1], zs[i][1]);
+          zs[i][2] = fmaf(xb, a[i][2], zs[i][2]);
+          zs[i][3] = fmaf(xb, a[i][3], zs[i][3]);
         }
       }
     }
@@ -503,10 +508,10 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
           x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
         }
         const uint32_t a[4] = {code_pair<0>(x[0]), code_pair<1>(x[0]), code_pair<0>(x[1]), code_pair<1>(x[1])};
-        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wh[0], wh[1]);
-        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wl[0], wl[1]);
         const uint32_t d[4] = {code_pair<2>(x[0]), code_pair<3>(x[0]), code_pair<2>(x[1]), code_pair<3>(x[1])};
+        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wh[0], wh[1]);
         mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wh[0], wh[1]);
+        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wl[0], wl[1]);
         mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wl[0], wl[1]);
       }
     }
@@ -837,14 +842,15 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
   }
   // 4 neighbouring entries a thread: history [0, cap), window from column wcol on
   const int n = max(0, min(p.lengths[b * p.lb + h * p.lh], p.cap));
-  const int key = (blockIdx.x - p.G) * KV4_MASS_KEYS + 4 * threadIdx.x;
+  const int k0 = (blockIdx.x - p.G) * KV4_MASS_KEYS, key = k0 + 4 * threadIdx.x;
+  if (k0 >= n && k0 + KV4_MASS_KEYS <= p.wcol) return;  // past the history, before the window
   float* mp = p.mass + b * p.mb + h * p.mh + key;
   float m[4], w[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = key + i < n ? mp[i] : 0.f;  // read while the attention kernel ends
   grid_wait();
   const int elen = p.state ? *p.used : p.exact_len, j = key - p.wcol;
-  if (blockIdx.x * KV4_MASS_KEYS - p.G * KV4_MASS_KEYS >= max(n, p.wcol + elen)) return;
+  if (k0 >= max(n, p.wcol + elen)) return;
   const bool some = key < n || (j >= 0 && j < elen);
   for (int g0 = 0; g0 < p.G; g0 += 8) {
     const int ng = min(8, p.G - g0);
