@@ -645,9 +645,9 @@ class KV4:
 
     @staticmethod
     def empty(batch, heads, rows, head_dim, device) -> "KV4":
-        c = torch.empty((2, batch, heads, rows, head_dim // 2), dtype=torch.uint8, device=device).unbind(0)
-        s = torch.empty((2, batch, heads, rows, head_dim // 16), dtype=torch.bfloat16, device=device).unbind(0)
-        return KV4(c[0], s[0], c[1], s[1])
+        c = torch.empty((batch, heads, rows, head_dim // 2), dtype=torch.uint8, device=device)
+        s = torch.empty((batch, heads, rows, head_dim // 16), dtype=torch.bfloat16, device=device)
+        return KV4(c, s, torch.empty_like(c), torch.empty_like(s))
 
     def rows(self, n0, n1) -> "KV4":
         """The rows [n0, n1) of every head, as views."""
@@ -658,7 +658,8 @@ class KV4:
         d), when given); returns that shape and the strides of codes and scales over batch and head."""
         kc, ks, vc, vs = self.k_codes, self.k_scales, self.v_codes, self.v_scales
         L.same_device(what, like, kc, ks, vc, vs)
-        if kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.bfloat16 or vs.dtype != torch.bfloat16:
+        if (kc.dtype != torch.uint8 or vc.dtype != torch.uint8 or ks.dtype != torch.bfloat16
+                or vs.dtype != torch.bfloat16):
             raise TypeError(f"{what}: codes are uint8 and scales bf16")
         size = kc.shape
         if len(size) != 4 or size[3] not in (32, 64):
@@ -694,8 +695,10 @@ def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) ->
         raise ValueError(f"{what}: head_dim must be 64 or 128")
     if out is None:
         out = KV4.empty(B, H, M, D, k.device)
-    _, st = out.check(what, k, (B, H, M, D))
-    if k.numel() == 0:
+        st = (H * M * (D // 2), M * (D // 2), H * M * (D // 16), M * (D // 16))
+    else:
+        _, st = out.check(what, k, (B, H, M, D))
+    if B * H * M == 0:
         return out
     L.check(L.load().dab_kv4_quantize(
         k.data_ptr(), L.int64s(k.stride()), v.data_ptr(), L.int64s(v.stride()), out.k_codes.data_ptr(),
@@ -709,14 +712,15 @@ def kv4_dequantize(hist: KV4, dtype: torch.dtype = torch.bfloat16):
     (bf16, fp16 or fp32) from fp32."""
     what = "kv4_dequantize"
     (B, H, M, D), st = hist.check(what, hist.k_codes)
-    k, v = torch.empty((2, B, H, M, D), dtype=dtype, device=hist.k_codes.device).unbind(0)
+    k = torch.empty((B, H, M, D), dtype=dtype, device=hist.k_codes.device)
+    v = torch.empty_like(k)
     code = L.dtype_code(k)
-    if k.numel() == 0:
+    if B * H * M == 0:
         return k, v
     L.check(L.load().dab_kv4_dequantize(
         hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), L.int64s(st[:2]), hist.k_scales.data_ptr(),
-        hist.v_scales.data_ptr(), L.int64s(st[2:]), k.data_ptr(), v.data_ptr(), L.int64s(k.stride()), code, B, H, M, D,
-        L.stream_of(k)), what)
+        hist.v_scales.data_ptr(), L.int64s(st[2:]), k.data_ptr(), v.data_ptr(), L.int64s((H * M * D, M * D, D)), code,
+        B, H, M, D, L.stream_of(k)), what)
     return k, v
 
 
@@ -869,8 +873,8 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
         q.data_ptr(), out.data_ptr(), hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), hist.k_scales.data_ptr(),
         hist.v_scales.data_ptr(), counts.data_ptr(), _ptr(mass), lengths.data_ptr(), _ptr(k_exact), _ptr(v_exact),
         _ptr(exact_mass), _ptr(seq_state), 1 if advance else 0, exact_len, strides,
-        float(D ** -0.5 if sm_scale is None else sm_scale), _HALF[dtype], B, H, Hq // H, D, cap, W, workspace.data_ptr(),
-        workspace.numel(), st), what)
+        float(D ** -0.5 if sm_scale is None else sm_scale), _HALF[dtype], B, H, Hq // H, D, cap, W,
+        workspace.data_ptr(), workspace.numel(), st), what)
     return out
 
 
