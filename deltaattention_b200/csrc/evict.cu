@@ -33,7 +33,7 @@ constexpr int SEL_THREADS = 1024, SEL_MAX_CTAS = 8;  // of a cluster
 constexpr int SEL_KEYS = 16;                         // a thread's keys in registers; longer slices are read again
 constexpr int SEL_BINS = 2048;
 constexpr int SEL_CHUNK = SEL_THREADS * SEL_KEYS;
-constexpr int MOVE_THREADS = 128;
+constexpr int MOVE_THREADS = 256;
 enum { ERR_EVICT_WAIT = 0x501 };
 
 // Unsigned key of a weight in the order of floats: NaN below everything, -0 equal to +0.
@@ -402,7 +402,7 @@ size_t evict_workspace(int64_t B, int64_t H, int64_t cap) {
 
 cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   if (p.B * p.H == 0 || p.cap == 0) return cudaSuccess;
-  // tiles of up to 128 entries and 80 KB of rows
+  // tiles of up to 256 entries and 80 KB of rows
   int bytes = 0;
   for (int r = 0; r < p.n_rows; ++r) bytes += p.bytes[r];
   p.tile = MOVE_THREADS;
