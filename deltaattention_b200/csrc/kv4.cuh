@@ -64,7 +64,6 @@ struct Kv4Attn {
   int* used;                                     // with state: the window length this call attends with
   int64_t sstride; int wcol;                     // columns of a row of scores, the window's first
   int splits, pieces;                            // per head, or in all
-  int* err;                                      // error word
 };
 
 // x rounded down (towards -inf) to bf16, as fp32

@@ -5,21 +5,23 @@
 //   q . k_j  = sum_g scale_jg (sum_{d in g} q_d code_jd) + sum_g zero_jg qsum_g
 //   sum_j p_j v_jd = sum_j (p_j scale_jg) code_jd + sum_j p_j zero_jg
 // so the matrix instructions take the codes themselves, and nothing is dequantised.
-//  * Scores: keys are the rows of the product, q-heads its 8 columns. A code in the mantissa of 256.0
-//    or 16.0 is the fp16 number 256 + code or 16 + code: two shifts and four and-or operations give
-//    8 operands. q goes in as fp16, scaled by a power of two so that its largest element is in [2^13,
-//    2^14): what is below 2^-30 of that is rounded, all else exact. One accumulator per group,
-//    multiplied by the group's scale in fp32. What the 256 and 16 bring in and the zeros are two
-//    more products: rows are the stored (scales, zeros), columns the coefficients in three bf16
-//    parts (24 bits).
-//    (8-bit float operands, a code's byte being code * 2^-9, took 125 us where this took 112 at
-//    4 x 65536 x 8 heads: this matrix path converts them to fp16 first.)
+//  * Scores: keys are the rows of the product, q-heads its 8 columns. A code alone in the low byte
+//    of a half is an fp16 subnormal, code 2^-24 or code 2^-20: one shift and four ands give 8
+//    operands, and nothing has to be taken off again. q goes in as fp16, scaled by a power of two so
+//    that its largest element is in [2^13, 2^14), every second pair by 2^-4 of that: what is below
+//    2^-26 of the largest is rounded, all else exact. One accumulator per group, multiplied by the
+//    group's scale in fp32. The zeros are one more product: their coefficients, the sums of q, go in
+//    as three bf16 parts (24 bits).
+//    (16-bit numbers 256 + code and 16 + code, the offsets taken off with the zeros, took two shifts,
+//    one product more and lost 4 bits of the sums; 8-bit float operands took a quarter longer: this
+//    matrix path converts them to fp16 first.)
 //  * Values: elements are the rows, q-heads the columns. A code in the mantissa of 16.0 is the bf16
 //    number 16 + code. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every
 //    weight); p alone, in two parts, times the stored (scales, zeros) gives what the 16 brought in
 //    and the zeros, added once at the end.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 
 #include "kv4.cuh"
 #include "mma16.cuh"
@@ -73,12 +75,6 @@ template <int I>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
   return (x & 0x00780078u) | 0x41804180u;
-}
-// fp16: 256 + code (I even), 16 + code (I odd) for the codes at bits 4 I.. of both halves, from w << 2
-// (I = 0, 1) or w >> 6 (I = 2, 3)
-template <int I>
-__device__ __forceinline__ uint32_t code_pair_h(uint32_t x) {
-  return I & 1 ? (x & 0x03C003C0u) | 0x4C004C00u : (x & 0x003C003Cu) | 0x5C005C00u;
 }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -209,17 +205,24 @@ struct Kv4Acc {
   }
 };
 
+// the second part of p s, into x where `second` is set: x there holds the first part, p_hi s rounded
+__device__ __forceinline__ void second_part(uint32_t& x, uint32_t hi, uint32_t lo, uint32_t s, bool second) {
+  asm("{\n\t.reg .pred p;\n\t.reg .b32 n;\n\tsetp.ne.b32 p, %4, 0;\n\tneg.bf16x2 n, %0;\n\t"
+      "@p fma.rn.bf16x2 %0, %1, %3, n;\n\t@p fma.rn.bf16x2 %0, %2, %3, %0;\n\t}"
+      : "+r"(x) : "r"(hi), "r"(lo), "r"(s), "r"(static_cast<uint32_t>(second)));
+}
+
 // q of up to 8 heads as column fragments of the score product, and the coefficients of the stored
 // scales and zeros
-template <typename T, int D>
+template <typename T, int D, bool FOLD>
 struct Kv4Query {
   static constexpr int NG = D / 32;
-  uint32_t zc[3];        // coefficient pairs of a row's word of (scales, zeros), in three parts
+  uint32_t zc[2];        // coefficients of a row's zeros: sums of q in three parts
   float back[2];         // of heads 2 t, 2 t + 1: what takes the product to log2 units
 
   // `frag` gets the pairs (8 t + 2 half + {0, 1}, + 4) of every group, [group][lane][2 half + ..]
   __device__ __forceinline__ void load(const T* q, int64_t stride, int ng, float scale_log2, uint4* frag) {
-    const int lane = threadIdx.x & 31, t = lane & 3, head = lane >> 2;
+    const int lane = threadIdx.x & 31, t = lane & 3, head = (lane >> 2) & (FOLD ? 3 : 7);
     uint4 w[NG];
     float top = 0.f;
 #pragma unroll
@@ -236,42 +239,30 @@ struct Kv4Query {
     const int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
     const int k = top > 0.f && ex < 128 ? max(-126, min(126, 13 - ex)) : 0;
     const float f = __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
-    float qsum[NG], osum[NG];  // of the elements, and of the elements times what their codes carry
+    float qsum[NG];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const T* e = reinterpret_cast<const T*>(&w[g]);
-      float even = 0.f, odd = 0.f;
+      float sum = 0.f;
       uint32_t b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // elements i, i + 4
-        const __half2 x = __floats2half2_rn(to_f32(e[i]) * f, to_f32(e[i + 4]) * f);
+      for (int i = 0; i < 4; ++i) {  // elements i, i + 4; odd i meet codes 2^4 higher
+        const float u = i & 1 ? f * 0.0625f : f;
+        const __half2 x = __floats2half2_rn(to_f32(e[i]) * u, to_f32(e[i + 4]) * u);
         const float2 y = __half22float2(x);
         b[i] = *reinterpret_cast<const uint32_t*>(&x);
-        if (i & 1) odd += y.x + y.y;
-        else even += y.x + y.y;
+        sum = fmaf(y.x + y.y, i & 1 ? 16.f : 1.f, sum);
       }
       if (threadIdx.x < 32) frag[g * 32 + lane] = make_uint4(b[0], b[1], b[2], b[3]);
 #pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        even += __shfl_xor_sync(0xFFFFFFFFu, even, o);
-        odd += __shfl_xor_sync(0xFFFFFFFFu, odd, o);
-      }
-      qsum[g] = even + odd;
-      osum[g] = -fmaf(256.f, even, 16.f * odd);
+      for (int o = 1; o <= 2; o <<= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      qsum[g] = sum * 0x1p-24f;  // in units of the codes
     }
-    // word j of a row: values 2 j, 2 j + 1 of (scales, zeros)
+    // pairs of zeros; lane t takes pair t (NG = 4: pairs 0, 1, 0, 1; NG = 2: the only one)
     float x[2];
-    const int j = NG == 4 ? t : t & 1;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int v = 2 * j + e;
-      x[e] = 0.f;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        if (v == g) x[e] = osum[g];
-        if (v == NG + g) x[e] = qsum[g];
-      }
-    }
+    const bool second = NG == 4 && (t & 1);
+    x[0] = second ? qsum[NG - 2] : qsum[0];
+    x[1] = second ? qsum[NG - 1] : qsum[1];
     uint32_t part[3];
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
@@ -279,14 +270,16 @@ struct Kv4Query {
       x[0] -= lo_f32(part[i]);
       x[1] -= hi_f32(part[i]);
     }
-    if constexpr (NG == 4) {  // products (part 0, part 1) and (part 2, -)
-      zc[0] = part[0]; zc[1] = part[1]; zc[2] = part[2];
-    } else {                  // words 2, 3 stand for words 0, 1 again: (part 0 | part 1), (part 2 | -)
+    if constexpr (NG == 4) {
       zc[0] = t < 2 ? part[0] : part[1];
       zc[1] = t < 2 ? part[2] : 0u;
-      zc[2] = 0u;
+    } else {
+      zc[0] = t == 0 ? part[0] : t == 1 ? part[1] : t == 2 ? part[2] : 0u;
+      zc[1] = 0u;
     }
-    const float bk = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    // 2^24 2^-k; finite, so that a score of 0 stays one
+    const float unit = scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - k) << 23) * 0x1p24f;
+    const float bk = fmaxf(fminf(unit, FLT_MAX), -FLT_MAX);
     back[0] = __shfl_sync(0xFFFFFFFFu, bk, 8 * t);
     back[1] = __shfl_sync(0xFFFFFFFFu, bk, 8 * t + 4);
   }
@@ -303,7 +296,7 @@ __device__ __forceinline__ int kv4_units(int n, int elen) {
 }
 
 // Units [u0, u1) of group z (8 q-heads) of head bh, by the whole CTA.
-template <typename T, int D, bool MASS>
+template <typename T, int D, bool MASS, bool FOLD>
 __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uint4* frag, int bh, int z, int n, int elen, int u0,
                                             int u1, int slot) {
   using St = Kv4Stage<D>;
@@ -321,6 +314,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   const uint32_t k_at = St::K + (NG == 4 ? St::piece(gq, t) : St::piece(gq, t >> 1) + 8 * (t & 1));
   const uint32_t v_at = St::V + (NG == 4 ? St::piece(2 * t, gq >> 1) : St::piece(2 * t, gq >> 2) + 8 * ((gq >> 1) & 1));
   const uint32_t ks_at = St::KS + gq * St::SROW, vs_at = St::VS + 2 * t * St::SROW;
+  const uint32_t zk_at = ks_at + 2 * NG + (NG == 4 ? 4 * (t & 1) : 0);  // a pair of zeros
   // A lane copies pieces lane + 32 i of a tile's codes (they are contiguous), its row's scales and
   // count.
   const int last = min(u1, n4);  // history tiles of this segment end here
@@ -374,7 +368,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   for (int s = 0; s < KV4_STAGES - 1; ++s) issue(s);
 
   const T* qp = static_cast<const T*>(p.q) + b * p.qb + (static_cast<int64_t>(h) * p.G + h0) * p.qh;
-  Kv4Query<T, D> q;
+  Kv4Query<T, D, FOLD> q;
   q.load(qp, p.qh, ng, p.scale_log2, frag);
   __syncthreads();  // the fragments are there
   Kv4Acc<D> acc;
@@ -382,6 +376,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   float* sc0 = MASS ? p.scores + (row0 + 2 * t) * p.sstride + gq : nullptr;
   const uint32_t frag_at = smem_u32(frag + lane);
   const bool head0 = 2 * t < ng, head1 = 2 * t + 1 < ng;
+  const bool second = FOLD && gq >= 4;  // this lane's column takes the second parts
 
   int unit = u0 + warp, stage = 0;
   for (; unit < last; unit += KV4_NW) {
@@ -413,15 +408,10 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
           lds_words<NG>(w[i][f], sp + k_at + r * St::ROW);
           lds_words<NG / 2>(s2[i][f], sp + ks_at + r * St::SROW);
         }
-        uint32_t zw[4];  // word t of (scales, zeros) of both rows, twice
-        if constexpr (NG == 4) {
-          ldsm_x4<false>(zw, sp + St::KS + (lane & 15) * St::SROW + 16 * i * St::SROW);
-        } else {
+        uint32_t zw[2];  // pairs of zeros of both rows, the same for every part
 #pragma unroll
-          for (int f = 0; f < 2; ++f) zw[f] = zw[f + 2] = lds32(sp + ks_at + 4 * (t & 1) + (16 * i + 8 * f) * St::SROW);
-        }
-        mma16816_set<__nv_bfloat16>(zs[i], zw[0], zw[1], zw[2], zw[3], q.zc[0], q.zc[1]);
-        if constexpr (NG == 4) mma16816<__nv_bfloat16>(zs[i], zw[0], zw[1], zw[2], zw[3], q.zc[2], 0u);
+        for (int f = 0; f < 2; ++f) zw[f] = lds32(sp + zk_at + (16 * i + 8 * f) * St::SROW);
+        mma16816_set<__nv_bfloat16>(zs[i], zw[0], zw[1], zw[0], zw[1], q.zc[0], q.zc[1]);
       }
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -430,15 +420,13 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         float a[2][4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t x[2] = {w[i][0][g] << 2, w[i][1][g] << 2};
-          mma16816_set<__half>(a[i], code_pair_h<0>(x[0]), code_pair_h<0>(x[1]), code_pair_h<1>(x[0]), code_pair_h<1>(x[1]),
-                               qf[0], qf[1]);
+          const uint32_t x[2] = {w[i][0][g], w[i][1][g]};
+          mma16816_set<__half>(a[i], x[0] & 0x000F000Fu, x[1] & 0x000F000Fu, x[0] & 0x00F000F0u, x[1] & 0x00F000F0u, qf[0], qf[1]);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint32_t x[2] = {w[i][0][g] >> 6, w[i][1][g] >> 6};
-          mma16816<__half>(a[i], code_pair_h<2>(x[0]), code_pair_h<2>(x[1]), code_pair_h<3>(x[0]), code_pair_h<3>(x[1]),
-                           qf[2], qf[3]);
+          const uint32_t x[2] = {w[i][0][g] >> 8, w[i][1][g] >> 8};
+          mma16816<__half>(a[i], x[0] & 0x000F000Fu, x[1] & 0x000F000Fu, x[0] & 0x00F000F0u, x[1] & 0x00F000F0u, qf[2], qf[3]);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -465,24 +453,32 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         if (head1) { o[p.sstride] = zs[i][1]; o[p.sstride + 8] = zs[i][3]; }
       }
     }
-    acc.template weights<2>(zs);
-    // ---- values
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t ph[2], pl[2];  // weights of keys 2 t, 2 t + 1 (+ 8) for head lane / 4, two parts
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        split2<__nv_bfloat16>(zs[i][2 * f], zs[i][2 * f + 1], ph[f], pl[f]);
-        ph[f] = movm(ph[f]);
-        pl[f] = movm(pl[f]);
-      }
-      uint32_t w[4][NG], s[4][NG / 2];  // codes and scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+    // value codes and scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9; those of the first 16 keys are
+    // loaded before the exponentials, which hide the latency
+    uint32_t w[4][NG], s[4][NG / 2];
+    auto load_values = [&](int i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 16 * i + (k & 1) + 8 * (k >> 1);
         lds_words<NG>(w[k], sp + v_at + r * St::ROW);
         lds_words<NG / 2>(s[k], sp + vs_at + r * St::SROW);
       }
+    };
+    load_values(0);
+    acc.template weights<2>(zs);
+    // ---- values
+    uint32_t ph[2][2], pl[2][2];  // weights of keys 2 t, 2 t + 1 (+ 8) for head lane / 4, two parts
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        split2<__nv_bfloat16>(zs[i][2 * f], zs[i][2 * f + 1], ph[i][f], pl[i][f]);
+        ph[i][f] = movm(ph[i][f]);
+        pl[i][f] = movm(pl[i][f]);
+      }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i) load_values(1);
       // sums of p scale and p zero: rows are the stored values (and again, for whole operands)
       using B = __nv_bfloat16;
       uint32_t v[4];
@@ -494,8 +490,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         v[0] = v[1] = prmt(v[0], v[1], 0x5410);
         v[2] = v[3] = prmt(v[2], v[3], 0x5410);
       }
-      mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], ph[0], ph[1]);
-      mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], pl[0], pl[1]);
+      mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], second ? pl[i][0] : ph[i][0], second ? pl[i][1] : ph[i][1]);
+      if constexpr (!FOLD) mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], pl[i][0], pl[i][1]);
       const uint32_t half = gq & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -503,16 +499,19 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const uint32_t sc = prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u);
-          wh[f] = bmul2(ph[f], sc);
-          wl[f] = bfma2(pl[f], sc, bfms2(ph[f], sc, wh[f]));
+          wh[f] = bmul2(ph[i][f], sc);
+          if constexpr (FOLD) second_part(wh[f], ph[i][f], pl[i][f], sc, second);
+          else wl[f] = bfma2(pl[i][f], sc, bfms2(ph[i][f], sc, wh[f]));
           x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
         }
         const uint32_t a[4] = {code_pair<0>(x[0]), code_pair<1>(x[0]), code_pair<0>(x[1]), code_pair<1>(x[1])};
         const uint32_t d[4] = {code_pair<2>(x[0]), code_pair<3>(x[0]), code_pair<2>(x[1]), code_pair<3>(x[1])};
         mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wh[0], wh[1]);
         mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wh[0], wh[1]);
-        mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wl[0], wl[1]);
-        mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wl[0], wl[1]);
+        if constexpr (!FOLD) {
+          mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wl[0], wl[1]);
+          mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wl[0], wl[1]);
+        }
       }
     }
     stage = stage == KV4_STAGES - 1 ? 0 : stage + 1;
@@ -520,6 +519,13 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   cp_wait<0>();
 
   // what the 16 of the codes brought in comes off, the zeros go on
+  if constexpr (FOLD) {  // in the columns of the first parts
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float x = acc.sz[e] + __shfl_xor_sync(0xFFFFFFFFu, acc.sz[e], 2);
+      acc.sz[e] = t < 2 ? x : 0.f;
+    }
+  }
   float sum_s[NG][2], sum_z[NG][2];
 #pragma unroll
   for (int g = 0; g < NG; ++g)
@@ -547,7 +553,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (gq < ng) w = *reinterpret_cast<const uint4*>(qp + gq * p.qh + 32 * g + 8 * t);
+      const int head = gq & (FOLD ? 3 : 7);
+      if (head < ng) w = *reinterpret_cast<const uint4*>(qp + head * p.qh + 32 * g + 8 * t);
       qw[g][0][0] = prmt(w.x, w.z, 0x5410);
       qw[g][0][1] = prmt(w.x, w.z, 0x7632);
       qw[g][1][0] = prmt(w.y, w.w, 0x5410);
@@ -584,8 +591,12 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
       split2<T>(zs[0][2 * f], zs[0][2 * f + 1], ph[f], pl[f]);
-      ph[f] = movm(ph[f]);
-      pl[f] = movm(pl[f]);
+      if constexpr (FOLD) {  // column 4 + j: the second part of head j
+        ph[f] = movm(t < 2 ? ph[f] : pl[f]);
+      } else {
+        ph[f] = movm(ph[f]);
+        pl[f] = movm(pl[f]);
+      }
     }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -601,10 +612,18 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
       const uint32_t d[4] = {prmt(x[0].y, x[1].y, 0x5410), prmt(x[0].y, x[1].y, 0x7632), prmt(x[2].y, x[3].y, 0x5410),
                              prmt(x[2].y, x[3].y, 0x7632)};
       mma16816<T>(acc.o[2 * g], a[0], a[1], a[2], a[3], ph[0], ph[1]);
-      mma16816<T>(acc.o[2 * g], a[0], a[1], a[2], a[3], pl[0], pl[1]);
       mma16816<T>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], ph[0], ph[1]);
-      mma16816<T>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], pl[0], pl[1]);
+      if constexpr (!FOLD) {
+        mma16816<T>(acc.o[2 * g], a[0], a[1], a[2], a[3], pl[0], pl[1]);
+        mma16816<T>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], pl[0], pl[1]);
+      }
     }
+  }
+  if constexpr (FOLD) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc.o[i][e] += __shfl_xor_sync(0xFFFFFFFFu, acc.o[i][e], 2);
   }
 
   // ---- the warps' parts to one: common maximum, then sums through shared memory
@@ -684,7 +703,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 // CTAs run at once and end together, and a piece may begin and end inside a head. Heads in several
 // pieces are joined from their parts (a CTA's first segment is its part 0, a later one its part 1), a
 // head inside one piece is written here.
-template <typename T, int D, bool MASS>
+template <typename T, int D, bool MASS, bool FOLD>
 __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(const __grid_constant__ Kv4Attn p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint4 frag[D];  // q's fragments: D / 32 groups of 32 lanes
@@ -765,7 +784,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
       }
       p.info[bh * hg + z] = info;
     }
-    kv4_segment<T, D, MASS>(p, smem, frag, bh, z, n, elen, u0, u1, slot);
+    kv4_segment<T, D, MASS, FOLD>(p, smem, frag, bh, z, n, elen, u0, u1, slot);
     left -= u1 - u0;
     start += u1 - u0;
     at += u1 - u0;
@@ -922,7 +941,7 @@ size_t kv4_attn_workspace(int64_t B, int64_t H, int64_t G, int64_t D, int64_t ca
   return static_cast<size_t>(kv4_plan(B, H, G, D, cap, W, mass, kv4_sms()).total);
 }
 
-template <typename T, int D, bool MASS>
+template <typename T, int D, bool MASS, bool FOLD>
 static cudaError_t kv4_start(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
   constexpr int RING = KV4_NW * KV4_STAGES * Kv4Stage<D>::BYTES, OUT = KV4_NW * 8 * (D + 4) * 4;
   constexpr int SMEM = RING > OUT ? RING : OUT;
@@ -932,17 +951,19 @@ static cudaError_t kv4_start(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const uint64_t bit = 1ull << (dev & 63);
   if (!(set.load() & bit)) {
-    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, MASS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    e = cudaFuncSetAttribute(kv4_attn_kernel<T, D, MASS, FOLD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     if (e != cudaSuccess) return e;
     set.fetch_or(bit);
   }
-  kv4_attn_kernel<T, D, MASS><<<static_cast<unsigned>(ctas), KV4_NW * 32, SMEM, st>>>(p);
+  kv4_attn_kernel<T, D, MASS, FOLD><<<static_cast<unsigned>(ctas), KV4_NW * 32, SMEM, st>>>(p);
   return cudaGetLastError();
 }
 
 template <typename T, int D>
 static cudaError_t kv4_run(const Kv4Attn& p, int64_t ctas, cudaStream_t st) {
-  const cudaError_t e = p.scores ? kv4_start<T, D, true>(p, ctas, st) : kv4_start<T, D, false>(p, ctas, st);
+  cudaError_t e;
+  if (p.G <= 4) e = p.scores ? kv4_start<T, D, true, true>(p, ctas, st) : kv4_start<T, D, false, true>(p, ctas, st);
+  else e = p.scores ? kv4_start<T, D, true, false>(p, ctas, st) : kv4_start<T, D, false, false>(p, ctas, st);
   if (e != cudaSuccess) return e;
   const int mass = p.scores ? static_cast<int>((p.sstride + KV4_MASS_KEYS - 1) / KV4_MASS_KEYS) : 0;
   cudaLaunchConfig_t cfg = {};
@@ -963,7 +984,6 @@ cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaSt
   const Kv4Plan w = kv4_plan(p.B, p.H, p.G, D, p.cap, p.W, mass, kv4_sms());
   p.splits = w.splits;
   p.pieces = w.pieces;
-  p.err = reinterpret_cast<int*>(ws);
   p.sstride = w.sstride;
   p.wcol = w.wcol;
   p.info = reinterpret_cast<int2*>(ws + w.info);

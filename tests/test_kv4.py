@@ -227,6 +227,50 @@ def test_attention(ops, case, gaps):
         assert torch.equal(got.cpu()[w == 0], was[w == 0])
 
 
+SHARED = [  # B, Hq, H, D, dtype, capacity, W: more work than one wave of pieces; more heads than pieces
+    (16, 32, 8, 128, "bf16", 1000, 100), (16, 8, 8, 64, "fp16", 1400, 33), (8, 48, 4, 128, "fp16", 3000, 0),
+    (8, 20, 4, 64, "bf16", 4700, 64), (60, 60, 30, 128, "bf16", 70, 5), (70, 210, 35, 64, "fp16", 33, 16),
+    (9, 8, 8, 64, "bf16", 3000, 16),
+]
+
+
+@gpu
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("case", SHARED, ids=str)
+def test_attention_with_many_heads(ops, case, ragged):
+    """Pieces that begin and end inside heads, and one piece a head."""
+    B, Hq, H, D, dt, cap, W = case
+    dtype = DT[dt]
+    hist, g = history(ops, B, H, cap, D, dt, cap + Hq)
+    counts = torch.randint(1, 9, (B, H, cap), generator=g).int()
+    lengths = torch.full((B, H), cap, dtype=torch.int32)
+    if ragged:
+        counts = torch.where(torch.rand(B, H, cap, generator=g) < 0.1, 0, counts).int()
+        lengths = torch.randint(0, cap + 1, (B, H), generator=g).int()
+        lengths[torch.rand(B, H, generator=g) < 0.3] = 0
+        lengths[1, 0], counts[1, 0] = cap, 0
+        lengths[2] = 1
+    q = (1.5 * torch.randn(B, Hq, D, generator=g)).to(dtype)
+    ke = torch.randn(B, H, W, D, generator=g).to(dtype) if W else None
+    ve = torch.randn(B, H, W, D, generator=g).to(dtype) if W else None
+    E = W - W // 3
+    mass, emass = torch.rand(B, H, cap, generator=g), torch.rand(B, H, W, generator=g)
+    m, em = mass.cuda(), emass.cuda()
+    dev = lambda t: None if t is None else t.cuda()  # noqa: E731
+    args = (dev(q), hist, dev(counts), dev(lengths), dev(ke), dev(ve))
+    out = ops.decode_attention_kv4(*args, exact_len=E, mass=m, exact_mass=em)
+    plain = ops.decode_attention_kv4(*args, exact_len=E)
+    k, v = values64(hist.k_codes, hist.k_scales), values64(hist.v_codes, hist.v_scales)
+    ref, wp, we = attend64(q, k, v, counts, lengths, ke, ve, E, D ** -0.5)
+    vmax = max(v.abs().max().item(), 0.0 if ve is None else ve.abs().max().item())
+    check_attend(out, ref, vmax, dtype)
+    check_attend(plain, ref, vmax, dtype)
+    for got, was, w in ((m, mass, wp), (em, emass, we)):
+        err = (got.cpu().double() - (was.double() + w)).abs()
+        assert (err <= 2.0 ** -14 * w + 2.0 ** -23 * got.cpu().abs()).all()
+        assert torch.equal(got.cpu()[w == 0], was[w == 0])
+
+
 @gpu
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
 def test_attention_masked_places_hold_anything(ops, dt):
@@ -487,6 +531,42 @@ def test_evict(ops, case):
             for got, want in zip((m, *rows), (mass, *was)):
                 a, w = got[b, h].cpu().contiguous(), want[b, h, kept].contiguous()
                 assert torch.equal(a.view(torch.uint8), w.view(torch.uint8))
+
+
+@gpu
+@pytest.mark.parametrize("B,H,cap,budget,first,recent,width", [
+    (10, 8, 20000, 9000, 4, 100, 1), (1, 1, 140001, 70000, 3, 64, 2), (1, 2, 900, 611, 0, 7, 1000), (2, 40, 600, 257, 1, 1, 1021)])
+def test_evict_long_heads_and_wide_rows(ops, B, H, cap, budget, first, recent, width):
+    """Heads longer than one pass of their CTAs holds, and entries of up to 4096 bytes with the mass."""
+    g = torch.Generator().manual_seed(cap)
+    mass = torch.rand(B, H, cap, generator=g).mul(4096).floor()  # ties too
+    n = torch.randint(cap - 300, cap + 1, (B, H), generator=g).int()
+    rows = [torch.arange(cap, dtype=torch.int32).expand(B, H, cap).contiguous().cuda(),
+            torch.randint(-9, 9, (B, H, cap, width), generator=g).int().cuda()]
+    was = [r.cpu().clone() for r in rows]
+    m, length = mass.cuda(), n.cuda()
+    ops.evict_by_mass(m, length, rows, budget, keep_first=first, keep_recent=recent)
+    assert (length == budget).all()
+    for b in range(B):
+        for h in range(H):
+            kept = evict64(mass[b, h], int(n[b, h]), budget, first, recent) + list(range(budget, cap))
+            for got, want in zip((m, *rows), (mass, *was)):
+                assert torch.equal(got[b, h].cpu(), want[b, h, kept])
+
+
+@gpu
+def test_evict_row_limit(ops):
+    """Rows of 4096 bytes are the widest."""
+    m, n = torch.rand(1, 1, 64, device="cuda"), torch.full((1, 1), 64, dtype=torch.int32, device="cuda")
+    row = torch.arange(64 * 1025, dtype=torch.int32, device="cuda").view(1, 1, 64, 1025)
+    with pytest.raises((ValueError, RuntimeError)):
+        ops.evict_by_mass(m, n, [row], 8)
+    assert int(n) == 64
+    row = row[..., :1024].contiguous()
+    kept = evict64(m[0, 0].cpu(), 64, 8, 0, 0)
+    want = row[0, 0, kept].clone()
+    ops.evict_by_mass(m, n, [row], 8)
+    assert int(n) == 8 and torch.equal(row[0, 0, :8], want)
 
 
 # ------------------------------------------------------------------------------------ refusals
