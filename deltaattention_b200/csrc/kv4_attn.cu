@@ -15,10 +15,14 @@
 //    (16-bit numbers 256 + code and 16 + code, the offsets taken off with the zeros, took two shifts,
 //    one product more and lost 4 bits of the sums; 8-bit float operands took a quarter longer: this
 //    matrix path converts them to fp16 first.)
-//  * Values: elements are the rows, q-heads the columns. A code in the mantissa of 16.0 is the bf16
-//    number 16 + code. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every
-//    weight); p alone, in two parts, times the stored (scales, zeros) gives what the 16 brought in
-//    and the zeros, added once at the end.
+//  * Values: elements are the rows, q-heads the columns, in bf16, whose range the scales need. Up to
+//    255 a byte is a bf16 number too, byte 2^-133, so again a shift and four ands give 8 operands.
+//    The weights carry 2^64, which keeps products in fp32's normal range: scales of 2^-40 to 2^54
+//    have it all. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every weight);
+//    p alone, in two parts, times the stored (scales, zeros) gives the zeros' share, added at the end.
+//    (Numbers 16 + code took a shift for every operand.)
+//    With up to 4 q-heads the columns 4 to 7 hold them again: the first parts go into columns 0 to 3,
+//    the rest into 4 to 7, and one product does for two.
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -33,6 +37,7 @@ constexpr int KV4_TILE = 32;   // keys per tile
 constexpr int KV4_STAGES = 2;  // tiles in a warp's ring
 constexpr int KV4_MAX_PIECES = 1024, KV4_MAX_HEADS = 2048;  // that are cut into pieces
 constexpr int KV4_MIN_UNITS = 8;  // of a piece: two tiles a warp
+constexpr int KV4_BIAS = 64;      // log2 of what history weights carry until they are joined with the window's
 constexpr float KV4_SLACK = 8.f;  // log2 units a score may exceed the running maximum by before it moves
 
 // one stage of a warp's ring
@@ -69,13 +74,6 @@ __device__ __forceinline__ float lg2(float x) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// 16 + code for the codes at bits 4 I.. of both halves of w, as a pair of bf16
-template <int I>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w) {
-  const uint32_t x = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (x & 0x00780078u) | 0x41804180u;
-}
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 __device__ __forceinline__ float lo_f32(uint32_t w) { return __uint_as_float(w << 16); }
@@ -151,7 +149,7 @@ template <int D>
 struct Kv4Acc {
   float m[2], l[2];
   float o[D / 16][4];  // [2 g + i / 2]: element 32 g + 4 (lane / 4) + i in [2 (i % 2) + head]
-  float sz[4];         // sums of p scale_g and p zero_g: value lane / 4 of the stored row in [0], [1]
+  float sz[4];         // sums of p zero_g: value lane / 4 of the stored row (scales, zeros) in [0], [1]
 
   __device__ __forceinline__ void init() {
     m[0] = m[1] = -INFINITY;
@@ -167,7 +165,7 @@ struct Kv4Acc {
   // Scores of 16 NT keys (lane: rows lane / 4 + 8 f of each 16, heads 2 t + e in [2 f + e]) to
   // weights. The maximum moves only when a score is KV4_SLACK above it: weights stay below
   // 2^KV4_SLACK, and the accumulators are hardly ever rescaled.
-  template <int NT>
+  template <int NT, int BIAS>
   __device__ __forceinline__ void weights(float (&z)[NT][4]) {
     float a = -INFINITY, b = -INFINITY;
 #pragma unroll
@@ -194,7 +192,7 @@ struct Kv4Acc {
       }
       sz[0] *= fa; sz[1] *= fb;
     }
-    const float ra = m[0] == -INFINITY ? 0.f : m[0], rb = m[1] == -INFINITY ? 0.f : m[1];
+    const float ra = (m[0] == -INFINITY ? 0.f : m[0]) - BIAS, rb = (m[1] == -INFINITY ? 0.f : m[1]) - BIAS;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -465,7 +463,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
       }
     };
     load_values(0);
-    acc.template weights<2>(zs);
+    acc.template weights<2, KV4_BIAS>(zs);
     // ---- values
     uint32_t ph[2][2], pl[2][2];  // weights of keys 2 t, 2 t + 1 (+ 8) for head lane / 4, two parts
 #pragma unroll
@@ -479,7 +477,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (i) load_values(1);
-      // sums of p scale and p zero: rows are the stored values (and again, for whole operands)
+      // sums of p zero: rows are the stored values (and again, for whole operands)
       using B = __nv_bfloat16;
       uint32_t v[4];
       if constexpr (NG == 4) {
@@ -504,8 +502,9 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
           else wl[f] = bfma2(pl[i][f], sc, bfms2(ph[i][f], sc, wh[f]));
           x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
         }
-        const uint32_t a[4] = {code_pair<0>(x[0]), code_pair<1>(x[0]), code_pair<0>(x[1]), code_pair<1>(x[1])};
-        const uint32_t d[4] = {code_pair<2>(x[0]), code_pair<3>(x[0]), code_pair<2>(x[1]), code_pair<3>(x[1])};
+        const uint32_t y[2] = {x[0] >> 8, x[1] >> 8};
+        const uint32_t a[4] = {x[0] & 0x000F000Fu, x[0] & 0x00F000F0u, x[1] & 0x000F000Fu, x[1] & 0x00F000F0u};
+        const uint32_t d[4] = {y[0] & 0x000F000Fu, y[0] & 0x00F000F0u, y[1] & 0x000F000Fu, y[1] & 0x00F000F0u};
         mma16816<B>(acc.o[2 * g], a[0], a[1], a[2], a[3], wh[0], wh[1]);
         mma16816<B>(acc.o[2 * g + 1], d[0], d[1], d[2], d[3], wh[0], wh[1]);
         if constexpr (!FOLD) {
@@ -518,32 +517,25 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   }
   cp_wait<0>();
 
-  // what the 16 of the codes brought in comes off, the zeros go on
-  if constexpr (FOLD) {  // in the columns of the first parts
+  // sums of codes to values: units and the weights' bias, then the zeros
+  constexpr float EVEN = 0x1p69f, ODD = 0x1p65f, UNBIAS = 0x1p-64f;
+  static_assert(KV4_BIAS == 64, "2^(133 - 64), 2^(129 - 64), 2^-64");
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+  for (int e = 0; e < 2; ++e) {
+    acc.l[e] *= UNBIAS;
+    if constexpr (FOLD) {  // in the columns of the first parts
       const float x = acc.sz[e] + __shfl_xor_sync(0xFFFFFFFFu, acc.sz[e], 2);
       acc.sz[e] = t < 2 ? x : 0.f;
     }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float z = __shfl_sync(0xFFFFFFFFu, acc.sz[e], 4 * (NG + g) + t) * UNBIAS;
+      acc.o[2 * g][e] = fmaf(acc.o[2 * g][e], EVEN, z);
+      acc.o[2 * g][2 + e] = fmaf(acc.o[2 * g][2 + e], ODD, z);
+      acc.o[2 * g + 1][e] = fmaf(acc.o[2 * g + 1][e], EVEN, z);
+      acc.o[2 * g + 1][2 + e] = fmaf(acc.o[2 * g + 1][2 + e], ODD, z);
+    }
   }
-  float sum_s[NG][2], sum_z[NG][2];
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      sum_s[g][e] = __shfl_sync(0xFFFFFFFFu, acc.sz[e], 4 * g + t);
-      sum_z[g][e] = __shfl_sync(0xFFFFFFFFu, acc.sz[e], 4 * (NG + g) + t);
-    }
-#pragma unroll
-  for (int g = 0; g < NG; ++g)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float off = fmaf(-16.f, sum_s[g][e], sum_z[g][e]);
-      acc.o[2 * g][e] += off;
-      acc.o[2 * g][2 + e] += off;
-      acc.o[2 * g + 1][e] += off;
-      acc.o[2 * g + 1][2 + e] += off;
-    }
 
   // ---- window rows, 16 at a time, straight from memory
   const T* ke = static_cast<const T*>(p.k_exact) + b * p.eb + h * p.eh;
@@ -586,7 +578,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
       zs[0][e] = ok ? s[e] * p.scale_log2 : -INFINITY;
       if (MASS && (e & 1 ? head1 : head0) && ok) sc0[(e & 1) * p.sstride + p.wcol + j0 + 8 * (e >> 1)] = zs[0][e];
     }
-    acc.template weights<1>(zs);
+    acc.template weights<1, 0>(zs);
     uint32_t ph[2], pl[2];
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
