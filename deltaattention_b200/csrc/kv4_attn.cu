@@ -113,12 +113,11 @@ __device__ __forceinline__ void lds_words(uint32_t* w, uint32_t at) {
   else
     w[0] = lds32(at);
 }
-template <bool TRANS>
-__device__ __forceinline__ void ldsm_x4(uint32_t* r, uint32_t at) {
-  if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t* r, uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
 }
 __device__ __forceinline__ void sts32(uint32_t at, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
@@ -202,13 +201,6 @@ struct Kv4Acc {
       }
   }
 };
-
-// the second part of p s, into x where `second` is set: x there holds the first part, p_hi s rounded
-__device__ __forceinline__ void second_part(uint32_t& x, uint32_t hi, uint32_t lo, uint32_t s, bool second) {
-  asm("{\n\t.reg .pred p;\n\t.reg .b32 n;\n\tsetp.ne.b32 p, %4, 0;\n\tneg.bf16x2 n, %0;\n\t"
-      "@p fma.rn.bf16x2 %0, %1, %3, n;\n\t@p fma.rn.bf16x2 %0, %2, %3, %0;\n\t}"
-      : "+r"(x) : "r"(hi), "r"(lo), "r"(s), "r"(static_cast<uint32_t>(second)));
-}
 
 // q of up to 8 heads as column fragments of the score product, and the coefficients of the stored
 // scales and zeros
@@ -305,13 +297,14 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   const int n4 = (n + KV4_TILE - 1) / KV4_TILE;
   const int64_t row0 = static_cast<int64_t>(bh) * p.G + h0;
 
-  // Shared-memory addresses of this lane, within a stage of its warp's ring; rows 8 and 16 further
+  // Shared-memory addresses of this lane in the first stage of its warp's ring; rows 8 and 16 further
   // have the same rotation (Kv4Stage::piece).
   constexpr int PPR = St::ROW / 16;  // 16-byte pieces per row
   const uint32_t ring = smem_u32(smem) + warp * (KV4_STAGES * St::BYTES);
-  const uint32_t k_at = St::K + (NG == 4 ? St::piece(gq, t) : St::piece(gq, t >> 1) + 8 * (t & 1));
-  const uint32_t v_at = St::V + (NG == 4 ? St::piece(2 * t, gq >> 1) : St::piece(2 * t, gq >> 2) + 8 * ((gq >> 1) & 1));
-  const uint32_t ks_at = St::KS + gq * St::SROW, vs_at = St::VS + 2 * t * St::SROW;
+  const uint32_t k_at = ring + St::K + (NG == 4 ? St::piece(gq, t) : St::piece(gq, t >> 1) + 8 * (t & 1));
+  const uint32_t v_at = ring + St::V + (NG == 4 ? St::piece(2 * t, gq >> 1) : St::piece(2 * t, gq >> 2) + 8 * ((gq >> 1) & 1));
+  const uint32_t ks_at = ring + St::KS + gq * St::SROW, vs_at = ring + St::VS + 2 * t * St::SROW;
+  const uint32_t vl_at = ring + St::VS + ((lane & 7) + ((lane >> 1) & 8)) * St::SROW;  // for ldmatrix
   const uint32_t zk_at = ks_at + 2 * NG + (NG == 4 ? 4 * (t & 1) : 0);  // a pair of zeros
   // A lane copies pieces lane + 32 i of a tile's codes (they are contiguous), its row's scales and
   // count.
@@ -381,16 +374,16 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
     cp_wait<KV4_STAGES - 2>();
     __syncwarp();  // and every lane has read the tile before this one: its stage may be filled again
     issue(stage == 0 ? KV4_STAGES - 1 : stage - 1);
-    const uint32_t sp = ring + stage * St::BYTES;
+    const uint32_t su = stage * St::BYTES;  // the last term of addresses: the same for all lanes
     // log2 of the counts; entries that take no part have -inf, and their scales, which may be
     // anything, are set to 0
-    const int32_t count = static_cast<int32_t>(lds32(sp + St::C + 4 * lane));
-    sts32(sp + St::C + 4 * lane, __float_as_uint(count > 0 ? lg2(static_cast<float>(count)) : -INFINITY));
+    const int32_t count = static_cast<int32_t>(lds32((ring + 4 * lane) + su + St::C));
+    sts32((ring + 4 * lane) + su + St::C, __float_as_uint(count > 0 ? lg2(static_cast<float>(count)) : -INFINITY));
     if (count <= 0) {
 #pragma unroll
       for (int i = 0; i < St::SROW / 4; ++i) {
-        sts32(sp + St::KS + lane * St::SROW + 4 * i, 0u);
-        sts32(sp + St::VS + lane * St::SROW + 4 * i, 0u);
+        sts32((ring + lane * St::SROW) + su + St::KS + 4 * i, 0u);
+        sts32((ring + lane * St::SROW) + su + St::VS + 4 * i, 0u);
       }
     }
     __syncwarp();
@@ -403,12 +396,12 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const int r = 16 * i + 8 * f;
-          lds_words<NG>(w[i][f], sp + k_at + r * St::ROW);
-          lds_words<NG / 2>(s2[i][f], sp + ks_at + r * St::SROW);
+          lds_words<NG>(w[i][f], k_at + su + r * St::ROW);
+          lds_words<NG / 2>(s2[i][f], ks_at + su + r * St::SROW);
         }
         uint32_t zw[2];  // pairs of zeros of both rows, the same for every part
 #pragma unroll
-        for (int f = 0; f < 2; ++f) zw[f] = lds32(sp + zk_at + (16 * i + 8 * f) * St::SROW);
+        for (int f = 0; f < 2; ++f) zw[f] = lds32(zk_at + su + (16 * i + 8 * f) * St::SROW);
         mma16816_set<__nv_bfloat16>(zs[i], zw[0], zw[1], zw[0], zw[1], q.zc[0], q.zc[1]);
       }
 #pragma unroll
@@ -441,7 +434,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        const float lg = __uint_as_float(lds32(sp + 4 * gq + St::C + 64 * i + 32 * f));
+        const float lg = __uint_as_float(lds32((ring + 4 * gq) + su + St::C + 64 * i + 32 * f));
         zs[i][2 * f] = fmaf(zs[i][2 * f], q.back[0], lg);
         zs[i][2 * f + 1] = fmaf(zs[i][2 * f + 1], q.back[1], lg);
       }
@@ -458,8 +451,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 16 * i + (k & 1) + 8 * (k >> 1);
-        lds_words<NG>(w[k], sp + v_at + r * St::ROW);
-        lds_words<NG / 2>(s[k], sp + vs_at + r * St::SROW);
+        lds_words<NG>(w[k], v_at + su + r * St::ROW);
+        lds_words<NG / 2>(s[k], vs_at + su + r * St::SROW);
       }
     };
     load_values(0);
@@ -481,10 +474,10 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
       using B = __nv_bfloat16;
       uint32_t v[4];
       if constexpr (NG == 4) {
-        ldsm_x4<true>(v, sp + St::VS + ((lane & 7) + ((lane >> 1) & 8)) * St::SROW + 16 * i * St::SROW);
+        ldsm_x4_trans(v, vl_at + su + 16 * i * St::SROW);
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = lds16(sp + vs_at + 2 * (gq & 3) + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW);
+        for (int k = 0; k < 4; ++k) v[k] = lds16(vs_at + su + 2 * (gq & 3) + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW);
         v[0] = v[1] = prmt(v[0], v[1], 0x5410);
         v[2] = v[3] = prmt(v[2], v[3], 0x5410);
       }
@@ -498,8 +491,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         for (int f = 0; f < 2; ++f) {
           const uint32_t sc = prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u);
           wh[f] = bmul2(ph[i][f], sc);
-          if constexpr (FOLD) second_part(wh[f], ph[i][f], pl[i][f], sc, second);
-          else wl[f] = bfma2(pl[i][f], sc, bfms2(ph[i][f], sc, wh[f]));
+          wl[f] = bfma2(pl[i][f], sc, bfms2(ph[i][f], sc, wh[f]));
+          if constexpr (FOLD) wh[f] = second ? wl[f] : wh[f];
           x[f] = prmt(w[2 * f][g], w[2 * f + 1][g], half);
         }
         const uint32_t y[2] = {x[0] >> 8, x[1] >> 8};

@@ -301,6 +301,25 @@ def test_attention_masked_places_hold_anything(ops, dt):
 
 
 @gpu
+@pytest.mark.parametrize("G", [2, 6])
+@pytest.mark.parametrize("qs,vs", [(2.0 ** -100, 1.0), (0.0, 1.0), (2.0 ** 30, 1.0), (1.0, 2.0 ** 40), (1.0, 2.0 ** -30)])
+def test_attention_ranges(ops, G, qs, vs):
+    """Queries and values of sizes far from one; the scores' size is put right by sm_scale."""
+    B, H, D, cap, W = 1, 2, 128, 777, 20
+    g = torch.Generator().manual_seed(31)
+    k, v = torch.randn(B, H, cap, D, generator=g), torch.randn(B, H, cap, D, generator=g) * vs
+    hist = ops.kv4_quantize(k.bfloat16().cuda(), v.bfloat16().cuda())
+    counts, lengths = torch.randint(1, 9, (B, H, cap), generator=g).int(), torch.tensor([[777, 300]], dtype=torch.int32)
+    q = (torch.randn(B, G * H, D, generator=g) * qs).bfloat16()
+    ke, ve = torch.randn(B, H, W, D, generator=g).bfloat16(), (torch.randn(B, H, W, D, generator=g) * vs).bfloat16()
+    scale = D ** -0.5 / (qs if qs > 0 else 1.0)
+    out = ops.decode_attention_kv4(q.cuda(), hist, counts.cuda(), lengths.cuda(), ke.cuda(), ve.cuda(), sm_scale=scale)
+    vv = values64(hist.v_codes, hist.v_scales)
+    ref, _, _ = attend64(q, values64(hist.k_codes, hist.k_scales), vv, counts, lengths, ke, ve, W, scale)
+    check_attend(out, ref, max(vv.abs().max().item(), ve.abs().max().item()), torch.bfloat16)
+
+
+@gpu
 def test_attention_extreme_scores(ops):
     """One entry far above the others, after and before them, and scores far below zero."""
     B, H, D, cap = 1, 1, 64, 400
