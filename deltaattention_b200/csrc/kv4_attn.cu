@@ -683,6 +683,15 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   __syncthreads();  // the ring may be filled again
 }
 
+// Bound by what the SMs issue: 16 keys take a warp about 310 instructions, 18 of them products, which
+// hold up the other pipes too, so that about half the issue slots are used. Copies wait for nobody:
+// with all tiles from one address the time falls by 8 %. 12 warps an SM of 168 registers; 16 of 128
+// registers spill and take 7 % longer, a ring of 3 tiles changes nothing. bf16, d = 128, 4 q-heads
+// per kv-head, device times with the join:
+//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 74 us, 4.7 TB/s
+//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 35.5 us, with mass 42 us
+//   1 sequence of 8192 entries: 12.4 us, most of it the latencies of two launches
+//
 // With `splits` every head is cut into that many pieces (as many as it has units). Otherwise the
 // units of all heads in a row are cut into even pieces, one per CTA, whatever the heads' lengths: all
 // CTAs run at once and end together, and a piece may begin and end inside a head. Heads in several
@@ -783,7 +792,9 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
 
 // ---------------------------------------------------------------------------------- joining
 // Launched while the attention kernel ends (programmatic dependent launch): grid_wait returns once
-// that kernel's writes are there.
+// that kernel's writes are there. Joining is a chain of dependent reads (the head's parts, their
+// maxima and sums, their outputs), 6.8 us alone. The mass reads the scores again and adds 6 us for 16
+// sequences of 1024 to 8192 entries: 4 G bytes a key written and read, where a key has 5 D / 4.
 // blockIdx.y: kv-head. The first G CTAs join the parts of one q-head each and write its output;
 // the others add the weights of 1024 entries each (history, then window) to their mass.
 constexpr int KV4_MASS_KEYS = 1024;
@@ -975,7 +986,7 @@ cudaError_t launch_kv4_attn(int dtype, int64_t D, Kv4Attn p, uint8_t* ws, cudaSt
   p.row_stats = reinterpret_cast<float2*>(ws + w.row_stats);
   p.stats = reinterpret_cast<float2*>(ws + w.stats);
   p.part = reinterpret_cast<float*>(ws + w.part);
-  p.used = reinterpret_cast<int*>(ws + 64);
+  p.used = reinterpret_cast<int*>(ws);
   p.scores = mass ? reinterpret_cast<float*>(ws + w.scores) : nullptr;
   if (dtype == BF16) return D == 64 ? kv4_run<__nv_bfloat16, 64>(p, w.ctas, st) : kv4_run<__nv_bfloat16, 128>(p, w.ctas, st);
   return D == 64 ? kv4_run<__half, 64>(p, w.ctas, st) : kv4_run<__half, 128>(p, w.ctas, st);

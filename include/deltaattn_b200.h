@@ -375,7 +375,7 @@ int dab_decode_update_kv4(const void* k_new, const void* v_new, void* k_codes, v
                           const int64_t* strides, float threshold, int use_cosine, int dtype, int64_t batch,
                           int64_t heads, int64_t head_dim, int64_t capacity, int64_t exact_window, int* err_word,
                           void* stream);
-/* Scratch bytes dab_decode_attention_kv4 needs. Zero it once, then reuse it on one stream. */
+/* Scratch bytes dab_decode_attention_kv4 needs, whatever they hold; used on one stream at a time. */
 size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim,
                                                int64_t capacity, int64_t exact_window, int with_mass);
 /* Single-token attention over a 4-bit history and the exact window: q / out [B, heads * kv_group,
@@ -383,7 +383,9 @@ size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int
  * with a positive count (others draw nothing, whatever they hold) and sm_scale * q . k over the
  * first exact_len window rows. A query row with no entry left gives 0. With `mass` (fp32, else
  * NULL) every entry's attention weight, summed over the kv-head's q-heads, is added to mass and
- * exact_mass. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
+ * exact_mass. Weights are held in 16 bits or more, sums in 32; elements of a query row below 2^-26
+ * of its largest are rounded to that step, and scales of values outside 2^-40 .. 2^54 lose
+ * precision or overflow. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
  * and `advance` as in dab_decode_attention_dev; without it exact_len is the argument.
  * `strides` (17): q (b, h), out (b, h), codes (b, h), scales (b, h), counts / mass (b, h), lengths
  * (b, h), exact K / V (b, h, row), exact_mass (b, h). Query and exact rows contiguous, 16-byte
