@@ -689,8 +689,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 // registers spill and take 7 % longer, a ring of 3 tiles changes nothing. bf16, d = 128, 4 q-heads
 // per kv-head, device times with the join:
 //   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 74 us, 4.7 TB/s
-//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 35.5 us, with mass 42 us
-//   1 sequence of 8192 entries: 12.4 us, most of it the latencies of two launches
+//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 33 us, with mass 39 us
+//   1 sequence of 8192 entries: 12 us, most of it the latencies of two launches
 //
 // With `splits` every head is cut into that many pieces (as many as it has units). Otherwise the
 // units of all heads in a row are cut into even pieces, one per CTA, whatever the heads' lengths: all
@@ -705,6 +705,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   __shared__ int lens[KV4_MAX_HEADS];
   __shared__ int s_bh, s_at;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hg = (p.G + 7) / 8;
+  grid_next();  // the joining CTAs take the places that ending CTAs leave, and wait there for the last
   int elen = p.exact_len;
   if (p.state) elen = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.W), p.state[0] + p.lag)));
   if (p.state && blockIdx.x == 0 && tid == 0) *p.used = elen;
@@ -787,14 +788,14 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
       ++bh;
     }
   }
-  grid_next();
 }
 
 // ---------------------------------------------------------------------------------- joining
 // Launched while the attention kernel ends (programmatic dependent launch): grid_wait returns once
 // that kernel's writes are there. Joining is a chain of dependent reads (the head's parts, their
 // maxima and sums, their outputs), 6.8 us alone. The mass reads the scores again and adds 6 us for 16
-// sequences of 1024 to 8192 entries: 4 G bytes a key written and read, where a key has 5 D / 4.
+// sequences of 1024 to 8192 entries: 4 G bytes a key written and read, where a key has 5 D / 4. Four
+// q-heads at a time keep enough of its CTAs resident (eight at a time: 1.6 us more).
 // blockIdx.y: kv-head. The first G CTAs join the parts of one q-head each and write its output;
 // the others add the weights of 1024 entries each (history, then window) to their mass.
 constexpr int KV4_MASS_KEYS = 1024;
@@ -822,7 +823,7 @@ __device__ __forceinline__ float2 row_stats(const Kv4Attn& p, int64_t row, int h
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4Attn p) {
-  __shared__ float2 st[8];
+  __shared__ float2 st[4];
   __shared__ float wgt[KV4_MAX_PIECES];
   __shared__ float red[256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hg = (p.G + 7) / 8;
@@ -867,21 +868,21 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
   const int elen = p.state ? *p.used : p.exact_len, j = key - p.wcol;
   if (k0 >= max(n, p.wcol + elen)) return;
   const bool some = key < n || (j >= 0 && j < elen);
-  for (int g0 = 0; g0 < p.G; g0 += 8) {
-    const int ng = min(8, p.G - g0);
+  for (int g0 = 0; g0 < p.G; g0 += 4) {
+    const int ng = min(4, p.G - g0);
     const int64_t row = static_cast<int64_t>(bh) * p.G + g0;
-    float4 sc[8];
+    float4 sc[4];
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
+    for (int g = 0; g < 4; ++g)
       if (g < ng && some) sc[g] = *reinterpret_cast<const float4*>(p.scores + (row + g) * p.sstride + key);
     if (g0) __syncthreads();
     if (warp < ng) {
-      const float2 r = row_stats(p, row + warp, warp, p.info[bh * hg + g0 / 8], lane);
+      const float2 r = row_stats(p, row + warp, (g0 & 4) + warp, p.info[bh * hg + g0 / 8], lane);
       if (lane == 0) st[warp] = r;
     }
     __syncthreads();
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
+    for (int g = 0; g < 4; ++g)
       if (g < ng && some) {
         w[0] = fmaf(ex2(sc[g].x - st[g].x), st[g].y, w[0]);
         w[1] = fmaf(ex2(sc[g].y - st[g].x), st[g].y, w[1]);
