@@ -803,19 +803,34 @@ constexpr int KV4_MASS_KEYS = 1024;
 // part k of a row whose first part and last piece are `info`: part 0 of piece after piece
 __device__ __forceinline__ int64_t part_of(int2 info, int k) { return k == 0 ? info.x : (info.x / 2 + k) * int64_t{2}; }
 
-// (max, 1 / sum) of a row, by one warp; 1 / sum is 0 where nothing is left
+// (max, 1 / sum) of a row, by one warp; 1 / sum is 0 where nothing is left. A lane has the loads of 8
+// parts in flight.
 __device__ __forceinline__ float2 row_stats(const Kv4Attn& p, int64_t row, int head, int2 info, int lane) {
   if (info.x < 0) return p.row_stats[row];
   const int parts = info.y - info.x / 2 + 1;
   float m = -INFINITY, l = 0.f;
-  for (int k = lane; k < parts; k += 32) m = fmaxf(m, p.stats[part_of(info, k) * 8 + head].x);
+  for (int k0 = 0; k0 < parts; k0 += 256) {
+    float2 s[8];
+    float top = m;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-  const float ref = m == -INFINITY ? 0.f : m;
-  for (int k = lane; k < parts; k += 32) {
-    const float2 s = p.stats[part_of(info, k) * 8 + head];
-    l = fmaf(s.y, ex2(s.x - ref), l);
+    for (int j = 0; j < 8; ++j) {
+      const int k = k0 + 32 * j + lane;
+      s[j] = make_float2(-INFINITY, 0.f);
+      if (k < parts) s[j] = p.stats[part_of(info, k) * 8 + head];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    l *= ex2(m - ref);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) l = fmaf(s[j].y, ex2(s[j].x - ref), l);
+    m = top;
   }
+  float all = m;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+  const float ref = all == -INFINITY ? 0.f : all;
+  l *= ex2(m - ref);
 #pragma unroll
   for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
   return make_float2(ref, l == 0.f ? 0.f : 1.f / l);
@@ -824,8 +839,7 @@ __device__ __forceinline__ float2 row_stats(const Kv4Attn& p, int64_t row, int h
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4Attn p) {
   __shared__ float2 st[4];
-  __shared__ float wgt[KV4_MAX_PIECES];
-  __shared__ float red[256];
+  __shared__ float4 red[256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hg = (p.G + 7) / 8;
   const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   if (static_cast<int>(blockIdx.x) < p.G) {
@@ -837,22 +851,30 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
     }
     const int2 info = p.info[bh * hg + blockIdx.x / 8];
     if (info.x < 0) return;  // written already
+    // a part's row is read by D / 4 lanes, and every warp works out the row's maximum and sum
+    constexpr int LANES = D / 4, ROWS = 256 / LANES;
     const int parts = info.y - info.x / 2 + 1, head = blockIdx.x & 7;
-    if (warp == 0) {
-      const float2 r = row_stats(p, 0, head, info, lane);
-      for (int k = lane; k < parts; k += 32) wgt[k] = ex2(p.stats[part_of(info, k) * 8 + head].x - r.x) * r.y;
-    }
-    __syncthreads();
-    const int d = threadIdx.x % D;
-    float a = 0.f;
+    const int d = threadIdx.x % LANES, first = threadIdx.x / LANES;
+    const float2 r = row_stats(p, 0, head, info, lane);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int k = threadIdx.x / D; k < parts; k += 256 / D) a = fmaf(p.part[(part_of(info, k) * 8 + head) * D + d], wgt[k], a);
+    for (int k = first; k < parts; k += ROWS) {
+      const int64_t at = part_of(info, k) * 8 + head;
+      const float w = ex2(p.stats[at].x - r.x) * r.y;
+      const float4 x = *reinterpret_cast<const float4*>(p.part + at * D + 4 * d);
+      a.x = fmaf(x.x, w, a.x);
+      a.y = fmaf(x.y, w, a.y);
+      a.z = fmaf(x.z, w, a.z);
+      a.w = fmaf(x.w, w, a.w);
+    }
     red[threadIdx.x] = a;
     __syncthreads();
     if (threadIdx.x < D) {
+      const float* e = reinterpret_cast<const float*>(red) + threadIdx.x;
+      float sum = 0.f;
 #pragma unroll
-      for (int i = 1; i < 256 / D; ++i) a += red[threadIdx.x + i * D];
-      static_cast<T*>(p.out)[b * p.ob + (static_cast<int64_t>(h) * p.G + blockIdx.x) * p.oh + d] = from_f32<T>(a);
+      for (int i = 0; i < ROWS; ++i) sum += e[i * D];
+      static_cast<T*>(p.out)[b * p.ob + (static_cast<int64_t>(h) * p.G + blockIdx.x) * p.oh + threadIdx.x] = from_f32<T>(sum);
     }
     return;
   }
