@@ -37,6 +37,7 @@ constexpr int KV4_TILE = 32;   // keys per tile
 constexpr int KV4_STAGES = 2;  // tiles in a warp's ring
 constexpr int KV4_MAX_PIECES = 1024, KV4_MAX_HEADS = 2048;  // that are cut into pieces
 constexpr int KV4_MIN_UNITS = 8;  // of a piece: two tiles a warp
+constexpr int KV4_START = 6;      // units that beginning and ending a head costs as much as
 constexpr int KV4_BIAS = 64;      // log2 of what history weights carry until they are joined with the window's
 constexpr float KV4_SLACK = 8.f;  // log2 units a score may exceed the running maximum by before it moves
 
@@ -728,7 +729,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     for (int k = tid; k < heads; k += KV4_NW * 32) lens[k] = kv4_len(p, k);
     __syncthreads();
     int64_t mine = 0;
-    for (int k = tid * per; k < min(heads, (tid + 1) * per); ++k) mine += kv4_units(lens[k], elen);
+    for (int k = tid * per; k < min(heads, (tid + 1) * per); ++k) mine += kv4_units(lens[k], elen) + KV4_START;
     mine *= hg;
     int64_t incl = mine;
 #pragma unroll
@@ -754,7 +755,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
       int k = tid * per;
       int64_t pos = first;
       while (true) {
-        const int64_t u = static_cast<int64_t>(hg) * kv4_units(lens[k], elen);
+        const int64_t u = static_cast<int64_t>(hg) * (kv4_units(lens[k], elen) + KV4_START);
         if (start < pos + u) break;
         pos += u;
         ++k;
@@ -766,24 +767,30 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     bh = s_bh;
     at = s_at;
   }
-  for (int part = 0; left > 0; part = 1) {
-    const int n = p.splits ? kv4_len(p, bh) : lens[bh], un = kv4_units(n, elen), z = at / un;
-    const int u0 = at - z * un, u1 = min(un, u0 + left);
-    int slot = -1;
-    if (u1 - u0 < un) slot = blockIdx.x * 2 + part;
-    if (u0 == 0 && tid == 0) {
-      // the head's first part and its last piece; -1: no parts
-      int2 info = make_int2(-1, 0);
-      if (slot >= 0) {
-        info = make_int2(slot, p.splits ? static_cast<int>(blockIdx.x) + ns - 1 : static_cast<int>((start + un - 1) / piece));
+  const int ahead = p.splits ? 0 : KV4_START;  // units before a head's first that stand for its cost
+  for (int part = 0; left > 0;) {
+    const int n = p.splits ? kv4_len(p, bh) : lens[bh], un = kv4_units(n, elen), z = at / (un + ahead);
+    const int v0 = at - z * (un + ahead), v1 = min(un + ahead, v0 + left);
+    const int u0 = max(0, v0 - ahead), u1 = v1 - ahead;
+    if (u0 < u1) {
+      int slot = -1;
+      if (u1 - u0 < un) slot = blockIdx.x * 2 + part;
+      if (u0 == 0 && tid == 0) {
+        // the head's first part and its last piece; -1: no parts
+        int2 info = make_int2(-1, 0);
+        if (slot >= 0) {
+          info = make_int2(slot, p.splits ? static_cast<int>(blockIdx.x) + ns - 1
+                                          : static_cast<int>((start - v0 + ahead + un - 1) / piece));
+        }
+        p.info[bh * hg + z] = info;
       }
-      p.info[bh * hg + z] = info;
+      kv4_segment<T, D, MASS, FOLD>(p, smem, frag, bh, z, n, elen, u0, u1, slot);
+      part = 1;
     }
-    kv4_segment<T, D, MASS, FOLD>(p, smem, frag, bh, z, n, elen, u0, u1, slot);
-    left -= u1 - u0;
-    start += u1 - u0;
-    at += u1 - u0;
-    if (at == hg * un) {
+    left -= v1 - v0;
+    start += v1 - v0;
+    at += v1 - v0;
+    if (at == hg * (un + ahead)) {
       at = 0;
       ++bh;
     }
