@@ -123,6 +123,9 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t* r, uint32_t at) {
 __device__ __forceinline__ void sts32(uint32_t at, uint32_t v) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t v) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(static_cast<uint16_t>(v)) : "memory");
+}
 __device__ __forceinline__ uint32_t movm(uint32_t x) {  // transpose of an 8 x 8 fragment of 16-bit numbers
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -367,6 +370,11 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   acc.init();
   float* sc0 = MASS ? p.scores + (row0 + 2 * t) * p.sstride + gq : nullptr;
   const uint32_t frag_at = smem_u32(frag + lane);
+  // A tile's value scales by group, in the order in which lanes want them: a lane's keys 2 t, 2 t + 1,
+  // 2 t + 8, 2 t + 9 of each 16 (the lane of a key writes them; 8 selections a lane and 16 keys saved)
+  __shared__ __align__(16) uint8_t turned[KV4_NW * NG * 64];
+  const uint32_t turn = smem_u32(turned) + warp * (NG * 64), turn_r = turn + 16 * t;
+  const uint32_t turn_w = turn + 8 * (lane & 6) + 8 * (lane >> 4) + 4 * ((lane >> 3) & 1) + 2 * (lane & 1);
   const bool head0 = 2 * t < ng, head1 = 2 * t + 1 < ng;
   const bool second = FOLD && gq >= 4;  // this lane's column takes the second parts
 
@@ -380,6 +388,10 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
     // anything, are set to 0
     const int32_t count = static_cast<int32_t>(lds32((ring + 4 * lane) + su + St::C));
     sts32((ring + 4 * lane) + su + St::C, __float_as_uint(count > 0 ? lg2(static_cast<float>(count)) : -INFINITY));
+    uint32_t own[NG / 2];
+    lds_words<NG / 2>(own, ring + lane * St::SROW + su + St::VS);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) sts16(turn_w + g * 64, count > 0 ? (g & 1 ? own[g >> 1] >> 16 : own[g >> 1]) : 0u);
     if (count <= 0) {
 #pragma unroll
       for (int i = 0; i < St::SROW / 4; ++i) {
@@ -445,16 +457,17 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         if (head1) { o[p.sstride] = zs[i][1]; o[p.sstride + 8] = zs[i][3]; }
       }
     }
-    // value codes and scales of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9; those of the first 16 keys are
-    // loaded before the exponentials, which hide the latency
-    uint32_t w[4][NG], s[4][NG / 2];
+    // value codes of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 and their scales in pairs; those of the first
+    // 16 keys are loaded before the exponentials, which hide the latency
+    uint32_t w[4][NG], s[NG][2];
     auto load_values = [&](int i) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int r = 16 * i + (k & 1) + 8 * (k >> 1);
         lds_words<NG>(w[k], v_at + su + r * St::ROW);
-        lds_words<NG / 2>(s[k], vs_at + su + r * St::SROW);
       }
+#pragma unroll
+      for (int g = 0; g < NG; ++g) lds_words<2>(s[g], turn_r + g * 64 + 8 * i);
     };
     load_values(0);
     acc.template weights<2, KV4_BIAS>(zs);
@@ -490,7 +503,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         uint32_t wh[2], wl[2], x[2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const uint32_t sc = prmt(s[2 * f][g >> 1], s[2 * f + 1][g >> 1], g & 1 ? 0x7632u : 0x5410u);
+          const uint32_t sc = s[g][f];
           wh[f] = bmul2(ph[i][f], sc);
           wl[f] = bfma2(pl[i][f], sc, bfms2(ph[i][f], sc, wh[f]));
           if constexpr (FOLD) wh[f] = second ? wl[f] : wh[f];

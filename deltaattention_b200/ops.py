@@ -820,8 +820,8 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
 
     With ``mass`` [B, Hkv, capacity] and ``exact_mass`` [B, Hkv, W] (fp32), every entry's attention
     weight, summed over the q-heads of its kv-head, is added to them: what ``evict_by_mass`` goes
-    by. ``workspace`` (uint8, zero-filled once, ``kv4_attention_workspace`` bytes, used by one
-    stream at a time) replaces the library's own. Returns out [B, Hq, d]."""
+    by. ``workspace`` (uint8, ``kv4_attention_workspace`` bytes of any content, used by one stream
+    at a time) replaces the library's own. Returns out [B, Hq, d]."""
     what = "decode_attention_kv4"
     (B, H, cap, D), hs = hist.check(what, q)
     dev = L.same_device(what, q, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
@@ -900,11 +900,11 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
     the largest ``mass`` [B, H, capacity] (fp32; ties go to the lowest index, NaN is the lightest).
     Entries keep their order; mass and every tensor of ``rows`` ([B, H, capacity, ...], up to 8,
     contiguous from the third dimension on, entries of a multiple of 4 bytes, 4096 bytes together)
-    move together, and
-    ``lengths`` [B, H] (int32) become ``budget``. Slots from ``budget`` on keep what they held.
+    move together, and ``lengths`` [B, H] (int32) become ``budget``. Slots from ``budget`` on keep what they held.
     Lengths are read on the device: no host synchronisation, and the call can be captured in a
     CUDA graph and replayed at every token, where it only does work once a head passes
-    ``trigger``. ``workspace`` as in ``decode_attention_kv4`` (``evict_workspace`` bytes)."""
+    ``trigger``. ``workspace`` (uint8, ``evict_workspace`` bytes, zero-filled once, used by one
+    stream at a time) replaces the library's own."""
     what = "evict_by_mass"
     L.same_device(what, mass, lengths, workspace, *rows)
     size = mass.shape
