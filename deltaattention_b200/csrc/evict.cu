@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
       if (r < rank) { base_s += v.x; base_t += v.y; }
     }
   }
-  int* first = p.first_tile + static_cast<int64_t>(bh) * p.max_tiles;
+  uint4* begins = p.begins + static_cast<int64_t>(bh) * p.max_tiles;
   for (int t = t0; t < t1; t += SEL_THREADS) {  // kept and ties before every tile; where result tiles begin
     const int u = t + tid;
     uint2 v = make_uint2(0u, 0u), w = make_uint2(run_s, run_t);
@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
     if (u < t1) {
       const uint32_t at = base_s + v.x + min(base_t + v.y, k), end = base_s + w.x + min(base_t + w.y, k);
       before[u] = make_uint2(at, base_t + v.y);
-      for (uint32_t d = (at + p.tile - 1) >> p.tile_shift; (d << p.tile_shift) < end; ++d) first[d] = u;
+      for (uint32_t d = (at + p.tile - 1) >> p.tile_shift; (d << p.tile_shift) < end; ++d)
+        begins[d] = make_uint4(u, at, base_t + v.y, 0u);
     }
     __syncthreads();
   }
@@ -283,26 +284,62 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
   if (n == 0) return;  // left alone
   const int tile = s_tile, d0 = tile << p.tile_shift, rows_n = min(p.tile, p.budget - d0);
   const uint2* before = p.before + static_cast<int64_t>(bh) * p.max_tiles;
-  const int from = p.first_tile[static_cast<int64_t>(bh) * p.max_tiles + tile];
+  const uint4 f = p.begins[static_cast<int64_t>(bh) * p.max_tiles + tile];
+  const int from = static_cast<int>(f.x);
   // the tiles of the result that come from the entries this one overwrites: from the `on`th to `upto`
   const int on = static_cast<int>(before[tile].x) >> p.tile_shift;
   const int next = tile + 1 < (n + p.tile - 1) >> p.tile_shift ? static_cast<int>(before[tile + 1].x) : p.budget;
   const int upto = max(static_cast<int>(before[tile].x), next - 1) >> p.tile_shift;
-  // the kept entries d0, d0 + 1, .. of the result, 32 source entries a thread
+  // the kept entries d0, d0 + 1, .. of the result, from words of 32 source entries
+  static_assert(MOVE_THREADS == 256, "eight warps");
   int* src = reinterpret_cast<int*>(mv_smem);
-  uint2 at = before[from];
+  uint2 at = make_uint2(f.y, f.z);  // kept entries of both kinds before the first word of a round
   const uint2* words = p.words + static_cast<int64_t>(bh) * p.max_words;
   const int nw = (n + 31) / 32;
-  for (int w0 = (from << p.tile_shift) / 32; static_cast<int>(at.x) < d0 + rows_n && w0 < nw; w0 += MOVE_THREADS) {
-    uint2 w = make_uint2(0u, 0u);
-    if (w0 + tid < nw) w = words[w0 + tid];
-    uint2 x = make_uint2(__popc(w.x), __popc(w.y));
-    const uint2 own = x;
+  int w0 = (from << p.tile_shift) / 32;
+  auto word = [&](int i) { return i < nw ? words[i] : make_uint2(0u, 0u); };
+  auto sums = [&](uint2 x) {  // up to and with this lane's
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t s = __shfl_up_sync(0xFFFFFFFFu, x.x, o), q = __shfl_up_sync(0xFFFFFFFFu, x.y, o);
       if (lane >= o) { x.x += s; x.y += q; }
     }
+    return x;
+  };
+  // word `base` + lane, with `pre` (surely kept, ties) before it in the round; `mine`: words to write out
+  auto place = [&](uint2 w, uint2 pre, int base, uint32_t mine) {
+    // of its ties the lowest are kept, as long as fewer than `need` came before
+    const uint32_t ties = __popc(w.y), t0 = at.y + pre.y;
+    const uint32_t keep = min(t0 + ties, need) - min(t0, need);
+    const uint32_t bits = w.x | (keep == ties ? w.y : keep == 0 ? 0u : w.y & ((1u << __fns(w.y, 0, keep + 1)) - 1u));
+    const int pos = static_cast<int>(at.x + pre.x + min(t0, need) - min(at.y, need)) - d0;
+    uint32_t some = __ballot_sync(0xFFFFFFFFu, bits && pos < rows_n && pos + __popc(bits) > 0);
+#pragma unroll 1
+    for (some &= mine; some; some &= some - 1) {  // a lane a bit
+      const int l = __ffs(some) - 1;
+      const uint32_t wb = __shfl_sync(0xFFFFFFFFu, bits, l);
+      const int wp = __shfl_sync(0xFFFFFFFFu, pos, l) + __popc(wb & ((1u << lane) - 1u));
+      if ((wb >> lane & 1u) && wp >= 0 && wp < rows_n) src[wp] = (base + l) * 32 + lane;
+    }
+  };
+  auto pass = [&](uint2 all) {
+    at.x += all.x + min(at.y + all.y, need) - min(at.y, need);
+    at.y += all.y;
+  };
+  auto more = [&] { return static_cast<int>(at.x) < d0 + rows_n && w0 < nw; };
+  // Two rounds of 32 words, by every warp alike and without a barrier, are enough where one entry in
+  // eight or more is kept; after them 256 words a round.
+  uint2 w = word(w0 + lane), ahead = word(w0 + 32 + lane);
+#pragma unroll 1
+  for (int round = 0; round < 2 && more(); ++round, w0 += 32, w = ahead) {
+    const uint2 own = make_uint2(__popc(w.x), __popc(w.y)), x = sums(own);
+    place(w, make_uint2(x.x - own.x, x.y - own.y), w0, 0x01010101u << warp);
+    pass(make_uint2(__shfl_sync(0xFFFFFFFFu, x.x, 31), __shfl_sync(0xFFFFFFFFu, x.y, 31)));
+  }
+#pragma unroll 1
+  for (; more(); w0 += MOVE_THREADS) {
+    w = word(w0 + tid);
+    const uint2 own = make_uint2(__popc(w.x), __popc(w.y)), x = sums(own);
     __syncthreads();
     if (lane == 31) wsum[warp] = x;
     __syncthreads();
@@ -314,22 +351,8 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
       all.x += y.x;
       all.y += y.y;
     }
-    // ties kept before this thread's, and of its own the lowest
-    const uint32_t t0 = at.y + pre.y, t_all = min(t0, need) - min(at.y, need);
-    const uint32_t mine = min(t0 + own.y, need) - min(t0, need);
-    uint32_t bits = w.x | (mine == own.y ? w.y : mine == 0 ? 0u : w.y & ((1u << __fns(w.y, 0, mine + 1)) - 1u));
-    // `at` counts kept entries of both kinds before the first word
-    int pos = static_cast<int>(at.x + pre.x + t_all) - d0;
-    // a warp writes out its words one after another, a lane a bit
-#pragma unroll 1
-    for (uint32_t some = __ballot_sync(0xFFFFFFFFu, bits && pos < rows_n && pos + __popc(bits) > 0); some; some &= some - 1) {
-      const int l = __ffs(some) - 1;
-      const uint32_t wb = __shfl_sync(0xFFFFFFFFu, bits, l);
-      const int wp = __shfl_sync(0xFFFFFFFFu, pos, l) + __popc(wb & ((1u << lane) - 1u));
-      if ((wb >> lane & 1u) && wp >= 0 && wp < rows_n) src[wp] = (w0 + warp * 32 + l) * 32 + lane;
-    }
-    at.x += all.x + min(at.y + all.y, need) - min(at.y, need);
-    at.y += all.y;
+    place(w, pre, w0 + warp * 32, 0xFFFFFFFFu);
+    pass(all);
   }
   __syncthreads();
   const bool still = src[0] == d0 && src[rows_n - 1] == d0 + rows_n - 1;  // nothing moves
@@ -396,7 +419,8 @@ int64_t evict_up(int64_t x) { return (x + 255) & ~int64_t{255}; }
 
 size_t evict_workspace(int64_t B, int64_t H, int64_t cap) {
   const int64_t tiles = (cap + EVICT_MIN_TILE - 1) / EVICT_MIN_TILE, heads = B * H;
-  return static_cast<size_t>(256 + evict_up(heads * 16) + evict_up(heads * tiles * 8) + 2 * evict_up(heads * tiles * 4) +
+  return static_cast<size_t>(256 + evict_up(heads * 16) + evict_up(heads * tiles * 8) + evict_up(heads * tiles * 4) +
+                             evict_up(heads * tiles * 16) +
                              evict_up(heads * ((cap + 31) / 32) * 8));
 }
 
@@ -421,7 +445,7 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   p.cut = reinterpret_cast<uint4*>(take(heads * 16));
   p.before = reinterpret_cast<uint2*>(take(heads * p.max_tiles * 8));
   p.loaded = reinterpret_cast<uint32_t*>(take(heads * p.max_tiles * 4));
-  p.first_tile = reinterpret_cast<int*>(take(heads * p.max_tiles * 4));
+  p.begins = reinterpret_cast<uint4*>(take(heads * p.max_tiles * 16));
   p.words = reinterpret_cast<uint2*>(take(heads * p.max_words * 8));
   // 4096 entries a CTA keep a pass near its latency, as long as all CTAs run at once (one an SM)
   int C = 1;

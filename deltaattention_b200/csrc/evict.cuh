@@ -22,13 +22,14 @@ struct EvictParams {
   int tile, tile_shift;                  // entries per moved tile, a power of two
   int max_tiles, max_words;              // of a full head: tiles, words of 32 entries
   // workspace: error word; per head (threshold key, ties kept, length or 0 if left alone, ticket);
-  // per head and tile (kept, ties before it); per tile of the result whether its rows have been read
-  // and the tile its first entry comes from; per 32 entries (surely kept, ties)
+  // per head and tile (kept, ties before it); per tile of the result whether its rows have been read,
+  // and the tile its first entry comes from with (kept, ties before that); per 32 entries (surely
+  // kept, ties)
   int* err;
   uint4* cut;
   uint2* before;
   uint32_t* loaded;
-  int* first_tile;
+  uint4* begins;
   uint2* words;
 };
 
