@@ -491,7 +491,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         ldsm_x4_trans(v, vl_at + su + 16 * i * St::SROW);
       } else {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = lds16(vs_at + su + 2 * (gq & 3) + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW);
+        for (int k = 0; k < 4; ++k)
+          v[k] = lds16(vs_at + su + 2 * (gq & 3) + (16 * i + (k & 1) + 8 * (k >> 1)) * St::SROW);
         v[0] = v[1] = prmt(v[0], v[1], 0x5410);
         v[2] = v[3] = prmt(v[2], v[3], 0x5410);
       }
@@ -698,13 +699,13 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
 }
 
 // Bound by what the SMs issue: 16 keys take a warp about 310 instructions, 18 of them products, which
-// hold up the other pipes too, so that about half the issue slots are used. Copies wait for nobody:
+// hold up the other pipes too, so that 60 % of the issue slots are used. Copies wait for nobody:
 // with all tiles from one address the time falls by 8 %. 12 warps an SM of 168 registers; 16 of 128
 // registers spill and take 7 % longer, a ring of 3 tiles changes nothing. bf16, d = 128, 4 q-heads
 // per kv-head, device times with the join:
-//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 74 us, 4.7 TB/s
-//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 33 us, with mass 39 us
-//   1 sequence of 8192 entries: 12 us, most of it the latencies of two launches
+//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 70 us, 4.9 TB/s
+//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 31 us, with mass 37 us
+//   1 sequence of 8192 entries: 10.8 us, most of it the latencies of two launches
 //
 // With `splits` every head is cut into that many pieces (as many as it has units). Otherwise the
 // units of all heads in a row are cut into even pieces, one per CTA, whatever the heads' lengths: all
@@ -813,7 +814,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
 // ---------------------------------------------------------------------------------- joining
 // Launched while the attention kernel ends (programmatic dependent launch): grid_wait returns once
 // that kernel's writes are there. Joining is a chain of dependent reads (the head's parts, their
-// maxima and sums, their outputs), 6.8 us alone. The mass reads the scores again and adds 6 us for 16
+// maxima and sums, their outputs), 5.3 us alone. The mass reads the scores again and adds 6 us for 16
 // sequences of 1024 to 8192 entries: 4 G bytes a key written and read, where a key has 5 D / 4. Four
 // q-heads at a time keep enough of its CTAs resident (eight at a time: 1.6 us more).
 // blockIdx.y: kv-head. The first G CTAs join the parts of one q-head each and write its output;
