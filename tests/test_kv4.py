@@ -574,6 +574,37 @@ def test_evict_long_heads_and_wide_rows(ops, B, H, cap, budget, first, recent, w
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["ends", "ties_before", "ties_between", "thin"])
+def test_evict_long_stretches_without_kept_entries(ops, kind):
+    """One tile of the result whose entries lie tens of thousands of entries apart."""
+    cap, budget = 50000, 900
+    g = torch.Generator().manual_seed(len(kind))
+    mass = 0.5 * torch.rand(1, 2, cap, generator=g)
+    at = torch.tensor([3, 40, 41, 63, 64, 1000, 30011, 30012, 47000])
+    mass[..., at] = 2.0
+    if kind == "ends":             # the heaviest at both ends
+        mass[..., :500] += 1
+        mass[..., -391:] += 1
+    elif kind == "ties_before":    # more ties at the cut than are kept, near the beginning
+        mass[..., 100:2100] = 1.0
+    elif kind == "ties_between":   # ties at the cut in the middle of a long stretch
+        mass[..., 20000:22000] = 1.0
+    else:                          # one entry in some 56
+        mass[..., ::56] += 1
+    n = torch.tensor([[cap, cap - 7]], dtype=torch.int32)
+    rows = [torch.arange(cap, dtype=torch.int32).expand(1, 2, cap).contiguous().cuda(),
+            torch.randn(1, 2, cap, 5, generator=g).cuda()]
+    was = [r.cpu().clone() for r in rows]
+    m, length = mass.cuda(), n.cuda()
+    ops.evict_by_mass(m, length, rows, budget, keep_first=1, keep_recent=2)
+    assert (length == budget).all()
+    for h in range(2):
+        kept = evict64(mass[0, h], int(n[0, h]), budget, 1, 2) + list(range(budget, cap))
+        for got, want in zip((m, *rows), (mass, *was)):
+            assert torch.equal(got[0, h].cpu(), want[0, h, kept])
+
+
+@gpu
 def test_evict_row_limit(ops):
     """Rows of 4096 bytes are the widest."""
     m, n = torch.rand(1, 1, 64, device="cuda"), torch.full((1, 1), 64, dtype=torch.int32, device="cuda")
