@@ -22,7 +22,7 @@
 //    p alone, in two parts, times the stored (scales, zeros) gives the zeros' share, added at the end.
 //    (Numbers 16 + code took a shift for every operand.)
 //    With up to 4 q-heads the columns 4 to 7 hold them again: the first parts go into columns 0 to 3,
-//    the rest into 4 to 7, and one product does for two.
+//    the rest into 4 to 7, and one product does for two (70 us where 8 q-heads take 75, below).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -36,8 +36,11 @@ constexpr int KV4_NW = 4;      // warps per CTA, each with its own tiles and its
 constexpr int KV4_TILE = 32;   // keys per tile
 constexpr int KV4_STAGES = 2;  // tiles in a warp's ring
 constexpr int KV4_MAX_PIECES = 1024, KV4_MAX_HEADS = 2048;  // that are cut into pieces
-constexpr int KV4_MIN_UNITS = 8;  // of a piece: two tiles a warp
-constexpr int KV4_START = 6;      // units that beginning and ending a head costs as much as
+// of a piece: two tiles a warp (8 heads of 8192: 10.7 us; pieces of 4: 14.4, of 12: 11.9)
+constexpr int KV4_MIN_UNITS = 8;
+// units that beginning and ending a head costs as much as (4 sequences of 65536 / 16 ragged ones with
+// mass: 71.5 / 36.7 us; none: 73.4 / 38.8; 3: 72.3 / 37.2; 9: 71.4 / 36.6)
+constexpr int KV4_START = 6;
 constexpr int KV4_BIAS = 64;      // log2 of what history weights carry until they are joined with the window's
 constexpr float KV4_SLACK = 8.f;  // log2 units a score may exceed the running maximum by before it moves
 
@@ -953,8 +956,11 @@ Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_
   const int64_t slots = std::min<int64_t>((D == 64 ? 4 : 3) * static_cast<int64_t>(sms), KV4_MAX_PIECES);
   const int64_t units = std::max<int64_t>(1, (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16);
   w.splits = w.pieces = 0;
-  if (heads >= std::min<int64_t>(4 * slots, KV4_MAX_HEADS)) w.splits = 1;  // so many even out by themselves
-  else if (heads * units <= slots * KV4_MIN_UNITS)  // everything at once: where a piece begins needs no search
+  // Very many heads even out by themselves (2048 of 512: 71 us, as pieces 76; of 20 to 512: 62, 66).
+  // Few units run at once: where a piece begins needs no search (8 heads of 20000, just above the
+  // limit, took 17 us as pieces and 15 cut alike, before pieces counted the heads' beginnings).
+  if (heads >= std::min<int64_t>(4 * slots, KV4_MAX_HEADS)) w.splits = 1;
+  else if (heads * units <= slots * KV4_MIN_UNITS)
     w.splits = static_cast<int>((units + KV4_MIN_UNITS - 1) / KV4_MIN_UNITS);
   else w.pieces = static_cast<int>(slots);
   w.ctas = w.pieces ? w.pieces : heads * w.splits;
