@@ -17,12 +17,17 @@
 //    matrix path converts them to fp16 first.)
 //  * Values: elements are the rows, q-heads the columns, in bf16, whose range the scales need. Up to
 //    255 a byte is a bf16 number too, byte 2^-133, so again a shift and four ands give 8 operands.
-//    The weights carry 2^64, which keeps products in fp32's normal range: scales of 2^-40 to 2^54
-//    have it all. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every weight);
-//    p alone, in two parts, times the stored (scales, zeros) gives the zeros' share, added at the end.
+//    The weights carry 2^64, which keeps products in fp32's normal range: scales from 2^-40 and values
+//    below 2^50 have it all. p scale_g goes in as two bf16 parts, high and the rest (16 bits of every
+//    weight); p alone, in two parts, times the stored (scales, zeros) gives the zeros' share.
 //    (Numbers 16 + code took a shift for every operand.)
+//    The zeros are added to the codes' sums after every tile. Over a long history of flat weights both
+//    are hundreds of times larger than what is left of them, and a product rounds the sum it adds to
+//    towards zero: added at the end, 100003 entries were 4e-6 of the terms off, all in one
+//    direction, 25 times the rounding of an fp16 output. Tile by tile, 1e-9 (8 shuffles and 32 FMA a
+//    tile, 3 us of the 72 below).
 //    With up to 4 q-heads the columns 4 to 7 hold them again: the first parts go into columns 0 to 3,
-//    the rest into 4 to 7, and one product does for two (70 us where 8 q-heads take 75, below).
+//    the rest into 4 to 7, and one product does for two (72 us where 8 q-heads take 77, below).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -155,7 +160,6 @@ template <int D>
 struct Kv4Acc {
   float m[2], l[2];
   float o[D / 16][4];  // [2 g + i / 2]: element 32 g + 4 (lane / 4) + i in [2 (i % 2) + head]
-  float sz[4];         // sums of p zero_g: value lane / 4 of the stored row (scales, zeros) in [0], [1]
 
   __device__ __forceinline__ void init() {
     m[0] = m[1] = -INFINITY;
@@ -164,8 +168,6 @@ struct Kv4Acc {
     for (int i = 0; i < D / 16; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sz[e] = 0.f;
   }
 
   // Scores of 16 NT keys (lane: rows lane / 4 + 8 f of each 16, heads 2 t + e in [2 f + e]) to
@@ -196,7 +198,6 @@ struct Kv4Acc {
         o[i][0] *= fa; o[i][1] *= fb;
         o[i][2] *= fa; o[i][3] *= fb;
       }
-      sz[0] *= fa; sz[1] *= fb;
     }
     const float ra = (m[0] == -INFINITY ? 0.f : m[0]) - BIAS, rb = (m[1] == -INFINITY ? 0.f : m[1]) - BIAS;
 #pragma unroll
@@ -475,6 +476,7 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
     load_values(0);
     acc.template weights<2, KV4_BIAS>(zs);
     // ---- values
+    float sz[4] = {0.f, 0.f, 0.f, 0.f};  // the tile's sums of p zero_g: value lane / 4 of the stored row in [0], [1]
     uint32_t ph[2][2], pl[2][2];  // weights of keys 2 t, 2 t + 1 (+ 8) for head lane / 4, two parts
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -499,8 +501,8 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         v[0] = v[1] = prmt(v[0], v[1], 0x5410);
         v[2] = v[3] = prmt(v[2], v[3], 0x5410);
       }
-      mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], second ? pl[i][0] : ph[i][0], second ? pl[i][1] : ph[i][1]);
-      if constexpr (!FOLD) mma16816<B>(acc.sz, v[0], v[1], v[2], v[3], pl[i][0], pl[i][1]);
+      mma16816<B>(sz, v[0], v[1], v[2], v[3], second ? pl[i][0] : ph[i][0], second ? pl[i][1] : ph[i][1]);
+      if constexpr (!FOLD) mma16816<B>(sz, v[0], v[1], v[2], v[3], pl[i][0], pl[i][1]);
       const uint32_t half = gq & 1 ? 0x7632u : 0x5410u;
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
@@ -524,27 +526,31 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
         }
       }
     }
+    // the zeros, in the units of the codes
+    constexpr float EVEN = 0x1p-133f, ODD = 0x1p-129f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float z = __shfl_sync(0xFFFFFFFFu, sz[e], 4 * (NG + g) + t);
+        acc.o[2 * g][e] = fmaf(z, EVEN, acc.o[2 * g][e]);
+        acc.o[2 * g][2 + e] = fmaf(z, ODD, acc.o[2 * g][2 + e]);
+        acc.o[2 * g + 1][e] = fmaf(z, EVEN, acc.o[2 * g + 1][e]);
+        acc.o[2 * g + 1][2 + e] = fmaf(z, ODD, acc.o[2 * g + 1][2 + e]);
+      }
     stage = stage == KV4_STAGES - 1 ? 0 : stage + 1;
   }
   cp_wait<0>();
 
-  // sums of codes to values: units and the weights' bias, then the zeros
-  constexpr float EVEN = 0x1p69f, ODD = 0x1p65f, UNBIAS = 0x1p-64f;
+  // sums of codes to values: their units and the weights' bias
   static_assert(KV4_BIAS == 64, "2^(133 - 64), 2^(129 - 64), 2^-64");
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    acc.l[e] *= UNBIAS;
-    if constexpr (FOLD) {  // in the columns of the first parts
-      const float x = acc.sz[e] + __shfl_xor_sync(0xFFFFFFFFu, acc.sz[e], 2);
-      acc.sz[e] = t < 2 ? x : 0.f;
-    }
+    acc.l[e] *= 0x1p-64f;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float z = __shfl_sync(0xFFFFFFFFu, acc.sz[e], 4 * (NG + g) + t) * UNBIAS;
-      acc.o[2 * g][e] = fmaf(acc.o[2 * g][e], EVEN, z);
-      acc.o[2 * g][2 + e] = fmaf(acc.o[2 * g][2 + e], ODD, z);
-      acc.o[2 * g + 1][e] = fmaf(acc.o[2 * g + 1][e], EVEN, z);
-      acc.o[2 * g + 1][2 + e] = fmaf(acc.o[2 * g + 1][2 + e], ODD, z);
+    for (int i = 0; i < D / 16; ++i) {
+      acc.o[i][e] *= 0x1p69f;
+      acc.o[i][2 + e] *= 0x1p65f;
     }
   }
 
@@ -701,13 +707,13 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   __syncthreads();  // the ring may be filled again
 }
 
-// Bound by what the SMs issue: 16 keys take a warp about 310 instructions, 18 of them products, which
+// Bound by what the SMs issue: 16 keys take a warp about 330 instructions, 18 of them products, which
 // hold up the other pipes too, so that 60 % of the issue slots are used. Copies wait for nobody:
 // with all tiles from one address the time falls by 8 %. 12 warps an SM of 168 registers; 16 of 128
 // registers spill and take 7 % longer, a ring of 3 tiles changes nothing. bf16, d = 128, 4 q-heads
 // per kv-head, device times with the join:
-//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 70 us, 4.9 TB/s
-//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 31 us, with mass 37 us
+//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 72 us, 4.8 TB/s
+//   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 32 us, with mass 37 us
 //   1 sequence of 8192 entries: 10.8 us, most of it the latencies of two launches
 //
 // With `splits` every head is cut into that many pieces (as many as it has units). Otherwise the

@@ -383,9 +383,10 @@ size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int
  * with a positive count (others draw nothing, whatever they hold) and sm_scale * q . k over the
  * first exact_len window rows. A query row with no entry left gives 0. With `mass` (fp32, else
  * NULL) every entry's attention weight, summed over the kv-head's q-heads, is added to mass and
- * exact_mass. Weights are held in 16 bits or more, sums in 32; elements of a query row below 2^-26
- * of its largest are rounded to that step, and scales of values outside 2^-40 .. 2^54 lose
- * precision or overflow. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
+ * exact_mass. Weights are held in 16 bits or more, sums in 32 (of a history, within 2^-21 of the sum of
+ * weight * (|zero| + scale * code) over its entries, whatever its length); elements of a query row
+ * below 2^-26 of its largest are rounded to that step, value scales below 2^-40 lose precision and
+ * values from 2^50 on may overflow. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
  * and `advance` as in dab_decode_attention_dev; without it exact_len is the argument.
  * `strides` (17): q (b, h), out (b, h), codes (b, h), scales (b, h), counts / mass (b, h), lengths
  * (b, h), exact K / V (b, h, row), exact_mass (b, h). Query and exact rows contiguous, 16-byte
