@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(SEL_THREADS) evict_select_kernel(const __grid_
 #pragma unroll
     for (int j = 0; j < SEL_KEYS; ++j) key[j] = mass_key(__uint_as_float(key[j]));
   };
-  load(i0);
+  if (i0 < i1) load(i0);  // a head of fewer tiles than CTAs leaves some without entries
   const bool one = i1 - i0 <= SEL_CHUNK;
   for (int i = tid; i < 3 * SEL_BINS; i += SEL_THREADS) (&hist[0][0])[i] = 0;
   const int out_tiles = (p.budget + p.tile - 1) >> p.tile_shift;

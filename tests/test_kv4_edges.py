@@ -48,3 +48,37 @@ def test_attention_of_long_flat_histories(ops, D, G, dt):
         err = (out[0, h * G:(h + 1) * G].double() - ref).abs()
         tol = UNIT[DT[dt]] * ref.abs() + 2.0 ** -25 + 2.0 ** -21 * terms
         assert (err <= tol).all(), (h, (err / terms).max().item())
+
+
+# ------------------------------------------------------- eviction of short heads in large capacities
+def kept64(mass, n, budget, first, recent):
+    """Indices that a head of n > budget entries keeps, in order: a stable sort of the weights in 64 bits."""
+    mid = torch.sort(mass[first:n - recent].double(), descending=True, stable=True).indices[:budget - first - recent]
+    return torch.cat([torch.arange(first), first + mid.sort().values, torch.arange(n - recent, n)])
+
+
+@gpu
+@pytest.mark.parametrize("B,H,cap,budget,first,recent,lens", [
+    (1, 8, 5000, 20, 2, 3, (21, 31, 32, 33, 64, 100, 255, 256)),         # 2 CTAs a head
+    (1, 8, 8448, 100, 0, 1, (101, 250, 120, 128, 129, 256, 257, 3)),     # 4
+    (2, 4, 20000, 512, 4, 32, (700, 513, 512, 800, 1024, 1025, 2047, 20000)),  # 8
+    (1, 2, 131072, 256, 0, 0, (257, 300)), (1, 1, 140001, 1, 0, 1, (2,)), (1, 1, 40000, 33, 1, 1, (34,)),
+    (2, 4, 32768, 256, 16, 100, (257, 511, 513, 769, 1023, 1793, 2049, 300))])
+def test_evict_short_heads_in_large_capacities(ops, B, H, cap, budget, first, recent, lens):
+    """Capacities that give a head several CTAs, and heads with fewer tiles than CTAs."""
+    g = torch.Generator().manual_seed(cap + budget)
+    lengths = torch.tensor(lens, dtype=torch.int32).view(B, H)
+    mass = torch.randint(0, 50, (B, H, cap), generator=g).float()  # ties too
+    for rows in ([torch.arange(cap, dtype=torch.int32).expand(B, H, cap).contiguous()],
+                 [torch.arange(cap, dtype=torch.int32).expand(B, H, cap).contiguous(),
+                  torch.randint(-9, 9, (B, H, cap, 40), generator=g).int()]):
+        m, n, moved = mass.cuda(), lengths.cuda(), [r.cuda() for r in rows]
+        ops.evict_by_mass(m, n, moved, budget, keep_first=first, keep_recent=recent)
+        assert torch.equal(n.cpu(), lengths.clamp(max=budget))
+        for b in range(B):
+            for h in range(H):
+                length, kept = int(lengths[b, h]), torch.arange(cap)
+                if length > budget:
+                    kept[:budget] = kept64(mass[b, h], length, budget, first, recent)
+                for got, want in zip((m, *moved), (mass, *rows)):
+                    assert torch.equal(got[b, h].cpu(), want[b, h, kept])
