@@ -23,6 +23,8 @@
 //    130 us.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "evict.cuh"
 
 namespace dab {
@@ -34,6 +36,7 @@ constexpr int SEL_KEYS = 16;                         // a thread's keys in regis
 constexpr int SEL_BINS = 2048;
 constexpr int SEL_CHUNK = SEL_THREADS * SEL_KEYS;
 constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_BYTES = 80 * 1024;  // of a tile's rows, where it has more than EVICT_MIN_TILE entries
 enum { ERR_EVICT_WAIT = 0x501 };
 
 // Unsigned key of a weight in the order of floats: NaN below everything, -0 equal to +0.
@@ -414,6 +417,21 @@ __global__ void __launch_bounds__(MOVE_THREADS) evict_move_kernel(const __grid_c
 }
 
 namespace {
+// The kernel's shared-memory limit, raised once per device to the most that any call takes (the
+// smallest tile of the widest entries): it is one for all threads of the process.
+cudaError_t move_smem_limit() {
+  constexpr int MOST = EVICT_MIN_TILE * (4 + EVICT_MAX_BYTES + 4);
+  static_assert(MOST >= MOVE_THREADS * 4 + MOVE_BYTES, "larger tiles take no more");
+  static std::atomic<uint64_t> set{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (set.load() & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST);
+  if (e == cudaSuccess) set.fetch_or(bit);
+  return e;
+}
 int64_t evict_up(int64_t x) { return (x + 255) & ~int64_t{255}; }
 }  // namespace
 
@@ -426,11 +444,11 @@ size_t evict_workspace(int64_t B, int64_t H, int64_t cap) {
 
 cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
   if (p.B * p.H == 0 || p.cap == 0) return cudaSuccess;
-  // tiles of up to 256 entries and 80 KB of rows
+  // tiles of up to 256 entries and MOVE_BYTES of rows
   int bytes = 0;
   for (int r = 0; r < p.n_rows; ++r) bytes += p.bytes[r];
   p.tile = MOVE_THREADS;
-  while (p.tile > EVICT_MIN_TILE && p.tile * bytes > 80 * 1024) p.tile >>= 1;
+  while (p.tile > EVICT_MIN_TILE && p.tile * bytes > MOVE_BYTES) p.tile >>= 1;
   p.tile_shift = __builtin_ctz(static_cast<unsigned>(p.tile));
   p.max_tiles = (p.cap + p.tile - 1) / p.tile;
   p.max_words = (p.cap + 31) / 32;
@@ -456,9 +474,7 @@ cudaError_t launch_evict(EvictParams p, uint8_t* ws, cudaStream_t st) {
     p.shift[r] = (upr & (upr - 1)) == 0 ? __builtin_ctz(static_cast<unsigned>(upr)) : -1;
     move_smem += (p.tile * p.bytes[r] + 15) & ~15;
   }
-  cudaError_t e = cudaSuccess;
-  if (move_smem > 48 * 1024)
-    e = cudaFuncSetAttribute(evict_move_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, move_smem);
+  cudaError_t e = move_smem_limit();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(C), static_cast<unsigned>(heads));

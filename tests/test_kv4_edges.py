@@ -82,3 +82,37 @@ def test_evict_short_heads_in_large_capacities(ops, B, H, cap, budget, first, re
                     kept[:budget] = kept64(mass[b, h], length, budget, first, recent)
                 for got, want in zip((m, *moved), (mass, *rows)):
                     assert torch.equal(got[b, h].cpu(), want[b, h, kept])
+
+
+@gpu
+def test_evict_from_two_threads(ops):
+    """Host threads whose rows want different amounts of shared memory do not refuse one another's calls."""
+    import threading
+    cap, budget, rounds = 200, 70, 400
+    errors, heads = [], []
+
+    def work(width, seed):
+        try:
+            g = torch.Generator().manual_seed(seed)
+            mass, rows = torch.rand(1, 2, cap, generator=g), torch.randint(-9, 9, (1, 2, cap, width), generator=g).int()
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                m0, r0, n = mass.cuda(), rows.cuda(), torch.empty(1, 2, dtype=torch.int32, device="cuda")
+                for _ in range(rounds):
+                    m, r = m0.clone(), r0.clone()
+                    ops.evict_by_mass(m, n.fill_(cap), [r], budget)
+            stream.synchronize()
+            heads.append((mass, rows, r.cpu(), n.cpu()))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in ((1000, 1), (60, 2), (500, 3))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for mass, rows, r, n in heads:
+        assert (n == budget).all()
+        for h in range(2):
+            assert torch.equal(r[0, h, :budget], rows[0, h, kept64(mass[0, h], cap, budget, 0, 0)])
