@@ -174,7 +174,11 @@ class Kv4DecodeCache:
     is kept in 16 bits for the comparison.
 
     Attention adds every entry's weight to ``mass`` (history) and ``exact_mass`` (window; it moves with
-    the token into the history). ``evict`` cuts heads to their heaviest entries by it, in place."""
+    the token into the history). ``evict`` cuts heads to their heaviest entries by it, in place.
+
+    ``err`` (int32 [1] on the device) holds the first error until it is zeroed: 0x201, a token had to be
+    appended to a full history and was lost; 0x501, a wait inside an eviction ran out and the cache is
+    not valid."""
 
     def __init__(self, num_layers, batch, kv_heads, head_dim, capacity, exact_window, dtype=torch.bfloat16,
                  device="cuda", threshold=0.0, use_cosine=False, track_mass=True):
@@ -197,7 +201,10 @@ class Kv4DecodeCache:
         self.last_key = z(head_dim, dt=dtype)
         self.k_exact, self.v_exact = z(W, head_dim, dt=dtype), z(W, head_dim, dt=dtype)
         self.seq_state = torch.zeros((num_layers, 2), device=dev, dtype=torch.int64)  # (exact, total) per layer
-        self.err = torch.zeros((1,), device=dev, dtype=torch.int32)
+        # The eviction's workspace begins with its error word, and updates use the same one.
+        self._evict_ws = torch.zeros(ops.evict_workspace(batch, kv_heads, cap) if track_mass else 4, device=dev,
+                                     dtype=torch.uint8)
+        self.err = self._evict_ws[:4].view(torch.int32)
         self.hist = [ops.KV4(self._codes[0][i], self._scales[0][i], self._codes[1][i], self._scales[1][i])
                      for i in range(num_layers)]
         self._ws = {}
@@ -272,11 +279,10 @@ class Kv4DecodeCache:
         if keep_recent < 1:
             raise ValueError("Kv4DecodeCache.evict: keep_recent must be at least 1")
         h = self.hist[layer]
-        ws = self._workspace("evict", ops.evict_workspace(self.bsz, self.n_kv_heads, self.capacity))
         ops.evict_by_mass(self.mass[layer], self.packed_lengths[layer],
                           (h.k_codes, h.k_scales, h.v_codes, h.v_scales, self.packed_counts[layer],
                            self.packed_timestamps[layer]), budget, trigger=trigger, keep_first=keep_first,
-                          keep_recent=keep_recent, workspace=ws)
+                          keep_recent=keep_recent, workspace=self._evict_ws)
 
     def dequantize(self, layer, dtype=None):
         """The history's K and V rows [B, Hkv, capacity, d] (rows past a head's length hold anything)."""

@@ -116,3 +116,45 @@ def test_evict_from_two_threads(ops):
         assert (n == budget).all()
         for h in range(2):
             assert torch.equal(r[0, h, :budget], rows[0, h, kept64(mass[0, h], cap, budget, 0, 0)])
+
+
+# --------------------------------------------------------------------------------- the cache
+def small_cache(layers=2, B=2, H=2, D=64, cap=96, W=8, n=50, seed=0, **kw):
+    from deltaattention_b200.cache import Kv4DecodeCache
+    g = torch.Generator().manual_seed(seed)
+    c = Kv4DecodeCache(layers, B, H, D, cap, W, threshold=3.0, **kw)
+    r = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()  # noqa: E731
+    for layer in range(layers):
+        c.load_prefill(layer, r(B, H, n, D), r(B, H, n, D), torch.randint(1, 5, (B, H, n), generator=g).int().cuda(),
+                       torch.arange(n).int().cuda().expand(B, H, n), r(B, H, W, D), r(B, H, W, D), 4 * n)
+    return c, r
+
+
+@gpu
+def test_cache_reports_evictions_error_word(ops, monkeypatch):
+    """What an eviction writes into the first word of its workspace is seen in ``err``, and stays there."""
+    c, r = small_cache()
+    given, evict = [], ops.evict_by_mass
+
+    def noting(*a, workspace=None, **kw):
+        given.append(workspace)
+        return evict(*a, workspace=workspace, **kw)
+
+    monkeypatch.setattr(ops, "evict_by_mass", noting)
+    c.evict(0, 30)
+    c.evict(1, 30)
+    assert int(c.err) == 0 and (c.packed_lengths == 30).all()
+    for ws in list(given):
+        ws[:4].view(torch.int32).fill_(0x501)  # as a wait that ran out does
+        assert int(c.err) == 0x501
+        c.evict(0, 20)
+        assert int(c.err) == 0x501
+        c.err.zero_()
+    full, r = small_cache(cap=50)
+    for layer in range(2):
+        full.update(layer, 9 * r(2, 2, 1, 64), r(2, 2, 1, 64))
+    assert int(full.err) == 0x201
+    off, _ = small_cache(track_mass=False)
+    assert off.err.shape == c.err.shape == (1,) and off.err.dtype == c.err.dtype == torch.int32 and int(off.err) == 0
+    codes = L.workspace_errors()
+    assert not any(codes), codes
