@@ -239,11 +239,11 @@ class Kv4DecodeCache:
         return None if t is None else t[layer]
 
     def _workspace(self, name, nbytes):
-        """This cache's own scratch (a captured step keeps using it)."""
-        ws = self._ws.get(name)
-        if ws is None or ws.numel() < nbytes:
-            ws = self._ws[name] = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
-        return ws
+        """This cache's own scratch. Smaller ones stay for the life of the cache: a captured step may use them."""
+        kept = self._ws.setdefault(name, [])
+        if not kept or kept[-1].numel() < nbytes:
+            kept.append(torch.zeros(nbytes, dtype=torch.uint8, device=self.device))
+        return kept[-1]
 
     def update(self, layer, k_new, v_new, advance=True):
         """Takes one token per (batch, kv-head): k_new / v_new [B, Hkv, 1, d]; ``advance`` as in

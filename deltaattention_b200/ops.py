@@ -821,7 +821,8 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     With ``mass`` [B, Hkv, capacity] and ``exact_mass`` [B, Hkv, W] (fp32), every entry's attention
     weight, summed over the q-heads of its kv-head, is added to them: what ``evict_by_mass`` goes
     by. ``workspace`` (uint8, ``kv4_attention_workspace`` bytes of any content, used by one stream
-    at a time) replaces the library's own. Returns out [B, Hq, d]."""
+    at a time) replaces the library's own, which is given up when a later call needs a larger one: a call
+    that is captured in a CUDA graph takes the caller's. Returns out [B, Hq, d]."""
     what = "decode_attention_kv4"
     (B, H, cap, D), hs = hist.check(what, q)
     dev = L.same_device(what, q, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
@@ -904,7 +905,9 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
     Lengths are read on the device: no host synchronisation, and the call can be captured in a
     CUDA graph and replayed at every token, where it only does work once a head passes
     ``trigger``. ``workspace`` (uint8, ``evict_workspace`` bytes, zero-filled once, used by one
-    stream at a time) replaces the library's own."""
+    stream at a time) replaces the library's own, which is given up when a later call needs a larger
+    one: a captured call takes the caller's. With a budget of ``capacity`` or more nothing is done, as no
+    head can be longer."""
     what = "evict_by_mass"
     L.same_device(what, mass, lengths, workspace, *rows)
     size = mass.shape

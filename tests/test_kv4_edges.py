@@ -158,3 +158,38 @@ def test_cache_reports_evictions_error_word(ops, monkeypatch):
     assert off.err.shape == c.err.shape == (1,) and off.err.dtype == c.err.dtype == torch.int32 and int(off.err) == 0
     codes = L.workspace_errors()
     assert not any(codes), codes
+
+
+def test_cache_keeps_scratch_of_captured_steps():
+    """A buffer that was handed out lives as long as the cache, also when a later call needs a larger one."""
+    import weakref
+
+    from deltaattention_b200.cache import Kv4DecodeCache
+    c = Kv4DecodeCache.__new__(Kv4DecodeCache)
+    c._ws, c.device = {}, torch.device("cpu")
+    first = weakref.ref(c._workspace("attend", 100))
+    assert c._workspace("attend", 60) is first()
+    larger = c._workspace("attend", 200)
+    assert larger.numel() >= 200 and first() is not None and first().data_ptr() != larger.data_ptr()
+    assert c._workspace("attend", 200) is larger and c._workspace("attend", 100).numel() >= 100
+
+
+@gpu
+def test_captured_step_after_calls_with_more_heads(ops):
+    """A captured step does not write where later tensors are."""
+    (c, r), (eager, _) = small_cache(layers=1), small_cache(layers=1)
+    q, k, v = r(1, 2, 4, 64), r(1, 2, 2, 1, 64), r(1, 2, 2, 1, 64)
+    outs = torch.empty_like(q), torch.empty_like(q)
+    for cache, out in zip((c, eager), outs):
+        cache.step(0, q[0], k[0], v[0], out[0])
+    size = ops.kv4_attention_workspace(2, 4, 2, 64, 96, 8)
+    graph = c.capture_step(q, k, v, outs[0])
+    wide = r(2, 64, 64)
+    for cache in (c, eager):
+        cache.attend(0, wide)
+    others = [torch.full((size,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    for _ in range(3):
+        graph.replay()
+        eager.step(0, q[0], k[0], v[0], outs[1][0])
+    assert all((t == 0x5A).all() for t in others)
+    assert torch.equal(*outs) and torch.equal(c.mass, eager.mass)
