@@ -679,7 +679,7 @@ class KV4:
 def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) -> KV4:
     """K and V rows [B, Hkv, M, d] (any strides; bf16 / fp16, d 64 or 128) in 4 bits.
 
-    Per group of 32 elements of a row: zero = its minimum rounded down to bf16, scale = (maximum -
+    Per group of 32 elements of a row, in fp32: zero = its minimum rounded down to bf16, scale = (maximum -
     zero) / 15 rounded to bf16, code = round((x - zero) / scale) to even, cut to [0, 15]. A group
     that holds a NaN or an infinity reads back as NaN. ``out`` may be views of a cache
     (``KV4.rows``)."""

@@ -193,3 +193,52 @@ def test_captured_step_after_calls_with_more_heads(ops):
         eager.step(0, q[0], k[0], v[0], outs[1][0])
     assert all((t == 0x5A).all() for t in others)
     assert torch.equal(*outs) and torch.equal(c.mass, eager.mass)
+
+
+# ----------------------------------------------------------------- quantisation by the formula
+def plain_quantize(x, half=False):
+    """(codes, scales, zeros) of rows [.., D] by the formula, one fp32 operation at a time; with ``half`` of half the
+    elements, the scales and zeros doubled (the same numbers, without fp32's limit on the range)."""
+    x = x.float().cpu().unflatten(-1, (-1, 32)) * (0.5 if half else 1.0)
+    i = x.amin(-1).view(torch.int32)
+    zero = ((i + (i < 0).int() * 0xFFFF) & -0x10000).view(torch.float32)
+    scale = ((x.amax(-1) - zero) / 15).bfloat16().float()
+    code = ((x - zero[..., None]) / scale[..., None]).round().clamp(0, 15)
+    code = torch.where(scale[..., None] == 0, 0.0, code)
+    return code.flatten(-2), scale * (2 if half else 1), zero * (2 if half else 1)
+
+
+def check_quantized(ops, x, half=False):
+    """Both paths of the hand-off and the token update against the formula."""
+    B, H, N, D = x.shape
+    codes, scale, zero = plain_quantize(x, half)
+    wide = torch.zeros(B, H, N, D + 1, dtype=x.dtype, device="cuda")[..., 1:]
+    wide.copy_(x)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    taken = ops.KV4.empty(B, H, N, D, "cuda")
+    lengths, state = z(B, H), torch.tensor([1, 1], device="cuda")
+    last, new = torch.zeros(B, H, D, dtype=x.dtype, device="cuda"), torch.zeros(B, H, 1, D, dtype=x.dtype, device="cuda")
+    for n in range(N):  # every row leaves a window of one and is appended
+        ops.decode_update_kv4(new, new, taken, z(B, H, N), z(B, H, N), lengths, last, x[:, :, n:n + 1].clone(),
+                              x[:, :, n:n + 1].clone(), state, threshold=2.0, similarity="cosine")
+        assert (lengths == n + 1).all()
+    for hist in (ops.kv4_quantize(x, x), ops.kv4_quantize(wide, wide), taken):
+        for c, s in ((hist.k_codes, hist.k_scales), (hist.v_codes, hist.v_scales)):
+            assert torch.equal(s.cpu().float(), torch.cat([scale, zero], -1))
+            assert torch.equal(device_rows64(c, s)[0].cpu().float(), codes)
+
+
+@gpu
+@pytest.mark.parametrize("dt,low", [("bf16", 5), ("fp16", 2)])
+def test_quantize_scales_between_two_numbers(ops, dt, low):
+    """Ranges of 15 (m + 1/2) steps of bf16: the fifteenth lies between two bf16 numbers and goes to the even one."""
+    g = torch.Generator().manual_seed(15)
+    r = 15 * torch.arange(257, 512, 2)            # 15 times an odd number of 9 bits
+    b = (r >> low << low) if low == 2 else torch.where(r < 4096, r >> 4 << 4, r >> 5 << 5)
+    x = torch.rand(len(r), 64, generator=g) * r[:, None] - (r - b)[:, None]
+    x = torch.minimum(torch.maximum(x, (b - r)[:, None].float()), b[:, None].float()).to(DT[dt])
+    x[:, 3], x[:, 40], x[:, 20], x[:, 63] = (b - r).to(DT[dt]), (b - r).to(DT[dt]), b.to(DT[dt]), b.to(DT[dt])
+    x = torch.cat([x, x * 2.0 ** -9, x * 2.0 ** 2, -x]).view(2, 2, len(r), 64)
+    _, scale, _ = plain_quantize(x)
+    assert (scale[0, 0].view(torch.int32) >> 16 & 1 == 0).float().mean() > 0.9  # the range is as meant
+    check_quantized(ops, x.cuda())
