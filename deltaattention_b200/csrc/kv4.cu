@@ -28,7 +28,9 @@ template <> struct Pair<__half> {
 // Codes of 8 elements x (pairs of T) against scale s > 0 with reciprocal r, and zero. The quotient
 // a / s is corrected from a r by one step with the exact remainder (Markstein, IBM J. Res. Dev. 34,
 // 1990), so it rounds as a division does; adding 1.5 * 2^23 rounds it to an integer, half to even,
-// in the number's lowest bits. 0 <= a <= 15.06 s: codes need no clamp.
+// in the number's lowest bits. s is at least KV4_FAST: its reciprocal and the remainders are fp32
+// numbers, and as it is rounded by 2^-9 at most, 0 <= a <= 15.06 s and codes need no clamp.
+constexpr float KV4_FAST = 0x1p-100f;
 template <typename T>
 __device__ __forceinline__ uint32_t kv4_code8(const typename Pair<T>::V* x, float s, float r, float zero) {
   uint32_t w = 0u;
@@ -42,6 +44,22 @@ __device__ __forceinline__ uint32_t kv4_code8(const typename Pair<T>::V* x, floa
   }
   // less the constant's own contributions, 0x4B400000 << 4 i, i = 0..7 (those past bit 31 are gone)
   return w - (0x4B400000u + 0xB4000000u + 0x40000000u);
+}
+// 16 elements of a group with minimum mn and maximum mx, whatever its scale: (codes, codes, scale, zero).
+// Scales down to bf16's subnormals (groups within 2^-96 of one value) are rounded by up to a third, so
+// that quotients pass 15, and have no reciprocal: divided, and cut.
+template <typename T>
+__device__ __noinline__ uint4 kv4_code16_any(uint4 a, uint4 b, float mn, float mx) {
+  using V = typename Pair<T>::V;
+  float s, zero;
+  kv4_scale_zero<true>(mn, mx, s, zero);
+  uint32_t w[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float2 f = Pair<T>::f32(reinterpret_cast<const V*>(i < 8 ? &a : &b)[(i & 7) >> 1]);
+    w[i >> 3] |= kv4_code(i & 1 ? f.y : f.x, s, zero) << (4 * (i & 7));
+  }
+  return make_uint4(w[0], w[1], __float_as_uint(s), __float_as_uint(zero));
 }
 
 template <typename T, int D>
@@ -79,10 +97,21 @@ __global__ void __launch_bounds__(256) kv4_quantize_kernel(const T* __restrict__
     hi = __hmax2_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, 1));
     const float2 l2 = Pair<T>::f32(lo), h2 = Pair<T>::f32(hi);
     float scale, zero;
-    kv4_scale_zero(fmin_nan(l2.x, l2.y), fmax_nan(h2.x, h2.y), scale, zero);
-    const bool ok = scale > 0.f;  // not 0 (a constant group), not NaN
+    const float mn = fmin_nan(l2.x, l2.y), mx = fmax_nan(h2.x, h2.y);
+    kv4_scale_zero<false>(mn, mx, scale, zero);
+    bool ok = scale > 0.f;  // not 0 (a constant group), not NaN
     const float step = ok ? scale : 1.f, r = __frcp_rn(step);
-    const uint32_t w0 = kv4_code8<T>(e, step, r, zero), w1 = kv4_code8<T>(e + 4, step, r, zero);
+    uint32_t w0 = kv4_code8<T>(e, step, r, zero), w1 = kv4_code8<T>(e + 4, step, r, zero);
+    if constexpr (TypeOf<T>::value == BF16) {  // fp16 has no such small steps
+      if (scale < KV4_FAST && mx > mn) {
+        const uint4 any = kv4_code16_any<T>(raw[i][0], raw[i][1], mn, mx);
+        w0 = any.x;
+        w1 = any.y;
+        scale = __uint_as_float(any.z);
+        zero = __uint_as_float(any.w);
+        ok = true;
+      }
+    }
     if (n < N) {
       c[n * (D / 8)] = ok ? w0 : 0u;
       c[n * (D / 8) + NG] = ok ? w1 : 0u;

@@ -242,3 +242,16 @@ def test_quantize_scales_between_two_numbers(ops, dt, low):
     _, scale, _ = plain_quantize(x)
     assert (scale[0, 0].view(torch.int32) >> 16 & 1 == 0).float().mean() > 0.9  # the range is as meant
     check_quantized(ops, x.cuda())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_quantize_tiny_groups(ops, D):
+    """bf16 groups down to the smallest subnormals, where a scale may round to a third of what it should be, or to 0,
+    and has no reciprocal in fp32."""
+    g = torch.Generator().manual_seed(D)
+    x = torch.randn(2, 3, 120, D, generator=g)
+    x[0, 0] += 3 * torch.randn(120, 1, generator=g)
+    x[0, 1, :, :D // 2] = (torch.rand(120, D // 2, generator=g) < 0.1).float()
+    x = (x * 2.0 ** (-92 - torch.arange(120) % 48)[:, None].double()).bfloat16()
+    check_quantized(ops, x.cuda())
