@@ -1,5 +1,6 @@
 // A decode history in 4 bits (format in kv4.cuh): quantisation of packed K / V rows, reading
 // back, and the single-token cache update.
+#include <cfloat>
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -47,7 +48,8 @@ __device__ __forceinline__ uint32_t kv4_code8(const typename Pair<T>::V* x, floa
 }
 // 16 elements of a group with minimum mn and maximum mx, whatever its scale: (codes, codes, scale, zero).
 // Scales down to bf16's subnormals (groups within 2^-96 of one value) are rounded by up to a third, so
-// that quotients pass 15, and have no reciprocal: divided, and cut.
+// that quotients pass 15, and have no reciprocal: divided, and cut. So are very large ones, whose
+// elements may lie further apart than fp32's largest number.
 template <typename T>
 __device__ __noinline__ uint4 kv4_code16_any(uint4 a, uint4 b, float mn, float mx) {
   using V = typename Pair<T>::V;
@@ -99,22 +101,26 @@ __global__ void __launch_bounds__(256) kv4_quantize_kernel(const T* __restrict__
     float scale, zero;
     const float mn = fmin_nan(l2.x, l2.y), mx = fmax_nan(h2.x, h2.y);
     kv4_scale_zero<false>(mn, mx, scale, zero);
-    bool ok = scale > 0.f;  // not 0 (a constant group), not NaN
-    const float step = ok ? scale : 1.f, r = __frcp_rn(step);
+    const bool fast = scale >= KV4_FAST && scale < 0x1p100f;
+    const float step = fast ? scale : 1.f, r = __frcp_rn(step);
     uint32_t w0 = kv4_code8<T>(e, step, r, zero), w1 = kv4_code8<T>(e + 4, step, r, zero);
-    if constexpr (TypeOf<T>::value == BF16) {  // fp16 has no such small steps
-      if (scale < KV4_FAST && mx > mn) {
-        const uint4 any = kv4_code16_any<T>(raw[i][0], raw[i][1], mn, mx);
-        w0 = any.x;
-        w1 = any.y;
-        scale = __uint_as_float(any.z);
-        zero = __uint_as_float(any.w);
-        ok = true;
+    if (!fast) {
+      w0 = w1 = 0u;
+      if (mx - mn != 0.f) {  // not a constant group (NaN and infinities give NaN)
+        if constexpr (TypeOf<T>::value == BF16) {
+          const uint4 any = kv4_code16_any<T>(raw[i][0], raw[i][1], mn, mx);
+          w0 = any.x;
+          w1 = any.y;
+          scale = __uint_as_float(any.z);
+          zero = __uint_as_float(any.w);
+        } else {  // fp16 has no other steps
+          scale = zero = __int_as_float(0x7FC00000);
+        }
       }
     }
     if (n < N) {
-      c[n * (D / 8)] = ok ? w0 : 0u;
-      c[n * (D / 8) + NG] = ok ? w1 : 0u;
+      c[n * (D / 8)] = w0;
+      c[n * (D / 8) + NG] = w1;
       s[n * (2 * NG)] = __float2bfloat16_rn(t == 0 ? scale : zero);
     }
   }
@@ -140,6 +146,16 @@ __global__ void __launch_bounds__(256) kv4_quantize_any_kernel(const T* __restri
   uint8_t* c = (is_v ? out.v_codes : out.k_codes) + b * out.cb + h * out.ch + n * (D / 2);
   __nv_bfloat16* s = (is_v ? out.v_scales : out.k_scales) + b * out.sb + h * out.sh + n * (2 * NG);
   kv4_quantize_row<NG>(r, reinterpret_cast<uint32_t*>(c), s, lane);
+}
+
+// Two values rounded to T, those past its largest numbers cut to them: the zero and 15 steps of a group at the
+// type's limits may lie outside them, and a finite group reads back finite. NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_cut(float lo, float hi) {
+  uint32_t d;
+  if constexpr (TypeOf<T>::value == BF16) asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
 }
 
 template <typename T, int D>
@@ -175,12 +191,13 @@ __global__ void __launch_bounds__(256) kv4_dequantize_kernel(Kv4Hist in, T* __re
       x[e] = fmaf(scale, __uint_as_float(((w[i] >> (4 * e)) & 15u) | 0x4B000000u) - 8388608.f, zero);
     T* o = dst + n * on;
     if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = fmin_nan(x[e], FLT_MAX);
       __stcs(reinterpret_cast<float4*>(o), make_float4(x[0], x[1], x[2], x[3]));
       __stcs(reinterpret_cast<float4*>(o) + 1, make_float4(x[4], x[5], x[6], x[7]));
     } else {
-      constexpr int bf = TypeOf<T>::value == BF16;
       __stcs(reinterpret_cast<uint4*>(o),
-             make_uint4(pack2(x[0], x[1], bf), pack2(x[2], x[3], bf), pack2(x[4], x[5], bf), pack2(x[6], x[7], bf)));
+             make_uint4(pack_cut<T>(x[0], x[1]), pack_cut<T>(x[2], x[3]), pack_cut<T>(x[4], x[5]), pack_cut<T>(x[6], x[7])));
     }
   }
 }

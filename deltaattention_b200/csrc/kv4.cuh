@@ -86,17 +86,23 @@ __device__ __forceinline__ float kv4_fifteenth(float x) {
 }
 
 // (scale, zero) of a group from its minimum and maximum; NaN for both when either is not finite. Without
-// ANY the scale of a range below 2^-64 is right to its order only.
+// ANY the scale of a range below 2^-64 is right to its order only, and a range past fp32's largest
+// number gives an infinite one.
 template <bool ANY>
 __device__ __forceinline__ void kv4_scale_zero(float mn, float mx, float& scale, float& zero) {
   zero = floor_bf16(mn);
-  scale = round_as<__nv_bfloat16>(kv4_fifteenth<ANY>(__fsub_rn(mx, zero)));
+  const float range = __fsub_rn(mx, zero);
+  float x = kv4_fifteenth<ANY>(range);
+  if (ANY && range == INFINITY) x = 2.f * kv4_fifteenth<false>(__fsub_rn(0.5f * mx, 0.5f * zero));
+  scale = round_as<__nv_bfloat16>(x);
   // an infinity or NaN in either makes the scale one
-  if (!(scale < INFINITY)) scale = zero = __int_as_float(0x7FC00000);
+  if (ANY && !(scale < INFINITY)) scale = zero = __int_as_float(0x7FC00000);
 }
 
+// Differences past fp32's largest number are taken by halves: scales from 2^100 on have room for that.
 __device__ __forceinline__ uint32_t kv4_code(float x, float scale, float zero) {
-  const float q = rintf(__fdiv_rn(__fsub_rn(x, zero), scale));
+  const float f = scale < 0x1p100f ? 1.f : 0.5f;
+  const float q = rintf(__fdiv_rn(__fsub_rn(x * f, zero * f), scale * f));
   // NaN (scale 0 or NaN) compares false and gives 0
   return q > 0.f && scale > 0.f ? static_cast<uint32_t>(fminf(q, 15.f)) : 0u;
 }

@@ -709,7 +709,7 @@ def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) ->
 
 def kv4_dequantize(hist: KV4, dtype: torch.dtype = torch.bfloat16):
     """The K and V rows that a 4-bit history stands for, [B, Hkv, M, d] each, rounded to ``dtype``
-    (bf16, fp16 or fp32) from fp32."""
+    (bf16, fp16 or fp32) from fp32; values past ``dtype``'s largest numbers are cut to them."""
     what = "kv4_dequantize"
     (B, H, M, D), st = hist.check(what, hist.k_codes)
     k = torch.empty((B, H, M, D), dtype=dtype, device=hist.k_codes.device)

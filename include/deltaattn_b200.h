@@ -338,7 +338,8 @@ int64_t dab_nm_num_packed(int64_t seq_len, int64_t n_keep, int64_t m_group, int6
 
 /* A decode history in 4 bits (no counterpart in the reference, whose cache is 16-bit). K and V
  * rows are kept as codes [B, H, capacity, head_dim / 2] bytes and scales [B, H, capacity,
- * head_dim / 16] bf16, both with contiguous rows. Per group g of 32 elements of a row, in fp32:
+ * head_dim / 16] bf16, both with contiguous rows. Per group g of 32 elements of a row, in fp32 (a
+ * range past its largest number is taken by halves):
  *   zero  = min rounded down to bf16;  scale = (max - zero) / 15 rounded to bf16;
  *   code  = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0;  value = zero + scale * code.
  * A group with an element that is not finite reads back as NaN. With NG = head_dim / 32, word
@@ -353,8 +354,8 @@ int dab_kv4_quantize(const void* k, const int64_t* k_strides, const void* v, con
                      void* v_codes, const int64_t* code_strides, void* k_scales, void* v_scales,
                      const int64_t* scale_strides, int dtype, int64_t batch, int64_t heads, int64_t rows,
                      int64_t head_dim, void* stream);
-/* The values of both, rounded to `dtype` (DAB_F32 too); `out_strides` (b, h, n) hold for k and v,
- * whose rows are contiguous. */
+/* The values of both, rounded to `dtype` (DAB_F32 too) and cut to its finite range; `out_strides`
+ * (b, h, n) hold for k and v, whose rows are contiguous. */
 int dab_kv4_dequantize(const void* k_codes, const void* v_codes, const int64_t* code_strides, const void* k_scales,
                        const void* v_scales, const int64_t* scale_strides, void* k, void* v,
                        const int64_t* out_strides, int dtype, int64_t batch, int64_t heads, int64_t rows,

@@ -255,3 +255,47 @@ def test_quantize_tiny_groups(ops, D):
     x[0, 1, :, :D // 2] = (torch.rand(120, D // 2, generator=g) < 0.1).float()
     x = (x * 2.0 ** (-92 - torch.arange(120) % 48)[:, None].double()).bfloat16()
     check_quantized(ops, x.cuda())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_quantize_ranges_past_fp32(ops, D):
+    """Finite bf16 groups whose range is above the largest fp32 number."""
+    g = torch.Generator().manual_seed(D)
+    top = torch.finfo(torch.bfloat16).max
+    x = (torch.rand(2, 2, 70, D, generator=g) * 2 - 1).mul(top).bfloat16()
+    x[..., 0], x[..., 31], x[..., 32], x[..., D - 1] = -top, top, -0.75 * top, 0.5 * top
+    x[1, :, :, 5] = 0.0
+    assert x.isfinite().all()
+    check_quantized(ops, x.cuda(), half=True)
+    k, v = ops.kv4_dequantize(ops.kv4_quantize(x.cuda(), x.cuda()), torch.float32)
+    _, scale, _ = plain_quantize(x, half=True)
+    step = scale.repeat_interleave(32, -1)
+    for y in (k, v):
+        assert y.isfinite().all() and ((y.cpu().double() - x.double()).abs() <= 0.501 * step.double()).all()
+
+
+@gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_read_back_at_the_types_limits(ops, dt):
+    """Groups that reach a type's largest numbers read back finite, half a step or a rounding away at most."""
+    g = torch.Generator().manual_seed(1)
+    top = torch.finfo(DT[dt]).max
+    x = ((torch.rand(1, 2, 200, 64, generator=g, dtype=torch.float64) * 2 - 1) * top).to(DT[dt])
+    x[0, 0, :, ::7], x[0, 0, :, 1::7] = top, -top
+    x[0, 1] = (0.9 + 0.1 * torch.rand(200, 64, generator=g, dtype=torch.float64)).mul(top).to(DT[dt])
+    x[0, 1, ::2] *= -1
+    x[0, 1, :, 5::32] = x[0, 1, :, 5:6].sign() * top
+    assert x.isfinite().all()
+    hist = ops.kv4_quantize(x.cuda(), x.cuda())
+    step = hist.k_scales[..., :2].cpu().double().repeat_interleave(32, -1)
+    for out in (torch.float32, DT[dt]):
+        for y in ops.kv4_dequantize(hist, out):
+            y = y.cpu().double()
+            near = 0.501 * step + UNIT.get(out, 2.0 ** -24) * y.abs() + (2.0 ** -7 * top if dt == "fp16" else 0.0)
+            assert y.isfinite().all() and ((y - x.double()).abs() <= near).all()  # fp16's zeros round down to bf16
+    x[0, :, ::3, 40] = float("inf")
+    x[0, :, 1::3, 41] = float("nan")
+    x[0, :, 2::3, 42] = -float("inf")
+    for y in ops.kv4_dequantize(ops.kv4_quantize(x.cuda(), x.cuda()), DT[dt]):
+        assert y[..., 32:].isnan().all() and y[..., :32].isfinite().all()
