@@ -951,6 +951,7 @@ int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, cons
   if (!workspace || workspace_bytes < kv4_attn_workspace(batch, heads, kv_group, head_dim, capacity, exact_window,
                                                          mass || exact_mass))
     return fail(1, std::string(nm) + ": workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(1, std::string(nm) + ": workspace must be 16-byte aligned");
   Kv4Attn p;
   std::memset(&p, 0, sizeof(p));
   p.q = q; p.qb = s[0]; p.qh = s[1];
@@ -991,6 +992,7 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
   if (trigger < budget) return fail(1, std::string(nm) + ": trigger must be at least budget");
   if (!workspace || workspace_bytes < evict_workspace(batch, heads, capacity))
     return fail(1, std::string(nm) + ": workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(1, std::string(nm) + ": workspace must be 16-byte aligned");
   EvictParams p;
   std::memset(&p, 0, sizeof(p));
   int64_t total = 0;

@@ -752,6 +752,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _own_workspace(what, t):
+    if t.dtype != torch.uint8 or not t.is_contiguous():
+        raise ValueError(f"{what}: workspace must be contiguous uint8")
+
+
 def decode_update_kv4(k_new, v_new, hist: KV4, counts, timestamps, lengths, last_key, k_exact, v_exact, seq_state, *,
                       threshold: float, similarity: str = "euclidean", mass=None, exact_mass=None, err=None):
     """Takes one token per (batch, kv-head) into a 4-bit decode cache (deltaDecoding.py:9-104).
@@ -869,6 +874,8 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     if workspace is None:
         nbytes = _kv4_workspace(dev, B, H, Hq // H, D, cap, W, mass is not None)
         workspace = L.workspace(q.device, st.value, nbytes, tag="kv4")
+    else:
+        _own_workspace(what, workspace)
     strides = L.int64s((qs[0], qs[1], *out.stride()[:2], *hs, *ms, *lengths.stride(), *es, *em))
     L.check(L.load().dab_decode_attention_kv4(
         q.data_ptr(), out.data_ptr(), hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), hist.k_scales.data_ptr(),
@@ -947,6 +954,8 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
     st = L.stream_of(mass)
     if workspace is None:
         workspace = L.workspace(mass.device, st.value, _evict_workspace(B, H, cap), tag="evict")
+    else:
+        _own_workspace(what, workspace)
     L.check(L.load().dab_evict_by_mass(
         mass.data_ptr(), L.int64s(mass.stride()[:2]), lengths.data_ptr(), L.int64s(lengths.stride()), len(ptrs),
         (L.P * len(ptrs))(*ptrs), L.int64s(tuple(nbytes)), L.int64s(tuple(strides)), B, H, cap, budget, trigger,

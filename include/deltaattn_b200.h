@@ -376,7 +376,8 @@ int dab_decode_update_kv4(const void* k_new, const void* v_new, void* k_codes, v
                           const int64_t* strides, float threshold, int use_cosine, int dtype, int64_t batch,
                           int64_t heads, int64_t head_dim, int64_t capacity, int64_t exact_window, int* err_word,
                           void* stream);
-/* Scratch bytes dab_decode_attention_kv4 needs, whatever they hold; used on one stream at a time. */
+/* Scratch bytes dab_decode_attention_kv4 needs, whatever they hold, 16-byte aligned; used on one
+ * stream at a time. */
 size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim,
                                                int64_t capacity, int64_t exact_window, int with_mass);
 /* Single-token attention over a 4-bit history and the exact window: q / out [B, heads * kv_group,
@@ -399,7 +400,7 @@ int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, cons
                              int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim, int64_t capacity,
                              int64_t exact_window, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Scratch bytes dab_evict_by_mass needs. Zero it once, then reuse it on one stream. */
+/* Scratch bytes dab_evict_by_mass needs, 16-byte aligned. Zero it once, then reuse it on one stream. */
 size_t dab_evict_by_mass_workspace_size(int64_t batch, int64_t heads, int64_t capacity);
 /* Eviction from a cache by accumulated attention weight (no counterpart in the reference). Every
  * (batch, head) longer than `trigger` (>= budget) is cut to `budget` entries: its first

@@ -299,3 +299,43 @@ def test_read_back_at_the_types_limits(ops, dt):
     x[0, :, 2::3, 42] = -float("inf")
     for y in ops.kv4_dequantize(ops.kv4_quantize(x.cuda(), x.cuda()), DT[dt]):
         assert y[..., 32:].isnan().all() and y[..., :32].isfinite().all()
+
+
+# ------------------------------------------------------------------------- workspaces and limits
+@pytest.fixture(scope="module")
+def lib():
+    import os
+    if not os.path.exists(L.LIB_PATH):
+        from deltaattention_b200 import build
+        build.build()
+    return L.load()
+
+
+def test_workspace_alignment_is_checked_on_the_host(lib):
+    import ctypes
+    z, p = (ctypes.c_int64 * 24)(), ctypes.c_void_p(4096)
+    said = lambda: lib.dab_last_error().decode()  # noqa: E731
+    for odd in (1, 4, 8):
+        ws = ctypes.c_void_p(8192 + odd)
+        assert lib.dab_decode_attention_kv4(p, p, p, p, p, p, p, None, p, p, p, None, None, 0, 0, z, 1.0, 2, 1, 1, 4, 64, 16,
+                                            8, ws, 1 << 30, None) == 1 and "workspace must be 16-byte aligned" in said()
+        assert lib.dab_evict_by_mass(p, z, p, z, 0, None, None, None, 1, 1, 64, 4, 4, 0, 0, ws, 1 << 30, None) == 1
+        assert "workspace must be 16-byte aligned" in said()
+
+
+@gpu
+def test_workspaces_that_are_refused(ops):
+    B, H, D, cap = 1, 2, 64, 32
+    x = torch.zeros(B, H, cap, D, dtype=torch.bfloat16, device="cuda")
+    hist, q = ops.kv4_quantize(x, x), torch.zeros(B, 4, D, dtype=torch.bfloat16, device="cuda")
+    c, n = torch.ones(B, H, cap, dtype=torch.int32, device="cuda"), torch.full((B, H), cap, dtype=torch.int32, device="cuda")
+    m = torch.zeros(B, H, cap, device="cuda")
+    room = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    for ws in (room[8:], room[1:], room[::2], room[:1].expand(1 << 16), room.view(torch.float32)):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            ops.decode_attention_kv4(q, hist, c, n, workspace=ws)
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            ops.evict_by_mass(m, n, [c], 4, workspace=ws)
+    ops.decode_attention_kv4(q, hist, c, n, workspace=room[16:])
+    ops.evict_by_mass(m, n, [c], 4, workspace=room.zero_()[16:])
+    assert (n == 4).all() and not room.view(torch.int32)[4]
