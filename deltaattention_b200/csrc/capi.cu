@@ -944,6 +944,10 @@ int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, cons
   // strides: q(2) out(2) codes(2) scales(2) meta(2) lengths(2) exact(3) exact_mass(2) = 17
   const int64_t* s = strides;
   if (int rc = kv4_check(nm, k_codes, v_codes, k_scales, v_scales, s + 4, s + 6, batch, heads, capacity, head_dim)) return rc;
+  // columns of a row of scores, and a kv-head's units of work over its groups of 8 q-heads, are 32-bit
+  const int64_t units = (capacity + 31) / 32 + (exact_window + 15) / 16 + 64;
+  if (capacity + exact_window >= (int64_t{1} << 31) - 4096 || (kv_group + 7) / 8 * units >= (int64_t{1} << 31))
+    return fail(1, std::string(nm) + ": capacity and exact_window are too long together, or for this many q-heads");
   const uintptr_t any = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_exact) |
                         reinterpret_cast<uintptr_t>(v_exact);
   if (any % 16 || (s[0] | s[1] | s[12] | s[13] | s[14]) % 8)

@@ -734,8 +734,8 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   if (p.state) elen = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(p.W), p.state[0] + p.lag)));
   if (p.state && blockIdx.x == 0 && tid == 0) *p.used = elen;
   // this piece: `left` units from unit `at` of head `bh` (all its groups of q-heads in a row)
-  int bh, at, left, ns = 1, split = 0;
-  int64_t start = 0, piece = 1;
+  int bh, at, ns = 1, split = 0;
+  int64_t left, start = 0, piece = 1;
   if (p.splits) {
     const int w = blockIdx.x / p.splits, z = w % hg;
     bh = w / hg;
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     ns = min(p.splits, un);
     if (split >= ns) return;
     const int u0 = static_cast<int>(static_cast<int64_t>(un) * split / ns);
-    left = static_cast<int>(static_cast<int64_t>(un) * (split + 1) / ns) - u0;
+    left = static_cast<int64_t>(un) * (split + 1) / ns - u0;
     at = z * un + u0;
   } else {
     // where it begins: the heads' units summed up, each thread a run of heads
@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
     piece = max(piece, static_cast<int64_t>(KV4_MIN_UNITS));
     start = piece * blockIdx.x;
     if (start >= total) return;
-    left = static_cast<int>(min(piece, total - start));
+    left = min(piece, total - start);
     if (first <= start && start < first + mine) {
       int k = tid * per;
       int64_t pos = first;
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
   const int ahead = p.splits ? 0 : KV4_START;  // units before a head's first that stand for its cost
   for (int part = 0; left > 0;) {
     const int n = p.splits ? kv4_len(p, bh) : lens[bh], un = kv4_units(n, elen), z = at / (un + ahead);
-    const int v0 = at - z * (un + ahead), v1 = min(un + ahead, v0 + left);
+    const int v0 = at - z * (un + ahead), v1 = static_cast<int>(min(static_cast<int64_t>(un + ahead), v0 + left));
     const int u0 = max(0, v0 - ahead), u1 = v1 - ahead;
     if (u0 < u1) {
       int slot = -1;

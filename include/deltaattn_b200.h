@@ -388,7 +388,8 @@ size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int
  * exact_mass. Weights are held in 16 bits or more, sums in 32 (of a history, within 2^-21 of the sum of
  * weight * (|zero| + scale * code) over its entries, whatever its length); elements of a query row
  * below 2^-26 of its largest are rounded to that step, value scales below 2^-40 lose precision and
- * values from 2^50 on may overflow. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
+ * values from 2^50 on may overflow. capacity and exact_window are below 2^30, together below 2^31 - 4096,
+ * and ceil(kv_group / 8) * (capacity / 32 + exact_window / 16 + 64) below 2^31. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
  * and `advance` as in dab_decode_attention_dev; without it exact_len is the argument.
  * `strides` (17): q (b, h), out (b, h), codes (b, h), scales (b, h), counts / mass (b, h), lengths
  * (b, h), exact K / V (b, h, row), exact_mass (b, h). Query and exact rows contiguous, 16-byte

@@ -339,3 +339,14 @@ def test_workspaces_that_are_refused(ops):
     ops.decode_attention_kv4(q, hist, c, n, workspace=room[16:])
     ops.evict_by_mass(m, n, [c], 4, workspace=room.zero_()[16:])
     assert (n == 4).all() and not room.view(torch.int32)[4]
+
+
+def test_attention_sizes_past_its_indexes_are_refused(lib):
+    """Columns of a row of scores, and the units of work of one kv-head, are 32-bit numbers."""
+    import ctypes
+    z, p = (ctypes.c_int64 * 24)(), ctypes.c_void_p(4096)
+    said = lambda: lib.dab_last_error().decode()  # noqa: E731
+    most = 2 ** 30 - 1
+    for G, cap, W in ((4, most, most), (1024, 64, 2 ** 28), (1024, 2 ** 29, 0)):
+        assert lib.dab_decode_attention_kv4(p, p, p, p, p, p, p, p, p, p, p, p, None, 0, 0, z, 1.0, 2, 1, 1, G, 64, cap, W, p,
+                                            (1 << 64) - 1, None) == 1 and "too long" in said(), (G, cap, W, said())
