@@ -8,6 +8,7 @@
 #include <cstring>
 #include <initializer_list>
 #include <mutex>
+#include <numeric>
 #include <string>
 
 #include "evict.cuh"
@@ -975,6 +976,18 @@ int dab_decode_attention_kv4(const void* q, void* out, const void* k_codes, cons
                      "decode_attention_kv4");
 }
 
+namespace {
+// whether two of B x H elements at b * sb + h * sh are one
+bool shared(int64_t sb, int64_t sh, int64_t B, int64_t H) {
+  sb = sb < 0 ? -sb : sb;
+  sh = sh < 0 ? -sh : sh;
+  if ((B > 1 && sb == 0) || (H > 1 && sh == 0)) return true;
+  if (B < 2 || H < 2) return false;
+  const int64_t g = std::gcd(sb, sh);  // sh / g steps over batch are sb / g over heads
+  return sh / g < B && sb / g < H;
+}
+}  // namespace
+
 size_t dab_evict_by_mass_workspace_size(int64_t batch, int64_t heads, int64_t capacity) {
   if (batch < 0 || heads < 0 || capacity < 0) return 0;
   return evict_workspace(batch, heads, capacity);
@@ -994,6 +1007,8 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
   if (budget < 1 || keep_first < 0 || keep_recent < 0 || keep_first > budget || keep_recent > budget - keep_first)
     return fail(1, std::string(nm) + ": need budget >= 1 and keep_first + keep_recent <= budget");
   if (trigger < budget) return fail(1, std::string(nm) + ": trigger must be at least budget");
+  if (shared(length_strides[0], length_strides[1], batch, heads))
+    return fail(1, std::string(nm) + ": lengths of different heads share memory");
   if (!workspace || workspace_bytes < evict_workspace(batch, heads, capacity))
     return fail(1, std::string(nm) + ": workspace too small");
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(1, std::string(nm) + ": workspace must be 16-byte aligned");

@@ -698,6 +698,7 @@ def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) ->
         st = (H * M * (D // 2), M * (D // 2), H * M * (D // 16), M * (D // 16))
     else:
         _, st = out.check(what, k, (B, H, M, D))
+        _apart(what, B, H, st)
     if B * H * M == 0:
         return out
     L.check(L.load().dab_kv4_quantize(
@@ -752,6 +753,12 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _apart(what, B, H, strides):
+    """Refuses written tensors whose sequences or heads share memory; ``strides``: (over batch, over heads, ..)."""
+    if (B > 1 and 0 in strides[::2]) or (H > 1 and 0 in strides[1::2]):
+        raise ValueError(f"{what}: tensors that are written must not be expanded")
+
+
 def _own_workspace(what, t):
     if t.dtype != torch.uint8 or not t.is_contiguous():
         raise ValueError(f"{what}: workspace must be contiguous uint8")
@@ -801,9 +808,13 @@ def decode_update_kv4(k_new, v_new, hist: KV4, counts, timestamps, lengths, last
         raise ValueError(f"{what}: the exact window needs at least one row")
     if k_new.numel() == 0:
         return
+    lens = lengths.stride()
+    _apart(what, B, H, (*hs, *ms, *lens, ls[0], ls[1], es[0], es[1], *(em if mass is not None else ())))
+    if W > 1 and es[2] == 0:
+        raise ValueError(f"{what}: tensors that are written must not be expanded")
     use_cos = similarity == "cosine"
     kn, vn = k_new.stride(), v_new.stride()
-    strides = L.int64s((kn[0], kn[1], kn[3], vn[0], vn[1], vn[3], *hs, *ms, *lengths.stride(), ls[0], ls[1], *es, *em))
+    strides = L.int64s((kn[0], kn[1], kn[3], vn[0], vn[1], vn[3], *hs, *ms, *lens, ls[0], ls[1], *es, *em))
     L.check(L.load().dab_decode_update_kv4(
         k_new.data_ptr(), v_new.data_ptr(), hist.k_codes.data_ptr(), hist.v_codes.data_ptr(), hist.k_scales.data_ptr(),
         hist.v_scales.data_ptr(), counts.data_ptr(), timestamps.data_ptr(), _ptr(mass), lengths.data_ptr(),
@@ -864,10 +875,13 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
             raise ValueError(f"{what}: counts and mass must have the same strides")
         if exact_mass is not None:
             em = _plane(what, "exact_mass", exact_mass, (B, H, W), torch.float32)
+        _apart(what, B, H, (*ms, *em) if W > 0 else ms)
     if out is None:
         out = q.new_empty(size)
     elif out.shape != size or out.dtype != dtype or out.stride(2) != 1:
         raise ValueError(f"{what}: out must be like q, with contiguous rows")
+    else:
+        _apart(what, B, Hq, out.stride()[:2])
     if B == 0 or Hq == 0:
         return out
     st = L.stream_of(q)
@@ -951,13 +965,15 @@ def evict_by_mass(mass, lengths, rows, budget: int, *, trigger: Optional[int] = 
         strides += (st[0] * width, st[1] * width)
     if B == 0 or H == 0 or cap == 0:
         return
+    ms, ls = mass.stride()[:2], lengths.stride()
+    _apart(what, B, H, (*ms, *ls, *strides))
     st = L.stream_of(mass)
     if workspace is None:
         workspace = L.workspace(mass.device, st.value, _evict_workspace(B, H, cap), tag="evict")
     else:
         _own_workspace(what, workspace)
     L.check(L.load().dab_evict_by_mass(
-        mass.data_ptr(), L.int64s(mass.stride()[:2]), lengths.data_ptr(), L.int64s(lengths.stride()), len(ptrs),
+        mass.data_ptr(), L.int64s(ms), lengths.data_ptr(), L.int64s(ls), len(ptrs),
         (L.P * len(ptrs))(*ptrs), L.int64s(tuple(nbytes)), L.int64s(tuple(strides)), B, H, cap, budget, trigger,
         int(keep_first), int(keep_recent), workspace.data_ptr(), workspace.numel(), st), what)
 

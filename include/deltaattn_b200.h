@@ -411,7 +411,7 @@ size_t dab_evict_by_mass_workspace_size(int64_t batch, int64_t heads, int64_t ca
  * they held) and the length [B, H] becomes `budget`. Row buffer i has `row_bytes[i]` contiguous
  * bytes per entry (a multiple of 4) and strides over batch and head of row_strides[2 i], [2 i + 1]
  * bytes; at most 8 buffers and 4096 bytes per entry. Strides of mass and lengths (b, h) in
- * elements. A wait inside the kernel that runs out (2 s) writes 0x501 into the workspace's first
+ * elements; heads must not share memory in any of them. A wait inside the kernel that runs out (2 s) writes 0x501 into the workspace's first
  * word (dab_workspace_error reads it); the cache is not valid then. */
 int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths, const int64_t* length_strides,
                       int64_t num_rows, void* const* rows, const int64_t* row_bytes, const int64_t* row_strides,

@@ -350,3 +350,81 @@ def test_attention_sizes_past_its_indexes_are_refused(lib):
     for G, cap, W in ((4, most, most), (1024, 64, 2 ** 28), (1024, 2 ** 29, 0)):
         assert lib.dab_decode_attention_kv4(p, p, p, p, p, p, p, p, p, p, p, p, None, 0, 0, z, 1.0, 2, 1, 1, G, 64, cap, W, p,
                                             (1 << 64) - 1, None) == 1 and "too long" in said(), (G, cap, W, said())
+
+
+@gpu
+def test_expanded_tensors_are_not_written(ops):
+    """Heads or sequences that share memory may be read; written they would spoil one another."""
+    B, H, D, cap, W = 2, 3, 64, 32, 4
+    x = torch.randn(B, H, cap, D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    hist = ops.kv4_quantize(x, x)
+    z = lambda *s, dt=torch.int32: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
+
+    def forms(make, *size):  # expanded over batch, over heads, over both
+        for s in ((1, H), (B, 1), (1, 1)):
+            yield make(*s, *size).expand(B, H, *size)
+
+    f32, bf = (lambda *s: z(*s, dt=torch.float32)), (lambda *s: z(*s, dt=torch.bfloat16))
+    q, n = x[:, :, 0].repeat_interleave(2, 1), torch.full((B, H), cap, dtype=torch.int32, device="cuda")
+    c, m, em, ring = z(B, H, cap) + 1, f32(B, H, cap), f32(B, H, W), bf(B, H, W, D)
+    bad = []
+    for t in forms(f32, cap):
+        bad += [lambda t=t: ops.evict_by_mass(t, n, [c], 4),
+                lambda t=t: ops.decode_attention_kv4(q, hist, z(1, 1, cap).expand_as(t), n, mass=t, exact_mass=None)]
+    for t in forms(z):
+        bad.append(lambda t=t: ops.evict_by_mass(m, t, [c], 4))
+    for t in forms(z, cap):
+        bad.append(lambda t=t: ops.evict_by_mass(m, n, [c, t], 4))
+    for t in forms(f32, W):
+        bad.append(lambda t=t: ops.decode_attention_kv4(q, hist, c, n, ring, ring, mass=m, exact_mass=t))
+    for t in (bf(1, 2 * H, D).expand(B, 2 * H, D), bf(B, 1, D).expand(B, 2 * H, D)):
+        bad.append(lambda t=t: ops.decode_attention_kv4(q, hist, c, n, out=t))
+    wide = ops.KV4.empty(1, H, cap, D, "cuda")
+    shared = ops.KV4(*(t.expand(B, *t.shape[1:]) for t in (wide.k_codes, wide.k_scales, wide.v_codes, wide.v_scales)))
+    bad.append(lambda: ops.kv4_quantize(x, x, out=shared))
+    new, state = x[:, :, :1], torch.tensor([5, 9], device="cuda")
+
+    def update(**kw):
+        a = dict(hist=hist, counts=c, timestamps=z(B, H, cap), lengths=z(B, H), last_key=bf(B, H, D), k_exact=ring,
+                 v_exact=ring.clone(), seq_state=state, threshold=1.0, mass=m, exact_mass=em)
+        ops.decode_update_kv4(new, new, **{**a, **kw})
+
+    bad.append(lambda: update(hist=shared))
+    for t, u in zip(forms(z, cap), forms(f32, cap)):
+        bad.append(lambda t=t, u=u: update(counts=t, timestamps=t, mass=u))
+    for t in forms(z):
+        bad.append(lambda t=t: update(lengths=t))
+    for t in forms(bf, D):
+        bad.append(lambda t=t: update(last_key=t))
+    for t in (*forms(bf, W, D), bf(B, H, 1, D).expand(B, H, W, D)):
+        bad.append(lambda t=t: update(k_exact=t, v_exact=t))
+    for t in forms(f32, W):
+        bad.append(lambda t=t: update(exact_mass=t))
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    assert (n == cap).all()
+    # read, they are taken: one sequence's history for all of them, counts and window of one head for all
+    one = ops.KV4(*(t[:1].expand_as(t) for t in (hist.k_codes, hist.k_scales, hist.v_codes, hist.v_scales)))
+    ones, w = (z(1, 1, cap) + 1).expand(B, H, cap), x[:1, :1, :W].expand(B, H, W, D)
+    out = ops.decode_attention_kv4(q, one, ones, n[:1, :1].expand(B, H), w, w)
+    same = ops.KV4(*(t.contiguous() for t in (one.k_codes, one.k_scales, one.v_codes, one.v_scales)))
+    assert torch.equal(out, ops.decode_attention_kv4(q, same, c, n, w.contiguous(), w.contiguous()))
+    update()
+    one_by_one = torch.zeros(1, 1, cap, device="cuda").expand(1, 1, cap)  # a stride of a single head is no stride
+    ops.evict_by_mass(one_by_one, n[:1, :1], [], 4)
+    assert n.flatten().tolist() == [4] + [cap] * 5
+
+
+def test_lengths_that_share_memory_are_refused(lib):
+    """A head's CTAs read its length one after another, and the first writes it: it has to be the head's own."""
+    import ctypes
+    z, p = (ctypes.c_int64 * 24)(), ctypes.c_void_p(4096)
+    for B, H, st, fine in ((2, 1, (0, 7), False), (1, 2, (7, 0), False), (2, 3, (1, 1), False), (2, 3, (2, 1), False),
+                           (4, 3, (2, 3), False), (2, 3, (-2, 1), False), (2, 3, (3, 1), True), (2, 3, (1, 2), True),
+                           (2, 3, (2, 3), True), (1, 1, (0, 0), True), (5, 1, (1, 0), True)):
+        ls = (ctypes.c_int64 * 2)(*st)
+        rc = lib.dab_evict_by_mass(p, z, p, ls, 0, None, None, None, B, H, 64, 4, 4, 0, 0, p, 8, None)
+        said = lib.dab_last_error().decode()
+        assert rc == 1 and ("workspace too small" if fine else "share memory") in said, (B, H, st, said)
