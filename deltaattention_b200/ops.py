@@ -843,7 +843,7 @@ def decode_attention_kv4(q, hist: KV4, counts, lengths, k_exact=None, v_exact=No
     (B, H, cap, D), hs = hist.check(what, q)
     dev = L.same_device(what, q, counts, lengths, k_exact, v_exact, seq_state, mass, exact_mass, out, workspace)
     size, qs = q.shape, q.stride()
-    if len(size) != 3 or size[0] != B or size[2] != D or size[1] % max(H, 1) or qs[2] != 1:
+    if len(size) != 3 or size[0] != B or size[2] != D or (size[1] % H if H else size[1]) or qs[2] != 1:
         raise ValueError(f"{what}: q must be [{B}, a multiple of {H}, {D}] with contiguous rows")
     dtype, Hq = q.dtype, size[1]
     if dtype not in _HALF:

@@ -428,3 +428,12 @@ def test_lengths_that_share_memory_are_refused(lib):
         rc = lib.dab_evict_by_mass(p, z, p, ls, 0, None, None, None, B, H, 64, 4, 4, 0, 0, p, 8, None)
         said = lib.dab_last_error().decode()
         assert rc == 1 and ("workspace too small" if fine else "share memory") in said, (B, H, st, said)
+
+
+@gpu
+def test_queries_without_heads_to_read(ops):
+    """q-heads over a history of no heads are refused like any other number that does not fit."""
+    x = torch.zeros(1, 0, 4, 64, dtype=torch.bfloat16, device="cuda")
+    c, n = torch.zeros(1, 0, 4, dtype=torch.int32, device="cuda"), torch.zeros(1, 0, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        ops.decode_attention_kv4(torch.zeros(1, 4, 64, dtype=torch.bfloat16, device="cuda"), ops.kv4_quantize(x, x), c, n)
