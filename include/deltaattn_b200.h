@@ -388,9 +388,10 @@ size_t dab_decode_attention_kv4_workspace_size(int64_t batch, int64_t heads, int
  * exact_mass. Weights are held in 16 bits or more, sums in 32 (of a history, within 2^-21 of the sum of
  * weight * (|zero| + scale * code) over its entries, whatever its length); elements of a query row
  * below 2^-26 of its largest are rounded to that step, value scales below 2^-40 lose precision and
- * values from 2^50 on may overflow. capacity and exact_window are below 2^30, together below 2^31 - 4096,
- * and ceil(kv_group / 8) * (capacity / 32 + exact_window / 16 + 64) below 2^31. With seq_state, exact_len is min(seq_state[0], exact_window) read on the device,
- * and `advance` as in dab_decode_attention_dev; without it exact_len is the argument.
+ * values from 2^50 on may overflow. capacity and exact_window are below 2^30, together below
+ * 2^31 - 4096, and ceil(kv_group / 8) * (capacity / 32 + exact_window / 16 + 64) below 2^31. With
+ * seq_state, exact_len is min(seq_state[0], exact_window) read on the device, and `advance` as in
+ * dab_decode_attention_dev; without it exact_len is the argument.
  * `strides` (17): q (b, h), out (b, h), codes (b, h), scales (b, h), counts / mass (b, h), lengths
  * (b, h), exact K / V (b, h, row), exact_mass (b, h). Query and exact rows contiguous, 16-byte
  * aligned. */
@@ -411,8 +412,9 @@ size_t dab_evict_by_mass_workspace_size(int64_t batch, int64_t heads, int64_t ca
  * they held) and the length [B, H] becomes `budget`. Row buffer i has `row_bytes[i]` contiguous
  * bytes per entry (a multiple of 4) and strides over batch and head of row_strides[2 i], [2 i + 1]
  * bytes; at most 8 buffers and 4096 bytes per entry. Strides of mass and lengths (b, h) in
- * elements; heads must not share memory in any of them. A wait inside the kernel that runs out (2 s) writes 0x501 into the workspace's first
- * word (dab_workspace_error reads it); the cache is not valid then. */
+ * elements; heads must not share memory in any of them. A wait inside the kernel that runs out (2 s)
+ * writes 0x501 into the workspace's first word (dab_workspace_error reads it); the cache is not valid
+ * then. */
 int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths, const int64_t* length_strides,
                       int64_t num_rows, void* const* rows, const int64_t* row_bytes, const int64_t* row_strides,
                       int64_t batch, int64_t heads, int64_t capacity, int64_t budget, int64_t trigger,
