@@ -2,7 +2,7 @@
 //
 // A row of D elements is cut into NG = D / 32 groups of 32. Per group, in fp32:
 //   zero  = min rounded down to bf16           (never above any element, so codes are >= 0)
-//   scale = (max - zero) / 15 rounded to bf16
+//   scale = (max - zero) * (1 / 15, as fp32) rounded to bf16
 //   code  = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0
 //   value = zero + scale * code
 // A group with an element that is not finite has scale = zero = NaN and reads back as NaN.
@@ -72,28 +72,14 @@ __device__ __forceinline__ float floor_bf16(float x) {
   return __uint_as_float((i + ((i >> 31) ? 0xFFFFu : 0u)) & 0xFFFF0000u);
 }
 
-// x / 15 as a division rounds it, x >= 0 the distance of two bf16 or fp16 numbers: the product with the
-// reciprocal, corrected by one step with the exact remainder (Markstein, IBM J. Res. Dev. 34, 1990).
-// With ANY small x are multiplied by 2^64 first, so that the remainder is an fp32 number. Equal to the
-// division for all 2^23 mantissas; where the fifteenth is subnormal, all x give the same bf16 number.
-// (A branch to a division for those took the update of 512 heads from 5.5 to 6.1 us.)
-template <bool ANY>
-__device__ __forceinline__ float kv4_fifteenth(float x) {
-  const bool small = ANY && x < 0x1p-64f;
-  x *= small ? 0x1p64f : 1.f;
-  const float q = __fmul_rn(x, 1.f / 15.f);
-  return __fmul_rn(fmaf(fmaf(-q, 15.f, x), 1.f / 15.f, q), small ? 0x1p-64f : 1.f);
-}
-
 // (scale, zero) of a group from its minimum and maximum; NaN for both when either is not finite. Without
-// ANY the scale of a range below 2^-64 is right to its order only, and a range past fp32's largest
-// number gives an infinite one.
+// ANY a range past fp32's largest number gives an infinite scale.
 template <bool ANY>
 __device__ __forceinline__ void kv4_scale_zero(float mn, float mx, float& scale, float& zero) {
   zero = floor_bf16(mn);
   const float range = __fsub_rn(mx, zero);
-  float x = kv4_fifteenth<ANY>(range);
-  if (ANY && range == INFINITY) x = 2.f * kv4_fifteenth<false>(__fsub_rn(0.5f * mx, 0.5f * zero));
+  float x = __fmul_rn(range, 1.f / 15.f);
+  if (ANY && range == INFINITY) x = 2.f * __fmul_rn(__fsub_rn(0.5f * mx, 0.5f * zero), 1.f / 15.f);
   scale = round_as<__nv_bfloat16>(x);
   // an infinity or NaN in either makes the scale one
   if (ANY && !(scale < INFINITY)) scale = zero = __int_as_float(0x7FC00000);

@@ -680,8 +680,8 @@ def kv4_quantize(k: torch.Tensor, v: torch.Tensor, out: Optional[KV4] = None) ->
     """K and V rows [B, Hkv, M, d] (any strides; bf16 / fp16, d 64 or 128) in 4 bits.
 
     Per group of 32 elements of a row, in fp32: zero = its minimum rounded down to bf16, scale = (maximum -
-    zero) / 15 rounded to bf16, code = round((x - zero) / scale) to even, cut to [0, 15]. A group
-    that holds a NaN or an infinity reads back as NaN. ``out`` may be views of a cache
+    zero) * (1 / 15, as an fp32 number) rounded to bf16, code = round((x - zero) / scale) to even, cut to
+    [0, 15]. A group that holds a NaN or an infinity reads back as NaN. ``out`` may be views of a cache
     (``KV4.rows``)."""
     what = "kv4_quantize"
     L.same_device(what, k, v)

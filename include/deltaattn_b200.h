@@ -340,7 +340,7 @@ int64_t dab_nm_num_packed(int64_t seq_len, int64_t n_keep, int64_t m_group, int6
  * rows are kept as codes [B, H, capacity, head_dim / 2] bytes and scales [B, H, capacity,
  * head_dim / 16] bf16, both with contiguous rows. Per group g of 32 elements of a row, in fp32 (a
  * range past its largest number is taken by halves):
- *   zero  = min rounded down to bf16;  scale = (max - zero) / 15 rounded to bf16;
+ *   zero  = min rounded down to bf16;  scale = (max - zero) * (1 / 15, as fp32) rounded to bf16;
  *   code  = clamp(rint((x - zero) / scale), 0, 15), 0 where scale is 0;  value = zero + scale * code.
  * A group with an element that is not finite reads back as NaN. With NG = head_dim / 32, word
  * t * NG + g (32 bits, t = 0..3) of a row's codes holds elements 32 g + 8 t + i in bits 4 i..;
