@@ -173,6 +173,9 @@ class Kv4DecodeCache:
     can be captured. Merge and append decisions are those of the 16-bit cache: the last anchor's key
     is kept in 16 bits for the comparison.
 
+    ``packed_lengths`` are [num_layers, B, Hkv], the counts, timestamps and masses [num_layers, B, Hkv, ..]
+    (``DeviceDecodeCache`` has its lengths as [num_layers, B * Hkv]).
+
     Attention adds every entry's weight to ``mass`` (history) and ``exact_mass`` (window; it moves with
     the token into the history). ``evict`` cuts heads to their heaviest entries by it, in place.
 

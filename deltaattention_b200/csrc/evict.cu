@@ -19,7 +19,7 @@
 //    row is read and written once, with no second buffer. The chain of dependent reads of a tile
 //    (ticket, place, entries, rows, flag) takes about 7 us, so what counts is how many kept rows the
 //    tiles in an SM's shared memory hold: tiles of the result hold nothing else. 8 heads of 131072
-//    16-bit entries cut to half take 92 us, 6.0 TB/s; tiles of the source, half of them evicted, took
+//    16-bit entries cut to half take 93 us, 5.9 TB/s; tiles of the source, half of them evicted, took
 //    130 us.
 #include <cooperative_groups.h>
 

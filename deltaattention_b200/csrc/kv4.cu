@@ -12,8 +12,8 @@ namespace dab {
 // against 5 D / 8 bytes of codes and scales. To quantise, a lane takes 16 neighbouring elements (two
 // 16-byte pieces, two code words); the 2 lanes of a group exchange minimum and maximum once, and
 // the pieces of KV4_QROWS rows are in flight. To read back, a lane takes 8 elements of KV4_ROWS rows.
-// 16 x 8 heads x 8191 rows of 128, K and V, in bf16 (705 MB each way): quantising 131 us (8 elements a lane: 189,
-// the group's scale and reciprocal are found four times), reading back 117 us, 6.0 TB/s.
+// 16 x 8 heads x 8191 rows of 128, K and V, in bf16 (705 MB each way): quantising 128 us (8 elements a lane: 189,
+// the group's scale and reciprocal are found four times), reading back 116 us, 6.1 TB/s.
 constexpr int KV4_ROWS = 4, KV4_QROWS = 4;
 
 template <typename T> struct Pair;

@@ -25,9 +25,9 @@
 //    are hundreds of times larger than what is left of them, and a product rounds the sum it adds to
 //    towards zero: added at the end, 100003 entries were 4e-6 of the terms off, all in one
 //    direction, 25 times the rounding of an fp16 output. Tile by tile, 1e-9 (8 shuffles and 32 FMA a
-//    tile, 3 us of the 72 below).
+//    tile, 3 us of the 73 below).
 //    With up to 4 q-heads the columns 4 to 7 hold them again: the first parts go into columns 0 to 3,
-//    the rest into 4 to 7, and one product does for two (72 us where 8 q-heads take 77, below).
+//    the rest into 4 to 7, and one product does for two (73 us where 8 q-heads take 77, below).
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
@@ -41,10 +41,10 @@ constexpr int KV4_NW = 4;      // warps per CTA, each with its own tiles and its
 constexpr int KV4_TILE = 32;   // keys per tile
 constexpr int KV4_STAGES = 2;  // tiles in a warp's ring
 constexpr int KV4_MAX_PIECES = 1024, KV4_MAX_HEADS = 2048;  // that are cut into pieces
-// of a piece: two tiles a warp (8 heads of 8192: 10.7 us; pieces of 4: 14.4, of 12: 11.9)
+// of a piece: two tiles a warp (8 heads of 8192: 10.5 us; pieces of 4: 12.6, of 12: 11.7)
 constexpr int KV4_MIN_UNITS = 8;
 // units that beginning and ending a head costs as much as (4 sequences of 65536 / 16 ragged ones with
-// mass: 71.5 / 36.7 us; none: 73.4 / 38.8; 3: 72.3 / 37.2; 9: 71.4 / 36.6)
+// mass: 73.1 / 37.4 us; none: 74.9 / 38.6; 3: 74.4 / 37.9; 9: 72.7 / 36.9)
 constexpr int KV4_START = 6;
 constexpr int KV4_BIAS = 64;      // log2 of what history weights carry until they are joined with the window's
 constexpr float KV4_SLACK = 8.f;  // log2 units a score may exceed the running maximum by before it moves
@@ -707,14 +707,14 @@ __device__ __forceinline__ void kv4_segment(const Kv4Attn& p, uint8_t* smem, uin
   __syncthreads();  // the ring may be filled again
 }
 
-// Bound by what the SMs issue: 16 keys take a warp about 330 instructions, 18 of them products, which
-// hold up the other pipes too, so that 60 % of the issue slots are used. Copies wait for nobody:
-// with all tiles from one address the time falls by 8 %. 12 warps an SM of 168 registers; 16 of 128
-// registers spill and take 7 % longer, a ring of 3 tiles changes nothing. bf16, d = 128, 4 q-heads
-// per kv-head, device times with the join:
-//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 72 us, 4.8 TB/s
+// Bound by what the SMs issue: 16 keys take a warp about 335 instructions, 18 of them products, which
+// hold up the other pipes too, so that 62 % of the issue slots are used. Copies are not what it waits
+// for: with all tiles from one address an earlier form took 8 % less. 12 warps an SM of 168 registers;
+// 16 of 128 registers spill and took 7 % longer, a ring of 3 tiles changed nothing. bf16, d = 128, 4
+// q-heads per kv-head, device times with the join:
+//   4 sequences of 65536 entries a head, 8 kv-heads (346 MB): 73 us, 4.7 TB/s
 //   16 sequences of 1024 to 8192 entries, 8 kv-heads (108 MB): 32 us, with mass 37 us
-//   1 sequence of 8192 entries: 10.8 us, most of it the latencies of two launches
+//   1 sequence of 8192 entries: 10.5 us, most of it the latencies of two launches
 //
 // With `splits` every head is cut into that many pieces (as many as it has units). Otherwise the
 // units of all heads in a row are cut into even pieces, one per CTA, whatever the heads' lengths: all
@@ -823,7 +823,7 @@ __global__ void __launch_bounds__(KV4_NW * 32, D == 64 ? 4 : 3) kv4_attn_kernel(
 // ---------------------------------------------------------------------------------- joining
 // Launched while the attention kernel ends (programmatic dependent launch): grid_wait returns once
 // that kernel's writes are there. Joining is a chain of dependent reads (the head's parts, their
-// maxima and sums, their outputs), 5.3 us alone. The mass reads the scores again and adds 6 us for 16
+// maxima and sums, their outputs), 5.3 us alone. The mass reads the scores again and adds 5 us for 16
 // sequences of 1024 to 8192 entries: 4 G bytes a key written and read, where a key has 5 D / 4. Four
 // q-heads at a time keep enough of its CTAs resident (eight at a time: 1.6 us more).
 // blockIdx.y: kv-head. The first G CTAs join the parts of one q-head each and write its output;
@@ -962,9 +962,9 @@ Kv4Plan kv4_plan(int64_t B, int64_t H, int64_t G, int64_t D, int64_t cap, int64_
   const int64_t slots = std::min<int64_t>((D == 64 ? 4 : 3) * static_cast<int64_t>(sms), KV4_MAX_PIECES);
   const int64_t units = std::max<int64_t>(1, (cap + KV4_TILE - 1) / KV4_TILE + (W + 15) / 16);
   w.splits = w.pieces = 0;
-  // Very many heads even out by themselves (2048 of 512: 71 us, as pieces 76; of 20 to 512: 62, 66).
-  // Few units run at once: where a piece begins needs no search (8 heads of 20000, just above the
-  // limit, took 17 us as pieces and 15 cut alike, before pieces counted the heads' beginnings).
+  // Very many heads even out by themselves (2048 of 512: 73 us, as pieces 78; of 20 to 512: 63, 67).
+  // Few units run at once, and where a piece begins needs no search (8 heads of 8192: 10.5 us, as
+  // pieces 11.9; of 20000, above the limit: as pieces 16.2, cut alike 19.6).
   if (heads >= std::min<int64_t>(4 * slots, KV4_MAX_HEADS)) w.splits = 1;
   else if (heads * units <= slots * KV4_MIN_UNITS)
     w.splits = static_cast<int>((units + KV4_MIN_UNITS - 1) / KV4_MIN_UNITS);
