@@ -76,6 +76,11 @@ SIGNATURES = {
     "dab_evict_by_mass_workspace_size": (SZ, [I64, I64, I64]),
     "dab_evict_by_mass": (I32, [P, PI64, P, PI64, I64, ctypes.POINTER(P), PI64, PI64, I64, I64, I64, I64, I64, I64, I64,
                                 P, SZ, P]),
+    "dab_paged_append": (I32, [P] * 11 + [PI64, I32, I32] + [I64] * 9 + [P, P]),
+    "dab_paged_attention_workspace_size": (SZ, [I64] * 6),
+    "dab_flash_varlen": (I32, [P] * 5 + [PI64, F32, I32, I32] + [I64] * 5 + [P, SZ, P]),
+    "dab_flash_paged": (I32, [P] * 7 + [PI64, F32, I32, I32] + [I64] * 8 + [P, SZ, P]),
+    "dab_decode_attention_paged": (I32, [P] * 8 + [PI64, F32, I32] + [I64] * 8 + [P, SZ, P]),
 }
 
 _lib = None
@@ -188,11 +193,11 @@ def workspace(device: torch.device, stream: int, nbytes: int, tag: str = "attn")
 
 
 def workspace_errors() -> list:
-    """Read and clear the error word of every attention, key-compression, projection, packing and
-    eviction workspace (synchronises)."""
+    """Read and clear the error word of every attention, key-compression, projection, packing,
+    eviction and paged-attention workspace (synchronises)."""
     codes = []
     for (tag, dev, st), buf in list(_ws_cache.items()):
-        if tag not in ("attn", "compress", "proj", "pack", "evict"):
+        if tag not in ("attn", "compress", "proj", "pack", "evict", "paged"):
             continue
         code = ctypes.c_int(0)
         check(load().dab_workspace_error(ptr(buf), ctypes.byref(code), ctypes.c_void_p(st)), "workspace_error")

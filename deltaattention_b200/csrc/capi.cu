@@ -13,6 +13,7 @@
 
 #include "evict.cuh"
 #include "kv4.cuh"
+#include "paged.cuh"
 #include "params.cuh"
 #include "../../include/deltaattn_b200.h"
 
@@ -66,6 +67,9 @@ cudaError_t launch_kv4_attn(int, int64_t, Kv4Attn, uint8_t*, cudaStream_t);
 size_t kv4_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, bool);
 cudaError_t launch_evict(EvictParams, uint8_t*, cudaStream_t);
 size_t evict_workspace(int64_t, int64_t, int64_t);
+cudaError_t launch_paged_append(int, bool, int, const PagedAppend&, int, cudaStream_t);
+cudaError_t launch_paged_attn(int, int, const PagedAttn&, uint8_t*, int, cudaStream_t);
+size_t paged_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
 }  // namespace dab
 
 using namespace dab;
@@ -1044,6 +1048,161 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
   p.first = static_cast<int>(keep_first); p.recent = static_cast<int>(keep_recent);
   return cuda_status(launch_evict(p, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream)),
                      "evict_by_mass");
+}
+
+// ------------------------------------------------------------------------- paged cache
+namespace {
+// what every entry on a paged cache checks; sets `shift` to log2(page_size)
+int paged_check(const char* nm, const void* k, const void* v, const int32_t* table, const int32_t* lengths,
+                int64_t batch, int64_t heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                int64_t max_pages, int* shift) {
+  if (!k || !v || !table || !lengths) return fail(1, std::string(nm) + ": null pointer");
+  if (head_dim != 64 && head_dim != 128) return fail(1, std::string(nm) + ": head_dim must be 64 or 128");
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(1, std::string(nm) + ": page_size must be a power of two from 16 to 256");
+  if (batch < 0 || heads < 1 || heads > 65535 || num_pages < 1 || max_pages < 1 ||
+      batch >= (int64_t{1} << 24) || num_pages >= (int64_t{1} << 31) || max_pages * page_size >= (int64_t{1} << 30))
+    return fail(1, std::string(nm) + ": need at least one head, page and column of the page table, sequences below 2^24, "
+                                     "pages below 2^31 and rows of a sequence below 2^30");
+  *shift = 0;
+  while ((int64_t{1} << *shift) < page_size) ++*shift;
+  return 0;
+}
+bool rows16(std::initializer_list<const void*> ptrs, const int64_t* strides, int n) {
+  uintptr_t any = 0;
+  for (const void* p : ptrs) any |= reinterpret_cast<uintptr_t>(p);
+  for (int i = 0; i < n; ++i) any |= static_cast<uintptr_t>(strides[i]) << 1;
+  return any % 16 == 0;
+}
+}  // namespace
+
+int dab_paged_append(const void* k, const void* v, const void* q, void* q_out, void* k_pages, void* v_pages,
+                     const int32_t* page_table, const int32_t* lengths, const int32_t* cu_seqlens, const void* cos,
+                     const void* sin, const int64_t* strides, int dtype, int table_dtype, int64_t tokens, int64_t batch,
+                     int64_t heads, int64_t q_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                     int64_t max_pages, int64_t table_rows, int* err_word, void* stream) {
+  const char* nm = "dab_paged_append";
+  int shift;
+  if (int rc = paged_check(nm, k_pages, v_pages, page_table, lengths, batch, heads, head_dim, num_pages, page_size, max_pages,
+                           &shift))
+    return rc;
+  if (!k || !v || !strides || !cos != !sin || !q != !q_out) return fail(1, std::string(nm) + ": null pointer");
+  if (dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": rows must be bf16 or fp16");
+  if (cos && table_dtype != F32 && table_dtype != dtype)
+    return fail(1, std::string(nm) + ": rotation tables must be fp32 or of the rows' type");
+  if (q && !cos) return fail(1, std::string(nm) + ": queries are only taken with rotation tables");
+  if (tokens < 0 || tokens >= (int64_t{1} << 31) || q_heads < 0 || q_heads > 65535 || (!q && q_heads) ||
+      (!cu_seqlens && tokens != batch) || (cos && (table_rows < 0 || table_rows >= (int64_t{1} << 31))))
+    return fail(1, std::string(nm) + ": bad sizes");
+  // strides: k(2) v(2) q(2) q_out(2) pool(3) page table(1) tables(1) = 13
+  const int64_t* s = strides;
+  if (!rows16({k, v, q, q_out, k_pages, v_pages, cos, sin}, s, 11) || s[12] % (table_dtype == F32 ? 4 : 8))
+    return fail(1, std::string(nm) + ": rows must be 16-byte aligned");
+  if (batch == 0) return 0;
+  PagedAppend p;
+  std::memset(&p, 0, sizeof(p));
+  p.k = k; p.k_t = s[0]; p.k_h = s[1];
+  p.v = v; p.v_t = s[2]; p.v_h = s[3];
+  p.q = q; p.q_t = s[4]; p.q_h = s[5];
+  p.q_out = q_out; p.qo_t = s[6]; p.qo_h = s[7];
+  p.kp = k_pages; p.vp = v_pages; p.p_p = s[8]; p.p_h = s[9]; p.p_r = s[10];
+  p.table = page_table; p.table_stride = s[11];
+  p.lengths = lengths; p.cu = cu_seqlens; p.cos = cos; p.sin = sin; p.cs_r = s[12]; p.err = err_word;
+  p.T = static_cast<int>(tokens); p.B = static_cast<int>(batch); p.H = static_cast<int>(heads);
+  p.Hq = static_cast<int>(q_heads); p.max_pages = static_cast<int>(max_pages);
+  p.num_pages = static_cast<int>(num_pages); p.ps_shift = shift; p.table_rows = static_cast<int>(table_rows);
+  return cuda_status(launch_paged_append(dtype, table_dtype == F32, static_cast<int>(head_dim), p, num_sms(),
+                                         static_cast<cudaStream_t>(stream)),
+                     "paged_append");
+}
+
+size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_group,
+                                          int64_t head_dim, int64_t prefix_groups) {
+  if (tokens < 0 || batch < 0 || heads < 1 || kv_group < 1 || head_dim < 1) return 0;
+  return WS_HEADER + paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, prefix_groups);
+}
+
+namespace {
+int paged_attend(const char* nm, PagedAttn& p, const int64_t* s, float sm_scale, int dtype, int64_t tokens, int64_t batch,
+                 int64_t heads, int64_t kv_group, int64_t head_dim, int64_t groups, void* workspace,
+                 size_t workspace_bytes, void* stream) {
+  if (!p.q || !p.out || !s) return fail(1, std::string(nm) + ": null pointer");
+  if (dtype != BF16 && dtype != F16) return fail(1, std::string(nm) + ": queries must be bf16 or fp16");
+  if (head_dim != 64 && head_dim != 128) return fail(1, std::string(nm) + ": head_dim must be 64 or 128");
+  if (kv_group < 1 || kv_group > 128) return fail(1, std::string(nm) + ": need 1 to 128 q-heads per kv-head");
+  if (tokens < 0 || batch < 0 || heads < 1 || heads * kv_group > 65535 || tokens >= (int64_t{1} << 30) ||
+      batch >= (int64_t{1} << 24) || groups < 0)
+    return fail(1, std::string(nm) + ": need 1 to 65535 q-heads, tokens below 2^30 and sequences below 2^24");
+  // strides: q(2) out(2) k(3: page, head, row) v(3) page table(1) = 11
+  if (!rows16({p.q, p.out, p.k, p.v}, s, 10)) return fail(1, std::string(nm) + ": rows must be 16-byte aligned");
+  if (!workspace || workspace_bytes < dab_paged_attention_workspace_size(tokens, batch, heads, kv_group, head_dim, groups))
+    return fail(1, std::string(nm) + ": workspace too small");
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return fail(1, std::string(nm) + ": workspace must be 16-byte aligned");
+  if (tokens == 0 || batch == 0) return 0;
+  p.q_t = s[0]; p.q_h = s[1]; p.o_t = s[2]; p.o_h = s[3];
+  p.k_p = s[4]; p.k_h = s[5]; p.k_r = s[6]; p.v_p = s[7]; p.v_h = s[8]; p.v_r = s[9];
+  p.table_stride = s[10];
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.T = static_cast<int>(tokens); p.B = static_cast<int>(batch); p.H = static_cast<int>(heads);
+  p.G = static_cast<int>(kv_group); p.groups = static_cast<int>(groups);
+  p.err = static_cast<int*>(workspace);
+  return cuda_status(launch_paged_attn(dtype, static_cast<int>(head_dim), p,
+                                       static_cast<uint8_t*>(workspace) + WS_HEADER, num_sms(),
+                                       static_cast<cudaStream_t>(stream)),
+                     nm);
+}
+}  // namespace
+
+int dab_flash_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
+                     const int64_t* strides, float sm_scale, int causal, int dtype, int64_t tokens, int64_t batch,
+                     int64_t heads, int64_t kv_group, int64_t head_dim, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  const char* nm = "dab_flash_varlen";
+  if (!k || !v || !cu_seqlens) return fail(1, std::string(nm) + ": null pointer");
+  PagedAttn p;
+  std::memset(&p, 0, sizeof(p));
+  p.q = q; p.out = out; p.k = k; p.v = v; p.cu = cu_seqlens; p.causal = causal != 0;
+  return paged_attend(nm, p, strides, sm_scale, dtype, tokens, batch, heads, kv_group, head_dim, 0, workspace,
+                      workspace_bytes, stream);
+}
+
+int dab_flash_paged(const void* q, void* out, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                    const int32_t* lengths, const int32_t* cu_seqlens, const int64_t* strides, float sm_scale, int causal,
+                    int dtype, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim,
+                    int64_t num_pages, int64_t page_size, int64_t max_pages, void* workspace, size_t workspace_bytes,
+                    void* stream) {
+  const char* nm = "dab_flash_paged";
+  PagedAttn p;
+  std::memset(&p, 0, sizeof(p));
+  if (int rc = paged_check(nm, k_pages, v_pages, page_table, lengths, batch, heads, head_dim, num_pages, page_size, max_pages,
+                           &p.ps_shift))
+    return rc;
+  if (!cu_seqlens) return fail(1, std::string(nm) + ": null pointer");
+  p.q = q; p.out = out; p.k = k_pages; p.v = v_pages; p.table = page_table; p.lengths = lengths; p.cu = cu_seqlens;
+  p.max_pages = static_cast<int>(max_pages); p.num_pages = static_cast<int>(num_pages); p.causal = causal != 0;
+  return paged_attend(nm, p, strides, sm_scale, dtype, tokens, batch, heads, kv_group, head_dim, 0, workspace,
+                      workspace_bytes, stream);
+}
+
+int dab_decode_attention_paged(const void* q, void* out, const void* k_pages, const void* v_pages,
+                               const int32_t* page_table, const int32_t* lengths, const int32_t* prefix_cu,
+                               const int32_t* prefix_lengths, const int64_t* strides, float sm_scale, int dtype,
+                               int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim, int64_t num_pages,
+                               int64_t page_size, int64_t max_pages, int64_t prefix_groups, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  const char* nm = "dab_decode_attention_paged";
+  PagedAttn p;
+  std::memset(&p, 0, sizeof(p));
+  if (int rc = paged_check(nm, k_pages, v_pages, page_table, lengths, batch, heads, head_dim, num_pages, page_size, max_pages,
+                           &p.ps_shift))
+    return rc;
+  if (prefix_groups < 0 || prefix_groups > batch || (prefix_groups > 0 && (!prefix_cu || !prefix_lengths)))
+    return fail(1, std::string(nm) + ": need at most one group per sequence, with prefix_cu and prefix_lengths");
+  p.q = q; p.out = out; p.k = k_pages; p.v = v_pages; p.table = page_table; p.lengths = lengths;
+  if (prefix_groups > 0) { p.prefix_cu = prefix_cu; p.prefix_len = prefix_lengths; }
+  p.max_pages = static_cast<int>(max_pages); p.num_pages = static_cast<int>(num_pages);
+  return paged_attend(nm, p, strides, sm_scale, dtype, batch, batch, heads, kv_group, head_dim, prefix_groups, workspace,
+                      workspace_bytes, stream);
 }
 
 }  // extern "C"

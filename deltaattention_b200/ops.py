@@ -988,6 +988,276 @@ def evict_workspace(batch, heads, capacity) -> int:
     return _evict_workspace(batch, heads, capacity)
 
 
+@dataclass
+class PagedKV:
+    """A pool of pages for the K and V rows of many sequences: k and v [num_pages, Hkv, page_size, d]
+    (bf16 / fp16, d 64 or 128, page_size a power of two from 16 to 256; the same strides, rows contiguous and
+    16-byte aligned, so [num_pages, page_size, Hkv, d] seen through ``transpose(1, 2)`` will do). Row p of
+    sequence b is row p % page_size of page ``page_table[b, p // page_size]``."""
+    k: torch.Tensor
+    v: torch.Tensor
+
+    @staticmethod
+    def empty(num_pages, heads, page_size, head_dim, dtype, device) -> "PagedKV":
+        k = torch.empty((num_pages, heads, page_size, head_dim), dtype=dtype, device=device)
+        return PagedKV(k, torch.empty_like(k))
+
+    def check(self, what, page_table, lengths, *others):
+        """Raises unless pool, ``page_table`` (int32 [B, max_pages]) and ``lengths`` (int32 [B]) fit together
+        on one device with ``others``; returns (device, B, num_pages, Hkv, page_size, d, max_pages)."""
+        k, v = self.k, self.v
+        dev = L.same_device(what, k, v, page_table, lengths, *others)
+        if k.dtype not in _HALF or v.dtype != k.dtype:
+            raise TypeError(f"{what}: pages must be bf16 or fp16")
+        size, st = k.shape, k.stride()
+        if len(size) != 4 or v.shape != size or v.stride() != st:
+            raise ValueError(f"{what}: k and v must be [num_pages, Hkv, page_size, d], with the same strides")
+        P, H, ps, D = size
+        if D not in (64, 128) or ps not in (16, 32, 64, 128, 256):
+            raise ValueError(f"{what}: need head_dim 64 or 128 and a page_size of 16, 32, 64, 128 or 256")
+        if P < 1 or H < 1:
+            raise ValueError(f"{what}: the pool needs at least one page and head")
+        _rows16(what, "pages", k, v)
+        if any(x == 0 for x, n in zip(st, size) if n > 1):
+            raise ValueError(f"{what}: pages must not be expanded")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1 or (
+                page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError(f"{what}: page_table must be int32 [B, max_pages] with contiguous rows")
+        _ints(what, "lengths", lengths, page_table.shape[0])
+        return dev, page_table.shape[0], P, H, ps, D, page_table.shape[1]
+
+
+def _rows16(what, name, *tensors):
+    """Refuses tensors whose rows (the last dimension) are not contiguous and 16-byte aligned."""
+    for t in tensors:
+        st = t.stride()
+        if st[-1] != 1 or t.data_ptr() % 16 or any(x * t.element_size() % 16 for x, n in zip(st[:-1], t.shape) if n > 1):
+            raise ValueError(f"{what}: rows of {name} must be contiguous and 16-byte aligned")
+
+
+def _ints(what, name, t, n):
+    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+        raise ValueError(f"{what}: {name} must be contiguous int32 [{n}]")
+
+
+def _packed(what, name, t, dtype, tokens=None, heads=None, head_dim=None):
+    """Checks [T, H, d] rows; returns (T, H, d, stride over T, stride over H)."""
+    size = t.shape
+    if len(size) != 3 or (tokens is not None and size[0] != tokens) or (heads is not None and size[1] != heads) or (
+            head_dim is not None and size[2] != head_dim):
+        raise ValueError(f"{what}: {name} must be [{'T' if tokens is None else tokens}, "
+                         f"{'H' if heads is None else heads}, {'d' if head_dim is None else head_dim}]")
+    if t.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype}")
+    _rows16(what, name, t)
+    st = t.stride()
+    # extents of 1 never move
+    return (*size, st[0] if size[0] > 1 else 0, st[1] if size[1] > 1 else 0)
+
+
+def _not_expanded(what, name, t):
+    if any(x == 0 for x, n in zip(t.stride(), t.shape) if n > 1):
+        raise ValueError(f"{what}: {name} is written and must not be expanded")
+
+
+def paged_append(k, v, pool: PagedKV, page_table, lengths, *, cu_seqlens=None, cos=None, sin=None, q=None, q_out=None,
+                 err=None):
+    """New K and V rows into a paged cache, rotated on the way; returns the rotated queries (None without ``q``).
+
+    k / v [T, Hkv, d], any token and head strides (e.g. views of one projection's output). With
+    ``cu_seqlens`` (int32 [B + 1] on the device, rising from 0) sequence b's rows are tokens
+    cu_seqlens[b] .. cu_seqlens[b + 1] - 1, and tokens from cu_seqlens[B] on are left alone; without it token b is
+    sequence b's only one (a decode step). ``lengths`` (int32 [B]) count the new rows, which become the
+    last ones of their sequences, so that a step raises them once for all layers; a token at a negative position
+    (an idle place of the batch, length 0) is skipped.
+
+    With ``cos`` / ``sin`` ([n, d] or [1, n, d] tables by position, fp32 or the rows' type) K goes in rotated
+    (``rope``'s formula, in fp32 and rounded once) and q [T, Hq, d] is rotated into ``q_out`` (allocated by default;
+    q itself is fine; rows of skipped tokens are not written). Without them K goes in as it is. ``err`` (int32
+    [1]) gets the first of 0x601 (a page number outside the pool), 0x602 (a length past the page table) and 0x603
+    (a position past the tables); such rows are not stored. New rows must not share a place in the pool."""
+    what = "paged_append"
+    dev, B, P, H, ps, D, mp = pool.check(what, page_table, lengths, k, v, cu_seqlens, cos, sin, q, q_out, err)
+    dtype = pool.k.dtype
+    T, _, _, k_t, k_h = _packed(what, "k", k, dtype, None, H, D)
+    _, _, _, v_t, v_h = _packed(what, "v", v, dtype, T, H, D)
+    if cu_seqlens is None:
+        if T != B:
+            raise ValueError(f"{what}: {T} tokens for {B} sequences: cu_seqlens says which are whose")
+    else:
+        _ints(what, "cu_seqlens", cu_seqlens, B + 1)
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: cos and sin come together")
+    rows, cs, table_dtype = 0, 0, dtype
+    if cos is not None:
+        if cos.dim() == 3 and cos.shape[0] == 1:
+            cos = cos[0]
+        if sin.dim() == 3 and sin.shape[0] == 1:
+            sin = sin[0]
+        if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.stride() != cos.stride():
+            raise ValueError(f"{what}: cos and sin must be [n, {D}] (or [1, n, {D}]), with the same strides")
+        if cos.dtype not in (torch.float32, dtype) or sin.dtype != cos.dtype:
+            raise TypeError(f"{what}: cos and sin must be fp32 or {dtype}")
+        _rows16(what, "cos and sin", cos, sin)
+        rows, cs, table_dtype = cos.shape[0], cos.stride(0) if cos.shape[0] > 1 else 0, cos.dtype
+    Hq, q_t, q_h, o_t, o_h = 0, 0, 0, 0, 0
+    if q is not None:
+        if cos is None:
+            raise ValueError(f"{what}: queries are rotated: cos and sin are needed")
+        _, Hq, _, q_t, q_h = _packed(what, "q", q, dtype, T, None, D)
+        if q_out is None:
+            q_out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
+        else:
+            _not_expanded(what, "q_out", q_out)
+        _, _, _, o_t, o_h = _packed(what, "q_out", q_out, dtype, T, Hq, D)
+    elif q_out is not None:
+        raise ValueError(f"{what}: q_out without q")
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+        raise ValueError(f"{what}: err must be int32")
+    if T == 0 or B == 0:
+        return q_out
+    pp, ph, pr, _ = pool.k.stride()
+    strides = L.int64s((k_t, k_h, v_t, v_h, q_t, q_h, o_t, o_h, pp if P > 1 else 0, ph if H > 1 else 0, pr,
+                        page_table.stride(0), cs))
+    L.check(L.load().dab_paged_append(
+        k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), pool.k.data_ptr(), pool.v.data_ptr(), page_table.data_ptr(),
+        lengths.data_ptr(), _ptr(cu_seqlens), _ptr(cos), _ptr(sin), strides, _HALF[dtype],
+        0 if table_dtype == torch.float32 else _HALF[dtype], T, B, H, Hq, D, P, ps, mp, rows, _ptr(err),
+        L.stream_of(k)), what)
+    return q_out
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(device, tokens, batch, kv_heads, kv_group, head_dim, groups) -> int:
+    # asked with `device` current: the split of the work goes by its number of SMs
+    return int(L.load().dab_paged_attention_workspace_size(tokens, batch, kv_heads, kv_group, head_dim, groups))
+
+
+def paged_attention_workspace(tokens, batch, q_heads, kv_heads, head_dim, prefix_groups=0) -> int:
+    """Bytes of the ``workspace`` that ``flash_varlen``, ``flash_paged`` and ``decode_attention_paged``
+    (tokens = batch there) take on the current device."""
+    return _paged_workspace(torch.cuda.current_device(), tokens, batch, kv_heads, q_heads // kv_heads, head_dim,
+                            prefix_groups)
+
+
+def _paged_call(what, dev, q, out, workspace, B, H, D, dtype, groups=0):
+    """Checks queries, output and workspace of an attention call; returns (out, Hq / Hkv, their strides,
+    workspace, stream), out alone where there is nothing to do."""
+    T, Hq, _, q_t, q_h = _packed(what, "q", q, dtype, None, None, D)
+    if Hq % H:
+        raise ValueError(f"{what}: query heads must be a multiple of {H}")
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
+    else:
+        _not_expanded(what, "out", out)
+    _, _, _, o_t, o_h = _packed(what, "out", out, dtype, T, Hq, D)
+    if T == 0 or B == 0 or Hq == 0:
+        return out, None
+    st = L.stream_of(q)
+    if workspace is None:
+        workspace = L.workspace(q.device, st.value, _paged_workspace(dev, T, B, H, Hq // H, D, groups), tag="paged")
+    else:
+        _own_workspace(what, workspace)
+    return out, (T, Hq // H, (q_t, q_h, o_t, o_h), workspace, st)
+
+
+def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, workspace=None):
+    """Dense attention of sequences of different lengths packed back to back, in one launch: ``flash`` without
+    padding.
+
+    q [T, Hq, d], k / v [T, Hkv, d] (bf16 / fp16, d 64 or 128, any token and head strides; q-head h reads kv-head
+    h // (Hq / Hkv), at most 128 q-heads per kv-head), cu_seqlens int32 [B + 1] on the device, rising from 0: it
+    is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] from cu_seqlens[B] on are left
+    alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and may reach rows before it
+    within the same 128 keys.
+
+    ``workspace`` (uint8, ``paged_attention_workspace`` bytes, zero-filled once, used by one stream at a time)
+    replaces the library's own, which is given up when a later call needs a larger one: a call that is
+    captured in a CUDA graph takes the caller's."""
+    what = "flash_varlen"
+    dev = L.same_device(what, q, k, v, cu_seqlens, out, workspace)
+    if q.dtype not in _HALF:
+        raise TypeError(f"{what}: queries must be bf16 or fp16")
+    T, H, D, k_t, k_h = _packed(what, "k", k, q.dtype, q.shape[0])
+    if D not in (64, 128) or H < 1:
+        raise ValueError(f"{what}: need head_dim 64 or 128 and at least one kv-head")
+    _, _, _, v_t, v_h = _packed(what, "v", v, q.dtype, T, H, D)
+    B = cu_seqlens.numel() - 1
+    _ints(what, "cu_seqlens", cu_seqlens, max(B, 0) + 1)
+    out, call = _paged_call(what, dev, q, out, workspace, B, H, D, q.dtype)
+    if call is None:
+        return out
+    T, G, st4, ws, st = call
+    L.check(L.load().dab_flash_varlen(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(),
+        L.int64s((*st4, 0, k_h, k_t, 0, v_h, v_t, 0)), float(D ** -0.5 if sm_scale is None else sm_scale),
+        1 if causal else 0, _HALF[q.dtype], T, B, H, G, D, ws.data_ptr(), ws.numel(), st), what)
+    return out
+
+
+def _pool_strides(pool, page_table):
+    P, H = pool.k.shape[:2]
+    pp, ph, pr, _ = pool.k.stride()
+    one = (pp if P > 1 else 0, ph if H > 1 else 0, pr)
+    return (*one, *one, page_table.stride(0))
+
+
+def flash_paged(q, pool: PagedKV, page_table, lengths, cu_seqlens, *, causal=True, sm_scale=None, out=None,
+                workspace=None):
+    """``flash_varlen`` over a paged cache: sequence b's queries (tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 of q
+    [T, Hq, d]) are the last of its ``lengths[b]`` rows, which ``paged_append`` has put into the pool: a whole
+    prompt, a piece of one, or the prompt behind a prefix that is cached already. A query at a negative position
+    gives 0. Everything else as in ``flash_varlen``."""
+    what = "flash_paged"
+    dev, B, P, H, ps, D, mp = pool.check(what, page_table, lengths, q, cu_seqlens, out, workspace)
+    _ints(what, "cu_seqlens", cu_seqlens, B + 1)
+    out, call = _paged_call(what, dev, q, out, workspace, B, H, D, pool.k.dtype)
+    if call is None:
+        return out
+    T, G, st4, ws, st = call
+    L.check(L.load().dab_flash_paged(
+        q.data_ptr(), out.data_ptr(), pool.k.data_ptr(), pool.v.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+        cu_seqlens.data_ptr(), L.int64s((*st4, *_pool_strides(pool, page_table))),
+        float(D ** -0.5 if sm_scale is None else sm_scale), 1 if causal else 0, _HALF[q.dtype], T, B, H, G, D, P, ps, mp,
+        ws.data_ptr(), ws.numel(), st), what)
+    return out
+
+
+def decode_attention_paged(q, pool: PagedKV, page_table, lengths, *, prefix_cu=None, prefix_lengths=None, sm_scale=None,
+                           out=None, workspace=None):
+    """One token's attention per sequence over a paged cache: q [B, Hq, d] over the sequence's ``lengths[b]`` rows
+    (a sequence of length 0 gives 0).
+
+    Sequences that begin alike (answers to one prompt, users of one document) share pages. Groups of consecutive
+    ones are given by ``prefix_cu`` (int32 [G + 1] on the device, rising from 0: group g is sequences
+    prefix_cu[g] .. prefix_cu[g + 1] - 1, those from prefix_cu[G] on are in none) and ``prefix_lengths`` (int32
+    [G]): the first prefix_lengths[g] rows are the same for all members, whose page tables begin with the same
+    pages. Whole pages of them are read once for the group. Everything else as in ``flash_varlen``."""
+    what = "decode_attention_paged"
+    dev, B, P, H, ps, D, mp = pool.check(what, page_table, lengths, q, prefix_cu, prefix_lengths, out, workspace)
+    if q.dim() != 3 or q.shape[0] != B:
+        raise ValueError(f"{what}: q must be [{B}, Hq, {D}]")
+    if (prefix_cu is None) != (prefix_lengths is None):
+        raise ValueError(f"{what}: prefix_cu and prefix_lengths come together")
+    groups = 0
+    if prefix_cu is not None:
+        groups = prefix_lengths.numel()
+        _ints(what, "prefix_lengths", prefix_lengths, groups)
+        _ints(what, "prefix_cu", prefix_cu, groups + 1)
+        if groups > B:
+            raise ValueError(f"{what}: {groups} groups of {B} sequences")
+    out, call = _paged_call(what, dev, q, out, workspace, B, H, D, pool.k.dtype, groups)
+    if call is None:
+        return out
+    _, G, st4, ws, st = call
+    L.check(L.load().dab_decode_attention_paged(
+        q.data_ptr(), out.data_ptr(), pool.k.data_ptr(), pool.v.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+        _ptr(prefix_cu), _ptr(prefix_lengths), L.int64s((*st4, *_pool_strides(pool, page_table))),
+        float(D ** -0.5 if sm_scale is None else sm_scale), _HALF[q.dtype], B, H, G, D, P, ps, mp, groups,
+        ws.data_ptr(), ws.numel(), st), what)
+    return out
+
+
 def tile_count_periodic(N: int, r: int, W: int = 128) -> int:
     """128x128 tiles one head runs under the reference schedule with periodic-r packing."""
     nb = -(-N // 128)

@@ -420,6 +420,66 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
                       int64_t batch, int64_t heads, int64_t capacity, int64_t budget, int64_t trigger,
                       int64_t keep_first, int64_t keep_recent, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- paged K / V cache
+ * (no counterpart in the reference). A pool holds pages of `page_size` rows (a power of two, 16 to
+ * 256) for every K / V head: K and V [num_pages, heads, page_size, head_dim] by strides, rows
+ * contiguous and 16-byte aligned, head_dim 64 or 128, bf16 or fp16. Row p of sequence b is row p % page_size
+ * of page page_table[b][p / page_size]; the table [B, max_pages] (int32, row stride given) and `lengths`
+ * [B] (int32, the rows of every sequence) are on the device. A page number outside the pool, a length past
+ * the table, a position past the rotation tables and a sequence outside the tokens are never followed: they
+ * write 0x601, 0x602, 0x603, 0x604 into the error word (the first one stays) and that sequence's results are
+ * not valid. */
+
+/* New rows into the pages. k / v [tokens, heads, head_dim]: with cu_seqlens [B + 1] (int32, rising from 0;
+ * tokens from cu_seqlens[B] on are left alone) sequence b's are tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1,
+ * without it (NULL) token b is sequence b's only one, tokens = B. `lengths` count the new rows: they are the
+ * sequence's last ones. A token whose position would be negative (an idle sequence of length 0) is skipped.
+ * With cos / sin [table_rows, head_dim] (fp32 or `dtype`) K row x at position p goes in as
+ * x cos[p] + (-x[d/2:], x[:d/2]) sin[p], in fp32 and rounded once, and so do the q rows [tokens, q_heads,
+ * head_dim] into q_out (both or neither; q_out may be q). No two new rows may share a place in the pool.
+ * `strides` (13): k (token, head), v (token, head), q (token, head), q_out (token, head), pool (page, head, row;
+ * of K and V alike), page table (row), cos / sin (row). err_word (int32) may be NULL. */
+int dab_paged_append(const void* k, const void* v, const void* q, void* q_out, void* k_pages, void* v_pages,
+                     const int32_t* page_table, const int32_t* lengths, const int32_t* cu_seqlens, const void* cos,
+                     const void* sin, const int64_t* strides, int dtype, int table_dtype, int64_t tokens, int64_t batch,
+                     int64_t heads, int64_t q_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+                     int64_t max_pages, int64_t table_rows, int* err_word, void* stream);
+
+/* Scratch bytes of the three calls below (prefix_groups 0 but for decoding), 16-byte aligned. Zero it once,
+ * then reuse it on one stream; its first word is the error word (dab_workspace_error). */
+size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_group,
+                                          int64_t head_dim, int64_t prefix_groups);
+
+/* Attention of sequences packed back to back: q / out [tokens, heads * kv_group, head_dim], k / v [tokens, heads,
+ * head_dim], offsets cu_seqlens as above. q-head h reads K / V head h / kv_group; query i of a sequence sees its rows
+ * 0 .. i (causal) or all of them. `strides` (11): q (token, head), out (token, head), k (unused, head, token),
+ * v (unused, head, token), unused. */
+int dab_flash_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
+                     const int64_t* strides, float sm_scale, int causal, int dtype, int64_t tokens, int64_t batch,
+                     int64_t heads, int64_t kv_group, int64_t head_dim, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* The same over the pages: sequence b's queries are the last of its `lengths[b]` rows, which are in the pool
+ * already. A query at a negative position gives 0. `strides` (11): q (token, head), out (token, head), K pages
+ * (page, head, row), V pages (page, head, row), page table (row). */
+int dab_flash_paged(const void* q, void* out, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                    const int32_t* lengths, const int32_t* cu_seqlens, const int64_t* strides, float sm_scale, int causal,
+                    int dtype, int64_t tokens, int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim,
+                    int64_t num_pages, int64_t page_size, int64_t max_pages, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* One token per sequence: q / out [B, heads * kv_group, head_dim], over the sequence's lengths[b] rows (0: the
+ * output is 0). With prefix_groups > 0, sequences prefix_cu[g] .. prefix_cu[g + 1] - 1 (int32 [groups + 1],
+ * rising from 0, the sequences from prefix_cu[groups] on in no group) have the same first prefix_lengths[g] rows
+ * (int32): whole pages of them are read once for all, through the page table of a longest member. Strides as for
+ * dab_flash_paged. */
+int dab_decode_attention_paged(const void* q, void* out, const void* k_pages, const void* v_pages,
+                               const int32_t* page_table, const int32_t* lengths, const int32_t* prefix_cu,
+                               const int32_t* prefix_lengths, const int64_t* strides, float sm_scale, int dtype,
+                               int64_t batch, int64_t heads, int64_t kv_group, int64_t head_dim, int64_t num_pages,
+                               int64_t page_size, int64_t max_pages, int64_t prefix_groups, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
