@@ -4,6 +4,7 @@
 // stream, launches asynchronously on that stream and returns 0 or a nonzero status whose
 // message `dab_last_error()` returns. No entry point allocates device memory: scratch is
 // passed in by the caller (sizes from the *_workspace_size functions).
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <initializer_list>
@@ -68,8 +69,8 @@ size_t kv4_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, 
 cudaError_t launch_evict(EvictParams, uint8_t*, cudaStream_t);
 size_t evict_workspace(int64_t, int64_t, int64_t);
 cudaError_t launch_paged_append(int, bool, int, const PagedAppend&, int, cudaStream_t);
-cudaError_t launch_paged_attn(int, int, const PagedAttn&, uint8_t*, int, cudaStream_t);
-size_t paged_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
+cudaError_t launch_paged_attn(int, int, PagedAttn&, uint8_t*, int, cudaStream_t);
+size_t paged_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, bool, int);
 }  // namespace dab
 
 using namespace dab;
@@ -1118,11 +1119,34 @@ int dab_paged_append(const void* k, const void* v, const void* q, void* q_out, v
 
 size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_group,
                                           int64_t head_dim, int64_t prefix_groups) {
-  if (tokens < 0 || batch < 0 || heads < 1 || kv_group < 1 || head_dim < 1) return 0;
-  return WS_HEADER + paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, prefix_groups);
+  if (tokens < 0 || batch < 0 || heads < 1 || kv_group < 1 || kv_group > 128 || head_dim < 1 || prefix_groups < 0) return 0;
+  const int sms = num_sms();
+  size_t n = paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, 0, false, sms);
+  if (tokens == batch)
+    n = std::max(n, paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, prefix_groups, true, sms));
+  return WS_HEADER + n;
 }
 
 namespace {
+// 4-D map of 16-bit rows of d elements: extents and strides (elements) of the other dimensions, a box of 64
+// elements by `box`, 128-byte swizzle. Extents of 1 never move: their stride is a harmless legal one.
+bool encode_paged(CUtensorMap* m, const void* base, int dtype, int64_t d, const int64_t (&ext)[3], const int64_t (&str)[3],
+                  uint32_t box1, uint32_t box2) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return false;
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(d)}, strides[3];
+  for (int i = 0; i < 3; ++i) {
+    dims[i + 1] = static_cast<cuuint64_t>(ext[i]);
+    strides[i] = static_cast<cuuint64_t>(ext[i] > 1 ? str[i] * 2 : d * 2);
+    if (ext[i] < 1 || strides[i] % 16 != 0 || strides[i] == 0 || strides[i] >= (1ull << 40)) return false;
+  }
+  cuuint32_t box[4] = {64, box1, box2, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(m, dtype == BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 int paged_attend(const char* nm, PagedAttn& p, const int64_t* s, float sm_scale, int dtype, int64_t tokens, int64_t batch,
                  int64_t heads, int64_t kv_group, int64_t head_dim, int64_t groups, void* workspace,
                  size_t workspace_bytes, void* stream) {
@@ -1133,6 +1157,7 @@ int paged_attend(const char* nm, PagedAttn& p, const int64_t* s, float sm_scale,
   if (tokens < 0 || batch < 0 || heads < 1 || heads * kv_group > 65535 || tokens >= (int64_t{1} << 30) ||
       batch >= (int64_t{1} << 24) || groups < 0)
     return fail(1, std::string(nm) + ": need 1 to 65535 q-heads, tokens below 2^30 and sequences below 2^24");
+  if (!(sm_scale > 0.f) || sm_scale > 1e30f) return fail(1, std::string(nm) + ": sm_scale must be positive");
   // strides: q(2) out(2) k(3: page, head, row) v(3) page table(1) = 11
   if (!rows16({p.q, p.out, p.k, p.v}, s, 10)) return fail(1, std::string(nm) + ": rows must be 16-byte aligned");
   if (!workspace || workspace_bytes < dab_paged_attention_workspace_size(tokens, batch, heads, kv_group, head_dim, groups))
@@ -1146,6 +1171,19 @@ int paged_attend(const char* nm, PagedAttn& p, const int64_t* s, float sm_scale,
   p.T = static_cast<int>(tokens); p.B = static_cast<int>(batch); p.H = static_cast<int>(heads);
   p.G = static_cast<int>(kv_group); p.groups = static_cast<int>(groups);
   p.err = static_cast<int*>(workspace);
+  const uint32_t tpt = static_cast<uint32_t>(128 / kv_group), G = static_cast<uint32_t>(kv_group);
+  const int64_t ps = int64_t{1} << p.ps_shift;
+  bool ok = encode_paged(&p.tm_q, p.q, dtype, head_dim, {heads * kv_group, tokens, 1}, {p.q_h, p.q_t, 0}, G, tpt) &&
+            encode_paged(&p.tm_q1, p.q, dtype, head_dim, {heads * kv_group, tokens, 1}, {p.q_h, p.q_t, 0}, G, 1);
+  if (p.table) {
+    const uint32_t rows = static_cast<uint32_t>(ps < 128 ? ps : 128);
+    ok = ok && encode_paged(&p.tm_k, p.k, dtype, head_dim, {ps, heads, p.num_pages}, {p.k_r, p.k_h, p.k_p}, rows, 1) &&
+         encode_paged(&p.tm_v, p.v, dtype, head_dim, {ps, heads, p.num_pages}, {p.v_r, p.v_h, p.v_p}, rows, 1);
+  } else {
+    ok = ok && encode_paged(&p.tm_k, p.k, dtype, head_dim, {tokens, heads, 1}, {p.k_r, p.k_h, 0}, 128, 1) &&
+         encode_paged(&p.tm_v, p.v, dtype, head_dim, {tokens, heads, 1}, {p.v_r, p.v_h, 0}, 128, 1);
+  }
+  if (!ok) return fail(1, std::string(nm) + ": strides must be positive, and below 2^40 bytes");
   return cuda_status(launch_paged_attn(dtype, static_cast<int>(head_dim), p,
                                        static_cast<uint8_t*>(workspace) + WS_HEADER, num_sms(),
                                        static_cast<cudaStream_t>(stream)),
@@ -1200,6 +1238,7 @@ int dab_decode_attention_paged(const void* q, void* out, const void* k_pages, co
     return fail(1, std::string(nm) + ": need at most one group per sequence, with prefix_cu and prefix_lengths");
   p.q = q; p.out = out; p.k = k_pages; p.v = v_pages; p.table = page_table; p.lengths = lengths;
   if (prefix_groups > 0) { p.prefix_cu = prefix_cu; p.prefix_len = prefix_lengths; }
+  p.decode = 1;
   p.max_pages = static_cast<int>(max_pages); p.num_pages = static_cast<int>(num_pages);
   return paged_attend(nm, p, strides, sm_scale, dtype, batch, batch, heads, kv_group, head_dim, prefix_groups, workspace,
                       workspace_bytes, stream);

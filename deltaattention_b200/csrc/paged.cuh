@@ -28,6 +28,8 @@ struct PagedAppend {
 };
 
 struct PagedAttn {
+  // maps of the queries (a tile of tokens, and one token) and of the K / V rows, made at the launch
+  CUtensorMap tm_q, tm_q1, tm_k, tm_v;
   const void* q; void* out; int64_t q_t, q_h, o_t, o_h;          // [T, Hq, D]
   const void* k; const void* v; int64_t k_p, k_h, k_r, v_p, v_h, v_r;  // pool, or (table null) rows [T, H, D]
   const int32_t* table; int64_t table_stride;
@@ -37,6 +39,12 @@ struct PagedAttn {
   int* err;
   float scale_log2;                                              // sm_scale * log2(e)
   int T, B, H, G, max_pages, num_pages, ps_shift, groups, causal;
+  int decode;     // one token per sequence, the work cut into even ranges of key tiles
+  int may_split;  // prompts: the units may be too few for the SMs
+  int num_ctas;
+  // workspace: piece counter and finished CTAs, records of sequences and groups, partial results
+  unsigned* counter;
+  int64_t* rec_tile; int64_t* rec_row; float* part_o; float2* part_s;
 };
 
 // Records a wrong argument that only the device sees; the first one stays.

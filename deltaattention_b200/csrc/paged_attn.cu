@@ -1,88 +1,1306 @@
-// Attention of packed prompts, of prompts over a paged cache, and of one token per sequence over it.
+// Attention of packed prompts, of prompts over a paged cache, and of one token per sequence over it, on
+// tcgen05 tensor cores.
 //
-// out_i = sum_{j < limit_i} softmax_j(scale q_i . k_j) v_j, limit_i = the query's position + 1 (causal) or
-// the sequence's length; q-head h reads K / V head h / G. A row that sees nothing gives 0.
+//   out_i = sum_{j < limit_i} softmax_j(scale q_i . k_j) v_j,
+// limit_i = the query's position + 1 (causal) or the sequence's length; q-head h reads K / V head h / G.
 //
-// One block of 128 threads per (query, q-head): 128 keys at a time, a score per thread, the running
-// maximum and sum in fp32, then an output element per thread.
+// Rows of a 128-row query tile are (token, q-head of one K / V head) pairs, 128 / G tokens by G heads, so
+// that every K / V head's rows are loaded once for all of its q-heads. A unit is two such tiles over the
+// same keys, a piece a range of a unit's 128-key tiles. Three kinds of units:
+//   prompts   2 * (128 / G) consecutive tokens of a sequence; causal tiles end at their last row's limit;
+//   prefixes  as many sequences of a group that shares its first pages, one token each: these pages are
+//             read once for all of them;
+//   own       one token of one sequence over the rows behind its prefix: G rows. Bytes bound it, and the
+//             two tiles hold the same rows and take every other key tile, two chains at a time.
+// With `decode` the key tiles of all units, one after the other, are cut into one even range per CTA
+// (bytes and, for tiles of 256 rows, products cost the same per tile). Prompts take pieces from a counter,
+// heavy ones first; where whole units would leave SMs idle they are cut into chunks of L key tiles, the
+// units of one chunk next to each other so that they find its keys in L2. Pieces of cut units leave fp32
+// partial sums with their maxima, joined by a second kernel.
+//
+// One persistent CTA per SM, 384 threads: warp 0 fetches pieces, publishes them to all other warps and
+// loads Q and K; warp 3 loads V; warps 1 and 2 issue the products of the two tiles; warps 4-7 and 8-11 are
+// the tiles' softmax, a row per thread. The loads are TMA boxes of a page (or of 128 packed rows), scores
+// and weights live in TMEM, weights in the rows' 16-bit type: an error of half a step per weight, as large as
+// that of the rounded output. The running maximum moves only when a row outgrows it by 2^8.
+#include <type_traits>
+
 #include "paged.cuh"
 
 namespace dab {
 
-template <int D, typename T>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttn p) {
-  __shared__ float sq[D], sp[128], red[4];
-  __shared__ int sb;
-  const int t = blockIdx.x, hq = blockIdx.y, h = hq / p.G, tid = threadIdx.x;
-  if (tid < 32) {
-    const int b = p.cu ? paged_sequence(p.cu, p.B, t) : t;
-    if (tid == 0) sb = b;
-  }
-  if (tid < D) sq[tid] = to_f32(static_cast<const T*>(p.q)[t * p.q_t + hq * p.q_h + tid]) * p.scale_log2;
-  __syncthreads();
-  const int b = sb;
-  if (b < 0) return;
-  int c0, c1;
-  paged_tokens(p.cu, b, p.T, p.err, c0, c1);
-  const int n = c1 - c0;
-  const int len = p.table ? paged_length(p.lengths[b], p.max_pages, p.ps_shift, p.err) : n;
-  const int limit = p.causal ? len - n + (t - c0) + 1 : len;
-  float m = -INFINITY, l = 0.f, o = 0.f;
-  auto row_of = [&](int j, int64_t& ko, int64_t& vo) {
-    if (!p.table) {
-      ko = static_cast<int64_t>(c0 + j) * p.k_r + h * p.k_h;
-      vo = static_cast<int64_t>(c0 + j) * p.v_r + h * p.v_h;
-      return true;
-    }
-    const int page = p.table[b * p.table_stride + (j >> p.ps_shift)], r = j & ((1 << p.ps_shift) - 1);
-    if (page < 0 || page >= p.num_pages) {
-      paged_error(p.err, ERR_PAGE);
-      return false;
-    }
-    ko = page * p.k_p + h * p.k_h + r * p.k_r;
-    vo = page * p.v_p + h * p.v_h + r * p.v_r;
-    return true;
-  };
-  for (int j0 = 0; j0 < limit; j0 += 128) {
-    const int j = j0 + tid;
-    float s = -INFINITY;
-    int64_t ko, vo;
-    if (j < limit) {
-      s = 0.f;
-      if (row_of(j, ko, vo))
-        for (int d = 0; d < D; ++d) s += sq[d] * to_f32(static_cast<const T*>(p.k)[ko + d]);
-    }
-    float mx = s;
-    for (int o2 = 16; o2; o2 >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o2));
-    if ((tid & 31) == 0) red[tid >> 5] = mx;
-    __syncthreads();
-    const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float base = mn == -INFINITY ? 0.f : mn, f = ex2(m - base);
-    sp[tid] = ex2(s - base);
-    m = mn;
-    __syncthreads();
-    l *= f;
-    o *= f;
-    for (int i = 0; i < 128 && j0 + i < limit; ++i) {
-      l += sp[i];
-      if (tid < D && row_of(j0 + i, ko, vo)) o += sp[i] * to_f32(static_cast<const T*>(p.v)[vo + tid]);
-    }
-    __syncthreads();
-  }
-  if (tid < D) static_cast<T*>(p.out)[t * p.o_t + hq * p.o_h + tid] = from_f32<T>(limit > 0 ? o / l : 0.f);
+constexpr int PT_THREADS = 384;
+constexpr int PT_BN = 128;   // keys of a tile
+constexpr int PT_RING = 4;   // pieces published ahead
+constexpr int PT_ROWS = 256; // partial rows between the pieces of neighbouring CTAs
+constexpr int PT_MIN_CHUNK = 4;
+constexpr int PT_FILL = 3;   // chunks per SM that cut prompts aim at
+
+struct Piece {
+  int end;         // no more pieces
+  int tok0, ntok;  // first token, tokens
+  int h;           // K / V head
+  int trow;        // row of the page table; first row of the sequence for packed rows
+  int kb;          // first key of key tile 0
+  int kend;        // keys that exist: rows from here on are not read
+  int j0, nt0, nt1;  // key tiles: from j0 up to nt0 for tile 0, nt1 for tile 1
+  int alt;         // both tiles hold the same rows, tile x takes key tiles j0 + x, j0 + x + 2, ..
+  int lim0, lim_step;  // keys that token tok0 + i sees: lim0 + i * lim_step ..
+  int by_length;   // .. and no more than the token's sequence has
+  int split;       // partial results to rows orow0 / orow1, else the output
+  int q1;          // one token: the query box of one token
+  int64_t orow0, orow1;
+  __device__ __forceinline__ int jend() const { return max(nt0, nt1); }
+};
+
+template <int D> struct PtCfg {
+  static constexpr int QBYTES = 128 * D * 2;
+  static constexpr int KVBYTES = PT_BN * D * 2;
+  static constexpr int NK = (D == 128) ? 2 : 4;
+  static constexpr int NV = (D == 128) ? 2 : 4;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = 2 * QBYTES;
+  static constexpr int OFF_V = OFF_K + NK * KVBYTES;
+  static constexpr int EPI_PITCH = 80;  // 64 bytes of a row's output and 16 more against bank conflicts
+  static constexpr int OFF_EPI = OFF_V + NV * KVBYTES;
+  static constexpr int OFF_PIECE = OFF_EPI + 8 * 32 * EPI_PITCH;
+  static constexpr int OFF_BAR = OFF_PIECE + PT_RING * static_cast<int>(sizeof(Piece));
+  static constexpr int NBAR = 2 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 5 + 1 + 2;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int SMEM = OFF_MISC + 256 + 1024;  // and slack for alignment
+};
+
+// ------------------------------------------------------------------------------------ the work
+__device__ __forceinline__ int64_t shfl64(int64_t v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
+
+// Whether the groups of sequences rise inside the batch; the whole block calls it.
+__device__ __forceinline__ bool groups_ok(const PagedAttn& p) {
+  if (!p.groups) return true;
+  bool bad = false;
+  for (int g = threadIdx.x; g < p.groups; g += blockDim.x)
+    bad |= p.prefix_cu[g + 1] < p.prefix_cu[g] || p.prefix_cu[g] < 0 || p.prefix_cu[g + 1] > p.B;
+  const bool any = __syncthreads_or(bad);
+  if (any && threadIdx.x == 0) paged_error(p.err, ERR_STARTS);
+  return !any;
 }
 
-size_t paged_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t) { return 256; }
+// Rows of group g's prefix that are read for all: whole pages.
+__device__ __forceinline__ int prefix_rows(const PagedAttn& p, int g) {
+  const int64_t most = static_cast<int64_t>(p.max_pages) << p.ps_shift;
+  const int n = static_cast<int>(min(static_cast<int64_t>(max(p.prefix_len[g], 0)), most));
+  return n >> p.ps_shift << p.ps_shift;
+}
+// The group of sequence b, or -1.
+__device__ __forceinline__ int group_of(const PagedAttn& p, int groups, int b) {
+  if (!groups || b < p.prefix_cu[0] || b >= p.prefix_cu[groups]) return -1;
+  int lo = 0, hi = groups;  // cu[lo] <= b < cu[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.prefix_cu[mid] <= b) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
 
-cudaError_t launch_paged_attn(int dtype, int head_dim, const PagedAttn& p, uint8_t*, int, cudaStream_t st) {
-  if (p.T == 0) return cudaSuccess;
-  const dim3 grid(p.T, p.H * p.G);
-  if (dtype == BF16 && head_dim == 64) paged_attn_kernel<64, __nv_bfloat16><<<grid, 128, 0, st>>>(p);
-  else if (dtype == BF16 && head_dim == 128) paged_attn_kernel<128, __nv_bfloat16><<<grid, 128, 0, st>>>(p);
-  else if (dtype == F16 && head_dim == 64) paged_attn_kernel<64, __half><<<grid, 128, 0, st>>>(p);
-  else if (dtype == F16 && head_dim == 128) paged_attn_kernel<128, __half><<<grid, 128, 0, st>>>(p);
-  else return cudaErrorInvalidValue;
-  return cudaGetLastError();
+// Items of a decode step: the groups, then the sequences. Every item has `units` units for each K / V head, of
+// `tiles` key tiles each, and `rows` partial rows for each head.
+struct Item {
+  int first, count;  // sequences
+  int start, len;    // rows [start, len) of the sequences
+  int tiles, units, rows, alt;
+};
+__device__ __forceinline__ Item decode_item(const PagedAttn& p, int groups, int tpt, int i) {
+  Item it;
+  if (i < groups) {
+    it.first = p.prefix_cu[i];
+    it.count = p.prefix_cu[i + 1] - it.first;
+    it.start = 0;
+    it.len = it.count ? prefix_rows(p, i) : 0;
+    it.units = (it.count + 2 * tpt - 1) / (2 * tpt);
+    it.alt = it.count <= tpt;
+  } else {
+    const int b = i - groups;
+    const int g = group_of(p, groups, b);
+    it.first = b;
+    it.count = 1;
+    it.len = paged_length(p.lengths[b], p.max_pages, p.ps_shift, p.err);
+    it.start = g < 0 ? 0 : min(prefix_rows(p, g), it.len);
+    it.units = 1;
+    it.alt = 1;
+  }
+  it.tiles = (it.len - it.start + PT_BN - 1) / PT_BN;
+  it.rows = it.count * p.G * (it.alt ? 2 : 1);
+  return it;
+}
+
+// Exclusive sums over the block's threads of two numbers; returns the totals.
+__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t* smem, int64_t& ta, int64_t& tb) {
+  const int lane = lane_id(), warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  int64_t sa = a, sb = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t ua = __shfl_up_sync(0xFFFFFFFFu, sa, o), ub = __shfl_up_sync(0xFFFFFFFFu, sb, o);
+    if (lane >= o) {
+      sa += ua;
+      sb += ub;
+    }
+  }
+  if (lane == 31) {
+    smem[warp] = sa;
+    smem[nw + warp] = sb;
+  }
+  __syncthreads();
+  int64_t pa = 0, pb = 0;
+  ta = tb = 0;
+  for (int w = 0; w < nw; ++w) {
+    if (w == warp) {
+      pa = ta;
+      pb = tb;
+    }
+    ta += smem[w];
+    tb += smem[nw + w];
+  }
+  __syncthreads();
+  a = pa + sa - a;
+  b = pb + sb - b;
+}
+
+// A prompt's sequence: queries [c0, c1), `len` keys, `nq` units of 2 * tpt tokens and `mt` key tiles.
+struct Seq {
+  int c0, n, len, nq, mt;
+};
+__device__ __forceinline__ Seq prompt_seq(const PagedAttn& p, int utok, int b) {
+  Seq s;
+  int c1;
+  paged_tokens(p.cu, b, p.T, p.err, s.c0, c1);
+  s.n = c1 - s.c0;
+  s.len = s.n == 0 ? 0 : p.table ? paged_length(p.lengths[b], p.max_pages, p.ps_shift, p.err) : s.n;
+  s.nq = (s.n + utok - 1) / utok;
+  s.mt = max(1, (s.len + PT_BN - 1) / PT_BN);
+  return s;
+}
+// Key tiles of a chunk, or 0 where units stay whole.
+__device__ __forceinline__ int chunk_tiles(const PagedAttn& p, int64_t units, int64_t tiles) {
+  if (!p.may_split || units >= 2 * static_cast<int64_t>(p.num_ctas)) return 0;
+  const int64_t per = static_cast<int64_t>(PT_FILL) * p.num_ctas;
+  return static_cast<int>(min(max((tiles + per - 1) / per, static_cast<int64_t>(PT_MIN_CHUNK)), int64_t{1} << 24));
+}
+__device__ __forceinline__ int64_t prompt_pieces(const PagedAttn& p, const Seq& s, int chunk) {
+  return static_cast<int64_t>(p.H) * s.nq * (chunk ? (s.mt + chunk - 1) / chunk : 1);
+}
+
+// every lane of the warp waits; the outcome is warp-uniform
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t par, const Abort& ab, int code) {
+  const bool ok = mbar_wait(bar, par, ab, code);
+  return __all_sync(0xFFFFFFFFu, ok);
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ------------------------------------------------------------------------------------ pieces
+// The pieces of one CTA, in order; all lanes of warp 0 call it.
+struct Sched {
+  int64_t pos, end;             // decode: key tiles left
+  int i0, n;                    // items i0 .. i0 + 31 of n are in the lanes
+  int64_t base_t, base_r;       // tiles (pieces) and rows before item i0
+  int64_t cnt, inc_t, rows, inc_r;  // the lane's item: its count, the inclusive sums
+  Item item;
+  Seq seq;
+  int groups, tpt, chunk;
+
+  __device__ __forceinline__ void load(const PagedAttn& p) {
+    const int i = i0 + lane_id();
+    cnt = rows = 0;
+    if (i < n) {
+      if (p.decode) {
+        item = decode_item(p, groups, tpt, i);
+        cnt = static_cast<int64_t>(p.H) * item.units * item.tiles;
+        rows = static_cast<int64_t>(p.H) * item.rows;
+      } else {
+        seq = prompt_seq(p, 2 * tpt, i);
+        cnt = prompt_pieces(p, seq, chunk);
+      }
+    }
+    inc_t = cnt;
+    inc_r = rows;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t a = __shfl_up_sync(0xFFFFFFFFu, inc_t, o), b = __shfl_up_sync(0xFFFFFFFFu, inc_r, o);
+      if (lane_id() >= o) {
+        inc_t += a;
+        inc_r += b;
+      }
+    }
+  }
+  // the lane whose item has place `at`; -1 past the last item. Sets the place within it.
+  __device__ __forceinline__ int find(const PagedAttn& p, int64_t at, int64_t& off) {
+    while (at >= base_t + shfl64(inc_t, 31)) {
+      base_t += shfl64(inc_t, 31);
+      base_r += shfl64(inc_r, 31);
+      i0 += 32;
+      if (i0 >= n) return -1;
+      load(p);
+    }
+    const int src = __ffs(__ballot_sync(0xFFFFFFFFu, at < base_t + inc_t)) - 1;
+    off = at - base_t - (shfl64(inc_t, src) - shfl64(cnt, src));
+    return src;
+  }
+  __device__ __forceinline__ int get(int v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
+
+  __device__ __forceinline__ void next(const PagedAttn& p, Piece& pc) {
+    const int lane = lane_id();
+    pc.end = 1;
+    if (p.decode) {
+      if (pos >= end) return;
+      int64_t off;
+      const int src = find(p, pos, off);
+      if (src < 0) return;
+      const int first = get(item.first, src), count = get(item.count, src), start = get(item.start, src);
+      const int len = get(item.len, src), tiles = get(item.tiles, src), units = get(item.units, src);
+      const int irows = get(item.rows, src), alt = get(item.alt, src);
+      const int64_t row0 = base_r + shfl64(inc_r, src) - shfl64(rows, src);
+      const bool shared = i0 + src < groups;
+      const int u = static_cast<int>(off / tiles), up = u % units;
+      pc.h = u / units;
+      pc.j0 = static_cast<int>(off % tiles);
+      const int take = static_cast<int>(min(static_cast<int64_t>(tiles - pc.j0), end - pos));
+      pos += take;
+      pc.tok0 = first + up * 2 * tpt;
+      pc.ntok = min(2 * tpt, count - up * 2 * tpt);
+      pc.kb = start;
+      pc.kend = len;
+      pc.trow = first;
+      pc.by_length = 0;
+      if (shared) {
+        // the prefix is read through the first member that has all of it, or else through a longest one
+        int best = -1, best_len = 0;
+        for (int m0 = 0; m0 < count && best_len < len; m0 += 32) {
+          const int l = m0 + lane < count ? min(p.lengths[first + m0 + lane], len) : 0;
+          const int most = __reduce_max_sync(0xFFFFFFFFu, l);
+          if (most > best_len) {
+            best_len = most;
+            best = m0 + __ffs(__ballot_sync(0xFFFFFFFFu, l == most)) - 1;
+          }
+        }
+        pc.trow = first + max(best, 0);
+        pc.kend = best_len;
+        pc.by_length = 1;
+      }
+      pc.alt = alt;
+      pc.q1 = !shared;
+      pc.nt0 = pc.nt1 = pc.j0 + take;
+      if (!alt && pc.ntok <= tpt) pc.nt1 = 0;
+      pc.lim0 = pc.kend;
+      pc.lim_step = 0;
+      pc.split = 1;
+      pc.orow0 = row0 + static_cast<int64_t>(pc.h) * irows + static_cast<int64_t>(up) * 2 * tpt * p.G +
+                 static_cast<int64_t>(blockIdx.x) * PT_ROWS;
+      pc.orow1 = pc.orow0 + (alt ? count : tpt) * p.G;
+      pc.end = 0;
+      return;
+    }
+    while (true) {
+      unsigned id32 = 0;
+      if (lane == 0) id32 = atomicAdd(p.counter, 1u);
+      const int64_t id = __shfl_sync(0xFFFFFFFFu, id32, 0);
+      int64_t off64;
+      const int src = find(p, id, off64);
+      if (src < 0) return;
+      const int c0 = get(seq.c0, src), n_tok = get(seq.n, src), len = get(seq.len, src), nq = get(seq.nq, src);
+      const int mt = get(seq.mt, src);
+      const int nch = chunk ? (mt + chunk - 1) / chunk : 1;
+      int q, ch = 0;
+      if (nch == 1) {
+        pc.h = static_cast<int>(off64 % p.H);
+        q = nq - 1 - static_cast<int>(off64 / p.H);
+      } else {
+        q = nq - 1 - static_cast<int>(off64 % nq);
+        ch = static_cast<int>(off64 / nq % nch);
+        pc.h = static_cast<int>(off64 / nq / nch);
+      }
+      const int utok = 2 * tpt;
+      pc.tok0 = c0 + q * utok;
+      pc.ntok = min(utok, n_tok - q * utok);
+      const int pos0 = len - n_tok + q * utok;  // position of the first token
+      const int n0 = min(tpt, pc.ntok);
+      const int l0 = p.causal ? pos0 + n0 : len, l1 = pc.ntok > tpt ? (p.causal ? pos0 + pc.ntok : len) : 0;
+      pc.nt0 = (max(l0, 0) + PT_BN - 1) / PT_BN;
+      pc.nt1 = (max(l1, 0) + PT_BN - 1) / PT_BN;
+      pc.j0 = 0;
+      if (nch > 1) {
+        pc.j0 = ch * chunk;
+        if (max(pc.nt0, pc.nt1) <= pc.j0 && ch > 0) continue;  // nothing to see in this chunk
+        pc.nt0 = min(pc.nt0, pc.j0 + chunk);
+        pc.nt1 = min(pc.nt1, pc.j0 + chunk);
+      }
+      pc.kb = 0;
+      pc.kend = len;
+      pc.trow = p.table ? i0 + src : c0;
+      pc.alt = 0;
+      pc.q1 = 0;
+      pc.by_length = 0;
+      pc.lim0 = p.causal ? pos0 + 1 : len;
+      pc.lim_step = p.causal ? 1 : 0;
+      pc.split = nch > 1;
+      pc.orow0 = id * PT_ROWS;
+      pc.orow1 = pc.orow0 + 128;
+      pc.end = 0;
+      return;
+    }
+  }
+};
+
+// One key tile by the calling warp: lanes look pages up a batch of tiles ahead and load their own.
+struct TileLoader {
+  int npt, box;          // pages of a tile, rows of a box
+  int batch, page, ahead;  // the batch whose pages the lanes hold, and the next one's
+  __device__ __forceinline__ void init(const PagedAttn& p) {
+    box = min(1 << p.ps_shift, PT_BN);
+    npt = PT_BN / box;
+    batch = -1;
+  }
+  __device__ __forceinline__ int look(const PagedAttn& p, const Piece& pc, int bt) {
+    const int key = pc.kb + bt * 32 * box + lane_id() * box;
+    if (key >= pc.kend) return 0;
+    const int pg = __ldg(p.table + pc.trow * p.table_stride + (key >> p.ps_shift));
+    if (pg >= 0 && pg < p.num_pages) return pg;
+    paged_error(p.err, ERR_PAGE);
+    return p.num_pages;  // past the map: zeros
+  }
+  __device__ __forceinline__ void load(const PagedAttn& p, const Piece& pc, const CUtensorMap* map, int j, int D,
+                                       uint8_t* dst, uint64_t* bar) {
+    const int lane = lane_id();
+    if (!p.table) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(bar, PT_BN * D * 2);
+        for (int x = 0; x < D / 64; ++x)
+          tma_load_4d(dst + x * (PT_BN * 128), map, bar, x * 64, pc.trow + j * PT_BN, pc.h, 0);
+      }
+      return;
+    }
+    const int per = 32 / npt;  // tiles of a batch
+    const int bt = j / per;
+    if (bt != batch) {
+      page = batch >= 0 && bt == batch + 1 ? ahead : look(p, pc, bt);
+      ahead = look(p, pc, bt + 1);
+      batch = bt;
+    }
+    const int i = lane - (j - bt * per) * npt;  // the lane's page of this tile
+    const int key = pc.kb + j * PT_BN + i * box;
+    const bool mine = i >= 0 && i < npt && key < pc.kend;
+    const int n = __popc(__ballot_sync(0xFFFFFFFFu, mine));
+    if (lane == 0) mbar_arrive_expect_tx(bar, n * box * D * 2);
+    __syncwarp();
+    if (mine) {
+      const int row = key & ((1 << p.ps_shift) - 1);
+      for (int x = 0; x < D / 64; ++x)
+        tma_load_4d(dst + x * (PT_BN * 128) + i * box * 128, map, bar, x * 64, row, pc.h, page);
+    }
+  }
+};
+
+// ------------------------------------------------------------------------------------ the kernel
+template <int D, bool BF16>
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
+  using C = PtCfg<D>;
+  constexpr int NK = C::NK, NV = C::NV;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
+  uint64_t* q_full = bars;
+  uint64_t* q_empty = bars + 1;
+  uint64_t* k_full = bars + 2;          // [NK]
+  uint64_t* k_empty = k_full + NK;      // [NK]
+  uint64_t* v_full = k_empty + NK;      // [NV]
+  uint64_t* v_empty = v_full + NV;      // [NV]
+  uint64_t* w_full = v_empty + NV;      // [PT_RING] a piece is published
+  uint64_t* w_empty = w_full + PT_RING; // [PT_RING] and has been read by all
+  uint64_t* s_full = w_empty + PT_RING; // [2]
+  uint64_t* p_lo = s_full + 2;          // [2] weights of keys 0..63 stored
+  uint64_t* p_full = p_lo + 2;          // [2] all weights stored
+  uint64_t* o_full = p_full + 2;        // [2]
+  uint64_t* tile_free = o_full + 2;     // [2]
+  uint64_t* mma_done = tile_free + 2;
+  uint64_t* turn = mma_done + 1;        // [2]
+  Piece* pieces = reinterpret_cast<Piece*>(smem + C::OFF_PIECE);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
+  int64_t* start = reinterpret_cast<int64_t*>(smem + C::OFF_MISC + 16);  // item, its tiles' and rows' base, chunk
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + C::OFF_EPI);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 2);
+    for (int s = 0; s < NK; ++s) {
+      mbar_init(k_full + s, 1);
+      mbar_init(k_empty + s, 2);
+    }
+    for (int s = 0; s < NV; ++s) {
+      mbar_init(v_full + s, 1);
+      mbar_init(v_empty + s, 2);
+    }
+    for (int s = 0; s < PT_RING; ++s) {
+      mbar_init(w_full + s, 1);
+      mbar_init(w_empty + s, 11);
+    }
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_full + x, 1);
+      mbar_init(p_lo + x, 4);
+      mbar_init(p_full + x, 4);
+      mbar_init(o_full + x, 1);
+      mbar_init(tile_free + x, 4);
+      mbar_init(turn + x, 1);
+    }
+    mbar_init(mma_done, 2);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 3 && lane == 0) {
+    tma_prefetch_desc(&p.tm_q);
+    tma_prefetch_desc(&p.tm_q1);
+    tma_prefetch_desc(&p.tm_k);
+    tma_prefetch_desc(&p.tm_v);
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  // ---------------------------------------------------------------- where this CTA's work begins
+  const int tpt = 128 / p.G;
+  const int groups = p.decode && groups_ok(p) ? p.groups : 0;
+  int64_t pos = 0, pos_end = 0;
+  if (p.decode || p.may_split) {
+    const int n = p.decode ? groups + p.B : p.B;
+    const int per = (n + PT_THREADS - 1) / PT_THREADS;
+    const int a = min(n, static_cast<int>(threadIdx.x) * per), z = min(n, a + per);
+    int64_t t = 0, r = 0, tt, tr;
+    for (int i = a; i < z; ++i) {
+      if (p.decode) {
+        const Item it = decode_item(p, groups, tpt, i);
+        t += static_cast<int64_t>(p.H) * it.units * it.tiles;
+        r += static_cast<int64_t>(p.H) * it.rows;
+      } else {
+        const Seq s = prompt_seq(p, 2 * tpt, i);
+        t += static_cast<int64_t>(p.H) * s.nq * s.mt;
+        r += static_cast<int64_t>(p.H) * s.nq;
+      }
+    }
+    block_scan2(t, r, scan, tt, tr);
+    if (p.decode) {
+      const int64_t ctas = min(tt, static_cast<int64_t>(p.num_ctas));  // a tile at least for each
+      if (blockIdx.x < ctas) {
+        pos = tt * blockIdx.x / ctas;
+        pos_end = tt * (blockIdx.x + 1) / ctas;
+      }
+      if (threadIdx.x == 0 && blockIdx.x == 0) p.rec_tile[n] = tt;
+      for (int i = a; i < z; ++i) {
+        const Item it = decode_item(p, groups, tpt, i);
+        const int64_t c = static_cast<int64_t>(p.H) * it.units * it.tiles;
+        if (t <= pos && pos < t + c) {
+          start[0] = i;
+          start[1] = t;
+          start[2] = r;
+        }
+        if (blockIdx.x == 0) {
+          p.rec_tile[i] = t;
+          p.rec_row[i] = r;
+        }
+        t += c;
+        r += static_cast<int64_t>(p.H) * it.rows;
+      }
+    } else {
+      const int chunk = chunk_tiles(p, tr, tt);
+      if (threadIdx.x == 0) start[3] = chunk;
+      if (blockIdx.x == 0 && chunk) {
+        // the sequences' first pieces, for the joining kernel
+        int64_t c = 0, zero = 0, tc, tz;
+        for (int i = a; i < z; ++i) c += prompt_pieces(p, prompt_seq(p, 2 * tpt, i), chunk);
+        block_scan2(c, zero, scan, tc, tz);
+        for (int i = a; i < z; ++i) {
+          p.rec_tile[i] = c;
+          c += prompt_pieces(p, prompt_seq(p, 2 * tpt, i), chunk);
+        }
+      }
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_tile[n] = chunk;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint32_t tmem = *tmem_slot;
+  const Abort ab{abort_flag, p.err};
+
+  // the next published piece, for all warps but warp 0
+  int wpos = 0;
+  auto take = [&](Piece& pc, int code) -> bool {
+    const int s = wpos % PT_RING;
+    if (!pt_wait(w_full + s, (wpos / PT_RING) & 1, ab, code)) return false;
+    pc = pieces[s];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(w_empty + s);
+    ++wpos;
+    return !pc.end;
+  };
+
+  if (warp == 0) {
+    // ================================================================ pieces, Q and K
+    Sched sc;
+    sc.groups = groups;
+    sc.tpt = tpt;
+    sc.pos = pos;
+    sc.end = pos_end;
+    sc.n = p.decode ? groups + p.B : p.B;
+    sc.chunk = 0;
+    sc.i0 = 0;
+    sc.base_t = sc.base_r = 0;
+    if (p.decode && pos < pos_end) {
+      sc.i0 = static_cast<int>(start[0]);
+      sc.base_t = start[1];
+      sc.base_r = start[2];
+    }
+    if (!p.decode && p.may_split) sc.chunk = static_cast<int>(start[3]);
+    sc.load(p);
+    int published = 0;
+    auto publish = [&](const Piece& pc) -> bool {
+      const int s = published % PT_RING;
+      if (!pt_wait(w_empty + s, ((published / PT_RING) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER)) return false;
+      if (lane == 0) {
+        pieces[s] = pc;
+        mbar_arrive(w_full + s);
+      }
+      __syncwarp();
+      ++published;
+      return true;
+    };
+    TileLoader ld;
+    ld.init(p);
+    Piece nx;
+    uint32_t q_par = 1;
+    int kpos = 0, q_issued = 0;
+    sc.next(p, nx);
+    bool ok = publish(nx);
+    while (ok && !nx.end) {
+      const Piece pc = nx;
+      if (!pt_wait(q_empty, q_par, ab, ERR_TIMEOUT_PRODUCER)) break;
+      q_par ^= 1;
+      if (lane == 0) {
+        const bool two = pc.alt || pc.ntok > tpt;
+        const uint32_t box = (pc.q1 ? 1 : tpt) * p.G * 128;
+        mbar_arrive_expect_tx(q_full, box * (D / 64) * (two ? 2 : 1));
+        for (int x = 0; x < (two ? 2 : 1); ++x)
+          for (int d = 0; d < D / 64; ++d)
+            tma_load_4d(smem + C::OFF_Q + x * C::QBYTES + d * (128 * 128), pc.q1 ? &p.tm_q1 : &p.tm_q, q_full, d * 64,
+                        pc.h * p.G, pc.tok0 + (pc.alt ? 0 : x * tpt), 0);
+      }
+      __syncwarp();
+      ++q_issued;
+      bool ahead = false;
+      ld.batch = -1;
+      const int je = pc.jend();
+      for (int j = pc.j0; ok && j < je; ++j) {
+        const int slot = kpos % NK;
+        ok = pt_wait(k_empty + slot, ((kpos / NK) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
+        if (!ok) break;
+        ld.load(p, pc, &p.tm_k, j, D, smem + C::OFF_K + slot * C::KVBYTES, k_full + slot);
+        ++kpos;
+        // the next piece while this one's first tiles are on their way
+        if (!ahead && j - pc.j0 == NK - 1) {
+          sc.next(p, nx);
+          ok = publish(nx);
+          ahead = true;
+        }
+      }
+      if (ok && !ahead) {
+        sc.next(p, nx);
+        ok = publish(nx);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) {
+      // copies in flight must land before the CTA exits
+      bool drained = true;
+      for (int f = (kpos > NK ? kpos - NK : 0); f < kpos && drained; ++f)
+        drained = mbar_drain(k_full + f % NK, (f / NK) & 1, p.err);
+      if (drained && q_issued > 0) mbar_drain(q_full, (q_issued - 1) & 1, p.err);
+      // the last CTA leaves the counter as it found it
+      if (!p.decode && atomicAdd(p.counter + 1, 1u) == gridDim.x - 1) {
+        p.counter[0] = 0;
+        p.counter[1] = 0;
+      }
+    }
+  } else if (warp == 3) {
+    // ================================================================ V
+    TileLoader ld;
+    ld.init(p);
+    Piece pc;
+    int vpos = 0;
+    bool ok = true;
+    while (ok && take(pc, ERR_TIMEOUT_PRODUCER)) {
+      ld.batch = -1;
+      const int je = pc.jend();
+      for (int j = pc.j0; j < je; ++j) {
+        const int slot = vpos % NV;
+        ok = pt_wait(v_empty + slot, ((vpos / NV) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
+        if (!ok) break;
+        ld.load(p, pc, &p.tm_v, j, D, smem + C::OFF_V + slot * C::KVBYTES, v_full + slot);
+        ++vpos;
+      }
+    }
+    __syncwarp();
+    if (lane == 0) {
+      bool drained = true;
+      for (int f = (vpos > NV ? vpos - NV : 0); f < vpos && drained; ++f)
+        drained = mbar_drain(v_full + f % NV, (f / NV) & 1, p.err);
+    }
+  } else if (warp == 1 || warp == 2) {
+    // ================================================================ products of tile x
+    // The warp runs converged and one elected lane issues. Tiles of a pair walk the same key tiles; both
+    // warps wait for every fill, in order, and release it, so a slot's two arrivals are of one fill and no wait
+    // can take an earlier phase for its own. They issue their batches (a tile's P V and the next one's
+    // Q K^T) in turn, tile 0 first, which keeps the two softmax passes half a period apart. Tiles that share the
+    // rows (`alt`) take every other fill and pass the rest on; they need no turns.
+    const int x = warp - 1;
+    constexpr uint32_t IDESC_S = umma_idesc_f16(128, PT_BN, BF16, false);
+    constexpr uint32_t IDESC_PV = umma_idesc_f16(128, D, BF16, true);
+    const uint32_t tS = tmem + 128 * x;
+    const uint32_t tO = tmem + 256 + D * x;
+    const uint64_t qdesc = umma_desc_sw128(smem_u32(smem + C::OFF_Q + x * C::QBYTES), 16, 1024);
+    const uint64_t kdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
+    const uint64_t vdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_V), PT_BN * 128, 1024);
+    int kpos = 0, vpos = 0;
+    uint32_t q_par = 0, free_par = 1, p_par = 0, nbatch = 0;
+    Piece pc;
+    bool ok = true;
+    auto my_turn = [&]() -> bool {
+      if (x == 1) return pt_wait(turn + 0, nbatch & 1, ab, ERR_TIMEOUT_MMA);
+      return nbatch == 0 || pt_wait(turn + 1, (nbatch - 1) & 1, ab, ERR_TIMEOUT_MMA);
+    };
+    auto end_turn = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(turn + x);
+      ++nbatch;
+    };
+    while (ok && take(pc, ERR_TIMEOUT_MMA)) {
+      ok = pt_wait(q_full, q_par, ab, ERR_TIMEOUT_MMA);
+      if (!ok) break;
+      q_par ^= 1;
+      tc_fence_after();
+      const int je = pc.jend();
+      const bool mine = x == 0 || pc.alt || pc.ntok > tpt;
+      bool freed = false, o_init = false;
+      auto ensure_free = [&]() -> bool {
+        if (freed) return true;
+        if (!pt_wait(tile_free + x, free_par, ab, ERR_TIMEOUT_MMA)) return false;
+        free_par ^= 1;
+        tc_fence_after();
+        freed = true;
+        return true;
+      };
+      auto issue_S = [&](int f) {
+        const uint64_t kb = kdesc0 + static_cast<uint64_t>((f % NK) * (C::KVBYTES >> 4));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+          umma_ss(tS, qdesc + off, kb + off, IDESC_S, kk > 0);
+        }
+        umma_commit(s_full + x);
+      };
+      auto issue_PV = [&](int f, int half) {
+        const uint64_t vb = vdesc0 + static_cast<uint64_t>((f % NV) * (C::KVBYTES >> 4));
+#pragma unroll
+        for (int k4 = 0; k4 < PT_BN / 32; ++k4) {
+          const int kk = half * (PT_BN / 32) + k4;
+          umma_ts(tO, tS + kk * 8, vb + static_cast<uint64_t>((kk * 2048) >> 4), IDESC_PV, (o_init || kk > 0) ? 1u : 0u);
+        }
+        o_init = true;
+      };
+      auto weigh = [&](int f) -> bool {  // P V of the tile whose V is fill f
+        if (!pt_wait(p_lo + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        if (!ensure_free()) return false;
+        issue_PV(f, 0);
+        if (!pt_wait(p_full + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
+        p_par ^= 1;
+        tc_fence_after();
+        issue_PV(f, 1);
+        return true;
+      };
+      auto wait_k = [&](int f) -> bool {
+        if (!pt_wait(k_full + f % NK, (f / NK) & 1, ab, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        return true;
+      };
+      auto wait_v = [&](int f) -> bool {
+        if (!pt_wait(v_full + f % NV, (f / NV) & 1, ab, ERR_TIMEOUT_MMA)) return false;
+        tc_fence_after();
+        return true;
+      };
+      if (pc.alt) {
+        const int n = je - pc.j0;
+        int ki = 0, vi = 0;
+        auto pass_k = [&]() -> bool {  // the other tile's fill
+          if (!wait_k(kpos + ki)) return false;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(k_empty + (kpos + ki) % NK);
+          ++ki;
+          return true;
+        };
+        auto pass_v = [&]() -> bool {
+          if (!wait_v(vpos + vi)) return false;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_empty + (vpos + vi) % NV);
+          ++vi;
+          return true;
+        };
+        auto next_S = [&]() -> bool {
+          if ((ki & 1) != x && !pass_k()) return false;
+          if (!wait_k(kpos + ki)) return false;
+          issue_S(kpos + ki);
+          umma_commit(k_empty + (kpos + ki) % NK);
+          ++ki;
+          return true;
+        };
+        if (x < n) ok = next_S();
+        else umma_commit(q_empty);
+        for (int i = x; ok && i < n; i += 2) {
+          if (i + 2 >= n) umma_commit(q_empty);  // every score of this piece is issued
+          if (vi < i) ok = pass_v();
+          ok = ok && wait_v(vpos + i) && weigh(vpos + i);
+          if (!ok) break;
+          umma_commit(v_empty + (vpos + i) % NV);
+          ++vi;
+          if (i + 2 < n) ok = next_S();
+        }
+        if (ok && ki < n) ok = pass_k();
+        if (ok && vi < n) ok = pass_v();
+        if (!ok) break;
+        kpos += n;
+        vpos += n;
+      } else {
+        auto uses = [&](int j) { return mine && j < (x ? pc.nt1 : pc.nt0); };
+        if (pc.j0 < je) {
+          ok = wait_k(kpos) && my_turn();
+          if (!ok) break;
+          if (uses(pc.j0)) issue_S(kpos);
+          end_turn();
+          umma_commit(k_empty + kpos % NK);
+          ++kpos;
+        }
+        for (int j = pc.j0; j < je; ++j) {
+          const bool more = j + 1 < je;
+          ok = wait_v(vpos);
+          if (!ok) break;
+          if (!more) umma_commit(q_empty);  // every score of this piece is issued
+          ok = my_turn();
+          if (!ok) break;
+          if (uses(j)) {
+            ok = weigh(vpos);
+            if (!ok) break;
+          }
+          if (more) {
+            ok = wait_k(kpos);
+            if (!ok) break;
+            if (uses(j + 1)) issue_S(kpos);
+          }
+          end_turn();
+          umma_commit(v_empty + vpos % NV);
+          ++vpos;
+          if (more) {
+            umma_commit(k_empty + kpos % NK);
+            ++kpos;
+          }
+        }
+        if (!ok) break;
+        if (pc.j0 >= je) umma_commit(q_empty);
+      }
+      // The products' warp waits for the tile once a piece and always announces O; the epilogue always
+      // waits for that before it gives the tile back, so the parities cannot run apart.
+      if (mine) {
+        ok = ensure_free();
+        if (!ok) break;
+        umma_commit(o_full + x);
+      }
+    }
+    umma_commit(mma_done);
+    if (lane == 0) mbar_drain(mma_done, 0, p.err);
+    __syncwarp();
+  } else {
+    // ================================================================ softmax and epilogue of tile x
+    const int x = (warp - 4) >> 2;
+    const int wq = warp & 3;
+    const int r = wq * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>(wq * 32) << 16;
+    const uint32_t tS = tmem + lane_base + 128 * x;
+    const uint32_t tO = tmem + lane_base + 256 + D * x;
+    const float sl2 = p.scale_log2;
+    int vpos = 0;
+    uint32_t s_par = 0, o_par = 0;
+    Piece pc;
+    bool ok = true;
+    while (ok && take(pc, ERR_TIMEOUT_SOFTMAX)) {
+      const int je = pc.jend(), step = pc.alt ? 2 : 1;
+      const bool valid = x == 0 || pc.alt || pc.ntok > tpt;
+      const int ntok = pc.alt ? pc.ntok : max(0, min(tpt, pc.ntok - x * tpt));
+      const int nrows = ntok * p.G;
+      const bool warp_live = wq * 32 < nrows;
+      const bool live = r < nrows;
+      const int ti = r / p.G;                               // token of this row within the tile
+      const int tok = pc.tok0 + (pc.alt ? 0 : x * tpt) + ti;
+      int lim_row = 0;  // keys from kb on that this row sees
+      if (live) {
+        lim_row = pc.lim0 + (tok - pc.tok0) * pc.lim_step;
+        if (pc.by_length) lim_row = min(lim_row, p.lengths[tok]);
+        lim_row -= pc.kb;
+      }
+      // rows that do not exist get a reference no score exceeds, and weigh nothing
+      float m_used = live ? -INFINITY : 1e30f, l = 0.f;
+      bool o_has = false;
+      const int my_end = pc.alt ? je : (x ? pc.nt1 : pc.nt0);
+      for (int j = pc.j0 + (pc.alt ? x : 0); valid && j < my_end; j += step) {
+        const int f = vpos + (j - pc.j0);
+        const int n0 = j * PT_BN;
+        const int have = pc.kend - pc.kb - n0;  // rows of this tile that exist
+        const bool tail = have < PT_BN;
+        const int lim = live ? lim_row - n0 : PT_BN;
+        const bool masked = __any_sync(0xFFFFFFFFu, lim < PT_BN);
+        if (!pt_wait(s_full + x, s_par, ab, ERR_TIMEOUT_SOFTMAX)) { ok = false; break; }
+        s_par ^= 1;
+        if (tail) {
+          // V rows past the sequence hold anything: 0 in their place, before the products read them. (With this
+          // tile's scores there, every fill before the previous one has landed, so the wait is for this one.)
+          if (!pt_wait(v_full + f % NV, (f / NV) & 1, ab, ERR_TIMEOUT_SOFTMAX)) { ok = false; break; }
+          if (r >= have) {
+            uint8_t* row = smem + C::OFF_V + (f % NV) * C::KVBYTES + r * 128;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<uint4*>(row + c * (PT_BN * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+        }
+        tc_fence_after();
+        if (!warp_live) {  // no row of this warp exists: its weights go nowhere
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(p_lo + x);
+            mbar_arrive(p_full + x);
+          }
+          o_has = true;
+          continue;
+        }
+        if (masked) {
+          // scores past the row's limit become -inf in TMEM
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            if (!__any_sync(0xFFFFFFFFu, lim < c * 32 + 32)) continue;
+            uint32_t sc[32];
+            tmem_ld32(tS + c * 32, sc);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[e] = (c * 32 + e < lim) ? sc[e] : 0xFF800000u;
+            tmem_st32(tS + c * 32, sc);
+          }
+          tmem_st_wait();
+        }
+        auto chunk_max = [&](const uint32_t* sc) {  // the scale is positive
+          float m0 = __uint_as_float(sc[0]), m1 = __uint_as_float(sc[1]);
+#pragma unroll
+          for (int e = 2; e < 32; e += 4) {
+            m0 = fmax3(m0, __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
+            if (e + 2 < 32) m1 = fmax3(m1, __uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3]));
+          }
+          return fmaxf(m0, m1) * sl2;
+        };
+        float2 la = make_float2(0.f, 0.f), lb = la;
+        auto weights = [&](const uint32_t* sc, float nb, uint32_t* out) {
+          const float2 s2 = make_float2(sl2, sl2), n2 = make_float2(nb, nb);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float2 a01 = ffma2(make_float2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), s2, n2);
+            const float2 a23 = ffma2(make_float2(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), s2, n2);
+            float w[4];
+            w[0] = ex2(a01.x); w[1] = ex2(a01.y); w[2] = ex2(a23.x); w[3] = ex2(a23.y);
+            la = fadd2(la, make_float2(w[0], w[1]));
+            lb = fadd2(lb, make_float2(w[2], w[3]));
+            out[e / 2] = pack2(w[0], w[1], BF16);
+            out[e / 2 + 1] = pack2(w[2], w[3], BF16);
+          }
+        };
+        int stop = 0;          // first 32-column chunk that the stream did not finish
+        bool lo_sent = false;  // weights of keys 0..63 are final and announced
+        {
+          uint32_t sa[32], sb[32];
+          tmem_ld32_async(tS, sa);
+          tmem_ld32_wait(sa);
+          tmem_ld32_async(tS + 32, sb);
+          if (m_used == -INFINITY) {
+            const float m0 = chunk_max(sa);
+            m_used = m0 == -INFINITY ? 0.f : m0;
+          }
+          const float nb = -m_used, most = m_used + 8.f;
+          auto one = [&](int c, uint32_t(&cur)[32], uint32_t(&nxt)[32]) -> bool {
+            if (__any_sync(0xFFFFFFFFu, chunk_max(cur) > most)) {
+              tmem_ld32_wait(nxt);
+              stop = c;
+              return false;
+            }
+            uint32_t w[16];
+            weights(cur, nb, w);
+            tmem_st16(tS + c * 16, w);
+            tmem_ld32_wait(nxt);
+            tmem_ld32_async(tS + (c + 2) * 32, cur);
+            return true;
+          };
+          if (one(0, sa, sb) && one(1, sb, sa)) {
+            tmem_ld32_wait(sb);
+            if (__any_sync(0xFFFFFFFFu, fmaxf(chunk_max(sa), chunk_max(sb)) > most)) {
+              stop = 2;
+            } else {
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_lo + x);
+              lo_sent = true;
+              uint32_t w[16];
+              weights(sa, nb, w);
+              tmem_st16(tS + 32, w);
+              weights(sb, nb, w);
+              tmem_st16(tS + 48, w);
+              stop = 4;
+            }
+          }
+        }
+        if (stop < 4) {
+          // some row outgrew its reference: the maximum of what is left, everything so far rescaled, by whole
+          // octaves where weights of this tile are stored already, then the rest
+          tmem_st_wait();
+          float mt = -INFINITY;
+#pragma unroll 1
+          for (int c = stop; c < 4; ++c) {
+            uint32_t sc[32];
+            tmem_ld32(tS + c * 32, sc);
+            mt = fmaxf(mt, chunk_max(sc));
+          }
+          const bool need = mt > m_used + 8.f;
+          if (__any_sync(0xFFFFFFFFu, need)) {
+            float m_new = m_used, fac = 1.f;
+            if (need) {
+              if (stop > 0) {
+                const float k = ceilf(mt - m_used);
+                m_new = m_used + k;
+                fac = k < 127.f ? __int_as_float((127 - static_cast<int>(k)) << 23) : 0.f;
+              } else {
+                m_new = mt;
+                fac = ex2(m_used - m_new);
+              }
+            }
+            l *= fac;
+            la.x *= fac; la.y *= fac; lb.x *= fac; lb.y *= fac;
+            if (o_has) {
+#pragma unroll 1
+              for (int c = 0; c < D / 16; ++c) {
+                uint32_t o[16];
+                tmem_ld16(tO + c * 16, o);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fac);
+                tmem_st16(tO + c * 16, o);
+              }
+            }
+#pragma unroll 1
+            for (int c = 0; c < stop; ++c) {
+              uint32_t w[16];
+              tmem_ld16(tS + c * 16, w);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float2 v;
+                if (BF16) v = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
+                else v = __half22float2(*reinterpret_cast<__half2*>(&w[e]));
+                w[e] = pack2(v.x * fac, v.y * fac, BF16);
+              }
+              tmem_st16(tS + c * 16, w);
+            }
+            m_used = m_new;
+          }
+#pragma unroll 1
+          for (int c = stop; c < 4; ++c) {
+            uint32_t sc[32], w[16];
+            tmem_ld32(tS + c * 32, sc);
+            weights(sc, -m_used, w);
+            tmem_st16(tS + c * 16, w);
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (!lo_sent) mbar_arrive(p_lo + x);
+          mbar_arrive(p_full + x);
+        }
+        l += (la.x + la.y) + (lb.x + lb.y);
+        o_has = true;
+      }
+      if (!ok) break;
+      vpos += max(0, je - pc.j0);
+      if (!valid) continue;
+      // ---------------- epilogue
+      if (!pt_wait(o_full + x, o_par, ab, ERR_TIMEOUT_EPILOGUE)) break;
+      o_par ^= 1;
+      tc_fence_after();
+      if (warp_live) {
+        uint8_t* stg = smem + C::OFF_EPI + (warp - 4) * 32 * C::EPI_PITCH;
+        const int rr = lane >> 2, seg = lane & 3;  // the row and 16-byte piece this lane stores
+        const int left = nrows - wq * 32;          // rows of this warp
+        if (pc.split) {
+          const int64_t row0 = (x ? pc.orow1 : pc.orow0) + wq * 32;
+          if (live) p.part_s[row0 + lane] = make_float2(m_used, o_has ? l : 0.f);
+          if (o_has) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(tO + c * 16, o);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(stg + lane * C::EPI_PITCH + e * 16) =
+                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              __syncwarp();
+#pragma unroll
+              for (int q4 = 0; q4 < 4; ++q4) {
+                const int lr = q4 * 8 + rr;
+                if (lr < left)
+                  *reinterpret_cast<uint4*>(p.part_o + (row0 + lr) * D + c * 16 + seg * 4) =
+                      *reinterpret_cast<const uint4*>(stg + lr * C::EPI_PITCH + seg * 16);
+              }
+              __syncwarp();
+            }
+          }
+        } else {
+          using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+          const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing gives 0
+          const int64_t mine = live ? tok * p.o_t + (pc.h * p.G + r - ti * p.G) * p.o_h : 0;
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            if (o_has) {
+              tmem_ld32(tO + c * 32, o);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = 0u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, BF16);
+              w.y = pack2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv, BF16);
+              w.z = pack2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv, BF16);
+              w.w = pack2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv, BF16);
+              *reinterpret_cast<uint4*>(stg + lane * C::EPI_PITCH + e * 2) = w;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {
+              const int lr = q4 * 8 + rr;
+              const int64_t off = shfl64(mine, lr);
+              if (lr < left)
+                *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + off + c * 32 + seg * 8) =
+                    *reinterpret_cast<const uint4*>(stg + lr * C::EPI_PITCH + seg * 16);
+            }
+            __syncwarp();
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(tile_free + x);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------ joining
+// One warp per output row: the maxima and sums of all of its pieces, then their weighted sum. D / 32 elements
+// a lane. Pieces that hold nothing for the row (sum 0) are left out.
+template <int D, typename T> struct Joiner {
+  float acc[D / 32], m, l;
+  __device__ __forceinline__ Joiner() : m(-INFINITY), l(0.f) {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  }
+  // pieces i in [0, n) at partial row `row(i)`
+  template <typename F> __device__ __forceinline__ void add(const PagedAttn& p, int n, F row) {
+    const int lane = lane_id();
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float2 s = make_float2(-INFINITY, 0.f);
+      if (i0 + lane < n) s = __ldcg(p.part_s + row(i0 + lane));
+      const bool has = s.y != 0.f;  // NaN too
+      float mx = has ? s.x : -INFINITY;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+      const unsigned any = __ballot_sync(0xFFFFFFFFu, has);
+      if (!any) continue;
+      const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : ex2(m - mn);
+      m = mn;
+      const float w = has ? ex2(s.x - mn) : 0.f;
+      float sum = has ? w * s.y : 0.f;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+      l = l * f + sum;
+#pragma unroll
+      for (int e = 0; e < D / 32; ++e) acc[e] *= f;
+      const int most = min(32, n - i0);
+#pragma unroll 4
+      for (int i = 0; i < most; ++i) {
+        const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
+        if (!(any >> i & 1)) continue;
+        const float* src = p.part_o + row(i0 + i) * D + lane * (D / 32);
+        if constexpr (D == 128) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          acc[0] += wi * v.x; acc[1] += wi * v.y;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* dst) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) o[i] = from_f32<T>(acc[i] * inv);
+    if constexpr (D == 128) *reinterpret_cast<uint2*>(dst + lane_id() * 4) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint32_t*>(dst + lane_id() * 2) = *reinterpret_cast<const uint32_t*>(o);
+  }
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttn p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tpt = 128 / p.G, Hq = p.H * p.G;
+  const int groups = p.decode && groups_ok(p) ? p.groups : 0;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= static_cast<int64_t>(p.T) * Hq) return;
+  const int t = static_cast<int>(row / Hq), hq = static_cast<int>(row % Hq), h = hq / p.G, rg = hq % p.G;
+  T* dst = static_cast<T*>(p.out) + t * p.o_t + hq * p.o_h;
+  Joiner<D, T> jn;
+  if (p.decode) {
+    const int b = t;
+    const int64_t total = p.rec_tile[groups + p.B];
+    const int64_t ctas = min(total, static_cast<int64_t>(p.num_ctas));
+    auto unit = [&](int i, const Item& it, int up, int in_unit) {
+      if (!it.tiles) return;
+      const int64_t u0 = p.rec_tile[i] + (static_cast<int64_t>(h) * it.units + up) * it.tiles;
+      const int c0 = static_cast<int>(((u0 + 1) * ctas - 1) / total);
+      const int c1 = static_cast<int>(((u0 + it.tiles) * ctas - 1) / total);
+      const int64_t base = p.rec_row[i] + static_cast<int64_t>(h) * it.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
+                           static_cast<int64_t>(c0) * PT_ROWS + in_unit;
+      const int n = c1 - c0 + 1, second = it.count * p.G;
+      jn.add(p, it.alt ? 2 * n : n, [&](int k) {
+        return it.alt ? base + static_cast<int64_t>(k >> 1) * PT_ROWS + (k & 1) * second
+                      : base + static_cast<int64_t>(k) * PT_ROWS;
+      });
+    };
+    const int g = group_of(p, groups, b);
+    if (g >= 0) {
+      const Item it = decode_item(p, groups, tpt, g);
+      const int mi = b - it.first, up = mi / (2 * tpt);
+      unit(g, it, up, (mi - up * 2 * tpt) * p.G + rg);
+    }
+    unit(groups + b, decode_item(p, groups, tpt, groups + b), 0, rg);
+    jn.store(dst);
+    return;
+  }
+  const int chunk = static_cast<int>(p.rec_tile[p.B]);
+  if (!chunk) return;
+  const int b = paged_sequence(p.cu, p.B, t);
+  if (b < 0) return;
+  const Seq s = prompt_seq(p, 2 * tpt, b);
+  const int nch = (s.mt + chunk - 1) / chunk;
+  if (nch == 1 || t < s.c0 || t >= s.c0 + s.n) return;
+  const int q = (t - s.c0) / (2 * tpt), in = t - s.c0 - q * 2 * tpt, x = in / tpt;
+  const int last = min(2 * tpt, s.n - q * 2 * tpt);  // tokens of the unit
+  const int lim = p.causal ? max(0, s.len - s.n + q * 2 * tpt + last) : s.len;
+  const int n = max(1, ((lim + PT_BN - 1) / PT_BN + chunk - 1) / chunk);
+  const int64_t id0 = p.rec_tile[b] + static_cast<int64_t>(h) * nch * s.nq + (s.nq - 1 - q);
+  const int64_t base = id0 * PT_ROWS + x * 128 + (in - x * tpt) * p.G + rg;
+  const int64_t stride = static_cast<int64_t>(s.nq) * PT_ROWS;
+  jn.add(p, n, [&](int k) { return base + k * stride; });
+  jn.store(dst);
+}
+
+// ------------------------------------------------------------------------------------ launch
+namespace {
+struct Sizes {
+  int64_t rows, recs;  // partial rows, records of items
+  bool split;
+};
+Sizes sizes_of(int64_t T, int64_t B, int64_t H, int64_t G, int64_t groups, bool decode, int sms) {
+  Sizes s;
+  const int64_t utok = 2 * (128 / G);
+  if (decode) {
+    s.split = true;
+    s.rows = 4 * B * H * G + PT_ROWS * static_cast<int64_t>(sms);
+    s.recs = groups + B + 1;
+  } else {
+    // whole units where the tokens alone make two for every SM
+    s.split = H * (T / utok) < 2 * static_cast<int64_t>(sms);
+    const int64_t units = H * ((T + utok - 1) / utok + B);
+    const int64_t pieces = PT_FILL * static_cast<int64_t>(sms) + (units < 2 * sms ? units : 2 * sms);
+    s.rows = s.split ? pieces * PT_ROWS : 0;
+    s.recs = s.split ? B + 1 : 0;
+  }
+  return s;
+}
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+}  // namespace
+
+size_t paged_attn_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t groups, bool decode, int sms) {
+  const Sizes s = sizes_of(T, B, H, G, groups, decode, sms);
+  return 256 + 2 * up256(s.recs * 8) + up256(s.rows * 8) + up256(s.rows * D * 4);
+}
+
+template <int D, bool BF16>
+static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream_t st) {
+  using C = PtCfg<D>;
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const Sizes s = sizes_of(p.T, p.B, p.H, p.G, p.groups, p.decode, sms);
+  p.counter = reinterpret_cast<unsigned*>(ws);
+  ws += 256;
+  p.rec_tile = reinterpret_cast<int64_t*>(ws);
+  ws += up256(s.recs * 8);
+  p.rec_row = reinterpret_cast<int64_t*>(ws);
+  ws += up256(s.recs * 8);
+  p.part_s = reinterpret_cast<float2*>(ws);
+  ws += up256(s.rows * 8);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.may_split = s.split;
+  p.num_ctas = sms;
+  auto kfn = paged_attn_kernel<D, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  if (e != cudaSuccess) return e;
+  kfn<<<sms, PT_THREADS, C::SMEM, st>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess || !s.split) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.T) * p.H * p.G + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, T>, p);
+}
+
+cudaError_t launch_paged_attn(int dtype, int head_dim, PagedAttn& p, uint8_t* ws, int sms, cudaStream_t st) {
+  if (head_dim == 128)
+    return dtype == BF16 ? launch_paged_t<128, true>(p, ws, sms, st) : launch_paged_t<128, false>(p, ws, sms, st);
+  return dtype == BF16 ? launch_paged_t<64, true>(p, ws, sms, st) : launch_paged_t<64, false>(p, ws, sms, st);
 }
 
 }  // namespace dab

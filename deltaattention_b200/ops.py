@@ -1057,7 +1057,7 @@ def _packed(what, name, t, dtype, tokens=None, heads=None, head_dim=None):
 
 def _not_expanded(what, name, t):
     if any(x == 0 for x, n in zip(t.stride(), t.shape) if n > 1):
-        raise ValueError(f"{what}: {name} is written and must not be expanded")
+        raise ValueError(f"{what}: {name} must not be expanded")
 
 
 def paged_append(k, v, pool: PagedKV, page_table, lengths, *, cu_seqlens=None, cos=None, sin=None, q=None, q_out=None,
@@ -1144,6 +1144,7 @@ def _paged_call(what, dev, q, out, workspace, B, H, D, dtype, groups=0):
     """Checks queries, output and workspace of an attention call; returns (out, Hq / Hkv, their strides,
     workspace, stream), out alone where there is nothing to do."""
     T, Hq, _, q_t, q_h = _packed(what, "q", q, dtype, None, None, D)
+    _not_expanded(what, "q", q)
     if Hq % H:
         raise ValueError(f"{what}: query heads must be a multiple of {H}")
     if out is None:
@@ -1166,7 +1167,7 @@ def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, w
     padding.
 
     q [T, Hq, d], k / v [T, Hkv, d] (bf16 / fp16, d 64 or 128, any token and head strides; q-head h reads kv-head
-    h // (Hq / Hkv), at most 128 q-heads per kv-head), cu_seqlens int32 [B + 1] on the device, rising from 0: it
+    h // (Hq / Hkv), at most 128 q-heads per kv-head; sm_scale is positive), cu_seqlens int32 [B + 1] on the device, rising from 0: it
     is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] from cu_seqlens[B] on are left
     alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and may reach rows before it
     within the same 128 keys.
@@ -1182,6 +1183,8 @@ def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, w
     if D not in (64, 128) or H < 1:
         raise ValueError(f"{what}: need head_dim 64 or 128 and at least one kv-head")
     _, _, _, v_t, v_h = _packed(what, "v", v, q.dtype, T, H, D)
+    for name, t in (("k", k), ("v", v)):
+        _not_expanded(what, name, t)
     B = cu_seqlens.numel() - 1
     _ints(what, "cu_seqlens", cu_seqlens, max(B, 0) + 1)
     out, call = _paged_call(what, dev, q, out, workspace, B, H, D, q.dtype)

@@ -258,8 +258,9 @@ def test_prompts_scale(ops):
     q, k, v = prompt_inputs(n, Hq, H, D, "fp16", False, 0)
     out = ops.flash_varlen(q, k, v, starts(n), sm_scale=0.3)
     check(out, attend64(q, k, v, torch.arange(1, 51), 0.3), v)
-    out = ops.flash_varlen(q, k, v, starts(n), sm_scale=-0.2)
-    check(out, attend64(q, k, v, torch.arange(1, 51), -0.2), v)
+    for scale in (0.0, -0.2, math.nan, math.inf):
+        with pytest.raises(RuntimeError, match="sm_scale"):
+            ops.flash_varlen(q, k, v, starts(n), sm_scale=scale)
 
 
 # ------------------------------------------------------------------------ prompts over the pages
