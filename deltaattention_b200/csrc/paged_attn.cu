@@ -23,6 +23,7 @@
 // the tiles' softmax, a row per thread. The loads are TMA boxes of a page (or of 128 packed rows), scores
 // and weights live in TMEM, weights in the rows' 16-bit type: an error of half a step per weight, as large as
 // that of the rounded output. The running maximum moves only when a row outgrows it by 2^8.
+#include <atomic>
 #include <type_traits>
 
 #include "paged.cuh"
@@ -44,13 +45,15 @@ struct Piece {
   int kb;          // first key of key tile 0
   int kend;        // keys that exist: rows from here on are not read
   int j0, nt0, nt1;  // key tiles: from j0 up to nt0 for tile 0, nt1 for tile 1
-  int alt;         // both tiles hold the same rows, tile x takes key tiles j0 + x, j0 + x + 2, ..
+  int alt;         // both tiles hold the same rows and take every other key tile (by the parity of its fill)
   int lim0, lim_step;  // keys that token tok0 + i sees: lim0 + i * lim_step ..
   int by_length;   // .. and no more than the token's sequence has
   int split;       // partial results to rows orow0 / orow1, else the output
   int q1;          // one token: the query box of one token
   int64_t orow0, orow1;
   __device__ __forceinline__ int jend() const { return max(nt0, nt1); }
+  // query tiles it needs: tiles that hold the same rows share one
+  __device__ __forceinline__ int q_tiles(int tpt) const { return !alt && ntok > tpt ? 2 : 1; }
 };
 
 template <int D> struct PtCfg {
@@ -65,13 +68,19 @@ template <int D> struct PtCfg {
   static constexpr int OFF_EPI = OFF_V + NV * KVBYTES;
   static constexpr int OFF_PIECE = OFF_EPI + 8 * 32 * EPI_PITCH;
   static constexpr int OFF_BAR = OFF_PIECE + PT_RING * static_cast<int>(sizeof(Piece));
-  static constexpr int NBAR = 2 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 5 + 1 + 2;
+  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 5 + 1 + 2 + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_MISC + 256 + 1024;  // and slack for alignment
 };
 
 // ------------------------------------------------------------------------------------ the work
 __device__ __forceinline__ int64_t shfl64(int64_t v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
+
+// a / b of non-negative numbers, mostly below 2^32
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
 
 // Whether the groups of sequences rise inside the batch; the whole block calls it.
 __device__ __forceinline__ bool groups_ok(const PagedAttn& p) {
@@ -109,7 +118,9 @@ struct Item {
   int start, len;    // rows [start, len) of the sequences
   int tiles, units, rows, alt;
 };
-__device__ __forceinline__ Item decode_item(const PagedAttn& p, int groups, int tpt, int i) {
+// (Not inlined, like prompt_seq: a launch's first pass through code waits for instructions, and the copies of
+// these on the way to the first load cost more than the calls.)
+__device__ __noinline__ Item decode_item(const PagedAttn& p, int groups, int tpt, int i) {
   Item it;
   if (i < groups) {
     it.first = p.prefix_cu[i];
@@ -169,7 +180,7 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t* sme
 struct Seq {
   int c0, n, len, nq, mt;
 };
-__device__ __forceinline__ Seq prompt_seq(const PagedAttn& p, int utok, int b) {
+__device__ __noinline__ Seq prompt_seq(const PagedAttn& p, int utok, int b) {
   Seq s;
   int c1;
   paged_tokens(p.cu, b, p.T, p.err, s.c0, c1);
@@ -206,6 +217,7 @@ struct Sched {
   Item item;
   Seq seq;
   int groups, tpt, chunk;
+  bool loaded;
 
   __device__ __forceinline__ void load(const PagedAttn& p) {
     const int i = i0 + lane_id();
@@ -233,12 +245,18 @@ struct Sched {
   }
   // the lane whose item has place `at`; -1 past the last item. Sets the place within it.
   __device__ __forceinline__ int find(const PagedAttn& p, int64_t at, int64_t& off) {
-    while (at >= base_t + shfl64(inc_t, 31)) {
-      base_t += shfl64(inc_t, 31);
+    while (true) {
+      if (!loaded) {
+        if (i0 >= n) return -1;
+        load(p);
+        loaded = true;
+      }
+      const int64_t past = base_t + shfl64(inc_t, 31);
+      if (at < past) break;
+      base_t = past;
       base_r += shfl64(inc_r, 31);
       i0 += 32;
-      if (i0 >= n) return -1;
-      load(p);
+      loaded = false;
     }
     const int src = __ffs(__ballot_sync(0xFFFFFFFFu, at < base_t + inc_t)) - 1;
     off = at - base_t - (shfl64(inc_t, src) - shfl64(cnt, src));
@@ -252,16 +270,17 @@ struct Sched {
     if (p.decode) {
       if (pos >= end) return;
       int64_t off;
-      const int src = find(p, pos, off);
+      const int src = find(p, pos, off); 
       if (src < 0) return;
       const int first = get(item.first, src), count = get(item.count, src), start = get(item.start, src);
       const int len = get(item.len, src), tiles = get(item.tiles, src), units = get(item.units, src);
       const int irows = get(item.rows, src), alt = get(item.alt, src);
       const int64_t row0 = base_r + shfl64(inc_r, src) - shfl64(rows, src);
       const bool shared = i0 + src < groups;
-      const int u = static_cast<int>(off / tiles), up = u % units;
+      const int64_t u64 = quotient(off, tiles);
+      const int u = static_cast<int>(u64), up = u % units;
       pc.h = u / units;
-      pc.j0 = static_cast<int>(off % tiles);
+      pc.j0 = static_cast<int>(off - u64 * tiles);
       const int take = static_cast<int>(min(static_cast<int64_t>(tiles - pc.j0), end - pos));
       pos += take;
       pc.tok0 = first + up * 2 * tpt;
@@ -357,7 +376,9 @@ struct TileLoader {
     box = min(1 << p.ps_shift, PT_BN);
     npt = PT_BN / box;
     batch = -1;
+    page = ahead = 0;
   }
+  __device__ __forceinline__ int batch_of(int j) const { return j / (32 / npt); }
   __device__ __forceinline__ int look(const PagedAttn& p, const Piece& pc, int bt) {
     const int key = pc.kb + bt * 32 * box + lane_id() * box;
     if (key >= pc.kend) return 0;
@@ -406,9 +427,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* q_full = bars;
-  uint64_t* q_empty = bars + 1;
-  uint64_t* k_full = bars + 2;          // [NK]
+  uint64_t* q_full = bars;              // [2] a tile of queries each
+  uint64_t* q_empty = bars + 2;         // [2]
+  uint64_t* k_full = bars + 4;          // [NK]
   uint64_t* k_empty = k_full + NK;      // [NK]
   uint64_t* v_full = k_empty + NK;      // [NV]
   uint64_t* v_empty = v_full + NV;      // [NV]
@@ -421,6 +442,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   uint64_t* tile_free = o_full + 2;     // [2]
   uint64_t* mma_done = tile_free + 2;
   uint64_t* turn = mma_done + 1;        // [2]
+  uint64_t* level = turn + 2;           // [2] warp 1 + x is past its pieces of its own
   Piece* pieces = reinterpret_cast<Piece*>(smem + C::OFF_PIECE);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
@@ -429,8 +451,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 2);
     for (int s = 0; s < NK; ++s) {
       mbar_init(k_full + s, 1);
       mbar_init(k_empty + s, 2);
@@ -444,12 +464,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       mbar_init(w_empty + s, 11);
     }
     for (int x = 0; x < 2; ++x) {
+      mbar_init(q_full + x, 1);
+      mbar_init(q_empty + x, 2);
       mbar_init(s_full + x, 1);
       mbar_init(p_lo + x, 4);
       mbar_init(p_full + x, 4);
       mbar_init(o_full + x, 1);
       mbar_init(tile_free + x, 4);
       mbar_init(turn + x, 1);
+      mbar_init(level + x, 1);
     }
     mbar_init(mma_done, 2);
     *abort_flag = 0;
@@ -489,8 +512,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     if (p.decode) {
       const int64_t ctas = min(tt, static_cast<int64_t>(p.num_ctas));  // a tile at least for each
       if (blockIdx.x < ctas) {
-        pos = tt * blockIdx.x / ctas;
-        pos_end = tt * (blockIdx.x + 1) / ctas;
+        pos = quotient(tt * blockIdx.x, ctas);
+        pos_end = quotient(tt * (blockIdx.x + 1), ctas);
       }
       if (threadIdx.x == 0 && blockIdx.x == 0) p.rec_tile[n] = tt;
       for (int i = a; i < z; ++i) {
@@ -560,61 +583,69 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       sc.base_r = start[2];
     }
     if (!p.decode && p.may_split) sc.chunk = static_cast<int>(start[3]);
-    sc.load(p);
+    sc.loaded = false;
     int published = 0;
-    auto publish = [&](const Piece& pc) -> bool {
-      const int s = published % PT_RING;
-      if (!pt_wait(w_empty + s, ((published / PT_RING) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER)) return false;
-      if (lane == 0) {
-        pieces[s] = pc;
-        mbar_arrive(w_full + s);
-      }
-      __syncwarp();
-      ++published;
-      return true;
-    };
     TileLoader ld;
     ld.init(p);
-    Piece nx;
-    uint32_t q_par = 1;
-    int kpos = 0, q_issued = 0;
-    sc.next(p, nx);
-    bool ok = publish(nx);
-    while (ok && !nx.end) {
-      const Piece pc = nx;
-      if (!pt_wait(q_empty, q_par, ab, ERR_TIMEOUT_PRODUCER)) break;
-      q_par ^= 1;
-      if (lane == 0) {
-        const bool two = pc.alt || pc.ntok > tpt;
-        const uint32_t box = (pc.q1 ? 1 : tpt) * p.G * 128;
-        mbar_arrive_expect_tx(q_full, box * (D / 64) * (two ? 2 : 1));
-        for (int x = 0; x < (two ? 2 : 1); ++x)
-          for (int d = 0; d < D / 64; ++d)
-            tma_load_4d(smem + C::OFF_Q + x * C::QBYTES + d * (128 * 128), pc.q1 ? &p.tm_q1 : &p.tm_q, q_full, d * 64,
-                        pc.h * p.G, pc.tok0 + (pc.alt ? 0 : x * tpt), 0);
-      }
-      __syncwarp();
-      ++q_issued;
-      bool ahead = false;
-      ld.batch = -1;
-      const int je = pc.jend();
-      for (int j = pc.j0; ok && j < je; ++j) {
-        const int slot = kpos % NK;
-        ok = pt_wait(k_empty + slot, ((kpos / NK) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
-        if (!ok) break;
-        ld.load(p, pc, &p.tm_k, j, D, smem + C::OFF_K + slot * C::KVBYTES, k_full + slot);
-        ++kpos;
-        // the next piece while this one's first tiles are on their way
-        if (!ahead && j - pc.j0 == NK - 1) {
-          sc.next(p, nx);
-          ok = publish(nx);
-          ahead = true;
-        }
-      }
-      if (ok && !ahead) {
+    Piece nx, pc;
+    int kpos = 0, qpos = 0, j = 0, je = 0;
+    int pg0 = 0, pg1 = 0;  // the next piece's first pages, looked up early
+    bool want = true, have = false, ok = true;
+    while (true) {
+      if (want) {
+        // the next piece, while this one's first tiles are on their way
         sc.next(p, nx);
-        ok = publish(nx);
+        const int s = published % PT_RING;
+        ok = pt_wait(w_empty + s, ((published / PT_RING) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
+        if (!ok) break;
+        if (lane == 0) {
+          pieces[s] = nx;
+          mbar_arrive(w_full + s);
+        }
+        __syncwarp();
+        ++published;
+        if (p.table && !nx.end) {
+          pg0 = ld.look(p, nx, ld.batch_of(nx.j0));
+          pg1 = ld.look(p, nx, ld.batch_of(nx.j0) + 1);
+        }
+        want = false;
+        have = true;
       }
+      if (j >= je) {
+        if (!have) {
+          want = true;
+          continue;
+        }
+        if (nx.end) break;
+        pc = nx;
+        have = false;
+        j = pc.j0;
+        je = pc.jend();
+        ld.batch = ld.batch_of(j);
+        ld.page = pg0;
+        ld.ahead = pg1;
+        for (int x = 0; ok && x < pc.q_tiles(tpt); ++x, ++qpos) {
+          const int slot = qpos & 1;
+          ok = pt_wait(q_empty + slot, ((qpos >> 1) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(q_full + slot, (pc.q1 ? 1 : tpt) * p.G * 128 * (D / 64));
+            for (int d = 0; d < D / 64; ++d)
+              tma_load_4d(smem + C::OFF_Q + slot * C::QBYTES + d * (128 * 128), pc.q1 ? &p.tm_q1 : &p.tm_q,
+                          q_full + slot, d * 64, pc.h * p.G, pc.tok0 + x * tpt, 0);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (j >= je) continue;
+      }
+      const int slot = kpos % NK;
+      ok = pt_wait(k_empty + slot, ((kpos / NK) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
+      if (!ok) break;
+      ld.load(p, pc, &p.tm_k, j, D, smem + C::OFF_K + slot * C::KVBYTES, k_full + slot);
+      ++kpos;
+      ++j;
+      if (!have && j - pc.j0 == NK) want = true;
     }
     __syncwarp();
     if (lane == 0) {
@@ -622,7 +653,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       bool drained = true;
       for (int f = (kpos > NK ? kpos - NK : 0); f < kpos && drained; ++f)
         drained = mbar_drain(k_full + f % NK, (f / NK) & 1, p.err);
-      if (drained && q_issued > 0) mbar_drain(q_full, (q_issued - 1) & 1, p.err);
+      for (int f = (qpos > 2 ? qpos - 2 : 0); f < qpos && drained; ++f)
+        drained = mbar_drain(q_full + (f & 1), (f >> 1) & 1, p.err);
       // the last CTA leaves the counter as it found it
       if (!p.decode && atomicAdd(p.counter + 1, 1u) == gridDim.x - 1) {
         p.counter[0] = 0;
@@ -656,20 +688,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   } else if (warp == 1 || warp == 2) {
     // ================================================================ products of tile x
     // The warp runs converged and one elected lane issues. Tiles of a pair walk the same key tiles; both
-    // warps wait for every fill, in order, and release it, so a slot's two arrivals are of one fill and no wait
-    // can take an earlier phase for its own. They issue their batches (a tile's P V and the next one's
-    // Q K^T) in turn, tile 0 first, which keeps the two softmax passes half a period apart. Tiles that share the
-    // rows (`alt`) take every other fill and pass the rest on; they need no turns.
+    // warps wait for every fill, in order, and release it, so a slot's two arrivals are of one fill. They issue
+    // their batches (a tile's P V and the next one's Q K^T) in turn, tile 0 first, which keeps the two
+    // softmax passes half a period apart. Tiles that share the rows (`alt`) go apart: fills of even number are
+    // tile 0's, of odd number tile 1's, and their warp releases them with both arrivals. As the slots of a
+    // parity stay with a warp, it sees all of their phases; before a pair's piece, which it walks with the
+    // other one, they wait for each other, so that no earlier phase of the other's slots is still open.
     const int x = warp - 1;
     constexpr uint32_t IDESC_S = umma_idesc_f16(128, PT_BN, BF16, false);
     constexpr uint32_t IDESC_PV = umma_idesc_f16(128, D, BF16, true);
     const uint32_t tS = tmem + 128 * x;
     const uint32_t tO = tmem + 256 + D * x;
-    const uint64_t qdesc = umma_desc_sw128(smem_u32(smem + C::OFF_Q + x * C::QBYTES), 16, 1024);
+    const uint64_t qdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
     const uint64_t kdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
     const uint64_t vdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_V), PT_BN * 128, 1024);
-    int kpos = 0, vpos = 0;
-    uint32_t q_par = 0, free_par = 1, p_par = 0, nbatch = 0;
+    int fpos = 0, qpos = 0;  // fills of the K and V rings, of the query slots
+    uint32_t free_par = 1, p_par = 0, nbatch = 0, nlevel = 0;
+    bool apart = false;
     Piece pc;
     bool ok = true;
     auto my_turn = [&]() -> bool {
@@ -682,10 +717,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       ++nbatch;
     };
     while (ok && take(pc, ERR_TIMEOUT_MMA)) {
-      ok = pt_wait(q_full, q_par, ab, ERR_TIMEOUT_MMA);
+      const int nq = pc.q_tiles(tpt), q0 = qpos;
+      for (int f = q0; ok && f < q0 + nq; ++f) ok = pt_wait(q_full + (f & 1), (f >> 1) & 1, ab, ERR_TIMEOUT_MMA);
       if (!ok) break;
-      q_par ^= 1;
+      qpos += nq;
       tc_fence_after();
+      const uint64_t qdesc = qdesc0 + static_cast<uint64_t>(((q0 + (nq == 2 ? x : 0)) & 1) * (C::QBYTES >> 4));
+      auto free_q = [&]() {  // once every score of this piece is issued
+        for (int f = q0; f < q0 + nq; ++f) umma_commit(q_empty + (f & 1));
+      };
       const int je = pc.jend();
       const bool mine = x == 0 || pc.alt || pc.ntok > tpt;
       bool freed = false, o_init = false;
@@ -737,48 +777,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         return true;
       };
       if (pc.alt) {
+        apart = true;
         const int n = je - pc.j0;
-        int ki = 0, vi = 0;
-        auto pass_k = [&]() -> bool {  // the other tile's fill
-          if (!wait_k(kpos + ki)) return false;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(k_empty + (kpos + ki) % NK);
-          ++ki;
+        auto scores = [&](int f) -> bool {
+          if (!wait_k(f)) return false;
+          issue_S(f);
+          umma_commit(k_empty + f % NK);
+          umma_commit(k_empty + f % NK);
           return true;
         };
-        auto pass_v = [&]() -> bool {
-          if (!wait_v(vpos + vi)) return false;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(v_empty + (vpos + vi) % NV);
-          ++vi;
-          return true;
-        };
-        auto next_S = [&]() -> bool {
-          if ((ki & 1) != x && !pass_k()) return false;
-          if (!wait_k(kpos + ki)) return false;
-          issue_S(kpos + ki);
-          umma_commit(k_empty + (kpos + ki) % NK);
-          ++ki;
-          return true;
-        };
-        if (x < n) ok = next_S();
-        else umma_commit(q_empty);
-        for (int i = x; ok && i < n; i += 2) {
-          if (i + 2 >= n) umma_commit(q_empty);  // every score of this piece is issued
-          if (vi < i) ok = pass_v();
-          ok = ok && wait_v(vpos + i) && weigh(vpos + i);
+        const int first = (fpos ^ x) & 1;
+        if (first < n) ok = scores(fpos + first);
+        else free_q();
+        for (int i = first; ok && i < n; i += 2) {
+          if (i + 2 >= n) free_q();
+          ok = wait_v(fpos + i) && weigh(fpos + i);
           if (!ok) break;
-          umma_commit(v_empty + (vpos + i) % NV);
-          ++vi;
-          if (i + 2 < n) ok = next_S();
+          umma_commit(v_empty + (fpos + i) % NV);
+          umma_commit(v_empty + (fpos + i) % NV);
+          if (i + 2 < n) ok = scores(fpos + i + 2);
         }
-        if (ok && ki < n) ok = pass_k();
-        if (ok && vi < n) ok = pass_v();
         if (!ok) break;
-        kpos += n;
-        vpos += n;
+        fpos += n;
       } else {
         auto uses = [&](int j) { return mine && j < (x ? pc.nt1 : pc.nt0); };
+        if (apart) {
+          if (lane == 0) mbar_arrive(level + x);
+          ok = pt_wait(level + (1 - x), nlevel & 1, ab, ERR_TIMEOUT_MMA);
+          if (!ok) break;
+          ++nlevel;
+          apart = false;
+        }
+        int kpos = fpos, vpos = fpos;
         if (pc.j0 < je) {
           ok = wait_k(kpos) && my_turn();
           if (!ok) break;
@@ -791,7 +821,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           const bool more = j + 1 < je;
           ok = wait_v(vpos);
           if (!ok) break;
-          if (!more) umma_commit(q_empty);  // every score of this piece is issued
+          if (!more) free_q();
           ok = my_turn();
           if (!ok) break;
           if (uses(j)) {
@@ -812,7 +842,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           }
         }
         if (!ok) break;
-        if (pc.j0 >= je) umma_commit(q_empty);
+        if (pc.j0 >= je) free_q();
+        fpos = vpos;
       }
       // The products' warp waits for the tile once a piece and always announces O; the epilogue always
       // waits for that before it gives the tile back, so the parities cannot run apart.
@@ -857,7 +888,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       float m_used = live ? -INFINITY : 1e30f, l = 0.f;
       bool o_has = false;
       const int my_end = pc.alt ? je : (x ? pc.nt1 : pc.nt0);
-      for (int j = pc.j0 + (pc.alt ? x : 0); valid && j < my_end; j += step) {
+      for (int j = pc.j0 + (pc.alt ? (vpos ^ x) & 1 : 0); valid && j < my_end; j += step) {
         const int f = vpos + (j - pc.j0);
         const int n0 = j * PT_BN;
         const int have = pc.kend - pc.kb - n0;  // rows of this tile that exist
@@ -930,47 +961,32 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         };
         int stop = 0;          // first 32-column chunk that the stream did not finish
         bool lo_sent = false;  // weights of keys 0..63 are final and announced
-        {
-          uint32_t sa[32], sb[32];
-          tmem_ld32_async(tS, sa);
+        // two halves in a loop: a launch's first pass through code waits for its instructions
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t sa[32], sb[32], w[16];
+          tmem_ld32_async(tS + half * 64, sa);
+          tmem_ld32_async(tS + half * 64 + 32, sb);
           tmem_ld32_wait(sa);
-          tmem_ld32_async(tS + 32, sb);
+          tmem_ld32_wait(sb);
           if (m_used == -INFINITY) {
             const float m0 = chunk_max(sa);
             m_used = m0 == -INFINITY ? 0.f : m0;
           }
-          const float nb = -m_used, most = m_used + 8.f;
-          auto one = [&](int c, uint32_t(&cur)[32], uint32_t(&nxt)[32]) -> bool {
-            if (__any_sync(0xFFFFFFFFu, chunk_max(cur) > most)) {
-              tmem_ld32_wait(nxt);
-              stop = c;
-              return false;
-            }
-            uint32_t w[16];
-            weights(cur, nb, w);
-            tmem_st16(tS + c * 16, w);
-            tmem_ld32_wait(nxt);
-            tmem_ld32_async(tS + (c + 2) * 32, cur);
-            return true;
-          };
-          if (one(0, sa, sb) && one(1, sb, sa)) {
-            tmem_ld32_wait(sb);
-            if (__any_sync(0xFFFFFFFFu, fmaxf(chunk_max(sa), chunk_max(sb)) > most)) {
-              stop = 2;
-            } else {
-              tmem_st_wait();
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(p_lo + x);
-              lo_sent = true;
-              uint32_t w[16];
-              weights(sa, nb, w);
-              tmem_st16(tS + 32, w);
-              weights(sb, nb, w);
-              tmem_st16(tS + 48, w);
-              stop = 4;
-            }
+          if (__any_sync(0xFFFFFFFFu, fmaxf(chunk_max(sa), chunk_max(sb)) > m_used + 8.f)) break;
+          if (half) {
+            // nothing stored will be rescaled: P V of keys 0..63 may begin
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_lo + x);
+            lo_sent = true;
           }
+          weights(sa, -m_used, w);
+          tmem_st16(tS + half * 32, w);
+          weights(sb, -m_used, w);
+          tmem_st16(tS + half * 32 + 16, w);
+          stop += 2;
         }
         if (stop < 4) {
           // some row outgrew its reference: the maximum of what is left, everything so far rescaled, by whole
@@ -1055,7 +1071,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         if (pc.split) {
           const int64_t row0 = (x ? pc.orow1 : pc.orow0) + wq * 32;
           if (live) p.part_s[row0 + lane] = make_float2(m_used, o_has ? l : 0.f);
-          if (o_has) {
+          if (o_has && left <= 8) {
+            // a few rows: every lane writes its own
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
+              if (live) {
+                uint4* to = reinterpret_cast<uint4*>(p.part_o + (row0 + lane) * D + c * 32);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) to[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+              }
+            }
+          } else if (o_has) {
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
@@ -1194,8 +1222,8 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__
     auto unit = [&](int i, const Item& it, int up, int in_unit) {
       if (!it.tiles) return;
       const int64_t u0 = p.rec_tile[i] + (static_cast<int64_t>(h) * it.units + up) * it.tiles;
-      const int c0 = static_cast<int>(((u0 + 1) * ctas - 1) / total);
-      const int c1 = static_cast<int>(((u0 + it.tiles) * ctas - 1) / total);
+      const int c0 = static_cast<int>(quotient((u0 + 1) * ctas - 1, total));
+      const int c1 = static_cast<int>(quotient((u0 + it.tiles) * ctas - 1, total));
       const int64_t base = p.rec_row[i] + static_cast<int64_t>(h) * it.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
                            static_cast<int64_t>(c0) * PT_ROWS + in_unit;
       const int n = c1 - c0 + 1, second = it.count * p.G;
@@ -1280,7 +1308,14 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   p.may_split = s.split;
   p.num_ctas = sms;
   auto kfn = paged_attn_kernel<D, BF16>;
-  cudaError_t e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  // the limit is raised once per device: asking for it costs a microsecond
+  static std::atomic<bool> raised[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !raised[dev].load(std::memory_order_relaxed))) {
+    e = cudaFuncSetAttribute(kfn, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e == cudaSuccess && dev < 64) raised[dev].store(true, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) return e;
   kfn<<<sms, PT_THREADS, C::SMEM, st>>>(p);
   e = cudaGetLastError();

@@ -1002,62 +1002,113 @@ class PagedKV:
         k = torch.empty((num_pages, heads, page_size, head_dim), dtype=dtype, device=device)
         return PagedKV(k, torch.empty_like(k))
 
-    def check(self, what, page_table, lengths, *others):
-        """Raises unless pool, ``page_table`` (int32 [B, max_pages]) and ``lengths`` (int32 [B]) fit together
-        on one device with ``others``; returns (device, B, num_pages, Hkv, page_size, d, max_pages)."""
-        k, v = self.k, self.v
-        dev = L.same_device(what, k, v, page_table, lengths, *others)
-        if k.dtype not in _HALF or v.dtype != k.dtype:
-            raise TypeError(f"{what}: pages must be bf16 or fp16")
-        size, st = k.shape, k.stride()
-        if len(size) != 4 or v.shape != size or v.stride() != st:
-            raise ValueError(f"{what}: k and v must be [num_pages, Hkv, page_size, d], with the same strides")
-        P, H, ps, D = size
-        if D not in (64, 128) or ps not in (16, 32, 64, 128, 256):
-            raise ValueError(f"{what}: need head_dim 64 or 128 and a page_size of 16, 32, 64, 128 or 256")
-        if P < 1 or H < 1:
-            raise ValueError(f"{what}: the pool needs at least one page and head")
-        _rows16(what, "pages", k, v)
-        if any(x == 0 for x, n in zip(st, size) if n > 1):
-            raise ValueError(f"{what}: pages must not be expanded")
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[1] < 1 or (
-                page_table.shape[1] > 1 and page_table.stride(1) != 1):
-            raise ValueError(f"{what}: page_table must be int32 [B, max_pages] with contiguous rows")
-        _ints(what, "lengths", lengths, page_table.shape[0])
-        return dev, page_table.shape[0], P, H, ps, D, page_table.shape[1]
+
+# The checks of the paged calls go by shapes, strides and types alone, and are kept by these: a step calls with the
+# same ones for every layer and token, and the checks cost more than its smallest launches.
+def _meta(t):
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
-def _rows16(what, name, *tensors):
-    """Refuses tensors whose rows (the last dimension) are not contiguous and 16-byte aligned."""
-    for t in tensors:
-        st = t.stride()
-        if st[-1] != 1 or t.data_ptr() % 16 or any(x * t.element_size() % 16 for x, n in zip(st[:-1], t.shape) if n > 1):
-            raise ValueError(f"{what}: rows of {name} must be contiguous and 16-byte aligned")
+def _rows16(what, name, m):
+    """Refuses rows (the last dimension) that are not contiguous, or whose strides are no multiples of 16 bytes."""
+    size, st, dtype = m
+    if st[-1] != 1 or any(x * dtype.itemsize % 16 for x, n in zip(st[:-1], size) if n > 1):
+        raise ValueError(f"{what}: rows of {name} must be contiguous and 16-byte aligned")
 
 
-def _ints(what, name, t, n):
-    if t.dtype != torch.int32 or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
+def _ints(what, name, m, n):
+    size, st, dtype = m
+    if dtype != torch.int32 or size != (n,) or (n > 1 and st[0] != 1):
         raise ValueError(f"{what}: {name} must be contiguous int32 [{n}]")
 
 
-def _packed(what, name, t, dtype, tokens=None, heads=None, head_dim=None):
+def _not_expanded(what, name, m):
+    if any(x == 0 for x, n in zip(m[1], m[0]) if n > 1):
+        raise ValueError(f"{what}: {name} must not be expanded")
+
+
+def _packed(what, name, m, dtype, tokens=None, heads=None, head_dim=None):
     """Checks [T, H, d] rows; returns (T, H, d, stride over T, stride over H)."""
-    size = t.shape
+    size, st, dt = m
     if len(size) != 3 or (tokens is not None and size[0] != tokens) or (heads is not None and size[1] != heads) or (
             head_dim is not None and size[2] != head_dim):
         raise ValueError(f"{what}: {name} must be [{'T' if tokens is None else tokens}, "
                          f"{'H' if heads is None else heads}, {'d' if head_dim is None else head_dim}]")
-    if t.dtype != dtype:
+    if dt != dtype:
         raise TypeError(f"{what}: {name} must be {dtype}")
-    _rows16(what, name, t)
-    st = t.stride()
+    _rows16(what, name, m)
     # extents of 1 never move
     return (*size, st[0] if size[0] > 1 else 0, st[1] if size[1] > 1 else 0)
 
 
-def _not_expanded(what, name, t):
-    if any(x == 0 for x, n in zip(t.stride(), t.shape) if n > 1):
-        raise ValueError(f"{what}: {name} must not be expanded")
+def _pool(what, k, v, page_table, lengths):
+    """Checks a pool, its page table and lengths; returns (dtype, B, num_pages, Hkv, page_size, d, max_pages,
+    strides over page, head and row, the table's stride)."""
+    size, st, dtype = k
+    if dtype not in _HALF or v[2] != dtype:
+        raise TypeError(f"{what}: pages must be bf16 or fp16")
+    if len(size) != 4 or v[:2] != k[:2]:
+        raise ValueError(f"{what}: k and v must be [num_pages, Hkv, page_size, d], with the same strides")
+    P, H, ps, D = size
+    if D not in (64, 128) or ps not in (16, 32, 64, 128, 256):
+        raise ValueError(f"{what}: need head_dim 64 or 128 and a page_size of 16, 32, 64, 128 or 256")
+    if P < 1 or H < 1:
+        raise ValueError(f"{what}: the pool needs at least one page and head")
+    _rows16(what, "pages", k)
+    _not_expanded(what, "pages", k)
+    tsize, tst, tdt = page_table
+    if len(tsize) != 2 or tdt != torch.int32 or tsize[1] < 1 or (tsize[1] > 1 and tst[1] != 1):
+        raise ValueError(f"{what}: page_table must be int32 [B, max_pages] with contiguous rows")
+    _ints(what, "lengths", lengths, tsize[0])
+    return (dtype, tsize[0], P, H, ps, D, tsize[1], (st[0] if P > 1 else 0, st[1] if H > 1 else 0, st[2]),
+            tst[0] if tsize[0] > 1 else 0)
+
+
+def _aligned16(what, pointers):
+    if pointers & 15:
+        raise ValueError(f"{what}: rows must be 16-byte aligned")
+
+
+@functools.lru_cache(maxsize=4096)
+def _append_layout(what, k, v, pk, pv, page_table, lengths, cu_seqlens, cos, sin, q, q_out, err):
+    """(sizes of the call, its strides, the type and shape of q_out)."""
+    dtype, B, P, H, ps, D, mp, pool_st, table_st = _pool(what, pk, pv, page_table, lengths)
+    T, _, _, k_t, k_h = _packed(what, "k", k, dtype, None, H, D)
+    _, _, _, v_t, v_h = _packed(what, "v", v, dtype, T, H, D)
+    if cu_seqlens is None:
+        if T != B:
+            raise ValueError(f"{what}: {T} tokens for {B} sequences: cu_seqlens says which are whose")
+    else:
+        _ints(what, "cu_seqlens", cu_seqlens, B + 1)
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{what}: cos and sin come together")
+    rows, cs, table_dtype = 0, 0, dtype
+    if cos is not None:
+        size, st, table_dtype = cos
+        if sin[:2] != cos[:2] or size[-1] != D or not (len(size) == 2 or (len(size) == 3 and size[0] == 1)):
+            raise ValueError(f"{what}: cos and sin must be [n, {D}] (or [1, n, {D}]), with the same strides")
+        if table_dtype not in (torch.float32, dtype) or sin[2] != table_dtype:
+            raise TypeError(f"{what}: cos and sin must be fp32 or {dtype}")
+        _rows16(what, "cos and sin", cos)
+        rows, cs = size[-2], st[-2] if size[-2] > 1 else 0
+    Hq, q_t, q_h, o_t, o_h = 0, 0, 0, 0, 0
+    if q is not None:
+        if cos is None:
+            raise ValueError(f"{what}: queries are rotated: cos and sin are needed")
+        _, Hq, _, q_t, q_h = _packed(what, "q", q, dtype, T, None, D)
+        if q_out is None:
+            o_t, o_h = Hq * D, D
+        else:
+            _not_expanded(what, "q_out", q_out)
+            _, _, _, o_t, o_h = _packed(what, "q_out", q_out, dtype, T, Hq, D)
+    elif q_out is not None:
+        raise ValueError(f"{what}: q_out without q")
+    if err is not None and (err[2] != torch.int32 or 0 in err[0]):
+        raise ValueError(f"{what}: err must be int32")
+    strides = L.int64s((k_t, k_h, v_t, v_h, q_t, q_h, o_t, o_h, *pool_st, table_st, cs))
+    code = _HALF[dtype]
+    return ((strides, code, 0 if table_dtype == torch.float32 else code, T, B, H, Hq, D, P, ps, mp, rows),
+            None if q is None else (T, Hq, D))
 
 
 def paged_append(k, v, pool: PagedKV, page_table, lengths, *, cu_seqlens=None, cos=None, sin=None, q=None, q_out=None,
@@ -1077,53 +1128,19 @@ def paged_append(k, v, pool: PagedKV, page_table, lengths, *, cu_seqlens=None, c
     [1]) gets the first of 0x601 (a page number outside the pool), 0x602 (a length past the page table) and 0x603
     (a position past the tables); such rows are not stored. New rows must not share a place in the pool."""
     what = "paged_append"
-    dev, B, P, H, ps, D, mp = pool.check(what, page_table, lengths, k, v, cu_seqlens, cos, sin, q, q_out, err)
-    dtype = pool.k.dtype
-    T, _, _, k_t, k_h = _packed(what, "k", k, dtype, None, H, D)
-    _, _, _, v_t, v_h = _packed(what, "v", v, dtype, T, H, D)
-    if cu_seqlens is None:
-        if T != B:
-            raise ValueError(f"{what}: {T} tokens for {B} sequences: cu_seqlens says which are whose")
-    else:
-        _ints(what, "cu_seqlens", cu_seqlens, B + 1)
-    if (cos is None) != (sin is None):
-        raise ValueError(f"{what}: cos and sin come together")
-    rows, cs, table_dtype = 0, 0, dtype
-    if cos is not None:
-        if cos.dim() == 3 and cos.shape[0] == 1:
-            cos = cos[0]
-        if sin.dim() == 3 and sin.shape[0] == 1:
-            sin = sin[0]
-        if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.stride() != cos.stride():
-            raise ValueError(f"{what}: cos and sin must be [n, {D}] (or [1, n, {D}]), with the same strides")
-        if cos.dtype not in (torch.float32, dtype) or sin.dtype != cos.dtype:
-            raise TypeError(f"{what}: cos and sin must be fp32 or {dtype}")
-        _rows16(what, "cos and sin", cos, sin)
-        rows, cs, table_dtype = cos.shape[0], cos.stride(0) if cos.shape[0] > 1 else 0, cos.dtype
-    Hq, q_t, q_h, o_t, o_h = 0, 0, 0, 0, 0
-    if q is not None:
-        if cos is None:
-            raise ValueError(f"{what}: queries are rotated: cos and sin are needed")
-        _, Hq, _, q_t, q_h = _packed(what, "q", q, dtype, T, None, D)
-        if q_out is None:
-            q_out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
-        else:
-            _not_expanded(what, "q_out", q_out)
-        _, _, _, o_t, o_h = _packed(what, "q_out", q_out, dtype, T, Hq, D)
-    elif q_out is not None:
-        raise ValueError(f"{what}: q_out without q")
-    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
-        raise ValueError(f"{what}: err must be int32")
-    if T == 0 or B == 0:
+    pk, pv = pool.k, pool.v
+    L.same_device(what, k, v, pk, pv, page_table, lengths, cu_seqlens, cos, sin, q, q_out, err)
+    args, made = _append_layout(what, _meta(k), _meta(v), _meta(pk), _meta(pv), _meta(page_table), _meta(lengths),
+                                _meta(cu_seqlens), _meta(cos), _meta(sin), _meta(q), _meta(q_out), _meta(err))
+    if made is not None and q_out is None:
+        q_out = q.new_empty(made)
+    if args[3] == 0 or args[4] == 0:
         return q_out
-    pp, ph, pr, _ = pool.k.stride()
-    strides = L.int64s((k_t, k_h, v_t, v_h, q_t, q_h, o_t, o_h, pp if P > 1 else 0, ph if H > 1 else 0, pr,
-                        page_table.stride(0), cs))
-    L.check(L.load().dab_paged_append(
-        k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), pool.k.data_ptr(), pool.v.data_ptr(), page_table.data_ptr(),
-        lengths.data_ptr(), _ptr(cu_seqlens), _ptr(cos), _ptr(sin), strides, _HALF[dtype],
-        0 if table_dtype == torch.float32 else _HALF[dtype], T, B, H, Hq, D, P, ps, mp, rows, _ptr(err),
-        L.stream_of(k)), what)
+    ptrs = (k.data_ptr(), v.data_ptr(), _ptr(q), _ptr(q_out), pk.data_ptr(), pv.data_ptr())
+    at_cos, at_sin = _ptr(cos), _ptr(sin)
+    _aligned16(what, ptrs[0] | ptrs[1] | ptrs[4] | ptrs[5] | (at_cos or 0) | (at_sin or 0) | (ptrs[2] or 0) | (ptrs[3] or 0))
+    L.check(L.load().dab_paged_append(*ptrs, page_table.data_ptr(), lengths.data_ptr(), _ptr(cu_seqlens), at_cos, at_sin,
+                                      *args, _ptr(err), L.stream_of(k)), what)
     return q_out
 
 
@@ -1140,26 +1157,68 @@ def paged_attention_workspace(tokens, batch, q_heads, kv_heads, head_dim, prefix
                             prefix_groups)
 
 
-def _paged_call(what, dev, q, out, workspace, B, H, D, dtype, groups=0):
-    """Checks queries, output and workspace of an attention call; returns (out, Hq / Hkv, their strides,
-    workspace, stream), out alone where there is nothing to do."""
+def _queries(what, q, out, dtype, H, D):
+    """Checks queries and output; returns (T, Hq / Hkv, their strides)."""
     T, Hq, _, q_t, q_h = _packed(what, "q", q, dtype, None, None, D)
     _not_expanded(what, "q", q)
     if Hq % H:
         raise ValueError(f"{what}: query heads must be a multiple of {H}")
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=q.device)
-    else:
+    o_t, o_h = Hq * D, D
+    if out is not None:
         _not_expanded(what, "out", out)
-    _, _, _, o_t, o_h = _packed(what, "out", out, dtype, T, Hq, D)
-    if T == 0 or B == 0 or Hq == 0:
-        return out, None
+        _, _, _, o_t, o_h = _packed(what, "out", out, dtype, T, Hq, D)
+    return T, Hq // H, (q_t, q_h, o_t, o_h)
+
+
+@functools.lru_cache(maxsize=4096)
+def _varlen_layout(what, q, k, v, cu_seqlens, out):
+    dtype = q[2]
+    if dtype not in _HALF:
+        raise TypeError(f"{what}: queries must be bf16 or fp16")
+    T, H, D, k_t, k_h = _packed(what, "k", k, dtype, q[0][0] if q[0] else None)
+    if D not in (64, 128) or H < 1:
+        raise ValueError(f"{what}: need head_dim 64 or 128 and at least one kv-head")
+    _, _, _, v_t, v_h = _packed(what, "v", v, dtype, T, H, D)
+    _not_expanded(what, "k", k)
+    _not_expanded(what, "v", v)
+    if len(cu_seqlens[0]) != 1 or cu_seqlens[0][0] < 1:
+        raise ValueError(f"{what}: cu_seqlens must be int32 [B + 1]")
+    B = cu_seqlens[0][0] - 1
+    _ints(what, "cu_seqlens", cu_seqlens, B + 1)
+    T, G, st = _queries(what, q, out, dtype, H, D)
+    return (T, B, H, G, D, 0), L.int64s((*st, 0, k_h, k_t, 0, v_h, v_t, 0)), _HALF[dtype], (T, B, H, G, D)
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_layout(what, q, k, v, page_table, lengths, cu_seqlens, out, prefix_cu, prefix_lengths):
+    dtype, B, P, H, ps, D, mp, pool_st, table_st = _pool(what, k, v, page_table, lengths)
+    T, G, st = _queries(what, q, out, dtype, H, D)
+    strides = L.int64s((*st, *pool_st, *pool_st, table_st))
+    if cu_seqlens is not None:
+        _ints(what, "cu_seqlens", cu_seqlens, B + 1)
+        return (T, B, H, G, D, 0), strides, _HALF[dtype], (T, B, H, G, D, P, ps, mp)
+    if T != B:
+        raise ValueError(f"{what}: q must be [{B}, Hq, {D}]")
+    if (prefix_cu is None) != (prefix_lengths is None):
+        raise ValueError(f"{what}: prefix_cu and prefix_lengths come together")
+    groups = 0
+    if prefix_cu is not None:
+        groups = prefix_lengths[0][0] if len(prefix_lengths[0]) == 1 else -1
+        _ints(what, "prefix_lengths", prefix_lengths, groups)
+        _ints(what, "prefix_cu", prefix_cu, groups + 1)
+        if groups > B:
+            raise ValueError(f"{what}: {groups} groups of {B} sequences")
+    return (T, B, H, G, D, groups), strides, _HALF[dtype], (B, H, G, D, P, ps, mp, groups)
+
+
+def _paged_scratch(what, dev, q, sizes, workspace):
+    """(pointer, bytes, stream) of an attention call."""
     st = L.stream_of(q)
     if workspace is None:
-        workspace = L.workspace(q.device, st.value, _paged_workspace(dev, T, B, H, Hq // H, D, groups), tag="paged")
+        workspace = L.workspace(q.device, st.value, _paged_workspace(dev, *sizes), tag="paged")
     else:
         _own_workspace(what, workspace)
-    return out, (T, Hq // H, (q_t, q_h, o_t, o_h), workspace, st)
+    return workspace.data_ptr(), workspace.numel(), st
 
 
 def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, workspace=None):
@@ -1167,42 +1226,27 @@ def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, w
     padding.
 
     q [T, Hq, d], k / v [T, Hkv, d] (bf16 / fp16, d 64 or 128, any token and head strides; q-head h reads kv-head
-    h // (Hq / Hkv), at most 128 q-heads per kv-head; sm_scale is positive), cu_seqlens int32 [B + 1] on the device, rising from 0: it
-    is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] from cu_seqlens[B] on are left
-    alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and may reach rows before it
-    within the same 128 keys.
+    h // (Hq / Hkv), at most 128 q-heads per kv-head; sm_scale is positive), cu_seqlens int32 [B + 1] on the device,
+    rising from 0: it is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] from
+    cu_seqlens[B] on are left alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and
+    may reach rows before it within the same 128 keys.
 
     ``workspace`` (uint8, ``paged_attention_workspace`` bytes, zero-filled once, used by one stream at a time)
     replaces the library's own, which is given up when a later call needs a larger one: a call that is
     captured in a CUDA graph takes the caller's."""
     what = "flash_varlen"
     dev = L.same_device(what, q, k, v, cu_seqlens, out, workspace)
-    if q.dtype not in _HALF:
-        raise TypeError(f"{what}: queries must be bf16 or fp16")
-    T, H, D, k_t, k_h = _packed(what, "k", k, q.dtype, q.shape[0])
-    if D not in (64, 128) or H < 1:
-        raise ValueError(f"{what}: need head_dim 64 or 128 and at least one kv-head")
-    _, _, _, v_t, v_h = _packed(what, "v", v, q.dtype, T, H, D)
-    for name, t in (("k", k), ("v", v)):
-        _not_expanded(what, name, t)
-    B = cu_seqlens.numel() - 1
-    _ints(what, "cu_seqlens", cu_seqlens, max(B, 0) + 1)
-    out, call = _paged_call(what, dev, q, out, workspace, B, H, D, q.dtype)
-    if call is None:
+    sizes, strides, code, args = _varlen_layout(what, _meta(q), _meta(k), _meta(v), _meta(cu_seqlens), _meta(out))
+    if out is None:
+        out = q.new_empty(q.shape)
+    if 0 in sizes[:4]:
         return out
-    T, G, st4, ws, st = call
+    ptrs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr())
+    _aligned16(what, ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3])
     L.check(L.load().dab_flash_varlen(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_seqlens.data_ptr(),
-        L.int64s((*st4, 0, k_h, k_t, 0, v_h, v_t, 0)), float(D ** -0.5 if sm_scale is None else sm_scale),
-        1 if causal else 0, _HALF[q.dtype], T, B, H, G, D, ws.data_ptr(), ws.numel(), st), what)
+        *ptrs, cu_seqlens.data_ptr(), strides, sizes[4] ** -0.5 if sm_scale is None else float(sm_scale), 1 if causal else 0,
+        code, *args, *_paged_scratch(what, dev, q, sizes, workspace)), what)
     return out
-
-
-def _pool_strides(pool, page_table):
-    P, H = pool.k.shape[:2]
-    pp, ph, pr, _ = pool.k.stride()
-    one = (pp if P > 1 else 0, ph if H > 1 else 0, pr)
-    return (*one, *one, page_table.stride(0))
 
 
 def flash_paged(q, pool: PagedKV, page_table, lengths, cu_seqlens, *, causal=True, sm_scale=None, out=None,
@@ -1212,17 +1256,22 @@ def flash_paged(q, pool: PagedKV, page_table, lengths, cu_seqlens, *, causal=Tru
     prompt, a piece of one, or the prompt behind a prefix that is cached already. A query at a negative position
     gives 0. Everything else as in ``flash_varlen``."""
     what = "flash_paged"
-    dev, B, P, H, ps, D, mp = pool.check(what, page_table, lengths, q, cu_seqlens, out, workspace)
-    _ints(what, "cu_seqlens", cu_seqlens, B + 1)
-    out, call = _paged_call(what, dev, q, out, workspace, B, H, D, pool.k.dtype)
-    if call is None:
+    if cu_seqlens is None:
+        raise ValueError(f"{what}: cu_seqlens is needed")
+    pk, pv = pool.k, pool.v
+    dev = L.same_device(what, q, pk, pv, page_table, lengths, cu_seqlens, out, workspace)
+    sizes, strides, code, args = _paged_layout(what, _meta(q), _meta(pk), _meta(pv), _meta(page_table), _meta(lengths),
+                                               _meta(cu_seqlens), _meta(out), None, None)
+    if out is None:
+        out = q.new_empty(q.shape)
+    if 0 in sizes[:4]:
         return out
-    T, G, st4, ws, st = call
+    ptrs = (q.data_ptr(), out.data_ptr(), pk.data_ptr(), pv.data_ptr())
+    _aligned16(what, ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3])
     L.check(L.load().dab_flash_paged(
-        q.data_ptr(), out.data_ptr(), pool.k.data_ptr(), pool.v.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-        cu_seqlens.data_ptr(), L.int64s((*st4, *_pool_strides(pool, page_table))),
-        float(D ** -0.5 if sm_scale is None else sm_scale), 1 if causal else 0, _HALF[q.dtype], T, B, H, G, D, P, ps, mp,
-        ws.data_ptr(), ws.numel(), st), what)
+        *ptrs, page_table.data_ptr(), lengths.data_ptr(), cu_seqlens.data_ptr(), strides,
+        sizes[4] ** -0.5 if sm_scale is None else float(sm_scale), 1 if causal else 0, code, *args,
+        *_paged_scratch(what, dev, q, sizes, workspace)), what)
     return out
 
 
@@ -1237,27 +1286,20 @@ def decode_attention_paged(q, pool: PagedKV, page_table, lengths, *, prefix_cu=N
     [G]): the first prefix_lengths[g] rows are the same for all members, whose page tables begin with the same
     pages. Whole pages of them are read once for the group. Everything else as in ``flash_varlen``."""
     what = "decode_attention_paged"
-    dev, B, P, H, ps, D, mp = pool.check(what, page_table, lengths, q, prefix_cu, prefix_lengths, out, workspace)
-    if q.dim() != 3 or q.shape[0] != B:
-        raise ValueError(f"{what}: q must be [{B}, Hq, {D}]")
-    if (prefix_cu is None) != (prefix_lengths is None):
-        raise ValueError(f"{what}: prefix_cu and prefix_lengths come together")
-    groups = 0
-    if prefix_cu is not None:
-        groups = prefix_lengths.numel()
-        _ints(what, "prefix_lengths", prefix_lengths, groups)
-        _ints(what, "prefix_cu", prefix_cu, groups + 1)
-        if groups > B:
-            raise ValueError(f"{what}: {groups} groups of {B} sequences")
-    out, call = _paged_call(what, dev, q, out, workspace, B, H, D, pool.k.dtype, groups)
-    if call is None:
+    pk, pv = pool.k, pool.v
+    dev = L.same_device(what, q, pk, pv, page_table, lengths, prefix_cu, prefix_lengths, out, workspace)
+    sizes, strides, code, args = _paged_layout(what, _meta(q), _meta(pk), _meta(pv), _meta(page_table), _meta(lengths),
+                                               None, _meta(out), _meta(prefix_cu), _meta(prefix_lengths))
+    if out is None:
+        out = q.new_empty(q.shape)
+    if 0 in sizes[:4]:
         return out
-    _, G, st4, ws, st = call
+    ptrs = (q.data_ptr(), out.data_ptr(), pk.data_ptr(), pv.data_ptr())
+    _aligned16(what, ptrs[0] | ptrs[1] | ptrs[2] | ptrs[3])
     L.check(L.load().dab_decode_attention_paged(
-        q.data_ptr(), out.data_ptr(), pool.k.data_ptr(), pool.v.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-        _ptr(prefix_cu), _ptr(prefix_lengths), L.int64s((*st4, *_pool_strides(pool, page_table))),
-        float(D ** -0.5 if sm_scale is None else sm_scale), _HALF[q.dtype], B, H, G, D, P, ps, mp, groups,
-        ws.data_ptr(), ws.numel(), st), what)
+        *ptrs, page_table.data_ptr(), lengths.data_ptr(), _ptr(prefix_cu), _ptr(prefix_lengths), strides,
+        sizes[4] ** -0.5 if sm_scale is None else float(sm_scale), code, *args,
+        *_paged_scratch(what, dev, q, sizes, workspace)), what)
     return out
 
 
