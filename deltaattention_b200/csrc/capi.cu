@@ -1121,10 +1121,8 @@ size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t
                                           int64_t head_dim, int64_t prefix_groups) {
   if (tokens < 0 || batch < 0 || heads < 1 || kv_group < 1 || kv_group > 128 || head_dim < 1 || prefix_groups < 0) return 0;
   const int sms = num_sms();
-  size_t n = paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, 0, false, sms);
-  if (tokens == batch)
-    n = std::max(n, paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, prefix_groups, true, sms));
-  return WS_HEADER + n;
+  return WS_HEADER + std::max(paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, 0, false, sms),
+                              paged_attn_workspace(batch, batch, heads, kv_group, head_dim, prefix_groups, true, sms));
 }
 
 namespace {
@@ -1155,8 +1153,9 @@ int paged_attend(const char* nm, PagedAttn& p, const int64_t* s, float sm_scale,
   if (head_dim != 64 && head_dim != 128) return fail(1, std::string(nm) + ": head_dim must be 64 or 128");
   if (kv_group < 1 || kv_group > 128) return fail(1, std::string(nm) + ": need 1 to 128 q-heads per kv-head");
   if (tokens < 0 || batch < 0 || heads < 1 || heads * kv_group > 65535 || tokens >= (int64_t{1} << 30) ||
-      batch >= (int64_t{1} << 24) || groups < 0)
-    return fail(1, std::string(nm) + ": need 1 to 65535 q-heads, tokens below 2^30 and sequences below 2^24");
+      batch >= (int64_t{1} << 24) || groups < 0 || tokens * heads * kv_group >= (int64_t{1} << 31))
+    return fail(1, std::string(nm) + ": need 1 to 65535 q-heads, tokens below 2^30, sequences below 2^24 and rows of "
+                                     "queries below 2^31");
   if (!(sm_scale > 0.f) || sm_scale > 1e30f) return fail(1, std::string(nm) + ": sm_scale must be positive");
   // strides: q(2) out(2) k(3: page, head, row) v(3) page table(1) = 11
   if (!rows16({p.q, p.out, p.k, p.v}, s, 10)) return fail(1, std::string(nm) + ": rows must be 16-byte aligned");

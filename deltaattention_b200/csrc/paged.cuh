@@ -42,9 +42,10 @@ struct PagedAttn {
   int decode;     // one token per sequence, the work cut into even ranges of key tiles
   int may_split;  // prompts: the units may be too few for the SMs
   int num_ctas;
+  int w_start, w_pair, w_alt;  // decode: costs of beginning a unit, and of its key tiles
   // workspace: piece counter and finished CTAs, records of sequences and groups, partial results
   unsigned* counter;
-  int64_t* rec_tile; int64_t* rec_row; float* part_o; float2* part_s;
+  int64_t* rec_cost; int64_t* rec_row; float* part_o; float2* part_s;
 };
 
 // Records a wrong argument that only the device sees; the first one stays.

@@ -23,6 +23,7 @@
 // the tiles' softmax, a row per thread. The loads are TMA boxes of a page (or of 128 packed rows), scores
 // and weights live in TMEM, weights in the rows' 16-bit type: an error of half a step per weight, as large as
 // that of the rounded output. The running maximum moves only when a row outgrows it by 2^8.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -34,8 +35,12 @@ constexpr int PT_THREADS = 384;
 constexpr int PT_BN = 128;   // keys of a tile
 constexpr int PT_RING = 4;   // pieces published ahead
 constexpr int PT_ROWS = 256; // partial rows between the pieces of neighbouring CTAs
-constexpr int PT_MIN_CHUNK = 4;
-constexpr int PT_FILL = 3;   // chunks per SM that cut prompts aim at
+constexpr int PT_THIN = 8;  // most rows of a thin piece (its products are computed for 16)
+constexpr int PT_CHUNKS = 16;     // most chunks that a prompt's mean unit is cut into
+constexpr int PT_MIN_CHUNK = 2;
+constexpr int PT_FILL = 7;        // most chunks per SM: they bound the workspace
+constexpr int PT_PIECE = 2;
+constexpr int PT_JOIN = 3;
 
 struct Piece {
   int end;         // no more pieces
@@ -50,6 +55,7 @@ struct Piece {
   int by_length;   // .. and no more than the token's sequence has
   int split;       // partial results to rows orow0 / orow1, else the output
   int q1;          // one token: the query box of one token
+  int thin;        // at most PT_THIN rows: scores and output are computed transposed
   int64_t orow0, orow1;
   __device__ __forceinline__ int jend() const { return max(nt0, nt1); }
   // query tiles it needs: tiles that hold the same rows share one
@@ -66,9 +72,12 @@ template <int D> struct PtCfg {
   static constexpr int OFF_V = OFF_K + NK * KVBYTES;
   static constexpr int EPI_PITCH = 80;  // 64 bytes of a row's output and 16 more against bank conflicts
   static constexpr int OFF_EPI = OFF_V + NV * KVBYTES;
-  static constexpr int OFF_PIECE = OFF_EPI + 8 * 32 * EPI_PITCH;
+  static constexpr int OFF_P = OFF_EPI + 8 * 32 * EPI_PITCH;  // weights of thin pieces, [2][16 rows x 128 keys], rows from PT_THIN on unused
+  static constexpr int PBYTES = 16 * PT_BN * 2;
+  static constexpr int OFF_VOTE = OFF_P + 2 * PBYTES;  // [2 tiles][2][4 warps][PT_THIN] maxima, then flags
+  static constexpr int OFF_PIECE = OFF_VOTE + 2 * 2 * 4 * (PT_THIN + 1) * 4;
   static constexpr int OFF_BAR = OFF_PIECE + PT_RING * static_cast<int>(sizeof(Piece));
-  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 5 + 1 + 2 + 2;
+  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 6 + 1 + 2 + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_MISC + 256 + 1024;  // and slack for alignment
 };
@@ -77,7 +86,7 @@ template <int D> struct PtCfg {
 __device__ __forceinline__ int64_t shfl64(int64_t v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
 
 // a / b of non-negative numbers, mostly below 2^32
-__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+__device__ __noinline__ int64_t quotient(int64_t a, int64_t b) {
   if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
   return a / b;
 }
@@ -117,7 +126,18 @@ struct Item {
   int first, count;  // sequences
   int start, len;    // rows [start, len) of the sequences
   int tiles, units, rows, alt;
+  // what a unit and the item cost: a start for each unit, and its key tiles
+  __device__ __forceinline__ int tile_cost(const PagedAttn& p) const { return alt ? p.w_alt : p.w_pair; }
+  __device__ __forceinline__ int64_t unit_cost(const PagedAttn& p) const {
+    return tiles ? p.w_start + static_cast<int64_t>(tiles) * tile_cost(p) : 0;
+  }
+  __device__ __forceinline__ int64_t cost(const PagedAttn& p) const { return static_cast<int64_t>(p.H) * units * unit_cost(p); }
 };
+// CTAs that take part: the dearest key tile at least for each, so that a CTA whose range lies inside a unit has one of
+// its tiles
+__device__ __forceinline__ int64_t decode_ctas(const PagedAttn& p, int64_t total) {
+  return min(max(quotient(total, max(p.w_alt, p.w_pair)), total ? int64_t{1} : int64_t{0}), static_cast<int64_t>(p.num_ctas));
+}
 // (Not inlined, like prompt_seq: a launch's first pass through code waits for instructions, and the copies of
 // these on the way to the first load cost more than the calls.)
 __device__ __noinline__ Item decode_item(const PagedAttn& p, int groups, int tpt, int i) {
@@ -190,11 +210,22 @@ __device__ __noinline__ Seq prompt_seq(const PagedAttn& p, int utok, int b) {
   s.mt = max(1, (s.len + PT_BN - 1) / PT_BN);
   return s;
 }
-// Key tiles of a chunk, or 0 where units stay whole.
+// Key tiles of a chunk, or 0 where units stay whole: of the ways to cut the mean unit into 1 to 16 chunks, the one
+// with the least rounds of pieces times their length. A piece costs PT_PIECE key tiles beside its own.
 __device__ __forceinline__ int chunk_tiles(const PagedAttn& p, int64_t units, int64_t tiles) {
-  if (!p.may_split || units >= 2 * static_cast<int64_t>(p.num_ctas)) return 0;
-  const int64_t per = static_cast<int64_t>(PT_FILL) * p.num_ctas;
-  return static_cast<int>(min(max((tiles + per - 1) / per, static_cast<int64_t>(PT_MIN_CHUNK)), int64_t{1} << 24));
+  if (!p.may_split || units == 0 || units >= 2 * static_cast<int64_t>(p.num_ctas)) return 0;
+  const unsigned n = static_cast<unsigned>(units), mean = static_cast<unsigned>(quotient(tiles + units - 1, units));
+  const unsigned ctas = static_cast<unsigned>(p.num_ctas);
+  unsigned best = 0, least = 0xFFFFFFFFu;
+  for (unsigned k = 1; k <= PT_CHUNKS && (k == 1 || (mean >= PT_MIN_CHUNK * k && n * k <= PT_FILL * ctas)); ++k) {
+    // one chunk needs no joining, which costs some tiles' time as well
+    const unsigned len = (mean + k - 1) / k, cost = (n * k + ctas - 1) / ctas * (len + PT_PIECE) + (k > 1 ? PT_JOIN : 0);
+    if (cost < least) {
+      least = cost;
+      best = k == 1 ? 0 : len;
+    }
+  }
+  return static_cast<int>(best);
 }
 __device__ __forceinline__ int64_t prompt_pieces(const PagedAttn& p, const Seq& s, int chunk) {
   return static_cast<int64_t>(p.H) * s.nq * (chunk ? (s.mt + chunk - 1) / chunk : 1);
@@ -208,43 +239,48 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t par, const Abort
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ------------------------------------------------------------------------------------ pieces
-// The pieces of one CTA, in order; all lanes of warp 0 call it.
-struct Sched {
-  int64_t pos, end;             // decode: key tiles left
+// The pieces of one CTA, in order. All lanes of warp 0 call it and hold an item (a group or sequence of a decode step,
+// a prompt's sequence) each; the lane whose item is next works the piece out and writes it to `to`.
+// (Code that is rarely run waits for its instructions each time, so there is little of it.)
+template <bool DEC> struct Sched {
+  int64_t pos, end;             // decode: the range of costs left
   int i0, n;                    // items i0 .. i0 + 31 of n are in the lanes
-  int64_t base_t, base_r;       // tiles (pieces) and rows before item i0
-  int64_t cnt, inc_t, rows, inc_r;  // the lane's item: its count, the inclusive sums
-  Item item;
-  Seq seq;
+  int64_t base_t, base_r;       // costs (pieces) and partial rows before item i0
+  int64_t before_t, inc_t, before_r, inc_r;  // the lane's item: sums of costs and rows before and with it
+  typename std::conditional<DEC, Item, Seq>::type item;
   int groups, tpt, chunk;
   bool loaded;
 
   __device__ __forceinline__ void load(const PagedAttn& p) {
-    const int i = i0 + lane_id();
-    cnt = rows = 0;
-    if (i < n) {
-      if (p.decode) {
-        item = decode_item(p, groups, tpt, i);
-        cnt = static_cast<int64_t>(p.H) * item.units * item.tiles;
-        rows = static_cast<int64_t>(p.H) * item.rows;
-      } else {
-        seq = prompt_seq(p, 2 * tpt, i);
-        cnt = prompt_pieces(p, seq, chunk);
-      }
+    // lanes past the last item look at it too: a warp that runs apart is slow from here on
+    const bool has = i0 + lane_id() < n;
+    const int i = min(i0 + lane_id(), n - 1);
+    int64_t t, r = 0;
+    if constexpr (DEC) {
+      item = decode_item(p, groups, tpt, i);
+      t = item.cost(p);
+      r = static_cast<int64_t>(p.H) * item.rows;
+    } else {
+      item = prompt_seq(p, 2 * tpt, i);
+      t = prompt_pieces(p, item, chunk);
     }
-    inc_t = cnt;
-    inc_r = rows;
-#pragma unroll
+    inc_t = has ? t : 0;
+    inc_r = has ? r : 0;
+    before_t = inc_t;
+    before_r = inc_r;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t a = __shfl_up_sync(0xFFFFFFFFu, inc_t, o), b = __shfl_up_sync(0xFFFFFFFFu, inc_r, o);
+      const int64_t a = __shfl_up_sync(0xFFFFFFFFu, inc_t, o), b = DEC ? __shfl_up_sync(0xFFFFFFFFu, inc_r, o) : 0;
       if (lane_id() >= o) {
         inc_t += a;
         inc_r += b;
       }
     }
+    before_t = inc_t - before_t;
+    before_r = inc_r - before_r;
   }
-  // the lane whose item has place `at`; -1 past the last item. Sets the place within it.
-  __device__ __forceinline__ int find(const PagedAttn& p, int64_t at, int64_t& off) {
+  // the lane whose item has place `at`; -1 past the last item
+  __device__ __forceinline__ int find(const PagedAttn& p, int64_t at) {
     while (true) {
       if (!loaded) {
         if (i0 >= n) return -1;
@@ -254,117 +290,120 @@ struct Sched {
       const int64_t past = base_t + shfl64(inc_t, 31);
       if (at < past) break;
       base_t = past;
-      base_r += shfl64(inc_r, 31);
+      if (DEC) base_r += shfl64(inc_r, 31);
       i0 += 32;
       loaded = false;
     }
-    const int src = __ffs(__ballot_sync(0xFFFFFFFFu, at < base_t + inc_t)) - 1;
-    off = at - base_t - (shfl64(inc_t, src) - shfl64(cnt, src));
-    return src;
+    return __ffs(__ballot_sync(0xFFFFFFFFu, at < base_t + inc_t)) - 1;
   }
-  __device__ __forceinline__ int get(int v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
 
-  __device__ __forceinline__ void next(const PagedAttn& p, Piece& pc) {
+  __device__ __forceinline__ void next(const PagedAttn& p, Piece* to) {
     const int lane = lane_id();
-    pc.end = 1;
-    if (p.decode) {
-      if (pos >= end) return;
-      int64_t off;
-      const int src = find(p, pos, off); 
-      if (src < 0) return;
-      const int first = get(item.first, src), count = get(item.count, src), start = get(item.start, src);
-      const int len = get(item.len, src), tiles = get(item.tiles, src), units = get(item.units, src);
-      const int irows = get(item.rows, src), alt = get(item.alt, src);
-      const int64_t row0 = base_r + shfl64(inc_r, src) - shfl64(rows, src);
-      const bool shared = i0 + src < groups;
-      const int64_t u64 = quotient(off, tiles);
-      const int u = static_cast<int>(u64), up = u % units;
-      pc.h = u / units;
-      pc.j0 = static_cast<int>(off - u64 * tiles);
-      const int take = static_cast<int>(min(static_cast<int64_t>(tiles - pc.j0), end - pos));
-      pos += take;
-      pc.tok0 = first + up * 2 * tpt;
-      pc.ntok = min(2 * tpt, count - up * 2 * tpt);
-      pc.kb = start;
-      pc.kend = len;
-      pc.trow = first;
-      pc.by_length = 0;
-      if (shared) {
-        // the prefix is read through the first member that has all of it, or else through a longest one
-        int best = -1, best_len = 0;
-        for (int m0 = 0; m0 < count && best_len < len; m0 += 32) {
-          const int l = m0 + lane < count ? min(p.lengths[first + m0 + lane], len) : 0;
-          const int most = __reduce_max_sync(0xFFFFFFFFu, l);
-          if (most > best_len) {
-            best_len = most;
-            best = m0 + __ffs(__ballot_sync(0xFFFFFFFFu, l == most)) - 1;
-          }
-        }
-        pc.trow = first + max(best, 0);
-        pc.kend = best_len;
-        pc.by_length = 1;
-      }
-      pc.alt = alt;
-      pc.q1 = !shared;
-      pc.nt0 = pc.nt1 = pc.j0 + take;
-      if (!alt && pc.ntok <= tpt) pc.nt1 = 0;
-      pc.lim0 = pc.kend;
-      pc.lim_step = 0;
-      pc.split = 1;
-      pc.orow0 = row0 + static_cast<int64_t>(pc.h) * irows + static_cast<int64_t>(up) * 2 * tpt * p.G +
-                 static_cast<int64_t>(blockIdx.x) * PT_ROWS;
-      pc.orow1 = pc.orow0 + (alt ? count : tpt) * p.G;
-      pc.end = 0;
-      return;
-    }
+    Piece pc;
+    int src = -1;
+    bool shared = false;
     while (true) {
-      unsigned id32 = 0;
-      if (lane == 0) id32 = atomicAdd(p.counter, 1u);
-      const int64_t id = __shfl_sync(0xFFFFFFFFu, id32, 0);
-      int64_t off64;
-      const int src = find(p, id, off64);
-      if (src < 0) return;
-      const int c0 = get(seq.c0, src), n_tok = get(seq.n, src), len = get(seq.len, src), nq = get(seq.nq, src);
-      const int mt = get(seq.mt, src);
-      const int nch = chunk ? (mt + chunk - 1) / chunk : 1;
-      int q, ch = 0;
-      if (nch == 1) {
-        pc.h = static_cast<int>(off64 % p.H);
-        q = nq - 1 - static_cast<int>(off64 / p.H);
+      if constexpr (DEC) {
+        src = pos < end ? find(p, pos) : -1;
+        if (src < 0) break;
+        const int w = item.tile_cost(p), each = static_cast<int>(max(item.unit_cost(p), int64_t{1}));
+        const int64_t off = max(pos - base_t - before_t, int64_t{0});
+        const int64_t u = quotient(off, each);
+        // the place within the unit, and where the range ends in it; tile t begins at w_start + t * w
+        const int at = static_cast<int>(off - u * each);
+        const int stop = static_cast<int>(min(static_cast<int64_t>(each), at + end - pos));
+        pc.j0 = (max(at - p.w_start, 0) + w - 1) / w;
+        pc.nt0 = min((max(stop - p.w_start, 0) + w - 1) / w, item.tiles);
+        const bool any = __shfl_sync(0xFFFFFFFFu, pc.j0 < pc.nt0, src);
+        pos += __shfl_sync(0xFFFFFFFFu, stop - at, src);
+        if (!any) continue;
+        const int h = static_cast<int>(u) / max(item.units, 1), up = static_cast<int>(u) - h * item.units;
+        shared = i0 + src < groups;
+        pc.h = h;
+        pc.tok0 = item.first + up * 2 * tpt;
+        pc.ntok = min(2 * tpt, item.count - up * 2 * tpt);
+        pc.kb = item.start;
+        pc.kend = item.len;
+        pc.trow = item.first;
+        pc.alt = item.alt;
+        pc.q1 = !shared;
+        pc.thin = !shared && p.G <= PT_THIN;
+        pc.nt1 = item.alt || pc.ntok > tpt ? pc.nt0 : 0;
+        pc.lim0 = item.len;
+        pc.lim_step = 0;
+        pc.by_length = shared;
+        pc.split = 1;
+        pc.orow0 = base_r + before_r + static_cast<int64_t>(h) * item.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
+                   static_cast<int64_t>(blockIdx.x) * PT_ROWS;
+        pc.orow1 = pc.orow0 + (item.alt ? item.count : tpt) * p.G;
+        break;
       } else {
-        q = nq - 1 - static_cast<int>(off64 % nq);
-        ch = static_cast<int>(off64 / nq % nch);
-        pc.h = static_cast<int>(off64 / nq / nch);
-      }
-      const int utok = 2 * tpt;
-      pc.tok0 = c0 + q * utok;
-      pc.ntok = min(utok, n_tok - q * utok);
-      const int pos0 = len - n_tok + q * utok;  // position of the first token
-      const int n0 = min(tpt, pc.ntok);
-      const int l0 = p.causal ? pos0 + n0 : len, l1 = pc.ntok > tpt ? (p.causal ? pos0 + pc.ntok : len) : 0;
-      pc.nt0 = (max(l0, 0) + PT_BN - 1) / PT_BN;
-      pc.nt1 = (max(l1, 0) + PT_BN - 1) / PT_BN;
-      pc.j0 = 0;
-      if (nch > 1) {
+        unsigned id = 0;
+        if (lane == 0) id = atomicAdd(p.counter, 1u);
+        __syncwarp();
+        id = __shfl_sync(0xFFFFFFFFu, id, 0);
+        src = find(p, id);
+        if (src < 0) break;
+        const int64_t off = max(static_cast<int64_t>(id) - base_t - before_t, int64_t{0});
+        const int nq = max(item.nq, 1), utok = 2 * tpt;
+        const int nch = chunk ? (item.mt + chunk - 1) / chunk : 1;
+        // whole units: the heads of one place next to each other; cut ones: the places of one chunk
+        const int inner = nch == 1 ? p.H : nq;
+        const int64_t outer = quotient(off, inner);
+        const int in = static_cast<int>(off - outer * inner);
+        int place = static_cast<int>(outer), ch = 0;
+        pc.h = in;
+        if (nch > 1) {
+          place = in;
+          pc.h = static_cast<int>(outer) / nch;
+          ch = static_cast<int>(outer) - pc.h * nch;
+        }
+        const int q = nq - 1 - place;  // later tokens, which see more, first
+        pc.tok0 = item.c0 + q * utok;
+        pc.ntok = min(utok, item.n - q * utok);
+        const int pos0 = item.len - item.n + q * utok;  // position of the first token
+        const int l0 = p.causal ? pos0 + min(tpt, pc.ntok) : item.len;
+        const int l1 = pc.ntok <= tpt ? 0 : p.causal ? pos0 + pc.ntok : item.len;
+        pc.nt0 = (max(l0, 0) + PT_BN - 1) / PT_BN;
+        pc.nt1 = (max(l1, 0) + PT_BN - 1) / PT_BN;
         pc.j0 = ch * chunk;
-        if (max(pc.nt0, pc.nt1) <= pc.j0 && ch > 0) continue;  // nothing to see in this chunk
-        pc.nt0 = min(pc.nt0, pc.j0 + chunk);
-        pc.nt1 = min(pc.nt1, pc.j0 + chunk);
+        const bool none = ch > 0 && max(pc.nt0, pc.nt1) <= pc.j0;  // nothing to see in this chunk
+        if (__shfl_sync(0xFFFFFFFFu, none, src)) continue;
+        if (nch > 1) {
+          pc.nt0 = min(pc.nt0, pc.j0 + chunk);
+          pc.nt1 = min(pc.nt1, pc.j0 + chunk);
+        }
+        pc.kb = 0;
+        pc.kend = item.len;
+        pc.trow = p.table ? i0 + lane : item.c0;
+        pc.alt = pc.q1 = pc.thin = pc.by_length = 0;
+        pc.lim0 = p.causal ? pos0 + 1 : item.len;
+        pc.lim_step = p.causal ? 1 : 0;
+        pc.split = nch > 1;
+        pc.orow0 = static_cast<int64_t>(id) * PT_ROWS;
+        pc.orow1 = pc.orow0 + 128;
+        break;
       }
-      pc.kb = 0;
-      pc.kend = len;
-      pc.trow = p.table ? i0 + src : c0;
-      pc.alt = 0;
-      pc.q1 = 0;
-      pc.by_length = 0;
-      pc.lim0 = p.causal ? pos0 + 1 : len;
-      pc.lim_step = p.causal ? 1 : 0;
-      pc.split = nch > 1;
-      pc.orow0 = id * PT_ROWS;
-      pc.orow1 = pc.orow0 + 128;
-      pc.end = 0;
-      return;
     }
+    if constexpr (DEC) if (shared) {
+      // the prefix is read through the first member that has all of it, or else through a longest one
+      const int first = __shfl_sync(0xFFFFFFFFu, item.first, src), count = __shfl_sync(0xFFFFFFFFu, item.count, src);
+      const int len = __shfl_sync(0xFFFFFFFFu, item.len, src);
+      int best = 0, best_len = 0;
+      for (int m0 = 0; m0 < count && best_len < len; m0 += 32) {
+        const int l = m0 + lane < count ? min(p.lengths[first + m0 + lane], len) : 0;
+        const int most = __reduce_max_sync(0xFFFFFFFFu, l);
+        if (most > best_len) {
+          best_len = most;
+          best = m0 + __ffs(__ballot_sync(0xFFFFFFFFu, l == most)) - 1;
+        }
+      }
+      pc.trow = first + best;
+      pc.kend = pc.lim0 = best_len;
+    }
+    pc.end = src < 0;
+    if (src < 0 ? lane == 0 : lane == src) *to = pc;
+    __syncwarp();
   }
 };
 
@@ -416,11 +455,12 @@ struct TileLoader {
       for (int x = 0; x < D / 64; ++x)
         tma_load_4d(dst + x * (PT_BN * 128) + i * box * 128, map, bar, x * 64, row, pc.h, page);
     }
+    __syncwarp();
   }
 };
 
 // ------------------------------------------------------------------------------------ the kernel
-template <int D, bool BF16>
+template <int D, bool BF16, bool DEC>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_constant__ PagedAttn p) {
   using C = PtCfg<D>;
   constexpr int NK = C::NK, NV = C::NV;
@@ -440,7 +480,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   uint64_t* p_full = p_lo + 2;          // [2] all weights stored
   uint64_t* o_full = p_full + 2;        // [2]
   uint64_t* tile_free = o_full + 2;     // [2]
-  uint64_t* mma_done = tile_free + 2;
+  uint64_t* vote = tile_free + 2;       // [2] thin pieces: the tile's warps have looked at their scores
+  uint64_t* mma_done = vote + 2;
   uint64_t* turn = mma_done + 1;        // [2]
   uint64_t* level = turn + 2;           // [2] warp 1 + x is past its pieces of its own
   Piece* pieces = reinterpret_cast<Piece*>(smem + C::OFF_PIECE);
@@ -471,6 +512,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       mbar_init(p_full + x, 4);
       mbar_init(o_full + x, 1);
       mbar_init(tile_free + x, 4);
+      mbar_init(vote + x, 4);
       mbar_init(turn + x, 1);
       mbar_init(level + x, 1);
     }
@@ -490,62 +532,74 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   }
   // ---------------------------------------------------------------- where this CTA's work begins
   const int tpt = 128 / p.G;
-  const int groups = p.decode && groups_ok(p) ? p.groups : 0;
+  int groups = 0;
+  if constexpr (DEC) groups = groups_ok(p) ? p.groups : 0;
   int64_t pos = 0, pos_end = 0;
-  if (p.decode || p.may_split) {
-    const int n = p.decode ? groups + p.B : p.B;
+  if (DEC || p.may_split) {
+    // `per` items in a row for every thread; all threads take all turns, since a warp that parts here
+    // does not come together again, and runs apart through everything below
+    const int n = DEC ? groups + p.B : p.B;
     const int per = (n + PT_THREADS - 1) / PT_THREADS;
-    const int a = min(n, static_cast<int>(threadIdx.x) * per), z = min(n, a + per);
-    int64_t t = 0, r = 0, tt, tr;
-    for (int i = a; i < z; ++i) {
-      if (p.decode) {
-        const Item it = decode_item(p, groups, tpt, i);
-        t += static_cast<int64_t>(p.H) * it.units * it.tiles;
-        r += static_cast<int64_t>(p.H) * it.rows;
+    const int first = static_cast<int>(threadIdx.x) * per;
+    int64_t c = 0, r = 0, tc, tr;
+    Item it;
+    for (int k = 0; k < per; ++k) {
+      const int i = min(first + k, n - 1);
+      const bool has = first + k < n;
+      if constexpr (DEC) {
+        it = decode_item(p, groups, tpt, i);
+        c += has ? it.cost(p) : 0;
+        r += has ? static_cast<int64_t>(p.H) * it.rows : 0;
       } else {
         const Seq s = prompt_seq(p, 2 * tpt, i);
-        t += static_cast<int64_t>(p.H) * s.nq * s.mt;
-        r += static_cast<int64_t>(p.H) * s.nq;
+        c += has ? static_cast<int64_t>(p.H) * s.nq * s.mt : 0;
+        r += has ? static_cast<int64_t>(p.H) * s.nq : 0;
       }
     }
-    block_scan2(t, r, scan, tt, tr);
-    if (p.decode) {
-      const int64_t ctas = min(tt, static_cast<int64_t>(p.num_ctas));  // a tile at least for each
+    block_scan2(c, r, scan, tc, tr);
+    if constexpr (DEC) {
+      const int64_t ctas = decode_ctas(p, tc);
       if (blockIdx.x < ctas) {
-        pos = quotient(tt * blockIdx.x, ctas);
-        pos_end = quotient(tt * (blockIdx.x + 1), ctas);
+        pos = quotient(tc * blockIdx.x, ctas);
+        pos_end = quotient(tc * (blockIdx.x + 1), ctas);
       }
-      if (threadIdx.x == 0 && blockIdx.x == 0) p.rec_tile[n] = tt;
-      for (int i = a; i < z; ++i) {
-        const Item it = decode_item(p, groups, tpt, i);
-        const int64_t c = static_cast<int64_t>(p.H) * it.units * it.tiles;
-        if (t <= pos && pos < t + c) {
+      for (int k = 0; k < per; ++k) {
+        const int i = min(first + k, n - 1);
+        const bool has = first + k < n;
+        if (per > 1) it = decode_item(p, groups, tpt, i);
+        const int64_t ci = has ? it.cost(p) : 0;
+        if (c <= pos && pos < c + ci) {
           start[0] = i;
-          start[1] = t;
+          start[1] = c;
           start[2] = r;
         }
-        if (blockIdx.x == 0) {
-          p.rec_tile[i] = t;
+        if (blockIdx.x == 0 && has) {
+          p.rec_cost[i] = c;
           p.rec_row[i] = r;
         }
-        t += c;
+        c += ci;
         r += static_cast<int64_t>(p.H) * it.rows;
       }
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_cost[n] = tc;
     } else {
-      const int chunk = chunk_tiles(p, tr, tt);
+      const int chunk = chunk_tiles(p, tr, tc);
       if (threadIdx.x == 0) start[3] = chunk;
       if (blockIdx.x == 0 && chunk) {
         // the sequences' first pieces, for the joining kernel
-        int64_t c = 0, zero = 0, tc, tz;
-        for (int i = a; i < z; ++i) c += prompt_pieces(p, prompt_seq(p, 2 * tpt, i), chunk);
+        int64_t zero = 0, tz;
+        c = 0;
+        for (int k = 0; k < per; ++k)
+          c += first + k < n ? prompt_pieces(p, prompt_seq(p, 2 * tpt, min(first + k, n - 1)), chunk) : 0;
         block_scan2(c, zero, scan, tc, tz);
-        for (int i = a; i < z; ++i) {
-          p.rec_tile[i] = c;
-          c += prompt_pieces(p, prompt_seq(p, 2 * tpt, i), chunk);
+        for (int k = 0; k < per; ++k) {
+          const Seq s = prompt_seq(p, 2 * tpt, min(first + k, n - 1));
+          if (first + k < n) p.rec_cost[first + k] = c;
+          c += prompt_pieces(p, s, chunk);
         }
       }
-      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_tile[n] = chunk;
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_cost[n] = chunk;
     }
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
@@ -568,21 +622,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
 
   if (warp == 0) {
     // ================================================================ pieces, Q and K
-    Sched sc;
+    Sched<DEC> sc;
     sc.groups = groups;
     sc.tpt = tpt;
     sc.pos = pos;
     sc.end = pos_end;
-    sc.n = p.decode ? groups + p.B : p.B;
-    sc.chunk = 0;
+    sc.n = DEC ? groups + p.B : p.B;
+    sc.chunk = !DEC && p.may_split ? static_cast<int>(start[3]) : 0;
     sc.i0 = 0;
     sc.base_t = sc.base_r = 0;
-    if (p.decode && pos < pos_end) {
+    if (DEC && pos < pos_end) {
       sc.i0 = static_cast<int>(start[0]);
       sc.base_t = start[1];
       sc.base_r = start[2];
     }
-    if (!p.decode && p.may_split) sc.chunk = static_cast<int>(start[3]);
     sc.loaded = false;
     int published = 0;
     TileLoader ld;
@@ -594,14 +647,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     while (true) {
       if (want) {
         // the next piece, while this one's first tiles are on their way
-        sc.next(p, nx);
         const int s = published % PT_RING;
         ok = pt_wait(w_empty + s, ((published / PT_RING) & 1) ^ 1, ab, ERR_TIMEOUT_PRODUCER);
         if (!ok) break;
-        if (lane == 0) {
-          pieces[s] = nx;
-          mbar_arrive(w_full + s);
-        }
+        sc.next(p, pieces + s);
+        if (lane == 0) mbar_arrive(w_full + s);
+        nx = pieces[s];
         __syncwarp();
         ++published;
         if (p.table && !nx.end) {
@@ -656,7 +707,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       for (int f = (qpos > 2 ? qpos - 2 : 0); f < qpos && drained; ++f)
         drained = mbar_drain(q_full + (f & 1), (f >> 1) & 1, p.err);
       // the last CTA leaves the counter as it found it
-      if (!p.decode && atomicAdd(p.counter + 1, 1u) == gridDim.x - 1) {
+      if (!DEC && atomicAdd(p.counter + 1, 1u) == gridDim.x - 1) {
         p.counter[0] = 0;
         p.counter[1] = 0;
       }
@@ -697,10 +748,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     const int x = warp - 1;
     constexpr uint32_t IDESC_S = umma_idesc_f16(128, PT_BN, BF16, false);
     constexpr uint32_t IDESC_PV = umma_idesc_f16(128, D, BF16, true);
+    constexpr uint32_t IDESC_T = umma_idesc_f16(128, 16, BF16, false);  // thin: keys by rows
+    constexpr uint32_t IDESC_TV = IDESC_T | (1u << 15);  // thin: channels (V transposed: MN-major A) by rows
     const uint32_t tS = tmem + 128 * x;
     const uint32_t tO = tmem + 256 + D * x;
     const uint64_t qdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_Q), 16, 1024);
     const uint64_t kdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_K), 16, 1024);
+    const uint64_t pdesc = umma_desc_sw128(smem_u32(smem + C::OFF_P + x * C::PBYTES), 16, 1024);
     const uint64_t vdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_V), PT_BN * 128, 1024);
     int fpos = 0, qpos = 0;  // fills of the K and V rings, of the query slots
     uint32_t free_par = 1, p_par = 0, nbatch = 0, nlevel = 0;
@@ -742,9 +796,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint64_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-          umma_ss(tS, qdesc + off, kb + off, IDESC_S, kk > 0);
+          if (DEC && pc.thin) umma_ss(tS, kb + off, qdesc + off, IDESC_T, kk > 0);
+          else umma_ss(tS, qdesc + off, kb + off, IDESC_S, kk > 0);
         }
         umma_commit(s_full + x);
+      };
+      // O^T (+)= V^T P^T. With 64 channels the rows from 64 on are of whatever lies a tile behind, and not read.
+      auto issue_thin = [&](int f) {
+        const uint64_t vb = vdesc0 + static_cast<uint64_t>((f % NV) * (C::KVBYTES >> 4));
+#pragma unroll
+        for (int kk = 0; kk < PT_BN / 16; ++kk)
+          umma_ss(tO, vb + static_cast<uint64_t>((kk * 2048) >> 4),
+                  pdesc + static_cast<uint64_t>(((kk >> 2) * (16 * 128) + (kk & 3) * 32) >> 4), IDESC_TV,
+                  (o_init || kk > 0) ? 1u : 0u);
+        o_init = true;
       };
       auto issue_PV = [&](int f, int half) {
         const uint64_t vb = vdesc0 + static_cast<uint64_t>((f % NV) * (C::KVBYTES >> 4));
@@ -759,6 +824,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         if (!pt_wait(p_lo + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
         tc_fence_after();
         if (!ensure_free()) return false;
+        if (DEC && pc.thin) {
+          if (!pt_wait(p_full + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
+          p_par ^= 1;
+          tc_fence_after();
+          issue_thin(f);
+          return true;
+        }
         issue_PV(f, 0);
         if (!pt_wait(p_full + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
         p_par ^= 1;
@@ -776,74 +848,63 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         tc_fence_after();
         return true;
       };
-      if (pc.alt) {
+      if (DEC && pc.alt) {
         apart = true;
-        const int n = je - pc.j0;
-        auto scores = [&](int f) -> bool {
-          if (!wait_k(f)) return false;
+        const int n = je - pc.j0, first = (fpos ^ x) & 1;
+        if (first >= n) free_q();
+        for (int i = first; first < n; i += 2) {
+          if (i > first) {
+            const int f = fpos + i - 2;
+            if (i >= n) free_q();
+            ok = wait_v(f) && weigh(f);
+            if (!ok) break;
+            umma_commit(v_empty + f % NV);
+            umma_commit(v_empty + f % NV);
+            if (i >= n) break;
+          }
+          const int f = fpos + i;
+          ok = wait_k(f);
+          if (!ok) break;
           issue_S(f);
           umma_commit(k_empty + f % NK);
           umma_commit(k_empty + f % NK);
-          return true;
-        };
-        const int first = (fpos ^ x) & 1;
-        if (first < n) ok = scores(fpos + first);
-        else free_q();
-        for (int i = first; ok && i < n; i += 2) {
-          if (i + 2 >= n) free_q();
-          ok = wait_v(fpos + i) && weigh(fpos + i);
-          if (!ok) break;
-          umma_commit(v_empty + (fpos + i) % NV);
-          umma_commit(v_empty + (fpos + i) % NV);
-          if (i + 2 < n) ok = scores(fpos + i + 2);
         }
         if (!ok) break;
         fpos += n;
       } else {
         auto uses = [&](int j) { return mine && j < (x ? pc.nt1 : pc.nt0); };
-        if (apart) {
+        if (DEC && apart) {
           if (lane == 0) mbar_arrive(level + x);
           ok = pt_wait(level + (1 - x), nlevel & 1, ab, ERR_TIMEOUT_MMA);
           if (!ok) break;
           ++nlevel;
           apart = false;
         }
-        int kpos = fpos, vpos = fpos;
-        if (pc.j0 < je) {
-          ok = wait_k(kpos) && my_turn();
-          if (!ok) break;
-          if (uses(pc.j0)) issue_S(kpos);
-          end_turn();
-          umma_commit(k_empty + kpos % NK);
-          ++kpos;
-        }
-        for (int j = pc.j0; j < je; ++j) {
-          const bool more = j + 1 < je;
-          ok = wait_v(vpos);
+        if (pc.j0 >= je) free_q();
+        // batch j: P V of tile j - 1, Q K^T of tile j
+        for (int j = pc.j0; pc.j0 < je && j <= je; ++j, ++fpos) {
+          const bool before = j > pc.j0, more = j < je;
+          if (before) ok = wait_v(fpos - 1);
+          else ok = wait_k(fpos);
           if (!ok) break;
           if (!more) free_q();
           ok = my_turn();
           if (!ok) break;
-          if (uses(j)) {
-            ok = weigh(vpos);
+          if (before && uses(j - 1)) {
+            ok = weigh(fpos - 1);
             if (!ok) break;
           }
           if (more) {
-            ok = wait_k(kpos);
+            if (before) ok = wait_k(fpos);
             if (!ok) break;
-            if (uses(j + 1)) issue_S(kpos);
+            if (uses(j)) issue_S(fpos);
           }
           end_turn();
-          umma_commit(v_empty + vpos % NV);
-          ++vpos;
-          if (more) {
-            umma_commit(k_empty + kpos % NK);
-            ++kpos;
-          }
+          if (before) umma_commit(v_empty + (fpos - 1) % NV);
+          if (more) umma_commit(k_empty + fpos % NK);
         }
         if (!ok) break;
-        if (pc.j0 >= je) free_q();
-        fpos = vpos;
+        if (pc.j0 < je) --fpos;
       }
       // The products' warp waits for the tile once a piece and always announces O; the epilogue always
       // waits for that before it gives the tile back, so the parities cannot run apart.
@@ -866,10 +927,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     const uint32_t tO = tmem + lane_base + 256 + D * x;
     const float sl2 = p.scale_log2;
     int vpos = 0;
-    uint32_t s_par = 0, o_par = 0;
+    uint32_t s_par = 0, o_par = 0, votes = 0;
     Piece pc;
     bool ok = true;
     while (ok && take(pc, ERR_TIMEOUT_SOFTMAX)) {
+      if (!DEC) pc.alt = pc.by_length = 0;
       const int je = pc.jend(), step = pc.alt ? 2 : 1;
       const bool valid = x == 0 || pc.alt || pc.ntok > tpt;
       const int ntok = pc.alt ? pc.ntok : max(0, min(tpt, pc.ntok - x * tpt));
@@ -883,6 +945,163 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         lim_row = pc.lim0 + (tok - pc.tok0) * pc.lim_step;
         if (pc.by_length) lim_row = min(lim_row, p.lengths[tok]);
         lim_row -= pc.kb;
+      }
+      if (DEC && pc.thin) {
+        // ------------ transposed: a key per thread, a query row per column. All of the tile's warps hold the
+        // same references; a warp that finds a score more than 2^8 above one says so in the vote that
+        // every key tile has, and O^T (a channel per thread) moves to the new references before the next product.
+        float* vmax = reinterpret_cast<float*>(smem + C::OFF_VOTE) + x * 2 * 4 * PT_THIN;
+        int* vflag = reinterpret_cast<int*>(smem + C::OFF_VOTE + 2 * 2 * 4 * PT_THIN * 4) + x * 2 * 4;
+        uint8_t* ps = smem + C::OFF_P + x * C::PBYTES + (r >> 6) * (16 * 128) + (r & 7) * 2;
+        float m[PT_THIN], ls[PT_THIN];
+#pragma unroll
+        for (int g = 0; g < PT_THIN; ++g) {
+          m[g] = -INFINITY;
+          ls[g] = 0.f;
+        }
+        bool has = false;
+        auto reduce = [&](float (&v)[PT_THIN], bool sum) -> float {  // lane g: column g's maximum or sum over the warp
+          float mine = 0.f;
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g) {
+            if (g < p.G) {
+#pragma unroll
+              for (int o = 16; o; o >>= 1) {
+                const float u = __shfl_xor_sync(0xFFFFFFFFu, v[g], o);
+                v[g] = sum ? v[g] + u : fmaxf(v[g], u);
+              }
+            }
+            if (lane == g) mine = v[g];
+          }
+          return mine;
+        };
+        auto cast_vote = [&](float mine, bool put, bool flag) -> bool {
+          const int at = (votes & 1) * 4 + wq;
+          if (put && lane < PT_THIN) vmax[at * PT_THIN + lane] = mine;
+          if (lane == 0) vflag[at] = flag;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(vote + x);
+          const bool all = pt_wait(vote + x, votes & 1, ab, ERR_TIMEOUT_SOFTMAX);
+          ++votes;
+          return all;
+        };
+        for (int j = pc.j0 + ((vpos ^ x) & 1); j < je; j += 2) {
+          const int f = vpos + (j - pc.j0);
+          const int have = pc.kend - pc.kb - j * PT_BN;
+          if (!pt_wait(s_full + x, s_par, ab, ERR_TIMEOUT_SOFTMAX)) { ok = false; break; }
+          s_par ^= 1;
+          tc_fence_after();
+          uint32_t sc[PT_THIN];
+          tmem_ld8(tS, sc);
+          float s[PT_THIN];
+          bool over = false;
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g) {
+            s[g] = g < p.G && r < have ? __uint_as_float(sc[g]) * sl2 : -INFINITY;
+            over |= s[g] > m[g] + 8.f;
+          }
+          over = __any_sync(0xFFFFFFFFu, over);
+          float mine = 0.f;
+          if (over) {
+            float t[PT_THIN];
+#pragma unroll
+            for (int g = 0; g < PT_THIN; ++g) t[g] = s[g];
+            mine = reduce(t, false);
+          }
+          ok = cast_vote(mine, over, over);
+          if (!ok) break;
+          const int seen = (votes & 1) ^ 1;
+          const int4 fl = *reinterpret_cast<const int4*>(vflag + seen * 4);
+          if (fl.x | fl.y | fl.z | fl.w) {
+            float mn[PT_THIN];
+#pragma unroll
+            for (int g = 0; g < PT_THIN; ++g) mn[g] = m[g];
+#pragma unroll 1
+            for (int w = 0; w < 4; ++w) {
+              if (!vflag[seen * 4 + w]) continue;
+              const float4* v = reinterpret_cast<const float4*>(vmax + (seen * 4 + w) * PT_THIN);
+#pragma unroll
+              for (int q = 0; q < PT_THIN / 4; ++q) {
+                const float4 u = v[q];
+                mn[4 * q] = fmaxf(mn[4 * q], u.x);
+                mn[4 * q + 1] = fmaxf(mn[4 * q + 1], u.y);
+                mn[4 * q + 2] = fmaxf(mn[4 * q + 2], u.z);
+                mn[4 * q + 3] = fmaxf(mn[4 * q + 3], u.w);
+              }
+            }
+            uint32_t o[PT_THIN];
+            if (has) tmem_ld8(tO, o);
+#pragma unroll
+            for (int g = 0; g < PT_THIN; ++g) {
+              const float fac = m[g] == -INFINITY ? 0.f : ex2(m[g] - mn[g]);
+              m[g] = mn[g];
+              ls[g] = fac == 0.f ? 0.f : ls[g] * fac;
+              o[g] = !has || fac == 0.f ? 0u : __float_as_uint(__uint_as_float(o[g]) * fac);
+            }
+            if (has) {
+              tmem_st8(tO, o);
+              tmem_st_wait();
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g) {
+            const float w = g < p.G && r < have ? ex2(s[g] - m[g]) : 0.f;
+            ls[g] += w;
+            const int at = g * 128 + ((((r & 63) >> 3) ^ g) << 4);
+            if (BF16) *reinterpret_cast<__nv_bfloat16*>(ps + at) = __float2bfloat16_rn(w);
+            else *reinterpret_cast<__half*>(ps + at) = __float2half_rn(w);
+          }
+          if (have < PT_BN) {
+            // V rows past the sequence hold anything: 0 in their place, before the products read them. (With this
+            // tile's scores there, the slot's earlier fills have been read, so the wait is for this one.)
+            if (!pt_wait(v_full + f % NV, (f / NV) & 1, ab, ERR_TIMEOUT_SOFTMAX)) { ok = false; break; }
+            if (r >= have) {
+              uint8_t* row = smem + C::OFF_V + (f % NV) * C::KVBYTES + r * 128;
+#pragma unroll 1
+              for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  *reinterpret_cast<uint4*>(row + c * (PT_BN * 128) + e * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_async_smem();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(p_lo + x);
+            mbar_arrive(p_full + x);
+          }
+          has = true;
+        }
+        if (!ok) break;
+        vpos += je - pc.j0;
+        // the sums over the tile's keys: the warp's, then the four warps' through the votes' memory
+        if (!cast_vote(reduce(ls, true), true, false)) break;
+        const int64_t row0 = x ? pc.orow1 : pc.orow0;
+        if (wq == 0) {
+          float my_m = 0.f;
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g) my_m = lane == g ? m[g] : my_m;
+          if (lane < p.G) {
+            const float* v = vmax + ((votes & 1) ^ 1) * 4 * PT_THIN + lane;
+            const float sum = (v[0] + v[PT_THIN]) + (v[2 * PT_THIN] + v[3 * PT_THIN]);
+            p.part_s[row0 + lane] = make_float2(my_m, has ? sum : 0.f);
+          }
+        }
+        if (!pt_wait(o_full + x, o_par, ab, ERR_TIMEOUT_EPILOGUE)) break;
+        o_par ^= 1;
+        tc_fence_after();
+        if (has && wq * 32 < D) {
+          uint32_t o[PT_THIN];
+          tmem_ld8(tO, o);
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g)
+            if (g < p.G) p.part_o[(row0 + g) * D + r] = __uint_as_float(o[g]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tile_free + x);
+        continue;
       }
       // rows that do not exist get a reference no score exceeds, and weigh nothing
       float m_used = live ? -INFINITY : 1e30f, l = 0.f;
@@ -961,32 +1180,48 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         };
         int stop = 0;          // first 32-column chunk that the stream did not finish
         bool lo_sent = false;  // weights of keys 0..63 are final and announced
-        // two halves in a loop: a launch's first pass through code waits for its instructions
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t sa[32], sb[32], w[16];
-          tmem_ld32_async(tS + half * 64, sa);
-          tmem_ld32_async(tS + half * 64 + 32, sb);
+        {
+          uint32_t sa[32], sb[32];
+          tmem_ld32_async(tS, sa);
           tmem_ld32_wait(sa);
-          tmem_ld32_wait(sb);
+          tmem_ld32_async(tS + 32, sb);
           if (m_used == -INFINITY) {
             const float m0 = chunk_max(sa);
             m_used = m0 == -INFINITY ? 0.f : m0;
           }
-          if (__any_sync(0xFFFFFFFFu, fmaxf(chunk_max(sa), chunk_max(sb)) > m_used + 8.f)) break;
-          if (half) {
-            // nothing stored will be rescaled: P V of keys 0..63 may begin
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_lo + x);
-            lo_sent = true;
+          const float nb = -m_used, most = m_used + 8.f;
+          auto one = [&](int c, uint32_t(&cur)[32], uint32_t(&nxt)[32]) -> bool {
+            if (__any_sync(0xFFFFFFFFu, chunk_max(cur) > most)) {
+              tmem_ld32_wait(nxt);
+              stop = c;
+              return false;
+            }
+            uint32_t w[16];
+            weights(cur, nb, w);
+            tmem_st16(tS + c * 16, w);
+            tmem_ld32_wait(nxt);
+            tmem_ld32_async(tS + (c + 2) * 32, cur);
+            return true;
+          };
+          if (one(0, sa, sb) && one(1, sb, sa)) {
+            tmem_ld32_wait(sb);
+            if (__any_sync(0xFFFFFFFFu, fmaxf(chunk_max(sa), chunk_max(sb)) > most)) {
+              stop = 2;
+            } else {
+              // nothing stored will be rescaled: P V of keys 0..63 may begin
+              tmem_st_wait();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_lo + x);
+              lo_sent = true;
+              uint32_t w[16];
+              weights(sa, nb, w);
+              tmem_st16(tS + 32, w);
+              weights(sb, nb, w);
+              tmem_st16(tS + 48, w);
+              stop = 4;
+            }
           }
-          weights(sa, -m_used, w);
-          tmem_st16(tS + half * 32, w);
-          weights(sb, -m_used, w);
-          tmem_st16(tS + half * 32 + 16, w);
-          stop += 2;
         }
         if (stop < 4) {
           // some row outgrew its reference: the maximum of what is left, everything so far rescaled, by whole
@@ -1150,8 +1385,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
 }
 
 // ------------------------------------------------------------------------------------ joining
-// One warp per output row: the maxima and sums of all of its pieces, then their weighted sum. D / 32 elements
-// a lane. Pieces that hold nothing for the row (sum 0) are left out.
+// Prompts, whose many rows have a few pieces each: one warp per output row, the maxima and sums of its pieces, then
+// their weighted sum, D / 32 elements a lane. Pieces that hold nothing for the row (sum 0) are left out.
 template <int D, typename T> struct Joiner {
   float acc[D / 32], m, l;
   __device__ __forceinline__ Joiner() : m(-INFINITY), l(0.f) {
@@ -1180,17 +1415,26 @@ template <int D, typename T> struct Joiner {
 #pragma unroll
       for (int e = 0; e < D / 32; ++e) acc[e] *= f;
       const int most = min(32, n - i0);
-#pragma unroll 4
-      for (int i = 0; i < most; ++i) {
-        const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
-        if (!(any >> i & 1)) continue;
-        const float* src = p.part_o + row(i0 + i) * D + lane * (D / 32);
-        if constexpr (D == 128) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] += wi * v.x; acc[1] += wi * v.y; acc[2] += wi * v.z; acc[3] += wi * v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] += wi * v.x; acc[1] += wi * v.y;
+      for (int i = 0; i < most; i += 8) {
+        // eight pieces' rows on their way at once; a piece without a sum may hold anything
+        float v[8][D / 32];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bool live = i + k < most && (any >> (i + k) & 1);
+          const float* src = p.part_o + row(i0 + (live ? i + k : 0)) * D + lane * (D / 32);
+          if constexpr (D == 128) {
+            const float4 f4 = live ? __ldcg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[k][0] = f4.x; v[k][1] = f4.y; v[k][2] = f4.z; v[k][3] = f4.w;
+          } else {
+            const float2 f2 = live ? __ldcg(reinterpret_cast<const float2*>(src)) : make_float2(0.f, 0.f);
+            v[k][0] = f2.x; v[k][1] = f2.y;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float wk = __shfl_sync(0xFFFFFFFFu, w, (i + k) & 31);
+#pragma unroll
+          for (int e = 0; e < D / 32; ++e) acc[e] += (i + k < most ? wk : 0.f) * v[k][e];
         }
       }
     }
@@ -1206,58 +1450,132 @@ template <int D, typename T> struct Joiner {
 };
 
 template <int D, typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const __grid_constant__ PagedAttn p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+__global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant__ PagedAttn p) {
   const int tpt = 128 / p.G, Hq = p.H * p.G;
-  const int groups = p.decode && groups_ok(p) ? p.groups : 0;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= static_cast<int64_t>(p.T) * Hq) return;
   const int t = static_cast<int>(row / Hq), hq = static_cast<int>(row % Hq), h = hq / p.G, rg = hq % p.G;
-  T* dst = static_cast<T*>(p.out) + t * p.o_t + hq * p.o_h;
-  Joiner<D, T> jn;
-  if (p.decode) {
-    const int b = t;
-    const int64_t total = p.rec_tile[groups + p.B];
-    const int64_t ctas = min(total, static_cast<int64_t>(p.num_ctas));
-    auto unit = [&](int i, const Item& it, int up, int in_unit) {
-      if (!it.tiles) return;
-      const int64_t u0 = p.rec_tile[i] + (static_cast<int64_t>(h) * it.units + up) * it.tiles;
-      const int c0 = static_cast<int>(quotient((u0 + 1) * ctas - 1, total));
-      const int c1 = static_cast<int>(quotient((u0 + it.tiles) * ctas - 1, total));
-      const int64_t base = p.rec_row[i] + static_cast<int64_t>(h) * it.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
-                           static_cast<int64_t>(c0) * PT_ROWS + in_unit;
-      const int n = c1 - c0 + 1, second = it.count * p.G;
-      jn.add(p, it.alt ? 2 * n : n, [&](int k) {
-        return it.alt ? base + static_cast<int64_t>(k >> 1) * PT_ROWS + (k & 1) * second
-                      : base + static_cast<int64_t>(k) * PT_ROWS;
-      });
-    };
-    const int g = group_of(p, groups, b);
-    if (g >= 0) {
-      const Item it = decode_item(p, groups, tpt, g);
-      const int mi = b - it.first, up = mi / (2 * tpt);
-      unit(g, it, up, (mi - up * 2 * tpt) * p.G + rg);
-    }
-    unit(groups + b, decode_item(p, groups, tpt, groups + b), 0, rg);
-    jn.store(dst);
-    return;
-  }
-  const int chunk = static_cast<int>(p.rec_tile[p.B]);
-  if (!chunk) return;
+  // what goes by the inputs alone comes before the wait for the partial results
   const int b = paged_sequence(p.cu, p.B, t);
   if (b < 0) return;
   const Seq s = prompt_seq(p, 2 * tpt, b);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int chunk = static_cast<int>(p.rec_cost[p.B]);
+  if (!chunk) return;
   const int nch = (s.mt + chunk - 1) / chunk;
   if (nch == 1 || t < s.c0 || t >= s.c0 + s.n) return;
   const int q = (t - s.c0) / (2 * tpt), in = t - s.c0 - q * 2 * tpt, x = in / tpt;
   const int last = min(2 * tpt, s.n - q * 2 * tpt);  // tokens of the unit
   const int lim = p.causal ? max(0, s.len - s.n + q * 2 * tpt + last) : s.len;
   const int n = max(1, ((lim + PT_BN - 1) / PT_BN + chunk - 1) / chunk);
-  const int64_t id0 = p.rec_tile[b] + static_cast<int64_t>(h) * nch * s.nq + (s.nq - 1 - q);
+  const int64_t id0 = p.rec_cost[b] + static_cast<int64_t>(h) * nch * s.nq + (s.nq - 1 - q);
   const int64_t base = id0 * PT_ROWS + x * 128 + (in - x * tpt) * p.G + rg;
   const int64_t stride = static_cast<int64_t>(s.nq) * PT_ROWS;
+  Joiner<D, T> jn;
   jn.add(p, n, [&](int k) { return base + k * stride; });
-  jn.store(dst);
+  jn.store(static_cast<T*>(p.out) + t * p.o_t + hq * p.o_h);
+}
+
+// Decoding, whose few rows have many pieces each (two for every CTA that had a part of the unit, of the prefix and
+// of the own rows): a block per row, every fourth piece to a warp, eight of them on their way at once and
+// before the maxima are known.
+template <int D, typename T>
+__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ PagedAttn p) {
+  constexpr int E = D / 32;
+  __shared__ float acc_s[4][D], l_s[4];
+  const int tpt = 128 / p.G, Hq = p.H * p.G, lane = lane_id(), warp = threadIdx.x >> 5;
+  const int b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / p.G, rg = hq % p.G;
+  const int groups = groups_ok(p) ? p.groups : 0;
+  const int g = group_of(p, groups, b);
+  const Item own = decode_item(p, groups, tpt, groups + b);
+  Item shared = own;
+  if (g >= 0) shared = decode_item(p, groups, tpt, g);
+  // everything above goes by the inputs alone
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t total = p.rec_cost[groups + p.B], ctas = decode_ctas(p, total);
+  // pieces of a unit: one in every CTA from that of its first key tile to that of its last
+  auto unit = [&](int i, const Item& it, int up, int in_unit, int& n, int64_t& base) {
+    n = 0;
+    base = 0;
+    if (!it.tiles) return;
+    const int64_t u0 = p.rec_cost[i] + (static_cast<int64_t>(h) * it.units + up) * it.unit_cost(p) + p.w_start;
+    const int c0 = static_cast<int>(quotient((u0 + 1) * ctas - 1, total));
+    const int c1 = static_cast<int>(quotient((u0 + static_cast<int64_t>(it.tiles - 1) * it.tile_cost(p) + 1) * ctas - 1, total));
+    n = (c1 - c0 + 1) * (it.alt ? 2 : 1);
+    base = p.rec_row[i] + static_cast<int64_t>(h) * it.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
+           static_cast<int64_t>(c0) * PT_ROWS + in_unit;
+  };
+  int n0 = 0, n1;
+  int64_t base0 = 0, base1;
+  if (g >= 0) {
+    const int mi = b - shared.first, up = mi / (2 * tpt);
+    unit(g, shared, up, (mi - up * 2 * tpt) * p.G + rg, n0, base0);
+  }
+  unit(groups + b, own, 0, rg, n1, base1);
+  const int n = n0 + n1;
+  auto row = [&](int i) -> int64_t {
+    const bool first = i < n0;
+    const int k = first ? i : i - n0;
+    const int64_t base = first ? base0 : base1;
+    if (!(first ? shared.alt : 1)) return base + static_cast<int64_t>(k) * PT_ROWS;
+    return base + static_cast<int64_t>(k >> 1) * PT_ROWS + (k & 1) * (first ? shared.count : 1) * p.G;
+  };
+  float acc[E], l = 0.f, m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float v[8][E];
+    float2 st[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = i0 + warp + 4 * k;
+      st[k] = make_float2(-INFINITY, 0.f);
+      if constexpr (D == 128) {
+        float4 f4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i < n) {
+          const int64_t at = row(i);
+          st[k] = __ldcg(p.part_s + at);
+          f4 = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + lane);
+        }
+        v[k][0] = f4.x; v[k][1] = f4.y; v[k][2] = f4.z; v[k][3] = f4.w;
+      } else {
+        float2 f2 = make_float2(0.f, 0.f);
+        if (i < n) {
+          const int64_t at = row(i);
+          st[k] = __ldcg(p.part_s + at);
+          f2 = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * D) + lane);
+        }
+        v[k][0] = f2.x; v[k][1] = f2.y;
+      }
+    }
+    if (i0 == 0) {
+      // the maximum over all pieces that hold something for the row
+      for (int i = lane; i < n; i += 32) {
+        const float2 s = __ldcg(p.part_s + row(i));
+        if (s.y != 0.f) m = fmaxf(m, s.x);
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool has = st[k].y != 0.f;  // NaN too
+      const float w = has ? ex2(st[k].x - m) : 0.f;
+      l += has ? w * st[k].y : 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += has ? w * v[k][e] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc_s[warp][lane * E + e] = acc[e];
+  if (lane == 0) l_s[warp] = l;
+  __syncthreads();
+  if (threadIdx.x < D) {
+    const int d = threadIdx.x;
+    const float sum = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
+    const float o = (acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d]);
+    static_cast<T*>(p.out)[b * p.o_t + hq * p.o_h + d] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
+  }
 }
 
 // ------------------------------------------------------------------------------------ launch
@@ -1277,7 +1595,9 @@ Sizes sizes_of(int64_t T, int64_t B, int64_t H, int64_t G, int64_t groups, bool 
     // whole units where the tokens alone make two for every SM
     s.split = H * (T / utok) < 2 * static_cast<int64_t>(sms);
     const int64_t units = H * ((T + utok - 1) / utok + B);
-    const int64_t pieces = PT_FILL * static_cast<int64_t>(sms) + (units < 2 * sms ? units : 2 * sms);
+    // of fewer than 2 * sms units; the chunks in the mean, and one more of each unit
+    const int64_t most = std::min<int64_t>(units, 2 * sms);
+    const int64_t pieces = std::min(PT_CHUNKS * most, PT_FILL * static_cast<int64_t>(sms)) + most;
     s.rows = s.split ? pieces * PT_ROWS : 0;
     s.recs = s.split ? B + 1 : 0;
   }
@@ -1291,14 +1611,14 @@ size_t paged_attn_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t 
   return 256 + 2 * up256(s.recs * 8) + up256(s.rows * 8) + up256(s.rows * D * 4);
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool DEC>
 static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream_t st) {
   using C = PtCfg<D>;
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Sizes s = sizes_of(p.T, p.B, p.H, p.G, p.groups, p.decode, sms);
   p.counter = reinterpret_cast<unsigned*>(ws);
   ws += 256;
-  p.rec_tile = reinterpret_cast<int64_t*>(ws);
+  p.rec_cost = reinterpret_cast<int64_t*>(ws);
   ws += up256(s.recs * 8);
   p.rec_row = reinterpret_cast<int64_t*>(ws);
   ws += up256(s.recs * 8);
@@ -1307,7 +1627,11 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   p.part_o = reinterpret_cast<float*>(ws);
   p.may_split = s.split;
   p.num_ctas = sms;
-  auto kfn = paged_attn_kernel<D, BF16>;
+  // In sixteenths of a microsecond on a full GPU, as measured: ...
+  p.w_start = 32;
+  p.w_pair = D == 128 ? 32 : 24;
+  p.w_alt = D == 128 ? 24 : 12;
+  auto kfn = paged_attn_kernel<D, BF16, DEC>;
   // the limit is raised once per device: asking for it costs a microsecond
   static std::atomic<bool> raised[64];
   int dev = 0;
@@ -1321,7 +1645,8 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   e = cudaGetLastError();
   if (e != cudaSuccess || !s.split) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.T) * p.H * p.G + 3) / 4));
+  const int64_t rows = static_cast<int64_t>(p.T) * p.H * p.G;
+  cfg.gridDim = dim3(static_cast<unsigned>(p.decode ? rows : (rows + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute at;
@@ -1329,13 +1654,16 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, T>, p);
+  if constexpr (DEC) return cudaLaunchKernelEx(&cfg, decode_join_kernel<D, T>, p);
+  else return cudaLaunchKernelEx(&cfg, prompt_join_kernel<D, T>, p);
 }
 
 cudaError_t launch_paged_attn(int dtype, int head_dim, PagedAttn& p, uint8_t* ws, int sms, cudaStream_t st) {
-  if (head_dim == 128)
-    return dtype == BF16 ? launch_paged_t<128, true>(p, ws, sms, st) : launch_paged_t<128, false>(p, ws, sms, st);
-  return dtype == BF16 ? launch_paged_t<64, true>(p, ws, sms, st) : launch_paged_t<64, false>(p, ws, sms, st);
+  const bool b = dtype == BF16;
+  if (head_dim == 128 && p.decode) return b ? launch_paged_t<128, true, true>(p, ws, sms, st) : launch_paged_t<128, false, true>(p, ws, sms, st);
+  if (head_dim == 128) return b ? launch_paged_t<128, true, false>(p, ws, sms, st) : launch_paged_t<128, false, false>(p, ws, sms, st);
+  if (p.decode) return b ? launch_paged_t<64, true, true>(p, ws, sms, st) : launch_paged_t<64, false, true>(p, ws, sms, st);
+  return b ? launch_paged_t<64, true, false>(p, ws, sms, st) : launch_paged_t<64, false, false>(p, ws, sms, st);
 }
 
 }  // namespace dab
