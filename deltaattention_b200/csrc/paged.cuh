@@ -27,6 +27,13 @@ struct PagedAppend {
   int T, B, H, Hq, max_pages, num_pages, ps_shift, table_rows;
 };
 
+// How the CTAs of a decode step are shared between the prefixes and the sequences' own rows: CTAs and first CTA of
+// each, and what each costs.
+struct Ctas {
+  int n[2], from[2];
+  int64_t cost[2];
+};
+
 struct PagedAttn {
   // maps of the queries (a tile of tokens, and one token) and of the K / V rows, made at the launch
   CUtensorMap tm_q, tm_q1, tm_k, tm_v;
@@ -42,10 +49,10 @@ struct PagedAttn {
   int decode;     // one token per sequence, the work cut into even ranges of key tiles
   int may_split;  // prompts: the units may be too few for the SMs
   int num_ctas;
-  int w_start, w_pair, w_alt;  // decode: costs of beginning a unit, and of its key tiles
+  int w_start, w_pair, w_thin;  // decode: costs of beginning a unit, and of its key tiles
   // workspace: piece counter and finished CTAs, records of sequences and groups, partial results
   unsigned* counter;
-  int64_t* rec_cost; int64_t* rec_row; float* part_o; float2* part_s;
+  int64_t* rec_cost; int64_t* rec_row; Ctas* rec_ctas; float* part_o; float2* part_s;
 };
 
 // Records a wrong argument that only the device sees; the first one stays.

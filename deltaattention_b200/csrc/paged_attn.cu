@@ -10,8 +10,9 @@
 //   prompts   2 * (128 / G) consecutive tokens of a sequence; causal tiles end at their last row's limit;
 //   prefixes  as many sequences of a group that shares its first pages, one token each: these pages are
 //             read once for all of them;
-//   own       one token of one sequence over the rows behind its prefix: G rows. Bytes bound it, and the
-//             two tiles hold the same rows and take every other key tile, two chains at a time.
+//   own       one token of one sequence over the rows behind its prefix: G rows. Bytes bound it. Up to 8 rows are
+//             computed transposed (thin): S^T = K Q^T has a key per row and 8 columns, which takes a warp a tenth
+//             of the time of 128 columns; the two tiles take every other key tile, two chains at a time.
 // With `decode` the key tiles of all units, one after the other, are cut into one even range per CTA
 // (bytes and, for tiles of 256 rows, products cost the same per tile). Prompts take pieces from a counter,
 // heavy ones first; where whole units would leave SMs idle they are cut into chunks of L key tiles, the
@@ -42,6 +43,13 @@ constexpr int PT_FILL = 7;        // most chunks per SM: they bound the workspac
 constexpr int PT_PIECE = 2;
 constexpr int PT_JOIN = 3;
 
+// A CTA's part of a decode step: costs [begin, end), its place among the CTAs in their order, its first item and what
+// lies before that. Of prompts only `item` is used, the key tiles of a chunk.
+struct Range {
+  int64_t begin, end, base_t, base_r;
+  int place, item;
+};
+
 struct Piece {
   int end;         // no more pieces
   int tok0, ntok;  // first token, tokens
@@ -50,16 +58,16 @@ struct Piece {
   int kb;          // first key of key tile 0
   int kend;        // keys that exist: rows from here on are not read
   int j0, nt0, nt1;  // key tiles: from j0 up to nt0 for tile 0, nt1 for tile 1
-  int alt;         // both tiles hold the same rows and take every other key tile (by the parity of its fill)
+  int thin;        // at most PT_THIN rows: both tiles hold them and take every other key tile (by the parity of its
+                   // fill), and scores and output are computed transposed
   int lim0, lim_step;  // keys that token tok0 + i sees: lim0 + i * lim_step ..
   int by_length;   // .. and no more than the token's sequence has
-  int split;       // partial results to rows orow0 / orow1, else the output
+  int split;       // partial results to rows orow0 / orow1 (thin: orow0), else the output
   int q1;          // one token: the query box of one token
-  int thin;        // at most PT_THIN rows: scores and output are computed transposed
   int64_t orow0, orow1;
   __device__ __forceinline__ int jend() const { return max(nt0, nt1); }
   // query tiles it needs: tiles that hold the same rows share one
-  __device__ __forceinline__ int q_tiles(int tpt) const { return !alt && ntok > tpt ? 2 : 1; }
+  __device__ __forceinline__ int q_tiles(int tpt) const { return !thin && ntok > tpt ? 2 : 1; }
 };
 
 template <int D> struct PtCfg {
@@ -75,9 +83,10 @@ template <int D> struct PtCfg {
   static constexpr int OFF_P = OFF_EPI + 8 * 32 * EPI_PITCH;  // weights of thin pieces, [2][16 rows x 128 keys], rows from PT_THIN on unused
   static constexpr int PBYTES = 16 * PT_BN * 2;
   static constexpr int OFF_VOTE = OFF_P + 2 * PBYTES;  // [2 tiles][2][4 warps][PT_THIN] maxima, then flags
-  static constexpr int OFF_PIECE = OFF_VOTE + 2 * 2 * 4 * (PT_THIN + 1) * 4;
+  static constexpr int OFF_X = OFF_VOTE + 2 * 2 * 4 * (PT_THIN + 1) * 4;  // thin: tile 1's O^T, maxima and sums
+  static constexpr int OFF_PIECE = OFF_X + PT_THIN * (D + 2) * 4;
   static constexpr int OFF_BAR = OFF_PIECE + PT_RING * static_cast<int>(sizeof(Piece));
-  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 6 + 1 + 2 + 2;
+  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 6 + 1 + 2 + 2 + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_MISC + 256 + 1024;  // and slack for alignment
 };
@@ -125,18 +134,38 @@ __device__ __forceinline__ int group_of(const PagedAttn& p, int groups, int b) {
 struct Item {
   int first, count;  // sequences
   int start, len;    // rows [start, len) of the sequences
-  int tiles, units, rows, alt;
+  int tiles, units, rows, thin;
   // what a unit and the item cost: a start for each unit, and its key tiles
-  __device__ __forceinline__ int tile_cost(const PagedAttn& p) const { return alt ? p.w_alt : p.w_pair; }
+  __device__ __forceinline__ int tile_cost(const PagedAttn& p) const { return thin ? p.w_thin : p.w_pair; }
   __device__ __forceinline__ int64_t unit_cost(const PagedAttn& p) const {
     return tiles ? p.w_start + static_cast<int64_t>(tiles) * tile_cost(p) : 0;
   }
   __device__ __forceinline__ int64_t cost(const PagedAttn& p) const { return static_cast<int64_t>(p.H) * units * unit_cost(p); }
 };
-// CTAs that take part: the dearest key tile at least for each, so that a CTA whose range lies inside a unit has one of
-// its tiles
-__device__ __forceinline__ int64_t decode_ctas(const PagedAttn& p, int64_t total) {
-  return min(max(quotient(total, max(p.w_alt, p.w_pair)), total ? int64_t{1} : int64_t{0}), static_cast<int64_t>(p.num_ctas));
+// The CTAs of a decode step: the first n[0] share the prefixes' costs, n[1] after them the own rows'. In each part the
+// dearest key tile at least for every CTA, so that one whose range lies inside a unit has one of its tiles. The first
+// part is even: products bound the prefixes of many sequences and bytes the own rows, and two neighbours on the chip
+// that do one each both run at a third of their speed (64 sequences over 32000 shared rows: 120 us where one
+// pair was mixed, 155 us where all were, .. without).
+__device__ __forceinline__ Ctas decode_ctas(const PagedAttn& p, int64_t prefixes, int64_t total) {
+  Ctas c;
+  c.cost[0] = prefixes;
+  c.cost[1] = total - prefixes;
+  int first = 0;
+  if (prefixes) {
+    first = static_cast<int>(quotient((prefixes + 1) / 2 * p.num_ctas, (total + 1) / 2));
+    first = (first + 1) & ~1;
+    if (c.cost[1]) first = min(max(first, 2), p.num_ctas - 2);
+    first = min(first, p.num_ctas);
+  }
+  c.from[0] = 0;
+  c.from[1] = first;
+  const int64_t w = max(p.w_thin, p.w_pair);
+  for (int k = 0; k < 2; ++k) {
+    const int most = k ? p.num_ctas - first : first;
+    c.n[k] = c.cost[k] ? static_cast<int>(min(max(quotient(c.cost[k], w), int64_t{1}), static_cast<int64_t>(most))) : 0;
+  }
+  return c;
 }
 // (Not inlined, like prompt_seq: a launch's first pass through code waits for instructions, and the copies of
 // these on the way to the first load cost more than the calls.)
@@ -148,7 +177,7 @@ __device__ __noinline__ Item decode_item(const PagedAttn& p, int groups, int tpt
     it.start = 0;
     it.len = it.count ? prefix_rows(p, i) : 0;
     it.units = (it.count + 2 * tpt - 1) / (2 * tpt);
-    it.alt = it.count <= tpt;
+    it.thin = 0;
   } else {
     const int b = i - groups;
     const int g = group_of(p, groups, b);
@@ -157,18 +186,18 @@ __device__ __noinline__ Item decode_item(const PagedAttn& p, int groups, int tpt
     it.len = paged_length(p.lengths[b], p.max_pages, p.ps_shift, p.err);
     it.start = g < 0 ? 0 : min(prefix_rows(p, g), it.len);
     it.units = 1;
-    it.alt = 1;
+    it.thin = p.G <= PT_THIN;
   }
   it.tiles = (it.len - it.start + PT_BN - 1) / PT_BN;
-  it.rows = it.count * p.G * (it.alt ? 2 : 1);
+  it.rows = it.count * p.G;
   return it;
 }
 
 // Exclusive sums over the block's threads of two numbers; returns the totals.
-__device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t* smem, int64_t& ta, int64_t& tb) {
+__device__ __noinline__ void block_scan2(int64_t& a, int64_t& b, int64_t* smem, int64_t& ta, int64_t& tb) {
   const int lane = lane_id(), warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   int64_t sa = a, sb = b;
-#pragma unroll
+#pragma unroll 1
   for (int o = 1; o < 32; o <<= 1) {
     const int64_t ua = __shfl_up_sync(0xFFFFFFFFu, sa, o), ub = __shfl_up_sync(0xFFFFFFFFu, sb, o);
     if (lane >= o) {
@@ -183,6 +212,7 @@ __device__ __forceinline__ void block_scan2(int64_t& a, int64_t& b, int64_t* sme
   __syncthreads();
   int64_t pa = 0, pb = 0;
   ta = tb = 0;
+#pragma unroll 1
   for (int w = 0; w < nw; ++w) {
     if (w == warp) {
       pa = ta;
@@ -217,6 +247,7 @@ __device__ __forceinline__ int chunk_tiles(const PagedAttn& p, int64_t units, in
   const unsigned n = static_cast<unsigned>(units), mean = static_cast<unsigned>(quotient(tiles + units - 1, units));
   const unsigned ctas = static_cast<unsigned>(p.num_ctas);
   unsigned best = 0, least = 0xFFFFFFFFu;
+#pragma unroll 1
   for (unsigned k = 1; k <= PT_CHUNKS && (k == 1 || (mean >= PT_MIN_CHUNK * k && n * k <= PT_FILL * ctas)); ++k) {
     // one chunk needs no joining, which costs some tiles' time as well
     const unsigned len = (mean + k - 1) / k, cost = (n * k + ctas - 1) / ctas * (len + PT_PIECE) + (k > 1 ? PT_JOIN : 0);
@@ -249,6 +280,7 @@ template <bool DEC> struct Sched {
   int64_t before_t, inc_t, before_r, inc_r;  // the lane's item: sums of costs and rows before and with it
   typename std::conditional<DEC, Item, Seq>::type item;
   int groups, tpt, chunk;
+  int place;                    // decode: of the CTA's range in the order of costs
   bool loaded;
 
   __device__ __forceinline__ void load(const PagedAttn& p) {
@@ -325,17 +357,16 @@ template <bool DEC> struct Sched {
         pc.kb = item.start;
         pc.kend = item.len;
         pc.trow = item.first;
-        pc.alt = item.alt;
         pc.q1 = !shared;
-        pc.thin = !shared && p.G <= PT_THIN;
-        pc.nt1 = item.alt || pc.ntok > tpt ? pc.nt0 : 0;
+        pc.thin = item.thin;
+        pc.nt1 = item.thin || pc.ntok > tpt ? pc.nt0 : 0;
         pc.lim0 = item.len;
         pc.lim_step = 0;
         pc.by_length = shared;
         pc.split = 1;
         pc.orow0 = base_r + before_r + static_cast<int64_t>(h) * item.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
-                   static_cast<int64_t>(blockIdx.x) * PT_ROWS;
-        pc.orow1 = pc.orow0 + (item.alt ? item.count : tpt) * p.G;
+                   static_cast<int64_t>(place) * PT_ROWS;
+        pc.orow1 = pc.orow0 + tpt * p.G;
         break;
       } else {
         unsigned id = 0;
@@ -376,7 +407,7 @@ template <bool DEC> struct Sched {
         pc.kb = 0;
         pc.kend = item.len;
         pc.trow = p.table ? i0 + lane : item.c0;
-        pc.alt = pc.q1 = pc.thin = pc.by_length = 0;
+        pc.q1 = pc.thin = pc.by_length = 0;
         pc.lim0 = p.causal ? pos0 + 1 : item.len;
         pc.lim_step = p.causal ? 1 : 0;
         pc.split = nch > 1;
@@ -483,11 +514,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   uint64_t* vote = tile_free + 2;       // [2] thin pieces: the tile's warps have looked at their scores
   uint64_t* mma_done = vote + 2;
   uint64_t* turn = mma_done + 1;        // [2]
+  uint64_t* xfer = turn + 4;            // [2] thin: tile 1's result is there, and has been read
   uint64_t* level = turn + 2;           // [2] warp 1 + x is past its pieces of its own
   Piece* pieces = reinterpret_cast<Piece*>(smem + C::OFF_PIECE);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
-  int64_t* start = reinterpret_cast<int64_t*>(smem + C::OFF_MISC + 16);  // item, its tiles' and rows' base, chunk
+  Range* range = reinterpret_cast<Range*>(smem + C::OFF_MISC + 16);
   int64_t* scan = reinterpret_cast<int64_t*>(smem + C::OFF_EPI);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -515,6 +547,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       mbar_init(vote + x, 4);
       mbar_init(turn + x, 1);
       mbar_init(level + x, 1);
+      mbar_init(xfer + x, 4);
     }
     mbar_init(mma_done, 2);
     *abort_flag = 0;
@@ -534,7 +567,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   const int tpt = 128 / p.G;
   int groups = 0;
   if constexpr (DEC) groups = groups_ok(p) ? p.groups : 0;
-  int64_t pos = 0, pos_end = 0;
   if (DEC || p.may_split) {
     // `per` items in a row for every thread; all threads take all turns, since a warp that parts here
     // does not come together again, and runs apart through everything below
@@ -543,6 +575,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     const int first = static_cast<int>(threadIdx.x) * per;
     int64_t c = 0, r = 0, tc, tr;
     Item it;
+#pragma unroll 1
     for (int k = 0; k < per; ++k) {
       const int i = min(first + k, n - 1);
       const bool has = first + k < n;
@@ -558,39 +591,67 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     }
     block_scan2(c, r, scan, tc, tr);
     if constexpr (DEC) {
-      const int64_t ctas = decode_ctas(p, tc);
-      if (blockIdx.x < ctas) {
-        pos = quotient(tc * blockIdx.x, ctas);
-        pos_end = quotient(tc * (blockIdx.x + 1), ctas);
+      int64_t prefixes = 0;
+      if (groups) {
+        // the prefixes' costs end where the first sequence's begin
+        int64_t at = c;
+#pragma unroll 1
+        for (int k = 0; k < per; ++k) {
+          if (per > 1) it = decode_item(p, groups, tpt, min(first + k, n - 1));
+          if (first + k == groups) range->base_t = at;
+          at += it.cost(p);
+        }
+        __syncthreads();
+        prefixes = range->base_t;
+        __syncthreads();
       }
+      const Ctas ct = decode_ctas(p, prefixes, tc);
+      const int bid = static_cast<int>(blockIdx.x), list = bid >= ct.from[1], nc = list ? ct.n[1] : ct.n[0];
+      int at = bid - (list ? ct.from[1] : 0);
+      int64_t pos = 0, pos_end = 0;
+      if (at < nc) {
+        // neighbours on the chip take ranges far from each other (64 sequences of 1000 rows: 69 -> 65 us)
+        at = at & 1 ? (nc + 1) / 2 + at / 2 : at / 2;
+        const int64_t total = list ? ct.cost[1] : prefixes, from = list ? prefixes : 0;
+        pos = from + quotient(total * at, nc);
+        pos_end = from + quotient(total * (at + 1), nc);
+      }
+      if (threadIdx.x == 0) {
+        range->begin = pos;
+        range->end = pos_end;
+        range->place = at + (list ? ct.from[1] : 0);
+        if (bid == 0) *p.rec_ctas = ct;
+      }
+#pragma unroll 1
       for (int k = 0; k < per; ++k) {
         const int i = min(first + k, n - 1);
         const bool has = first + k < n;
         if (per > 1) it = decode_item(p, groups, tpt, i);
         const int64_t ci = has ? it.cost(p) : 0;
         if (c <= pos && pos < c + ci) {
-          start[0] = i;
-          start[1] = c;
-          start[2] = r;
+          range->item = i;
+          range->base_t = c;
+          range->base_r = r;
         }
-        if (blockIdx.x == 0 && has) {
+        if (bid == 0 && has) {
           p.rec_cost[i] = c;
           p.rec_row[i] = r;
         }
         c += ci;
         r += static_cast<int64_t>(p.H) * it.rows;
       }
-      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_cost[n] = tc;
     } else {
       const int chunk = chunk_tiles(p, tr, tc);
-      if (threadIdx.x == 0) start[3] = chunk;
+      if (threadIdx.x == 0) range->item = chunk;
       if (blockIdx.x == 0 && chunk) {
         // the sequences' first pieces, for the joining kernel
         int64_t zero = 0, tz;
         c = 0;
+#pragma unroll 1
         for (int k = 0; k < per; ++k)
           c += first + k < n ? prompt_pieces(p, prompt_seq(p, 2 * tpt, min(first + k, n - 1)), chunk) : 0;
         block_scan2(c, zero, scan, tc, tz);
+#pragma unroll 1
         for (int k = 0; k < per; ++k) {
           const Seq s = prompt_seq(p, 2 * tpt, min(first + k, n - 1));
           if (first + k < n) p.rec_cost[first + k] = c;
@@ -625,16 +686,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     Sched<DEC> sc;
     sc.groups = groups;
     sc.tpt = tpt;
-    sc.pos = pos;
-    sc.end = pos_end;
     sc.n = DEC ? groups + p.B : p.B;
-    sc.chunk = !DEC && p.may_split ? static_cast<int>(start[3]) : 0;
-    sc.i0 = 0;
-    sc.base_t = sc.base_r = 0;
-    if (DEC && pos < pos_end) {
-      sc.i0 = static_cast<int>(start[0]);
-      sc.base_t = start[1];
-      sc.base_r = start[2];
+    sc.chunk = !DEC && p.may_split ? range->item : 0;
+    sc.i0 = sc.place = 0;
+    sc.base_t = sc.base_r = sc.pos = sc.end = 0;
+    if constexpr (DEC) {
+      sc.pos = range->begin;
+      sc.end = range->end;
+      if (sc.pos < sc.end) {
+        sc.place = range->place;
+        sc.i0 = range->item;
+        sc.base_t = range->base_t;
+        sc.base_r = range->base_r;
+      }
     }
     sc.loaded = false;
     int published = 0;
@@ -741,7 +805,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     // The warp runs converged and one elected lane issues. Tiles of a pair walk the same key tiles; both
     // warps wait for every fill, in order, and release it, so a slot's two arrivals are of one fill. They issue
     // their batches (a tile's P V and the next one's Q K^T) in turn, tile 0 first, which keeps the two
-    // softmax passes half a period apart. Tiles that share the rows (`alt`) go apart: fills of even number are
+    // softmax passes half a period apart. The two of a thin piece go apart: fills of even number are
     // tile 0's, of odd number tile 1's, and their warp releases them with both arrivals. As the slots of a
     // parity stay with a warp, it sees all of their phases; before a pair's piece, which it walks with the
     // other one, they wait for each other, so that no earlier phase of the other's slots is still open.
@@ -781,7 +845,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         for (int f = q0; f < q0 + nq; ++f) umma_commit(q_empty + (f & 1));
       };
       const int je = pc.jend();
-      const bool mine = x == 0 || pc.alt || pc.ntok > tpt;
+      const bool mine = x == 0 || pc.thin || pc.ntok > tpt;
       bool freed = false, o_init = false;
       auto ensure_free = [&]() -> bool {
         if (freed) return true;
@@ -796,8 +860,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint64_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
-          if (DEC && pc.thin) umma_ss(tS, kb + off, qdesc + off, IDESC_T, kk > 0);
-          else umma_ss(tS, qdesc + off, kb + off, IDESC_S, kk > 0);
+          umma_ss(tS, qdesc + off, kb + off, IDESC_S, kk > 0);
+        }
+        umma_commit(s_full + x);
+      };
+      auto issue_St = [&](int f) {
+        const uint64_t kb = kdesc0 + static_cast<uint64_t>((f % NK) * (C::KVBYTES >> 4));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t off = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+          umma_ss(tS, kb + off, qdesc + off, IDESC_T, kk > 0);
         }
         umma_commit(s_full + x);
       };
@@ -848,7 +920,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         tc_fence_after();
         return true;
       };
-      if (DEC && pc.alt) {
+      if (DEC && pc.thin) {
         apart = true;
         const int n = je - pc.j0, first = (fpos ^ x) & 1;
         if (first >= n) free_q();
@@ -865,7 +937,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           const int f = fpos + i;
           ok = wait_k(f);
           if (!ok) break;
-          issue_S(f);
+          issue_St(f);
           umma_commit(k_empty + f % NK);
           umma_commit(k_empty + f % NK);
         }
@@ -927,19 +999,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     const uint32_t tO = tmem + lane_base + 256 + D * x;
     const float sl2 = p.scale_log2;
     int vpos = 0;
-    uint32_t s_par = 0, o_par = 0, votes = 0;
+    uint32_t s_par = 0, o_par = 0, votes = 0, xfers = 0;
     Piece pc;
     bool ok = true;
     while (ok && take(pc, ERR_TIMEOUT_SOFTMAX)) {
-      if (!DEC) pc.alt = pc.by_length = 0;
-      const int je = pc.jend(), step = pc.alt ? 2 : 1;
-      const bool valid = x == 0 || pc.alt || pc.ntok > tpt;
-      const int ntok = pc.alt ? pc.ntok : max(0, min(tpt, pc.ntok - x * tpt));
+      if (!DEC) pc.by_length = 0;
+      const int je = pc.jend();
+      const bool valid = x == 0 || pc.ntok > tpt;  // (not of thin pieces)
+      const int ntok = max(0, min(tpt, pc.ntok - x * tpt));
       const int nrows = ntok * p.G;
       const bool warp_live = wq * 32 < nrows;
       const bool live = r < nrows;
       const int ti = r / p.G;                               // token of this row within the tile
-      const int tok = pc.tok0 + (pc.alt ? 0 : x * tpt) + ti;
+      const int tok = pc.tok0 + x * tpt + ti;
       int lim_row = 0;  // keys from kb on that this row sees
       if (live) {
         lim_row = pc.lim0 + (tok - pc.tok0) * pc.lim_step;
@@ -960,24 +1032,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           ls[g] = 0.f;
         }
         bool has = false;
-        auto reduce = [&](float (&v)[PT_THIN], bool sum) -> float {  // lane g: column g's maximum or sum over the warp
-          float mine = 0.f;
+        // Column lane / 4's maximum or sum over the warp: the lanes halve the columns among themselves three times.
+        auto reduce = [&](const float (&in)[PT_THIN], bool sum) -> float {
+          float v[PT_THIN];
 #pragma unroll
-          for (int g = 0; g < PT_THIN; ++g) {
-            if (g < p.G) {
+          for (int g = 0; g < PT_THIN; ++g) v[g] = in[g];
 #pragma unroll
-              for (int o = 16; o; o >>= 1) {
-                const float u = __shfl_xor_sync(0xFFFFFFFFu, v[g], o);
-                v[g] = sum ? v[g] + u : fmaxf(v[g], u);
+          for (int o = 16, n = PT_THIN / 2; o; o >>= 1, n >>= 1) {
+            if (n) {
+              const bool up = lane & o;
+#pragma unroll
+              for (int g = 0; g < n; ++g) {
+                const float keep = up ? v[g + n] : v[g], give = up ? v[g] : v[g + n];
+                const float got = __shfl_xor_sync(0xFFFFFFFFu, give, o);
+                v[g] = sum ? keep + got : fmaxf(keep, got);
               }
+            } else {
+              const float got = __shfl_xor_sync(0xFFFFFFFFu, v[0], o);
+              v[0] = sum ? v[0] + got : fmaxf(v[0], got);
             }
-            if (lane == g) mine = v[g];
           }
-          return mine;
+          return v[0];
         };
         auto cast_vote = [&](float mine, bool put, bool flag) -> bool {
           const int at = (votes & 1) * 4 + wq;
-          if (put && lane < PT_THIN) vmax[at * PT_THIN + lane] = mine;
+          if (put && (lane & 3) == 0) vmax[at * PT_THIN + (lane >> 2)] = mine;
           if (lane == 0) vflag[at] = flag;
           __syncwarp();
           if (lane == 0) mbar_arrive(vote + x);
@@ -1002,12 +1081,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           }
           over = __any_sync(0xFFFFFFFFu, over);
           float mine = 0.f;
-          if (over) {
-            float t[PT_THIN];
-#pragma unroll
-            for (int g = 0; g < PT_THIN; ++g) t[g] = s[g];
-            mine = reduce(t, false);
-          }
+          if (over) mine = reduce(s, false);
           ok = cast_vote(mine, over, over);
           if (!ok) break;
           const int seen = (votes & 1) ^ 1;
@@ -1077,37 +1151,53 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         vpos += je - pc.j0;
         // the sums over the tile's keys: the warp's, then the four warps' through the votes' memory
         if (!cast_vote(reduce(ls, true), true, false)) break;
-        const int64_t row0 = x ? pc.orow1 : pc.orow0;
-        if (wq == 0) {
-          float my_m = 0.f;
-#pragma unroll
-          for (int g = 0; g < PT_THIN; ++g) my_m = lane == g ? m[g] : my_m;
-          if (lane < p.G) {
-            const float* v = vmax + ((votes & 1) ^ 1) * 4 * PT_THIN + lane;
-            const float sum = (v[0] + v[PT_THIN]) + (v[2 * PT_THIN] + v[3 * PT_THIN]);
-            p.part_s[row0 + lane] = make_float2(my_m, has ? sum : 0.f);
-          }
-        }
+        const float* sums = vmax + ((votes & 1) ^ 1) * 4 * PT_THIN;
         if (!pt_wait(o_full + x, o_par, ab, ERR_TIMEOUT_EPILOGUE)) break;
         o_par ^= 1;
         tc_fence_after();
-        if (has && wq * 32 < D) {
-          uint32_t o[PT_THIN];
-          tmem_ld8(tO, o);
-#pragma unroll
-          for (int g = 0; g < PT_THIN; ++g)
-            if (g < p.G) p.part_o[(row0 + g) * D + r] = __uint_as_float(o[g]);
-        }
+        uint32_t o[PT_THIN];
+        tmem_ld8(tO, o);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(tile_free + x);
+        // tile 1 hands its O^T, maxima and sums over, tile 0 adds them to its own and stores the piece's
+        float* xo = reinterpret_cast<float*>(smem + C::OFF_X);
+        float* xm = xo + PT_THIN * D;
+        float* xl = xm + PT_THIN;
+        if (!pt_wait(xfer + (x ^ 1), (xfers & 1) ^ x, ab, ERR_TIMEOUT_EPILOGUE)) break;
+        ++xfers;
+        if (x) {
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g) {
+            if (r < D) xo[g * D + r] = __uint_as_float(o[g]);
+            if (r == g) {
+              xm[g] = m[g];
+              xl[g] = has ? (sums[g] + sums[PT_THIN + g]) + (sums[2 * PT_THIN + g] + sums[3 * PT_THIN + g]) : 0.f;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int g = 0; g < PT_THIN; ++g) {
+            if (g >= p.G) continue;
+            const float l0 = has ? (sums[g] + sums[PT_THIN + g]) + (sums[2 * PT_THIN + g] + sums[3 * PT_THIN + g]) : 0.f;
+            const float l1 = xl[g], m1 = xm[g];
+            // a tile that has nothing for the row (sum 0; not NaN) takes no part
+            const float mm = l0 == 0.f ? m1 : l1 == 0.f ? m[g] : fmaxf(m[g], m1);
+            const float a0 = l0 == 0.f ? 0.f : ex2(m[g] - mm), a1 = l1 == 0.f ? 0.f : ex2(m1 - mm);
+            if (r < D)
+              p.part_o[(pc.orow0 + g) * D + r] = (l0 == 0.f ? 0.f : a0 * __uint_as_float(o[g])) + (l1 == 0.f ? 0.f : a1 * xo[g * D + r]);
+            if (r == g) p.part_s[pc.orow0 + g] = make_float2(mm, (l0 == 0.f ? 0.f : a0 * l0) + (l1 == 0.f ? 0.f : a1 * l1));
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(xfer + x);
         continue;
       }
       // rows that do not exist get a reference no score exceeds, and weigh nothing
       float m_used = live ? -INFINITY : 1e30f, l = 0.f;
       bool o_has = false;
-      const int my_end = pc.alt ? je : (x ? pc.nt1 : pc.nt0);
-      for (int j = pc.j0 + (pc.alt ? (vpos ^ x) & 1 : 0); valid && j < my_end; j += step) {
+      const int my_end = x ? pc.nt1 : pc.nt0;
+      for (int j = pc.j0; valid && j < my_end; ++j) {
         const int f = vpos + (j - pc.j0);
         const int n0 = j * PT_BN;
         const int have = pc.kend - pc.kb - n0;  // rows of this tile that exist
@@ -1320,22 +1410,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             }
           } else if (o_has) {
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld16(tO + c * 16, o);
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + c * 32, o);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                *reinterpret_cast<uint4*>(stg + lane * C::EPI_PITCH + e * 16) =
-                    make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-              __syncwarp();
+              for (int hf = 0; hf < 2; ++hf) {
 #pragma unroll
-              for (int q4 = 0; q4 < 4; ++q4) {
-                const int lr = q4 * 8 + rr;
-                if (lr < left)
-                  *reinterpret_cast<uint4*>(p.part_o + (row0 + lr) * D + c * 16 + seg * 4) =
-                      *reinterpret_cast<const uint4*>(stg + lr * C::EPI_PITCH + seg * 16);
+                for (int e = 0; e < 4; ++e)
+                  *reinterpret_cast<uint4*>(stg + lane * C::EPI_PITCH + e * 16) = make_uint4(
+                      o[hf * 16 + 4 * e], o[hf * 16 + 4 * e + 1], o[hf * 16 + 4 * e + 2], o[hf * 16 + 4 * e + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4) {
+                  const int lr = q4 * 8 + rr;
+                  if (lr < left)
+                    *reinterpret_cast<uint4*>(p.part_o + (row0 + lr) * D + c * 32 + hf * 16 + seg * 4) =
+                        *reinterpret_cast<const uint4*>(stg + lr * C::EPI_PITCH + seg * 16);
+                }
+                __syncwarp();
               }
-              __syncwarp();
             }
           }
         } else {
@@ -1476,105 +1569,113 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant_
   jn.store(static_cast<T*>(p.out) + t * p.o_t + hq * p.o_h);
 }
 
-// Decoding, whose few rows have many pieces each (two for every CTA that had a part of the unit, of the prefix and
-// of the own rows): a block per row, every fourth piece to a warp, eight of them on their way at once and
-// before the maxima are known.
-template <int D, typename T>
-__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ PagedAttn p) {
+// Decoding, whose few rows have many pieces each (one for every CTA that had a part of the prefix or of the own rows):
+// eight of them on their way at once. WPR warps share a row's pieces, and their sums meet in shared memory: four where a
+// block per row fits the GPU at once, one for more rows (see launch_paged_t).
+template <int D, typename T, int WPR>
+__global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_constant__ PagedAttn p) {
   constexpr int E = D / 32;
-  __shared__ float acc_s[4][D], l_s[4];
+  __shared__ float acc_s[4][D];
+  __shared__ float2 s_s[4];
   const int tpt = 128 / p.G, Hq = p.H * p.G, lane = lane_id(), warp = threadIdx.x >> 5;
-  const int b = blockIdx.x / Hq, hq = blockIdx.x % Hq, h = hq / p.G, rg = hq % p.G;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WPR) + warp / WPR;
   const int groups = groups_ok(p) ? p.groups : 0;
+  if (row >= static_cast<int64_t>(p.B) * Hq) return;
+  const int b = static_cast<int>(row / Hq), hq = static_cast<int>(row % Hq), h = hq / p.G, rg = hq % p.G;
   const int g = group_of(p, groups, b);
   const Item own = decode_item(p, groups, tpt, groups + b);
   Item shared = own;
   if (g >= 0) shared = decode_item(p, groups, tpt, g);
   // everything above goes by the inputs alone
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t total = p.rec_cost[groups + p.B], ctas = decode_ctas(p, total);
+  const Ctas ct = *p.rec_ctas;
+  int n0 = 0, n1 = 0;
+  int64_t base0 = 0, base1 = 0;
   // pieces of a unit: one in every CTA from that of its first key tile to that of its last
-  auto unit = [&](int i, const Item& it, int up, int in_unit, int& n, int64_t& base) {
-    n = 0;
-    base = 0;
-    if (!it.tiles) return;
-    const int64_t u0 = p.rec_cost[i] + (static_cast<int64_t>(h) * it.units + up) * it.unit_cost(p) + p.w_start;
-    const int c0 = static_cast<int>(quotient((u0 + 1) * ctas - 1, total));
-    const int c1 = static_cast<int>(quotient((u0 + static_cast<int64_t>(it.tiles - 1) * it.tile_cost(p) + 1) * ctas - 1, total));
-    n = (c1 - c0 + 1) * (it.alt ? 2 : 1);
-    base = p.rec_row[i] + static_cast<int64_t>(h) * it.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
-           static_cast<int64_t>(c0) * PT_ROWS + in_unit;
-  };
-  int n0 = 0, n1;
-  int64_t base0 = 0, base1;
-  if (g >= 0) {
-    const int mi = b - shared.first, up = mi / (2 * tpt);
-    unit(g, shared, up, (mi - up * 2 * tpt) * p.G + rg, n0, base0);
+  if (own.tiles) {
+    const int64_t u0 = p.rec_cost[groups + b] - ct.cost[0] + h * own.unit_cost(p) + p.w_start;
+    const int c0 = static_cast<int>(quotient((u0 + 1) * ct.n[1] - 1, ct.cost[1]));
+    n1 = static_cast<int>(quotient((u0 + static_cast<int64_t>(own.tiles - 1) * own.tile_cost(p) + 1) * ct.n[1] - 1, ct.cost[1])) - c0 + 1;
+    base1 = p.rec_row[groups + b] + static_cast<int64_t>(h) * own.rows + static_cast<int64_t>(c0 + ct.from[1]) * PT_ROWS + rg;
   }
-  unit(groups + b, own, 0, rg, n1, base1);
+  if (g >= 0 && shared.tiles) {
+    const int in = b - shared.first, up = in / (2 * tpt);
+    const int64_t u0 = p.rec_cost[g] + (static_cast<int64_t>(h) * shared.units + up) * shared.unit_cost(p) + p.w_start;
+    const int c0 = static_cast<int>(quotient((u0 + 1) * ct.n[0] - 1, ct.cost[0]));
+    n0 = static_cast<int>(quotient((u0 + static_cast<int64_t>(shared.tiles - 1) * shared.tile_cost(p) + 1) * ct.n[0] - 1, ct.cost[0])) - c0 + 1;
+    base0 = p.rec_row[g] + static_cast<int64_t>(h) * shared.rows + in * p.G + static_cast<int64_t>(c0) * PT_ROWS + rg;
+  }
   const int n = n0 + n1;
-  auto row = [&](int i) -> int64_t {
-    const bool first = i < n0;
-    const int k = first ? i : i - n0;
-    const int64_t base = first ? base0 : base1;
-    if (!(first ? shared.alt : 1)) return base + static_cast<int64_t>(k) * PT_ROWS;
-    return base + static_cast<int64_t>(k >> 1) * PT_ROWS + (k & 1) * (first ? shared.count : 1) * p.G;
-  };
+  base1 -= static_cast<int64_t>(n0) * PT_ROWS;
   float acc[E], l = 0.f, m = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
+#pragma unroll 1
+  for (int i0 = warp % WPR; i0 < n; i0 += 8 * WPR) {
     float v[8][E];
     float2 st[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int i = i0 + warp + 4 * k;
-      st[k] = make_float2(-INFINITY, 0.f);
+      const int i = min(i0 + WPR * k, n - 1);  // the last one again where there are fewer
+      const int64_t at = (i < n0 ? base0 : base1) + static_cast<int64_t>(i) * PT_ROWS;
+      st[k] = __ldcg(p.part_s + at);
       if constexpr (D == 128) {
-        float4 f4 = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (i < n) {
-          const int64_t at = row(i);
-          st[k] = __ldcg(p.part_s + at);
-          f4 = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + lane);
-        }
+        const float4 f4 = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + lane);
         v[k][0] = f4.x; v[k][1] = f4.y; v[k][2] = f4.z; v[k][3] = f4.w;
       } else {
-        float2 f2 = make_float2(0.f, 0.f);
-        if (i < n) {
-          const int64_t at = row(i);
-          st[k] = __ldcg(p.part_s + at);
-          f2 = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * D) + lane);
-        }
+        const float2 f2 = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * D) + lane);
         v[k][0] = f2.x; v[k][1] = f2.y;
       }
     }
-    if (i0 == 0) {
-      // the maximum over all pieces that hold something for the row
-      for (int i = lane; i < n; i += 32) {
-        const float2 s = __ldcg(p.part_s + row(i));
-        if (s.y != 0.f) m = fmaxf(m, s.x);
-      }
-#pragma unroll
-      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    }
+    // pieces that hold nothing for the row (sum 0; not NaN) take no part
+    float mn = m;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const bool has = st[k].y != 0.f;  // NaN too
+      if (i0 + WPR * k >= n) st[k].y = 0.f;
+      if (st[k].y != 0.f) mn = fmaxf(mn, st[k].x);
+    }
+    const float f = m == -INFINITY ? 0.f : ex2(m - mn);
+    m = mn;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const bool has = st[k].y != 0.f;
       const float w = has ? ex2(st[k].x - m) : 0.f;
       l += has ? w * st[k].y : 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] += has ? w * v[k][e] : 0.f;
     }
   }
+  T* dst = static_cast<T*>(p.out) + b * p.o_t + hq * p.o_h;
+  if constexpr (WPR == 1) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T o[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc_s[warp][lane * E + e] = acc[e];
-  if (lane == 0) l_s[warp] = l;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    const int d = threadIdx.x;
-    const float sum = (l_s[0] + l_s[1]) + (l_s[2] + l_s[3]);
-    const float o = (acc_s[0][d] + acc_s[1][d]) + (acc_s[2][d] + acc_s[3][d]);
-    static_cast<T*>(p.out)[b * p.o_t + hq * p.o_h + d] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
+    for (int e = 0; e < E; ++e) o[e] = from_f32<T>(acc[e] * inv);
+    if constexpr (D == 128) *reinterpret_cast<uint2*>(dst + lane * E) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint32_t*>(dst + lane * E) = *reinterpret_cast<const uint32_t*>(o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc_s[warp][lane * E + e] = acc[e];
+    if (lane == 0) s_s[warp] = make_float2(m, l);
+    __syncthreads();
+    if (threadIdx.x < D) {
+      const int d = threadIdx.x;
+      float mn = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        if (s_s[w].y != 0.f) mn = fmaxf(mn, s_s[w].x);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (s_s[w].y == 0.f) continue;
+        const float f = ex2(s_s[w].x - mn);
+        sum += f * s_s[w].y;
+        o += f * acc_s[w][d];
+      }
+      dst[d] = from_f32<T>(sum == 0.f ? 0.f : o / sum);
+    }
   }
 }
 
@@ -1589,8 +1690,8 @@ Sizes sizes_of(int64_t T, int64_t B, int64_t H, int64_t G, int64_t groups, bool 
   const int64_t utok = 2 * (128 / G);
   if (decode) {
     s.split = true;
-    s.rows = 4 * B * H * G + PT_ROWS * static_cast<int64_t>(sms);
-    s.recs = groups + B + 1;
+    s.rows = 2 * B * H * G + PT_ROWS * static_cast<int64_t>(sms);
+    s.recs = groups + B;
   } else {
     // whole units where the tokens alone make two for every SM
     s.split = H * (T / utok) < 2 * static_cast<int64_t>(sms);
@@ -1617,6 +1718,7 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Sizes s = sizes_of(p.T, p.B, p.H, p.G, p.groups, p.decode, sms);
   p.counter = reinterpret_cast<unsigned*>(ws);
+  p.rec_ctas = reinterpret_cast<Ctas*>(ws + 64);
   ws += 256;
   p.rec_cost = reinterpret_cast<int64_t*>(ws);
   ws += up256(s.recs * 8);
@@ -1630,7 +1732,7 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   // In sixteenths of a microsecond on a full GPU, as measured: ...
   p.w_start = 32;
   p.w_pair = D == 128 ? 32 : 24;
-  p.w_alt = D == 128 ? 24 : 12;
+  p.w_thin = D == 128 ? 24 : 12;
   auto kfn = paged_attn_kernel<D, BF16, DEC>;
   // the limit is raised once per device: asking for it costs a microsecond
   static std::atomic<bool> raised[64];
@@ -1646,7 +1748,8 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   if (e != cudaSuccess || !s.split) return e;
   cudaLaunchConfig_t cfg = {};
   const int64_t rows = static_cast<int64_t>(p.T) * p.H * p.G;
-  cfg.gridDim = dim3(static_cast<unsigned>(p.decode ? rows : (rows + 3) / 4));
+  const bool wide = DEC && rows <= 6 * sms;
+  cfg.gridDim = dim3(static_cast<unsigned>(wide ? rows : (rows + 3) / 4));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute at;
@@ -1654,7 +1757,7 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if constexpr (DEC) return cudaLaunchKernelEx(&cfg, decode_join_kernel<D, T>, p);
+  if constexpr (DEC) return cudaLaunchKernelEx(&cfg, wide ? decode_join_kernel<D, T, 4> : decode_join_kernel<D, T, 1>, p);
   else return cudaLaunchKernelEx(&cfg, prompt_join_kernel<D, T>, p);
 }
 
