@@ -22,6 +22,8 @@ kernels (tests/test_gpu_parity.py).
 
 ``Kv4DecodeCache`` keeps the packed history in 4 bits and can go on when it is full: heads are cut
 to the entries that drew the most attention.
+
+``PagedDecodeCache`` keeps every token (no anchors) of many sequences that come, go and share prompts, in pages.
 """
 from __future__ import annotations
 
@@ -309,3 +311,221 @@ class Kv4DecodeCache:
                     self.evict(layer, **evict)
         torch.cuda.current_stream(self.device).wait_stream(s)
         return g
+
+
+class PagedDecodeCache:
+    """All K and V rows of many sequences in pages of one pool per layer: sequences are opened, forked and closed
+    one by one, and those that begin alike share pages (``ops.paged_append`` and its attention calls).
+
+    A sequence has a place in the batch, [0, places). ``open`` takes one for a prompt, ``fork`` takes consecutive
+    ones for sequences that go on from it: these hold its whole pages in common and are a group, whose shared rows
+    every step reads once for all. ``advance`` makes room for one more token in every open sequence and raises the
+    ``lengths``; ``step`` then runs one layer. Places that are not open have length 0: a step's q, k and v rows for
+    them are not looked at, and their outputs are 0.
+
+    The bookkeeping of pages is the host's (``open``, ``fork``, ``advance``, ``close``); ``page_table`` [places,
+    max_pages] and ``lengths`` [places] (int32) as well as the groups are on the device, and calls on them go out in
+    the current stream's order. A step itself only launches kernels: ``capture_step`` captures one over all layers,
+    to be replayed after every ``advance``.
+
+    ``err`` (int32 [1] on the device) is the appends' error word, ``workspace_error`` reads the attention's."""
+
+    def __init__(self, num_layers, places, q_heads, kv_heads, head_dim, num_pages, page_size, max_length,
+                 dtype=torch.bfloat16, device="cuda", max_tokens=0):
+        if dtype not in (torch.bfloat16, torch.float16) or head_dim not in (64, 128):
+            raise ValueError("PagedDecodeCache: bf16 / fp16 and head_dim 64 / 128 only")
+        if page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("PagedDecodeCache: page_size must be 16, 32, 64, 128 or 256")
+        if min(num_layers, places, kv_heads, num_pages, max_length) < 1 or q_heads < 1 or q_heads % kv_heads:
+            raise ValueError("PagedDecodeCache: sizes must be positive, and q_heads a multiple of kv_heads")
+        self.num_layers, self.places, self.page_size = num_layers, places, page_size
+        self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
+        self.num_pages, self.max_pages, self.max_length = num_pages, -(-max_length // page_size), max_length
+        self.dtype, self.device, self.max_tokens = dtype, torch.device(device), max(int(max_tokens), places)
+        shape = (num_layers, num_pages, kv_heads, page_size, head_dim)
+        self._k = torch.zeros(shape, dtype=dtype, device=self.device)
+        self._v = torch.zeros_like(self._k)
+        self.pools = [ops.PagedKV(self._k[i], self._v[i]) for i in range(num_layers)]
+        i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.device)  # noqa: E731
+        self.page_table, self.lengths, self.err = i32(places, self.max_pages), i32(places), i32(1)
+        self._open = i32(places)  # 1 for open places: what advance adds
+        # one group per place at most: unused ones are empty
+        self.prefix_cu, self.prefix_lengths = i32(places + 1), i32(places)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._users = [0] * num_pages
+        self._pages = [None] * places  # a place's pages, None while it is free
+        self._length = [0] * places
+        self._groups = {}  # first place -> (places, shared rows)
+        self._ws = None
+
+    # ------------------------------------------------------------------ bookkeeping on the host
+    def _take(self, n):
+        if n > len(self._free):
+            raise RuntimeError(f"PagedDecodeCache: {n} pages wanted, {len(self._free)} of {self.num_pages} are free")
+        got = [self._free.pop() for _ in range(n)]
+        for p in got:
+            self._users[p] = 1
+        return got
+
+    def _run(self, n):
+        """The first of n consecutive free places."""
+        run = 0
+        for b in range(self.places):
+            run = run + 1 if self._pages[b] is None else 0
+            if run == n:
+                return b - n + 1
+        raise RuntimeError(f"PagedDecodeCache: no {n} consecutive places are free")
+
+    def _write(self, entries):
+        """Page numbers [(place, column, page)] into the device's table."""
+        if entries:
+            b, c, p = (torch.tensor(x, dtype=torch.int64).to(self.device, non_blocking=True) for x in zip(*entries))
+            self.page_table[b, c] = p.to(torch.int32)
+
+    def _set_lengths(self, places):
+        at = torch.tensor(places, dtype=torch.int64).to(self.device, non_blocking=True)
+        self.lengths[at] = torch.tensor([self._length[b] for b in places], dtype=torch.int32).to(self.device)
+        self._open[at] = torch.tensor([0 if self._pages[b] is None else 1 for b in places],
+                                      dtype=torch.int32).to(self.device)
+
+    def _set_groups(self):
+        """prefix_cu / prefix_lengths: the groups and, between them, runs of places that share nothing."""
+        cu, rows, at = [0], [], 0
+        for b in sorted(self._groups):
+            n, shared = self._groups[b]
+            if b > at:
+                cu.append(b)
+                rows.append(0)
+            cu.append(b + n)
+            rows.append(shared)
+            at = b + n
+        cu += [cu[-1]] * (self.places + 1 - len(cu))
+        rows += [0] * (self.places - len(rows))
+        self.prefix_cu.copy_(torch.tensor(cu, dtype=torch.int32))
+        self.prefix_lengths.copy_(torch.tensor(rows, dtype=torch.int32))
+
+    def open(self, length):
+        """A place for a sequence of ``length`` tokens (its prompt, whose rows ``prefill`` or ``append`` puts in)."""
+        if not 1 <= length <= self.max_length:
+            raise ValueError(f"PagedDecodeCache.open: length must be in [1, {self.max_length}]")
+        b = self._run(1)
+        self._pages[b] = self._take(-(-length // self.page_size))
+        self._length[b] = int(length)
+        self._write([(b, c, p) for c, p in enumerate(self._pages[b])])
+        self._set_lengths([b])
+        return b
+
+    def fork(self, place, copies):
+        """``copies`` consecutive places that go on from ``place`` as it is now, and share its whole pages; the rows of
+        a last page that is partly filled are copied. Call it between steps. Returns the places."""
+        pages, length = self._pages[place], self._length[place]
+        if pages is None or copies < 1:
+            raise ValueError("PagedDecodeCache.fork: place must be open and copies positive")
+        whole = length // self.page_size
+        first = self._run(copies)
+        rest = length % self.page_size > 0
+        own = self._take(copies * rest)
+        entries = []
+        for i in range(copies):
+            mine = pages[:whole] + own[i:i + rest]
+            for p in pages[:whole]:
+                self._users[p] += 1
+            self._pages[first + i], self._length[first + i] = mine, length
+            entries += [(first + i, c, p) for c, p in enumerate(mine)]
+        if rest:
+            at = torch.tensor(own, dtype=torch.int64).to(self.device)
+            for t in (self._k, self._v):
+                t[:, at] = t[:, pages[whole]].clone().unsqueeze(1)
+        self._write(entries)
+        places = list(range(first, first + copies))
+        self._set_lengths(places)
+        if copies > 1 and whole:
+            self._groups[first] = (copies, whole * self.page_size)
+            self._set_groups()
+        return places
+
+    def close(self, place):
+        """Gives the place and the pages that nobody else has back."""
+        pages = self._pages[place]
+        if pages is None:
+            raise ValueError("PagedDecodeCache.close: place is not open")
+        for p in pages:
+            self._users[p] -= 1
+            if self._users[p] == 0:
+                self._free.append(p)
+        self._pages[place], self._length[place] = None, 0
+        self._set_lengths([place])
+        for b, (n, shared) in list(self._groups.items()):
+            if b <= place < b + n:
+                # the places on either side go on as groups; this one is for anybody now
+                del self._groups[b]
+                for first, count in ((b, place - b), (place + 1, b + n - place - 1)):
+                    if count > 1:
+                        self._groups[first] = (count, shared)
+                self._set_groups()
+
+    def advance(self):
+        """Room for one more token in every open sequence; raises ``lengths`` by it."""
+        new = []
+        grow = [b for b in range(self.places) if self._pages[b] is not None]
+        if any(self._length[b] >= self.max_length for b in grow):
+            raise RuntimeError(f"PagedDecodeCache: a sequence has {self.max_length} tokens already")
+        need = [b for b in grow if self._length[b] % self.page_size == 0]
+        for b, p in zip(need, self._take(len(need))):
+            new.append((b, len(self._pages[b]), p))
+            self._pages[b].append(p)
+        for b in grow:
+            self._length[b] += 1
+        self._write(new)
+        self.lengths.add_(self._open)
+
+    # ------------------------------------------------------------------ on the device
+    def _workspace(self):
+        """This cache's own scratch, of one size for its life: a captured step uses it."""
+        if self._ws is None:
+            with torch.cuda.device(self.device):
+                n = ops.paged_attention_workspace(self.max_tokens, self.places, self.q_heads, self.kv_heads, self.head_dim,
+                                                  self.places)
+            self._ws = torch.zeros(n, dtype=torch.uint8, device=self.device)
+        return self._ws
+
+    def prefill(self, layer, places, q, k, v, cu_seqlens, cos=None, sin=None, out=None, sm_scale=None):
+        """Prompts, or the last tokens of them, of the sequences at ``places`` (a list): rows q [T, Hq, d], k / v [T,
+        Hkv, d] packed by ``cu_seqlens`` (int32 on the device) go into the pages (rotated with cos / sin, see
+        ``ops.paged_append``) and attend over everything before them. T is at most ``max_tokens``. Returns [T, Hq, d]."""
+        if q.shape[0] > self.max_tokens:
+            raise ValueError(f"PagedDecodeCache.prefill: {q.shape[0]} tokens, made for at most {self.max_tokens}")
+        at = torch.tensor(places, dtype=torch.int64).to(self.device)
+        table, lengths = self.page_table[at], self.lengths[at]
+        turned = ops.paged_append(k, v, self.pools[layer], table, lengths, cu_seqlens=cu_seqlens, cos=cos, sin=sin,
+                                  q=None if cos is None else q, err=self.err)
+        return ops.flash_paged(q if cos is None else turned, self.pools[layer], table, lengths, cu_seqlens, out=out,
+                               sm_scale=sm_scale, workspace=self._workspace())
+
+    def step(self, layer, q, k_new, v_new, cos=None, sin=None, out=None, sm_scale=None):
+        """One layer's token of every place: q [places, Hq, d], k_new / v_new [places, Hkv, d], after ``advance``."""
+        turned = ops.paged_append(k_new, v_new, self.pools[layer], self.page_table, self.lengths, cos=cos, sin=sin,
+                                  q=None if cos is None else q, err=self.err)
+        return ops.decode_attention_paged(
+            q if cos is None else turned, self.pools[layer], self.page_table, self.lengths, prefix_cu=self.prefix_cu,
+            prefix_lengths=self.prefix_lengths, out=out, sm_scale=sm_scale, workspace=self._workspace())
+
+    def capture_step(self, q, k_new, v_new, out, cos=None, sin=None):
+        """One step over every layer in a CUDA graph: q / out [layers, places, Hq, d], k_new / v_new [layers, places,
+        Hkv, d] are static device buffers. Replay it after ``advance``."""
+        self._workspace()
+        s = torch.cuda.Stream(self.device)
+        s.wait_stream(torch.cuda.current_stream(self.device))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            for layer in range(self.num_layers):
+                self.step(layer, q[layer], k_new[layer], v_new[layer], cos, sin, out[layer])
+        torch.cuda.current_stream(self.device).wait_stream(s)
+        return g
+
+    def workspace_error(self):
+        """Reads and clears the attention calls' error word (a synchronising call)."""
+        import ctypes
+        ws, code = self._workspace(), ctypes.c_int(0)
+        L.check(L.load().dab_workspace_error(L.ptr(ws), ctypes.byref(code), L.stream_of(ws)), "workspace_error")
+        return code.value

@@ -479,3 +479,301 @@ def test_empty_calls(ops):
     assert ops.flash_paged(z, pool.kv, pool.table, pool.lengths, starts([0])).shape == (0, 2, 64)
     assert ops.decode_attention_paged(z, pool.kv, pool.table[:0], none).shape == (0, 2, 64)
     assert ops.paged_append(zk, zk, pool.kv, pool.table[:0], none) is None
+
+
+def test_decode_matches_itself_in_any_grouping_sizes():
+    """The workspace covers every grouping of a batch, and never shrinks with more of it."""
+    lib = L.load()
+    size = lib.dab_paged_attention_workspace_size
+    assert size(5, 5, 2, 4, 64, 5) >= size(5, 5, 2, 4, 64, 0) > 0
+    assert size(600, 5, 2, 4, 64, 0) >= size(5, 5, 2, 4, 64, 0)
+    assert size(5, 5, 2, 129, 64, 0) == 0 and size(-1, 5, 2, 4, 64, 0) == 0
+
+
+# ------------------------------------------------------------------------------------ more edges
+@gpu
+def test_members_shorter_than_their_prefix(ops):
+    """Members that end inside the shared rows, the first one among them; and no member that has all of them."""
+    for lens in ([100, 300, 0, 290, 256], [100, 0, 37, 200]):
+        pool = Pool(ops, len(lens), 2, 128, 16, lens, "bf16", 21, share=256)
+        q = torch.randn(len(lens), 8, 128).bfloat16().cuda()
+        cu = torch.tensor([0, len(lens)], dtype=torch.int32).cuda()
+        n = torch.tensor([256], dtype=torch.int32).cuda()
+        out = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, prefix_cu=cu, prefix_lengths=n)
+        for b, m in enumerate(lens):
+            k, v = pool.rows(b)
+            check(out[b:b + 1], attend64(q[b:b + 1], k, v, [m], 128 ** -0.5), pool.v)
+
+
+@gpu
+@pytest.mark.parametrize("Hq,H,D,dt", [(9, 1, 64, "bf16"), (32, 2, 128, "fp16"), (64, 1, 128, "bf16"), (12, 4, 128, "bf16")])
+def test_decode_many_query_heads(ops, Hq, H, D, dt):
+    """More than 8 query heads per K / V head take another path than up to 8; with and without a prefix."""
+    lens = [700, 513, 40, 1000]
+    pool = Pool(ops, 4, H, D, 32, lens, dt, 22, share=512)
+    q = (2 * torch.randn(4, Hq, D)).to(DT[dt]).cuda()
+    cu = torch.tensor([0, 2, 4], dtype=torch.int32).cuda()
+    n = torch.tensor([512, 512], dtype=torch.int32).cuda()
+    for kw in ({}, dict(prefix_cu=cu, prefix_lengths=n)):
+        out = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, **kw)
+        for b, m in enumerate(lens):
+            k, v = pool.rows(b)
+            check(out[b:b + 1], attend64(q[b:b + 1], k, v, [m], D ** -0.5), pool.v)
+
+
+@gpu
+@pytest.mark.parametrize("D,dt", [(64, "fp16"), (128, "bf16")])
+def test_decode_with_rising_scores(ops, D, dt):
+    """Scores that grow along the keys move the references of both kinds of pieces, by a little and by a lot."""
+    lens = [1500] * 40
+    pool = Pool(ops, 40, 1, D, 64, lens, dt, 23, share=640)
+    q = torch.ones(40, 4, D).to(DT[dt]).cuda()
+    cu = torch.tensor([0, 20], dtype=torch.int32).cuda()
+    n = torch.tensor([640], dtype=torch.int32).cuda()
+    for step in (0.002, 0.03, -0.03):
+        for b in range(40):
+            p = torch.arange(1500)
+            page, row = pool.table[b].cpu().long()[p // 64].cuda(), (p % 64).cuda()
+            pool.k[page, :, row] = (step * p.cuda().float())[:, None, None].to(DT[dt]).expand(-1, 1, D)
+        out = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, prefix_cu=cu, prefix_lengths=n)
+        for b in (0, 19, 20, 39):
+            k, v = pool.rows(b)
+            # scores of up to 45 * sqrt(128) = 509 in 32-bit sums: off by 2^-24 * 509 * 8, 2^-12 of a weight; the check's
+            # 2^-13 max|v| and the unit roundoffs leave that much room (weights sum to one, values to half of max|v|)
+            check(out[b:b + 1], attend64(q[b:b + 1], k, v, [1500], D ** -0.5), pool.v)
+
+
+@gpu
+def test_non_finite_rows_stay_with_those_who_see_them(ops):
+    """A NaN in one sequence's own rows, and one in shared rows past a member's length, reach nobody else."""
+    lens = [300, 290, 100]
+    pool = Pool(ops, 3, 1, 64, 32, lens, "bf16", 24, share=256)
+    q = torch.randn(3, 4, 64).bfloat16().cuda()
+    cu = torch.tensor([0, 3], dtype=torch.int32).cuda()
+    n = torch.tensor([256], dtype=torch.int32).cuda()
+    ref = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, prefix_cu=cu, prefix_lengths=n)
+    pool.k[pool.table[0, 9].long(), :, 2] = float("nan")  # row 290 of the first
+    out = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, prefix_cu=cu, prefix_lengths=n)
+    assert out[0].isnan().all() and torch.equal(out[1:], ref[1:])
+
+
+@gpu
+def test_calls_on_streams_and_in_graphs(ops):
+    """Calls on two streams at once, and captured ones replayed with new contents of the same tensors, give what
+    eager calls give; a captured call leaves its workspace fit for the next."""
+    pool = Pool(ops, 6, 2, 128, 16, [900, 40, 700, 0, 333, 512], "bf16", 25, share=0)
+    pool2 = Pool(ops, 3, 2, 128, 16, [2000, 100, 1500], "bf16", 26)
+    q = torch.randn(6, 8, 128).bfloat16().cuda()
+    q2 = torch.randn(300, 8, 128).bfloat16().cuda()
+    cu2 = starts([100, 60, 140])
+    ref = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths)
+    ref2 = ops.flash_paged(q2, pool2.kv, pool2.table, pool2.lengths, cu2)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(s1):
+            a = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths)
+        with torch.cuda.stream(s2):
+            b = ops.flash_paged(q2, pool2.kv, pool2.table, pool2.lengths, cu2)
+        got.append((a, b))
+    torch.cuda.synchronize()
+    for a, b in got:
+        assert torch.equal(a, ref) and torch.equal(b, ref2)
+    ws = torch.zeros(ops.paged_attention_workspace(300, 6, 8, 2, 128), dtype=torch.uint8, device="cuda")
+    out, out2 = torch.empty_like(q), torch.empty_like(q2)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s1):
+        ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, out=out, workspace=ws)
+        ops.flash_paged(q2, pool2.kv, pool2.table, pool2.lengths, cu2, out=out2, workspace=ws)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref) and torch.equal(out2, ref2)
+    # other lengths and rows in the same tensors
+    pool.lengths.copy_(torch.tensor([33, 900, 0, 128, 500, 1], dtype=torch.int32))
+    q.copy_(torch.randn_like(q))
+    cu2.copy_(starts([10, 0, 250]))
+    want = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths)
+    want2 = ops.flash_paged(q2, pool2.kv, pool2.table, pool2.lengths, cu2)
+    for _ in range(3):
+        out.zero_()
+        out2.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(out2[:260], want2[:260]) and (out2[260:] == 0).all()
+    assert int(ws[:4].view(torch.int32)) == 0
+
+
+@gpu
+def test_prompts_cut_and_whole_agree(ops):
+    """The same sequences in a small call, whose units are cut into chunks, and in a large one, where they stay whole."""
+    g = torch.Generator().manual_seed(27)
+    n = [700, 64, 1, 400]
+    many = n + [300] * 60
+    q, k, v = (torch.randn(sum(many), h, 128, generator=g).bfloat16().cuda() for h in (8, 2, 2))
+    big = ops.flash_varlen(q, k, v, starts(many))
+    T = sum(n)
+    small = ops.flash_varlen(q[:T], k[:T], v[:T], starts(n))
+    # each is within one rounding of the output and the weights' 16 bits of the formula
+    tol = 2 * (2 * UNIT[torch.bfloat16] + 2.0 ** -13) * v.float().abs().max().item()
+    assert (big[:T].float() - small.float()).abs().max().item() <= tol
+    at = 0
+    for m in n:
+        check(small[at:at + m], attend64(q[at:at + m], k[at:at + m], v[at:at + m], torch.arange(1, m + 1), 128 ** -0.5), v)
+        at += m
+
+
+@gpu
+def test_long_cache_offsets(ops):
+    """Pages whose element offsets pass 2^31: rows there are written and read in place."""
+    H, D, ps = 8, 128, 64
+    P = (1 << 31) // (H * D * ps) + 40  # about 2^31 elements, 4.3 GB for K and as much for V
+    kv = ops.PagedKV.empty(P, H, ps, D, torch.bfloat16, "cuda")
+    lens = [150, 97]
+    table = torch.tensor([[P - 1, 0, P - 3], [P - 2, P - 9, 1]], dtype=torch.int32).cuda()
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    g = torch.Generator().manual_seed(28)
+    x, y = (torch.randn(sum(lens), H, D, generator=g).bfloat16().cuda() for _ in range(2))
+    ops.paged_append(x, y, kv, table, n, cu_seqlens=starts(lens))
+    q = torch.randn(2, 32, D, generator=g).bfloat16().cuda()
+    out = ops.decode_attention_paged(q, kv, table, n)
+    at = 0
+    for b, m in enumerate(lens):
+        check(out[b:b + 1], attend64(q[b:b + 1], x[at:at + m], y[at:at + m], [m], D ** -0.5), y)
+        at += m
+    qq = torch.randn(sum(lens), 8, D, generator=g).bfloat16().cuda()
+    assert torch.equal(ops.flash_paged(qq, kv, table, n, starts(lens)), ops.flash_varlen(qq, x, y, starts(lens)))
+
+
+# ------------------------------------------------------------------------------------ the cache
+def test_cache_bookkeeping():
+    """Pages, places and groups, on the host alone."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    c = PagedDecodeCache(2, 6, 4, 2, 64, 12, 16, 64, device="cpu")
+    a = c.open(40)
+    assert a == 0 and c.lengths.tolist() == [40, 0, 0, 0, 0, 0] and len(c._free) == 9
+    c._k[:, c._pages[0][2]] = 3.0
+    f = c.fork(a, 4)
+    assert f == [1, 2, 3, 4] and len(c._free) == 5  # a page each for the partly filled one
+    assert all(c._pages[b][:2] == c._pages[0][:2] for b in f) and len({c._pages[b][2] for b in f}) == 4
+    assert all((c._k[:, c._pages[b][2]] == 3).all() for b in f)
+    assert c.prefix_cu.tolist() == [0, 1, 5, 5, 5, 5, 5] and c.prefix_lengths.tolist()[:2] == [0, 32]
+    assert c.page_table[2, :3].tolist() == c._pages[2]
+    c.close(a)
+    assert c._users[c._pages[1][0]] == 4 and len(c._free) == 6
+    c.close(2)  # the group splits, and the place is anybody's
+    assert c._groups == {3: (2, 32)} and c.prefix_cu.tolist()[:3] == [0, 3, 5]
+    b = c.open(16)
+    assert b == 0
+    assert c.open(16) == 2 and c.prefix_cu.tolist()[:3] == [0, 3, 5]
+    before = len(c._free)
+    c.advance()
+    assert c.lengths.tolist() == [17, 41, 17, 41, 41, 0] and len(c._free) == before - 2
+    with pytest.raises(RuntimeError, match="free"):
+        c.open(64)
+    with pytest.raises(RuntimeError, match="consecutive"):
+        c.fork(0, 2)
+    with pytest.raises(ValueError):
+        c.open(65)
+    with pytest.raises(ValueError):
+        c.close(5)
+    for _ in range(7):
+        c.advance()
+    assert len(c._free) == 3 and c.open(16) == 5
+    with pytest.raises(RuntimeError, match="wanted"):
+        c.advance()  # 4 sequences are at a page's end, 2 pages are free
+    assert c.lengths.tolist() == [24, 48, 24, 48, 48, 16]
+    for x in (0, 1, 2, 3, 4, 5):
+        c.close(x)
+    assert sorted(c._free) == list(range(12)) and not c._groups and c.lengths.sum() == 0
+    for bad in (dict(head_dim=32), dict(page_size=8), dict(q_heads=3), dict(num_pages=0)):
+        with pytest.raises(ValueError):
+            PagedDecodeCache(**{**dict(num_layers=1, places=2, q_heads=4, kv_heads=2, head_dim=64, num_pages=2, page_size=16,
+                                       max_length=64, device="cpu"), **bad})
+
+
+@gpu
+@pytest.mark.parametrize("dt,D,ps", [("bf16", 128, 16), ("fp16", 64, 32)])
+def test_cache_end_to_end(ops, dt, D, ps):
+    """Prompts of different lengths, answers that share one, eager and captured steps, places that close and are taken
+    again: every output against the formula over the rows that a plain list of them holds."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    layers, places, Hq, H, dtype, u = 2, 7, 8, 2, DT[dt], UNIT[DT[dt]]
+    g = torch.Generator().manual_seed(30)
+    c = PagedDecodeCache(layers, places, Hq, H, D, 80, ps, 300, dtype=dtype, max_tokens=400)
+    pos = torch.arange(300).double()[:, None] * 1e4 ** (-torch.arange(0, D, 2).double() / D)
+    cos, sin = (torch.cat([f(pos), f(pos)], 1).float().cuda() for f in (torch.cos, torch.sin))
+    held = [{} for _ in range(layers)]  # per layer, place -> (rotated K rows, V rows), as rounded in the cache
+
+    def rows(n, h):
+        return torch.randn(n, h, D, generator=g).to(dtype)
+
+    def turned(x, p):
+        """In 64 bits, rounded to the cache's type (a double's two roundings meet fp32's only at ties)."""
+        return rotate64(x.double(), cos.cpu().double()[p], sin.cpu().double()[p]).to(dtype)
+
+    def agree(out, qt, k, v, see):
+        # An element whose rotation lies within fp32's error of a tie (2^-22 of it; one in 2^13 to 2^10) may be rounded the
+        # other way here: that moves its score by 2 u |q k| / sqrt(D), u / 4 of a weight for |q k| = 1 at D = 64. Two
+        # such elements in a row's largest weights: u / 2.
+        ref = attend64(qt, k, v, see, D ** -0.5)
+        tol = (2 * u + 2.0 ** -13 + 0.5 * u) * v.float().abs().max().item()
+        assert (out.cpu().double() - ref).abs().max().item() <= tol
+
+    def prefill(places_, news):
+        cu = starts(news)
+        for layer in range(layers):
+            q, k, v = rows(sum(news), Hq), rows(sum(news), H), rows(sum(news), H)
+            out = c.prefill(layer, places_, q.cuda(), k.cuda(), v.cuda(), cu, cos, sin)
+            at = 0
+            for b, m in zip(places_, news):
+                old = c._length[b] - m
+                p = torch.arange(old, old + m)
+                k0, v0 = held[layer].get(b, (k[:0], v[:0]))
+                kk, vv = torch.cat([k0[:old], turned(k[at:at + m], p)]), torch.cat([v0[:old], v[at:at + m]])
+                held[layer][b] = kk, vv
+                agree(out[at:at + m], turned(q[at:at + m], p), kk, vv, old + torch.arange(1, m + 1))
+                at += m
+
+    a, b = c.open(75), c.open(2 * ps)
+    prefill([a, b], [75, 2 * ps])
+    f = c.fork(a, 3)
+    for layer in range(layers):
+        for x in f:
+            held[layer][x] = held[layer][a]
+    q, k, v = (torch.zeros(layers, places, h, D, dtype=dtype, device="cuda") for h in (Hq, H, H))
+    out = torch.zeros_like(q)
+    graph = None
+    for step in range(24):
+        if step == 6:
+            c.close(f[1])
+            d = c.open(50)
+            assert d == f[1]  # the middle of the group is taken by another sequence
+            prefill([d], [50])
+        if step == 9:
+            c.close(b)
+        c.advance()
+        qs, ks, vs = rows(layers * places, Hq), rows(layers * places, H), rows(layers * places, H)
+        for t, x in ((q, qs), (k, ks), (v, vs)):
+            t.copy_(x.view(t.shape))
+        out.fill_(7)
+        if step < 3:
+            for layer in range(layers):
+                c.step(layer, q[layer], k[layer], v[layer], cos, sin, out[layer])
+        else:
+            if graph is None:
+                graph = c.capture_step(q, k, v, out, cos, sin)
+            graph.replay()
+        for layer in range(layers):
+            for x in range(places):
+                n = c._length[x]
+                if n == 0:
+                    assert (out[layer, x] == 0).all()
+                    continue
+                p = torch.tensor([n - 1])
+                i = layer * places + x
+                kk, vv = held[layer][x]
+                kk, vv = torch.cat([kk[:n - 1], turned(ks[i:i + 1], p)]), torch.cat([vv[:n - 1], vs[i:i + 1]])
+                held[layer][x] = kk, vv
+                agree(out[layer, x:x + 1], turned(qs[i:i + 1], p), kk, vv, [n])
+    assert int(c.err) == 0 and c.workspace_error() == 0
