@@ -40,8 +40,8 @@ constexpr int PT_THIN = 8;  // most rows of a thin piece (its products are compu
 constexpr int PT_CHUNKS = 16;     // most chunks that a prompt's mean unit is cut into
 constexpr int PT_MIN_CHUNK = 2;
 constexpr int PT_FILL = 7;        // most chunks per SM: they bound the workspace
-constexpr int PT_PIECE = 2;
-constexpr int PT_JOIN = 3;
+constexpr int PT_PIECE = 5;       // what beginning and ending a piece costs, in key tiles of a pair
+constexpr int PT_JOIN = 3;        // and the joining kernel, with 3 / 100 for every piece
 
 // A CTA's part of a decode step: costs [begin, end), its place among the CTAs in their order, its first item and what
 // lies before that. Of prompts only `item` is used, the key tiles of a chunk.
@@ -241,7 +241,7 @@ __device__ __noinline__ Seq prompt_seq(const PagedAttn& p, int utok, int b) {
   return s;
 }
 // Key tiles of a chunk, or 0 where units stay whole: of the ways to cut the mean unit into 1 to 16 chunks, the one
-// with the least rounds of pieces times their length. A piece costs PT_PIECE key tiles beside its own.
+// with the least rounds of pieces times their length, joining counted.
 __device__ __forceinline__ int chunk_tiles(const PagedAttn& p, int64_t units, int64_t tiles) {
   if (!p.may_split || units == 0 || units >= 2 * static_cast<int64_t>(p.num_ctas)) return 0;
   const unsigned n = static_cast<unsigned>(units), mean = static_cast<unsigned>(quotient(tiles + units - 1, units));
@@ -249,8 +249,8 @@ __device__ __forceinline__ int chunk_tiles(const PagedAttn& p, int64_t units, in
   unsigned best = 0, least = 0xFFFFFFFFu;
 #pragma unroll 1
   for (unsigned k = 1; k <= PT_CHUNKS && (k == 1 || (mean >= PT_MIN_CHUNK * k && n * k <= PT_FILL * ctas)); ++k) {
-    // one chunk needs no joining, which costs some tiles' time as well
-    const unsigned len = (mean + k - 1) / k, cost = (n * k + ctas - 1) / ctas * (len + PT_PIECE) + (k > 1 ? PT_JOIN : 0);
+    const unsigned len = (mean + k - 1) / k;
+    const unsigned cost = (n * k + ctas - 1) / ctas * (len + PT_PIECE) + (k > 1 ? PT_JOIN + n * k * 3 / 100 : 0);
     if (cost < least) {
       least = cost;
       best = k == 1 ? 0 : len;
