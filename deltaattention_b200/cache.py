@@ -320,7 +320,8 @@ class PagedDecodeCache:
     A sequence has a place in the batch, [0, places). ``open`` takes one for a prompt, ``fork`` takes consecutive
     ones for sequences that go on from it: these hold its whole pages in common and are a group, whose shared rows
     every step reads once for all. ``advance`` makes room for one more token in every open sequence and raises the
-    ``lengths``; ``step`` then runs one layer. Places that are not open have length 0: a step's q, k and v rows for
+    ``lengths``; ``step`` then runs one layer. ``extend`` makes room for many tokens of one sequence (the next turn of a
+    conversation, the next piece of a prompt), which ``prefill`` puts in. Places that are not open have length 0: a step's q, k and v rows for
     them are not looked at, and their outputs are 0.
 
     The bookkeeping of pages is the host's (``open``, ``fork``, ``advance``, ``close``); ``page_table`` [places,
@@ -336,8 +337,9 @@ class PagedDecodeCache:
             raise ValueError("PagedDecodeCache: bf16 / fp16 and head_dim 64 / 128 only")
         if page_size not in (16, 32, 64, 128, 256):
             raise ValueError("PagedDecodeCache: page_size must be 16, 32, 64, 128 or 256")
-        if min(num_layers, places, kv_heads, num_pages, max_length) < 1 or q_heads < 1 or q_heads % kv_heads:
-            raise ValueError("PagedDecodeCache: sizes must be positive, and q_heads a multiple of kv_heads")
+        if min(num_layers, places, kv_heads, num_pages, max_length) < 1 or q_heads < 1 or q_heads % kv_heads or \
+                q_heads > 128 * kv_heads:
+            raise ValueError("PagedDecodeCache: sizes must be positive, and q_heads a multiple of kv_heads (at most 128 of each)")
         self.num_layers, self.places, self.page_size = num_layers, places, page_size
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.num_pages, self.max_pages, self.max_length = num_pages, -(-max_length // page_size), max_length
@@ -366,6 +368,10 @@ class PagedDecodeCache:
         for p in got:
             self._users[p] = 1
         return got
+
+    def _opened(self, what, place):
+        if not 0 <= place < self.places or self._pages[place] is None:
+            raise ValueError(f"PagedDecodeCache.{what}: place {place} is not open")
 
     def _run(self, n):
         """The first of n consecutive free places."""
@@ -418,9 +424,10 @@ class PagedDecodeCache:
     def fork(self, place, copies):
         """``copies`` consecutive places that go on from ``place`` as it is now, and share its whole pages; the rows of
         a last page that is partly filled are copied. Call it between steps. Returns the places."""
+        self._opened("fork", place)
+        if copies < 1:
+            raise ValueError("PagedDecodeCache.fork: copies must be positive")
         pages, length = self._pages[place], self._length[place]
-        if pages is None or copies < 1:
-            raise ValueError("PagedDecodeCache.fork: place must be open and copies positive")
         whole = length // self.page_size
         first = self._run(copies)
         rest = length % self.page_size > 0
@@ -444,12 +451,22 @@ class PagedDecodeCache:
             self._set_groups()
         return places
 
+    def extend(self, place, tokens):
+        """Room for ``tokens`` more rows of the sequence at ``place``; raises its length by them."""
+        self._opened("extend", place)
+        pages, length = self._pages[place], self._length[place] + int(tokens)
+        if tokens < 1 or length > self.max_length:
+            raise ValueError(f"PagedDecodeCache.extend: tokens must be positive and the length at most {self.max_length}")
+        new = self._take(-(-length // self.page_size) - len(pages))
+        self._write([(place, len(pages) + i, p) for i, p in enumerate(new)])
+        pages += new
+        self._length[place] = length
+        self._set_lengths([place])
+
     def close(self, place):
         """Gives the place and the pages that nobody else has back."""
-        pages = self._pages[place]
-        if pages is None:
-            raise ValueError("PagedDecodeCache.close: place is not open")
-        for p in pages:
+        self._opened("close", place)
+        for p in self._pages[place]:
             self._users[p] -= 1
             if self._users[p] == 0:
                 self._free.append(p)
@@ -492,9 +509,14 @@ class PagedDecodeCache:
     def prefill(self, layer, places, q, k, v, cu_seqlens, cos=None, sin=None, out=None, sm_scale=None):
         """Prompts, or the last tokens of them, of the sequences at ``places`` (a list): rows q [T, Hq, d], k / v [T,
         Hkv, d] packed by ``cu_seqlens`` (int32 on the device) go into the pages (rotated with cos / sin, see
-        ``ops.paged_append``) and attend over everything before them. T is at most ``max_tokens``. Returns [T, Hq, d]."""
+        ``ops.paged_append``) and attend over everything before them. T is at most ``max_tokens``. Rows that lie in pages
+        shared with forks are written for all of these. Returns [T, Hq, d]."""
         if q.shape[0] > self.max_tokens:
             raise ValueError(f"PagedDecodeCache.prefill: {q.shape[0]} tokens, made for at most {self.max_tokens}")
+        for b in places:
+            self._opened("prefill", b)
+        if len(set(places)) != len(places):
+            raise ValueError("PagedDecodeCache.prefill: a place is given twice")
         at = torch.tensor(places, dtype=torch.int64).to(self.device)
         table, lengths = self.page_table[at], self.lengths[at]
         turned = ops.paged_append(k, v, self.pools[layer], table, lengths, cu_seqlens=cu_seqlens, cos=cos, sin=sin,

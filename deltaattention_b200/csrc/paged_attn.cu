@@ -13,17 +13,27 @@
 //   own       one token of one sequence over the rows behind its prefix: G rows. Bytes bound it. Up to 8 rows are
 //             computed transposed (thin): S^T = K Q^T has a key per row and 8 columns, which takes a warp a tenth
 //             of the time of 128 columns; the two tiles take every other key tile, two chains at a time.
-// With `decode` the key tiles of all units, one after the other, are cut into one even range per CTA
-// (bytes and, for tiles of 256 rows, products cost the same per tile). Prompts take pieces from a counter,
-// heavy ones first; where whole units would leave SMs idle they are cut into chunks of L key tiles, the
+// A decode step's units, one after the other, are cut into even ranges of cost, one per CTA. Prompts take pieces
+// from a counter, heavy ones first; where whole units would leave SMs idle they are cut into chunks of key tiles, the
 // units of one chunk next to each other so that they find its keys in L2. Pieces of cut units leave fp32
-// partial sums with their maxima, joined by a second kernel.
+// partial sums with their maxima, joined by a second kernel that is launched early (programmatic dependent launch).
 //
 // One persistent CTA per SM, 384 threads: warp 0 fetches pieces, publishes them to all other warps and
 // loads Q and K; warp 3 loads V; warps 1 and 2 issue the products of the two tiles; warps 4-7 and 8-11 are
 // the tiles' softmax, a row per thread. The loads are TMA boxes of a page (or of 128 packed rows), scores
 // and weights live in TMEM, weights in the rows' 16-bit type: an error of half a step per weight, as large as
 // that of the rounded output. The running maximum moves only when a row outgrows it by 2^8.
+//
+// Measured (device time, 32 q-heads on 8 K / V heads of 128, bf16; floors at 6550 GB/s and 1680 TFLOP/s):
+//   prompt of 32768 tokens            7.75 ms, 1135 TFLOP/s (floor 5.24): a pair of tiles over 128 keys takes 3300 cycles
+//     at the 1.5 GHz that the power limit leaves, of which the tensor pipe is busy for 1700. What it waits for is
+//     each tile's chain of scores, softmax (1700 cycles) and P V; two chains alternate. Scoring a tile in two halves
+//     to shorten the chain (13 % slower), exponentials in part as polynomials (4 % slower), fewer issue
+//     instructions and an earlier change of turns (no gain) did not help.
+//   16 sequences of 32000 rows        310 us, 6.8 TB/s (floor 320); 48 of 500 to 12000: 200 us (floor 185)
+//   64 sequences, 32000 rows shared and up to 1000 own: 84 us (floor 40). Neither bytes (38 % of nominal) nor products (19 %)
+//     fill it: the prefix's CTAs are bound by the chain above, and beginning and joining the pieces is a fifth
+//   1 sequence of 1900 rows (d 64)    17 us: two launches, each a chain of reads, code that is fetched, one key tile
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -36,12 +46,12 @@ constexpr int PT_THREADS = 384;
 constexpr int PT_BN = 128;   // keys of a tile
 constexpr int PT_RING = 4;   // pieces published ahead
 constexpr int PT_ROWS = 256; // partial rows between the pieces of neighbouring CTAs
-constexpr int PT_THIN = 8;  // most rows of a thin piece (its products are computed for 16)
-constexpr int PT_CHUNKS = 16;     // most chunks that a prompt's mean unit is cut into
+constexpr int PT_THIN = 8;   // most rows of a thin piece (its products are computed for 16)
+constexpr int PT_CHUNKS = 16;   // most chunks that a prompt's mean unit is cut into, of PT_MIN_CHUNK key tiles at least
 constexpr int PT_MIN_CHUNK = 2;
-constexpr int PT_FILL = 7;        // most chunks per SM: they bound the workspace
-constexpr int PT_PIECE = 5;       // what beginning and ending a piece costs, in key tiles of a pair
-constexpr int PT_JOIN = 3;        // and the joining kernel, with 3 / 100 for every piece
+constexpr int PT_FILL = 7;      // most chunks per SM: they bound the workspace
+constexpr int PT_PIECE = 5;     // what beginning and ending a piece costs, in key tiles of a pair
+constexpr int PT_JOIN = 3;      // and the joining kernel, with 3 / 100 for every piece
 
 // A CTA's part of a decode step: costs [begin, end), its place among the CTAs in their order, its first item and what
 // lies before that. Of prompts only `item` is used, the key tiles of a chunk.
@@ -80,7 +90,8 @@ template <int D> struct PtCfg {
   static constexpr int OFF_V = OFF_K + NK * KVBYTES;
   static constexpr int EPI_PITCH = 80;  // 64 bytes of a row's output and 16 more against bank conflicts
   static constexpr int OFF_EPI = OFF_V + NV * KVBYTES;
-  static constexpr int OFF_P = OFF_EPI + 8 * 32 * EPI_PITCH;  // weights of thin pieces, [2][16 rows x 128 keys], rows from PT_THIN on unused
+  // weights of thin pieces, [2][16 rows x 128 keys], rows from PT_THIN on unused
+  static constexpr int OFF_P = OFF_EPI + 8 * 32 * EPI_PITCH;
   static constexpr int PBYTES = 16 * PT_BN * 2;
   static constexpr int OFF_VOTE = OFF_P + 2 * PBYTES;  // [2 tiles][2][4 warps][PT_THIN] maxima, then flags
   static constexpr int OFF_X = OFF_VOTE + 2 * 2 * 4 * (PT_THIN + 1) * 4;  // thin: tile 1's O^T, maxima and sums
@@ -144,9 +155,9 @@ struct Item {
 };
 // The CTAs of a decode step: the first n[0] share the prefixes' costs, n[1] after them the own rows'. In each part the
 // dearest key tile at least for every CTA, so that one whose range lies inside a unit has one of its tiles. The first
-// part is even: products bound the prefixes of many sequences and bytes the own rows, and two neighbours on the chip
-// that do one each both run at a third of their speed (64 sequences over 32000 shared rows: 120 us where one
-// pair was mixed, 155 us where all were, .. without).
+// part is even: products bound the prefixes of many sequences and bytes the own rows, and two neighbouring CTAs
+// (two SMs that share a path to memory) that do one each both run at a third of their speed. 64 sequences over 32000
+// shared rows: 155 us where all neighbours were mixed, 120 us where one pair was, 95 us without.
 __device__ __forceinline__ Ctas decode_ctas(const PagedAttn& p, int64_t prefixes, int64_t total) {
   Ctas c;
   c.cost[0] = prefixes;
@@ -1729,7 +1740,9 @@ static cudaError_t launch_paged_t(PagedAttn& p, uint8_t* ws, int sms, cudaStream
   p.part_o = reinterpret_cast<float*>(ws);
   p.may_split = s.split;
   p.num_ctas = sms;
-  // In sixteenths of a microsecond on a full GPU, as measured: ...
+  // Sixteenths of a microsecond with all SMs at work, from traces: 2 to begin and end a unit; 2 for a pair of tiles over
+  // 128 keys of 128 (of 64: 1.5); 1.5 (0.75) for 128 keys of one token, which bytes bound. 1 to 4 for the first and 1.6 to
+  // 2.5 for the second were within 5 % over shared prefixes, or slower.
   p.w_start = 32;
   p.w_pair = D == 128 ? 32 : 24;
   p.w_thin = D == 128 ? 24 : 12;

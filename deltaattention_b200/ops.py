@@ -1227,8 +1227,8 @@ def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, w
 
     q [T, Hq, d], k / v [T, Hkv, d] (bf16 / fp16, d 64 or 128, any token and head strides; q-head h reads kv-head
     h // (Hq / Hkv), at most 128 q-heads per kv-head; sm_scale is positive), cu_seqlens int32 [B + 1] on the device,
-    rising from 0: it is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] from
-    cu_seqlens[B] on are left alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and
+    rising from 0: it is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] (q itself
+    will do) from cu_seqlens[B] on are left alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and
     may reach rows before it within the same 128 keys.
 
     ``workspace`` (uint8, ``paged_attention_workspace`` bytes, zero-filled once, used by one stream at a time)

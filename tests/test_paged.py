@@ -777,3 +777,150 @@ def test_cache_end_to_end(ops, dt, D, ps):
                 held[layer][x] = kk, vv
                 agree(out[layer, x:x + 1], turned(qs[i:i + 1], p), kk, vv, [n])
     assert int(c.err) == 0 and c.workspace_error() == 0
+
+
+# ------------------------------------------------------------------------- calls at the limits of what is allowed
+def test_cache_refuses_wrong_places():
+    """Places are host numbers: closed ones, ones outside the batch and ones given twice are refused before anything
+    is looked up on the device."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    c = PagedDecodeCache(1, 3, 4, 2, 64, 8, 16, 64, device="cpu")
+    a = c.open(20)
+    x = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    for bad in (-1, 1, 3):
+        for call in (lambda: c.close(bad), lambda: c.fork(bad, 1), lambda: c.extend(bad, 1),
+                     lambda: c.prefill(0, [a, bad], x, x[:, :2], x[:, :2], None)):
+            with pytest.raises(ValueError, match="not open"):
+                call()
+    with pytest.raises(ValueError, match="twice"):
+        c.prefill(0, [a, a], x, x[:, :2], x[:, :2], None)
+    for bad in (0, -3, 45):
+        with pytest.raises(ValueError):
+            c.extend(a, bad)
+    assert c.lengths.tolist() == [20, 0, 0] and len(c._free) == 6
+    c.extend(a, 12)  # fills the second page
+    assert c.lengths.tolist() == [32, 0, 0] and len(c._free) == 6
+    c.extend(a, 17)
+    assert c.lengths.tolist() == [49, 0, 0] and len(c._free) == 4 and c.page_table[0].tolist() == c._pages[0]
+    b, d = c.open(48), c.open(16)
+    with pytest.raises(RuntimeError, match="wanted"):
+        c.extend(b, 16)
+    assert c.lengths.tolist() == [49, 48, 16] and (b, d) == (1, 2)
+    with pytest.raises(ValueError):
+        PagedDecodeCache(1, 3, 258, 2, 64, 8, 16, 64, device="cpu")
+
+
+@gpu
+def test_cache_turns_of_a_conversation(ops):
+    """A prompt put in by pieces, and turns of many tokens behind it, one of them of a fork: as one prompt."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    g = torch.Generator().manual_seed(31)
+    c = PagedDecodeCache(1, 4, 8, 2, 64, 64, 16, 400, dtype=torch.float16, max_tokens=200)
+    q, k, v = (torch.randn(360, h, 64, generator=g).half().cuda() for h in (8, 2, 2))
+
+    def piece(place, at, n, q=q, k=k, v=v):
+        s = slice(at, at + n)
+        return c.prefill(0, [place], q[s], k[s], v[s], starts([n]))
+
+    a = c.open(100)
+    out = [piece(a, 0, 100)]
+    c.extend(a, 137)
+    out.append(piece(a, 100, 137))
+    b = c.fork(a, 1)[0]
+    q2, k2, v2 = (torch.randn(360, h, 64, generator=g).half().cuda() for h in (8, 2, 2))
+    c.extend(b, 50)
+    turn = piece(b, 237, 50, q2, k2, v2)
+    c.extend(a, 123)
+    out.append(piece(a, 237, 123))
+    check(torch.cat(out), attend64(q, k, v, torch.arange(1, 361), 64 ** -0.5), v)
+    kb, vb = (torch.cat([x[:237], y[237:287]]) for x, y in ((k, k2), (v, v2)))
+    check(turn, attend64(q2[237:287], kb, vb, torch.arange(238, 288), 64 ** -0.5), vb)
+    assert int(c.err) == 0 and c.workspace_error() == 0
+
+
+@gpu
+def test_groups_that_do_not_rise_are_reported(ops):
+    """Groups out of order or past the batch: the error word says so, and the step goes on without groups."""
+    lens = [300, 290, 100, 280]
+    pool = Pool(ops, 4, 2, 64, 32, lens, "bf16", 32, share=256)
+    q = torch.randn(4, 8, 64).bfloat16().cuda()
+    ref = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths)
+    n = torch.tensor([64, 64], dtype=torch.int32).cuda()
+    for cu in ([0, 3, 2], [0, 2, 5], [-1, 2, 4], [3, 1, 4], [0, 2 ** 31 - 1, 4]):
+        ws = torch.zeros(ops.paged_attention_workspace(4, 4, 8, 2, 64, 2), dtype=torch.uint8, device="cuda")
+        out = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, workspace=ws, prefix_lengths=n,
+                                         prefix_cu=torch.tensor(cu, dtype=torch.int32).cuda())
+        assert int(ws[:4].view(torch.int32)) == 0x604 and torch.equal(out, ref), cu
+    for rows in (-5, 2 ** 31 - 1):  # no rows; more than a table holds, and than any member has
+        n.fill_(rows)
+        pool.table[1:4, :8] = pool.table[0, :8]
+        same = torch.tensor([0, 1, 1], dtype=torch.int32).cuda()
+        out = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, prefix_cu=same, prefix_lengths=n)
+        for b, m in enumerate(lens):
+            k, v = pool.rows(b)
+            check(out[b:b + 1], attend64(q[b:b + 1], k, v, [m], 64 ** -0.5), pool.v)
+
+
+@gpu
+@pytest.mark.parametrize("B,groups", [(5000, 0), (3000, 700)])
+def test_decode_of_thousands_of_sequences(ops, B, groups):
+    """More sequences and groups than a block has threads, many of them empty or of one member."""
+    g = torch.Generator().manual_seed(B)
+    H, D, ps = 1, 64, 16
+    lens = torch.randint(0, 90, (B,), generator=g)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int64), torch.randint(0, B, (groups,), generator=g).sort()[0]]).to(torch.int32)
+    table = torch.randint(0, 4000, (B, 6), generator=g)
+    for a, b in zip(cu[:-1].tolist(), cu[1:].tolist()):
+        table[a:b, :2] = table[a, :2].clone()
+    pages = torch.randn(2, 4000, H, ps, D, generator=g).half()
+    q = torch.randn(B, 2, D, generator=g).half()
+    kw = dict(prefix_cu=cu.cuda(), prefix_lengths=torch.full((groups,), 32, dtype=torch.int32).cuda()) if groups else {}
+    out = ops.decode_attention_paged(q.cuda(), ops.PagedKV(pages[0].cuda(), pages[1].cuda()), table.int().cuda(),
+                                     lens.int().cuda(), **kw)
+    k, v = (x[table].transpose(1, 2).reshape(B, H, 6 * ps, D).double() for x in pages)
+    s = q.double() @ k[:, 0].transpose(1, 2) / 8
+    s = s.masked_fill(torch.arange(6 * ps)[None, None] >= lens[:, None, None], -math.inf)
+    ref = (s.softmax(-1) @ v[:, 0]).nan_to_num(0.0)
+    check(out, ref, v)
+
+
+@gpu
+def test_prompts_by_the_thousand(ops):
+    g = torch.Generator().manual_seed(33)
+    n = torch.randint(0, 5, (3000,), generator=g).tolist()
+    T = sum(n)
+    q, k, v = (torch.randn(T, h, 64, generator=g).half() for h in (3, 1, 1))
+    out = ops.flash_varlen(q.cuda(), k.cuda(), v.cuda(), starts(n)).cpu()
+    own = torch.repeat_interleave(torch.arange(3000), torch.tensor(n))
+    ref = torch.empty(T, 3, 64, dtype=torch.float64)
+    for a in range(0, T, 500):
+        b, lo = min(a + 500, T), max(0, a - 4)
+        see = (own[a:b, None] == own[None, lo:b]) & (torch.arange(lo, b)[None] <= torch.arange(a, b)[:, None])
+        s = torch.einsum("thd,sd->hts", q[a:b].double(), k[lo:b, 0].double()) / 8
+        ref[a:b] = torch.einsum("hts,sd->thd", s.masked_fill(~see, -math.inf).softmax(-1), v[lo:b, 0].double())
+    check(out, ref, v)
+
+
+@gpu
+def test_outputs_over_the_queries(ops):
+    """``out`` may be q itself: every row is read before it is written, whichever parts a unit is cut into."""
+    g = torch.Generator().manual_seed(34)
+    lens = [600, 3000, 0, 512, 700] + [513 + i for i in range(60)]
+    pool = Pool(ops, len(lens), 2, 128, 16, lens, "bf16", 34, share=512)
+    cu = torch.tensor([0, 4, 40], dtype=torch.int32).cuda()
+    n = torch.tensor([512, 512], dtype=torch.int32).cuda()
+    for Hq in (8, 40):
+        q = torch.randn(len(lens), Hq, 128, generator=g).bfloat16().cuda()
+        ref = ops.decode_attention_paged(q, pool.kv, pool.table, pool.lengths, prefix_cu=cu, prefix_lengths=n)
+        for _ in range(5):
+            x = q.clone()
+            ops.decode_attention_paged(x, pool.kv, pool.table, pool.lengths, prefix_cu=cu, prefix_lengths=n, out=x)
+            assert torch.equal(x, ref)
+    for news in ([200, 130, 1], [40] * 150):
+        q, k, v = prompt_inputs(news, 8, 2, 128, "bf16")
+        ref = ops.flash_varlen(q, k, v, starts(news))
+        T = sum(news)
+        for _ in range(5):
+            x = q.clone()
+            ops.flash_varlen(x, k, v, starts(news), out=x)
+            assert torch.equal(x[:T], ref[:T]) and torch.equal(x[T:], q[T:])
