@@ -25,14 +25,17 @@
 // that of the rounded output. The running maximum moves only when a row outgrows it by 2^8.
 //
 // Measured (device time, 32 q-heads on 8 K / V heads of 128, bf16; floors at 6550 GB/s and 1680 TFLOP/s):
-//   prompt of 32768 tokens            7.75 ms, 1135 TFLOP/s (floor 5.24): a pair of tiles over 128 keys takes 3300 cycles
-//     at the 1.5 GHz that the power limit leaves, of which the tensor pipe is busy for 1700. What it waits for is
-//     each tile's chain of scores, softmax (1700 cycles) and P V; two chains alternate. Scoring a tile in two halves
-//     to shorten the chain (13 % slower), exponentials in part as polynomials (4 % slower), fewer issue
-//     instructions and an earlier change of turns (no gain) did not help.
+//   prompt of 32768 tokens            7.8 ms, 1120 TFLOP/s (floor 5.24): a pair of tiles over 128 keys takes 3300 cycles at
+//     the 1.5 GHz that the power limit leaves. Its products take 2050 of the tensor pipe (64 each, measured alone) and its
+//     exponentials 2050 of their units, but neither is what it waits for: that is each tile's chain of scores, softmax (1700
+//     cycles), P V of the last 64 keys and two hand-overs; two chains alternate. Tried: one area of scores for both tiles and
+//     one of weights for each, so that scores are computed a tile ahead (the softmax then holds 128 scores in registers and
+//     takes 2700: 18 % slower); a tile scored in two halves (13 %; products of N = 64 take 60 cycles); exponentials in part
+//     as polynomials (4 %); turns of the products' warps that end before the scores (9 %) or none (12 %); every wait before
+//     the turn, one election for a batch of products (no gain); a single lane for the products' role (12 %)
 //   16 sequences of 32000 rows        310 us, 6.8 TB/s (floor 320); 48 of 500 to 12000: 200 us (floor 185)
 //   64 sequences, 32000 rows shared and up to 1000 own: 84 us (floor 40). Neither bytes (38 % of nominal) nor products (19 %)
-//     fill it: the prefix's CTAs are bound by the chain above, and beginning and joining the pieces is a fifth
+//     fill it: the prefix's CTAs are bound by the chain above, and the join ends 8 us after the last piece
 //   1 sequence of 1900 rows (d 64)    17 us: two launches, each a chain of reads, code that is fetched, one key tile
 #include <algorithm>
 #include <atomic>
@@ -816,7 +819,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     // The warp runs converged and one elected lane issues. Tiles of a pair walk the same key tiles; both
     // warps wait for every fill, in order, and release it, so a slot's two arrivals are of one fill. They issue
     // their batches (a tile's P V and the next one's Q K^T) in turn, tile 0 first, which keeps the two
-    // softmax passes half a period apart. The two of a thin piece go apart: fills of even number are
+    // softmax passes half a period apart; a tile on its own takes no turns (16 x 32 tokens over 4000 rows: 83 -> 77 us).
+    // The two of a thin piece go apart: fills of even number are
     // tile 0's, of odd number tile 1's, and their warp releases them with both arrivals. As the slots of a
     // parity stay with a warp, it sees all of their phases; before a pair's piece, which it walks with the
     // other one, they wait for each other, so that no earlier phase of the other's slots is still open.
@@ -856,7 +860,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         for (int f = q0; f < q0 + nq; ++f) umma_commit(q_empty + (f & 1));
       };
       const int je = pc.jend();
-      const bool mine = x == 0 || pc.thin || pc.ntok > tpt;
+      const bool pair = pc.ntok > tpt;  // (not of thin pieces)
+      const bool mine = x == 0 || pc.thin || pair;
       bool freed = false, o_init = false;
       auto ensure_free = [&]() -> bool {
         if (freed) return true;
@@ -971,7 +976,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           else ok = wait_k(fpos);
           if (!ok) break;
           if (!more) free_q();
-          ok = my_turn();
+          ok = !pair || my_turn();
           if (!ok) break;
           if (before && uses(j - 1)) {
             ok = weigh(fpos - 1);
@@ -982,7 +987,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             if (!ok) break;
             if (uses(j)) issue_S(fpos);
           }
-          end_turn();
+          if (pair) end_turn();
           if (before) umma_commit(v_empty + (fpos - 1) % NV);
           if (more) umma_commit(k_empty + fpos % NK);
         }
