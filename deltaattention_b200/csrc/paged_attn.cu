@@ -31,8 +31,8 @@
 //     cycles), P V of the last 64 keys and two hand-overs; two chains alternate. Tried: one area of scores for both tiles and
 //     one of weights for each, so that scores are computed a tile ahead (the softmax then holds 128 scores in registers and
 //     takes 2700: 18 % slower); a tile scored in two halves (13 %; products of N = 64 take 60 cycles); exponentials in part
-//     as polynomials (4 %); turns of the products' warps that end before the scores (9 %) or none (12 %); every wait before
-//     the turn, one election for a batch of products (no gain); a single lane for the products' role (12 %)
+//     as polynomials (4 %); turns of the products' warps that end before the scores (9 %) or none (12 %); one election for
+//     a batch of products (no gain); a single lane for the products' role (12 %)
 //   16 sequences of 32000 rows        310 us, 6.8 TB/s (floor 320); 48 of 500 to 12000: 200 us (floor 185)
 //   64 sequences, 32000 rows shared and up to 1000 own: 84 us (floor 40). Neither bytes (38 % of nominal) nor products (19 %)
 //     fill it: the prefix's CTAs are bound by the chain above, and the join ends 8 us after the last piece
@@ -908,10 +908,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         }
         o_init = true;
       };
-      auto weigh = [&](int f) -> bool {  // P V of the tile whose V is fill f
+      auto weights = [&]() -> bool {  // the first half of them is there, and O may be written
         if (!pt_wait(p_lo + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
         tc_fence_after();
-        if (!ensure_free()) return false;
+        return ensure_free();
+      };
+      auto weigh = [&](int f) -> bool {  // P V of the tile whose V is fill f
         if (DEC && pc.thin) {
           if (!pt_wait(p_full + x, p_par, ab, ERR_TIMEOUT_MMA)) return false;
           p_par ^= 1;
@@ -944,7 +946,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           if (i > first) {
             const int f = fpos + i - 2;
             if (i >= n) free_q();
-            ok = wait_v(f) && weigh(f);
+            ok = wait_v(f) && weights() && weigh(f);
             if (!ok) break;
             umma_commit(v_empty + f % NV);
             umma_commit(v_empty + f % NV);
@@ -972,8 +974,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         // batch j: P V of tile j - 1, Q K^T of tile j
         for (int j = pc.j0; pc.j0 < je && j <= je; ++j, ++fpos) {
           const bool before = j > pc.j0, more = j < je;
-          if (before) ok = wait_v(fpos - 1);
-          else ok = wait_k(fpos);
+          // nothing is waited for in a turn that could be before it
+          ok = (!before || wait_v(fpos - 1)) && (!more || wait_k(fpos)) && (!before || !uses(j - 1) || weights());
           if (!ok) break;
           if (!more) free_q();
           ok = !pair || my_turn();
@@ -982,11 +984,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             ok = weigh(fpos - 1);
             if (!ok) break;
           }
-          if (more) {
-            if (before) ok = wait_k(fpos);
-            if (!ok) break;
-            if (uses(j)) issue_S(fpos);
-          }
+          if (more && uses(j)) issue_S(fpos);
           if (pair) end_turn();
           if (before) umma_commit(v_empty + (fpos - 1) % NV);
           if (more) umma_commit(k_empty + fpos % NK);
@@ -1270,10 +1268,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           return fmaxf(m0, m1) * sl2;
         };
         float2 la = make_float2(0.f, 0.f), lb = la;
-        auto weights = [&](const uint32_t* sc, float nb, uint32_t* out) {
+        auto half = [&](const uint32_t* sc, float nb, uint32_t* out) {
           const float2 s2 = make_float2(sl2, sl2), n2 = make_float2(nb, nb);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
+          for (int e = 0; e < 16; e += 4) {
             const float2 a01 = ffma2(make_float2(__uint_as_float(sc[e]), __uint_as_float(sc[e + 1])), s2, n2);
             const float2 a23 = ffma2(make_float2(__uint_as_float(sc[e + 2]), __uint_as_float(sc[e + 3])), s2, n2);
             float w[4];
@@ -1284,35 +1282,42 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
             out[e / 2 + 1] = pack2(w[2], w[3], BF16);
           }
         };
+        auto weights = [&](const uint32_t* sc, float nb, uint32_t* out) {
+          half(sc, nb, out);
+          half(sc + 16, nb, out + 8);
+        };
         int stop = 0;          // first 32-column chunk that the stream did not finish
         bool lo_sent = false;  // weights of keys 0..63 are final and announced
         {
-          uint32_t sa[32], sb[32];
+          // A chunk's maximum is taken among the exponentials of the chunk before it (prompts: 2 % with the waits before
+          // the turns).
+          uint32_t sa[32], sb[32], w[16];
           tmem_ld32_async(tS, sa);
           tmem_ld32_wait(sa);
           tmem_ld32_async(tS + 32, sb);
-          if (m_used == -INFINITY) {
-            const float m0 = chunk_max(sa);
-            m_used = m0 == -INFINITY ? 0.f : m0;
-          }
+          const float m0 = chunk_max(sa);
+          if (m_used == -INFINITY) m_used = m0 == -INFINITY ? 0.f : m0;
           const float nb = -m_used, most = m_used + 8.f;
-          auto one = [&](int c, uint32_t(&cur)[32], uint32_t(&nxt)[32]) -> bool {
-            if (__any_sync(0xFFFFFFFFu, chunk_max(cur) > most)) {
-              tmem_ld32_wait(nxt);
-              stop = c;
-              return false;
-            }
-            uint32_t w[16];
-            weights(cur, nb, w);
-            tmem_st16(tS + c * 16, w);
+          bool over = __any_sync(0xFFFFFFFFu, m0 > most);
+          auto one = [&](int c, uint32_t(&cur)[32], uint32_t(&nxt)[32]) {  // weights of chunk c, maximum of the next
+            half(cur, nb, w);
             tmem_ld32_wait(nxt);
+            half(cur + 16, nb, w + 8);
+            const float mn = chunk_max(nxt);
+            tmem_st16(tS + c * 16, w);
             tmem_ld32_async(tS + (c + 2) * 32, cur);
-            return true;
+            over = __any_sync(0xFFFFFFFFu, mn > most);
+            stop = c + 1;
           };
-          if (one(0, sa, sb) && one(1, sb, sa)) {
+          if (!over) one(0, sa, sb);
+          if (!over) one(1, sb, sa);
+          if (!over) {
+            const float2 la0 = la, lb0 = lb;
+            half(sa, nb, w);
             tmem_ld32_wait(sb);
-            if (__any_sync(0xFFFFFFFFu, fmaxf(chunk_max(sa), chunk_max(sb)) > most)) {
-              stop = 2;
+            if (__any_sync(0xFFFFFFFFu, chunk_max(sb) > most)) {
+              la = la0;
+              lb = lb0;
             } else {
               // nothing stored will be rescaled: P V of keys 0..63 may begin
               tmem_st_wait();
@@ -1320,13 +1325,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
               __syncwarp();
               if (lane == 0) mbar_arrive(p_lo + x);
               lo_sent = true;
-              uint32_t w[16];
-              weights(sa, nb, w);
+              half(sa + 16, nb, w + 8);
               tmem_st16(tS + 32, w);
               weights(sb, nb, w);
               tmem_st16(tS + 48, w);
               stop = 4;
             }
+          } else {
+            tmem_ld32_wait(sa);
+            tmem_ld32_wait(sb);
           }
         }
         if (stop < 4) {
