@@ -71,6 +71,7 @@ size_t evict_workspace(int64_t, int64_t, int64_t);
 cudaError_t launch_paged_append(int, bool, int, const PagedAppend&, int, cudaStream_t);
 cudaError_t launch_paged_attn(int, int, PagedAttn&, uint8_t*, int, cudaStream_t);
 size_t paged_attn_workspace(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, bool, int);
+int64_t paged_attn_split_tokens(int64_t, int64_t, int);
 }  // namespace dab
 
 using namespace dab;
@@ -1121,7 +1122,9 @@ size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t
                                           int64_t head_dim, int64_t prefix_groups) {
   if (tokens < 0 || batch < 0 || heads < 1 || kv_group < 1 || kv_group > 128 || head_dim < 1 || prefix_groups < 0) return 0;
   const int sms = num_sms();
-  return WS_HEADER + std::max(paged_attn_workspace(tokens, batch, heads, kv_group, head_dim, 0, false, sms),
+  // the largest of all calls of up to `tokens`: prompts of more than `most` are not cut and need less than those of `most`
+  const int64_t most = std::min(tokens, paged_attn_split_tokens(heads, kv_group, sms));
+  return WS_HEADER + std::max(paged_attn_workspace(most, batch, heads, kv_group, head_dim, 0, false, sms),
                               paged_attn_workspace(batch, batch, heads, kv_group, head_dim, prefix_groups, true, sms));
 }
 

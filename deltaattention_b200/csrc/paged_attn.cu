@@ -1730,9 +1730,17 @@ Sizes sizes_of(int64_t T, int64_t B, int64_t H, int64_t G, int64_t groups, bool 
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 }  // namespace
 
+// Scratch of one call. It rises with every size but a prompt's tokens: units stay whole from paged_attn_split_tokens
+// on, and need none.
 size_t paged_attn_workspace(int64_t T, int64_t B, int64_t H, int64_t G, int64_t D, int64_t groups, bool decode, int sms) {
   const Sizes s = sizes_of(T, B, H, G, groups, decode, sms);
   return 256 + 2 * up256(s.recs * 8) + up256(s.rows * 8) + up256(s.rows * D * 4);
+}
+
+// The most tokens of prompts whose units may be cut: the last T with H * (T / utok) < 2 * sms.
+int64_t paged_attn_split_tokens(int64_t H, int64_t G, int sms) {
+  const int64_t utok = 2 * (128 / G);
+  return ((2 * static_cast<int64_t>(sms) - 1) / H + 1) * utok - 1;
 }
 
 template <int D, bool BF16, bool DEC>

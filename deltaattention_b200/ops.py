@@ -1151,8 +1151,9 @@ def _paged_workspace(device, tokens, batch, kv_heads, kv_group, head_dim, groups
 
 
 def paged_attention_workspace(tokens, batch, q_heads, kv_heads, head_dim, prefix_groups=0) -> int:
-    """Bytes of the ``workspace`` that ``flash_varlen`` and ``flash_paged`` of ``tokens`` queries and
-    ``decode_attention_paged`` of ``batch`` sequences in ``prefix_groups`` groups take on the current device."""
+    """Bytes of the ``workspace`` that ``flash_varlen`` and ``flash_paged`` of up to ``tokens`` queries of up to ``batch``
+    sequences, and ``decode_attention_paged`` of up to ``batch`` sequences in up to ``prefix_groups`` groups, take on the
+    current device."""
     return _paged_workspace(torch.cuda.current_device(), tokens, batch, kv_heads, q_heads // kv_heads, head_dim,
                             prefix_groups)
 

@@ -445,8 +445,9 @@ int dab_paged_append(const void* k, const void* v, const void* q, void* q_out, v
                      int64_t heads, int64_t q_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
                      int64_t max_pages, int64_t table_rows, int* err_word, void* stream);
 
-/* Scratch bytes of the three calls below (prefix_groups 0 but for decoding), 16-byte aligned. Zero it once,
- * then reuse it on one stream; its first word is the error word (dab_workspace_error). */
+/* Scratch bytes of the three calls below of up to `tokens` queries, `batch` sequences and `prefix_groups` groups (0 but
+ * for decoding): scratch of one size serves every smaller call too. 16-byte aligned. Zero it once, then reuse it on
+ * one stream; its first word is the error word (dab_workspace_error). */
 size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t heads, int64_t kv_group,
                                           int64_t head_dim, int64_t prefix_groups);
 

@@ -1,0 +1,71 @@
+"""The paged operators and their cache at the edges of what they take: scratch of one size for calls of many, starts and
+positions that only the device sees, calls with nothing in them.
+
+Tolerances are test_paged.py's: 2 u of the largest |v| for 16-bit weights and the output's rounding, 2^-13 of it for
+32-bit scores.
+"""
+import pytest
+import torch
+
+from deltaattention_b200 import _lib as L
+from test_paged import DT, UNIT, Pool, check, no_device_errors, ops, starts  # noqa: F401  (the fixtures)
+
+gpu = pytest.mark.gpu
+
+
+def exact(q, k, v, see, scale):
+    """test_paged.py's attend64 on the tensors' device, a whole head at a time: q [n, Hq, D], k / v [L, H, D], query i
+    sees the first see[i] rows."""
+    G = q.shape[1] // k.shape[1]
+    hidden = torch.arange(len(k), device=q.device) >= see.to(q.device)[:, None]
+    out = torch.empty(q.shape, dtype=torch.float64, device=q.device)
+    for h in range(q.shape[1]):
+        s = q[:, h].double() @ k[:, h // G].double().T * scale
+        w = torch.where(hidden, 0.0, s.masked_fill(hidden, -torch.inf).softmax(-1))
+        out[:, h] = w @ v[:, h // G].double()
+    return out.cpu()
+
+
+# ------------------------------------------------------------------------------------ scratch
+@pytest.mark.parametrize("H,G,D", [(8, 4, 128), (1, 1, 64), (4, 7, 128), (128, 1, 64), (2, 128, 64), (300, 1, 64)])
+def test_scratch_rises_with_every_size(H, G, D):
+    """Scratch for some tokens, sequences and groups serves every call with fewer of them."""
+    size = L.load().dab_paged_attention_workspace_size
+    for B in (1, 16, 700):
+        last = 0
+        for T in range(0, 9000 if H > 1 else 90000, 1 if H > 1 else 17):
+            now = size(T, B, H, G, D, 0)
+            assert now >= last, (T, B)
+            last = now
+    for T in (1, 500, 2367, 2368, 9000):
+        sizes = [size(T, B, H, G, D, 0) for B in range(1, 400)]
+        assert sizes == sorted(sizes)
+        assert size(T, 50, H, G, D, 20) >= size(T, 50, H, G, D, 3) >= sizes[49]
+
+
+@gpu
+@pytest.mark.parametrize("Hq,H,D,dt,most,news", [
+    (32, 8, 128, "bf16", 8192, [1, 300, 2000, 2367, 2368, 3500]), (128, 128, 64, "fp16", 2000, [1, 100, 767, 768, 1030])])
+def test_cache_for_long_prompts_takes_short_ones(ops, Hq, H, D, dt, most, news):
+    """A cache made for many tokens at a time takes prompts of any fewer, whole and behind others, and steps."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    g = torch.Generator(device="cuda").manual_seed(40)
+    rows = lambda n, h: torch.randn(n, h, D, generator=g, device="cuda").to(DT[dt])  # noqa: E731
+    c = PagedDecodeCache(1, 16, Hq, H, D, 80, 128, 5000, dtype=DT[dt], max_tokens=most)
+    for n in news:
+        a = c.open(n)
+        q, k, v = rows(n, Hq), rows(n, H), rows(n, H)
+        out = c.prefill(0, [a], q, k, v, starts([n]))
+        check(out, exact(q, k, v, torch.arange(1, n + 1), D ** -0.5), v)
+        c.extend(a, 37)
+        q2, k2, v2 = rows(37, Hq), rows(37, H), rows(37, H)
+        out = c.prefill(0, [a], q2, k2, v2, starts([37]))
+        k, v = torch.cat([k, k2]), torch.cat([v, v2])
+        check(out, exact(q2, k, v, n + torch.arange(1, 38), D ** -0.5), v)
+        c.advance()
+        x, y, z = rows(16, Hq), rows(16, H), rows(16, H)
+        out = c.step(0, x, y, z)
+        k, v = torch.cat([k, y[a:a + 1]]), torch.cat([v, z[a:a + 1]])
+        check(out[a:a + 1], exact(x[a:a + 1], k, v, torch.tensor([n + 38]), D ** -0.5), v)
+        c.close(a)
+    assert int(c.err) == 0 and c.workspace_error() == 0
