@@ -125,6 +125,16 @@ __device__ __forceinline__ bool groups_ok(const PagedAttn& p) {
   return !any;
 }
 
+// Whether sequence b's start lies behind its end. (paged_tokens cuts starts that rise to the tokens.)
+__device__ __forceinline__ bool start_falls(const PagedAttn& p, int b) { return p.cu[b + 1] < p.cu[b]; }
+// The whole block calls it with what its threads have seen. Where a start falls sequences overlap, and there may be more
+// units than the scratch was made for.
+__device__ __forceinline__ bool starts_ok(const PagedAttn& p, bool bad) {
+  const bool any = __syncthreads_or(bad);
+  if (any && threadIdx.x == 0) paged_error(p.err, ERR_STARTS);
+  return !any;
+}
+
 // Rows of group g's prefix that are read for all: whole pages.
 __device__ __forceinline__ int prefix_rows(const PagedAttn& p, int g) {
   const int64_t most = static_cast<int64_t>(p.max_pages) << p.ps_shift;
@@ -581,13 +591,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   const int tpt = 128 / p.G;
   int groups = 0;
   if constexpr (DEC) groups = groups_ok(p) ? p.groups : 0;
+  const int n = DEC ? groups + p.B : p.B;
+  bool rising = true;
+  if (!DEC && !p.may_split) {
+    bool bad = false;
+    for (int b = threadIdx.x; b < p.B; b += PT_THREADS) bad |= start_falls(p, b);
+    rising = starts_ok(p, bad);
+  }
   if (DEC || p.may_split) {
     // `per` items in a row for every thread; all threads take all turns, since a warp that parts here
     // does not come together again, and runs apart through everything below
-    const int n = DEC ? groups + p.B : p.B;
     const int per = (n + PT_THREADS - 1) / PT_THREADS;
     const int first = static_cast<int>(threadIdx.x) * per;
     int64_t c = 0, r = 0, tc, tr;
+    bool bad = false;
     Item it;
 #pragma unroll 1
     for (int k = 0; k < per; ++k) {
@@ -598,6 +615,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         c += has ? it.cost(p) : 0;
         r += has ? static_cast<int64_t>(p.H) * it.rows : 0;
       } else {
+        bad |= start_falls(p, i);
         const Seq s = prompt_seq(p, 2 * tpt, i);
         c += has ? static_cast<int64_t>(p.H) * s.nq * s.mt : 0;
         r += has ? static_cast<int64_t>(p.H) * s.nq : 0;
@@ -655,7 +673,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         r += static_cast<int64_t>(p.H) * it.rows;
       }
     } else {
-      const int chunk = chunk_tiles(p, tr, tc);
+      rising = starts_ok(p, bad);
+      const int chunk = rising ? chunk_tiles(p, tr, tc) : 0;
       if (threadIdx.x == 0) range->item = chunk;
       if (blockIdx.x == 0 && chunk) {
         // the sequences' first pieces, for the joining kernel
@@ -672,7 +691,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           c += prompt_pieces(p, s, chunk);
         }
       }
-      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_cost[n] = chunk;
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.rec_cost[p.B] = chunk;
     }
     __syncwarp();
   }
@@ -700,7 +719,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     Sched<DEC> sc;
     sc.groups = groups;
     sc.tpt = tpt;
-    sc.n = DEC ? groups + p.B : p.B;
+    sc.n = rising ? n : 0;
     sc.chunk = !DEC && p.may_split ? range->item : 0;
     sc.i0 = sc.place = 0;
     sc.base_t = sc.base_r = sc.pos = sc.end = 0;

@@ -1228,7 +1228,8 @@ def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, w
 
     q [T, Hq, d], k / v [T, Hkv, d] (bf16 / fp16, d 64 or 128, any token and head strides; q-head h reads kv-head
     h // (Hq / Hkv), at most 128 q-heads per kv-head; sm_scale is positive), cu_seqlens int32 [B + 1] on the device,
-    rising from 0: it is only read there, so the call can be captured. Rows of ``out`` [T, Hq, d] (q itself
+    rising from 0: it is only read there, so the call can be captured. Starts that fall are reported (0x604 in the
+    workspace's first word) and nothing is computed. Rows of ``out`` [T, Hq, d] (q itself
     will do) from cu_seqlens[B] on are left alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and
     may reach rows before it within the same 128 keys.
 

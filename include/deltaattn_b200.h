@@ -428,7 +428,8 @@ int dab_evict_by_mass(float* mass, const int64_t* mass_strides, int32_t* lengths
  * [B] (int32, the rows of every sequence) are on the device. A page number outside the pool, a length past
  * the table, a position past the rotation tables and a sequence outside the tokens are never followed: they
  * write 0x601, 0x602, 0x603, 0x604 into the error word (the first one stays) and that sequence's results are
- * not valid. */
+ * not valid. Starts cu_seqlens that fall anywhere are 0x604 too, and prompts' attention then writes no output at all;
+ * the append does not look for 0x604: it gives every token to one sequence that has it, and stays in the pool. */
 
 /* New rows into the pages. k / v [tokens, heads, head_dim]: with cu_seqlens [B + 1] (int32, rising from 0;
  * tokens from cu_seqlens[B] on are left alone) sequence b's are tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1,

@@ -69,3 +69,35 @@ def test_cache_for_long_prompts_takes_short_ones(ops, Hq, H, D, dt, most, news):
         check(out[a:a + 1], exact(x[a:a + 1], k, v, torch.tensor([n + 38]), D ** -0.5), v)
         c.close(a)
     assert int(c.err) == 0 and c.workspace_error() == 0
+
+
+# ------------------------------------------------------------------------- contents that only the device sees
+@gpu
+@pytest.mark.parametrize("cu", [[0, 512] * 8 + [0], [0, 512, 0, 512], [0, 512, 511], [9, 3, 512], [512, 0]])
+@pytest.mark.parametrize("T", [512, 40000])
+def test_starts_that_fall(ops, T, cu):
+    """Sequences that overlap, over rows that many chunks would be cut from: reported, nothing computed, nothing
+    written behind the scratch, and the scratch is fit for the next call. (With 40000 tokens units stay whole.)"""
+    B, rows = len(cu) - 1, 128000
+    kv = ops.PagedKV(*(torch.randn(1, 1, 256, 64, device="cuda").half() for _ in range(2)))
+    table = torch.zeros(B, rows // 256, dtype=torch.int32, device="cuda")
+    lengths = torch.full((B,), rows, dtype=torch.int32, device="cuda")
+    starts_ = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    q = torch.randn(T, 4, 64, device="cuda").half()
+    n = ops.paged_attention_workspace(T, B, 4, 1, 64)
+    whole = torch.zeros(n + (64 << 20), dtype=torch.uint8, device="cuda")
+    ws, guard = whole[:n], whole[n:]
+    guard.fill_(77)
+    k = torch.randn(T, 1, 64, device="cuda").half()
+    for call in (lambda out: ops.flash_paged(q, kv, table, lengths, starts_, out=out, workspace=ws),
+                 lambda out: ops.flash_varlen(q, k, k, starts_, out=out, workspace=ws)):
+        out = torch.full_like(q, 7.0)
+        call(out)
+        assert int(ws[:4].view(torch.int32)) == 0x604
+        assert (out == 7).all() and (guard == 77).all()
+        ws[:4] = 0
+        good = starts([100, 200])
+        got = ops.flash_varlen(q[:300], k[:300], k[:300], good, workspace=ws)
+        for a, b in ((0, 100), (100, 300)):
+            check(got[a:b], exact(q[a:b], k[a:b], k[a:b], torch.arange(1, b - a + 1), 64 ** -0.5), k)
+        assert int(ws[:4].view(torch.int32)) == 0 and (guard == 77).all()
