@@ -1588,13 +1588,14 @@ template <int D, typename T>
 __global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant__ PagedAttn p) {
   const int tpt = 128 / p.G, Hq = p.H * p.G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<int64_t>(p.T) * Hq) return;
   const int t = static_cast<int>(row / Hq), hq = static_cast<int>(row % Hq), h = hq / p.G, rg = hq % p.G;
-  // what goes by the inputs alone comes before the wait for the partial results
-  const int b = paged_sequence(p.cu, p.B, t);
-  if (b < 0) return;
-  const Seq s = prompt_seq(p, 2 * tpt, b);
+  // What goes by the inputs alone comes before the wait for the partial results. Warps that have nothing to join wait
+  // too: a grid of which none did could end before the attention kernel, and the stream's next call begin on its scratch.
+  const int b = row < static_cast<int64_t>(p.T) * Hq ? paged_sequence(p.cu, p.B, t) : -1;
+  Seq s = {};
+  if (b >= 0) s = prompt_seq(p, 2 * tpt, b);
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (b < 0) return;
   const int chunk = static_cast<int>(p.rec_cost[p.B]);
   if (!chunk) return;
   const int nch = (s.mt + chunk - 1) / chunk;
@@ -1622,7 +1623,7 @@ __global__ void __launch_bounds__(128, 6) decode_join_kernel(const __grid_consta
   const int tpt = 128 / p.G, Hq = p.H * p.G, lane = lane_id(), warp = threadIdx.x >> 5;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * (4 / WPR) + warp / WPR;
   const int groups = groups_ok(p) ? p.groups : 0;
-  if (row >= static_cast<int64_t>(p.B) * Hq) return;
+  if (row >= static_cast<int64_t>(p.B) * Hq) return;  // (every block has rows, whose warps wait)
   const int b = static_cast<int>(row / Hq), hq = static_cast<int>(row % Hq), h = hq / p.G, rg = hq % p.G;
   const int g = group_of(p, groups, b);
   const Item own = decode_item(p, groups, tpt, groups + b);

@@ -101,3 +101,38 @@ def test_starts_that_fall(ops, T, cu):
         for a, b in ((0, 100), (100, 300)):
             check(got[a:b], exact(q[a:b], k[a:b], k[a:b], torch.arange(1, b - a + 1), 64 ** -0.5), k)
         assert int(ws[:4].view(torch.int32)) == 0 and (guard == 77).all()
+
+
+@gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_with_nothing_in_them(ops, captured):
+    """A padded call whose tokens belong to no sequence, before and after others on one scratch and one stream."""
+    g = torch.Generator(device="cuda").manual_seed(41)
+    q = torch.randn(700, 8, 64, generator=g, device="cuda").half()
+    k, v = (torch.randn(700, 2, 64, generator=g, device="cuda").half() for _ in range(2))
+    cu = starts([300, 0, 390])
+    ref = ops.flash_varlen(q, k, v, cu)
+    check(ref[:300], exact(q[:300], k[:300], v[:300], torch.arange(1, 301), 64 ** -0.5), v)
+    nobody = [torch.zeros(4, dtype=torch.int32, device="cuda"), torch.full((4,), 700, dtype=torch.int32, device="cuda")]
+    ws = torch.zeros(ops.paged_attention_workspace(700, 3, 8, 2, 64), dtype=torch.uint8, device="cuda")
+    empty, outs = torch.full_like(q, 7.0), [torch.full_like(q, 7.0) for _ in range(40)]
+
+    def calls():
+        for i, out in enumerate(outs):
+            for _ in range(1 + i % 3):
+                ops.flash_varlen(q, k, v, nobody[i % 2], out=empty, workspace=ws)
+            ops.flash_varlen(q, k, v, cu, out=out, workspace=ws)
+
+    if captured:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            calls()
+        for _ in range(5):
+            graph.replay()
+    else:
+        calls()
+    assert (empty == 7).all() and int(ws[:4].view(torch.int32)) == 0
+    for out in outs:
+        assert torch.equal(out[:690], ref[:690]) and (out[690:] == 7).all()
