@@ -75,6 +75,7 @@ struct Piece {
                    // fill), and scores and output are computed transposed
   int lim0, lim_step;  // keys that token tok0 + i sees: lim0 + i * lim_step ..
   int by_length;   // .. and no more than the token's sequence has
+  int before;      // prompts: tokens at negative positions, which see nothing
   int split;       // partial results to rows orow0 / orow1 (thin: orow0), else the output
   int q1;          // one token: the query box of one token
   int64_t orow0, orow1;
@@ -387,6 +388,7 @@ template <bool DEC> struct Sched {
         pc.lim0 = item.len;
         pc.lim_step = 0;
         pc.by_length = shared;
+        pc.before = 0;
         pc.split = 1;
         pc.orow0 = base_r + before_r + static_cast<int64_t>(h) * item.rows + static_cast<int64_t>(up) * 2 * tpt * p.G +
                    static_cast<int64_t>(place) * PT_ROWS;
@@ -434,6 +436,7 @@ template <bool DEC> struct Sched {
         pc.q1 = pc.thin = pc.by_length = 0;
         pc.lim0 = p.causal ? pos0 + 1 : item.len;
         pc.lim_step = p.causal ? 1 : 0;
+        pc.before = max(-pos0, 0);
         pc.split = nch > 1;
         pc.orow0 = static_cast<int64_t>(id) * PT_ROWS;
         pc.orow1 = pc.orow0 + 128;
@@ -1048,6 +1051,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       int lim_row = 0;  // keys from kb on that this row sees
       if (live) {
         lim_row = pc.lim0 + (tok - pc.tok0) * pc.lim_step;
+        if (!DEC && tok - pc.tok0 < pc.before) lim_row = 0;
         if (pc.by_length) lim_row = min(lim_row, p.lengths[tok]);
         lim_row -= pc.kb;
       }
@@ -1475,14 +1479,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
           }
         } else {
           using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-          const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing gives 0
+          const bool none = l == 0.f;  // a row that sees nothing gives 0, whatever 0 times V was
+          const float inv = none ? 0.f : 1.f / l;
           const int64_t mine = live ? tok * p.o_t + (pc.h * p.G + r - ti * p.G) * p.o_h : 0;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
-            if (o_has) {
-              tmem_ld32(tO + c * 32, o);
-            } else {
+            if (o_has) tmem_ld32(tO + c * 32, o);
+            if (!o_has || none) {
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] = 0u;
             }

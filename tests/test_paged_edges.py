@@ -136,3 +136,40 @@ def test_calls_with_nothing_in_them(ops, captured):
     assert (empty == 7).all() and int(ws[:4].view(torch.int32)) == 0
     for out in outs:
         assert torch.equal(out[:690], ref[:690]) and (out[690:] == 7).all()
+
+
+@gpu
+@pytest.mark.parametrize("news,lens,Hq,H,D,dt", [
+    ([5, 2], [3, 0], 2, 1, 64, "fp16"), ([300, 40, 200], [170, 40, 333], 8, 2, 128, "bf16"), ([130], [1], 3, 3, 64, "bf16"),
+    ([900, 64], [129, 65], 16, 4, 64, "fp16"), ([2500] * 4, [1300] * 4, 32, 8, 64, "bf16")])
+def test_queries_before_the_first_row(ops, news, lens, Hq, H, D, dt):
+    """More queries than rows: those at negative positions give 0, causal or not, whatever parts the keys are cut into."""
+    pool = Pool(ops, len(lens), H, D, 16, lens, dt, 42)
+    q = torch.randn(sum(news), Hq, D, generator=torch.Generator().manual_seed(sum(news))).to(DT[dt]).cuda()
+    for causal in (True, False):
+        out = ops.flash_paged(q, pool.kv, pool.table, pool.lengths, starts(news), causal=causal)
+        at = 0
+        for b, (m, n) in enumerate(zip(news, lens)):
+            k, v = (x.cuda() for x in pool.rows(b))
+            none = max(0, m - n)
+            assert (out[at:at + none] == 0).all()
+            s = slice(at + none, at + m)
+            see = n - m + none + torch.arange(1, m - none + 1) if causal else torch.full((m - none,), n)
+            if m > none:
+                check(out[s], exact(q[s], k, v, see, D ** -0.5), pool.v)
+            at += m
+
+
+@gpu
+@pytest.mark.parametrize("news,lens", [([300, 40], [170, 40]), ([2500] * 4, [1300] * 4)])
+def test_queries_that_see_nothing_of_rows_that_are_nan(ops, news, lens):
+    """A query at a negative position gives 0 whatever the rows hold, in units that are cut and in whole ones."""
+    pool = Pool(ops, len(lens), 8, 64, 16, lens, "bf16", 43)
+    q = torch.randn(sum(news), 32, 64, generator=torch.Generator().manual_seed(43)).bfloat16().cuda()
+    pool.v.fill_(float("nan"))
+    for causal in (True, False):
+        out = ops.flash_paged(q, pool.kv, pool.table, pool.lengths, starts(news), causal=causal)
+        at = 0
+        for m, n in zip(news, lens):
+            assert (out[at:at + max(0, m - n)] == 0).all() and out[at + max(0, m - n):at + m].isnan().all()
+            at += m
