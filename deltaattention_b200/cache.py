@@ -343,10 +343,11 @@ class PagedDecodeCache:
         self.num_layers, self.places, self.page_size = num_layers, places, page_size
         self.q_heads, self.kv_heads, self.head_dim = q_heads, kv_heads, head_dim
         self.num_pages, self.max_pages, self.max_length = num_pages, -(-max_length // page_size), max_length
-        self.dtype, self.device, self.max_tokens = dtype, torch.device(device), max(int(max_tokens), places)
+        self.dtype, self.max_tokens = dtype, max(int(max_tokens), places)
         shape = (num_layers, num_pages, kv_heads, page_size, head_dim)
-        self._k = torch.zeros(shape, dtype=dtype, device=self.device)
+        self._k = torch.zeros(shape, dtype=dtype, device=device)
         self._v = torch.zeros_like(self._k)
+        self.device = self._k.device  # with its number: "cuda" alone would follow the current device
         self.pools = [ops.PagedKV(self._k[i], self._v[i]) for i in range(num_layers)]
         i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=self.device)  # noqa: E731
         self.page_table, self.lengths, self.err = i32(places, self.max_pages), i32(places), i32(1)

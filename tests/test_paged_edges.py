@@ -173,3 +173,12 @@ def test_queries_that_see_nothing_of_rows_that_are_nan(ops, news, lens):
         for m, n in zip(news, lens):
             assert (out[at:at + max(0, m - n)] == 0).all() and out[at + max(0, m - n):at + m].isnan().all()
             at += m
+
+
+# ------------------------------------------------------------------------------------ the cache
+@gpu
+def test_cache_knows_its_device(ops):
+    """The bookkeeping goes to the device that the cache was made on, not to the one current later."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    c = PagedDecodeCache(1, 2, 2, 1, 64, 4, 16, 64)
+    assert c.device == c.page_table.device == c._k.device and c.device.index is not None
