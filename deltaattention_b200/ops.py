@@ -1231,7 +1231,8 @@ def flash_varlen(q, k, v, cu_seqlens, *, causal=True, sm_scale=None, out=None, w
     rising from 0: it is only read there, so the call can be captured. Starts that fall are reported (0x604 in the
     workspace's first word) and nothing is computed. Rows of ``out`` [T, Hq, d] (q itself
     will do) from cu_seqlens[B] on are left alone. A NaN or an infinity in V reaches the rows of its sequence that see it, and
-    may reach rows before it within the same 128 keys.
+    may reach rows before it within the same 128 keys. Scaled scores are up to 2^26 in size, as ``flash`` takes them:
+    beyond that fp32 does not resolve what the weights are made of, and rows may become NaN.
 
     ``workspace`` (uint8, ``paged_attention_workspace`` bytes, zero-filled once, used by one stream at a time)
     replaces the library's own, which is given up when a later call needs a larger one: a call that is
