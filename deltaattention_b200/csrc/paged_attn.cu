@@ -13,7 +13,8 @@
 //   own       one token of one sequence over the rows behind its prefix: G rows. Bytes bound it. Up to 8 rows are
 //             computed transposed (thin): S^T = K Q^T has a key per row and 8 columns, which takes a warp a tenth
 //             of the time of 128 columns; the two tiles take every other key tile, two chains at a time.
-// A decode step's units, one after the other, are cut into even ranges of cost, one per CTA. Prompts take pieces
+// A decode step's prefixes are cut into even ranges of cost, one for each of the first CTAs, its own units into ranges for
+// the others, so that a CTA's pieces are all of one kind: thin ones or pairs. Prompts take pieces
 // from a counter, heavy ones first; where whole units would leave SMs idle they are cut into chunks of key tiles, the
 // units of one chunk next to each other so that they find its keys in L2. Pieces of cut units leave fp32
 // partial sums with their maxima, joined by a second kernel that is launched early (programmatic dependent launch).
@@ -101,7 +102,7 @@ template <int D> struct PtCfg {
   static constexpr int OFF_X = OFF_VOTE + 2 * 2 * 4 * (PT_THIN + 1) * 4;  // thin: tile 1's O^T, maxima and sums
   static constexpr int OFF_PIECE = OFF_X + PT_THIN * (D + 2) * 4;
   static constexpr int OFF_BAR = OFF_PIECE + PT_RING * static_cast<int>(sizeof(Piece));
-  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 6 + 1 + 2 + 2 + 2;
+  static constexpr int NBAR = 4 + 2 * NK + 2 * NV + 2 * PT_RING + 2 * 6 + 1 + 2 + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int SMEM = OFF_MISC + 256 + 1024;  // and slack for alignment
 };
@@ -541,8 +542,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   uint64_t* vote = tile_free + 2;       // [2] thin pieces: the tile's warps have looked at their scores
   uint64_t* mma_done = vote + 2;
   uint64_t* turn = mma_done + 1;        // [2]
-  uint64_t* xfer = turn + 4;            // [2] thin: tile 1's result is there, and has been read
-  uint64_t* level = turn + 2;           // [2] warp 1 + x is past its pieces of its own
+  uint64_t* xfer = turn + 2;            // [2] thin: tile 1's result is there, and has been read
   Piece* pieces = reinterpret_cast<Piece*>(smem + C::OFF_PIECE);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 8);
@@ -573,7 +573,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
       mbar_init(tile_free + x, 4);
       mbar_init(vote + x, 4);
       mbar_init(turn + x, 1);
-      mbar_init(level + x, 1);
       mbar_init(xfer + x, 4);
     }
     mbar_init(mma_done, 2);
@@ -844,8 +843,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     // softmax passes half a period apart; a tile on its own takes no turns (16 x 32 tokens over 4000 rows: 83 -> 77 us).
     // The two of a thin piece go apart: fills of even number are
     // tile 0's, of odd number tile 1's, and their warp releases them with both arrivals. As the slots of a
-    // parity stay with a warp, it sees all of their phases; before a pair's piece, which it walks with the
-    // other one, they wait for each other, so that no earlier phase of the other's slots is still open.
+    // parity stay with a warp, it sees all of their phases: no CTA has a pair's piece beside a thin one.
     const int x = warp - 1;
     constexpr uint32_t IDESC_S = umma_idesc_f16(128, PT_BN, BF16, false);
     constexpr uint32_t IDESC_PV = umma_idesc_f16(128, D, BF16, true);
@@ -858,8 +856,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
     const uint64_t pdesc = umma_desc_sw128(smem_u32(smem + C::OFF_P + x * C::PBYTES), 16, 1024);
     const uint64_t vdesc0 = umma_desc_sw128(smem_u32(smem + C::OFF_V), PT_BN * 128, 1024);
     int fpos = 0, qpos = 0;  // fills of the K and V rings, of the query slots
-    uint32_t free_par = 1, p_par = 0, nbatch = 0, nlevel = 0;
-    bool apart = false;
+    uint32_t free_par = 1, p_par = 0, nbatch = 0;
     Piece pc;
     bool ok = true;
     auto my_turn = [&]() -> bool {
@@ -961,7 +958,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         return true;
       };
       if (DEC && pc.thin) {
-        apart = true;
         const int n = je - pc.j0, first = (fpos ^ x) & 1;
         if (first >= n) free_q();
         for (int i = first; first < n; i += 2) {
@@ -985,13 +981,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         fpos += n;
       } else {
         auto uses = [&](int j) { return mine && j < (x ? pc.nt1 : pc.nt0); };
-        if (DEC && apart) {
-          if (lane == 0) mbar_arrive(level + x);
-          ok = pt_wait(level + (1 - x), nlevel & 1, ab, ERR_TIMEOUT_MMA);
-          if (!ok) break;
-          ++nlevel;
-          apart = false;
-        }
         if (pc.j0 >= je) free_q();
         // batch j: P V of tile j - 1, Q K^T of tile j
         for (int j = pc.j0; pc.j0 < je && j <= je; ++j, ++fpos) {
