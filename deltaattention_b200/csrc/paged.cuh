@@ -68,20 +68,22 @@ __device__ __forceinline__ int paged_length(int len, int max_pages, int ps_shift
   return max_pages << ps_shift;
 }
 
-// Tokens [c0, c1) of sequence b, kept inside [0, T].
-__device__ __forceinline__ void paged_tokens(const int32_t* cu, int b, int T, int* err, int& c0, int& c1) {
+// Tokens [c0, c1) of sequence b, kept inside [0, T]; returns whether its start lies behind its end.
+__device__ __forceinline__ bool paged_tokens(const int32_t* cu, int b, int T, int* err, int& c0, int& c1) {
   if (!cu) {
     c0 = b;
     c1 = b + 1;
-    return;
+    return false;
   }
   c0 = cu[b];
   c1 = cu[b + 1];
+  const bool falls = c1 < c0;
   if (c0 < 0 || c1 > T || c1 < c0) {
     paged_error(err, ERR_STARTS);
     c0 = min(max(c0, 0), T);
     c1 = min(max(c1, c0), T);
   }
+  return falls;
 }
 
 // The last b in [0, B) with cu[b] <= t, for t in [cu[0], cu[B]); -1 for other tokens. The whole warp

@@ -127,16 +127,6 @@ __device__ __forceinline__ bool groups_ok(const PagedAttn& p) {
   return !any;
 }
 
-// Whether sequence b's start lies behind its end. (paged_tokens cuts starts that rise to the tokens.)
-__device__ __forceinline__ bool start_falls(const PagedAttn& p, int b) { return p.cu[b + 1] < p.cu[b]; }
-// The whole block calls it with what its threads have seen. Where a start falls sequences overlap, and there may be more
-// units than the scratch was made for.
-__device__ __forceinline__ bool starts_ok(const PagedAttn& p, bool bad) {
-  const bool any = __syncthreads_or(bad);
-  if (any && threadIdx.x == 0) paged_error(p.err, ERR_STARTS);
-  return !any;
-}
-
 // Rows of group g's prefix that are read for all: whole pages.
 __device__ __forceinline__ int prefix_rows(const PagedAttn& p, int g) {
   const int64_t most = static_cast<int64_t>(p.max_pages) << p.ps_shift;
@@ -255,11 +245,12 @@ __device__ __noinline__ void block_scan2(int64_t& a, int64_t& b, int64_t* smem, 
 // A prompt's sequence: queries [c0, c1), `len` keys, `nq` units of 2 * tpt tokens and `mt` key tiles.
 struct Seq {
   int c0, n, len, nq, mt;
+  bool falls;  // its start lies behind its end
 };
 __device__ __noinline__ Seq prompt_seq(const PagedAttn& p, int utok, int b) {
   Seq s;
   int c1;
-  paged_tokens(p.cu, b, p.T, p.err, s.c0, c1);
+  s.falls = paged_tokens(p.cu, b, p.T, p.err, s.c0, c1);
   s.n = c1 - s.c0;
   s.len = s.n == 0 ? 0 : p.table ? paged_length(p.lengths[b], p.max_pages, p.ps_shift, p.err) : s.n;
   s.nq = (s.n + utok - 1) / utok;
@@ -594,11 +585,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
   int groups = 0;
   if constexpr (DEC) groups = groups_ok(p) ? p.groups : 0;
   const int n = DEC ? groups + p.B : p.B;
+  // Where a start falls sequences overlap, and there may be more units than the scratch was made for: there are none then.
   bool rising = true;
   if (!DEC && !p.may_split) {
     bool bad = false;
-    for (int b = threadIdx.x; b < p.B; b += PT_THREADS) bad |= start_falls(p, b);
-    rising = starts_ok(p, bad);
+    for (int b = threadIdx.x; b < p.B; b += PT_THREADS) bad |= p.cu[b + 1] < p.cu[b];
+    rising = !__syncthreads_or(bad);
+    if (!rising && threadIdx.x == 0) paged_error(p.err, ERR_STARTS);
   }
   if (DEC || p.may_split) {
     // `per` items in a row for every thread; all threads take all turns, since a warp that parts here
@@ -617,8 +610,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         c += has ? it.cost(p) : 0;
         r += has ? static_cast<int64_t>(p.H) * it.rows : 0;
       } else {
-        bad |= start_falls(p, i);
         const Seq s = prompt_seq(p, 2 * tpt, i);
+        bad |= s.falls;
         c += has ? static_cast<int64_t>(p.H) * s.nq * s.mt : 0;
         r += has ? static_cast<int64_t>(p.H) * s.nq : 0;
       }
@@ -675,7 +668,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_attn_kernel(const __grid_
         r += static_cast<int64_t>(p.H) * it.rows;
       }
     } else {
-      rising = starts_ok(p, bad);
+      rising = !__syncthreads_or(bad);  // (prompt_seq has reported it)
       const int chunk = rising ? chunk_tiles(p, tr, tc) : 0;
       if (threadIdx.x == 0) range->item = chunk;
       if (blockIdx.x == 0 && chunk) {
@@ -1581,14 +1574,17 @@ template <int D, typename T>
 __global__ void __launch_bounds__(128) prompt_join_kernel(const __grid_constant__ PagedAttn p) {
   const int tpt = 128 / p.G, Hq = p.H * p.G;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= static_cast<int64_t>(p.T) * Hq) return;  // (every block has rows, whose warps wait)
   const int t = static_cast<int>(row / Hq), hq = static_cast<int>(row % Hq), h = hq / p.G, rg = hq % p.G;
   // What goes by the inputs alone comes before the wait for the partial results. Warps that have nothing to join wait
   // too: a grid of which none did could end before the attention kernel, and the stream's next call begin on its scratch.
-  const int b = row < static_cast<int64_t>(p.T) * Hq ? paged_sequence(p.cu, p.B, t) : -1;
-  Seq s = {};
-  if (b >= 0) s = prompt_seq(p, 2 * tpt, b);
+  const int b = paged_sequence(p.cu, p.B, t);
+  if (b < 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
+  const Seq s = prompt_seq(p, 2 * tpt, b);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (b < 0) return;
   const int chunk = static_cast<int>(p.rec_cost[p.B]);
   if (!chunk) return;
   const int nch = (s.mt + chunk - 1) / chunk;
