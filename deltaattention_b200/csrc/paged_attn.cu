@@ -35,7 +35,7 @@
 //     as polynomials (4 %); turns of the products' warps that end before the scores (9 %) or none (12 %); one election for
 //     a batch of products (no gain); a single lane for the products' role (12 %)
 //   16 sequences of 32000 rows        310 us, 6.8 TB/s (floor 320); 48 of 500 to 12000: 200 us (floor 185)
-//   64 sequences, 32000 rows shared and up to 1000 own: 84 us (floor 40). Neither bytes (38 % of nominal) nor products (19 %)
+//   64 sequences, 32000 rows shared and up to 1000 own: 85 us (floor 40). Neither bytes (38 % of nominal) nor products (19 %)
 //     fill it: the prefix's CTAs are bound by the chain above, and the join ends 8 us after the last piece
 //   1 sequence of 1900 rows (d 64)    17 us: two launches, each a chain of reads, code that is fetched, one key tile
 #include <algorithm>

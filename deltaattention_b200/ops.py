@@ -1126,7 +1126,8 @@ def paged_append(k, v, pool: PagedKV, page_table, lengths, *, cu_seqlens=None, c
     (``rope``'s formula, in fp32 and rounded once) and q [T, Hq, d] is rotated into ``q_out`` (allocated by default;
     q itself is fine; rows of skipped tokens are not written). Without them K goes in as it is. ``err`` (int32
     [1]) gets the first of 0x601 (a page number outside the pool), 0x602 (a length past the page table) and 0x603
-    (a position past the tables); such rows are not stored. New rows must not share a place in the pool."""
+    (a position past the tables); such rows are not stored, and without ``err`` nothing says so. New rows must not
+    share a place in the pool."""
     what = "paged_append"
     pk, pv = pool.k, pool.v
     L.same_device(what, k, v, pk, pv, page_table, lengths, cu_seqlens, cos, sin, q, q_out, err)
