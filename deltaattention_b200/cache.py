@@ -359,7 +359,13 @@ class PagedDecodeCache:
         self._pages = [None] * places  # a place's pages, None while it is free
         self._length = [0] * places
         self._groups = {}  # first place -> (places, shared rows)
+        # This cache's own scratch, of one size for its life: captured steps use it. It is zeroed here, so that no capture
+        # takes the zeroing in (the calls before its replay would then work on anything).
         self._ws = None
+        if self.device.type == "cuda":
+            with torch.cuda.device(self.device):
+                n = ops.paged_attention_workspace(self.max_tokens, places, q_heads, kv_heads, head_dim, places)
+            self._ws = torch.zeros(n, dtype=torch.uint8, device=self.device)
 
     # ------------------------------------------------------------------ bookkeeping on the host
     def _take(self, n):
@@ -498,15 +504,6 @@ class PagedDecodeCache:
         self.lengths.add_(self._open)
 
     # ------------------------------------------------------------------ on the device
-    def _workspace(self):
-        """This cache's own scratch, of one size for its life: a captured step uses it."""
-        if self._ws is None:
-            with torch.cuda.device(self.device):
-                n = ops.paged_attention_workspace(self.max_tokens, self.places, self.q_heads, self.kv_heads, self.head_dim,
-                                                  self.places)
-            self._ws = torch.zeros(n, dtype=torch.uint8, device=self.device)
-        return self._ws
-
     def prefill(self, layer, places, q, k, v, cu_seqlens, cos=None, sin=None, out=None, sm_scale=None):
         """Prompts, or the last tokens of them, of the sequences at ``places`` (a list): rows q [T, Hq, d], k / v [T,
         Hkv, d] packed by ``cu_seqlens`` (int32 on the device) go into the pages (rotated with cos / sin, see
@@ -523,7 +520,7 @@ class PagedDecodeCache:
         turned = ops.paged_append(k, v, self.pools[layer], table, lengths, cu_seqlens=cu_seqlens, cos=cos, sin=sin,
                                   q=None if cos is None else q, err=self.err)
         return ops.flash_paged(q if cos is None else turned, self.pools[layer], table, lengths, cu_seqlens, out=out,
-                               sm_scale=sm_scale, workspace=self._workspace())
+                               sm_scale=sm_scale, workspace=self._ws)
 
     def step(self, layer, q, k_new, v_new, cos=None, sin=None, out=None, sm_scale=None):
         """One layer's token of every place: q [places, Hq, d], k_new / v_new [places, Hkv, d], after ``advance``."""
@@ -531,12 +528,11 @@ class PagedDecodeCache:
                                   q=None if cos is None else q, err=self.err)
         return ops.decode_attention_paged(
             q if cos is None else turned, self.pools[layer], self.page_table, self.lengths, prefix_cu=self.prefix_cu,
-            prefix_lengths=self.prefix_lengths, out=out, sm_scale=sm_scale, workspace=self._workspace())
+            prefix_lengths=self.prefix_lengths, out=out, sm_scale=sm_scale, workspace=self._ws)
 
     def capture_step(self, q, k_new, v_new, out, cos=None, sin=None):
         """One step over every layer in a CUDA graph: q / out [layers, places, Hq, d], k_new / v_new [layers, places,
         Hkv, d] are static device buffers. Replay it after ``advance``."""
-        self._workspace()
         s = torch.cuda.Stream(self.device)
         s.wait_stream(torch.cuda.current_stream(self.device))
         g = torch.cuda.CUDAGraph()
@@ -549,6 +545,6 @@ class PagedDecodeCache:
     def workspace_error(self):
         """Reads and clears the attention calls' error word (a synchronising call)."""
         import ctypes
-        ws, code = self._workspace(), ctypes.c_int(0)
+        ws, code = self._ws, ctypes.c_int(0)
         L.check(L.load().dab_workspace_error(L.ptr(ws), ctypes.byref(code), L.stream_of(ws)), "workspace_error")
         return code.value

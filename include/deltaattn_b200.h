@@ -454,8 +454,8 @@ size_t dab_paged_attention_workspace_size(int64_t tokens, int64_t batch, int64_t
 
 /* Attention of sequences packed back to back: q / out [tokens, heads * kv_group, head_dim], k / v [tokens, heads,
  * head_dim], offsets cu_seqlens as above. q-head h reads K / V head h / kv_group (at most 128); query i of a sequence
- * sees its rows 0 .. i (causal) or all of them; sm_scale is positive, scaled scores up to 2^26 in size. `strides` (11): q (token, head), out (token, head), k (unused, head, token),
- * v (unused, head, token), unused. */
+ * sees its rows 0 .. i (causal) or all of them; sm_scale is positive, scaled scores up to 2^26 in size. `strides` (11):
+ * q (token, head), out (token, head), k (unused, head, token), v (unused, head, token), unused. */
 int dab_flash_varlen(const void* q, const void* k, const void* v, void* out, const int32_t* cu_seqlens,
                      const int64_t* strides, float sm_scale, int causal, int dtype, int64_t tokens, int64_t batch,
                      int64_t heads, int64_t kv_group, int64_t head_dim, void* workspace, size_t workspace_bytes,

@@ -182,3 +182,30 @@ def test_cache_knows_its_device(ops):
     from deltaattention_b200.cache import PagedDecodeCache
     c = PagedDecodeCache(1, 2, 2, 1, 64, 4, 16, 64)
     assert c.device == c.page_table.device == c._k.device and c.device.index is not None
+
+
+@gpu
+def test_step_captured_before_anything_else(ops):
+    """A caller's own capture of a cache's step, before its first prompt: the prompt's call finds its scratch zeroed
+    though the graph has not run yet, and the graph then gives what an eager step gives."""
+    from deltaattention_b200.cache import PagedDecodeCache
+    g = torch.Generator(device="cuda").manual_seed(45)
+    rows = lambda n, h: torch.randn(n, h, 64, generator=g, device="cuda").half()  # noqa: E731
+    c = PagedDecodeCache(1, 2, 8, 2, 64, 40, 16, 400, dtype=torch.float16, max_tokens=300)
+    ws = c._ws
+    assert ws is not None  # made by the capture it would be the graph's, and zeroed by its replays alone
+    x, y, z = rows(2, 8), rows(2, 2), rows(2, 2)
+    out = torch.zeros_like(x)
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=s):
+        c.step(0, x, y, z, out=out)
+    assert c._ws is ws and int(ws.count_nonzero()) == 0
+    a = c.open(300)
+    q, k, v = rows(300, 8), rows(300, 2), rows(300, 2)
+    got = c.prefill(0, [a], q, k, v, starts([300]))
+    check(got, exact(q, k, v, torch.arange(1, 301), 64 ** -0.5), v)
+    c.advance()
+    graph.replay()
+    check(out[a:a + 1], exact(x[a:a + 1], torch.cat([k, y[a:a + 1]]), torch.cat([v, z[a:a + 1]]), torch.tensor([301]), 64 ** -0.5), v)
+    assert torch.equal(out, c.step(0, x, y, z)) and int(c.err) == 0 and c.workspace_error() == 0
